@@ -21,6 +21,45 @@ struct MlaArgs {
   float* part_m;            // partials: [n_split][rows], [n_split][rows], [n_split][rows][512]
   float* part_l;
   float* part_acc;
+  // window > 0: a row of n keys attends to the keys p >= n - window and p < sinks only
+  int window, sinks;
 };
+
+// The 8-bit latent cache: blocks of `1 << shift` tokens x 512 values, one fp32 scale a block; a key is scale * value.
+enum : int { CACHE_F16 = 0, CACHE_I8 = 1, CACHE_E4M3 = 2 };
+struct MlaPaged {
+  uint8_t* data;            // [n_blocks][block][512]
+  float* scales;            // [n_blocks]
+  int64_t n_blocks;
+  int shift;
+  const int* table;         // [n_seqs][table_stride] block numbers; null: one sequence, block i of it is block i
+  int table_stride, n_seqs;
+  const int* row_seq;       // sequence of a query row (null: sequence 0); outside [0, n_seqs): a row without keys
+  // block of position p of a sequence; negative: none (behind the table, or an entry that names no block)
+  __device__ __forceinline__ int64_t block_of(int seq, int p) const {
+    const int b = p >> shift;
+    if (p < 0 || (table && b >= table_stride)) return -1;
+    const int64_t phys = table ? table[(size_t)seq * table_stride + b] : b;
+    return phys < n_blocks ? phys : -1;
+  }
+  __device__ __forceinline__ int seq_of(int r) const {
+    const int s = row_seq ? row_seq[r] : 0;
+    return s >= n_seqs ? -1 : s;
+  }
+};
+
+// The keys that a row attends to, as a list: the first `head` positions, then lo .. n - 1.
+struct KeyList {
+  int head, lo, n;
+  __device__ __forceinline__ int count() const { return head + n - lo; }
+  __device__ __forceinline__ int at(int i) const { return i < head ? i : lo + i - head; }
+};
+__device__ __forceinline__ KeyList key_list(int n, int window, int sinks) {
+  KeyList k;
+  k.n = n > 0 ? n : 0;
+  k.lo = window > 0 && k.n > window ? k.n - window : 0;
+  k.head = sinks < k.lo ? sinks : k.lo;
+  return k;
+}
 
 }  // namespace hk

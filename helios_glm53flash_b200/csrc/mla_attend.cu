@@ -14,6 +14,9 @@ namespace hk {
 // implemented in mla_flash_tc.cu; returns HK_ERR_UNSUPPORTED when the shape is not covered
 int mla_flash_tc_launch(const MlaArgs& a, cudaStream_t s, bool clusters = false);
 int mla_flash_tc_auto_splits(int m, int n_keys);
+// implemented in mla8_cache.cu
+bool mla8_paged(MlaPaged* pg, const void* ckv8, const float* scales, int dtype, int64_t n_blocks, int block, const int* block_table,
+                int table_stride, int n_seqs, const int* row_seq);
 bool mla_flash_cluster_shape(int m, int tiles, int* n_split);
 
 static inline size_t align_up(size_t v, size_t a) { return (v + a - 1) / a * a; }
@@ -49,20 +52,22 @@ static int simt_auto_splits(int m, int n_heads, int n_keys) {
   return s;
 }
 
-static int launch_simt(const MlaArgs& a, cudaStream_t s) {
+template <int FMT>
+static int launch_simt_as(const MlaArgs& a, const MlaPaged& pg, cudaStream_t s) {
   static bool attr_set[64] = {false};
   int dev = 0;
   cudaGetDevice(&dev);
   if (dev >= 0 && dev < 64 && !attr_set[dev]) {
-    if (cudaFuncSetAttribute(mla_simt_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+    if (cudaFuncSetAttribute(mla_simt_kernel<FMT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                              (int)MLA_SIMT_SMEM) != cudaSuccess)
       return HK_ERR_CUDA;
     attr_set[dev] = true;
   }
   dim3 grid(a.n_heads / SIMT_HG, a.n_split, a.m);
-  mla_simt_kernel<<<grid, 256, MLA_SIMT_SMEM, s>>>(a);
+  mla_simt_kernel<FMT><<<grid, 256, MLA_SIMT_SMEM, s>>>(a, pg);
   return cudaPeekAtLastError() == cudaSuccess ? HK_OK : HK_ERR_CUDA;
 }
+static int launch_simt(const MlaArgs& a, cudaStream_t s) { return launch_simt_as<CACHE_F16>(a, MlaPaged{}, s); }
 
 template <int GROUPS>
 static int combine_launch(const float* pm, const float* pl, const float* pa, int n_split, int64_t rows, __half* out,
@@ -94,11 +99,17 @@ static int combine(const float* pm, const float* pl, const float* pa, int n_spli
   return combine_launch<LSE_GROUPS>(pm, pl, pa, n_split, rows, out, s);
 }
 
+// Keys in the tiles that a row of n keys (0: not known) reads under a window: whole tiles of sinks and of the window.
+int mla_window_keys(int n, int window, int sinks) {
+  const int64_t tiles = (sinks + 63LL) / 64 + (window + 62LL) / 64 + 1, all = n > 0 ? (n + 63LL) / 64 : tiles;
+  return (int)((tiles < all ? tiles : all) * 64 > INT32_MAX ? INT32_MAX : (tiles < all ? tiles : all) * 64);
+}
+
 // common driver: final output, optionally through split partials in the workspace.  `choose`: the caller leaves the form to the library,
 // which may then merge one row's splits in clusters; a number of splits that the caller gives means that many CTAs a row.
 static int attend(MlaArgs a, int n_keys_hint, int n_split, bool choose, void* workspace, size_t workspace_bytes,
                   cudaStream_t s) {
-  const bool tc = (a.n_heads == 64) && !force_simt();
+  const bool tc = (a.n_heads == 64) && !force_simt() && a.window == 0;
   if (n_split <= 0)
     n_split = tc ? mla_flash_tc_auto_splits(a.m, n_keys_hint)
                  : simt_auto_splits(a.m, a.n_heads, n_keys_hint);
@@ -134,7 +145,87 @@ static int attend(MlaArgs a, int n_keys_hint, int n_split, bool choose, void* wo
   return HK_OK;
 }
 
+static int mla8_auto_splits(int m, int n_heads, int n_keys) { return simt_auto_splits(m, n_heads, n_keys); }
+
+// the 8-bit cache: final output, through split partials in the workspace where there is more than one split
+static int attend8(MlaArgs a, const MlaPaged& pg, int dtype, int n_keys_hint, int n_split, void* workspace, size_t workspace_bytes,
+                   cudaStream_t s) {
+  if (n_split <= 0) n_split = mla8_auto_splits(a.m, a.n_heads, n_keys_hint);
+  if (n_split > LSE_MAX_SPLITS) return HK_ERR_UNSUPPORTED;
+  const int64_t rows = (int64_t)a.m * a.n_heads;
+  __half* final_out = a.out;
+  a.n_split = n_split;
+  if (n_split > 1) {
+    const PartialLayout pl = partial_layout(n_split, rows);
+    if (!workspace || workspace_bytes < pl.total) return HK_ERR_WORKSPACE;
+    if (!aligned(workspace, 256)) return HK_ERR_INVALID;
+    char* ws = (char*)workspace;
+    a.part_m = (float*)ws;
+    a.part_l = (float*)(ws + pl.off_l);
+    a.part_acc = (float*)(ws + pl.off_acc);
+    a.out = nullptr;
+  }
+  const int st = dtype == HK_I8 ? launch_simt_as<CACHE_I8>(a, pg, s) : launch_simt_as<CACHE_E4M3>(a, pg, s);
+  if (st != HK_OK || n_split == 1) return st;
+  return combine(a.part_m, a.part_l, a.part_acc, n_split, rows, final_out, s);
+}
+
+// keys of a row, for choosing the splits of a dense call
+static int mla8_dense_keys(int m, int pos_start, int n_keys_hint, int window, int sinks, bool per_row) {
+  const int n = !per_row ? pos_start + m : n_keys_hint > 0 ? n_keys_hint : 4096;
+  return window > 0 ? mla_window_keys(n, window, sinks) : n;
+}
+
 }  // namespace hk
+
+HK_API int hk_mla8_auto_splits(int m, int n_heads, int n_keys) {
+  if (m <= 0 || n_keys <= 0 || n_heads < hk::SIMT_HG) return 1;
+  return hk::mla8_auto_splits(m, n_heads, n_keys);
+}
+
+HK_API size_t hk_mla8_dense_workspace_bytes(int m, int n_heads, int pos_start, int n_keys_hint, int window, int sinks, int per_row) {
+  if (m <= 0 || n_heads < hk::SIMT_HG || pos_start < 0 || sinks < 0) return 0;
+  const int splits = hk::mla8_auto_splits(m, n_heads, hk::mla8_dense_keys(m, pos_start, n_keys_hint, window, sinks, per_row));
+  return splits > 1 ? hk_mla_partial_bytes(splits, (int64_t)m * n_heads) : 0;
+}
+
+HK_API int hk_mla8_dense(const void* q_lat, const void* ckv8, const float* scales, int dtype, int64_t n_blocks, int block,
+                         const int* block_table, int table_stride, int n_seqs, const int* row_seq, const int* kv_len, int pos_start,
+                         int window, int sinks, void* lat_out, int m, int n_heads, float scale, int n_split, int n_keys_hint, void* workspace,
+                         size_t workspace_bytes, void* stream) {
+  using namespace hk;
+  MlaPaged pg;
+  HK_REQUIRE(mla8_paged(&pg, ckv8, scales, dtype, n_blocks, block, block_table, table_stride, n_seqs, row_seq));
+  HK_REQUIRE(q_lat && lat_out && aligned(q_lat, 16) && aligned(lat_out, 16));
+  HK_REQUIRE(m >= 0 && pos_start >= 0 && (int64_t)pos_start + m <= INT32_MAX && window >= 0 && sinks >= 0 && n_heads > 0 && n_heads % SIMT_HG == 0);
+  if (m == 0) return HK_OK;
+  MlaArgs a{};
+  a.q_lat = (const __half*)q_lat;
+  a.kv_len = kv_len; a.pos_start = pos_start;
+  a.m = m; a.n_heads = n_heads; a.scale = scale;
+  a.out = (__half*)lat_out;
+  a.window = window; a.sinks = sinks;
+  const bool per_row = kv_len || row_seq;
+  return attend8(a, pg, dtype, mla8_dense_keys(m, pos_start, n_keys_hint, window, sinks, per_row), n_split, workspace, workspace_bytes,
+                 as_stream(stream));
+}
+
+HK_API int hk_mla8_sparse(const void* q_lat, const void* ckv8, const float* scales, int dtype, int64_t n_blocks, int block,
+                          const int* block_table, int table_stride, int n_seqs, const int* row_seq, const int* raw_idx, int kidx,
+                          void* lat_out, int m, int n_heads, float scale, int n_split, void* workspace, size_t workspace_bytes, void* stream) {
+  using namespace hk;
+  MlaPaged pg;
+  HK_REQUIRE(mla8_paged(&pg, ckv8, scales, dtype, n_blocks, block, block_table, table_stride, n_seqs, row_seq));
+  HK_REQUIRE(q_lat && lat_out && raw_idx && aligned(q_lat, 16) && aligned(lat_out, 16));
+  HK_REQUIRE(m >= 0 && kidx >= 0 && n_heads > 0 && n_heads % SIMT_HG == 0);
+  if (m == 0) return HK_OK;
+  MlaArgs a{};
+  a.q_lat = (const __half*)q_lat;
+  a.raw_idx = raw_idx; a.kidx = kidx;
+  a.m = m; a.n_heads = n_heads; a.scale = scale;
+  a.out = (__half*)lat_out;
+  return attend8(a, pg, dtype, kidx, n_split, workspace, workspace_bytes, as_stream(stream));
+}
 
 HK_API size_t hk_mla_partial_bytes(int n_split, int64_t rows) {
   if (n_split <= 0 || rows <= 0) return 0;
@@ -442,5 +533,26 @@ HK_API int hk_mla_splitkv_sparse_step(const void* q_lat, const void* ckv_shard, 
                           max_wait_ms, signal, as_stream(stream));
 }
 
+
+// Attention with a window and sinks over the fp16 cache: hk_mla_dense whose row of n keys sees p >= n - window and p < sinks only.
+HK_API int hk_mla_window(const void* q_lat, const void* ckv, int64_t ckv_rows, const int64_t* kv_base, const int* kv_len, int pos_start,
+                         int window, int sinks, void* lat_out, int m, int n_heads, float scale, int n_split, void* workspace,
+                         size_t workspace_bytes, void* stream) {
+  using namespace hk;
+  HK_REQUIRE(q_lat && ckv && lat_out && ckv_rows >= 0 && window >= 1 && sinks >= 0);
+  HK_REQUIRE(m >= 0 && pos_start >= 0 && n_heads > 0 && n_heads % SIMT_HG == 0 && (int64_t)pos_start + m <= INT32_MAX);
+  if (ckv_rows > 0 && !kv_base && !kv_len) HK_REQUIRE((int64_t)pos_start + m <= ckv_rows);
+  HK_REQUIRE(aligned(q_lat, 16) && aligned(ckv, 16) && aligned(lat_out, 16));
+  if (m == 0) return HK_OK;
+  if (n_split > LSE_MAX_SPLITS) return HK_ERR_UNSUPPORTED;
+  MlaArgs a{};
+  a.q_lat = (const __half*)q_lat; a.ckv = (const __half*)ckv; a.ckv_rows = ckv_rows;
+  a.kv_base = kv_base; a.kv_len = kv_len; a.pos_start = pos_start;
+  a.m = m; a.n_heads = n_heads; a.scale = scale;
+  a.out = (__half*)lat_out;
+  a.window = window; a.sinks = sinks;
+  return attend(a, mla_window_keys(kv_len ? pos_start : pos_start + m, window, sinks), n_split, n_split <= 0, workspace, workspace_bytes,
+                as_stream(stream));
+}
 
 #include "mla_splitkv_heads.cuh"

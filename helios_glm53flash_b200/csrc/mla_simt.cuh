@@ -4,6 +4,7 @@
 // src/cuda/attn/attn.cu:517-533).
 #pragma once
 #include "hk_common.cuh"
+#include "latent8.cuh"
 #include "mla_args.cuh"
 
 namespace hk {
@@ -12,9 +13,30 @@ constexpr int SIMT_HG = 4;  // heads per CTA
 
 
 
+// 16 values of a key as fp32: fp16 row, or 8-bit row and its block's scale
+template <int FMT>
+__device__ __forceinline__ void simt_key(const void* row, float scale, float (&kf)[16]) {
+  if (FMT == CACHE_F16) {
+    const uint4 u0 = *reinterpret_cast<const uint4*>(row), u1 = *(reinterpret_cast<const uint4*>(row) + 1);
+    const __half2* p0 = reinterpret_cast<const __half2*>(&u0);
+    const __half2* p1 = reinterpret_cast<const __half2*>(&u1);
+#pragma unroll
+    for (int u = 0; u < 4; u++) {
+      float2 f0 = __half22float2(p0[u]), f1 = __half22float2(p1[u]);
+      kf[2 * u] = f0.x; kf[2 * u + 1] = f0.y; kf[8 + 2 * u] = f1.x; kf[8 + 2 * u + 1] = f1.y;
+    }
+  } else {
+    const uint4 v = *reinterpret_cast<const uint4*>(row);
+    const uint8_t* b = reinterpret_cast<const uint8_t*>(&v);
+#pragma unroll
+    for (int u = 0; u < 16; u++) kf[u] = scale * latent8_value<FMT>(b[u]);
+  }
+}
+
 // grid (n_heads/4, n_split, m), 256 threads.  Warp w walks keys k0+w, k0+w+8, ...; lane owns 16
 // channels; the 8 warps are merged through shared memory at the end.
-__global__ __launch_bounds__(256) void mla_simt_kernel(MlaArgs a) {
+template <int FMT>
+__global__ __launch_bounds__(256) void mla_simt_kernel(MlaArgs a, MlaPaged pg) {
   extern __shared__ float smem[];
   float* w_acc = smem;                           // [8][4][512]
   float* w_m = smem + 8 * SIMT_HG * LATENT;      // [8][4]
@@ -23,13 +45,17 @@ __global__ __launch_bounds__(256) void mla_simt_kernel(MlaArgs a) {
   const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5;
   const int h0 = hg * SIMT_HG;
   const bool sparse = a.raw_idx != nullptr;
+  const int seq = FMT == CACHE_F16 ? 0 : pg.seq_of(r);
   int n;
   int64_t base = 0;
-  if (sparse) n = a.kidx;
+  KeyList list = {0, 0, 0};
+  if (sparse) n = seq < 0 ? 0 : a.kidx;
   else {
     n = a.kv_len ? a.kv_len[r] : a.pos_start + r + 1;
     base = a.kv_base ? a.kv_base[r] : 0;
-    if (a.ckv_rows > 0) n = (int)max((int64_t)0, min((int64_t)n, a.ckv_rows - base));
+    if (FMT == CACHE_F16 && a.ckv_rows > 0 && a.window <= 0) n = (int)max((int64_t)0, min((int64_t)n, a.ckv_rows - base));
+    list = key_list(seq < 0 ? 0 : n, a.window, a.sinks);
+    n = list.count();
   }
   const int per = (n + a.n_split - 1) / a.n_split;
   const int k0 = sp * per, k1 = min(n, k0 + per);
@@ -38,15 +64,9 @@ __global__ __launch_bounds__(256) void mla_simt_kernel(MlaArgs a) {
 #pragma unroll
   for (int h = 0; h < SIMT_HG; h++) {
     const __half* q = a.q_lat + ((size_t)r * a.n_heads + h0 + h) * LATENT + lane * 16;
-    uint4 u0 = *reinterpret_cast<const uint4*>(q), u1 = *reinterpret_cast<const uint4*>(q + 8);
-    const __half2* p0 = reinterpret_cast<const __half2*>(&u0);
-    const __half2* p1 = reinterpret_cast<const __half2*>(&u1);
+    simt_key<CACHE_F16>(q, 1.f, qf[h]);
 #pragma unroll
-    for (int u = 0; u < 4; u++) {
-      float2 f0 = __half22float2(p0[u]), f1 = __half22float2(p1[u]);
-      qf[h][2 * u] = f0.x * a.scale; qf[h][2 * u + 1] = f0.y * a.scale;
-      qf[h][8 + 2 * u] = f1.x * a.scale; qf[h][8 + 2 * u + 1] = f1.y * a.scale;
-    }
+    for (int u = 0; u < 16; u++) qf[h][u] *= a.scale;
   }
   float m_i[SIMT_HG], l_i[SIMT_HG], acc[SIMT_HG][16];
 #pragma unroll
@@ -57,17 +77,15 @@ __global__ __launch_bounds__(256) void mla_simt_kernel(MlaArgs a) {
     for (int u = 0; u < 16; u++) acc[h][u] = 0.f;
   }
   for (int i = k0 + wid; i < k1; i += 8) {
-    int64_t tok = sparse ? (int64_t)a.raw_idx[(size_t)r * a.kidx + i] : base + i;
-    if (tok < 0 || (a.ckv_rows > 0 && tok >= a.ckv_rows)) continue;  // warp-uniform
-    const __half* crow = a.ckv + (size_t)tok * LATENT + lane * 16;
-    uint4 u0 = *reinterpret_cast<const uint4*>(crow), u1 = *reinterpret_cast<const uint4*>(crow + 8);
-    const __half2* p0 = reinterpret_cast<const __half2*>(&u0);
-    const __half2* p1 = reinterpret_cast<const __half2*>(&u1);
+    int64_t tok = sparse ? (int64_t)a.raw_idx[(size_t)r * a.kidx + i] : base + list.at(i);
     float kf[16];
-#pragma unroll
-    for (int u = 0; u < 4; u++) {
-      float2 f0 = __half22float2(p0[u]), f1 = __half22float2(p1[u]);
-      kf[2 * u] = f0.x; kf[2 * u + 1] = f0.y; kf[8 + 2 * u] = f1.x; kf[8 + 2 * u + 1] = f1.y;
+    if (FMT == CACHE_F16) {
+      if (tok < 0 || (a.ckv_rows > 0 && tok >= a.ckv_rows)) continue;  // warp-uniform
+      simt_key<CACHE_F16>(a.ckv + (size_t)tok * LATENT + lane * 16, 1.f, kf);
+    } else {
+      const int64_t b = pg.block_of(seq, (int)tok);
+      if (b < 0) continue;
+      simt_key<FMT>(pg.data + (((size_t)b << pg.shift) + ((int)tok & ((1 << pg.shift) - 1))) * LATENT + lane * 16, pg.scales[b], kf);
     }
 #pragma unroll
     for (int h = 0; h < SIMT_HG; h++) {
@@ -113,10 +131,14 @@ __global__ __launch_bounds__(256) void mla_simt_kernel(MlaArgs a) {
         gl += sc * w_l[w * SIMT_HG + h];
         o += sc * w_acc[(w * SIMT_HG + h) * LATENT + ch];
       }
+    } else if (FMT != CACHE_F16) {                         // no key, or scores that are no numbers: NaN stays NaN
+#pragma unroll
+      for (int w = 0; w < 8; w++) gl += w_l[w * SIMT_HG + h];
+      o = gl;
     }
     const size_t rh = (size_t)r * a.n_heads + h0 + h;
     if (a.out) {
-      a.out[rh * LATENT + ch] = __float2half_rn(gl > 0.f ? o / gl : 0.f);
+      a.out[rh * LATENT + ch] = __float2half_rn(gl > 0.f || (FMT != CACHE_F16 && gl != 0.f) ? o / gl : 0.f);
     } else {
       a.part_acc[((size_t)sp * rows + rh) * LATENT + ch] = o;
       if (ch == 0) {

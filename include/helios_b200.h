@@ -36,8 +36,8 @@ typedef enum hk_status {
   HK_ERR_TIMEOUT = 5       /* a bounded device-side wait expired (see hk_read_device_status)      */
 } hk_status;
 
-/* dtype tags for the entry points that accept either 16-bit float format */
-enum { HK_F16 = 0, HK_BF16 = 1, HK_F32 = 2 };
+/* dtype tags for the entry points that accept either 16-bit float format; HK_I8 / HK_E4M3: values of the 8-bit latent cache */
+enum { HK_F16 = 0, HK_BF16 = 1, HK_F32 = 2, HK_I8 = 3, HK_E4M3 = 4 };
 
 const char* hk_status_string(int status);
 int hk_abi_version(void);
@@ -290,7 +290,64 @@ int hk_mla_dense(const void* q_lat, const void* ckv, int64_t ckv_rows, const int
                  int pos_start, void* lat_out, int m, int n_heads, float scale, int n_split,
                  void* workspace, size_t workspace_bytes, void* stream);
 
-/* Same two, but writing un-normalised split partials only (no combine): the building block of
+/* hk_mla_dense with a window and sinks: a row of n keys attends to its last `window` keys (p >= n - window) and to the first `sinks`
+ * (p < sinks), each key once; window >= 1, sinks >= 0.  Rows outside are not read (tiles of 64 keys that hold none that the row sees are
+ * skipped), and what lies there - infinities and NaN too - has no effect.  Other arguments as in hk_mla_dense; n stays what it is where
+ * ckv_rows cuts the range.  The library chooses the splits by the keys under the window.                                          */
+int hk_mla_window(const void* q_lat, const void* ckv, int64_t ckv_rows, const int64_t* kv_base, const int* kv_len,
+                  int pos_start, int window, int sinks, void* lat_out, int m, int n_heads, float scale, int n_split,
+                  void* workspace, size_t workspace_bytes, void* stream);
+
+/* ---------------------------------------------------------------------------------------------
+ * (b'') the latent cache in 8 bits, paged
+ *
+ *   ckv8 [n_blocks][block][512] int8 (HK_I8) or e4m3 (HK_E4M3), scales [n_blocks] f32: a latent is scales[b] * value; half the bytes of the
+ *   fp16 cache.  block: tokens of a block (a page), 16, 32, 64 or 128; n_blocks <= 2^31 - 1; ckv8 16-byte aligned, scales >= 0.
+ *   block_table [n_seqs][table_stride] int32: block number of a sequence's i-th block.  NULL: one sequence (n_seqs 1), block i is block i.
+ *   Positions behind the table, and entries that name no block (negative, >= n_blocks), hold no keys: they are skipped, never read.
+ *   row_seq [m]: the sequence of each query row (NULL: sequence 0); a number outside [0, n_seqs) makes a row without keys, whose output is 0.
+ * No counterpart in the reference, whose cache is fp16.  Calls that read and calls that write a block are ordered by the caller (a stream).
+ * ------------------------------------------------------------------------------------------- */
+
+/* RMS norm of new compressed-KV rows, y = kv_pre * ln_w * rsqrt(mean(kv_pre^2) + epsilon) as in hk_mla_cache_append, into the 8-bit cache.
+ * kv_pre [n][512] f32 (16-byte aligned), ln_w [512] f16 (16-byte aligned).  Sequence s appends rows seq_start[s] .. seq_start[s+1] - 1 (seq_start
+ * [n_seqs + 1] on the device; NULL: n / n_seqs rows each) at positions pos[s] .. (pos [n_seqs] int32 on the device); pos[s] < 0 skips the
+ * sequence, rows whose position has no block are dropped.
+ * A block without earlier rows of its sequence gets the scale max |y| / 127 (int8) or / 448 (e4m3); one with earlier rows (positions before pos[s]) keeps
+ * its scale, or, if a new row needs a larger one, takes that and its earlier rows are rounded again.  Rows of the block behind the new ones stay
+ * as they are.  A row that is not finite makes its block's scale NaN (and so every later output over it) until the block is begun anew.
+ * ckv_new (optional, 16-byte aligned) [n][512] f16: the rows as the cache holds them after the call (rows that are dropped: left as they were).
+ * A block may be written for one sequence of a call only.                                                                          */
+int hk_mla8_append(const float* kv_pre, const void* ln_w_f16, void* ckv8, float* scales, int dtype, int64_t n_blocks, int block,
+                   const int* block_table, int table_stride, int n_seqs, const int* seq_start, const int* pos, int n, float epsilon,
+                   void* ckv_new, void* stream);
+
+/* Positions pos .. pos + n - 1 of one sequence (block_table: its row of the table, or NULL) as fp16 rows: out [n][512] = f16(scale * value),
+ * zeros where there is no block; 16-byte aligned.                                                                                  */
+int hk_mla8_read(const void* ckv8, const float* scales, int dtype, int64_t n_blocks, int block, const int* block_table,
+                 int table_stride, int pos, int n, void* out_f16, void* stream);
+
+/* Number of splits that the library picks for m rows of n_keys keys over the 8-bit cache, and the workspace of a dense call that leaves the
+ * number to it (per_row: kv_len or row_seq is given, the keys of a row are then n_keys_hint, 4,096 where that is 0).  A call that gives
+ * n_split needs hk_mla_partial_bytes(n_split, m * n_heads) where n_split > 1; so does hk_mla8_sparse with hk_mla8_auto_splits.      */
+int hk_mla8_auto_splits(int m, int n_heads, int n_keys);
+size_t hk_mla8_dense_workspace_bytes(int m, int n_heads, int pos_start, int n_keys_hint, int window, int sinks, int per_row);
+
+/* hk_mla_dense over the 8-bit cache: row r attends to the first kv_len[r] positions of its sequence (kv_len NULL: pos_start + r + 1).
+ * window > 0: of these the last `window` and the first `sinks` only, as in hk_mla_window; window = 0: all.  n_heads: a multiple of 4.
+ * Scores and sums are fp32; a row without keys gives zeros.                                                                         */
+int hk_mla8_dense(const void* q_lat, const void* ckv8, const float* scales, int dtype, int64_t n_blocks, int block,
+                  const int* block_table, int table_stride, int n_seqs, const int* row_seq, const int* kv_len, int pos_start,
+                  int window, int sinks, void* lat_out, int m, int n_heads, float scale, int n_split, int n_keys_hint,
+                  void* workspace, size_t workspace_bytes, void* stream);
+
+/* hk_mla_sparse over the 8-bit cache: raw_idx [m][kidx] holds positions of the row's sequence (negative = skipped; duplicates count twice).  */
+int hk_mla8_sparse(const void* q_lat, const void* ckv8, const float* scales, int dtype, int64_t n_blocks, int block,
+                   const int* block_table, int table_stride, int n_seqs, const int* row_seq, const int* raw_idx, int kidx,
+                   void* lat_out, int m, int n_heads, float scale, int n_split, void* workspace, size_t workspace_bytes,
+                   void* stream);
+
+/* hk_mla_sparse and hk_mla_dense, but writing un-normalised split partials only (no combine): the building block of
  * split-KV across GPUs.  part_* point at storage for ONE split: m[rows], l[rows], acc[rows][512]. */
 int hk_mla_dense_partial(const void* q_lat, const void* ckv, const int64_t* kv_base,
                          const int* kv_len, int pos_start, float* part_m, float* part_l,

@@ -1,0 +1,415 @@
+"""The 8-bit paged latent cache (append, read, dense and sparse attention) and attention with a window and sinks, against 64 bits."""
+import math
+
+import pytest
+import torch
+
+import helios_glm53flash_b200 as hk
+import latent8_ref as ref
+from latent8_ref import STORE, attend, cache, check_append, rows_of, table_for, visible
+
+pytestmark = pytest.mark.gpu
+
+
+def gen_of(seed):
+    return torch.Generator(device="cuda").manual_seed(seed)
+
+
+def ints(v):
+    return torch.tensor(v, dtype=torch.int32, device="cuda")
+
+
+def queries(gen, m, heads):
+    return (torch.randn(m, heads, 512, device="cuda", generator=gen) * 0.7).half()
+
+
+def close(out, want):
+    """want: a list of (output, bound) per row"""
+    for r, (o, tol) in enumerate(want):
+        off = (out[r].double() - o).abs()
+        assert bool((off <= tol).all()), "row %d: off %.3e of %.3e" % (r, float((off - tol).max()), float(tol.max()))
+
+
+def finish():
+    torch.cuda.synchronize()
+    assert hk.read_device_status() == 0
+
+
+def inputs(gen, n, dtype=torch.float32):
+    x = torch.randn(n, 512, device="cuda", generator=gen) * torch.exp(torch.randn(n, 1, device="cuda", generator=gen))
+    return x, (1.0 + 0.1 * torch.randn(512, device="cuda", generator=gen)).half()
+
+
+# ---------------------------------------------------------------------------------------------
+# append, read
+# ---------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("kind", ["i8", "e4m3"])
+@pytest.mark.parametrize("block", [16, 32, 64, 128])
+@pytest.mark.parametrize("pos,rows", [([0], [1]), ([0], [16]), ([7], [1]), ([13], [200]), ([128], [128]), ([127], [2]),
+                                      ([0, 5, 130, 63], [1, 1, 1, 1]), ([3, 0, 40], [0, 300, 17])])
+def test_append(kind, block, pos, rows):
+    gen = gen_of(block + len(pos))
+    starts = [0]
+    for r in rows:
+        starts.append(starts[-1] + r)
+    blocks = max((p + r - 1) // block + 1 for p, r in zip(pos, rows))
+    n_blocks = blocks * len(pos) + 2
+    ckv8, scales = cache(gen, kind, n_blocks, block)
+    scales *= torch.exp(0.5 * torch.randn(n_blocks, device="cuda", generator=gen))       # some grow, some stay
+    scales *= 0.02
+    table = table_for(gen, len(pos), blocks, n_blocks)
+    x, w = inputs(gen, starts[-1])
+    old, old_s = ckv8.clone(), scales.clone()
+    new = torch.full((starts[-1], 512), 7.0, dtype=torch.float16, device="cuda")
+    kw = dict(seq_start=ints(starts)) if len(set(rows)) > 1 else {}
+    hk.mla8_cache_append(x, w, ckv8, scales, ints(pos), starts[-1], ref.EPS, block_table=table, n_seqs=len(pos), ckv_new=new, **kw)
+    finish()
+    check_append(old, old_s, ckv8, scales, x, w, table.cpu(), pos, starts, kind, ckv_new=new)
+    again, again_s = ckv8.clone(), scales.clone()
+    hk.mla8_cache_append(x, w, ckv8, scales, ints(pos), starts[-1], ref.EPS, block_table=table, n_seqs=len(pos), **kw)
+    finish()
+    assert torch.equal(ckv8.view(torch.uint8), again.view(torch.uint8)) and torch.equal(scales, again_s), "the same rows again change nothing"
+
+
+@pytest.mark.parametrize("kind", ["i8", "e4m3"])
+def test_append_one_token_after_another_and_read(kind):
+    """a block fills token by token: each step against the definition from the state before it; then everything read back"""
+    gen, block, n = gen_of(5), 32, 75
+    ckv8, scales = torch.zeros(4, block, 512, dtype=torch.int8, device="cuda").view(STORE[kind]), torch.full((4,), math.nan, device="cuda")
+    scales[3] = 0.5
+    table = ints([[2, 0, 1]])
+    x, w = inputs(gen, n)
+    roundings = torch.zeros(n, dtype=torch.float64, device="cuda")     # of each row so far
+    for p in range(n):
+        old, old_s = ckv8.clone(), scales.clone()
+        hk.mla8_cache_append(x[p:p + 1], w, ckv8, scales, ints([p]), 1, ref.EPS, block_table=table)
+        finish()
+        if p % block == 0:
+            old_s[table[0, p // block].item()] = 0.0             # a new block's old scale says nothing
+        check_append(old, old_s, ckv8, scales, x[p:p + 1], w, table.cpu(), [p], [0, 1], kind)
+        b = table[0, p // block].item()
+        roundings[p // block * block:p] += float(scales[b] != old_s[b])
+        roundings[p] = 1
+    out = torch.full((n + 30, 512), 3.0, dtype=torch.float16, device="cuda")
+    hk.mla8_cache_read(ckv8, scales, out, 0, n, block_table=table)
+    finish()
+    assert torch.equal(out[:n], rows_of(ckv8, scales, table[0], torch.arange(n, device="cuda")).half())
+    assert (out[n:] == 3.0).all()
+    # k roundings of a value: int8, half a step of a scale that only grows each time; e4m3, relative 2^-4 each time, or half the smallest step
+    y, s, k = ref.normed(x, w), scales[table[0].long()].double().repeat_interleave(block)[:n, None], roundings[:, None]
+    tol = k * s / 2 if kind == "i8" else y.abs() * ((1 + 2.0 ** -4) ** k - 1) + k * s * 2.0 ** -10
+    assert bool(((out[:n].double() - y).abs() <= tol * (1 + 2.0 ** -10) + y.abs() * 2.0 ** -10).all())
+
+
+@pytest.mark.parametrize("kind", ["i8", "e4m3"])
+def test_append_edges(kind):
+    """sequences without a place: a negative position, positions behind the table, entries that name no block; rows of zeros; rows
+    that are not finite"""
+    gen, block = gen_of(9), 16
+    ckv8, scales = cache(gen, kind, 8, block)
+    old, old_s = ckv8.clone(), scales.clone()
+    table = ints([[0, 1], [-1, 2], [3, 99], [4, 5]])
+    x, w = inputs(gen, 4 * 20)
+    x[60:80] = 0.0
+    pos, starts = [-1, 10, 14, 3], [0, 20, 40, 60, 80]
+    new = torch.full((80, 512), 7.0, dtype=torch.float16, device="cuda")
+    hk.mla8_cache_append(x, w, ckv8, scales, ints(pos), 80, ref.EPS, block_table=table, n_seqs=4, ckv_new=new)
+    finish()
+    check_append(old, old_s, ckv8, scales, x, w, table.cpu(), pos, starts, kind)
+    assert (new[:20] == 7).all() and (new[20:26] == 7).all() and (new[26:40] != 7).any() and (new[42:60] == 7).all()
+    assert (ckv8[5].view(torch.uint8)[:7] == 0).all() and scales[5] == 0, "a new block of zero rows"
+    assert torch.equal(ckv8[4].view(torch.uint8)[:3], old[4].view(torch.uint8)[:3]) and scales[4] == old_s[4]
+    for bad in (math.nan, math.inf, -math.inf):
+        x, w = inputs(gen, 3)
+        x[1, 77] = bad
+        hk.mla8_cache_append(x, w, ckv8, scales, ints([0]), 3, ref.EPS, block_table=table[:1].contiguous())
+        finish()
+        assert math.isnan(float(scales[0])) and torch.isfinite(scales[1:]).all()
+        hk.mla8_cache_append(x[:1], w, ckv8, scales, ints([5]), 1, ref.EPS, block_table=table[:1].contiguous())
+        finish()
+        assert math.isnan(float(scales[0])), "stays one until the block is begun anew"
+        hk.mla8_cache_append(x[:1], w, ckv8, scales, ints([0]), 1, ref.EPS, block_table=table[:1].contiguous())
+        finish()
+        assert math.isfinite(float(scales[0]))
+
+
+def test_read_of_holes_and_without_a_table():
+    gen = gen_of(3)
+    ckv8, scales = cache(gen, "i8", 4, 16)
+    out = torch.full((70, 512), 3.0, dtype=torch.float16, device="cuda")
+    hk.mla8_cache_read(ckv8, scales, out, 10, 60, block_table=ints([2, -1, 7, 0]))
+    finish()
+    want = torch.zeros(60, 512, dtype=torch.float16, device="cuda")
+    v = (ref.as_f64(ckv8) * scales.double()[:, None, None]).half()
+    want[:6], want[38:54] = v[2, 10:], v[0]
+    assert torch.equal(out[:60], want) and (out[60:] == 3).all()
+    hk.mla8_cache_read(ckv8, scales, out, 0, 64)
+    finish()
+    assert torch.equal(out[:64], v.view(64, 512))
+
+
+# ---------------------------------------------------------------------------------------------
+# attention over the 8-bit cache
+# ---------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("kind,block,heads,lens,window,sinks,n_split", [
+    ("i8", 64, 64, [1], 0, 0, 0), ("i8", 16, 64, [63, 64, 65], 0, 0, 1), ("e4m3", 32, 64, [1000], 0, 0, 0), ("i8", 128, 64, [129, 1, 517], 0, 0, 3),
+    ("e4m3", 16, 16, [300, 17, 0, 450], 0, 0, 0), ("i8", 64, 4, [700], 0, 0, 0), ("i8", 32, 128, [333, 90], 0, 0, 0), ("e4m3", 64, 100, [200], 0, 0, 2),
+    ("i8", 16, 64, [900, 100, 64, 5], 100, 4, 0), ("e4m3", 64, 64, [2000], 1, 0, 0), ("i8", 64, 32, [2000, 130], 64, 64, 2),
+    ("i8", 16, 64, [777], 129, 200, 1), ("e4m3", 128, 64, [1500, 1501], 1499, 1, 0), ("i8", 64, 64, [6000], 0, 0, 0)])
+def test_dense8_rows(kind, block, heads, lens, window, sinks, n_split):
+    """one query row a sequence, lengths on the device, pages anywhere"""
+    gen = gen_of(sum(lens) + block)
+    blocks = max(1, (max(lens) + block - 1) // block)
+    ckv8, scales = cache(gen, kind, blocks * len(lens) + 3, block, spread=1.0)
+    table = table_for(gen, len(lens), blocks, blocks * len(lens) + 3)
+    m = len(lens)
+    q = queries(gen, m, heads)
+    out = torch.full((m + 1, heads, 512), 5.0, dtype=torch.float16, device="cuda")
+    hk.mla8_dense_prefill(q, ckv8, scales, out, m, 0, n_heads=heads, block_table=table, row_seq=torch.arange(m, device="cuda", dtype=torch.int32),
+                          kv_len=ints(lens), window=window, sinks=sinks, n_split=n_split, n_keys_hint=max(lens))
+    finish()
+    close(out, [attend(q[r].double(), rows_of(ckv8, scales, table[r], visible(n, window, sinks)), 0.0625) for r, n in enumerate(lens)])
+    assert (out[m:] == 5.0).all()
+
+
+@pytest.mark.parametrize("kind,block,heads,pos,rows,window,sinks", [
+    ("i8", 64, 64, 0, 2, 0, 0), ("i8", 64, 64, 0, 70, 0, 0), ("e4m3", 32, 64, 333, 40, 0, 0), ("i8", 16, 16, 100, 9, 0, 0), ("i8", 64, 64, 1000, 130, 0, 0),
+    ("i8", 64, 64, 700, 90, 200, 4), ("e4m3", 128, 64, 10, 150, 64, 0), ("e4m3", 16, 64, 500, 80, 33, 130), ("i8", 32, 32, 50, 200, 1000, 7)])
+def test_dense8_chunk(kind, block, heads, pos, rows, window, sinks):
+    """a causal chunk of one sequence; blocks behind the sequence and spare blocks are NaN in scale"""
+    gen = gen_of(pos + rows)
+    blocks = (pos + rows + block - 1) // block
+    ckv8, scales = cache(gen, kind, blocks + 4, block, spread=0.5)
+    table = table_for(gen, 1, blocks + 1, blocks + 4)
+    spare = torch.ones(blocks + 4, dtype=torch.bool, device="cuda")
+    spare[table[0, :blocks].long()] = False
+    scales[spare] = math.nan
+    q = queries(gen, rows, heads)
+    out = torch.full((rows + 1, heads, 512), 5.0, dtype=torch.float16, device="cuda")
+    hk.mla8_dense_prefill(q, ckv8, scales, out, rows, pos, n_heads=heads, block_table=table, window=window, sinks=sinks)
+    finish()
+    close(out, [attend(q[r].double(), rows_of(ckv8, scales, table[0], visible(pos + r + 1, window, sinks)), 0.0625) for r in range(rows)])
+    assert (out[rows:] == 5.0).all()
+
+
+def test_dense8_without_a_table_and_another_scale():
+    gen = gen_of(2)
+    ckv8, scales = cache(gen, "i8", 9, 32)
+    q = queries(gen, 3, 64)
+    out = torch.empty(3, 64, 512, dtype=torch.float16, device="cuda")
+    hk.mla8_dense_prefill(q, ckv8, scales, out, 3, 280, scale=512 ** -0.5)
+    finish()
+    ident = torch.arange(9, device="cuda", dtype=torch.int32)
+    close(out, [attend(q[r].double(), rows_of(ckv8, scales, ident, visible(281 + r, 0, 0)), 512 ** -0.5) for r in range(3)])
+
+
+def test_dense8_rows_and_blocks_that_do_not_count():
+    """padding rows (a sequence number outside, a length of 0 or below), lengths behind the table, entries that name no block, blocks of
+    zeros, and blocks that no row sees which are NaN"""
+    gen, block = gen_of(4), 16
+    ckv8, scales = cache(gen, "e4m3", 12, block, spread=2.0)
+    ckv8[3] = 0.0
+    scales[3] = 0.0
+    ckv8[11] = math.nan
+    scales[11] = math.nan
+    table = ints([[0, 1, 2, 3], [4, -1, 12, 5], [11, 6, 7, 11]])
+    seqs, lens = [0, -1, 1, 3, 2, 0, 1, 0], [64, 64, 64, 64, 48, 0, 500, -5]
+    q = queries(gen, 8, 64)
+    out = torch.full((8, 64, 512), 5.0, dtype=torch.float16, device="cuda")
+    for splits in (0, 1, 4):
+        hk.mla8_dense_prefill(q, ckv8, scales, out, 8, 0, block_table=table, row_seq=ints(seqs), kv_len=ints(lens), window=32, sinks=0, n_split=splits,
+                              n_keys_hint=64)
+        finish()
+        want = []
+        for r, (s, n) in enumerate(zip(seqs, lens)):
+            p = visible(n, 32, 0) if 0 <= s < 3 else visible(0, 0, 0)
+            want.append(attend(q[r].double(), rows_of(ckv8, scales, table[max(s, 0) % 3], p), 0.0625))
+        close(out, want)
+        assert (out[[1, 3, 5, 6, 7]] == 0).all()
+
+
+def test_a_row_that_is_not_finite_is_seen_in_the_output():
+    gen = gen_of(6)
+    ckv8, scales = cache(gen, "i8", 4, 64)
+    scales[2] = math.nan
+    q = queries(gen, 1, 64)
+    out = torch.zeros(1, 64, 512, dtype=torch.float16, device="cuda")
+    for splits in (1, 2):
+        hk.mla8_dense_prefill(q, ckv8, scales, out, 1, 255, n_split=splits)
+        finish()
+        assert torch.isnan(out).all()
+        hk.mla8_dense_prefill(q, ckv8, scales, out, 1, 255, window=64, sinks=128, n_split=splits)
+        finish()
+        assert torch.isfinite(out).all()
+
+
+@pytest.mark.parametrize("kind,block,heads,m,kidx,n_split", [("i8", 64, 64, 1, 2052, 0), ("e4m3", 16, 64, 3, 130, 0), ("i8", 128, 16, 2, 1, 1), ("i8", 32, 64, 5, 64, 2),
+                                                             ("e4m3", 64, 64, 2, 700, 5), ("i8", 64, 64, 200, 70, 0)])
+def test_sparse8(kind, block, heads, m, kidx, n_split):
+    gen, n = gen_of(m + kidx), 3000
+    blocks = (n + block - 1) // block
+    ckv8, scales = cache(gen, kind, 2 * blocks + 1, block, spread=1.0)
+    table = table_for(gen, 2, blocks, 2 * blocks + 1)
+    seqs = [(i * 7) % 2 for i in range(m)]
+    idx = torch.randint(0, n, (m, kidx), device="cuda", generator=gen, dtype=torch.int32)
+    if kidx > 20:
+        idx[:, 3::7] = -1
+        idx[:, 4::50] = blocks * block + 5                      # behind the table
+        idx[0, 10:20] = idx[0, 0]                               # the same position again counts again
+        idx[m - 1, 64:] = -1
+    q = queries(gen, m, heads)
+    out = torch.full((m + 1, heads, 512), 5.0, dtype=torch.float16, device="cuda")
+    hk.mla8_sparse_decode(q, ckv8, scales, idx, kidx, out, m, n_heads=heads, block_table=table, row_seq=ints(seqs), n_split=n_split)
+    finish()
+    close(out, [attend(q[r].double(), rows_of(ckv8, scales, table[seqs[r]], idx[r][idx[r] >= 0].long()), 0.0625) for r in range(m)])
+    assert (out[m:] == 5.0).all()
+
+
+# ---------------------------------------------------------------------------------------------
+# window and sinks over the fp16 cache
+# ---------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("heads,lens,window,sinks,n_split", [
+    (64, [1], 1, 0, 0), (64, [64, 65, 200], 64, 0, 1), (64, [1000], 100, 4, 0), (64, [5000], 2000, 64, 0), (64, [900, 3, 0, 129], 128, 65, 0),
+    (64, [700, 701], 1, 0, 3), (16, [500, 40], 33, 2, 0), (64, [3000], 10000, 10000, 0), (64, [257], 64, 1, 2), (64, [4000], 63, 3999, 0)])
+def test_window_rows(heads, lens, window, sinks, n_split):
+    gen = gen_of(sum(lens) + window)
+    base = [sum(lens[:i]) for i in range(len(lens))]
+    ckv = torch.randn(sum(lens) + 1, 512, device="cuda", generator=gen).half()
+    for b, n in zip(base, lens):                               # what no row sees
+        hidden = torch.ones(n, dtype=torch.bool, device="cuda")
+        hidden[visible(n, window, sinks)] = False
+        ckv[b:b + n][hidden] = math.nan if n % 2 else math.inf
+    m = len(lens)
+    q = queries(gen, m, heads)
+    out = torch.full((m + 1, heads, 512), 5.0, dtype=torch.float16, device="cuda")
+    hk.mla_window_prefill(q, ckv, out, m, 0, window, sinks=sinks, n_heads=heads, kv_base=torch.tensor(base, device="cuda"), kv_len=ints(lens),
+                          n_split=n_split, n_keys_hint=max(lens))
+    finish()
+    close(out, [attend(q[r].double(), ckv[base[r]:base[r] + n][visible(n, window, sinks)].double(), 0.0625) for r, n in enumerate(lens)])
+    assert (out[m:] == 5.0).all()
+
+
+@pytest.mark.parametrize("pos,rows,window,sinks", [(0, 1, 1, 0), (0, 130, 64, 0), (500, 65, 100, 3), (1000, 37, 1000, 64), (200, 300, 1, 1), (3000, 21, 900, 130),
+                                                   (2000, 64, 1024, 4), (1500, 33, 1500, 0), (900, 150, 129, 0), (5000, 2, 4000, 10)])
+def test_window_chunk(pos, rows, window, sinks):
+    """a causal chunk; each row's first hidden key and everything before it is infinite or NaN for that row alone or for all"""
+    gen = gen_of(pos + rows)
+    ckv = torch.randn(pos + rows, 512, device="cuda", generator=gen).half()
+    lo = pos + 1 - window                                      # the first row's first key; the keys before it nobody sees
+    if lo > sinks:
+        ckv[sinks:lo] = math.nan
+    q = queries(gen, rows, 64)
+    out = torch.full((rows + 1, 64, 512), 5.0, dtype=torch.float16, device="cuda")
+    hk.mla_window_prefill(q, ckv, out, rows, pos, window, sinks=sinks)
+    finish()
+    close(out, [attend(q[r].double(), ckv[:pos + r + 1][visible(pos + r + 1, window, sinks)].double(), 0.0625) for r in range(rows)])
+    assert (out[rows:] == 5.0).all()
+
+
+@pytest.mark.parametrize("rows", [7, 8, 40])
+def test_window_rows_do_not_take_over_what_their_neighbours_see(rows):
+    """keys that leave the window one by one are infinite: the rows that still see one are not finite, the others are what they are without"""
+    gen, pos, window, sinks = gen_of(rows), 1200, 1000, 5
+    ckv = torch.randn(pos + rows, 512, device="cuda", generator=gen).half()
+    hot = pos + 1 - window + 3                                 # seen by rows 0 .. 3
+    ckv[hot] = math.inf
+    ckv[pos + rows - 1] = math.nan                             # the last row's own
+    q = queries(gen, rows, 64)
+    out = torch.empty(rows, 64, 512, dtype=torch.float16, device="cuda")
+    hk.mla_window_prefill(q, ckv, out, rows, pos, window, sinks=sinks)
+    finish()
+    clean = [r for r in range(rows - 1) if r > 3]
+    for r in clean:
+        o, tol = attend(q[r].double(), ckv[:pos + r + 1][visible(pos + r + 1, window, sinks)].double(), 0.0625)
+        assert bool(((out[r].double() - o).abs() <= tol).all()), r
+
+
+def test_window_cut_by_the_end_of_the_cache():
+    """a length behind the cache's end: the window stands where the length says, rows that are not there are skipped"""
+    gen = gen_of(8)
+    ckv = torch.randn(1000, 512, device="cuda", generator=gen).half()
+    q = queries(gen, 3, 64)
+    out = torch.empty(3, 64, 512, dtype=torch.float16, device="cuda")
+    hk.mla_window_prefill(q, ckv, out, 3, 0, 300, sinks=10, kv_base=torch.tensor([0, 200, 0], device="cuda"), kv_len=ints([1100, 900, 5000]), n_keys_hint=1000)
+    finish()
+    want = []
+    for base, n in ((0, 1100), (200, 900), (0, 5000)):
+        p = visible(n, 300, 10)
+        want.append(attend(q[len(want)].double(), ckv[base + p[base + p < 1000]].double(), 0.0625))
+    close(out, want)
+
+
+# ---------------------------------------------------------------------------------------------
+# together, as a server uses them
+# ---------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("kind", ["i8", "e4m3"])
+def test_prefill_then_decode_of_three_sequences(kind):
+    """chunks of three sequences into one pool of pages, then decode steps of all three: append, dense, windowed and sparse attention"""
+    gen, block, prompts, steps = gen_of(11), 16, [100, 37, 64], 5
+    blocks = 8
+    ckv8 = torch.zeros(3 * blocks, block, 512, dtype=torch.int8, device="cuda").view(STORE[kind])
+    scales = torch.zeros(3 * blocks, device="cuda")
+    table = table_for(gen, 3, blocks, 3 * blocks)
+    x, w = inputs(gen, sum(prompts))
+    starts = [0, 100, 137, 201]
+    held = torch.empty(sum(prompts), 512, dtype=torch.float16, device="cuda")
+    hk.mla8_cache_append(x, w, ckv8, scales, ints([0, 0, 0]), sum(prompts), ref.EPS, block_table=table, n_seqs=3, seq_start=ints(starts), ckv_new=held)
+    finish()
+    for s in range(3):
+        assert torch.equal(held[starts[s]:starts[s + 1]], rows_of(ckv8, scales, table[s], torch.arange(prompts[s], device="cuda")).half())
+    lens = ints(prompts)
+    row_seq = ints([0, 1, 2])
+    outs = torch.empty(3, 3, 64, 512, dtype=torch.float16, device="cuda")
+    for step in range(steps):
+        x, w2 = inputs(gen, 3)
+        before, before_s = ckv8.clone(), scales.clone()
+        hk.mla8_cache_append(x, w, ckv8, scales, lens, 3, ref.EPS, block_table=table, n_seqs=3)
+        pos = lens.tolist()
+        lens = lens + 1
+        q = queries(gen, 3, 64)
+        idx = torch.stack([torch.randint(0, n + 1, (40,), device="cuda", generator=gen) for n in pos]).int().contiguous()
+        args = dict(block_table=table, row_seq=row_seq)
+        hk.mla8_dense_prefill(q, ckv8, scales, outs[0], 3, 0, kv_len=lens, n_keys_hint=128, **args)
+        hk.mla8_dense_prefill(q, ckv8, scales, outs[1], 3, 0, kv_len=lens, n_keys_hint=128, window=20, sinks=2, **args)
+        hk.mla8_sparse_decode(q, ckv8, scales, idx, 40, outs[2], 3, **args)
+        finish()
+        check_append(before, before_s, ckv8, scales, x, w, table.cpu(), pos, [0, 1, 2, 3], kind)
+        for s, n in enumerate(pos):
+            for k, p in enumerate((visible(n + 1, 0, 0), visible(n + 1, 20, 2), idx[s].long())):
+                o, tol = attend(q[s].double(), rows_of(ckv8, scales, table[s], p), 0.0625)
+                assert bool(((outs[k, s].double() - o).abs() <= tol).all())
+
+
+def test_captured_decode_step_replayed():
+    """append and attention in one graph, positions and lengths on the device; the same bits as the calls, also on another stream"""
+    gen, block = gen_of(13), 64
+    ckv8, scales = cache(gen, "i8", 8, block)
+    table = ints([[5, 1], [0, 7]])
+    x, w = inputs(gen, 2)
+    q = queries(gen, 2, 64)
+    pos, lens, row_seq = ints([70, 13]), ints([71, 14]), ints([0, 1])
+    ws = torch.empty(max(256, hk.mla8_dense_workspace_bytes(2, 64, 0, 128, per_row=True)), dtype=torch.uint8, device="cuda")
+
+    def step(out, c, s, stream=None):
+        hk.mla8_cache_append(x, w, c, s, pos, 2, ref.EPS, block_table=table, n_seqs=2, stream=stream)
+        hk.mla8_dense_prefill(q, c, s, out, 2, 0, block_table=table, row_seq=row_seq, kv_len=lens, n_keys_hint=128, workspace=ws, stream=stream)
+
+    c2, s2 = ckv8.clone(), scales.clone()
+    out = torch.empty(2, 64, 512, dtype=torch.float16, device="cuda")
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        step(out, ckv8, scales)
+    want = torch.empty_like(out)
+    for k in range(3):
+        x.copy_(inputs(gen, 2)[0])
+        q.copy_(queries(gen, 2, 64))
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        step(want, c2, s2, stream=side if k == 1 else None)
+        finish()
+        assert torch.equal(out, want) and torch.equal(ckv8, c2) and torch.equal(scales, s2)
+        pos += 1
+        lens += 1
