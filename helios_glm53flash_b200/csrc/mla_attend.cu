@@ -14,6 +14,8 @@ namespace hk {
 // implemented in mla_flash_tc.cu; returns HK_ERR_UNSUPPORTED when the shape is not covered
 int mla_flash_tc_launch(const MlaArgs& a, cudaStream_t s, bool clusters = false);
 int mla_flash_tc_auto_splits(int m, int n_keys);
+// implemented in mla8_flash_tc.cu
+int mla8_flash_tc_launch(const MlaArgs& a, const MlaPaged& pg, int dtype, cudaStream_t s);
 // implemented in mla8_cache.cu
 bool mla8_paged(MlaPaged* pg, const void* ckv8, const float* scales, int dtype, int64_t n_blocks, int block, const int* block_table,
                 int table_stride, int n_seqs, const int* row_seq);
@@ -145,7 +147,12 @@ static int attend(MlaArgs a, int n_keys_hint, int n_split, bool choose, void* wo
   return HK_OK;
 }
 
-static int mla8_auto_splits(int m, int n_heads, int n_keys) { return simt_auto_splits(m, n_heads, n_keys); }
+// every 64 heads of a row are work of their own
+static int mla8_auto_splits(int m, int n_heads, int n_keys) {
+  if (force_simt()) return simt_auto_splits(m, n_heads, n_keys);
+  const int64_t rows = (int64_t)m * ((n_heads + 63) / 64);
+  return mla_flash_tc_auto_splits(rows > INT32_MAX ? INT32_MAX : (int)rows, n_keys);
+}
 
 // the 8-bit cache: final output, through split partials in the workspace where there is more than one split
 static int attend8(MlaArgs a, const MlaPaged& pg, int dtype, int n_keys_hint, int n_split, void* workspace, size_t workspace_bytes,
@@ -165,7 +172,8 @@ static int attend8(MlaArgs a, const MlaPaged& pg, int dtype, int n_keys_hint, in
     a.part_acc = (float*)(ws + pl.off_acc);
     a.out = nullptr;
   }
-  const int st = dtype == HK_I8 ? launch_simt_as<CACHE_I8>(a, pg, s) : launch_simt_as<CACHE_E4M3>(a, pg, s);
+  const int st = !force_simt() ? mla8_flash_tc_launch(a, pg, dtype, s)
+                 : dtype == HK_I8 ? launch_simt_as<CACHE_I8>(a, pg, s) : launch_simt_as<CACHE_E4M3>(a, pg, s);
   if (st != HK_OK || n_split == 1) return st;
   return combine(a.part_m, a.part_l, a.part_acc, n_split, rows, final_out, s);
 }
