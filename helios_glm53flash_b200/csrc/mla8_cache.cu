@@ -154,6 +154,7 @@ bool mla8_paged(MlaPaged* pg, const void* ckv8, const float* scales, int dtype, 
                 int table_stride, int n_seqs, const int* row_seq) {
   if (!ckv8 || !scales || (dtype != HK_I8 && dtype != HK_E4M3) || n_blocks < 1 || n_blocks > INT32_MAX || !aligned(ckv8, 16)) return false;
   if (block != 16 && block != 32 && block != 64 && block != 128) return false;
+  if (n_blocks * block > INT32_MAX) return false;          // rows are counted in 31 bits
   if (block_table ? table_stride < 1 || n_seqs < 1 : n_seqs != 1) return false;
   *pg = MlaPaged{};
   pg->data = (uint8_t*)ckv8;

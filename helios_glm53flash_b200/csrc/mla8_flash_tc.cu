@@ -11,6 +11,8 @@
 // Work item = (query row, 64 heads, key split) -> one CTA.  Roles, tensor-memory plan and products are those of mla_flash_tc_kernel; what is
 // its own are eight warps in place of the copy engine, which load a tile of 64 keys x 512 bytes into registers one tile ahead, turn it into
 // fp16 and store it in the 128-byte-swizzle layout that both products read.  Rows that the query does not see become zeros there.
+#include <cuda.h>   // CUtensorMap
+
 #include "latent8.cuh"
 #include "mla_args.cuh"
 #include "tc05.cuh"
@@ -36,9 +38,9 @@ constexpr float F8_MOVE = 8.0f, F8_MOVE_SCALE = 16.0f;
 struct F8Misc {
   uint64_t full[F8_NBUF], free[F8_NBUF];          // tile slot: converted, may be overwritten
   uint64_t s_full[2], s_free[2], p_full[2], pv_done[2];   // per tile parity
-  uint64_t q_ready;
-  float sc[F8_NBUF][F8_KEYS];                     // the keys' scales; -1: not seen
-  float mx[2][128];                               // tile maxima by softmax thread and tile parity; then sums, in the place that is idle
+  uint64_t q_full, q_ready;
+  alignas(16) float sc[F8_NBUF][F8_KEYS];                     // the keys' scales; -1: not seen
+  float mx[2][128];                               // tile maxima by softmax thread and tile parity; at the end sums, and the heads' factors
   uint32_t tmem;
   int abort_flag;
 };
@@ -109,8 +111,18 @@ __device__ __forceinline__ float f8_ld_float(const float* p) {
   return v;
 }
 
+// 64 rows x 512 fp16 channels in the 128-byte-swizzle layout
+__device__ __forceinline__ void f8_tma_box(void* smem_dst, const CUtensorMap* tmap, int row, uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(
+          tc::smem_u32(smem_dst)),
+      "l"(reinterpret_cast<uint64_t>(tmap)), "r"(0), "r"(row), "r"(0), "r"(tc::smem_u32(bar))
+      : "memory");
+}
+
 template <bool GATHER, int FMT>
-__global__ __launch_bounds__(F8_THREADS, 1) void mla8_flash_tc_kernel(MlaArgs a, MlaPaged pg, int* __restrict__ status) {
+__global__ __launch_bounds__(F8_THREADS, 1) void mla8_flash_tc_kernel(MlaArgs a, MlaPaged pg, int* __restrict__ status,
+                                                                              const __grid_constant__ CUtensorMap tmap_q) {
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* smem = smem_raw + ((1024u - (tc::smem_u32(smem_raw) & 1023u)) & 1023u);
   F8Misc& ms = *reinterpret_cast<F8Misc*>(smem + F8S_MISC);
@@ -130,6 +142,7 @@ __global__ __launch_bounds__(F8_THREADS, 1) void mla8_flash_tc_kernel(MlaArgs a,
       tc::mbar_init(&ms.p_full[b], 128);
       tc::mbar_init(&ms.pv_done[b], 1);
     }
+    tc::mbar_init(&ms.q_full, 1);
     tc::mbar_init(&ms.q_ready, 128);
     tc::mbar_fence_init();
     ms.abort_flag = 0;
@@ -141,6 +154,8 @@ __global__ __launch_bounds__(F8_THREADS, 1) void mla8_flash_tc_kernel(MlaArgs a,
   __syncthreads();
   tc::fence_after_sync();
   const uint32_t tmem = ms.tmem;
+  // An item of at most two tiles (a decode split) does not need the last tile slot back: S reads Q from there, and moving it is saved.
+  const bool direct_q = it.n_tiles < F8_NBUF;
   const int n_tiles = it.n_tiles, h0 = it.hg * F8_HEADS, n_h = min(F8_HEADS, a.n_heads - h0);
   bool ok = true;
 
@@ -164,16 +179,18 @@ __global__ __launch_bounds__(F8_THREADS, 1) void mla8_flash_tc_kernel(MlaArgs a,
     uint4 v[F8_ROWS];
     float sc = -1.f;
     // asks for key i of a tile
-    auto request = [&](int i, int64_t row) {
-      const int64_t at = __shfl_sync(0xffffffffu, row, i);
+    const uint8_t* src = pg.data + lane * 16;
+    auto request = [&](int i, int row) {
+      const int at = __shfl_sync(0xffffffffu, row, i);
       v[i] = make_uint4(0u, 0u, 0u, 0u);
-      if (at >= 0) v[i] = ld_stream16(pg.data + (size_t)at * LATENT + lane * 16);
+      if (at >= 0) v[i] = ld_stream16(src + (size_t)at * LATENT);
     };
     int p0 = position(0), p1 = position(1), p2 = position(2);
     int e0 = entry(p0), e1 = entry(p1);
-    auto row_of = [&](int p, int e) -> int64_t { return e < 0 || e >= pg.n_blocks ? -1 : ((int64_t)e << pg.shift) + (p & in_block); };
+    // row of the cache, -1: none (rows of a cache are counted in 31 bits)
+    auto row_of = [&](int p, int e) -> int { return e < 0 || e >= pg.n_blocks ? -1 : (e << pg.shift) + (p & in_block); };
     {
-      const int64_t row = row_of(p0, e0);
+      const int row = row_of(p0, e0);
       sc = row >= 0 ? f8_ld_float(pg.scales + e0) : -1.f;
 #pragma unroll
       for (int i = 0; i < F8_ROWS; i++) request(i, row);
@@ -182,7 +199,7 @@ __global__ __launch_bounds__(F8_THREADS, 1) void mla8_flash_tc_kernel(MlaArgs a,
     for (int t = 0; t < n_tiles; t++) {
       const int b = t % F8_NBUF;
       // the next tile: its rows are known; the one after: its table entries; the third: its positions
-      const int64_t row = row_of(p1, e1);
+      const int row = row_of(p1, e1);
       const float sc_next = row >= 0 ? f8_ld_float(pg.scales + e1) : -1.f;
       p1 = p2;
       e1 = entry(p2);
@@ -194,11 +211,11 @@ __global__ __launch_bounds__(F8_THREADS, 1) void mla8_flash_tc_kernel(MlaArgs a,
       // 16 channels are two 16-byte chunks of a 128-byte row; lanes four apart write them in the other order (no bank conflicts)
 #pragma unroll
       for (int i = 0; i < F8_ROWS; i++) {
-        uint4 lo, hi;
-        f8_to_f16<FMT>(v[i], lo, hi);
+        uint4 lo, hi;                                      // the chunk that is written first, the other
+        f8_to_f16<FMT>(swap ? make_uint4(v[i].z, v[i].w, v[i].x, v[i].y) : v[i], lo, hi);
         const uint32_t a0 = i * 128 + (((c0 + swap) ^ i) << 4), a1 = i * 128 + (((c0 + 1 - swap) ^ i) << 4);
-        *reinterpret_cast<uint4*>(dst + a0) = swap ? hi : lo;
-        *reinterpret_cast<uint4*>(dst + a1) = swap ? lo : hi;
+        *reinterpret_cast<uint4*>(dst + a0) = lo;
+        *reinterpret_cast<uint4*>(dst + a1) = hi;
         request(i, row);
       }
       sc = sc_next;
@@ -220,13 +237,19 @@ __global__ __launch_bounds__(F8_THREADS, 1) void mla8_flash_tc_kernel(MlaArgs a,
     };
     if (warp == 4) {
       const uint32_t idesc = tc::make_idesc(64, F8_KEYS, tc::FMT_F16, tc::FMT_F16, false, false);
-      if (n_tiles > 0) wait_u(&ms.q_ready, 0, 43);
+      if (n_tiles > 0) wait_u(direct_q ? &ms.q_full : &ms.q_ready, 0, 43);
       for (int t = 0; t < n_tiles; t++) {
         const int b = t & 1, kb = t % F8_NBUF;
         wait_u(&ms.full[kb], (t / F8_NBUF) & 1, 44);
         if (t >= 2) wait_u(&ms.s_free[b], ((t - 2) >> 1) & 1, 45);
         tc::fence_after_sync();
-        const uint64_t kd = desc(smem + F8S_K + kb * F8_TILE, 16), qd = desc(smem + F8S_Q, 16);
+        const uint64_t kd = desc(smem + F8S_K + kb * F8_TILE, 16), qd = desc(direct_q ? smem + F8S_K + (F8_NBUF - 1) * F8_TILE : smem + F8S_Q, 16);
+        if (direct_q) {
+#pragma unroll
+          for (int kk = 0; kk < LATENT / 16; kk++)
+            tc::mma_ws_f16_if(leader, tmem + F8_S + b * 32, tc::sdesc_advance(qd, (kk >> 2) * F8_BLK + (kk & 3) * 32),
+                              tc::sdesc_advance(kd, (kk >> 2) * F8_BLK + (kk & 3) * 32), idesc, kk > 0);
+        } else
 #pragma unroll
         for (int kk = 0; kk < LATENT / 16; kk++) {
           const uint64_t bd = tc::sdesc_advance(kd, (kk >> 2) * F8_BLK + (kk & 3) * 32);
@@ -238,6 +261,11 @@ __global__ __launch_bounds__(F8_THREADS, 1) void mla8_flash_tc_kernel(MlaArgs a,
         tc::mma_commit_if(leader, &ms.s_full[b]);
       }
     } else {
+      if (n_tiles > 0 && lane == 0) {
+        tc::mbar_arrive_expect_tx(&ms.q_full, F8_TILE);
+        f8_tma_box(smem + F8S_K + (F8_NBUF - 1) * F8_TILE, &tmap_q, it.r * a.n_heads + h0, &ms.q_full);
+      }
+      __syncwarp();
       const uint32_t idesc = tc::make_idesc(64, 256, tc::FMT_F16, tc::FMT_F16, false, true);
       for (int t = 0; t < n_tiles; t++) {
         const int b = t & 1, kb = t % F8_NBUF;
@@ -260,25 +288,10 @@ __global__ __launch_bounds__(F8_THREADS, 1) void mla8_flash_tc_kernel(MlaArgs a,
     const uint32_t lanes = (uint32_t)(warp * 32) << 16;
     const float sc2 = a.scale * F8_LOG2E;
     auto wait_pv = [&](int t, int code) { ok = tc::mbar_wait<F8_POLL_NS>(&ms.pv_done[t & 1], (t >> 1) & 1, abort_flag, code) && ok; };
-    if (n_tiles > 0) {
-      // Q: memory -> the last tile slot in the operand's layout (heads past the end are zeros) -> shared-memory operand and tensor memory
-      const uint4* q = reinterpret_cast<const uint4*>(a.q_lat + ((size_t)it.r * a.n_heads + h0) * LATENT);
-      uint8_t* land = smem + F8S_K + (F8_NBUF - 1) * F8_TILE;
-#pragma unroll 1
-      for (int i0 = 0; i0 < 32; i0 += 16) {
-        uint4 w[16];
-#pragma unroll
-        for (int i = 0; i < 16; i++) {
-          const int j = tid + 128 * (i0 + i);              // 16-byte piece j % 64 of head j / 64
-          w[i] = j < n_h * 64 ? ld_stream16(q + j) : make_uint4(0u, 0u, 0u, 0u);
-        }
-#pragma unroll
-        for (int i = 0; i < 16; i++) {
-          const int j = tid + 128 * (i0 + i);
-          *reinterpret_cast<uint4*>(land + tc::sw128_off(j >> 6, j & 63, F8_BLK)) = w[i];
-        }
-      }
-      asm volatile("bar.sync 3, 128;" ::: "memory");
+    if (!direct_q) {
+      // Q: the last tile slot -> shared-memory operand and tensor memory (heads past the end: whatever rows follow, whose results are not used)
+      const uint8_t* land = smem + F8S_K + (F8_NBUF - 1) * F8_TILE;
+      ok = tc::mbar_wait<F8_POLL_NS>(&ms.q_full, 0, abort_flag, 38) && ok;
 #pragma unroll
       for (int i = 0; i < (int)(F8_QS * F8_HEADS * 2 / 16 / 128); i++)
         reinterpret_cast<uint4*>(smem + F8S_Q)[tid + 128 * i] = reinterpret_cast<const uint4*>(land)[tid + 128 * i];
@@ -301,23 +314,39 @@ __global__ __launch_bounds__(F8_THREADS, 1) void mla8_flash_tc_kernel(MlaArgs a,
     for (int t = 0; t < n_tiles; t++) {
       const int b = t & 1, kb = t % F8_NBUF;
       ok = tc::mbar_wait<F8_POLL_NS>(&ms.full[kb], (t / F8_NBUF) & 1, abort_flag, 47) && ok;   // makes the scales visible
-      const float tile_sc = fmaxf(fmaxf(ms.sc[kb][lane], ms.sc[kb][lane + 32]), 0.f);
+      const float sc_lo = ms.sc[kb][lane], sc_hi = ms.sc[kb][lane + 32];
+      const bool hidden = __any_sync(0xffffffffu, fminf(sc_lo, sc_hi) < 0.f);
+      const float top = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(fmaxf(fmaxf(sc_lo, sc_hi), 0.f))));
       ok = tc::mbar_wait<F8_POLL_NS>(&ms.s_full[b], (t >> 1) & 1, abort_flag, 48) && ok;
       tc::fence_after_sync();
       uint32_t sv[32];
       tc::tmem_ld32(tmem + F8_S + b * 32 + lanes, sv);
-      const float top = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(tile_sc)));
+      const ulonglong2* ksc = reinterpret_cast<const ulonglong2*>(&ms.sc[kb][32 * half]);   // two pairs of scales a piece
       tc::tmem_ld_wait();
       tc::fence_before_sync();
       tc::mbar_arrive(&ms.s_free[b]);
-      const float* ksc = &ms.sc[kb][32 * half];
       float tmax = -INFINITY;
+      const uint64_t sc22 = pack2(sc2, sc2);
 #pragma unroll
-      for (int j = 0; j < 32; j++) {
-        const float s = ksc[j], x = s < 0.f ? -INFINITY : __uint_as_float(sv[j]) * (s * sc2);
-        sv[j] = __float_as_uint(x);
-        tmax = fmaxf(tmax, x);
+      for (int j = 0; j < 8; j++) {
+        const ulonglong2 k = ksc[j];
+#pragma unroll
+        for (int e = 0; e < 2; e++) {
+          const uint64_t x = mul2(mul2(e ? k.y : k.x, sc22), pack2(__uint_as_float(sv[4 * j + 2 * e]), __uint_as_float(sv[4 * j + 2 * e + 1])));
+          float x0, x1;
+          unpack2(x, x0, x1);
+          sv[4 * j + 2 * e] = __float_as_uint(x0);
+          sv[4 * j + 2 * e + 1] = __float_as_uint(x1);
+        }
       }
+      if (hidden) {                                        // (the edges of a range, gathered holes)
+        const float* own = &ms.sc[kb][32 * half];
+#pragma unroll
+        for (int j = 0; j < 32; j++)
+          if (own[j] < 0.f) sv[j] = __float_as_uint(-INFINITY);
+      }
+#pragma unroll
+      for (int j = 0; j < 32; j++) tmax = fmaxf(tmax, __uint_as_float(sv[j]));
       ms.mx[b][tid] = tmax;
       asm volatile("bar.sync %0, 64;" ::"r"(1 + (warp & 1)) : "memory");   // the two warps of these heads
       tmax = fmaxf(tmax, ms.mx[b][tid ^ 64]);
@@ -352,97 +381,97 @@ __global__ __launch_bounds__(F8_THREADS, 1) void mla8_flash_tc_kernel(MlaArgs a,
       if (t >= 2) wait_pv(t - 2, 50);                      // this parity's P has been read
       uint8_t* prow = smem + F8S_P + b * F8_P_BYTES;
       const float mref = m == -INFINITY ? 0.f : m;         // no key so far: exp2(-inf) = 0 below
-      float sum = 0.f;
+      const uint64_t neg = pack2(-mref, -mref), one = pack2(1.f, 1.f), inv2 = pack2(inv, inv);
+      uint64_t sum[2] = {0, 0};
 #pragma unroll
       for (int v = 0; v < 4; v++) {
         uint4 w;
         uint32_t* wp = &w.x;
+        const ulonglong2 k[2] = {ksc[2 * v], ksc[2 * v + 1]};
 #pragma unroll
         for (int e = 0; e < 4; e++) {
           const int j = 8 * v + 2 * e;
-          const float p0 = exp2f(__uint_as_float(sv[j]) - mref), p1 = exp2f(__uint_as_float(sv[j + 1]) - mref);
-          sum += p0 + p1;
-          const __half2 hp = __floats2half2_rn(p0 * (ksc[j] * inv), p1 * (ksc[j + 1] * inv));
+          float x0, x1;
+          unpack2(fma2(pack2(__uint_as_float(sv[j]), __uint_as_float(sv[j + 1])), one, neg), x0, x1);
+          const uint64_t p = pack2(exp2f(x0), exp2f(x1));
+          sum[e & 1] = fma2(p, one, sum[e & 1]);
+          unpack2(mul2(p, mul2(e & 1 ? k[e >> 1].y : k[e >> 1].x, inv2)), x0, x1);
+          const __half2 hp = __floats2half2_rn(x0, x1);
           wp[e] = *reinterpret_cast<const uint32_t*>(&hp);
         }
         *reinterpret_cast<uint4*>(prow + tc::sw128_off(head, half * 4 + v, F8_BLK)) = w;
       }
-      l += sum;
+      {
+        float s0, s1, s2, s3;
+        unpack2(sum[0], s0, s1);
+        unpack2(sum[1], s2, s3);
+        l += (s0 + s1) + (s2 + s3);
+      }
       tc::fence_async_smem();
       tc::fence_before_sync();
       tc::mbar_arrive(&ms.p_full[b]);
     }
-    // ---- epilogue ----
     ms.mx[n_tiles & 1][tid] = l;
     if (n_tiles > 0) wait_pv(n_tiles - 1, 51);
-    tc::fence_after_sync();
     asm volatile("bar.sync 3, 128;" ::: "memory");
     l += ms.mx[n_tiles & 1][tid ^ 64];
     const bool none = l == 0.f;                            // (NaN: a score was none)
-    const float f = none ? 0.f : a.out ? sref / l : sref;
-    auto load_o = [&](int c, uint32_t (&o)[32]) {          // 32 of this thread's 256 channels
+    if (half == 0) {
+      ms.mx[(n_tiles + 1) & 1][head] = none ? 0.f : a.out ? sref / l : sref;
+      if (!a.out && head < n_h) {
+        const size_t at = (size_t)it.sp * a.m * a.n_heads + (size_t)it.r * a.n_heads + h0 + head;
+        a.part_m[at] = m == -INFINITY || none ? -INFINITY : m / F8_LOG2E;
+        a.part_l[at] = l;
+      }
+    }
+    tc::fence_before_sync();
+  }
+  // ---- epilogue: O leaves through the idle tiles.  The softmax and converter warps of a lane quarter take 2, 3 and 3 of its 8 pieces of 32
+  // channels; then all twelve store whole rows (a bulk copy a head moved 27 bytes a cycle: 2.5 us for 128 KB, 0.4 us more). ----
+  if (warp < 4 || warp >= 6) {
+    asm volatile("bar.sync 4, 384;" ::: "memory");         // factors, and every product is complete
+    tc::fence_after_sync();
+    const int quarter = warp & 3, head = (quarter & 1) * 32 + lane, half = quarter >> 1, member = warp < 4 ? 0 : warp < 10 ? 1 : 2;
+    const uint32_t elem = a.out ? 2 : 4, pitch = LATENT * elem + 16;
+    const float f = ms.mx[(n_tiles + 1) & 1][head];
+    uint8_t* orow = smem + F8S_K + head * pitch;
+    for (int c = 32 * (3 * member - (member > 0)); c < 32 * (3 * member + 2); c += 32) {
+      uint32_t o[32];
       if (n_tiles > 0) {
-        tc::tmem_ld32(tmem + F8_O + c + lanes, o);
+        tc::tmem_ld32(tmem + F8_O + c + ((uint32_t)(quarter * 32) << 16), o);
         tc::tmem_ld_wait();
       }
 #pragma unroll
-      for (int j = 0; j < 32; j++) o[j] = none ? 0u : __float_as_uint(__uint_as_float(o[j]) * f);
-    };
-    if (a.out) {
-      // four rounds of 2 x 64 channels through the P buffers: channels 256 (c / 128) + 128 half + c % 128 ... of all heads
-#pragma unroll 1
-      for (int c = 0; c < 256; c += 64) {
-        uint8_t* box = smem + F8S_P + half * F8_P_BYTES;
-        asm volatile("bar.sync 3, 128;" ::: "memory");     // the round before has been read
+      for (int j = 0; j < 32; j++) o[j] = f == 0.f ? 0u : __float_as_uint(__uint_as_float(o[j]) * f);
+      uint8_t* dst = orow + ((c >> 7) * 256 + half * 128 + (c & 127)) * elem;
+      if (a.out) {
 #pragma unroll
-        for (int hc = 0; hc < 2; hc++) {
-          uint32_t o[32];
-          load_o(c + 32 * hc, o);
+        for (int v = 0; v < 4; v++) {
+          uint4 w;
+          uint32_t* wp = &w.x;
 #pragma unroll
-          for (int v = 0; v < 4; v++) {
-            uint4 w;
-            uint32_t* wp = &w.x;
-#pragma unroll
-            for (int e = 0; e < 4; e++) {
-              const __half2 h2 = __floats2half2_rn(__uint_as_float(o[8 * v + 2 * e]), __uint_as_float(o[8 * v + 2 * e + 1]));
-              wp[e] = *reinterpret_cast<const uint32_t*>(&h2);
-            }
-            *reinterpret_cast<uint4*>(box + tc::sw128_off(head, hc * 4 + v, F8_BLK)) = w;
+          for (int e = 0; e < 4; e++) {
+            const __half2 h2 = __floats2half2_rn(__uint_as_float(o[8 * v + 2 * e]), __uint_as_float(o[8 * v + 2 * e + 1]));
+            wp[e] = *reinterpret_cast<const uint32_t*>(&h2);
           }
+          *reinterpret_cast<uint4*>(dst + v * 16) = w;
         }
-        asm volatile("bar.sync 3, 128;" ::: "memory");
-        if (!*abort_flag) {
+      } else {
 #pragma unroll
-          for (int i = 0; i < 8; i++) {
-            const int j = tid + 128 * (i & 3), h = j >> 3, hf = i >> 2;
-            if (h < n_h)
-              *reinterpret_cast<uint4*>(a.out + ((size_t)it.r * a.n_heads + h0 + h) * LATENT + (c >> 7) * 256 + hf * 128 + (c & 127) + (j & 7) * 8) =
-                  *reinterpret_cast<const uint4*>(smem + F8S_P + hf * F8_P_BYTES + tc::sw128_off(h, j & 7, F8_BLK));
-          }
-        }
+        for (int v = 0; v < 8; v++) *reinterpret_cast<uint4*>(dst + v * 16) = make_uint4(o[4 * v], o[4 * v + 1], o[4 * v + 2], o[4 * v + 3]);
       }
-    } else {
-      // a partial: fp32 rows in the idle tiles, one bulk copy per head
-      const uint32_t pitch = LATENT * 4 + 16;
-      uint8_t* orow = smem + F8S_K + head * pitch;
-#pragma unroll 1
-      for (int c = 0; c < 256; c += 32) {
-        uint32_t o[32];
-        load_o(c, o);
-        const int ch = (c >> 7) * 256 + half * 128 + (c & 127);
-#pragma unroll
-        for (int v = 0; v < 8; v++)
-          *reinterpret_cast<uint4*>(orow + ch * 4 + v * 16) = make_uint4(o[4 * v], o[4 * v + 1], o[4 * v + 2], o[4 * v + 3]);
-      }
-      tc::fence_async_smem();
-      asm volatile("bar.sync 3, 128;" ::: "memory");
-      const size_t rows = (size_t)a.m * a.n_heads, rh = (size_t)it.r * a.n_heads + h0 + head;
-      if (half == 0 && head < n_h && !*abort_flag) {
-        tc::bulk_s2g(a.part_acc + ((size_t)it.sp * rows + rh) * LATENT, orow, LATENT * 4);
-        tc::bulk_commit();
-        a.part_m[(size_t)it.sp * rows + rh] = m == -INFINITY || none ? -INFINITY : m / F8_LOG2E;
-        a.part_l[(size_t)it.sp * rows + rh] = l;
-        tc::bulk_wait_read<0>();
+    }
+    asm volatile("bar.sync 4, 384;" ::: "memory");
+    if (!*abort_flag) {
+      const size_t first = (size_t)it.r * a.n_heads + h0;
+      uint8_t* dst = a.out ? reinterpret_cast<uint8_t*>(a.out + first * LATENT)
+                           : reinterpret_cast<uint8_t*>(a.part_acc + ((size_t)it.sp * a.m * a.n_heads + first) * LATENT);
+      const int team = warp < 4 ? warp : warp - 2;
+      const int per = a.out ? 2 : 4;                       // 512-byte pieces of a head
+#pragma unroll 8
+      for (int i = team; i < n_h * per; i += 12) {
+        const int h = a.out ? i >> 1 : i >> 2, c = (a.out ? i & 1 : i & 3) * 512 + lane * 16;
+        *reinterpret_cast<uint4*>(dst + (size_t)h * LATENT * elem + c) = *reinterpret_cast<const uint4*>(smem + F8S_K + h * pitch + c);
       }
     }
   }
@@ -453,7 +482,7 @@ __global__ __launch_bounds__(F8_THREADS, 1) void mla8_flash_tc_kernel(MlaArgs a,
 }
 
 template <bool GATHER, int FMT>
-int f8_launch(const MlaArgs& a, const MlaPaged& pg, cudaStream_t s) {
+int f8_launch(const MlaArgs& a, const MlaPaged& pg, const CUtensorMap& q, cudaStream_t s) {
   static bool attr_set[64] = {false};
   const int dev = device_index();
   if (!attr_set[dev]) {
@@ -463,15 +492,20 @@ int f8_launch(const MlaArgs& a, const MlaPaged& pg, cudaStream_t s) {
   }
   const int64_t items = (int64_t)a.n_split * a.m * ((a.n_heads + F8_HEADS - 1) / F8_HEADS);
   if (items > INT32_MAX) return HK_ERR_UNSUPPORTED;
-  const cudaError_t e = pdl_launch(mla8_flash_tc_kernel<GATHER, FMT>, dim3((unsigned)items), dim3(F8_THREADS), F8_SMEM, s, a, pg, device_status_ptr());
+  const cudaError_t e = pdl_launch(mla8_flash_tc_kernel<GATHER, FMT>, dim3((unsigned)items), dim3(F8_THREADS), F8_SMEM, s, a, pg, device_status_ptr(), q);
   return e == cudaSuccess && cudaPeekAtLastError() == cudaSuccess ? HK_OK : HK_ERR_CUDA;
 }
 
 }  // namespace
 
+// implemented in mla_flash_tc.cu
+bool mla_rows_map(CUtensorMap* m, const void* rows, int64_t n);
+
 int mla8_flash_tc_launch(const MlaArgs& a, const MlaPaged& pg, int dtype, cudaStream_t s) {
-  if (a.raw_idx) return dtype == HK_I8 ? f8_launch<true, CACHE_I8>(a, pg, s) : f8_launch<true, CACHE_E4M3>(a, pg, s);
-  return dtype == HK_I8 ? f8_launch<false, CACHE_I8>(a, pg, s) : f8_launch<false, CACHE_E4M3>(a, pg, s);
+  alignas(64) CUtensorMap q;
+  if (!mla_rows_map(&q, a.q_lat, (int64_t)a.m * a.n_heads)) return HK_ERR_UNSUPPORTED;
+  if (a.raw_idx) return dtype == HK_I8 ? f8_launch<true, CACHE_I8>(a, pg, q, s) : f8_launch<true, CACHE_E4M3>(a, pg, q, s);
+  return dtype == HK_I8 ? f8_launch<false, CACHE_I8>(a, pg, q, s) : f8_launch<false, CACHE_E4M3>(a, pg, q, s);
 }
 
 }  // namespace hk

@@ -172,8 +172,8 @@ static int attend8(MlaArgs a, const MlaPaged& pg, int dtype, int n_keys_hint, in
     a.part_acc = (float*)(ws + pl.off_acc);
     a.out = nullptr;
   }
-  const int st = !force_simt() ? mla8_flash_tc_launch(a, pg, dtype, s)
-                 : dtype == HK_I8 ? launch_simt_as<CACHE_I8>(a, pg, s) : launch_simt_as<CACHE_E4M3>(a, pg, s);
+  int st = force_simt() ? HK_ERR_UNSUPPORTED : mla8_flash_tc_launch(a, pg, dtype, s);
+  if (st == HK_ERR_UNSUPPORTED) st = dtype == HK_I8 ? launch_simt_as<CACHE_I8>(a, pg, s) : launch_simt_as<CACHE_E4M3>(a, pg, s);
   if (st != HK_OK || n_split == 1) return st;
   return combine(a.part_m, a.part_l, a.part_acc, n_split, rows, final_out, s);
 }

@@ -772,6 +772,15 @@ static FtEncodeFn ft_encode_fn() {
   return fn;
 }
 
+// tensor map of n rows of 512 fp16 channels in boxes of 64 rows x 512 channels, 128-byte swizzle
+bool mla_rows_map(CUtensorMap* m, const void* rows, int64_t n) {
+  const FtEncodeFn encode = ft_encode_fn();
+  const cuuint64_t dims[3] = {64, (cuuint64_t)n, 8}, strides[2] = {LATENT * 2, 128};
+  const cuuint32_t box[3] = {64, 64, 8}, ones[3] = {1, 1, 1};
+  return encode && encode(m, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, const_cast<void*>(rows), dims, strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                          CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 int mla_flash_tc_launch(const MlaArgs& a, cudaStream_t s, bool clusters) {
   FtEncodeFn encode = ft_encode_fn();
   if (a.n_heads != FT_HEADS || !encode) return HK_ERR_UNSUPPORTED;

@@ -302,7 +302,7 @@ int hk_mla_window(const void* q_lat, const void* ckv, int64_t ckv_rows, const in
  * (b'') the latent cache in 8 bits, paged
  *
  *   ckv8 [n_blocks][block][512] int8 (HK_I8) or e4m3 (HK_E4M3), scales [n_blocks] f32: a latent is scales[b] * value; half the bytes of the
- *   fp16 cache.  block: tokens of a block (a page), 16, 32, 64 or 128; n_blocks <= 2^31 - 1; ckv8 16-byte aligned, scales >= 0.
+ *   fp16 cache.  block: tokens of a block (a page), 16, 32, 64 or 128; n_blocks * block < 2^31; ckv8 16-byte aligned, scales >= 0.
  *   block_table [n_seqs][table_stride] int32: block number of a sequence's i-th block.  NULL: one sequence (n_seqs 1), block i is block i.
  *   Positions behind the table, and entries that name no block (negative, >= n_blocks), hold no keys: they are skipped, never read.
  *   row_seq [m]: the sequence of each query row (NULL: sequence 0); a number outside [0, n_seqs) makes a row without keys, whose output is 0.
