@@ -454,7 +454,7 @@ def mla_window_prefill(q_lat, ckv, lat_out, qlen, pos_start, window, sinks=0, st
     if splits > 1 and ws is None:
         ws = _scratch(mla_partial_bytes(splits, qlen * n_heads), q_lat.device, stream)
     _run("hk_mla_window", q_lat, ckv, ckv if ckv_rows is None else ckv_rows, kv_base, kv_len, pos_start, window, sinks, lat_out, qlen,
-         n_heads, scale, splits, ws, ws, stream)
+         n_heads, scale, n_split if n_heads == 64 else splits, ws, ws, stream)
 
 
 # ---- the latent cache in 8 bits, paged: ckv8 [n_blocks, block, 512] of torch.int8 or torch.float8_e4m3fn, scales [n_blocks] float32,

@@ -111,7 +111,7 @@ int mla_window_keys(int n, int window, int sinks) {
 // which may then merge one row's splits in clusters; a number of splits that the caller gives means that many CTAs a row.
 static int attend(MlaArgs a, int n_keys_hint, int n_split, bool choose, void* workspace, size_t workspace_bytes,
                   cudaStream_t s) {
-  const bool tc = (a.n_heads == 64) && !force_simt() && a.window == 0;
+  const bool tc = (a.n_heads == 64) && !force_simt();
   if (n_split <= 0)
     n_split = tc ? mla_flash_tc_auto_splits(a.m, n_keys_hint)
                  : simt_auto_splits(a.m, a.n_heads, n_keys_hint);
@@ -124,7 +124,7 @@ static int attend(MlaArgs a, int n_keys_hint, int n_split, bool choose, void* wo
     if (!aligned(workspace, 256)) return HK_ERR_INVALID;
     // Few rows of few tiles: one kernel whose clusters merge the splits.  The rows' tiles are known for gathered rows and causal
     // ranges; where each row has a length of its own on the device, fewer splits than the GPU has room for mean two tiles each.
-    const int tiles = a.raw_idx || !a.kv_len ? (n_keys_hint + 63) / 64 : (int64_t)a.m * (n_split + 1) <= sm_count() ? 2 * n_split : 1 << 20;
+    const int tiles = a.raw_idx || !a.kv_len || a.window ? (n_keys_hint + 63) / 64 : (int64_t)a.m * (n_split + 1) <= sm_count() ? 2 * n_split : 1 << 20;
     MlaArgs c = a;
     // That is the form for a call that has the GPU to itself: its 64 SMs where the splits alone are 17 CTAs cost several calls side by
     // side more than each gains, which the library cannot see and the caller says with a number of splits (a step of 11 MLA layers at

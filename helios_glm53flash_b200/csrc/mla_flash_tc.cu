@@ -101,12 +101,19 @@ struct FtItem {
   int r, sp, cs, k0, k1, n_tiles;                 // cs: part of the output channels (cluster form)
   bool mini;                                      // cluster form: the ragged last tile comes first, from memory of its own
   int64_t base;
-  __device__ __forceinline__ int keys(int t) const { return min(FT_KEYS, k1 - k0 - t * FT_KEYS); }
+  // window form: keys p >= lo and p < head of the row's k1 are seen; tile i of its list is tile i, or i + jump behind the sinks' tiles
+  int head, lo, head_tiles, jump, t0;
+  bool win;
+  __device__ __forceinline__ int key0(int t) const { return win ? (t0 + t < head_tiles ? t0 + t : t0 + t + jump) * FT_KEYS : k0 + t * FT_KEYS; }   // first key of a tile
+  __device__ __forceinline__ int keys(int t) const { return min(FT_KEYS, k1 - key0(t)); }
+  __device__ __forceinline__ bool sees(int p) const { return !win || p >= lo || p < head; }
+  __device__ __forceinline__ bool whole(int t) const { return keys(t) == FT_KEYS && (!win || key0(t) >= lo || key0(t) + FT_KEYS <= head); }
   __device__ __forceinline__ int nth(int i) const { return mini ? (i ? i - 1 : n_tiles - 1) : i; }   // the tile that is i-th in turn
 };
-template <bool G4, bool CL>
+template <bool G4, bool CL, bool WIN>
 __device__ __forceinline__ FtItem ft_item(const MlaArgs& a, int idx) {
   FtItem it;
+  it.win = WIN;
   it.sp = idx % a.n_split;
   it.r = idx / a.n_split;
   it.cs = 0;
@@ -123,10 +130,30 @@ __device__ __forceinline__ FtItem ft_item(const MlaArgs& a, int idx) {
   } else {
     n = a.kv_len ? a.kv_len[it.r] : a.pos_start + it.r + 1;
     it.base = a.kv_base ? a.kv_base[it.r] : 0;
+    if (WIN) {
+      const KeyList k = key_list(n, a.window, a.sinks);
+      it.lo = k.lo;
+      it.head = k.head;
+      n = k.n;
+    }
     if (a.ckv_rows > 0) n = (int)max((int64_t)0, min((int64_t)n, a.ckv_rows - it.base));   // never past the end of the cache
   }
   // split boundaries on tile granularity
-  const int tiles = (n + FT_KEYS - 1) / FT_KEYS, per = (tiles + a.n_split - 1) / a.n_split;
+  int tiles = (n + FT_KEYS - 1) / FT_KEYS;
+  if (WIN) {                                               // (where the cache's end cuts the range, its last tiles may hold no key that is seen)
+    it.head_tiles = min((it.head + FT_KEYS - 1) / FT_KEYS, tiles);
+    it.jump = max(min(it.lo / FT_KEYS, tiles) - it.head_tiles, 0);
+    tiles -= it.jump;
+  }
+  const int per = (tiles + a.n_split - 1) / a.n_split;
+  if (WIN) {
+    it.t0 = min(tiles, CL ? tiles * it.sp / a.n_split : it.sp * per);
+    it.n_tiles = min(tiles, CL ? tiles * (it.sp + 1) / a.n_split : (it.sp + 1) * per) - it.t0;
+    it.k0 = 0;
+    it.k1 = n;
+    it.mini = CL && it.n_tiles > 2 && it.keys(it.n_tiles - 1) <= FT_MINI;
+    return it;
+  }
   // (cluster form: a fixed number of splits, so the tiles are shared out evenly)
   it.k0 = min(n, (CL ? tiles * it.sp / a.n_split : it.sp * per) * FT_KEYS);
   it.k1 = min(n, (CL ? tiles * (it.sp + 1) / a.n_split : (it.sp + 1) * per) * FT_KEYS);
@@ -171,7 +198,8 @@ __device__ __forceinline__ void tma_gather4_rows(uint32_t leader, uint32_t smem_
 // What bounds it is latency, one thing after another on 64 SMs: row numbers 1,200 cycles, gathered keys 2,800, two tiles of S, softmax and
 // P V 3,800, laying out and the barrier of the cluster 1,700, the shares 2,200, the merge 1,600.  2,052 gathered rows of one query 10.8 ->
 // 9.2 us; MLA layer of one token at 5,001 32.1 -> 28.9, selection and attention at 262,144 23.8 -> 21.8.
-template <bool G4, bool CL>
+// WIN: dense ranges of which a row sees its last keys and its first ones only (a.window, a.sinks).
+template <bool G4, bool CL, bool WIN>
 __global__ __launch_bounds__(FT_THREADS, 1) void mla_flash_tc_kernel(
     MlaArgs a, int* __restrict__ status, const __grid_constant__ CUtensorMap tmap_box, const __grid_constant__ CUtensorMap tmap_rows,
     const __grid_constant__ CUtensorMap tmap_q, const __grid_constant__ CUtensorMap tmap_o) {
@@ -209,7 +237,7 @@ __global__ __launch_bounds__(FT_THREADS, 1) void mla_flash_tc_kernel(
   }
   if (warp == 0) tc::tmem_alloc(&ms.tmem, 512);
   pdl_wait();
-  if (!CL && step >= n_items) direct_q = ft_item<G4, CL>(a, blockIdx.x).n_tiles < FT_NBUF;
+  if (!CL && step >= n_items) direct_q = ft_item<G4, CL, WIN>(a, blockIdx.x).n_tiles < FT_NBUF;
   tc::fence_before_sync();
   __syncthreads();
   tc::fence_after_sync();
@@ -229,8 +257,8 @@ __global__ __launch_bounds__(FT_THREADS, 1) void mla_flash_tc_kernel(
     const uint32_t leader = tc::elect_one();
     // cache row of key slot lw * SLOTS + lane of a tile, -1 = hole; volatile, so that a look-ahead load is issued where it stands
     auto row_of = [&](const FtItem& it, int tile) -> int {
-      const int p = it.k0 + tile * FT_KEYS + lw * FT_SLOTS + lane;
-      if (lane >= FT_SLOTS || p >= it.k1) return -1;
+      const int p = it.key0(tile) + lw * FT_SLOTS + lane;
+      if (lane >= FT_SLOTS || p >= it.k1 || !it.sees(p)) return -1;
       if (!G4) return (int)(it.base + p);
       int v;
       asm volatile("ld.global.nc.s32 %0, [%1];" : "=r"(v) : "l"(a.raw_idx + (size_t)it.r * a.kidx + p));
@@ -240,14 +268,14 @@ __global__ __launch_bounds__(FT_THREADS, 1) void mla_flash_tc_kernel(
     auto in_cache = [&](int v) -> int { return (v < 0 || (a.ckv_rows > 0 && (int64_t)v >= a.ckv_rows)) ? -1 : v; };
     // Gathered row numbers are fetched two tiles ahead (the row list of a query is read once, from HBM), across rows.
     int cur = -1, nxt = -1, ahead_item = blockIdx.x, ahead_tile = 0;
-    FtItem ahead = ft_item<G4, CL>(a, ahead_item);
+    FtItem ahead = ft_item<G4, CL, WIN>(a, ahead_item);
     auto fetch = [&]() -> int {
       if (!G4 || ahead_item >= n_items || ahead.n_tiles == 0) return -1;   // (gathered rows: every item has the same keys)
       const int v = row_of(ahead, ahead.nth(ahead_tile));
       if (++ahead_tile == ahead.n_tiles) {
         ahead_tile = 0;
         ahead_item += step;
-        if (ahead_item < n_items) ahead = ft_item<G4, CL>(a, ahead_item);
+        if (ahead_item < n_items) ahead = ft_item<G4, CL, WIN>(a, ahead_item);
       }
       return v;
     };
@@ -264,7 +292,7 @@ __global__ __launch_bounds__(FT_THREADS, 1) void mla_flash_tc_kernel(
       return b;
     };
     for (int idx = blockIdx.x; idx < n_items; idx += step) {
-      const FtItem it = ft_item<G4, CL>(a, idx);
+      const FtItem it = ft_item<G4, CL, WIN>(a, idx);
       if (it.n_tiles == 0) continue;
       {
         const int b = next_slot(it, -1);
@@ -291,11 +319,11 @@ __global__ __launch_bounds__(FT_THREADS, 1) void mla_flash_tc_kernel(
         const int b = next_slot(it, i);
         if (lane < FT_SLOTS / 8) ms.mask[b][lw * (FT_SLOTS / 8) + lane] = (uint8_t)(valid >> (8 * lane));
         __syncwarp();
-        if (!G4 && it.keys(tile) == FT_KEYS) {             // a whole tile of a dense range: one box
+        if (!G4 && it.whole(tile)) {                       // a whole tile of a dense range: one box
           if (lane == 0) {
             if (lw == 0) {
               tc::mbar_arrive_expect_tx(&ms.full[b], FT_TILE);
-              tma_load_tile(smem + FS_K + b * FT_TILE, &tmap_box, (int)(it.base + it.k0 + tile * FT_KEYS), &ms.full[b]);
+              tma_load_tile(smem + FS_K + b * FT_TILE, &tmap_box, (int)(it.base + it.key0(tile)), &ms.full[b]);
             } else {
               tc::mbar_arrive(&ms.full[b]);
             }
@@ -343,7 +371,7 @@ __global__ __launch_bounds__(FT_THREADS, 1) void mla_flash_tc_kernel(
         return tc::make_sdesc_sw128(addr, 16, 1024);
       };
       for (int idx = blockIdx.x; idx < n_items; idx += step) {
-        const FtItem it = ft_item<G4, CL>(a, idx);
+        const FtItem it = ft_item<G4, CL, WIN>(a, idx);
         const int n_tiles = it.n_tiles;
         if (n_tiles == 0) continue;
         if (direct_q) wait_u(&ms.full[0], 0, 15);
@@ -380,7 +408,7 @@ __global__ __launch_bounds__(FT_THREADS, 1) void mla_flash_tc_kernel(
     } else {
       const uint32_t idesc = tc::make_idesc(64, 256, tc::FMT_F16, tc::FMT_F16, false, true);
       for (int idx = blockIdx.x; idx < n_items; idx += step) {
-        const FtItem it = ft_item<G4, CL>(a, idx);
+        const FtItem it = ft_item<G4, CL, WIN>(a, idx);
         if (it.n_tiles == 0) continue;
         u++;
         for (int tile = 0; tile < it.n_tiles; tile++, u++, g++) {
@@ -451,14 +479,14 @@ __global__ __launch_bounds__(FT_THREADS, 1) void mla_flash_tc_kernel(
       u++;
     };
     auto next_row = [&](int idx) {                         // the first item from idx on that has keys
-      while (idx < n_items && ft_item<G4, CL>(a, idx).n_tiles == 0) idx += step;
+      while (idx < n_items && ft_item<G4, CL, WIN>(a, idx).n_tiles == 0) idx += step;
       return idx;
     };
     int q_item = next_row(blockIdx.x);                     // the row whose Q is moved next
     if (direct_q) u = 1;
     else if (q_item < n_items) move_q();
     for (int idx = blockIdx.x; idx < n_items; idx += step) {
-      const FtItem it = ft_item<G4, CL>(a, idx);
+      const FtItem it = ft_item<G4, CL, WIN>(a, idx);
       float m = -INFINITY, l = 0.f;
       for (int tile = 0; tile < it.n_tiles; tile++, u++, g++) {
         const int b = g & 1, kb = slot_of(it, u, tile);
@@ -647,7 +675,7 @@ __global__ __launch_bounds__(FT_THREADS, 1) void mla_flash_tc_kernel(
     }
     ok = tc::mbar_wait(&ms.q_ready, 0, abort_flag, 16) && ok;   // every split's share of this CTA's heads has arrived
     cluster_arrive();
-    const FtItem it = ft_item<G4, CL>(a, blockIdx.x);
+    const FtItem it = ft_item<G4, CL, WIN>(a, blockIdx.x);
     const int n_h = FT_HEADS / a.n_split, row = FT_CL_ROW, share = n_h * (row + 8), chunks = row / 16;
     if (!*abort_flag) {
       for (int i = tid; i < n_h * chunks; i += FT_THREADS) {
@@ -709,13 +737,13 @@ static int ft_prepare() {
   int dev = 0;
   cudaGetDevice(&dev);
   if (dev >= 0 && dev < 64 && !attr_set[dev]) {
-    if (cudaFuncSetAttribute(mla_flash_tc_kernel<false, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)FS_SMEM) != cudaSuccess ||
-        cudaFuncSetAttribute(mla_flash_tc_kernel<true, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)FS_SMEM) != cudaSuccess ||
-        cudaFuncSetAttribute(mla_flash_tc_kernel<false, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)FS_SMEM) != cudaSuccess ||
-        cudaFuncSetAttribute(mla_flash_tc_kernel<true, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)FS_SMEM) != cudaSuccess ||
-        cudaFuncSetAttribute(mla_pair_tc_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)FS_SMEM) != cudaSuccess ||
-        cudaFuncSetAttribute(mla_flash_tc_kernel<false, true>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess ||
-        cudaFuncSetAttribute(mla_flash_tc_kernel<true, true>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess)
+    auto whole_sm = [](auto* kernel) { return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)FS_SMEM) == cudaSuccess; };
+    auto any_cluster = [](auto* kernel) { return cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) == cudaSuccess; };
+    if (!whole_sm(mla_flash_tc_kernel<false, false, false>) || !whole_sm(mla_flash_tc_kernel<true, false, false>) ||
+        !whole_sm(mla_flash_tc_kernel<false, true, false>) || !whole_sm(mla_flash_tc_kernel<true, true, false>) ||
+        !whole_sm(mla_flash_tc_kernel<false, false, true>) || !whole_sm(mla_flash_tc_kernel<false, true, true>) || !whole_sm(mla_pair_tc_kernel) ||
+        !any_cluster(mla_flash_tc_kernel<false, true, false>) || !any_cluster(mla_flash_tc_kernel<true, true, false>) ||
+        !any_cluster(mla_flash_tc_kernel<false, true, true>))
       return HK_ERR_CUDA;
     attr_set[dev] = true;
   }
@@ -747,7 +775,7 @@ bool mla_flash_cluster_shape(int m, int tiles, int* n_split) {
     cfg.attrs = attr;
     cfg.numAttrs = 1;
     int n = 0;
-    if (cudaOccupancyMaxActiveClusters(&n, mla_flash_tc_kernel<true, true>, &cfg) != cudaSuccess) n = 0;
+    if (cudaOccupancyMaxActiveClusters(&n, mla_flash_tc_kernel<true, true, false>, &cfg) != cudaSuccess) n = 0;
     fit[dev][lg] = n + 1;
   }
   const int room = fit[dev][lg] - 1;
@@ -815,7 +843,7 @@ int mla_flash_tc_launch(const MlaArgs& a, cudaStream_t s, bool clusters) {
   // Two rows of a causal chunk share their keys.  Below 700 keys a row on average the pair's own costs (a cluster to start, the later row's own
   // key as a tile) are more than it gains: us, a CTA a row / pairs, 148 rows at 300 15.3 / 15.4, at 600 19.7 / 19.5, at 1,000 25.5 / 24.2;
   // 500 at 300 65.7 / 67.8, at 700 89.7 / 86.5; 1,200 at 0 151 / 154, 1,500 209 / 208, 2,500 470 / 431.
-  const bool pairs = !clusters && !a.raw_idx && !a.kv_len && !a.kv_base && a.out && a.n_split == 1 && a.m >= 2 && a.pos_start + a.m / 2 >= FT_PAIR_KEYS;
+  const bool pairs = !clusters && !a.window && !a.raw_idx && !a.kv_len && !a.kv_base && a.out && a.n_split == 1 && a.m >= 2 && a.pos_start + a.m / 2 >= FT_PAIR_KEYS;
   if (!box_map(&qmap, a.q_lat, q_rows) || (!a.raw_idx && !pairs && !box_map(&box, a.ckv, extent))) return HK_ERR_UNSUPPORTED;
   if (a.out) {
     const cuuint64_t dims[2] = {LATENT, q_rows};
@@ -836,17 +864,14 @@ int mla_flash_tc_launch(const MlaArgs& a, cudaStream_t s, bool clusters) {
   // each (600 rows at 32,768 keys 2.72 ms, persistent 2.85).  Partials always: their rows leave through the idle ring.
   if (clusters) {
     const dim3 grid((unsigned)(a.m * FT_CS * a.n_split));
-    const cudaError_t e = a.raw_idx ? pdl_launch_cluster(a.n_split, mla_flash_tc_kernel<true, true>, grid, dim3(FT_THREADS), FS_SMEM, s, a,
-                                                         device_status_ptr(), box, rows, qmap, omap)
-                                    : pdl_launch_cluster(a.n_split, mla_flash_tc_kernel<false, true>, grid, dim3(FT_THREADS), FS_SMEM, s, a,
-                                                         device_status_ptr(), box, rows, qmap, omap);
+    const auto kernel = a.raw_idx ? mla_flash_tc_kernel<true, true, false> : a.window ? mla_flash_tc_kernel<false, true, true> : mla_flash_tc_kernel<false, true, false>;
+    const cudaError_t e = pdl_launch_cluster(a.n_split, kernel, grid, dim3(FT_THREADS), FS_SMEM, s, a, device_status_ptr(), box, rows, qmap, omap);
     return e == cudaSuccess && cudaPeekAtLastError() == cudaSuccess ? HK_OK : HK_ERR_CUDA;
   }
   const int64_t items = (int64_t)a.n_split * a.m;
   const dim3 grid((unsigned)(a.raw_idx && a.out && items > sm_count() ? sm_count() : items));
-  const cudaError_t e =
-      a.raw_idx ? pdl_launch(mla_flash_tc_kernel<true, false>, grid, dim3(FT_THREADS), FS_SMEM, s, a, device_status_ptr(), box, rows, qmap, omap)
-                : pdl_launch(mla_flash_tc_kernel<false, false>, grid, dim3(FT_THREADS), FS_SMEM, s, a, device_status_ptr(), box, rows, qmap, omap);
+  const auto kernel = a.raw_idx ? mla_flash_tc_kernel<true, false, false> : a.window ? mla_flash_tc_kernel<false, false, true> : mla_flash_tc_kernel<false, false, false>;
+  const cudaError_t e = pdl_launch(kernel, grid, dim3(FT_THREADS), FS_SMEM, s, a, device_status_ptr(), box, rows, qmap, omap);
   return e == cudaSuccess && cudaPeekAtLastError() == cudaSuccess ? HK_OK : HK_ERR_CUDA;
 }
 
