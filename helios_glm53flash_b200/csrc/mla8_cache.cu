@@ -127,24 +127,42 @@ __global__ void __launch_bounds__(1024) mla8_append_kernel(AppendArgs a) {
   }
 }
 
+// rows i of out: position i of the sequence below `head`, i + shift from there on; f16(scale * value), zeros where there is no block.
+// A warp four rows, a lane eight channels and the eight 256 further on (8-byte loads, 16-byte stores).
+constexpr int READ_ROWS = 4;
 template <int FMT>
-__global__ void __launch_bounds__(256) mla8_read_kernel(MlaPaged pg, int pos, int n, __half* __restrict__ out) {
+__global__ void __launch_bounds__(256) mla8_read_kernel(MlaPaged pg, int head, int shift, int n, __half* __restrict__ out) {
   pdl_release();
   pdl_wait();
-  const int lane = threadIdx.x & 31, i = (blockIdx.x * blockDim.x + threadIdx.x) >> 5;
-  if (i >= n) return;
-  const int p = pos + i;
-  const int64_t b = pg.block_of(0, p);
-  uint4 v = make_uint4(0u, 0u, 0u, 0u);
-  float s = 0.f;
-  if (b >= 0) {
-    v = *reinterpret_cast<const uint4*>(pg.data + (((size_t)b << pg.shift) + (p & ((1 << pg.shift) - 1))) * LATENT + lane * 16);
-    s = pg.scales[b];
-  }
-  const uint8_t* v8 = reinterpret_cast<const uint8_t*>(&v);
-  __half* dst = out + (size_t)i * LATENT + lane * 16;
+  const int lane = threadIdx.x & 31, i0 = (blockIdx.x * 8 + (threadIdx.x >> 5)) * READ_ROWS;
+  uint2 v[READ_ROWS][2];
+  float s[READ_ROWS];
 #pragma unroll
-  for (int c = 0; c < 16; c++) dst[c] = __float2half_rn(latent8_value<FMT>(v8[c]) * s);
+  for (int k = 0; k < READ_ROWS; k++) {
+    const int i = i0 + k, p = i < head ? i : i + shift;
+    const int64_t b = i < n ? pg.block_of(0, p) : -1;
+    s[k] = 0.f;
+    v[k][0] = v[k][1] = make_uint2(0u, 0u);
+    if (b >= 0) {
+      const uint2* row = reinterpret_cast<const uint2*>(pg.data + (((size_t)b << pg.shift) + (p & ((1 << pg.shift) - 1))) * LATENT);
+      v[k][0] = row[lane];
+      v[k][1] = row[lane + 32];
+      s[k] = pg.scales[b];
+    }
+  }
+#pragma unroll
+  for (int k = 0; k < READ_ROWS; k++) {
+    if (i0 + k >= n) break;
+#pragma unroll
+    for (int h = 0; h < 2; h++) {
+      const uint8_t* v8 = reinterpret_cast<const uint8_t*>(&v[k][h]);
+      uint4 w;
+      __half2* w2 = reinterpret_cast<__half2*>(&w);
+#pragma unroll
+      for (int c = 0; c < 4; c++) w2[c] = __floats2half2_rn(latent8_value<FMT>(v8[2 * c]) * s[k], latent8_value<FMT>(v8[2 * c + 1]) * s[k]);
+      reinterpret_cast<uint4*>(out + (size_t)(i0 + k) * LATENT)[lane + 32 * h] = w;
+    }
+  }
 }
 
 }  // namespace
@@ -166,6 +184,14 @@ bool mla8_paged(MlaPaged* pg, const void* ckv8, const float* scales, int dtype, 
   pg->n_seqs = n_seqs;
   pg->row_seq = row_seq;
   return true;
+}
+
+// n rows of sequence 0 as fp16: positions 0 .. head - 1, then head + shift ..
+int mla8_read_launch(const MlaPaged& pg, int dtype, int head, int shift, int n, __half* out, cudaStream_t s) {
+  return pdl_launch(dtype == HK_I8 ? mla8_read_kernel<CACHE_I8> : mla8_read_kernel<CACHE_E4M3>, dim3((unsigned)((n + 8 * READ_ROWS - 1) / (8 * READ_ROWS))),
+                    dim3(256), 0, s, pg, head, shift, n, out) == cudaSuccess
+             ? HK_OK
+             : HK_ERR_CUDA;
 }
 
 }  // namespace hk
@@ -200,9 +226,5 @@ HK_API int hk_mla8_read(const void* ckv8, const float* scales, int dtype, int64_
   MlaPaged pg;
   HK_REQUIRE(out_f16 && pos >= 0 && n >= 0 && (int64_t)pos + n <= INT32_MAX && aligned(out_f16, 16));
   HK_REQUIRE(mla8_paged(&pg, ckv8, scales, dtype, n_blocks, block, block_table, table_stride, 1, nullptr));
-  if (n == 0) return HK_OK;
-  return pdl_launch(dtype == HK_I8 ? mla8_read_kernel<CACHE_I8> : mla8_read_kernel<CACHE_E4M3>, dim3((n + 7) / 8), dim3(256), 0,
-                    as_stream(stream), pg, pos, n, (__half*)out_f16) == cudaSuccess
-             ? HK_OK
-             : HK_ERR_CUDA;
+  return n == 0 ? HK_OK : mla8_read_launch(pg, dtype, 0, pos, n, (__half*)out_f16, as_stream(stream));
 }

@@ -187,11 +187,12 @@ __global__ __launch_bounds__(F8_THREADS, 1) void mla8_flash_tc_kernel(MlaArgs a,
     };
     int p0 = position(0), p1 = position(1), p2 = position(2);
     int e0 = entry(p0), e1 = entry(p1);
-    // row of the cache, -1: none (rows of a cache are counted in 31 bits)
+    // row of the cache, -1: none (rows of a cache are counted in 31 bits).  In a chunk a seen position without a block is a key of zeros.
+    const bool zeros = !GATHER && !a.kv_len && !pg.row_seq;
     auto row_of = [&](int p, int e) -> int { return e < 0 || e >= pg.n_blocks ? -1 : (e << pg.shift) + (p & in_block); };
     {
       const int row = row_of(p0, e0);
-      sc = row >= 0 ? f8_ld_float(pg.scales + e0) : -1.f;
+      sc = row >= 0 ? f8_ld_float(pg.scales + e0) : zeros && p0 >= 0 ? 0.f : -1.f;
 #pragma unroll
       for (int i = 0; i < F8_ROWS; i++) request(i, row);
     }
@@ -200,7 +201,7 @@ __global__ __launch_bounds__(F8_THREADS, 1) void mla8_flash_tc_kernel(MlaArgs a,
       const int b = t % F8_NBUF;
       // the next tile: its rows are known; the one after: its table entries; the third: its positions
       const int row = row_of(p1, e1);
-      const float sc_next = row >= 0 ? f8_ld_float(pg.scales + e1) : -1.f;
+      const float sc_next = row >= 0 ? f8_ld_float(pg.scales + e1) : zeros && p1 >= 0 ? 0.f : -1.f;
       p1 = p2;
       e1 = entry(p2);
       p2 = position(t + 3);

@@ -23,6 +23,7 @@ struct MlaArgs {
   float* part_acc;
   // window > 0: a row of n keys attends to the keys p >= n - window and p < sinks only
   int window, sinks;
+  int keep_nan;             // scores that are no numbers make outputs that are none (0: zeros, as the fp16 cache's callers know it)
 };
 
 // The 8-bit latent cache: blocks of `1 << shift` tokens x 512 values, one fp32 scale a block; a key is scale * value.

@@ -567,7 +567,8 @@ __global__ __launch_bounds__(FT_THREADS, 1) void mla_flash_tc_kernel(
       tc::fence_after_sync();
       asm volatile("bar.sync 3, 128;" ::: "memory");
       l += ms.l[tid ^ 64];
-      const float f = l > 0.f ? (final_out && !CL ? 1.f / l : 1.f) : 0.f;
+      const bool some = l > 0.f || (a.keep_nan && l != 0.f);
+      const float f = some ? (final_out && !CL ? 1.f / l : 1.f) : 0.f;
       if (CL) cluster_arrive();                            // this CTA's ring is idle
       auto load_o = [&](int c0, uint32_t (&o)[32]) {       // 32 of this thread's 256 channels, weighed
         if (it.n_tiles > 0) {
@@ -575,7 +576,7 @@ __global__ __launch_bounds__(FT_THREADS, 1) void mla_flash_tc_kernel(
           tc::tmem_ld_wait();
         }
 #pragma unroll
-        for (int j = 0; j < 32; j++) o[j] = l > 0.f ? __float_as_uint(__uint_as_float(o[j]) * f) : 0u;
+        for (int j = 0; j < 32; j++) o[j] = some ? __float_as_uint(__uint_as_float(o[j]) * f) : 0u;
       };
       if (CL) {
         // The accumulator goes to the cluster's CTAs by heads: CTA j merges n_h of them.  It is laid out by destination in the idle
@@ -697,7 +698,7 @@ __global__ __launch_bounds__(FT_THREADS, 1) void mla_flash_tc_kernel(
           gl = fmaf(w, x.y, gl);
           o.x = fmaf(w, v.x, o.x); o.y = fmaf(w, v.y, o.y); o.z = fmaf(w, v.z, o.z); o.w = fmaf(w, v.w, o.w);
         }
-        const float inv = gl > 0.f ? 1.f / gl : 0.f;
+        const float inv = gl > 0.f || (a.keep_nan && gl != 0.f) ? 1.f / gl : 0.f;
         const __half2 h0 = __floats2half2_rn(o.x * inv, o.y * inv), h1 = __floats2half2_rn(o.z * inv, o.w * inv);
         uint2 w;
         w.x = *reinterpret_cast<const uint32_t*>(&h0);

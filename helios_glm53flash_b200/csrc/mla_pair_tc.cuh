@@ -388,7 +388,8 @@ __global__ __launch_bounds__(PT_THREADS, 1) void mla_pair_tc_kernel(
     tc::fence_after_sync();
     asm volatile("bar.sync 3, 128;" ::: "memory");
     l += ms.l[tid ^ 64];
-    const float f = l > 0.f ? 1.f / l : 0.f;
+    const bool some = l > 0.f || (a.keep_nan && l != 0.f);
+    const float f = some ? 1.f / l : 0.f;
 #pragma unroll 1
     for (int c0 = 0; c0 < 256; c0 += 64) {
       uint8_t* box = smem + FS_P + half * FP_BYTES;
@@ -405,7 +406,7 @@ __global__ __launch_bounds__(PT_THREADS, 1) void mla_pair_tc_kernel(
           uint32_t* wp = &w.x;
 #pragma unroll
           for (int e = 0; e < 4; e++) {
-            const float x0 = l > 0.f ? __uint_as_float(o[8 * v + 2 * e]) * f : 0.f, x1 = l > 0.f ? __uint_as_float(o[8 * v + 2 * e + 1]) * f : 0.f;
+            const float x0 = some ? __uint_as_float(o[8 * v + 2 * e]) * f : 0.f, x1 = some ? __uint_as_float(o[8 * v + 2 * e + 1]) * f : 0.f;
             const __half2 h2 = __floats2half2_rn(x0, x1);
             wp[e] = *reinterpret_cast<const uint32_t*>(&h2);
           }

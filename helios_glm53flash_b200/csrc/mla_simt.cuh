@@ -84,8 +84,11 @@ __global__ __launch_bounds__(256) void mla_simt_kernel(MlaArgs a, MlaPaged pg) {
       simt_key<CACHE_F16>(a.ckv + (size_t)tok * LATENT + lane * 16, 1.f, kf);
     } else {
       const int64_t b = pg.block_of(seq, (int)tok);
-      if (b < 0) continue;
-      simt_key<FMT>(pg.data + (((size_t)b << pg.shift) + ((int)tok & ((1 << pg.shift) - 1))) * LATENT + lane * 16, pg.scales[b], kf);
+      if (b < 0 && (sparse || a.kv_len || pg.row_seq)) continue;   // (in a chunk: a key of zeros)
+      if (b < 0) {
+#pragma unroll
+        for (int u = 0; u < 16; u++) kf[u] = 0.f;
+      } else simt_key<FMT>(pg.data + (((size_t)b << pg.shift) + ((int)tok & ((1 << pg.shift) - 1))) * LATENT + lane * 16, pg.scales[b], kf);
     }
 #pragma unroll
     for (int h = 0; h < SIMT_HG; h++) {

@@ -335,7 +335,10 @@ size_t hk_mla8_dense_workspace_bytes(int m, int n_heads, int pos_start, int n_ke
 
 /* hk_mla_dense over the 8-bit cache: row r attends to the first kv_len[r] positions of its sequence (kv_len NULL: pos_start + r + 1).
  * window > 0: of these the last `window` and the first `sinks` only, as in hk_mla_window; window = 0: all.  n_heads: a multiple of 4.
- * Scores and sums are fp32; a row without keys gives zeros.                                                                         */
+ * Scores and sums are fp32; a row without keys gives zeros.
+ * A chunk (kv_len and row_seq NULL) is checked on the host, pos_start + m positions have a place in the table (else HK_ERR_INVALID); in it a
+ * position whose entry names no block is a latent of zeros, as hk_mla8_read gives it.  A chunk of 64 heads and 64 rows or more, with n_split <= 0,
+ * reads its positions as fp16 rows into the workspace first and attends to those (latents beyond 65,504 are infinite there).        */
 int hk_mla8_dense(const void* q_lat, const void* ckv8, const float* scales, int dtype, int64_t n_blocks, int block,
                   const int* block_table, int table_stride, int n_seqs, const int* row_seq, const int* kv_len, int pos_start,
                   int window, int sinks, void* lat_out, int m, int n_heads, float scale, int n_split, int n_keys_hint,

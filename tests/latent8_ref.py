@@ -75,12 +75,13 @@ def visible(n, window, sinks):
     return p[(p >= n - window) | (p < sinks)] if window else p
 
 
-def attend(q, keys, scale):
+def attend(q, keys, scale, rows16=False):
     """q [heads][512], keys [n][512] in 64 bits -> (output, what it may be off by).
 
     P and the output are rounded to fp16 (half a step is 2^-11 relative), scores are fp32 sums of 512 products scaled twice: with S the sum of
     magnitudes, 520 roundings at most of relative 2^-24 of it, which move a weight by as much relatively, and the normaliser too.  Weights
-    below 2^-10 of the largest may be subnormal in fp16: 2^-25 absolute, times 16 where a block's scale is that much below the largest."""
+    below 2^-10 of the largest may be subnormal in fp16: 2^-25 absolute, times 16 where a block's scale is that much below the largest.
+    rows16: the keys have been rounded to fp16 first, 2^-11 relative of each product of a score and of each value that is weighed."""
     if not keys.shape[0]:
         z = torch.zeros(q.shape[0], 512, dtype=torch.float64, device=q.device)
         return z, z
@@ -88,9 +89,9 @@ def attend(q, keys, scale):
     p = torch.exp(s - s.amax(1, keepdim=True))
     tot = p.sum(1, keepdim=True)
     o, mag = p @ keys / tot, p @ keys.abs() / tot
-    eta = 2.0 ** -24 * 520 * (q.abs() @ keys.abs().T).amax(1, keepdim=True) * scale + 2.0 ** -20 * (1 + s.abs().amax(1, keepdim=True)) + keys.shape[0] * 2.0 ** -24
+    eta = (2.0 ** -24 * 520 + (2.0 ** -11 if rows16 else 0.0)) * (q.abs() @ keys.abs().T).amax(1, keepdim=True) * scale + 2.0 ** -20 * (1 + s.abs().amax(1, keepdim=True)) + keys.shape[0] * 2.0 ** -24
     small = (p < 2.0 ** -10).sum(1, keepdim=True) * 2.0 ** -25 * 16 * keys.abs().max() / tot
-    return o, 2.0 ** -11 * (mag + o.abs()) * 1.01 + 2 * eta * mag + small + 2.0 ** -25
+    return o, 2.0 ** -11 * (mag * (2 if rows16 else 1) + o.abs()) * 1.01 + 2 * eta * mag + small + 2.0 ** -25
 
 
 def cache(gen, kind, n_blocks, block, spread=0.0):

@@ -188,8 +188,38 @@ def test_dense8_chunk(kind, block, heads, pos, rows, window, sinks):
     out = torch.full((rows + 1, heads, 512), 5.0, dtype=torch.float16, device="cuda")
     hk.mla8_dense_prefill(q, ckv8, scales, out, rows, pos, n_heads=heads, block_table=table, window=window, sinks=sinks)
     finish()
-    close(out, [attend(q[r].double(), rows_of(ckv8, scales, table[0], visible(pos + r + 1, window, sinks)), 0.0625) for r in range(rows)])
+    rows16 = rows >= 64 and heads == 64
+    close(out, [attend(q[r].double(), rows_of(ckv8, scales, table[0], visible(pos + r + 1, window, sinks)), 0.0625, rows16) for r in range(rows)])
     assert (out[rows:] == 5.0).all()
+
+
+@pytest.mark.parametrize("rows", [10, 70])
+def test_dense8_chunk_with_a_position_without_a_block_and_a_row_that_is_not_finite(rows):
+    """short chunks read the cache as they go, long ones as fp16 rows first: an entry that names no block is 16 latents of zeros in both, and a
+    scale that is NaN makes the outputs of the rows that see it NaN, under a window only of those that see it"""
+    gen, pos = gen_of(rows), 100
+    ckv8, scales = cache(gen, "i8", 14, 16)
+    table = table_for(gen, 1, 11, 14)
+    table[0, 2] = -1
+    q = queries(gen, rows, 64)
+    out = torch.empty(rows, 64, 512, dtype=torch.float16, device="cuda")
+    hk.mla8_dense_prefill(q, ckv8, scales, out, rows, pos, block_table=table)
+    finish()
+    zero = torch.zeros(16, 512, dtype=torch.float64, device="cuda")
+    want = []
+    for r in range(rows):
+        p = visible(pos + r + 1, 0, 0)
+        keys = torch.cat((rows_of(ckv8, scales, table[0], p[:32]), zero, rows_of(ckv8, scales, table[0], p[48:])))
+        want.append(attend(q[r].double(), keys, 0.0625, rows >= 64))
+    close(out, want)
+    scales[table[0, 6]] = math.nan                            # positions 96 .. 111
+    hk.mla8_dense_prefill(q, ckv8, scales, out, rows, pos, block_table=table)
+    finish()
+    assert torch.isnan(out).all()
+    hk.mla8_dense_prefill(q, ckv8, scales, out, rows, pos, block_table=table, window=5, sinks=17)
+    finish()
+    bad = torch.tensor([pos + r + 1 - 5 <= 111 for r in range(rows)], device="cuda")
+    assert torch.isnan(out[bad]).all() and torch.isfinite(out[~bad]).all()
 
 
 def test_dense8_without_a_table_and_another_scale():

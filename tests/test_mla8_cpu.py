@@ -35,7 +35,9 @@ BAD_ROWS = [dict(q=None), dict(out=None), dict(q=A + 2), dict(out=A + 8), dict(n
     ("hk_mla8_append", APPEND, BAD_CACHE + [dict(kv_pre=None), dict(ln_w=None), dict(pos=None), dict(n=-1), dict(kv_pre=A + 4), dict(ln_w=A + 8),
                                             dict(new=A + 2), dict(n_seqs=0), dict(n_seqs=70000), dict(n=5, seq_start=None), dict(table=None)]),
     ("hk_mla8_read", READ, BAD_CACHE + [dict(out=None), dict(out=A + 2), dict(pos=-1), dict(n=-1), dict(pos=2 ** 31 - 1, n=1)]),
-    ("hk_mla8_dense", DENSE, BAD_CACHE + BAD_ROWS + [dict(pos_start=-1), dict(window=-1), dict(sinks=-1), dict(pos_start=2 ** 31 - 1, m=1), dict(table=None)]),
+    ("hk_mla8_dense", DENSE, BAD_CACHE + BAD_ROWS + [dict(pos_start=-1), dict(window=-1), dict(sinks=-1), dict(pos_start=2 ** 31 - 1, m=1), dict(table=None),
+                                                    dict(kv_len=None, row_seq=None, pos_start=250, m=7),
+                                                    dict(kv_len=None, row_seq=None, table=None, n_seqs=1, pos_start=500, m=13)]),
     ("hk_mla8_sparse", SPARSE, BAD_CACHE + BAD_ROWS + [dict(raw_idx=None), dict(kidx=-1), dict(table=None)]),
     ("hk_mla_window", WINDOW, [dict(q=None), dict(ckv=None), dict(out=None), dict(window=0), dict(window=-3), dict(sinks=-1), dict(n_heads=6), dict(m=-1),
                                dict(ckv_rows=-1), dict(pos_start=-1), dict(m=101), dict(q=A + 2), dict(ckv=A + 2), dict(out=A + 2),
