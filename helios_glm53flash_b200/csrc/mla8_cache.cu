@@ -14,14 +14,13 @@
 namespace hk {
 namespace {
 
-// 16 values of a lane as 8 bits: channels 16 lane .. + 15
+// four values as 8 bits each
 template <int FMT>
-__device__ __forceinline__ uint4 round16(const float (&y)[16], float f) {
-  uint4 v;
-  uint8_t* b = reinterpret_cast<uint8_t*>(&v);
-#pragma unroll
-  for (int i = 0; i < 16; i++) b[i] = latent8_round<FMT>(y[i] * f);
-  return v;
+__device__ __forceinline__ uint32_t round4(float a, float b, float c, float d) {
+  if (FMT == CACHE_I8)
+    return (uint32_t)latent8_round<FMT>(a) | (uint32_t)latent8_round<FMT>(b) << 8 | (uint32_t)latent8_round<FMT>(c) << 16 | (uint32_t)latent8_round<FMT>(d) << 24;
+  return (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3) |
+         (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(c, d), __NV_SATFINITE, __NV_E4M3) << 16;
 }
 
 struct AppendArgs {
@@ -35,13 +34,17 @@ struct AppendArgs {
   __half* ckv_new;          // optional [n][512]: the rows as the cache now holds them
 };
 
-// One CTA a block that gets rows.  grid (blocks of a sequence, sequences), THREADS = 32 warps; a warp a row at a time.
-template <int FMT>
-__global__ void __launch_bounds__(1024) mla8_append_kernel(AppendArgs a) {
-  __shared__ float s_amax[32];
+// One CTA of sixteen warps a block that gets rows; grid (blocks of a sequence, sequences).  A warp has rows w, w + 16, ... of the block, a lane the
+// channels 4 lane .. + 3 of each quarter of a row (16-byte loads, 4-byte stores, whole lines both).  Up to four rows a warp stay in registers
+// between the largest magnitude and the rounding (KEEP); a block of 128 tokens is read twice, the second time from L2.
+constexpr int APPEND_WARPS = 16;
+template <int FMT, int ROWS, bool KEEP>
+__global__ void __launch_bounds__(APPEND_WARPS * 32) mla8_append_kernel(AppendArgs a) {
+  __shared__ float s_amax[2][APPEND_WARPS];
   pdl_release();
   pdl_wait();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, seq = blockIdx.y, block = 1 << a.pg.shift;
+  const int p0 = a.pos[seq];
   int r0, r1;
   if (a.seq_start) {
     r0 = min(max(a.seq_start[seq], 0), a.n);
@@ -51,80 +54,123 @@ __global__ void __launch_bounds__(1024) mla8_append_kernel(AppendArgs a) {
     r0 = seq * each;
     r1 = r0 + each;
   }
-  const int p0 = a.pos[seq];
   if (p0 < 0) return;
-  const float top = latent8_top<FMT>();
-  for (int64_t lb = (p0 >> a.pg.shift) + blockIdx.x; (lb << a.pg.shift) < (int64_t)p0 + (r1 - r0); lb += gridDim.x) {
+  constexpr float top = latent8_top<FMT>();
+  const int64_t end = min((int64_t)p0 + (r1 - r0), (int64_t)INT32_MAX);
+  int turn = 0;
+  for (int64_t lb = (p0 >> a.pg.shift) + blockIdx.x; (lb << a.pg.shift) < end; lb += gridDim.x, turn ^= 1) {
     const int64_t start = lb << a.pg.shift;
-    if (start > INT32_MAX) break;
-    const int64_t b = a.pg.block_of(seq, (int)start);
-    if (b < 0) continue;
-    const int first = (int)max((int64_t)0, p0 - start), last = (int)min((int64_t)block, p0 + (int64_t)(r1 - r0) - start);   // new rows of the block
-    uint8_t* rows = a.pg.data + ((size_t)b << a.pg.shift) * LATENT;
-    auto normed = [&](int i, float (&y)[16]) {             // row i of the block, 16 channels a lane
-      const float* x = a.kv_pre + (size_t)(r0 + (start + i - p0)) * LATENT + lane * 16;
-      float ss = 0.f;
+    const int first = (int)max((int64_t)0, p0 - start), last = (int)min((int64_t)block, end - start);   // new rows of the block
+    float y[KEEP ? ROWS : 1][16];
+    float f[ROWS];
+    auto load = [&](int i, float (&x)[16]) {               // row i of the block
+      const float4* src = reinterpret_cast<const float4*>(a.kv_pre + (size_t)(r0 + (start + i - p0)) * LATENT);
 #pragma unroll
-      for (int c = 0; c < 16; c++) {
-        y[c] = x[c];
-        ss = fmaf(y[c], y[c], ss);
+      for (int j = 0; j < 4; j++) {
+        const float4 v = __ldg(src + j * 32 + lane);
+        x[4 * j] = v.x; x[4 * j + 1] = v.y; x[4 * j + 2] = v.z; x[4 * j + 3] = v.w;
       }
-      const float f = rsqrtf(warp_sum(ss) / (float)LATENT + a.eps);
-#pragma unroll
-      for (int c = 0; c < 16; c++) y[c] = y[c] * __half2float(a.ln_w[lane * 16 + c]) * f;
     };
+    if (KEEP) {
+#pragma unroll
+      for (int k = 0; k < ROWS; k++)
+        if (const int i = warp + APPEND_WARPS * k; i >= first && i < last) load(i, y[k]);
+    }
+    const int64_t b = a.pg.block_of(seq, (int)start);
+    uint2 lw[4];
+#pragma unroll
+    for (int j = 0; j < 4; j++) lw[j] = __ldg(reinterpret_cast<const uint2*>(a.ln_w) + j * 32 + lane);
+    auto weigh = [&](float (&x)[16]) {
+#pragma unroll
+      for (int j = 0; j < 4; j++) {
+        const float2 w0 = __half22float2(*reinterpret_cast<const __half2*>(&lw[j].x)), w1 = __half22float2(*reinterpret_cast<const __half2*>(&lw[j].y));
+        x[4 * j] *= w0.x; x[4 * j + 1] *= w0.y; x[4 * j + 2] *= w1.x; x[4 * j + 3] *= w1.y;
+      }
+    };
+    const float s0 = b >= 0 && first > 0 ? a.pg.scales[b] : 0.f;
     float amax = 0.f;
     bool bad = false;
-    for (int i = first + warp; i < last; i += 32) {
-      float y[16];
-      normed(i, y);
 #pragma unroll
-      for (int c = 0; c < 16; c++) {
-        amax = fmaxf(amax, fabsf(y[c]));
-        bad |= !(fabsf(y[c]) < INFINITY);
+    for (int k = 0; k < ROWS; k++) {
+      const int i = warp + APPEND_WARPS * k;
+      float(&x)[16] = y[KEEP ? k : 0];
+      if (i >= first && i < last) {
+        if (!KEEP) load(i, x);
+        float ss = 0.f;
+#pragma unroll
+        for (int c = 0; c < 16; c++) ss = fmaf(x[c], x[c], ss);
+        f[k] = rsqrtf(warp_sum(ss) / (float)LATENT + a.eps);
+        weigh(x);
+        float top_x = 0.f;
+#pragma unroll
+        for (int c = 0; c < 16; c++) {
+          bad |= !(fabsf(x[c] * f[k]) < INFINITY);
+          top_x = fmaxf(top_x, fabsf(x[c]));
+        }
+        amax = fmaxf(amax, top_x * f[k]);
       }
     }
-    if (bad) amax = INFINITY;
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
-    __syncthreads();
-    if (lane == 0) s_amax[warp] = amax;
-    __syncthreads();
-    amax = s_amax[lane];
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+    amax = bad ? INFINITY : amax;
+    amax = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(amax)));   // (not negative: ordered as integers)
+    if (lane == 0) s_amax[turn][warp] = amax;
+    __syncthreads();                                       // every warp has s0 and this turn's maximum
+    amax = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(s_amax[turn][lane % APPEND_WARPS])));
+    if (b < 0) continue;
     const float need = amax > 1e-25f ? (amax < INFINITY ? __fdiv_rn(amax, top) : NAN) : 0.f;
-    const float s0 = first > 0 ? a.pg.scales[b] : 0.f;
-    __syncthreads();                                       // everyone has s0
     const bool grow = need > s0 || need != need;
-    const float s = s0 != s0 ? s0 : grow ? need : s0;
+    const float s = s0 != s0 ? s0 : grow ? need : s0, inv = s > 0.f ? __fdiv_rn(1.f, s) : 0.f;
     if (threadIdx.x == 0) a.pg.scales[b] = s;
-    const float inv = s > 0.f ? __fdiv_rn(1.f, s) : 0.f;
+    uint8_t* rows = a.pg.data + ((size_t)b << a.pg.shift) * LATENT;
     if (grow && s == s) {
       const float ratio = __fdiv_rn(s0, s);
-      for (int i = warp; i < first; i += 32) {
+      for (int i = warp; i < first; i += APPEND_WARPS) {
         uint4* q = reinterpret_cast<uint4*>(rows + (size_t)i * LATENT + lane * 16);
-        const uint4 v = *q;
-        const uint8_t* v8 = reinterpret_cast<const uint8_t*>(&v);
-        float y[16];
+        uint4 v = *q;
+        uint32_t* v4 = &v.x;
 #pragma unroll
-        for (int c = 0; c < 16; c++) y[c] = latent8_value<FMT>(v8[c]);
-        *q = round16<FMT>(y, ratio);
+        for (int c = 0; c < 4; c++) {
+          float o[4];
+#pragma unroll
+          for (int e = 0; e < 4; e++) o[e] = latent8_value<FMT>((uint8_t)(v4[c] >> (8 * e))) * ratio;
+          v4[c] = round4<FMT>(o[0], o[1], o[2], o[3]);
+        }
+        *q = v;
       }
     }
-    for (int i = first + warp; i < last; i += 32) {
-      float y[16];
-      normed(i, y);
-      const uint4 v = round16<FMT>(y, inv);
-      *reinterpret_cast<uint4*>(rows + (size_t)i * LATENT + lane * 16) = v;
-      if (a.ckv_new) {
-        const uint8_t* v8 = reinterpret_cast<const uint8_t*>(&v);
-        __half* dst = a.ckv_new + (size_t)(r0 + (start + i - p0)) * LATENT + lane * 16;
 #pragma unroll
-        for (int c = 0; c < 16; c++) dst[c] = __float2half_rn(latent8_value<FMT>(v8[c]) * s);
+    for (int k = 0; k < ROWS; k++) {
+      const int i = warp + APPEND_WARPS * k;
+      float(&x)[16] = y[KEEP ? k : 0];
+      if (i >= first && i < last) {
+        if (!KEEP) {
+          load(i, x);
+          weigh(x);
+        }
+        const float g = s == s ? f[k] * inv : 0.f;
+        __half* dst = a.ckv_new ? a.ckv_new + (size_t)(r0 + (start + i - p0)) * LATENT : nullptr;
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+          const uint32_t q = s == s ? round4<FMT>(x[4 * j] * g, x[4 * j + 1] * g, x[4 * j + 2] * g, x[4 * j + 3] * g) : 0u;
+          *reinterpret_cast<uint32_t*>(rows + (size_t)i * LATENT + j * 128 + lane * 4) = q;
+          if (dst) {
+            float o[4];
+#pragma unroll
+            for (int e = 0; e < 4; e++) o[e] = latent8_value<FMT>((uint8_t)(q >> (8 * e))) * s;
+            const __half2 h0 = __floats2half2_rn(o[0], o[1]), h1 = __floats2half2_rn(o[2], o[3]);
+            *reinterpret_cast<uint2*>(dst + j * 128 + lane * 4) = make_uint2(*reinterpret_cast<const uint32_t*>(&h0), *reinterpret_cast<const uint32_t*>(&h1));
+          }
+        }
       }
     }
   }
+}
+
+template <int FMT>
+cudaError_t append_launch(const AppendArgs& a, dim3 grid, cudaStream_t s) {
+  const auto kernel = a.pg.shift == 4 ? mla8_append_kernel<FMT, 1, true>
+                      : a.pg.shift == 5 ? mla8_append_kernel<FMT, 2, true>
+                      : a.pg.shift == 6 ? mla8_append_kernel<FMT, 4, true> : mla8_append_kernel<FMT, 8, false>;
+  return pdl_launch(kernel, grid, dim3(APPEND_WARPS * 32), 0, s, a);
 }
 
 // rows i of out: position i of the sequence below `head`, i + shift from there on; f16(scale * value), zeros where there is no block.
@@ -213,9 +259,16 @@ HK_API int hk_mla8_append(const float* kv_pre, const void* ln_w_f16, void* ckv8,
   a.n = n;
   a.eps = epsilon;
   a.ckv_new = (__half*)ckv_new;
-  const dim3 grid((unsigned)((n / n_seqs + block - 1) / block + 1), (unsigned)n_seqs);
-  return pdl_launch(dtype == HK_I8 ? mla8_append_kernel<CACHE_I8> : mla8_append_kernel<CACHE_E4M3>, grid, dim3(1024), 0, as_stream(stream), a) ==
-                 cudaSuccess
+  // Blocks that a sequence's rows touch: as many CTAs where every sequence has n / n_seqs rows, else enough for the average, and for one
+  // sequence with all of them as long as the grid stays within eight CTAs an SM (a CTA walks blocks gridDim.x apart).
+  auto touched = [&](int rows) { return (int)(((int64_t)rows + block - 2) / block + 1); };
+  int blocks = touched((n + n_seqs - 1) / n_seqs);
+  if (seq_start) {
+    const int room = 8 * sm_count() / n_seqs, all = touched(n);
+    blocks = blocks > (all < room ? all : room) ? blocks : (all < room ? all : room);
+  }
+  const dim3 grid((unsigned)blocks, (unsigned)n_seqs);
+  return (dtype == HK_I8 ? append_launch<CACHE_I8>(a, grid, as_stream(stream)) : append_launch<CACHE_E4M3>(a, grid, as_stream(stream))) == cudaSuccess
              ? HK_OK
              : HK_ERR_CUDA;
 }
