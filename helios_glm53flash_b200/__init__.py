@@ -89,7 +89,7 @@ SIGNATURES = {
     "hk_mla_window": (_i, [_vp, _vp, _i64, _vp, _vp, _i, _i, _i, _vp, _i, _i, _f, _i, _vp, _sz, _vp]),
     "hk_mla8_append": (_i, [_vp, _vp, _vp, _vp, _i, _i64, _i, _vp, _i, _i, _vp, _vp, _i, _f, _vp, _vp]),
     "hk_mla8_read": (_i, [_vp, _vp, _i, _i64, _i, _vp, _i, _i, _i, _vp, _vp]),
-    "hk_mla8_auto_splits": (_i, [_i, _i, _i]),
+    "hk_mla8_sparse_workspace_bytes": (_sz, [_i, _i, _i]),
     "hk_mla8_dense_workspace_bytes": (_sz, [_i, _i, _i, _i, _i, _i, _i]),
     "hk_mla8_dense": (_i, [_vp, _vp, _vp, _i, _i64, _i, _vp, _i, _i, _vp, _vp, _i, _i, _i, _vp, _i, _i, _f, _i, _i, _vp, _sz, _vp]),
     "hk_mla8_sparse": (_i, [_vp, _vp, _vp, _i, _i64, _i, _vp, _i, _i, _vp, _vp, _i, _vp, _i, _i, _f, _i, _vp, _sz, _vp]),
@@ -459,83 +459,60 @@ def mla_window_prefill(q_lat, ckv, lat_out, qlen, pos_start, window, sinks=0, st
 
 # ---- the latent cache in 8 bits, paged: ckv8 [n_blocks, block, 512] of torch.int8 or torch.float8_e4m3fn, scales [n_blocks] float32,
 # block_table [n_seqs, blocks of a sequence] int32 (None: one sequence whose i-th block is block i) ----
-_cache8_types = {}
-
-
-def _cache8(ckv8, scales, block_table):
-    """(dtype tag, n_blocks, block, table, its stride) of a cache's tensors; what the library cannot check by address is checked here"""
-    if not _cache8_types:
-        import torch
-        _cache8_types.update({torch.int8: HK_I8, torch.float8_e4m3fn: HK_E4M3, "scales": torch.float32, "table": torch.int32})
-    tag = _cache8_types.get(ckv8.dtype)
-    if tag is None or ckv8.dim() != 3 or ckv8.shape[2] != 512 or not ckv8.is_contiguous():
-        raise ValueError("ckv8: a contiguous [n_blocks, block, 512] tensor of int8 or float8_e4m3fn")
-    if scales.dtype != _cache8_types["scales"] or scales.numel() != ckv8.shape[0] or not scales.is_contiguous():
-        raise ValueError("scales: a contiguous float32 tensor, one a block")
-    if block_table is None:
-        return tag, ckv8.shape[0], ckv8.shape[1], None, 0
-    if block_table.dtype != _cache8_types["table"] or not 1 <= block_table.dim() <= 2 or not block_table.is_contiguous() or not block_table.numel():
-        raise ValueError("block_table: a contiguous [n_seqs, blocks of a sequence] tensor of int32")
-    return tag, ckv8.shape[0], ckv8.shape[1], block_table, block_table.shape[-1]
-
-
-def _n_seqs(table):
-    return 1 if table is None or table.dim() == 1 else table.shape[0]
-
-
 def mla8_cache_append(kv_pre, ln_w, ckv8, scales, pos, n, eps, block_table=None, n_seqs=1, seq_start=None, ckv_new=None, stream=None):
     """RMS norm of n new latent rows into the 8-bit cache (hk_mla8_append).  pos: device int32 [n_seqs], position of each sequence's
     first new row; seq_start: device int32 [n_seqs + 1], its rows of kv_pre (None: n / n_seqs each); ckv_new: fp16 [n, 512], the rows as the
     cache holds them."""
-    tag, n_blocks, block, table, stride = _cache8(ckv8, scales, block_table)
-    if n_seqs > _n_seqs(table):
+    tag, n_blocks, block, stride, seqs = _native.cache8(ckv8, scales, block_table)
+    if n_seqs > seqs:
         raise ValueError("block_table: fewer sequences than n_seqs")
-    _run("hk_mla8_append", kv_pre, ln_w, ckv8, scales, tag, n_blocks, block, table, stride, n_seqs, seq_start, pos, n, eps, ckv_new, stream)
+    _run("hk_mla8_append", kv_pre, ln_w, ckv8, scales, tag, n_blocks, block, block_table, stride, n_seqs, seq_start, pos, n, eps, ckv_new, stream)
 
 
 def mla8_cache_read(ckv8, scales, out, pos, n, block_table=None, stream=None):
     """positions pos .. pos + n - 1 of one sequence as fp16 rows (hk_mla8_read); block_table: the sequence's row of the table"""
-    tag, n_blocks, block, table, stride = _cache8(ckv8, scales, block_table)
-    if _n_seqs(table) != 1:
+    tag, n_blocks, block, stride, seqs = _native.cache8(ckv8, scales, block_table)
+    if seqs != 1:
         raise ValueError("block_table: one sequence's row of the table")
-    _run("hk_mla8_read", ckv8, scales, tag, n_blocks, block, table, stride, pos, n, out, stream)
-
-
-def mla8_auto_splits(m, n_heads, n_keys):
-    return load_library().hk_mla8_auto_splits(m, n_heads, n_keys)
+    _run("hk_mla8_read", ckv8, scales, tag, n_blocks, block, block_table, stride, pos, n, out, stream)
 
 
 def mla8_dense_workspace_bytes(m, n_heads, pos_start, n_keys_hint=0, window=0, sinks=0, per_row=False):
     return load_library().hk_mla8_dense_workspace_bytes(m, n_heads, pos_start, n_keys_hint or 0, window, sinks, int(per_row))
 
 
+def mla8_sparse_workspace_bytes(m, n_heads, kidx):
+    return load_library().hk_mla8_sparse_workspace_bytes(m, n_heads, kidx)
+
+
 def mla8_dense_prefill(q_lat, ckv8, scales, lat_out, qlen, pos_start, stream=None, scale=0.0625, n_heads=64, block_table=None, row_seq=None,
                        kv_len=None, window=0, sinks=0, n_split=0, workspace=None, n_keys_hint=None):
     """mla_dense_prefill over the 8-bit cache (hk_mla8_dense): a chunk of one sequence (kv_len and row_seq None), or rows of sequences
-    row_seq[r] (device int32, None: sequence 0) with kv_len[r] keys each (device int32).  window > 0: the last `window` keys of a row and
-    the first `sinks` only."""
-    tag, n_blocks, block, table, stride = _cache8(ckv8, scales, block_table)
-    per_row = 1 if kv_len is not None or row_seq is not None else 0
+    row_seq[r] (device int32, None: sequence 0) with kv_len[r] keys each (device int32), the longest about n_keys_hint.  window > 0: the
+    last `window` keys of a row and the first `sinks` only."""
+    tag, n_blocks, block, stride, seqs = _native.cache8(ckv8, scales, block_table)
     ws, hint = workspace, n_keys_hint or 0
     if ws is None:
-        need = (_native.hk_mla8_dense_workspace_bytes(qlen, n_heads, pos_start, hint, window, sinks, per_row) if n_split <= 0
-                else mla_partial_bytes(n_split, qlen * n_heads) if n_split > 1 else 0)
+        need = (_native.hk_mla8_dense_workspace_bytes(qlen, n_heads, pos_start, hint, window, sinks, 1 if kv_len is not None or row_seq is not None else 0)
+                if n_split <= 0 else _native.hk_mla_partial_bytes(n_split, qlen * n_heads) if n_split > 1 else 0)
         if need:
             ws = _scratch(need, q_lat.device, stream)
-    _run("hk_mla8_dense", q_lat, ckv8, scales, tag, n_blocks, block, table, stride, _n_seqs(table), row_seq, kv_len,
-         pos_start, window, sinks, lat_out, qlen, n_heads, scale, n_split, hint, ws, ws, stream)
+    _run("hk_mla8_dense", q_lat, ckv8, scales, tag, n_blocks, block, block_table, stride, seqs, row_seq, kv_len, pos_start, window, sinks, lat_out,
+         qlen, n_heads, scale, n_split, hint, ws, ws, stream)
 
 
 def mla8_sparse_decode(q_lat, ckv8, scales, raw_idx, kidx, lat_out, m, stream=None, scale=0.0625, n_heads=64, block_table=None, row_seq=None,
                        n_split=0, workspace=None):
     """mla_sparse_decode over the 8-bit cache (hk_mla8_sparse): raw_idx holds positions of the row's sequence"""
-    tag, n_blocks, block, table, stride = _cache8(ckv8, scales, block_table)
-    splits = n_split if n_split > 0 else _native.hk_mla8_auto_splits(m, n_heads, kidx)
+    tag, n_blocks, block, stride, seqs = _native.cache8(ckv8, scales, block_table)
     ws = workspace
-    if splits > 1 and ws is None:
-        ws = _scratch(mla_partial_bytes(splits, m * n_heads), q_lat.device, stream)
-    _run("hk_mla8_sparse", q_lat, ckv8, scales, tag, n_blocks, block, table, stride, _n_seqs(table), row_seq, raw_idx, kidx,
-         lat_out, m, n_heads, scale, splits, ws, ws, stream)
+    if ws is None:
+        need = (_native.hk_mla8_sparse_workspace_bytes(m, n_heads, kidx) if n_split <= 0
+                else _native.hk_mla_partial_bytes(n_split, m * n_heads) if n_split > 1 else 0)
+        if need:
+            ws = _scratch(need, q_lat.device, stream)
+    _run("hk_mla8_sparse", q_lat, ckv8, scales, tag, n_blocks, block, block_table, stride, seqs, row_seq, raw_idx, kidx, lat_out, m, n_heads, scale,
+         n_split, ws, ws, stream)
 
 
 def mla_dense_partial(q_lat, ckv, kv_base, kv_len, pos_start, part_m, part_l, part_acc, m,

@@ -173,8 +173,8 @@ struct Entry<R (*)(A...)> {
   X(hk_lse_combine, true) X(hk_q_latent, true) X(hk_o_absorb, true) X(hk_wuv_transpose, true) X(hk_o_absorb_t, true)         \
   X(hk_q_latent_beside, true) X(hk_o_absorb_beside, true) X(hk_kda_decode_layer_beside, true)                                \
   X(hk_mla_cache_append, true) X(hk_layernorm_f16, true) X(hk_mla_decode_prologue, true) X(hk_mla_window, true)              \
-  X(hk_mla8_append, true) X(hk_mla8_read, true) X(hk_mla8_dense, true) X(hk_mla8_sparse, true) X(hk_mla8_auto_splits, false)  \
-  X(hk_mla8_dense_workspace_bytes, false)
+  X(hk_mla8_append, true) X(hk_mla8_read, true) X(hk_mla8_dense, true) X(hk_mla8_sparse, true)                                \
+  X(hk_mla8_dense_workspace_bytes, false) X(hk_mla8_sparse_workspace_bytes, false)
 
 #define X(name, stream)                                                                      \
   decltype(&::name) p_##name = nullptr;                                                      \
@@ -203,8 +203,41 @@ PyObject* py_bind(PyObject*, PyObject* d) {
   Py_RETURN_NONE;
 }
 
+// cache8(ckv8, scales, block_table or None) -> (dtype tag, n_blocks, block, table stride, n_seqs): the arguments that an 8-bit latent cache's
+// tensors stand for.  What the library cannot see from addresses is checked here.
+PyObject* py_cache8(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  auto refuse = [](const char* what) -> PyObject* {
+    PyErr_SetString(PyExc_ValueError, what);
+    return nullptr;
+  };
+  if (n != 3 || !THPVariable_Check(args[0]) || !THPVariable_Check(args[1]) || !(args[2] == Py_None || THPVariable_Check(args[2]))) {
+    bad_arg("cache8: the cache's tensors");
+    return nullptr;
+  }
+  try {
+    const at::Tensor &c = THPVariable_Unpack(args[0]), &s = THPVariable_Unpack(args[1]);
+    const bool i8 = c.scalar_type() == at::kChar;
+    if ((!i8 && c.scalar_type() != at::kFloat8_e4m3fn) || c.dim() != 3 || c.size(2) != 512 || !c.is_contiguous())
+      return refuse("ckv8: a contiguous [n_blocks, block, 512] tensor of int8 or float8_e4m3fn");
+    if (s.scalar_type() != at::kFloat || s.numel() != c.size(0) || !s.is_contiguous()) return refuse("scales: a contiguous float32 tensor, one a block");
+    long long stride = 0, seqs = 1;
+    if (args[2] != Py_None) {
+      const at::Tensor& t = THPVariable_Unpack(args[2]);
+      if (t.scalar_type() != at::kInt || t.dim() < 1 || t.dim() > 2 || !t.is_contiguous() || t.numel() == 0)
+        return refuse("block_table: a contiguous [n_seqs, blocks of a sequence] tensor of int32");
+      stride = t.size(-1);
+      seqs = t.numel() / stride;
+    }
+    return Py_BuildValue("(iLLLL)", i8 ? HK_I8 : HK_E4M3, (long long)c.size(0), (long long)c.size(1), stride, seqs);
+  } catch (const std::exception& e) {
+    PyErr_SetString(PyExc_RuntimeError, e.what());
+    return nullptr;
+  }
+}
+
 #define X(name, stream) {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(py_##name)), METH_FASTCALL, nullptr},
-PyMethodDef methods[] = {HK_ENTRIES(X){"bind", py_bind, METH_O, nullptr}, {nullptr, nullptr, 0, nullptr}};
+PyMethodDef methods[] = {HK_ENTRIES(X){"cache8", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(py_cache8)), METH_FASTCALL, nullptr},
+                         {"bind", py_bind, METH_O, nullptr}, {nullptr, nullptr, 0, nullptr}};
 #undef X
 
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_binding", "native call path of the hk_* entry points", -1, methods,

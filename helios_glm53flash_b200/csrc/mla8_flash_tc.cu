@@ -14,6 +14,7 @@
 #include <cuda.h>   // CUtensorMap
 
 #include "latent8.cuh"
+#include "lse_reduce.cuh"
 #include "mla_args.cuh"
 #include "tc05.cuh"
 
@@ -32,6 +33,7 @@ constexpr uint32_t F8_SMEM = F8S_MISC + 2048 + 1024;             // + slack to a
 constexpr uint32_t F8_O = 0, F8_S = 256, F8_Q = 320;             // tensor-memory columns: O 2 x 128, S 2 x 32, Q 192
 constexpr int F8_POLL_NS = 40;
 constexpr int F8_CONV_WARPS = 8, F8_ROWS = F8_KEYS / F8_CONV_WARPS, F8_THREADS = (6 + F8_CONV_WARPS) * 32;
+constexpr int F8_SHARE_ROWS = 160, F8_MIN_TILES = 2;   // rows whose splits are shared out on the device; tiles that a split is worth
 constexpr float F8_LOG2E = 1.4426950408889634f;
 constexpr float F8_MOVE = 8.0f, F8_MOVE_SCALE = 16.0f;
 
@@ -46,31 +48,112 @@ struct F8Misc {
 };
 static_assert(sizeof(F8Misc) <= 2048, "misc area");
 
-// the tiles of a work item
-struct F8Item {
-  int r, hg, sp, seq;
+// the tiles that a row attends to
+struct F8Row {
+  int seq;
   KeyList keys;
-  int head_tiles, jump;                           // tile i of the row's list is tile i, or i + jump behind the sinks' tiles
-  int t0, n_tiles;
-  __device__ __forceinline__ int tile(int i) const { return t0 + i < head_tiles ? t0 + i : t0 + i + jump; }
+  int head_tiles, jump, tiles;                    // tile i of the row's list is tile i, or i + jump behind the sinks' tiles
 };
+template <bool GATHER>
+__device__ __forceinline__ F8Row f8_row(const MlaArgs& a, const MlaPaged& pg, int r) {
+  F8Row w;
+  w.seq = pg.seq_of(r);
+  w.keys = key_list(w.seq < 0 ? 0 : GATHER ? a.kidx : a.kv_len ? a.kv_len[r] : a.pos_start + r + 1, a.window, a.sinks);
+  w.head_tiles = (w.keys.head + F8_KEYS - 1) / F8_KEYS;
+  w.jump = max(w.keys.lo / F8_KEYS - w.head_tiles, 0);
+  w.tiles = w.keys.n / F8_KEYS + (w.keys.n % F8_KEYS != 0) - w.jump;
+  return w;
+}
+struct F8Item {
+  int r, hg, sp, n_sp, first;                     // row, 64 heads, split of how many, unit of split 0 (shared out splits); r < 0: nothing to do
+  F8Row row;
+  int t0, n_tiles;
+  __device__ __forceinline__ int tile(int i) const { return t0 + i < row.head_tiles ? t0 + i : t0 + i + row.jump; }
+};
+
+// Splits shared out on the device, where alone the lengths are known: `units` CTAs (of 64 heads) for m <= units rows.  Every split has at most
+// `per` tiles, the smallest number found with which all rows' splits fit; a row has one at least.  Executed by a whole warp.
+__device__ __forceinline__ void f8_share(const MlaArgs& a, const MlaPaged& pg, int unit, int units, F8Item& it, int& per) {
+  const int lane = threadIdx.x & 31, each = (a.m + 31) / 32;
+  int t[F8_SHARE_ROWS / 32], sum = 0;
+#pragma unroll
+  for (int k = 0; k < F8_SHARE_ROWS / 32; k++) {
+    const int r = lane * each + k;
+    t[k] = -1;
+    if (k < each && r < a.m) sum += t[k] = f8_row<false>(a, pg, r).tiles;
+  }
+  sum = __reduce_add_sync(0xffffffffu, sum);
+  float inv;
+  auto splits = [&](int tiles) {                           // ceil(tiles / per): the quotient in fp32 may be one too small
+    int n = (int)((float)tiles * inv);
+    n += n * per < tiles;
+    n += n * per < tiles;
+    return max(n, 1);
+  };
+  per = max((sum + units - 1) / units, F8_MIN_TILES);
+  int mine;
+  for (int tries = 0;; tries++) {
+    mine = 0;
+    inv = 1.f / (float)per;
+#pragma unroll
+    for (int k = 0; k < F8_SHARE_ROWS / 32; k++)
+      if (k < each && t[k] >= 0) mine += splits(t[k]);
+    if ((int)__reduce_add_sync(0xffffffffu, mine) <= units) break;
+    per += tries < 4 ? 1 : per / 4;                        // (rows of very different lengths; ends where every row has one split)
+  }
+  int before = mine;                                       // splits of the lanes up to this one
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int x = __shfl_up_sync(0xffffffffu, before, o);
+    if (lane >= o) before += x;
+  }
+  before -= mine;
+  int row = -1, first = 0, n_sp = 0;
+#pragma unroll
+  for (int k = 0; k < F8_SHARE_ROWS / 32; k++) {
+    if (k >= each || t[k] < 0) break;
+    const int n = splits(t[k]);
+    if (unit >= before && unit < before + n) {
+      row = lane * each + k;
+      first = before;
+      n_sp = n;
+    }
+    before += n;
+  }
+  const uint32_t who = __ballot_sync(0xffffffffu, row >= 0);
+  const int from = max(__ffs(who) - 1, 0);
+  it.r = __shfl_sync(0xffffffffu, row, from);
+  it.first = __shfl_sync(0xffffffffu, first, from);
+  it.n_sp = __shfl_sync(0xffffffffu, n_sp, from);
+  it.sp = unit - it.first;
+}
+
 template <bool GATHER>
 __device__ __forceinline__ F8Item f8_item(const MlaArgs& a, const MlaPaged& pg, int idx) {
   F8Item it;
   const int groups = (a.n_heads + F8_HEADS - 1) / F8_HEADS;
-  it.sp = idx % a.n_split;
-  idx /= a.n_split;
-  it.hg = idx % groups;
-  it.r = idx / groups;
-  if (!GATHER && !a.kv_len) it.r = a.m - 1 - it.r;         // rows of a causal chunk grow: the longest first
-  it.seq = pg.seq_of(it.r);
-  const int n = it.seq < 0 ? 0 : GATHER ? a.kidx : a.kv_len ? a.kv_len[it.r] : a.pos_start + it.r + 1;
-  it.keys = key_list(n, a.window, a.sinks);
-  it.head_tiles = (it.keys.head + F8_KEYS - 1) / F8_KEYS;
-  it.jump = max(it.keys.lo / F8_KEYS - it.head_tiles, 0);
-  const int tiles = it.keys.n / F8_KEYS + (it.keys.n % F8_KEYS != 0) - it.jump, per = (tiles + a.n_split - 1) / a.n_split;
-  it.t0 = min(tiles, it.sp * per);
-  it.n_tiles = min(tiles, it.t0 + per) - it.t0;
+  int per;
+  if (!GATHER && a.n_split == 0) {
+    it.hg = idx % groups;
+    f8_share(a, pg, idx / groups, gridDim.x / groups, it, per);
+    if (it.r < 0) {
+      it.n_tiles = it.t0 = 0;
+      return it;
+    }
+    it.row = f8_row<GATHER>(a, pg, it.r);
+  } else {
+    it.n_sp = a.n_split;
+    it.first = 0;
+    it.sp = idx % a.n_split;
+    idx /= a.n_split;
+    it.hg = idx % groups;
+    it.r = idx / groups;
+    if (!GATHER && !a.kv_len) it.r = a.m - 1 - it.r;       // rows of a causal chunk grow: the longest first
+    it.row = f8_row<GATHER>(a, pg, it.r);
+    per = (it.row.tiles + a.n_split - 1) / a.n_split;
+  }
+  it.t0 = min(it.row.tiles, it.sp * per);
+  it.n_tiles = min(it.row.tiles, it.t0 + per) - it.t0;
   return it;
 }
 
@@ -156,6 +239,10 @@ __global__ __launch_bounds__(F8_THREADS, 1) void mla8_flash_tc_kernel(MlaArgs a,
   const uint32_t tmem = ms.tmem;
   // An item of at most two tiles (a decode split) does not need the last tile slot back: S reads Q from there, and moving it is saved.
   const bool direct_q = it.n_tiles < F8_NBUF;
+  // Final rows, or a partial: with a number of splits [split][row, head], shared out [CTA][64 heads].
+  const bool final_out = it.n_sp == 1;
+  const size_t part_row = a.n_split == 0 ? (size_t)blockIdx.x * F8_HEADS : ((size_t)it.sp * a.m + it.r) * a.n_heads + it.hg * F8_HEADS;
+  if (a.n_split == 0 && it.r >= 0 && it.sp == 0 && it.hg == 0 && tid == 0) a.shares[it.r] = make_int2(it.first, it.n_sp);
   const int n_tiles = it.n_tiles, h0 = it.hg * F8_HEADS, n_h = min(F8_HEADS, a.n_heads - h0);
   bool ok = true;
 
@@ -167,13 +254,13 @@ __global__ __launch_bounds__(F8_THREADS, 1) void mla8_flash_tc_kernel(MlaArgs a,
       if (lane >= F8_ROWS || t >= n_tiles) return -1;
       const int p = it.tile(t) * F8_KEYS + k8 + lane;
       if (GATHER) return p < a.kidx ? f8_ld_int(a.raw_idx + (size_t)it.r * a.kidx + p) : -1;
-      return p < it.keys.n && (p >= it.keys.lo || p < it.keys.head) ? p : -1;
+      return p < it.row.keys.n && (p >= it.row.keys.lo || p < it.row.keys.head) ? p : -1;
     };
     // its entry of the table (a block of the cache, or what is there in the place of one)
     auto entry = [&](int p) -> int {
       const int b = p >> pg.shift;
       if (p < 0 || (pg.table && b >= pg.table_stride)) return -1;
-      return pg.table ? f8_ld_int(pg.table + (size_t)it.seq * pg.table_stride + b) : b;
+      return pg.table ? f8_ld_int(pg.table + (size_t)it.row.seq * pg.table_stride + b) : b;
     };
     const int in_block = (1 << pg.shift) - 1;
     uint4 v[F8_ROWS];
@@ -418,9 +505,9 @@ __global__ __launch_bounds__(F8_THREADS, 1) void mla8_flash_tc_kernel(MlaArgs a,
     l += ms.mx[n_tiles & 1][tid ^ 64];
     const bool none = l == 0.f;                            // (NaN: a score was none)
     if (half == 0) {
-      ms.mx[(n_tiles + 1) & 1][head] = none ? 0.f : a.out ? sref / l : sref;
-      if (!a.out && head < n_h) {
-        const size_t at = (size_t)it.sp * a.m * a.n_heads + (size_t)it.r * a.n_heads + h0 + head;
+      ms.mx[(n_tiles + 1) & 1][head] = none ? 0.f : final_out ? sref / l : sref;
+      if (!final_out && it.r >= 0 && head < n_h) {
+        const size_t at = part_row + head;
         a.part_m[at] = m == -INFINITY || none ? -INFINITY : m / F8_LOG2E;
         a.part_l[at] = l;
       }
@@ -429,11 +516,11 @@ __global__ __launch_bounds__(F8_THREADS, 1) void mla8_flash_tc_kernel(MlaArgs a,
   }
   // ---- epilogue: O leaves through the idle tiles.  The softmax and converter warps of a lane quarter take 2, 3 and 3 of its 8 pieces of 32
   // channels; then all twelve store whole rows (a bulk copy a head moved 27 bytes a cycle: 2.5 us for 128 KB, 0.4 us more). ----
-  if (warp < 4 || warp >= 6) {
+  if (it.r >= 0 && (warp < 4 || warp >= 6)) {
     asm volatile("bar.sync 4, 384;" ::: "memory");         // factors, and every product is complete
     tc::fence_after_sync();
     const int quarter = warp & 3, head = (quarter & 1) * 32 + lane, half = quarter >> 1, member = warp < 4 ? 0 : warp < 10 ? 1 : 2;
-    const uint32_t elem = a.out ? 2 : 4, pitch = LATENT * elem + 16;
+    const uint32_t elem = final_out ? 2 : 4, pitch = LATENT * elem + 16;
     const float f = ms.mx[(n_tiles + 1) & 1][head];
     uint8_t* orow = smem + F8S_K + head * pitch;
     for (int c = 32 * (3 * member - (member > 0)); c < 32 * (3 * member + 2); c += 32) {
@@ -445,7 +532,7 @@ __global__ __launch_bounds__(F8_THREADS, 1) void mla8_flash_tc_kernel(MlaArgs a,
 #pragma unroll
       for (int j = 0; j < 32; j++) o[j] = f == 0.f ? 0u : __float_as_uint(__uint_as_float(o[j]) * f);
       uint8_t* dst = orow + ((c >> 7) * 256 + half * 128 + (c & 127)) * elem;
-      if (a.out) {
+      if (final_out) {
 #pragma unroll
         for (int v = 0; v < 4; v++) {
           uint4 w;
@@ -464,14 +551,13 @@ __global__ __launch_bounds__(F8_THREADS, 1) void mla8_flash_tc_kernel(MlaArgs a,
     }
     asm volatile("bar.sync 4, 384;" ::: "memory");
     if (!*abort_flag) {
-      const size_t first = (size_t)it.r * a.n_heads + h0;
-      uint8_t* dst = a.out ? reinterpret_cast<uint8_t*>(a.out + first * LATENT)
-                           : reinterpret_cast<uint8_t*>(a.part_acc + ((size_t)it.sp * a.m * a.n_heads + first) * LATENT);
+      uint8_t* dst = final_out ? reinterpret_cast<uint8_t*>(a.out + ((size_t)it.r * a.n_heads + h0) * LATENT)
+                               : reinterpret_cast<uint8_t*>(a.part_acc + part_row * LATENT);
       const int team = warp < 4 ? warp : warp - 2;
-      const int per = a.out ? 2 : 4;                       // 512-byte pieces of a head
+      const int per = final_out ? 2 : 4;                       // 512-byte pieces of a head
 #pragma unroll 8
       for (int i = team; i < n_h * per; i += 12) {
-        const int h = a.out ? i >> 1 : i >> 2, c = (a.out ? i & 1 : i & 3) * 512 + lane * 16;
+        const int h = final_out ? i >> 1 : i >> 2, c = (final_out ? i & 1 : i & 3) * 512 + lane * 16;
         *reinterpret_cast<uint4*>(dst + (size_t)h * LATENT * elem + c) = *reinterpret_cast<const uint4*>(smem + F8S_K + h * pitch + c);
       }
     }
@@ -491,10 +577,31 @@ int f8_launch(const MlaArgs& a, const MlaPaged& pg, const CUtensorMap& q, cudaSt
       return HK_ERR_CUDA;
     attr_set[dev] = true;
   }
-  const int64_t items = (int64_t)a.n_split * a.m * ((a.n_heads + F8_HEADS - 1) / F8_HEADS);
+  const int groups = (a.n_heads + F8_HEADS - 1) / F8_HEADS;
+  const int64_t items = (a.n_split == 0 ? (int64_t)a.units : (int64_t)a.n_split * a.m) * groups;
   if (items > INT32_MAX) return HK_ERR_UNSUPPORTED;
   const cudaError_t e = pdl_launch(mla8_flash_tc_kernel<GATHER, FMT>, dim3((unsigned)items), dim3(F8_THREADS), F8_SMEM, s, a, pg, device_status_ptr(), q);
   return e == cudaSuccess && cudaPeekAtLastError() == cudaSuccess ? HK_OK : HK_ERR_CUDA;
+}
+
+// Merge of the splits that the attention kernel shared out: one CTA a (row, head).  Rows of one split are finished.
+template <int GROUPS>
+__global__ __launch_bounds__(128 * GROUPS) void mla8_merge_kernel(MlaArgs a) {
+  pdl_release();
+  pdl_wait();
+  const int r = blockIdx.x / a.n_heads, h = blockIdx.x % a.n_heads, stride = (a.n_heads + F8_HEADS - 1) / F8_HEADS * F8_HEADS;
+  const int2 share = __ldcg(a.shares + r);
+  if (share.y <= 1) return;
+  const size_t row0 = (size_t)share.x * stride;
+  float gm, gl;
+  float4 o;
+  lse_reduce_row<false, GROUPS>(a.part_m + row0, a.part_l + row0, a.part_acc + row0 * LATENT, nullptr, nullptr, nullptr, share.y, stride, h, gm, gl, o);
+  if (threadIdx.x < 128) {
+    const float inv = gl > 0.f ? 1.f / gl : 0.f;           // (NaN: the sums are, and stay so)
+    const __half2 h0 = __floats2half2_rn(o.x * inv, o.y * inv), h1 = __floats2half2_rn(o.z * inv, o.w * inv);
+    *reinterpret_cast<uint2*>(a.out + (size_t)blockIdx.x * LATENT + threadIdx.x * 4) =
+        make_uint2(*reinterpret_cast<const uint32_t*>(&h0), *reinterpret_cast<const uint32_t*>(&h1));
+  }
 }
 
 }  // namespace
@@ -502,11 +609,39 @@ int f8_launch(const MlaArgs& a, const MlaPaged& pg, const CUtensorMap& q, cudaSt
 // implemented in mla_flash_tc.cu
 bool mla_rows_map(CUtensorMap* m, const void* rows, int64_t n);
 
+// CTAs (of 64 heads) among which the splits of m rows of up to n_keys keys are shared out; 0: every row gets as many splits.  Sharing costs
+// 2.3 us (lengths, splits and where a row's lie are found out on the device), so it is for rows where equal numbers would mean 8 tiles a
+// split or more: 8 rows of 17,000 to 32,768 keys 55.3 -> 51.2 us (29 -> 23 tiles the longest), 48 rows of 17 tiles 20.8 -> 23.5.
+int mla8_units(int m, int n_heads, int n_keys) {
+  const int groups = (n_heads + F8_HEADS - 1) / F8_HEADS, units = sm_count() / groups;
+  if (m < 2 || m > units || m > F8_SHARE_ROWS) return 0;
+  const int64_t tiles = ((int64_t)n_keys + F8_KEYS - 1) / F8_KEYS, each = units / m;
+  return (tiles + each - 1) / each >= 8 ? units : 0;
+}
+
+size_t mla8_units_bytes(int units, int m, int n_heads, MlaArgs* a, void* workspace) {
+  const size_t rows = (size_t)units * ((n_heads + F8_HEADS - 1) / F8_HEADS) * F8_HEADS, ml = (rows * sizeof(float) + 255) / 256 * 256;
+  if (a) {
+    uint8_t* ws = (uint8_t*)workspace;
+    a->part_acc = (float*)ws;
+    a->part_m = (float*)(ws + rows * LATENT * sizeof(float));
+    a->part_l = (float*)(ws + rows * LATENT * sizeof(float) + ml);
+    a->shares = (int2*)(ws + rows * LATENT * sizeof(float) + 2 * ml);
+  }
+  return rows * LATENT * sizeof(float) + 2 * ml + ((size_t)m * sizeof(int2) + 255) / 256 * 256;
+}
+
+// a.n_split == 0: splits shared out among a.units CTAs, and merged
 int mla8_flash_tc_launch(const MlaArgs& a, const MlaPaged& pg, int dtype, cudaStream_t s) {
   alignas(64) CUtensorMap q;
   if (!mla_rows_map(&q, a.q_lat, (int64_t)a.m * a.n_heads)) return HK_ERR_UNSUPPORTED;
-  if (a.raw_idx) return dtype == HK_I8 ? f8_launch<true, CACHE_I8>(a, pg, q, s) : f8_launch<true, CACHE_E4M3>(a, pg, q, s);
-  return dtype == HK_I8 ? f8_launch<false, CACHE_I8>(a, pg, q, s) : f8_launch<false, CACHE_E4M3>(a, pg, q, s);
+  const int st = a.raw_idx ? (dtype == HK_I8 ? f8_launch<true, CACHE_I8>(a, pg, q, s) : f8_launch<true, CACHE_E4M3>(a, pg, q, s))
+                           : (dtype == HK_I8 ? f8_launch<false, CACHE_I8>(a, pg, q, s) : f8_launch<false, CACHE_E4M3>(a, pg, q, s));
+  if (st != HK_OK || a.n_split > 0) return st;
+  const unsigned rows = (unsigned)(a.m * a.n_heads);
+  const cudaError_t e = a.units / a.m > LSE_FEW_SPLITS ? pdl_launch(mla8_merge_kernel<LSE_GROUPS>, dim3(rows), dim3(LSE_THREADS), 0, s, a)
+                                                       : pdl_launch(mla8_merge_kernel<LSE_GROUPS_FEW>, dim3(rows), dim3(128 * LSE_GROUPS_FEW), 0, s, a);
+  return e == cudaSuccess ? HK_OK : HK_ERR_CUDA;
 }
 
 }  // namespace hk

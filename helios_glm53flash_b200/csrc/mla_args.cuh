@@ -23,6 +23,9 @@ struct MlaArgs {
   float* part_acc;
   // window > 0: a row of n keys attends to the keys p >= n - window and p < sinks only
   int window, sinks;
+  // n_split == 0 (8-bit cache): splits shared out on the device among `units` CTAs, whose first and number each row's first CTA stores
+  int units;
+  int2* shares;
   int keep_nan;             // scores that are no numbers make outputs that are none (0: zeros, as the fp16 cache's callers know it)
 };
 

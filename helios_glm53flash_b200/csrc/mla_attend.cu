@@ -16,6 +16,8 @@ int mla_flash_tc_launch(const MlaArgs& a, cudaStream_t s, bool clusters = false)
 int mla_flash_tc_auto_splits(int m, int n_keys);
 // implemented in mla8_flash_tc.cu
 int mla8_flash_tc_launch(const MlaArgs& a, const MlaPaged& pg, int dtype, cudaStream_t s);
+int mla8_units(int m, int n_heads, int n_keys);
+size_t mla8_units_bytes(int units, int m, int n_heads, MlaArgs* a, void* workspace);
 // implemented in mla8_cache.cu
 int mla8_read_launch(const MlaPaged& pg, int dtype, int head, int shift, int n, __half* out, cudaStream_t s);
 bool mla8_paged(MlaPaged* pg, const void* ckv8, const float* scales, int dtype, int64_t n_blocks, int block, const int* block_table,
@@ -148,35 +150,50 @@ static int attend(MlaArgs a, int n_keys_hint, int n_split, bool choose, void* wo
   return HK_OK;
 }
 
-// every 64 heads of a row are work of their own
-static int mla8_auto_splits(int m, int n_heads, int n_keys) {
+// Splits of a call over the 8-bit cache that gives no number of them; units: the CTAs that they are shared out among on the device (0: not)
+static int attend8_splits(int m, int n_heads, int n_keys, bool dense, int* units) {
+  *units = dense && !force_simt() ? mla8_units(m, n_heads, n_keys) : 0;
   if (force_simt()) return simt_auto_splits(m, n_heads, n_keys);
-  const int64_t rows = (int64_t)m * ((n_heads + 63) / 64);
+  const int64_t rows = (int64_t)m * ((n_heads + 63) / 64);  // every 64 heads of a row are work of their own
   return mla_flash_tc_auto_splits(rows > INT32_MAX ? INT32_MAX : (int)rows, n_keys);
 }
+static size_t attend8_bytes(int m, int n_heads, int n_split, int units) {
+  return units > 0 ? mla8_units_bytes(units, m, n_heads, nullptr, nullptr) : n_split > 1 ? partial_layout(n_split, (int64_t)m * n_heads).total : 0;
+}
 
-// the 8-bit cache: final output, through split partials in the workspace where there is more than one split
+// the 8-bit cache: final output, through partials in the workspace where rows have more than one split
 static int attend8(MlaArgs a, const MlaPaged& pg, int dtype, int n_keys_hint, int n_split, void* workspace, size_t workspace_bytes,
                    cudaStream_t s) {
-  if (n_split <= 0) n_split = mla8_auto_splits(a.m, a.n_heads, n_keys_hint);
+  int units = 0;
+  if (n_split <= 0) n_split = attend8_splits(a.m, a.n_heads, n_keys_hint, !a.raw_idx, &units);
   if (n_split > LSE_MAX_SPLITS) return HK_ERR_UNSUPPORTED;
+  const size_t need = attend8_bytes(a.m, a.n_heads, n_split, units);
+  if (need && (!workspace || workspace_bytes < need)) return HK_ERR_WORKSPACE;
+  if (need && !aligned(workspace, 256)) return HK_ERR_INVALID;
+  if (units > 0) {
+    a.units = units;
+    mla8_units_bytes(units, a.m, a.n_heads, &a, workspace);
+    const int st = mla8_flash_tc_launch(a, pg, dtype, s);
+    if (st != HK_ERR_UNSUPPORTED) return st;
+    n_split = 1;                                           // (no tensor-map encoder)
+  }
   const int64_t rows = (int64_t)a.m * a.n_heads;
-  __half* final_out = a.out;
   a.n_split = n_split;
   if (n_split > 1) {
     const PartialLayout pl = partial_layout(n_split, rows);
-    if (!workspace || workspace_bytes < pl.total) return HK_ERR_WORKSPACE;
-    if (!aligned(workspace, 256)) return HK_ERR_INVALID;
     char* ws = (char*)workspace;
     a.part_m = (float*)ws;
     a.part_l = (float*)(ws + pl.off_l);
     a.part_acc = (float*)(ws + pl.off_acc);
-    a.out = nullptr;
   }
   int st = force_simt() ? HK_ERR_UNSUPPORTED : mla8_flash_tc_launch(a, pg, dtype, s);
-  if (st == HK_ERR_UNSUPPORTED) st = dtype == HK_I8 ? launch_simt_as<CACHE_I8>(a, pg, s) : launch_simt_as<CACHE_E4M3>(a, pg, s);
+  if (st == HK_ERR_UNSUPPORTED) {
+    MlaArgs c = a;
+    if (n_split > 1) c.out = nullptr;
+    st = dtype == HK_I8 ? launch_simt_as<CACHE_I8>(c, pg, s) : launch_simt_as<CACHE_E4M3>(c, pg, s);
+  }
   if (st != HK_OK || n_split == 1) return st;
-  return combine(a.part_m, a.part_l, a.part_acc, n_split, rows, final_out, s);
+  return combine(a.part_m, a.part_l, a.part_acc, n_split, rows, a.out, s);
 }
 
 // keys of a row, for choosing the splits of a dense call
@@ -207,9 +224,9 @@ static ChunkPlan chunk_plan(int m, int n_heads, int pos_start, int window, int s
 
 }  // namespace hk
 
-HK_API int hk_mla8_auto_splits(int m, int n_heads, int n_keys) {
-  if (m <= 0 || n_keys <= 0 || n_heads < hk::SIMT_HG) return 1;
-  return hk::mla8_auto_splits(m, n_heads, n_keys);
+HK_API size_t hk_mla8_sparse_workspace_bytes(int m, int n_heads, int kidx) {
+  int units = 0;
+  return m > 0 && n_heads >= hk::SIMT_HG && kidx > 0 ? hk::attend8_bytes(m, n_heads, hk::attend8_splits(m, n_heads, kidx, false, &units), 0) : 0;
 }
 
 HK_API size_t hk_mla8_dense_workspace_bytes(int m, int n_heads, int pos_start, int n_keys_hint, int window, int sinks, int per_row) {
@@ -220,8 +237,9 @@ HK_API size_t hk_mla8_dense_workspace_bytes(int m, int n_heads, int pos_start, i
     const int splits = hk::mla_flash_tc_auto_splits(m, keys);
     return c.bytes + (splits > 1 ? hk_mla_partial_bytes(splits, (int64_t)m * n_heads) : 0);
   }
-  const int splits = hk::mla8_auto_splits(m, n_heads, keys);
-  return splits > 1 ? hk_mla_partial_bytes(splits, (int64_t)m * n_heads) : 0;
+  int units = 0;
+  const int splits = hk::attend8_splits(m, n_heads, keys, true, &units);
+  return hk::attend8_bytes(m, n_heads, splits, units);
 }
 
 HK_API int hk_mla8_dense(const void* q_lat, const void* ckv8, const float* scales, int dtype, int64_t n_blocks, int block,

@@ -327,11 +327,11 @@ int hk_mla8_append(const float* kv_pre, const void* ln_w_f16, void* ckv8, float*
 int hk_mla8_read(const void* ckv8, const float* scales, int dtype, int64_t n_blocks, int block, const int* block_table,
                  int table_stride, int pos, int n, void* out_f16, void* stream);
 
-/* Number of splits that the library picks for m rows of n_keys keys over the 8-bit cache, and the workspace of a dense call that leaves the
- * number to it (per_row: kv_len or row_seq is given, the keys of a row are then n_keys_hint, 4,096 where that is 0).  A call that gives
- * n_split needs hk_mla_partial_bytes(n_split, m * n_heads) where n_split > 1; so does hk_mla8_sparse with hk_mla8_auto_splits.      */
-int hk_mla8_auto_splits(int m, int n_heads, int n_keys);
+/* Workspace of calls over the 8-bit cache that leave the splits to the library (n_split <= 0); those of several long rows are shared out on the
+ * device by the rows' lengths.  per_row: kv_len or row_seq is given; n_keys_hint: about the keys of the longest row then, 4,096 where it is 0 (a smaller number costs
+ * time where rows are longer, no more).  A call that gives n_split > 1 needs hk_mla_partial_bytes(n_split, m * n_heads).               */
 size_t hk_mla8_dense_workspace_bytes(int m, int n_heads, int pos_start, int n_keys_hint, int window, int sinks, int per_row);
+size_t hk_mla8_sparse_workspace_bytes(int m, int n_heads, int kidx);
 
 /* hk_mla_dense over the 8-bit cache: row r attends to the first kv_len[r] positions of its sequence (kv_len NULL: pos_start + r + 1).
  * window > 0: of these the last `window` and the first `sinks` only, as in hk_mla_window; window = 0: all.  n_heads: a multiple of 4.

@@ -57,14 +57,33 @@ def test_workspace_too_small(lib):
         assert call(lib, name, args, m=2, n_split=2000, ws=A, ws_bytes=1 << 60) in (hk.HK_ERR_UNSUPPORTED, hk.HK_ERR_WORKSPACE)
 
 
-def test_tensors_that_are_no_cache_raise():
+def test_tensors_that_are_no_cache_raise(lib):
     import torch
+    from helios_glm53flash_b200 import _binding as nb
     ok = torch.zeros(4, 16, 512, dtype=torch.int8)
     scales, table = torch.zeros(4), torch.zeros(2, 2, dtype=torch.int32)
-    assert hk._cache8(ok, scales, None) == (hk.HK_I8, 4, 16, None, 0)
-    assert hk._cache8(ok.view(torch.float8_e4m3fn), scales, table)[0] == hk.HK_E4M3
+    assert nb.cache8(ok, scales, None) == (hk.HK_I8, 4, 16, 0, 1)
+    assert nb.cache8(ok.view(torch.float8_e4m3fn), scales, table) == (hk.HK_E4M3, 4, 16, 2, 2)
+    assert nb.cache8(ok, scales, table[0]) == (hk.HK_I8, 4, 16, 2, 1)
     for args in ((ok.view(torch.uint8), scales, None), (ok[:, :, :256], scales, None), (ok.view(-1), scales, None), (ok[:, ::2], scales, None),
                  (ok, scales[:3], None), (ok, scales.double(), None), (ok, torch.zeros(8)[::2], None), (ok, scales, table.long()),
-                 (ok, scales, table[:, :1]), (ok, scales, table.view(1, 2, 2)), (ok, scales, table[:, :0])):
+                 (ok, scales, table[:, :1]), (ok, scales, table.view(1, 2, 2)), (ok, scales, table[:, :0]), (ok, scales, torch.tensor(3, dtype=torch.int32))):
         with pytest.raises(ValueError):
-            hk._cache8(*args)
+            nb.cache8(*args)
+    for args in ((ok, scales), (ok, None, None), (3, scales, None), (ok, scales, 5)):
+        with pytest.raises(TypeError):
+            nb.cache8(*args)
+
+
+def test_workspaces_are_enough_and_no_more(lib):
+    """sizes that the calls then ask for, on the host: one byte less is refused before any launch"""
+    per_row = lib.hk_mla8_dense_workspace_bytes(2, 64, 0, 5000, 0, 0, 1)
+    chunk = lib.hk_mla8_dense_workspace_bytes(100, 64, 1000, 0, 0, 0, 0)
+    sparse = lib.hk_mla8_sparse_workspace_bytes(1, 64, 2052)
+    assert per_row > 64 * 2056 and chunk >= 1100 * 1024 and sparse > 64 * 2056
+    assert call(lib, "hk_mla8_dense", DENSE, m=2, hint=5000, ws=A, ws_bytes=per_row - 1) == hk.HK_ERR_WORKSPACE
+    assert call(lib, "hk_mla8_dense", DENSE, m=100, kv_len=None, row_seq=None, pos_start=1000, stride=20, ws=A, ws_bytes=chunk - 1) == hk.HK_ERR_WORKSPACE
+    assert call(lib, "hk_mla8_sparse", SPARSE, m=1, kidx=2052, ws=A, ws_bytes=sparse - 1) == hk.HK_ERR_WORKSPACE
+    assert call(lib, "hk_mla8_sparse", SPARSE, m=1, kidx=2052, ws=A + 64, ws_bytes=sparse) == hk.HK_ERR_INVALID
+    assert lib.hk_mla8_dense_workspace_bytes(2, 64, 0, 5000, 64, 4, 1) < per_row, "fewer keys under a window"
+    assert lib.hk_mla8_sparse_workspace_bytes(5000, 64, 2052) == 0 and lib.hk_mla8_sparse_workspace_bytes(1, 64, 64) == 0
