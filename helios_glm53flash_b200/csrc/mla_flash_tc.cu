@@ -63,6 +63,7 @@ constexpr float RESCALE_THRESHOLD = 8.0f;         // log2 units: P stays below 2
 constexpr int FT_LOAD_WARPS = 4, FT_THREADS = (6 + FT_LOAD_WARPS) * 32, FT_SLOTS = FT_KEYS / FT_LOAD_WARPS;   // key slots per loader warp
 
 constexpr int FT_PAIR_KEYS = 700;                 // keys of a row, on average, from which on two rows of a chunk go to a pair of CTAs
+constexpr int FT_WINDOW_PAIR_KEYS = 2300;         // the same where a window limits them
 constexpr int FT_MINI = 16;                       // keys of a tile in Q's place
 constexpr int FT_MAX_CL = 16;                     // CTAs of a cluster
 // Parts that a row's output channels are shared out in, a cluster each.  Four: a quarter of the product, of the accumulator and of the
@@ -718,6 +719,8 @@ __global__ __launch_bounds__(FT_THREADS, 1) void mla_flash_tc_kernel(
 #include "mla_pair_tc.cuh"
 namespace hk {
 
+int mla_window_keys(int n, int window, int sinks);        // mla_attend.cu
+
 int mla_flash_tc_auto_splits(int m, int n_keys) {
   // At most one CTA per SM (a second wave would double the time), at least two tiles per split, splits of equal tile counts.  With
   // the merge, 1 / 2 / 3 tiles per split, us: 2,052 gathered rows of one query 12.1 / 11.3 / 12.7, of four 16.9 / 12.6 / 13.5 (more
@@ -742,7 +745,8 @@ static int ft_prepare() {
     auto any_cluster = [](auto* kernel) { return cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) == cudaSuccess; };
     if (!whole_sm(mla_flash_tc_kernel<false, false, false>) || !whole_sm(mla_flash_tc_kernel<true, false, false>) ||
         !whole_sm(mla_flash_tc_kernel<false, true, false>) || !whole_sm(mla_flash_tc_kernel<true, true, false>) ||
-        !whole_sm(mla_flash_tc_kernel<false, false, true>) || !whole_sm(mla_flash_tc_kernel<false, true, true>) || !whole_sm(mla_pair_tc_kernel) ||
+        !whole_sm(mla_flash_tc_kernel<false, false, true>) || !whole_sm(mla_flash_tc_kernel<false, true, true>) || !whole_sm(mla_pair_tc_kernel<false>) ||
+        !whole_sm(mla_pair_tc_kernel<true>) ||
         !any_cluster(mla_flash_tc_kernel<false, true, false>) || !any_cluster(mla_flash_tc_kernel<true, true, false>) ||
         !any_cluster(mla_flash_tc_kernel<false, true, true>))
       return HK_ERR_CUDA;
@@ -844,7 +848,12 @@ int mla_flash_tc_launch(const MlaArgs& a, cudaStream_t s, bool clusters) {
   // Two rows of a causal chunk share their keys.  Below 700 keys a row on average the pair's own costs (a cluster to start, the later row's own
   // key as a tile) are more than it gains: us, a CTA a row / pairs, 148 rows at 300 15.3 / 15.4, at 600 19.7 / 19.5, at 1,000 25.5 / 24.2;
   // 500 at 300 65.7 / 67.8, at 700 89.7 / 86.5; 1,200 at 0 151 / 154, 1,500 209 / 208, 2,500 470 / 431.
-  const bool pairs = !clusters && !a.window && !a.raw_idx && !a.kv_len && !a.kv_base && a.out && a.n_split == 1 && a.m >= 2 && a.pos_start + a.m / 2 >= FT_PAIR_KEYS;
+  // Under a window the keys of a row are few enough that a row's own costs count, which a persistent grid of single CTAs hides and pairs do
+  // not: 2,048 rows at 30,000, persistent / pairs, us, window 1,500 430 / 455, 2,000 535 / 542, 2,800 714 / 702, 4,096 1,003 / 957, 16,384
+  // 3,989 / 3,484.
+  const int seen = a.window > 0 ? min(a.pos_start + a.m / 2, mla_window_keys(0, a.window, a.sinks)) : a.pos_start + a.m / 2;
+  const bool pairs = !clusters && !a.raw_idx && !a.kv_len && !a.kv_base && a.out && a.n_split == 1 && a.m >= 2 &&
+                     seen >= (a.window > 0 ? FT_WINDOW_PAIR_KEYS : FT_PAIR_KEYS);
   if (!box_map(&qmap, a.q_lat, q_rows) || (!a.raw_idx && !pairs && !box_map(&box, a.ckv, extent))) return HK_ERR_UNSUPPORTED;
   if (a.out) {
     const cuuint64_t dims[2] = {LATENT, q_rows};
@@ -857,11 +866,11 @@ int mla_flash_tc_launch(const MlaArgs& a, cudaStream_t s, bool clusters) {
   if (pairs) {
     alignas(64) CUtensorMap vbox;
     if (!box_map(&box, a.ckv, extent, 32, 8) || !box_map(&vbox, a.ckv, extent, 32, 4)) return HK_ERR_UNSUPPORTED;
-    const cudaError_t e = pdl_launch_cluster(2, mla_pair_tc_kernel, dim3((unsigned)((a.m + 1) / 2 * 2)), dim3(PT_THREADS), FS_SMEM, s, a,
+    const cudaError_t e = pdl_launch_cluster(2, a.window > 0 ? mla_pair_tc_kernel<true> : mla_pair_tc_kernel<false>, dim3((unsigned)((a.m + 1) / 2 * 2)), dim3(PT_THREADS), FS_SMEM, s, a,
                                              device_status_ptr(), box, vbox, rows, qmap, omap);
     return e == cudaSuccess && cudaPeekAtLastError() == cudaSuccess ? HK_OK : HK_ERR_CUDA;
   }
-  // Gathered rows: at most a CTA per SM (592 rows of 2,048 keys 180 -> 166 us).  Dense rows, whose loads start faster: a CTA
+  // Gathered rows and windows: at most a CTA per SM (592 rows of 2,048 keys 180 -> 166 us; 2,048 rows under a window of 1,023 367 -> 324).  Dense rows, whose loads start faster: a CTA
   // each (600 rows at 32,768 keys 2.72 ms, persistent 2.85).  Partials always: their rows leave through the idle ring.
   if (clusters) {
     const dim3 grid((unsigned)(a.m * FT_CS * a.n_split));
@@ -870,7 +879,7 @@ int mla_flash_tc_launch(const MlaArgs& a, cudaStream_t s, bool clusters) {
     return e == cudaSuccess && cudaPeekAtLastError() == cudaSuccess ? HK_OK : HK_ERR_CUDA;
   }
   const int64_t items = (int64_t)a.n_split * a.m;
-  const dim3 grid((unsigned)(a.raw_idx && a.out && items > sm_count() ? sm_count() : items));
+  const dim3 grid((unsigned)((a.raw_idx || a.window > 0) && a.out && items > sm_count() ? sm_count() : items));
   const auto kernel = a.raw_idx ? mla_flash_tc_kernel<true, false, false> : a.window ? mla_flash_tc_kernel<false, false, true> : mla_flash_tc_kernel<false, false, false>;
   const cudaError_t e = pdl_launch(kernel, grid, dim3(FT_THREADS), FS_SMEM, s, a, device_status_ptr(), box, rows, qmap, omap);
   return e == cudaSuccess && cudaPeekAtLastError() == cudaSuccess ? HK_OK : HK_ERR_CUDA;

@@ -15,6 +15,10 @@
 // its barriers count the arrivals of both, and commits arrive at both.
 // The later row's own key is a tile of its own, whose P V leaves the earlier row's accumulator alone (a mask of lanes): a weight of
 // zero would not do where the cache row holds infinities or NaN.
+// WIN: the rows see their last a.window keys and the first a.sinks.  Both see the later row's; the key that leaves the window between
+// them, the earlier row's alone, is key 16 of the last tile, whose product leaves the later row's accumulator alone.  Tiles at the edge of
+// what is seen arrive whole, and the softmax warps clear the other keys' rows of V (by four rows at a time, as a ragged tile comes, the three
+// or four such tiles of a pair cost 2,048 rows under a window of 1,023 392 us where they now take 343).
 #pragma once
 
 namespace hk {
@@ -62,14 +66,15 @@ __device__ __forceinline__ void pt_mma_tmem_a(uint32_t leader, uint32_t d, uint3
       "r"(a), "l"(bd), "r"(idesc), "r"((uint32_t)acc), "r"(leader)
       : "memory");
 }
-// the second CTA's accumulator only: the first one's 128 lanes are left alone
-__device__ __forceinline__ void pt_mma_second(uint32_t leader, uint32_t d, uint64_t ad, uint64_t bd, uint32_t idesc, bool acc) {
+// one CTA's accumulator only: the other one's 128 lanes are left alone
+__device__ __forceinline__ void pt_mma_one(int rank, uint32_t leader, uint32_t d, uint64_t ad, uint64_t bd, uint32_t idesc, bool acc) {
+  const uint32_t skip_first = rank == 0 ? 0u : 0xffffffffu;
   asm volatile(
       "{\n\t.reg .pred p, q;\n\t"
       "setp.ne.b32 p, %4, 0;\n\t"
       "setp.ne.b32 q, %5, 0;\n\t"
       "@q tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, {%6, %6, %6, %6, %7, %7, %7, %7}, p;\n\t}" ::"r"(d),
-      "l"(ad), "l"(bd), "r"(idesc), "r"((uint32_t)acc), "r"(leader), "r"(0xffffffffu), "r"(0u)
+      "l"(ad), "l"(bd), "r"(idesc), "r"((uint32_t)acc), "r"(leader), "r"(skip_first), "r"(~skip_first)
       : "memory");
 }
 // Arrives at this barrier in both CTAs, some time after the products.  Each such arrival is waited for in both CTAs before either may leave (a
@@ -117,6 +122,7 @@ __device__ __forceinline__ bool pt_wait(uint64_t* bar, uint32_t parity, volatile
 
 // grid = 2 CTAs a pair of rows, cluster of 2.  tmap_k / tmap_v: boxes of 32 keys x 512 and x 256 channels; tmap_rows, tmap_q, tmap_o as in
 // mla_flash_tc_kernel.
+template <bool WIN>
 __global__ __launch_bounds__(PT_THREADS, 1) void mla_pair_tc_kernel(
     MlaArgs a, int* __restrict__ status, const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ CUtensorMap tmap_v,
     const __grid_constant__ CUtensorMap tmap_rows, const __grid_constant__ CUtensorMap tmap_q, const __grid_constant__ CUtensorMap tmap_o) {
@@ -131,9 +137,22 @@ __global__ __launch_bounds__(PT_THREADS, 1) void mla_pair_tc_kernel(
   const int r1 = a.m - 1 - 2 * (int)(blockIdx.x >> 1), r0 = max(0, r1 - 1), row = rank == 0 ? r0 : r1;
   const bool lone = r1 == 0, mine = !(lone && rank == 1);
   const int n = a.pos_start + r0 + 1;                      // the keys of both rows
-  const int whole = (n + FT_KEYS - 1) / FT_KEYS, n_tiles = whole + (lone ? 0 : 1);
-  auto keys = [&](int t) -> int { return t < whole ? min(FT_KEYS, n - t * FT_KEYS) : 1; };
-  auto key0 = [&](int t) -> int { return t < whole ? t * FT_KEYS : n; };
+  // window form: both see the keys p >= lo and p < first_keys of the n; tile t is tile t, or t + jump behind the sinks' tiles; gone: the key that
+  // the earlier row alone sees (-1: none)
+  int lo = 0, first_keys = 0, first_tiles = 0, jump = 0, gone = -1;
+  if (WIN) {
+    const KeyList early = key_list(n, a.window, a.sinks), late = lone ? early : key_list(n + 1, a.window, a.sinks);
+    lo = late.lo;
+    first_keys = late.head;
+    if (late.lo > early.lo && early.lo >= a.sinks) gone = early.lo;
+    first_tiles = (first_keys + FT_KEYS - 1) / FT_KEYS;
+    jump = max(lo / FT_KEYS - first_tiles, 0);
+  }
+  const int whole = (n + FT_KEYS - 1) / FT_KEYS - jump, n_tiles = whole + (lone ? 0 : 1);
+  auto key0 = [&](int t) -> int { return t >= whole ? n : WIN && t >= first_tiles ? (t + jump) * FT_KEYS : t * FT_KEYS; };
+  auto keys = [&](int t) -> int { return t < whole ? min(FT_KEYS, n - key0(t)) : 1; };
+  auto edge = [&](int t) -> bool { return WIN && t < whole && keys(t) == FT_KEYS && key0(t) < lo && key0(t) + FT_KEYS > first_keys; };
+  const int last_quads = gone >= 0 ? 2 : 1;                // window form: groups of four keys of the last tile (keys 0 and 16)
 
   if (tid == 0) {
     for (int b = 0; b < FT_NBUF; b++) {
@@ -170,12 +189,15 @@ __global__ __launch_bounds__(PT_THREADS, 1) void mla_pair_tc_kernel(
   auto slot = [&](int t) -> uint8_t* { return smem + FS_K + t % FT_NBUF * FT_TILE; };
   auto turn = [](int t) -> uint32_t { return t / FT_NBUF & 1; };
   const int other = 32 * (1 - rank);                       // the other CTA's keys of a tile
-  // a ragged tile: four rows at a time, those past the end read as zeros
+  // a ragged tile: four rows at a time, those past the end (and those that are not seen) read as zeros
   auto gather = [&](uint32_t leader, int t, int k0, int blk0, int blocks, uint32_t dst, uint64_t* bar) {
     const int base = key0(t), valid = keys(t);
-    auto at = [&](int k) -> int { return k < valid ? base + k : -1; };
+    auto at = [&](int k) -> int {
+      if (WIN && t == whole && k == 16) return gone;
+      return k < valid && (!WIN || t == whole || base + k >= lo || base + k < first_keys) ? base + k : -1;
+    };
 #pragma unroll 1
-    for (int q = 0; q < 8; q++)
+    for (int q = 0; q < (WIN && t == whole ? 4 * last_quads : 8); q += WIN && t == whole ? 4 : 1)
 #pragma unroll 1
       for (int blk = 0; blk < blocks; blk++)
         tma_gather4_rows(leader, dst + blk * PT_BLK + q * 512, &tmap_rows, (blk0 + blk) * 64, at(k0 + 4 * q), at(k0 + 4 * q + 1), at(k0 + 4 * q + 2),
@@ -196,8 +218,10 @@ __global__ __launch_bounds__(PT_THREADS, 1) void mla_pair_tc_kernel(
         ok = tc::mbar_wait<FT_POLL_NS>(&ms.k_free[b], turn(t) ^ 1, abort_flag, 22) && ok;
         ok = tc::mbar_wait<FT_POLL_NS>(&ms.v_here[b], turn(t) ^ 1, abort_flag, 34) && ok;
       }
-      if (lane == 0) tc::mbar_arrive_expect_tx(&ms.k_here[b], PT_V);
+      const bool last = WIN && t == whole;                 // its two keys are the first CTA's
+      if (lane == 0) tc::mbar_arrive_expect_tx(&ms.k_here[b], !last ? PT_V : rank == 0 ? last_quads * 8 * 512 : 0);
       __syncwarp();
+      if (last && rank == 1) continue;
       if (keys(t) < FT_KEYS) gather(leader, t, 32 * rank, 0, 8, tc::smem_u32(slot(t)), &ms.k_here[b]);
       else if (lane == 0) pt_tma_box(slot(t), &tmap_k, key0(t) + 32 * rank, 0, &ms.k_here[b]);
       __syncwarp();
@@ -209,10 +233,12 @@ __global__ __launch_bounds__(PT_THREADS, 1) void mla_pair_tc_kernel(
       const int b = t % FT_NBUF;
       if (t == 2) ok = tc::mbar_wait<FT_POLL_NS>(&ms.q_moved, 0, abort_flag, 21) && ok;
       if (t >= FT_NBUF) ok = tc::mbar_wait<FT_POLL_NS>(&ms.v_free[b], turn(t) ^ 1, abort_flag, 35) && ok;
-      if (lane == 0) tc::mbar_arrive_expect_tx(&ms.v_here[b], 2 * PT_V_HALF);
+      const bool last = WIN && t == whole;
+      if (lane == 0) tc::mbar_arrive_expect_tx(&ms.v_here[b], !last ? 2 * PT_V_HALF : PT_V_HALF + (rank == 1 ? last_quads * 4 * 512 : 0));
       __syncwarp();
       uint8_t* const dst = slot(t) + PT_V + (1 - rank) * PT_V_HALF;
-      if (keys(t) < FT_KEYS) gather(leader, t, other, 4 * rank, 4, tc::smem_u32(dst), &ms.v_here[b]);
+      if (last && rank == 0) {
+      } else if (keys(t) < FT_KEYS) gather(leader, t, other, 4 * rank, 4, tc::smem_u32(dst), &ms.v_here[b]);
       else if (lane == 0) pt_tma_box(dst, &tmap_v, key0(t) + other, 4 * rank, &ms.v_here[b]);
       __syncwarp();
       ok = tc::mbar_wait<FT_POLL_NS>(&ms.k_here[b], turn(t), abort_flag, 32) && ok;
@@ -275,8 +301,10 @@ __global__ __launch_bounds__(PT_THREADS, 1) void mla_pair_tc_kernel(
                        t > 0 || kk > 0);
         } else {
 #pragma unroll
-          for (int nh = 0; nh < 2; nh++)
-            pt_mma_second(leader, tmem + FT_O + nh * 128, pd, tc::sdesc_advance(vd, nh * 2 * PT_BLK), idesc, true);
+          for (int nh = 0; nh < 2; nh++) {
+            pt_mma_one(1, leader, tmem + FT_O + nh * 128, pd, tc::sdesc_advance(vd, nh * 2 * PT_BLK), idesc, !WIN || t > 0);
+            if (WIN && gone >= 0) pt_mma_one(0, leader, tmem + FT_O + nh * 128, tc::sdesc_advance(pd, 32), tc::sdesc_advance(vd, nh * 2 * PT_BLK + 2048), idesc, t > 0);
+          }
         }
         pt_commit(leader, &ms.pv_done[b]);
         if (t + FT_NBUF < n_tiles) pt_commit(leader, &ms.v_free[kb]);
@@ -326,7 +354,13 @@ __global__ __launch_bounds__(PT_THREADS, 1) void mla_pair_tc_kernel(
       arrive_first(&ms.s_free[b]);
       // keys of this thread: 32 half .. + 31 of the tile; the last tile is the second row's
       const int have = (t < whole || rank == 1 ? keys(t) : 0) - 32 * half;
-      const uint32_t mask = have >= 32 ? 0xffffffffu : have <= 0 ? 0u : (1u << have) - 1u;
+      uint32_t mask = have >= 32 ? 0xffffffffu : have <= 0 ? 0u : (1u << have) - 1u;
+      if (WIN && t < whole) {
+        const int p = key0(t) + 32 * half, from = lo - p, to = first_keys - p;   // keys from `from` on and below `to` are seen
+        mask &= (from <= 0 ? 0xffffffffu : from >= 32 ? 0u : 0xffffffffu << from) | (to <= 0 ? 0u : to >= 32 ? 0xffffffffu : (1u << to) - 1u);
+      } else if (WIN && rank == 0 && half == 0 && gone >= 0) {
+        mask = 1u << 16;
+      }
       float tmax = -INFINITY;
 #pragma unroll
       for (int j = 0; j < 32; j++) {
@@ -377,6 +411,17 @@ __global__ __launch_bounds__(PT_THREADS, 1) void mla_pair_tc_kernel(
       }
       l += sum;
       ok = tc::mbar_wait<FT_POLL_NS>(&ms.v_here[t % FT_NBUF], (t / FT_NBUF) & 1, abort_flag, 33) && ok;   // this CTA's part of V
+      if (WIN && (edge(t) || t == whole)) {
+        // keys that are not seen weigh nothing, but nothing times infinity is NaN: their rows of V become zeros (of the last tile, which 32
+        // keys are multiplied of, all but keys 0 and 16)
+        const int k = tid & 63, p = key0(t) + k;
+        const bool seen = t == whole ? k >= 32 || k == 0 || (k == 16 && gone >= 0) : p >= lo || p < first_keys;
+        if (!seen) {
+          uint8_t* v_row = slot(t) + PT_V + (k >> 5) * PT_V_HALF + (tid >> 6) * 2 * PT_BLK + (k & 31) * 128;
+#pragma unroll
+          for (int c = 0; c < 16; c++) *reinterpret_cast<uint4*>(v_row + (c >> 3) * PT_BLK + (((c + lane) & 7) << 4)) = make_uint4(0u, 0u, 0u, 0u);
+        }
+      }
       tc::fence_async_smem();
       tc::fence_before_sync();
       arrive_first(&ms.p_full[b]);

@@ -258,6 +258,34 @@ def test_dense8_rows_and_blocks_that_do_not_count():
         assert (out[[1, 3, 5, 6, 7]] == 0).all()
 
 
+@pytest.mark.parametrize("kind,heads,lens,window,sinks", [
+    ("i8", 64, [3000, 700], 0, 0), ("e4m3", 64, [64, 5000, 1, 0, 2500, 129, 640], 0, 0), ("i8", 16, [100] * 40, 0, 0), ("i8", 100, [2000, 90, 1500], 0, 0),
+    ("e4m3", 64, [4000, 4000, 100], 700, 65), ("i8", 64, [(37 * i) % 300 for i in range(148)], 0, 0), ("i8", 64, [9000] + [3] * 100, 0, 0),
+    ("e4m3", 64, [0, 0, -4], 0, 0)])
+def test_dense8_splits_shared_out_by_length(kind, heads, lens, window, sinks):
+    """a hint of long rows: the splits are shared out on the device; one long row among short ones, empty ones, a row a CTA, sequences out of range"""
+    gen, block, m = gen_of(len(lens) + heads), 64, len(lens)
+    blocks = max(1, (max(lens) + block - 1) // block)
+    ckv8, scales = cache(gen, kind, min(4000, blocks * m + 2), block, spread=1.0)
+    table = torch.randint(0, ckv8.shape[0], (m, blocks), device="cuda", generator=gen, dtype=torch.int32)
+    seqs = list(range(m))
+    if m > 100:
+        seqs[7], seqs[m - 1] = -1, m
+    q = queries(gen, m, heads)
+    for _ in range(2):                                         # the second time the workspace holds other partials
+        out = torch.full((m + 1, heads, 512), 5.0, dtype=torch.float16, device="cuda")
+        hk.mla8_dense_prefill(q, ckv8, scales, out, m, 0, n_heads=heads, block_table=table, row_seq=ints(seqs), kv_len=ints(lens), window=window,
+                              sinks=sinks, n_keys_hint=1 << 20)
+        finish()
+        want = []
+        for r, n in enumerate(lens):
+            s = seqs[r]
+            p = visible(n if 0 <= s < m else 0, window, sinks)
+            want.append(attend(q[r].double(), rows_of(ckv8, scales, table[max(0, min(s, m - 1))], p), 0.0625))
+        close(out, want)
+        assert (out[m:] == 5.0).all()
+
+
 def test_a_row_that_is_not_finite_is_seen_in_the_output():
     gen = gen_of(6)
     ckv8, scales = cache(gen, "i8", 4, 64)
@@ -320,7 +348,9 @@ def test_window_rows(heads, lens, window, sinks, n_split):
 
 
 @pytest.mark.parametrize("pos,rows,window,sinks", [(0, 1, 1, 0), (0, 130, 64, 0), (500, 65, 100, 3), (1000, 37, 1000, 64), (200, 300, 1, 1), (3000, 21, 900, 130),
-                                                   (2000, 64, 1024, 4), (1500, 33, 1500, 0), (900, 150, 129, 0), (5000, 2, 4000, 10)])
+                                                   (2000, 64, 1024, 4), (1500, 33, 1500, 0), (900, 150, 129, 0), (5000, 2, 4000, 10), (2047, 6, 1, 900), (3000, 7, 2, 701), (1000, 9, 64, 640),
+                                                   (0, 1500, 800, 3), (2000, 301, 700, 0), (3000, 21, 2400, 130), (2500, 300, 2310, 70), (3000, 6, 1, 2500), (6000, 64, 4000, 0),
+                                                   (2350, 150, 2333, 1)])
 def test_window_chunk(pos, rows, window, sinks):
     """a causal chunk; each row's first hidden key and everything before it is infinite or NaN for that row alone or for all"""
     gen = gen_of(pos + rows)
@@ -336,10 +366,10 @@ def test_window_chunk(pos, rows, window, sinks):
     assert (out[rows:] == 5.0).all()
 
 
-@pytest.mark.parametrize("rows", [7, 8, 40])
-def test_window_rows_do_not_take_over_what_their_neighbours_see(rows):
+@pytest.mark.parametrize("rows,window", [(7, 1000), (8, 1000), (200, 1000), (7, 2500), (40, 2500)])      # single CTAs, a grid that walks rows, pairs of CTAs
+def test_window_rows_do_not_take_over_what_their_neighbours_see(rows, window):
     """keys that leave the window one by one are infinite: the rows that still see one are not finite, the others are what they are without"""
-    gen, pos, window, sinks = gen_of(rows), 1200, 1000, 5
+    gen, pos, sinks = gen_of(rows), window + 200, 5
     ckv = torch.randn(pos + rows, 512, device="cuda", generator=gen).half()
     hot = pos + 1 - window + 3                                 # seen by rows 0 .. 3
     ckv[hot] = math.inf
@@ -352,6 +382,11 @@ def test_window_rows_do_not_take_over_what_their_neighbours_see(rows):
     for r in clean:
         o, tol = attend(q[r].double(), ckv[:pos + r + 1][visible(pos + r + 1, window, sinks)].double(), 0.0625)
         assert bool(((out[r].double() - o).abs() <= tol).all()), r
+    ckv[hot] = 1.0
+    ckv[pos + rows - 1] = 1.0
+    hk.mla_window_prefill(q, ckv, out, rows, pos, window, sinks=sinks)
+    finish()
+    close(out, [attend(q[r].double(), ckv[:pos + r + 1][visible(pos + r + 1, window, sinks)].double(), 0.0625) for r in range(rows)])
 
 
 def test_window_cut_by_the_end_of_the_cache():
