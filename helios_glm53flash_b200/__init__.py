@@ -89,7 +89,7 @@ SIGNATURES = {
     "hk_mla_window": (_i, [_vp, _vp, _i64, _vp, _vp, _i, _i, _i, _vp, _i, _i, _f, _i, _vp, _sz, _vp]),
     "hk_mla8_append": (_i, [_vp, _vp, _vp, _vp, _i, _i64, _i, _vp, _i, _i, _vp, _vp, _i, _f, _vp, _vp]),
     "hk_mla8_read": (_i, [_vp, _vp, _i, _i64, _i, _vp, _i, _i, _i, _vp, _vp]),
-    "hk_mla8_sparse_workspace_bytes": (_sz, [_i, _i, _i]),
+    "hk_mla8_sparse_workspace_bytes": (_sz, [_i, _i, _i, _i64, _i]),
     "hk_mla8_dense_workspace_bytes": (_sz, [_i, _i, _i, _i, _i, _i, _i]),
     "hk_mla8_dense": (_i, [_vp, _vp, _vp, _i, _i64, _i, _vp, _i, _i, _vp, _vp, _i, _i, _i, _vp, _i, _i, _f, _i, _i, _vp, _sz, _vp]),
     "hk_mla8_sparse": (_i, [_vp, _vp, _vp, _i, _i64, _i, _vp, _i, _i, _vp, _vp, _i, _vp, _i, _i, _f, _i, _vp, _sz, _vp]),
@@ -481,8 +481,8 @@ def mla8_dense_workspace_bytes(m, n_heads, pos_start, n_keys_hint=0, window=0, s
     return load_library().hk_mla8_dense_workspace_bytes(m, n_heads, pos_start, n_keys_hint or 0, window, sinks, int(per_row))
 
 
-def mla8_sparse_workspace_bytes(m, n_heads, kidx):
-    return load_library().hk_mla8_sparse_workspace_bytes(m, n_heads, kidx)
+def mla8_sparse_workspace_bytes(m, n_heads, kidx, positions, per_row=False):
+    return load_library().hk_mla8_sparse_workspace_bytes(m, n_heads, kidx, positions, int(per_row))
 
 
 def mla8_dense_prefill(q_lat, ckv8, scales, lat_out, qlen, pos_start, stream=None, scale=0.0625, n_heads=64, block_table=None, row_seq=None,
@@ -507,7 +507,8 @@ def mla8_sparse_decode(q_lat, ckv8, scales, raw_idx, kidx, lat_out, m, stream=No
     tag, n_blocks, block, stride, seqs = _native.cache8(ckv8, scales, block_table)
     ws = workspace
     if ws is None:
-        need = (_native.hk_mla8_sparse_workspace_bytes(m, n_heads, kidx) if n_split <= 0
+        positions = (stride if stride else n_blocks) * block
+        need = (_native.hk_mla8_sparse_workspace_bytes(m, n_heads, kidx, positions, 0 if row_seq is None else 1) if n_split <= 0
                 else _native.hk_mla_partial_bytes(n_split, m * n_heads) if n_split > 1 else 0)
         if need:
             ws = _scratch(need, q_lat.device, stream)

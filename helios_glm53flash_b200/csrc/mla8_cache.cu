@@ -174,12 +174,23 @@ cudaError_t append_launch(const AppendArgs& a, dim3 grid, cudaStream_t s) {
 }
 
 // rows i of out: position i of the sequence below `head`, i + shift from there on; f16(scale * value), zeros where there is no block.
-// A warp four rows, a lane eight channels and the eight 256 further on (8-byte loads, 16-byte stores).
-constexpr int READ_ROWS = 4;
+// A warp four rows, a lane eight channels and the eight 256 further on (8-byte loads, 16-byte stores).  CTAs behind those of the rows: the
+// n_idx gathered positions of a sparse call, those without a block as -1.
+constexpr int READ_ROWS = 4, READ_IDX = 8;
 template <int FMT>
-__global__ void __launch_bounds__(256) mla8_read_kernel(MlaPaged pg, int head, int shift, int n, __half* __restrict__ out) {
+__global__ void __launch_bounds__(256) mla8_read_kernel(MlaPaged pg, int head, int shift, int n, __half* __restrict__ out, const int* __restrict__ idx,
+                                                        int64_t n_idx, int* __restrict__ idx_out) {
   pdl_release();
   pdl_wait();
+  const int row_ctas = (n + 8 * READ_ROWS - 1) / (8 * READ_ROWS);
+  if ((int)blockIdx.x >= row_ctas) {
+#pragma unroll
+    for (int k = 0; k < READ_IDX; k++) {
+      const int64_t i = ((int64_t)(blockIdx.x - row_ctas) * READ_IDX + k) * 256 + threadIdx.x;
+      if (i < n_idx) idx_out[i] = pg.block_of(0, idx[i]) >= 0 ? idx[i] : -1;
+    }
+    return;
+  }
   const int lane = threadIdx.x & 31, i0 = (blockIdx.x * 8 + (threadIdx.x >> 5)) * READ_ROWS;
   uint2 v[READ_ROWS][2];
   float s[READ_ROWS];
@@ -232,10 +243,12 @@ bool mla8_paged(MlaPaged* pg, const void* ckv8, const float* scales, int dtype, 
   return true;
 }
 
-// n rows of sequence 0 as fp16: positions 0 .. head - 1, then head + shift ..
-int mla8_read_launch(const MlaPaged& pg, int dtype, int head, int shift, int n, __half* out, cudaStream_t s) {
-  return pdl_launch(dtype == HK_I8 ? mla8_read_kernel<CACHE_I8> : mla8_read_kernel<CACHE_E4M3>, dim3((unsigned)((n + 8 * READ_ROWS - 1) / (8 * READ_ROWS))),
-                    dim3(256), 0, s, pg, head, shift, n, out) == cudaSuccess
+// n rows of sequence 0 as fp16: positions 0 .. head - 1, then head + shift ..; and n_idx gathered positions
+int mla8_read_launch(const MlaPaged& pg, int dtype, int head, int shift, int n, __half* out, cudaStream_t s, const int* idx, int64_t n_idx, int* idx_out) {
+  const int64_t ctas = ((int64_t)n + 8 * READ_ROWS - 1) / (8 * READ_ROWS) + (n_idx + READ_IDX * 256 - 1) / (READ_IDX * 256);
+  if (ctas > INT32_MAX) return HK_ERR_UNSUPPORTED;
+  return pdl_launch(dtype == HK_I8 ? mla8_read_kernel<CACHE_I8> : mla8_read_kernel<CACHE_E4M3>, dim3((unsigned)ctas), dim3(256), 0, s, pg, head, shift, n,
+                    out, idx, n_idx, idx_out) == cudaSuccess
              ? HK_OK
              : HK_ERR_CUDA;
 }
@@ -279,5 +292,5 @@ HK_API int hk_mla8_read(const void* ckv8, const float* scales, int dtype, int64_
   MlaPaged pg;
   HK_REQUIRE(out_f16 && pos >= 0 && n >= 0 && (int64_t)pos + n <= INT32_MAX && aligned(out_f16, 16));
   HK_REQUIRE(mla8_paged(&pg, ckv8, scales, dtype, n_blocks, block, block_table, table_stride, 1, nullptr));
-  return n == 0 ? HK_OK : mla8_read_launch(pg, dtype, 0, pos, n, (__half*)out_f16, as_stream(stream));
+  return n == 0 ? HK_OK : mla8_read_launch(pg, dtype, 0, pos, n, (__half*)out_f16, as_stream(stream), nullptr, 0, nullptr);
 }

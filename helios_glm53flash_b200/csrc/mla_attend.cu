@@ -19,7 +19,8 @@ int mla8_flash_tc_launch(const MlaArgs& a, const MlaPaged& pg, int dtype, cudaSt
 int mla8_units(int m, int n_heads, int n_keys);
 size_t mla8_units_bytes(int units, int m, int n_heads, MlaArgs* a, void* workspace);
 // implemented in mla8_cache.cu
-int mla8_read_launch(const MlaPaged& pg, int dtype, int head, int shift, int n, __half* out, cudaStream_t s);
+int mla8_read_launch(const MlaPaged& pg, int dtype, int head, int shift, int n, __half* out, cudaStream_t s, const int* idx = nullptr, int64_t n_idx = 0,
+                     int* idx_out = nullptr);
 bool mla8_paged(MlaPaged* pg, const void* ckv8, const float* scales, int dtype, int64_t n_blocks, int block, const int* block_table,
                 int table_stride, int n_seqs, const int* row_seq);
 bool mla_flash_cluster_shape(int m, int tiles, int* n_split);
@@ -203,17 +204,19 @@ static int mla8_dense_keys(int m, int pos_start, int n_keys_hint, int window, in
 }
 
 // A chunk of many rows turns the positions that it sees into fp16 rows once, in the workspace, and attends to those: the fp16 kernels share a
-// tile between two rows and do not convert it again for each (1,000 rows at 8,192 1,264 -> FILL us).  One more rounding, to the 11 bits that the
-// fp16 cache has.  Positions under a window: whole tiles of the sinks, then from the tile of the first row's window on, `shift` positions left out.
+// tile between two rows and do not convert it again for each (1,000 rows at 8,192 1,264 -> 841 us).  One more rounding, to the 11 bits that the
+// fp16 cache has.  Rows x keys from which on that is faster, us, rows as they are / read first: 16 x 2,016 19.7 / 22.3, 32 x 2,032 33.4 / 31.3,
+// 8 x 8,200 26.4 / 27.0, 16 x 8,208 38.1 / 35.8, 64 x 564 33.5 / 34.3, 96 x 596 39.6 / 20.5, 8 x 30,008 52.3 / 48.5, 4 x 100,004 79 / 90.
+// Positions under a window: whole tiles of the sinks, then from the tile of the first row's window on, `shift` positions left out.
 struct ChunkPlan {
   bool on;
   int head, shift, rows;
   size_t bytes;
 };
-constexpr int CHUNK_ROWS = 64;
-static ChunkPlan chunk_plan(int m, int n_heads, int pos_start, int window, int sinks, bool per_row) {
+constexpr int CHUNK_ROWS = 8, CHUNK_WORK = 65536;
+static ChunkPlan chunk_plan(int m, int n_heads, int pos_start, int keys, int window, int sinks, bool per_row) {
   ChunkPlan c{};
-  c.on = !per_row && n_heads == 64 && m >= CHUNK_ROWS && !force_simt();
+  c.on = !per_row && n_heads == 64 && m >= CHUNK_ROWS && (int64_t)m * keys >= CHUNK_WORK && !force_simt();
   const int64_t head = (sinks + 63LL) / 64 * 64, from = window > 0 && pos_start + 1 > window ? (pos_start + 1 - window) / 64 * 64 : 0;
   c.head = head < from ? (int)head : 0;
   c.shift = head < from ? (int)(from - head) : 0;
@@ -222,17 +225,37 @@ static ChunkPlan chunk_plan(int m, int n_heads, int pos_start, int window, int s
   return c;
 }
 
+// Likewise the gathered rows of a chunk of one sequence, where its positions are few against the keys that are gathered: the fp16 rows of all
+// positions, and the gathered numbers with -1 for those without a block.  2,052 keys a row, us, rows as they are / read first: 100 rows out of
+// 16,384 positions 50.7 / 48.1, 400 147 / 129, 800 299 / 251; 296 rows out of 65,536 (9 gathered keys a position) 101 / 108, 400 (13) 148 / 147,
+// 800 (25) 303 / 272.
+constexpr int GATHER_ROWS = 100, GATHER_TIMES = 16;
+struct GatherPlan {
+  bool on;
+  size_t rows, bytes;
+};
+static GatherPlan gather_plan(int m, int n_heads, int kidx, int64_t positions, bool per_row) {
+  GatherPlan g{};
+  g.on = !per_row && n_heads == 64 && m >= GATHER_ROWS && (int64_t)m * kidx >= GATHER_TIMES * positions && !force_simt();
+  g.rows = (size_t)positions * LATENT * sizeof(__half);
+  g.bytes = align_up(g.rows + (size_t)m * kidx * sizeof(int), 256);
+  return g;
+}
+
 }  // namespace hk
 
-HK_API size_t hk_mla8_sparse_workspace_bytes(int m, int n_heads, int kidx) {
+HK_API size_t hk_mla8_sparse_workspace_bytes(int m, int n_heads, int kidx, int64_t positions, int per_row) {
+  if (m <= 0 || n_heads < hk::SIMT_HG || kidx <= 0 || positions < 0 || positions > INT32_MAX) return 0;
   int units = 0;
-  return m > 0 && n_heads >= hk::SIMT_HG && kidx > 0 ? hk::attend8_bytes(m, n_heads, hk::attend8_splits(m, n_heads, kidx, false, &units), 0) : 0;
+  const hk::GatherPlan g = hk::gather_plan(m, n_heads, kidx, positions, per_row);
+  const int splits = g.on ? hk::mla_flash_tc_auto_splits(m, kidx) : hk::attend8_splits(m, n_heads, kidx, false, &units);
+  return (g.on ? g.bytes : 0) + hk::attend8_bytes(m, n_heads, splits, 0);
 }
 
 HK_API size_t hk_mla8_dense_workspace_bytes(int m, int n_heads, int pos_start, int n_keys_hint, int window, int sinks, int per_row) {
   if (m <= 0 || n_heads < hk::SIMT_HG || pos_start < 0 || sinks < 0) return 0;
   const int keys = hk::mla8_dense_keys(m, pos_start, n_keys_hint, window, sinks, per_row);
-  const hk::ChunkPlan c = hk::chunk_plan(m, n_heads, pos_start, window, sinks, per_row);
+  const hk::ChunkPlan c = hk::chunk_plan(m, n_heads, pos_start, keys, window, sinks, per_row);
   if (c.on) {
     const int splits = hk::mla_flash_tc_auto_splits(m, keys);
     return c.bytes + (splits > 1 ? hk_mla_partial_bytes(splits, (int64_t)m * n_heads) : 0);
@@ -262,7 +285,7 @@ HK_API int hk_mla8_dense(const void* q_lat, const void* ckv8, const float* scale
   a.window = window; a.sinks = sinks;
   const bool per_row = kv_len || row_seq;
   const int keys = mla8_dense_keys(m, pos_start, n_keys_hint, window, sinks, per_row);
-  const ChunkPlan c = chunk_plan(m, n_heads, pos_start, window, sinks, per_row);
+  const ChunkPlan c = chunk_plan(m, n_heads, pos_start, keys, window, sinks, per_row);
   if (c.on && n_split <= 0) {
     if (!workspace || workspace_bytes < c.bytes) return HK_ERR_WORKSPACE;
     if (!aligned(workspace, 256)) return HK_ERR_INVALID;
@@ -293,6 +316,20 @@ HK_API int hk_mla8_sparse(const void* q_lat, const void* ckv8, const float* scal
   a.raw_idx = raw_idx; a.kidx = kidx;
   a.m = m; a.n_heads = n_heads; a.scale = scale;
   a.out = (__half*)lat_out;
+  const int64_t positions = (block_table ? (int64_t)table_stride : n_blocks) * block;
+  const GatherPlan g = gather_plan(m, n_heads, kidx, positions, row_seq);
+  if (g.on && n_split <= 0) {
+    if (!workspace || workspace_bytes < g.bytes) return HK_ERR_WORKSPACE;
+    if (!aligned(workspace, 256)) return HK_ERR_INVALID;
+    int* idx = (int*)((char*)workspace + g.rows);
+    const int st = mla8_read_launch(pg, dtype, 0, 0, (int)positions, (__half*)workspace, as_stream(stream), raw_idx, (int64_t)m * kidx, idx);
+    if (st != HK_OK) return st;
+    a.ckv = (const __half*)workspace;
+    a.ckv_rows = positions;
+    a.raw_idx = idx;
+    a.keep_nan = 1;
+    return attend(a, kidx, 0, true, (char*)workspace + g.bytes, workspace_bytes - g.bytes, as_stream(stream));
+  }
   return attend8(a, pg, dtype, kidx, n_split, workspace, workspace_bytes, as_stream(stream));
 }
 

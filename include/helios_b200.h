@@ -329,22 +329,25 @@ int hk_mla8_read(const void* ckv8, const float* scales, int dtype, int64_t n_blo
 
 /* Workspace of calls over the 8-bit cache that leave the splits to the library (n_split <= 0); those of several long rows are shared out on the
  * device by the rows' lengths.  per_row: kv_len or row_seq is given; n_keys_hint: about the keys of the longest row then, 4,096 where it is 0 (a smaller number costs
- * time where rows are longer, no more).  A call that gives n_split > 1 needs hk_mla_partial_bytes(n_split, m * n_heads).               */
+ * time where rows are longer, no more); per_row of a sparse call: row_seq is given, positions: table_stride * block, or n_blocks * block without a
+ * table.  A call that gives n_split > 1 needs hk_mla_partial_bytes(n_split, m * n_heads).               */
 size_t hk_mla8_dense_workspace_bytes(int m, int n_heads, int pos_start, int n_keys_hint, int window, int sinks, int per_row);
-size_t hk_mla8_sparse_workspace_bytes(int m, int n_heads, int kidx);
+size_t hk_mla8_sparse_workspace_bytes(int m, int n_heads, int kidx, int64_t positions, int per_row);
 
 /* hk_mla_dense over the 8-bit cache: row r attends to the first kv_len[r] positions of its sequence (kv_len NULL: pos_start + r + 1).
  * window > 0: of these the last `window` and the first `sinks` only, as in hk_mla_window; window = 0: all.  n_heads: a multiple of 4.
  * Scores and sums are fp32; a row without keys gives zeros.
  * A chunk (kv_len and row_seq NULL) is checked on the host, pos_start + m positions have a place in the table (else HK_ERR_INVALID); in it a
- * position whose entry names no block is a latent of zeros, as hk_mla8_read gives it.  A chunk of 64 heads and 64 rows or more, with n_split <= 0,
- * reads its positions as fp16 rows into the workspace first and attends to those (latents beyond 65,504 are infinite there).        */
+ * position whose entry names no block is a latent of zeros, as hk_mla8_read gives it.  A chunk of 64 heads, 8 rows and 65,536 (row, key)
+ * pairs or more, with n_split <= 0, reads its positions as fp16 rows into the workspace first and attends to those (latents beyond 65,504 are infinite there).        */
 int hk_mla8_dense(const void* q_lat, const void* ckv8, const float* scales, int dtype, int64_t n_blocks, int block,
                   const int* block_table, int table_stride, int n_seqs, const int* row_seq, const int* kv_len, int pos_start,
                   int window, int sinks, void* lat_out, int m, int n_heads, float scale, int n_split, int n_keys_hint,
                   void* workspace, size_t workspace_bytes, void* stream);
 
-/* hk_mla_sparse over the 8-bit cache: raw_idx [m][kidx] holds positions of the row's sequence (negative = skipped; duplicates count twice).  */
+/* hk_mla_sparse over the 8-bit cache: raw_idx [m][kidx] holds positions of the row's sequence (negative = skipped; duplicates count twice).
+ * Many rows of one sequence (64 heads, row_seq NULL, n_split <= 0, 100 rows or more that gather 16 keys a position of the table or more) read its
+ * positions as fp16 rows into the workspace first, as a chunk of hk_mla8_dense does.                                                          */
 int hk_mla8_sparse(const void* q_lat, const void* ckv8, const float* scales, int dtype, int64_t n_blocks, int block,
                    const int* block_table, int table_stride, int n_seqs, const int* row_seq, const int* raw_idx, int kidx,
                    void* lat_out, int m, int n_heads, float scale, int n_split, void* workspace, size_t workspace_bytes,

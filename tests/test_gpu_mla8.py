@@ -172,7 +172,17 @@ def test_dense8_rows(kind, block, heads, lens, window, sinks, n_split):
     assert (out[m:] == 5.0).all()
 
 
+def read_first(pos, rows, heads, window, sinks):
+    """whether a chunk reads its positions as fp16 rows first"""
+    keys = pos + rows
+    if window:
+        keys = 64 * min(-(-sinks // 64) + (window + 62) // 64 + 1, -(-keys // 64))
+    return heads == 64 and rows >= 8 and rows * keys >= 65536
+
+
 @pytest.mark.parametrize("kind,block,heads,pos,rows,window,sinks", [
+    ("i8", 32, 64, 0, 300, 0, 0), ("e4m3", 64, 64, 9000, 9, 0, 0), ("i8", 16, 64, 2000, 200, 400, 70), ("e4m3", 128, 64, 3000, 150, 500, 0),
+    ("i8", 64, 64, 1000, 300, 100, 700), ("i8", 64, 64, 4000, 40, 2500, 3),
     ("i8", 64, 64, 0, 2, 0, 0), ("i8", 64, 64, 0, 70, 0, 0), ("e4m3", 32, 64, 333, 40, 0, 0), ("i8", 16, 16, 100, 9, 0, 0), ("i8", 64, 64, 1000, 130, 0, 0),
     ("i8", 64, 64, 700, 90, 200, 4), ("e4m3", 128, 64, 10, 150, 64, 0), ("e4m3", 16, 64, 500, 80, 33, 130), ("i8", 32, 32, 50, 200, 1000, 7)])
 def test_dense8_chunk(kind, block, heads, pos, rows, window, sinks):
@@ -188,18 +198,18 @@ def test_dense8_chunk(kind, block, heads, pos, rows, window, sinks):
     out = torch.full((rows + 1, heads, 512), 5.0, dtype=torch.float16, device="cuda")
     hk.mla8_dense_prefill(q, ckv8, scales, out, rows, pos, n_heads=heads, block_table=table, window=window, sinks=sinks)
     finish()
-    rows16 = rows >= 64 and heads == 64
+    rows16 = read_first(pos, rows, heads, window, sinks)
     close(out, [attend(q[r].double(), rows_of(ckv8, scales, table[0], visible(pos + r + 1, window, sinks)), 0.0625, rows16) for r in range(rows)])
     assert (out[rows:] == 5.0).all()
 
 
-@pytest.mark.parametrize("rows", [10, 70])
+@pytest.mark.parametrize("rows", [10, 300])
 def test_dense8_chunk_with_a_position_without_a_block_and_a_row_that_is_not_finite(rows):
     """short chunks read the cache as they go, long ones as fp16 rows first: an entry that names no block is 16 latents of zeros in both, and a
     scale that is NaN makes the outputs of the rows that see it NaN, under a window only of those that see it"""
     gen, pos = gen_of(rows), 100
-    ckv8, scales = cache(gen, "i8", 14, 16)
-    table = table_for(gen, 1, 11, 14)
+    ckv8, scales = cache(gen, "i8", 30, 16)
+    table = table_for(gen, 1, 26, 30)
     table[0, 2] = -1
     q = queries(gen, rows, 64)
     out = torch.empty(rows, 64, 512, dtype=torch.float16, device="cuda")
@@ -210,13 +220,13 @@ def test_dense8_chunk_with_a_position_without_a_block_and_a_row_that_is_not_fini
     for r in range(rows):
         p = visible(pos + r + 1, 0, 0)
         keys = torch.cat((rows_of(ckv8, scales, table[0], p[:32]), zero, rows_of(ckv8, scales, table[0], p[48:])))
-        want.append(attend(q[r].double(), keys, 0.0625, rows >= 64))
+        want.append(attend(q[r].double(), keys, 0.0625, read_first(pos, rows, 64, 0, 0)))
     close(out, want)
     scales[table[0, 6]] = math.nan                            # positions 96 .. 111
     hk.mla8_dense_prefill(q, ckv8, scales, out, rows, pos, block_table=table)
     finish()
     assert torch.isnan(out).all()
-    hk.mla8_dense_prefill(q, ckv8, scales, out, rows, pos, block_table=table, window=5, sinks=17)
+    hk.mla8_dense_prefill(q, ckv8, scales, out, rows, pos, block_table=table, window=5, sinks=17 if rows < 300 else 90)
     finish()
     bad = torch.tensor([pos + r + 1 - 5 <= 111 for r in range(rows)], device="cuda")
     assert torch.isnan(out[bad]).all() and torch.isfinite(out[~bad]).all()
@@ -321,6 +331,30 @@ def test_sparse8(kind, block, heads, m, kidx, n_split):
     finish()
     close(out, [attend(q[r].double(), rows_of(ckv8, scales, table[seqs[r]], idx[r][idx[r] >= 0].long()), 0.0625) for r in range(m)])
     assert (out[m:] == 5.0).all()
+
+
+@pytest.mark.parametrize("kind,block,m,kidx,blocks", [("i8", 32, 100, 480, 90), ("e4m3", 16, 300, 65, 25), ("i8", 128, 200, 513, 16), ("e4m3", 64, 130, 2052, 30)])
+def test_sparse8_of_many_rows(kind, block, m, kidx, blocks):
+    """rows that gather many keys of few positions: read as fp16 rows first; a block that is none, positions behind the table, a scale that is NaN"""
+    gen, n = gen_of(m + kidx), blocks * block
+    ckv8, scales = cache(gen, kind, blocks + 3, block, spread=0.5)
+    table = table_for(gen, 1, blocks, blocks + 3)
+    table[0, 3], table[0, 5] = -1, blocks + 3
+    idx = torch.randint(0, n, (m, kidx), device="cuda", generator=gen, dtype=torch.int32)
+    idx[:, 3::7] = -1
+    idx[:, 4::50] = n + 5
+    idx[1] = 3 * block + 1                                    # nothing but a block that is none
+    q = queries(gen, m, 64)
+    out = torch.full((m + 1, 64, 512), 5.0, dtype=torch.float16, device="cuda")
+    hk.mla8_sparse_decode(q, ckv8, scales, idx, kidx, out, m, block_table=table)
+    finish()
+    close(out, [attend(q[r].double(), rows_of(ckv8, scales, table[0], idx[r][idx[r] >= 0].long()), 0.0625, rows16=True) for r in range(m)])
+    assert (out[m:] == 5.0).all() and (out[1] == 0).all()
+    scales[table[0, 0]] = math.nan
+    hk.mla8_sparse_decode(q, ckv8, scales, idx, kidx, out, m, block_table=table)
+    finish()
+    hit = ((idx >= 0) & (idx < block)).any(1)
+    assert torch.isnan(out[:m][hit]).all() and torch.isfinite(out[:m][~hit]).all()
 
 
 # ---------------------------------------------------------------------------------------------

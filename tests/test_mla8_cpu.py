@@ -79,11 +79,14 @@ def test_workspaces_are_enough_and_no_more(lib):
     """sizes that the calls then ask for, on the host: one byte less is refused before any launch"""
     per_row = lib.hk_mla8_dense_workspace_bytes(2, 64, 0, 5000, 0, 0, 1)
     chunk = lib.hk_mla8_dense_workspace_bytes(100, 64, 1000, 0, 0, 0, 0)
-    sparse = lib.hk_mla8_sparse_workspace_bytes(1, 64, 2052)
+    sparse = lib.hk_mla8_sparse_workspace_bytes(1, 64, 2052, 256, 1)
+    gathered = lib.hk_mla8_sparse_workspace_bytes(300, 64, 70, 256, 0)                 # 82 keys a position
     assert per_row > 64 * 2056 and chunk >= 1100 * 1024 and sparse > 64 * 2056
     assert call(lib, "hk_mla8_dense", DENSE, m=2, hint=5000, ws=A, ws_bytes=per_row - 1) == hk.HK_ERR_WORKSPACE
     assert call(lib, "hk_mla8_dense", DENSE, m=100, kv_len=None, row_seq=None, pos_start=1000, stride=20, ws=A, ws_bytes=chunk - 1) == hk.HK_ERR_WORKSPACE
     assert call(lib, "hk_mla8_sparse", SPARSE, m=1, kidx=2052, ws=A, ws_bytes=sparse - 1) == hk.HK_ERR_WORKSPACE
     assert call(lib, "hk_mla8_sparse", SPARSE, m=1, kidx=2052, ws=A + 64, ws_bytes=sparse) == hk.HK_ERR_INVALID
     assert lib.hk_mla8_dense_workspace_bytes(2, 64, 0, 5000, 64, 4, 1) < per_row, "fewer keys under a window"
-    assert lib.hk_mla8_sparse_workspace_bytes(5000, 64, 2052) == 0 and lib.hk_mla8_sparse_workspace_bytes(1, 64, 64) == 0
+    assert gathered >= 256 * 1024 + 300 * 70 * 4
+    assert call(lib, "hk_mla8_sparse", SPARSE, m=300, kidx=70, row_seq=None, ws=A, ws_bytes=gathered - 1) == hk.HK_ERR_WORKSPACE
+    assert lib.hk_mla8_sparse_workspace_bytes(5000, 64, 2052, 256, 1) == 0 and lib.hk_mla8_sparse_workspace_bytes(1, 64, 64, 256, 1) == 0
