@@ -14,7 +14,6 @@
 #include <cuda.h>   // CUtensorMap
 
 #include "latent8.cuh"
-#include "lse_reduce.cuh"
 #include "mla_args.cuh"
 #include "tc05.cuh"
 
@@ -584,24 +583,59 @@ int f8_launch(const MlaArgs& a, const MlaPaged& pg, const CUtensorMap& q, cudaSt
   return e == cudaSuccess && cudaPeekAtLastError() == cudaSuccess ? HK_OK : HK_ERR_CUDA;
 }
 
-// Merge of the splits that the attention kernel shared out: one CTA a (row, head).  Rows of one split are finished.
-template <int GROUPS>
-__global__ __launch_bounds__(128 * GROUPS) void mla8_merge_kernel(MlaArgs a) {
+// Merge of the splits that the attention kernel shared out: one CTA a (row, head), a thread four channels.  Rows of one split are finished.
+__global__ __launch_bounds__(128) void mla8_merge_kernel(MlaArgs a) {
+  __shared__ float s_w[F8_SHARE_ROWS];                     // (a row has no more splits than there are CTAs)
   pdl_release();
   pdl_wait();
-  const int r = blockIdx.x / a.n_heads, h = blockIdx.x % a.n_heads, stride = (a.n_heads + F8_HEADS - 1) / F8_HEADS * F8_HEADS;
+  const int r = blockIdx.x / a.n_heads, h = blockIdx.x % a.n_heads, lane = threadIdx.x & 31;
+  const size_t stride = (size_t)((a.n_heads + F8_HEADS - 1) / F8_HEADS) * F8_HEADS;
   const int2 share = __ldcg(a.shares + r);
-  if (share.y <= 1) return;
-  const size_t row0 = (size_t)share.x * stride;
-  float gm, gl;
-  float4 o;
-  lse_reduce_row<false, GROUPS>(a.part_m + row0, a.part_l + row0, a.part_acc + row0 * LATENT, nullptr, nullptr, nullptr, share.y, stride, h, gm, gl, o);
-  if (threadIdx.x < 128) {
-    const float inv = gl > 0.f ? 1.f / gl : 0.f;           // (NaN: the sums are, and stay so)
-    const __half2 h0 = __floats2half2_rn(o.x * inv, o.y * inv), h1 = __floats2half2_rn(o.z * inv, o.w * inv);
-    *reinterpret_cast<uint2*>(a.out + (size_t)blockIdx.x * LATENT + threadIdx.x * 4) =
-        make_uint2(*reinterpret_cast<const uint32_t*>(&h0), *reinterpret_cast<const uint32_t*>(&h1));
+  const int n = min(share.y, F8_SHARE_ROWS);
+  if (n <= 1) return;
+  const size_t row0 = (size_t)share.x * stride + h;
+  const float4* acc = reinterpret_cast<const float4*>(a.part_acc + row0 * LATENT) + threadIdx.x;
+  constexpr int AHEAD = 12;
+  float4 v[AHEAD];
+  auto load = [&](int s0) {
+#pragma unroll
+    for (int u = 0; u < AHEAD; u++)
+      if (s0 + u < n) v[u] = __ldcg(acc + (size_t)(s0 + u) * stride * (LATENT / 4));
+  };
+  load(0);
+  // every warp for itself; split s in lane s % 32, the weights of all in shared memory
+  float m[F8_SHARE_ROWS / 32], l[F8_SHARE_ROWS / 32], gm = -INFINITY, gl = 0.f;
+#pragma unroll
+  for (int k = 0; k < F8_SHARE_ROWS / 32; k++) {
+    const int s = lane + 32 * k;
+    m[k] = s < n ? __ldcg(a.part_m + row0 + s * stride) : -INFINITY;
+    l[k] = s < n ? __ldcg(a.part_l + row0 + s * stride) : 0.f;
+    gm = fmaxf(gm, m[k]);
   }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) gm = fmaxf(gm, __shfl_xor_sync(0xffffffffu, gm, o));
+#pragma unroll
+  for (int k = 0; k < F8_SHARE_ROWS / 32; k++) {
+    const float w = m[k] == -INFINITY ? 0.f : __expf(m[k] - gm);
+    gl = fmaf(w, l[k], gl);
+    if (threadIdx.x < 32) s_w[lane + 32 * k] = w;
+  }
+  gl = warp_sum(gl);
+  __syncthreads();
+  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int s0 = 0; s0 < n; s0 += AHEAD) {
+    if (s0 > 0) load(s0);
+#pragma unroll
+    for (int u = 0; u < AHEAD; u++)
+      if (s0 + u < n) {
+        const float w = s_w[s0 + u];
+        o.x = fmaf(w, v[u].x, o.x); o.y = fmaf(w, v[u].y, o.y); o.z = fmaf(w, v[u].z, o.z); o.w = fmaf(w, v[u].w, o.w);
+      }
+  }
+  const float inv = gl > 0.f ? 1.f / gl : 0.f;             // (NaN: the sums are, and stay so)
+  const __half2 h0 = __floats2half2_rn(o.x * inv, o.y * inv), h1 = __floats2half2_rn(o.z * inv, o.w * inv);
+  *reinterpret_cast<uint2*>(a.out + (size_t)blockIdx.x * LATENT + threadIdx.x * 4) =
+      make_uint2(*reinterpret_cast<const uint32_t*>(&h0), *reinterpret_cast<const uint32_t*>(&h1));
 }
 
 }  // namespace
@@ -638,9 +672,7 @@ int mla8_flash_tc_launch(const MlaArgs& a, const MlaPaged& pg, int dtype, cudaSt
   const int st = a.raw_idx ? (dtype == HK_I8 ? f8_launch<true, CACHE_I8>(a, pg, q, s) : f8_launch<true, CACHE_E4M3>(a, pg, q, s))
                            : (dtype == HK_I8 ? f8_launch<false, CACHE_I8>(a, pg, q, s) : f8_launch<false, CACHE_E4M3>(a, pg, q, s));
   if (st != HK_OK || a.n_split > 0) return st;
-  const unsigned rows = (unsigned)(a.m * a.n_heads);
-  const cudaError_t e = a.units / a.m > LSE_FEW_SPLITS ? pdl_launch(mla8_merge_kernel<LSE_GROUPS>, dim3(rows), dim3(LSE_THREADS), 0, s, a)
-                                                       : pdl_launch(mla8_merge_kernel<LSE_GROUPS_FEW>, dim3(rows), dim3(128 * LSE_GROUPS_FEW), 0, s, a);
+  const cudaError_t e = pdl_launch(mla8_merge_kernel, dim3((unsigned)(a.m * a.n_heads)), dim3(128), 0, s, a);
   return e == cudaSuccess ? HK_OK : HK_ERR_CUDA;
 }
 

@@ -97,11 +97,12 @@ static int combine_cs_launch(const float* pm, const float* pl, const float* pa, 
 static int combine(const float* pm, const float* pl, const float* pa, int n_split, int64_t rows,
                    __half* out, cudaStream_t s) {
   if (n_split > LSE_MAX_SPLITS) return HK_ERR_UNSUPPORTED;
-  // few rows and few splits (sparse decode of one sequence: 64 rows x 22 splits): channel-split form, four CTAs per
-  // row (15.1 vs 16.1 us per layer for the sparse step).  With many splits (dense decode of one sequence, 137) the
-  // same form with 32 thread groups measured slower than eight groups of 128 lanes (24.5 vs 23.5 us): not used.
-  if (rows < 256 && n_split <= LSE_FEW_SPLITS) return combine_cs_launch<8>(pm, pl, pa, n_split, rows, out, s);
-  if (n_split <= LSE_FEW_SPLITS && rows >= 256) return combine_launch<LSE_GROUPS_FEW>(pm, pl, pa, n_split, rows, out, s);
+  if (n_split <= LSE_FEW_SPLITS && rows >= 256)
+    return pdl_launch(lse_combine_few_kernel, dim3((unsigned)rows), dim3(128), 0, s, pm, pl, pa, n_split, rows, out) == cudaSuccess ? HK_OK : HK_ERR_CUDA;
+  // Four CTAs a row, a quarter of the channels each.  Bits as with one CTA of 1,024 threads, which has the rest: the sums are the same eight, in the
+  // same order, as long as a thread has one split's weight.  One / four, us: 64 rows of 40 splits 4.0 / 3.0, of 137 5.9 / 4.4, 320 rows of 29
+  // 10.1 / 5.2, 1,024 of 100 57 / 37.
+  if (n_split <= 256) return combine_cs_launch<8>(pm, pl, pa, n_split, rows, out, s);
   return combine_launch<LSE_GROUPS>(pm, pl, pa, n_split, rows, out, s);
 }
 
