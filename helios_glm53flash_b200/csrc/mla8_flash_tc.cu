@@ -9,8 +9,16 @@
 // 2^8), so a weight stays below 2^12, and one that underflows weighs nothing next to what moved the references.
 //
 // Work item = (query row, 64 heads, key split) -> one CTA.  Roles, tensor-memory plan and products are those of mla_flash_tc_kernel; what is
-// its own are eight warps in place of the copy engine, which load a tile of 64 keys x 512 bytes into registers one tile ahead, turn it into
-// fp16 and store it in the 128-byte-swizzle layout that both products read.  Rows that the query does not see become zeros there.
+// its own are eight warps in place of the copy engine, which load tiles of 64 keys x 512 bytes into registers two ahead, turn them into fp16
+// and store them in the 128-byte-swizzle layout that both products read.  Rows that the query does not see become zeros there.
+//
+// What bounds it: about 2,400 cycles a tile, of which shared memory is busy 1,810 at 128 B a cycle (64 KB of fp16 stored, K and V read, Q 16, P
+// 24 KB) and the schedulers 1,500 (6,000 instructions of warps a tile: 2,600 for the conversion, 1,800 for the softmax); with the loads left out
+// it takes as long.  HBM could bring a tile in 1,400.  8 rows of 17,000 to 32,768 keys: 43.7 us and 4.3 to merge (105 MB: 2.2 TB/s, 0.33 of the
+// measured copy).  Tried: raw tiles by the copy engine, converted out of shared memory (296 KB a tile are 2,310 cycles and leave room for two
+// fp16 tiles only: no faster); sixteen converting warps, registers moved to the softmax (47.1 us); one tile ahead (46.6; splits of two tiles
+// 0.2 us faster); rows asked for in L2 three tiles ahead (slower); 16 bytes of two neighbouring keys a lane in place of the exchange of words
+// (64-byte pieces: slower).
 #include <cuda.h>   // CUtensorMap
 
 #include "latent8.cuh"
@@ -262,53 +270,66 @@ __global__ __launch_bounds__(F8_THREADS, 1) void mla8_flash_tc_kernel(MlaArgs a,
       return pg.table ? f8_ld_int(pg.table + (size_t)it.row.seq * pg.table_stride + b) : b;
     };
     const int in_block = (1 << pg.shift) - 1;
-    uint4 v[F8_ROWS];
-    float sc = -1.f;
-    // asks for key i of a tile
     const uint8_t* src = pg.data + lane * 16;
-    auto request = [&](int i, int row) {
+    // asks for key i of a tile
+    auto request = [&](uint4& v, int i, int row) {
       const int at = __shfl_sync(0xffffffffu, row, i);
-      v[i] = make_uint4(0u, 0u, 0u, 0u);
-      if (at >= 0) v[i] = ld_stream16(src + (size_t)at * LATENT);
+      v = make_uint4(0u, 0u, 0u, 0u);
+      if (at >= 0) v = ld_stream16(src + (size_t)at * LATENT);
     };
-    int p0 = position(0), p1 = position(1), p2 = position(2);
-    int e0 = entry(p0), e1 = entry(p1);
     // row of the cache, -1: none (rows of a cache are counted in 31 bits).  In a chunk a seen position without a block is a key of zeros.
     const bool zeros = !GATHER && !a.kv_len && !pg.row_seq;
     auto row_of = [&](int p, int e) -> int { return e < 0 || e >= pg.n_blocks ? -1 : (e << pg.shift) + (p & in_block); };
+    auto scale_of = [&](int row, int p, int e) -> float { return row >= 0 ? f8_ld_float(pg.scales + e) : zeros && p >= 0 ? 0.f : -1.f; };
+    // On their way: the keys of two tiles, in registers; table entries of the third; positions of the fourth.
+    uint4 v[2][F8_ROWS];
+    float sc[2];
+    int p2, e2, p3;
     {
-      const int row = row_of(p0, e0);
-      sc = row >= 0 ? f8_ld_float(pg.scales + e0) : zeros && p0 >= 0 ? 0.f : -1.f;
+      const int p0 = position(0), p1 = position(1);
+      p2 = position(2);
+      const int e0 = entry(p0), e1 = entry(p1);
+      const int row0 = row_of(p0, e0);
+      sc[0] = scale_of(row0, p0, e0);
 #pragma unroll
-      for (int i = 0; i < F8_ROWS; i++) request(i, row);
+      for (int i = 0; i < F8_ROWS; i++) request(v[0][i], i, row0);
+      const int row1 = row_of(p1, e1);
+      sc[1] = scale_of(row1, p1, e1);
+#pragma unroll
+      for (int i = 0; i < F8_ROWS; i++) request(v[1][i], i, row1);
+      e2 = entry(p2);
+      p3 = position(3);
     }
     const int blk = lane >> 2, c0 = (lane & 3) * 2, swap = (lane >> 2) & 1;
-    for (int t = 0; t < n_tiles; t++) {
+    auto convert = [&](int t, uint4 (&x)[F8_ROWS], float& scale) {
       const int b = t % F8_NBUF;
-      // the next tile: its rows are known; the one after: its table entries; the third: its positions
-      const int row = row_of(p1, e1);
-      const float sc_next = row >= 0 ? f8_ld_float(pg.scales + e1) : zeros && p1 >= 0 ? 0.f : -1.f;
-      p1 = p2;
-      e1 = entry(p2);
-      p2 = position(t + 3);
+      const int row = row_of(p2, e2);
+      const float sc2 = scale_of(row, p2, e2);
+      p2 = p3;
+      e2 = entry(p3);
+      p3 = position(t + 4);
       if (t == F8_NBUF - 1) ok = tc::mbar_wait<F8_POLL_NS>(&ms.q_ready, 0, abort_flag, 41) && ok;   // Q came through the last slot
       if (t >= F8_NBUF) ok = tc::mbar_wait<F8_POLL_NS>(&ms.free[b], (t / F8_NBUF - 1) & 1, abort_flag, 42) && ok;
-      if (lane < F8_ROWS) ms.sc[b][k8 + lane] = sc;
+      if (lane < F8_ROWS) ms.sc[b][k8 + lane] = scale;
       uint8_t* dst = smem + F8S_K + b * F8_TILE + blk * F8_BLK + k8 * 128;
       // 16 channels are two 16-byte chunks of a 128-byte row; lanes four apart write them in the other order (no bank conflicts)
 #pragma unroll
       for (int i = 0; i < F8_ROWS; i++) {
         uint4 lo, hi;                                      // the chunk that is written first, the other
-        f8_to_f16<FMT>(swap ? make_uint4(v[i].z, v[i].w, v[i].x, v[i].y) : v[i], lo, hi);
+        f8_to_f16<FMT>(swap ? make_uint4(x[i].z, x[i].w, x[i].x, x[i].y) : x[i], lo, hi);
         const uint32_t a0 = i * 128 + (((c0 + swap) ^ i) << 4), a1 = i * 128 + (((c0 + 1 - swap) ^ i) << 4);
         *reinterpret_cast<uint4*>(dst + a0) = lo;
         *reinterpret_cast<uint4*>(dst + a1) = hi;
-        request(i, row);
+        request(x[i], i, row);
       }
-      sc = sc_next;
+      scale = sc2;
       tc::fence_async_smem();
       __syncwarp();
       if (lane == 0) tc::mbar_arrive(&ms.full[b]);
+    };
+    for (int t = 0; t < n_tiles; t += 2) {
+      convert(t, v[0], sc[0]);
+      if (t + 1 < n_tiles) convert(t + 1, v[1], sc[1]);
     }
   } else if (warp >= 4) {
     // =========================== tensor-core issue (whole warp, one elected lane; see mla_flash_tc_kernel) ===========================
