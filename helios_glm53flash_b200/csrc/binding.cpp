@@ -17,6 +17,7 @@
 // the Python layer loaded (bind), so that both sides drive the same build.
 #define PY_SSIZE_T_CLEAN
 #include <Python.h>
+#include <c10/cuda/CUDAFunctions.h>
 #include <c10/cuda/CUDAStream.h>
 #include <c10/util/Exception.h>
 #include <torch/csrc/autograd/python_variable.h>
@@ -220,6 +221,11 @@ PyObject* py_cache8(PyObject*, PyObject* const* args, Py_ssize_t n) {
     if ((!i8 && c.scalar_type() != at::kFloat8_e4m3fn) || c.dim() != 3 || c.size(2) != 512 || !c.is_contiguous())
       return refuse("ckv8: a contiguous [n_blocks, block, 512] tensor of int8 or float8_e4m3fn");
     if (s.scalar_type() != at::kFloat || s.numel() != c.size(0) || !s.is_contiguous()) return refuse("scales: a contiguous float32 tensor, one a block");
+    // an address of the host, or of another GPU than the one that the call runs on, would be a fault there
+    static const int devices = c10::cuda::device_count();
+    auto elsewhere = [&](const at::Tensor& t) { return devices > 0 && (!t.is_cuda() || t.device().index() != c10::cuda::current_device()); };
+    if (elsewhere(c) || elsewhere(s) || (args[2] != Py_None && elsewhere(THPVariable_Unpack(args[2]))))
+      return refuse("the 8-bit cache's tensors: on the current CUDA device");
     long long stride = 0, seqs = 1;
     if (args[2] != Py_None) {
       const at::Tensor& t = THPVariable_Unpack(args[2]);

@@ -54,7 +54,7 @@ __global__ void __launch_bounds__(APPEND_WARPS * 32) mla8_append_kernel(AppendAr
     r0 = seq * each;
     r1 = r0 + each;
   }
-  if (p0 < 0) return;
+  if (p0 < 0 || r1 <= r0) return;                          // (nothing to append: the block may be another's by now)
   constexpr float top = latent8_top<FMT>();
   const int64_t end = min((int64_t)p0 + (r1 - r0), (int64_t)INT32_MAX);
   int turn = 0;
@@ -67,7 +67,7 @@ __global__ void __launch_bounds__(APPEND_WARPS * 32) mla8_append_kernel(AppendAr
       const float4* src = reinterpret_cast<const float4*>(a.kv_pre + (size_t)(r0 + (start + i - p0)) * LATENT);
 #pragma unroll
       for (int j = 0; j < 4; j++) {
-        const float4 v = __ldg(src + j * 32 + lane);
+        const float4 v = src[j * 32 + lane];
         x[4 * j] = v.x; x[4 * j + 1] = v.y; x[4 * j + 2] = v.z; x[4 * j + 3] = v.w;
       }
     };
@@ -79,7 +79,7 @@ __global__ void __launch_bounds__(APPEND_WARPS * 32) mla8_append_kernel(AppendAr
     const int64_t b = a.pg.block_of(seq, (int)start);
     uint2 lw[4];
 #pragma unroll
-    for (int j = 0; j < 4; j++) lw[j] = __ldg(reinterpret_cast<const uint2*>(a.ln_w) + j * 32 + lane);
+    for (int j = 0; j < 4; j++) lw[j] = reinterpret_cast<const uint2*>(a.ln_w)[j * 32 + lane];
     auto weigh = [&](float (&x)[16]) {
 #pragma unroll
       for (int j = 0; j < 4; j++) {
@@ -178,8 +178,7 @@ cudaError_t append_launch(const AppendArgs& a, dim3 grid, cudaStream_t s) {
 // n_idx gathered positions of a sparse call, those without a block as -1.
 constexpr int READ_ROWS = 4, READ_IDX = 8;
 template <int FMT>
-__global__ void __launch_bounds__(256) mla8_read_kernel(MlaPaged pg, int head, int shift, int n, __half* __restrict__ out, const int* __restrict__ idx,
-                                                        int64_t n_idx, int* __restrict__ idx_out) {
+__global__ void __launch_bounds__(256) mla8_read_kernel(MlaPaged pg, int head, int shift, int n, __half* out, const int* idx, int64_t n_idx, int* idx_out) {
   pdl_release();
   pdl_wait();
   const int row_ctas = (n + 8 * READ_ROWS - 1) / (8 * READ_ROWS);
@@ -275,7 +274,7 @@ HK_API int hk_mla8_append(const float* kv_pre, const void* ln_w_f16, void* ckv8,
   // Blocks that a sequence's rows touch: as many CTAs where every sequence has n / n_seqs rows, else enough for the average, and for one
   // sequence with all of them as long as the grid stays within eight CTAs an SM (a CTA walks blocks gridDim.x apart).
   auto touched = [&](int rows) { return (int)(((int64_t)rows + block - 2) / block + 1); };
-  int blocks = touched((n + n_seqs - 1) / n_seqs);
+  int blocks = touched((n - 1) / n_seqs + 1);
   if (seq_start) {
     const int room = 8 * sm_count() / n_seqs, all = touched(n);
     blocks = blocks > (all < room ? all : room) ? blocks : (all < room ? all : room);

@@ -66,6 +66,7 @@ __device__ __forceinline__ F8Row f8_row(const MlaArgs& a, const MlaPaged& pg, in
   F8Row w;
   w.seq = pg.seq_of(r);
   w.keys = key_list(w.seq < 0 ? 0 : GATHER ? a.kidx : a.kv_len ? a.kv_len[r] : a.pos_start + r + 1, a.window, a.sinks);
+  if (!GATHER) w.keys.cut(pg.room());                      // behind the table are no keys
   w.head_tiles = (w.keys.head + F8_KEYS - 1) / F8_KEYS;
   w.jump = max(w.keys.lo / F8_KEYS - w.head_tiles, 0);
   w.tiles = w.keys.n / F8_KEYS + (w.keys.n % F8_KEYS != 0) - w.jump;
@@ -190,14 +191,21 @@ __device__ __forceinline__ void f8_to_f16(const uint4& v, uint4& lo, uint4& hi) 
   hi = make_uint4(h[4], h[5], h[6], h[7]);
 }
 
-__device__ __forceinline__ int f8_ld_int(const int* p) {   // issued where it stands
+// Loads that are issued where they stand.  Not the read-only path: what the kernel before this one writes (positions, scales, keys) is read
+// behind the wait for it, but within this kernel's lifetime.
+__device__ __forceinline__ int f8_ld_int(const int* p) {
   int v;
-  asm volatile("ld.global.nc.s32 %0, [%1];" : "=r"(v) : "l"(p));
+  asm volatile("ld.global.s32 %0, [%1];" : "=r"(v) : "l"(p));
   return v;
 }
 __device__ __forceinline__ float f8_ld_float(const float* p) {
   float v;
-  asm volatile("ld.global.nc.f32 %0, [%1];" : "=f"(v) : "l"(p));
+  asm volatile("ld.global.f32 %0, [%1];" : "=f"(v) : "l"(p));
+  return v;
+}
+__device__ __forceinline__ uint4 f8_ld_key(const void* p) {
+  uint4 v;
+  asm volatile("ld.global.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
   return v;
 }
 
@@ -275,7 +283,7 @@ __global__ __launch_bounds__(F8_THREADS, 1) void mla8_flash_tc_kernel(MlaArgs a,
     auto request = [&](uint4& v, int i, int row) {
       const int at = __shfl_sync(0xffffffffu, row, i);
       v = make_uint4(0u, 0u, 0u, 0u);
-      if (at >= 0) v = ld_stream16(src + (size_t)at * LATENT);
+      if (at >= 0) v = f8_ld_key(src + (size_t)at * LATENT);
     };
     // row of the cache, -1: none (rows of a cache are counted in 31 bits).  In a chunk a seen position without a block is a key of zeros.
     const bool zeros = !GATHER && !a.kv_len && !pg.row_seq;

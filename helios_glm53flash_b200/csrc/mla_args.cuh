@@ -46,6 +46,7 @@ struct MlaPaged {
     const int64_t phys = table ? table[(size_t)seq * table_stride + b] : b;
     return phys < n_blocks ? phys : -1;
   }
+  __device__ __forceinline__ int64_t room() const { return (table ? (int64_t)table_stride : n_blocks) << shift; }   // positions of a sequence
   __device__ __forceinline__ int seq_of(int r) const {
     const int s = row_seq ? row_seq[r] : 0;
     return s >= n_seqs ? -1 : s;
@@ -55,8 +56,13 @@ struct MlaPaged {
 // The keys that a row attends to, as a list: the first `head` positions, then lo .. n - 1.
 struct KeyList {
   int head, lo, n;
-  __device__ __forceinline__ int count() const { return head + n - lo; }
+  __device__ __forceinline__ int count() const { return n - lo + head; }
   __device__ __forceinline__ int at(int i) const { return i < head ? i : lo + i - head; }
+  __device__ __forceinline__ void cut(int64_t room) {      // there are `room` positions; what is seen of them goes by the row's own length
+    n = (int)(n < room ? n : room);
+    lo = lo < n ? lo : n;
+    head = head < n ? head : n;
+  }
 };
 __device__ __forceinline__ KeyList key_list(int n, int window, int sinks) {
   KeyList k;

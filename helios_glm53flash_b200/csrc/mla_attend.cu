@@ -237,7 +237,7 @@ struct GatherPlan {
 };
 static GatherPlan gather_plan(int m, int n_heads, int kidx, int64_t positions, bool per_row) {
   GatherPlan g{};
-  g.on = !per_row && n_heads == 64 && m >= GATHER_ROWS && (int64_t)m * kidx >= GATHER_TIMES * positions && !force_simt();
+  g.on = !per_row && n_heads == 64 && m >= GATHER_ROWS && (int64_t)m * kidx >= GATHER_TIMES * positions && positions <= INT32_MAX && !force_simt();
   g.rows = (size_t)positions * LATENT * sizeof(__half);
   g.bytes = align_up(g.rows + (size_t)m * kidx * sizeof(int), 256);
   return g;

@@ -55,6 +55,7 @@ __global__ __launch_bounds__(256) void mla_simt_kernel(MlaArgs a, MlaPaged pg) {
     base = a.kv_base ? a.kv_base[r] : 0;
     if (FMT == CACHE_F16 && a.ckv_rows > 0 && a.window <= 0) n = (int)max((int64_t)0, min((int64_t)n, a.ckv_rows - base));
     list = key_list(seq < 0 ? 0 : n, a.window, a.sinks);
+    if (FMT != CACHE_F16) list.cut(pg.room());
     n = list.count();
   }
   const int per = (n + a.n_split - 1) / a.n_split;

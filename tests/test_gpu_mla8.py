@@ -133,6 +133,47 @@ def test_append_edges(kind):
         assert math.isfinite(float(scales[0]))
 
 
+def test_append_of_no_rows_touches_nothing():
+    """a sequence of the batch without new rows, in the middle of a block"""
+    gen = gen_of(21)
+    ckv8, scales = cache(gen, "i8", 4, 16)
+    old, old_s = ckv8.clone(), scales.clone()
+    scales[1] = old_s[1] = math.nan
+    x, w = inputs(gen, 5)
+    hk.mla8_cache_append(x, w, ckv8, scales, ints([5, 3, 20]), 5, ref.EPS, block_table=ints([[0, 1], [2, 2], [3, 1]]), n_seqs=3, seq_start=ints([0, 0, 5, 5]))
+    finish()
+    keep = torch.tensor([0, 1, 3], device="cuda")
+    assert torch.equal(ckv8[keep], old[keep]) and torch.equal(scales[0], old_s[0]) and torch.equal(scales[3], old_s[3]) and math.isnan(float(scales[1]))
+    assert not torch.equal(ckv8[2], old[2])
+
+
+def test_tensors_that_are_not_on_the_device_are_refused():
+    ckv8, scales = cache(gen_of(1), "i8", 2, 16)
+    out = torch.zeros(1, 64, 512, dtype=torch.float16, device="cuda")
+    for c, s, t in ((ckv8.cpu(), scales, None), (ckv8, scales.cpu(), None), (ckv8, scales, torch.zeros(1, 2, dtype=torch.int32))):
+        with pytest.raises(ValueError):
+            hk.mla8_dense_prefill(out, c, s, out, 1, 0, block_table=t)
+
+
+def test_lengths_that_are_far_too_long_end_with_the_table():
+    """garbage in a padding row's length: as many keys as the table has places, a window behind them sees the sinks alone"""
+    gen = gen_of(22)
+    ckv8, scales = cache(gen, "i8", 6, 32)
+    table = table_for(gen, 2, 3, 6)
+    q = queries(gen, 3, 64)
+    out = torch.empty(3, 64, 512, dtype=torch.float16, device="cuda")
+    lens = [2 ** 31 - 1, 50, 2 ** 30]
+    for window, sinks, hint in ((0, 0, 100), (64, 7, 100), (64, 0, 1 << 20), (2 ** 31 - 1, 2 ** 31 - 1, 1 << 20)):
+        hk.mla8_dense_prefill(q, ckv8, scales, out, 3, 0, block_table=table, row_seq=ints([0, 1, 0]), kv_len=ints(lens), window=window, sinks=sinks, n_keys_hint=hint)
+        finish()
+        want = []
+        for r, n in enumerate(lens):
+            p = torch.arange(min(n, 96), device="cuda")
+            p = p[(p >= n - window) | (p < sinks)] if window else p
+            want.append(attend(q[r].double(), rows_of(ckv8, scales, table[[0, 1, 0][r]], p), 0.0625))
+        close(out, want)
+
+
 def test_read_of_holes_and_without_a_table():
     gen = gen_of(3)
     ckv8, scales = cache(gen, "i8", 4, 16)
@@ -477,6 +518,27 @@ def test_prefill_then_decode_of_three_sequences(kind):
             for k, p in enumerate((visible(n + 1, 0, 0), visible(n + 1, 20, 2), idx[s].long())):
                 o, tol = attend(q[s].double(), rows_of(ckv8, scales, table[s], p), 0.0625)
                 assert bool(((outs[k, s].double() - o).abs() <= tol).all())
+
+
+def test_two_streams_at_once():
+    """two sequences' steps side by side, workspaces and caches of their own"""
+    gen, block = gen_of(31), 64
+    sides = [torch.cuda.Stream() for _ in range(2)]
+    states = []
+    for _ in sides:
+        ckv8, scales = cache(gen, "i8", 40, block)
+        states.append((ckv8, scales, queries(gen, 1, 64), torch.empty(1, 64, 512, dtype=torch.float16, device="cuda"), torch.randn(300, 512, device="cuda", generator=gen).half()))
+    torch.cuda.synchronize()
+    for _ in range(5):
+        for stream, (ckv8, scales, q, out, ckv) in zip(sides, states):
+            with torch.cuda.stream(stream):
+                hk.mla8_dense_prefill(q, ckv8, scales, out, 1, 2499)
+                hk.mla_window_prefill(q, ckv, out[:], 1, 299, 100, sinks=3)
+                hk.mla8_dense_prefill(q, ckv8, scales, out, 1, 2499)
+    finish()
+    ident = torch.arange(40, device="cuda", dtype=torch.int32)
+    for ckv8, scales, q, out, ckv in states:
+        close(out, [attend(q[0].double(), rows_of(ckv8, scales, ident, visible(2500, 0, 0)), 0.0625)])
 
 
 def test_captured_decode_step_replayed():
