@@ -40,7 +40,8 @@ constexpr uint32_t F8_SMEM = F8S_MISC + 2048 + 1024;             // + slack to a
 constexpr uint32_t F8_O = 0, F8_S = 256, F8_Q = 320;             // tensor-memory columns: O 2 x 128, S 2 x 32, Q 192
 constexpr int F8_POLL_NS = 40;
 constexpr int F8_CONV_WARPS = 8, F8_ROWS = F8_KEYS / F8_CONV_WARPS, F8_THREADS = (6 + F8_CONV_WARPS) * 32;
-constexpr int F8_SHARE_ROWS = 160, F8_MIN_TILES = 2;   // rows whose splits are shared out on the device; tiles that a split is worth
+constexpr int F8_SHARE_ROWS = 32, F8_SHARE_SPLITS = 160;   // rows whose splits are shared out on the device, and splits of one row then at most
+constexpr int F8_MIN_TILES = 2;                   // tiles that a split is worth
 constexpr float F8_LOG2E = 1.4426950408889634f;
 constexpr float F8_MOVE = 8.0f, F8_MOVE_SCALE = 16.0f;
 
@@ -74,75 +75,48 @@ __device__ __forceinline__ F8Row f8_row(const MlaArgs& a, const MlaPaged& pg, in
 }
 struct F8Item {
   int r, hg, sp, n_sp, first;                     // row, 64 heads, split of how many, unit of split 0 (shared out splits); r < 0: nothing to do
+  int part;                                       // part of the output channels
   F8Row row;
   int t0, n_tiles;
   __device__ __forceinline__ int tile(int i) const { return t0 + i < row.head_tiles ? t0 + i : t0 + i + row.jump; }
 };
 
-// Splits shared out on the device, where alone the lengths are known: `units` CTAs (of 64 heads) for m <= units rows.  Every split has at most
-// `per` tiles, the smallest number found with which all rows' splits fit; a row has one at least.  Executed by a whole warp.
+// Splits shared out on the device, where alone the lengths are known: `units` CTAs (of 64 heads) for m <= 32 rows, one a lane.  Every split has at
+// most `per` tiles, the smallest number found with which all rows' splits fit; a row has one at least.  Executed by a whole warp.
 __device__ __forceinline__ void f8_share(const MlaArgs& a, const MlaPaged& pg, int unit, int units, F8Item& it, int& per) {
-  const int lane = threadIdx.x & 31, each = (a.m + 31) / 32;
-  int t[F8_SHARE_ROWS / 32], sum = 0;
-#pragma unroll
-  for (int k = 0; k < F8_SHARE_ROWS / 32; k++) {
-    const int r = lane * each + k;
-    t[k] = -1;
-    if (k < each && r < a.m) sum += t[k] = f8_row<false>(a, pg, r).tiles;
-  }
-  sum = __reduce_add_sync(0xffffffffu, sum);
-  float inv;
-  auto splits = [&](int tiles) {                           // ceil(tiles / per): the quotient in fp32 may be one too small
-    int n = (int)((float)tiles * inv);
-    n += n * per < tiles;
-    n += n * per < tiles;
-    return max(n, 1);
-  };
-  per = max((sum + units - 1) / units, F8_MIN_TILES);
+  const int lane = threadIdx.x & 31;
+  const int t = lane < a.m ? f8_row<false>(a, pg, lane).tiles : 0;
+  per = max(((int)__reduce_add_sync(0xffffffffu, t) + units - 1) / units, F8_MIN_TILES);
   int mine;
   for (int tries = 0;; tries++) {
-    mine = 0;
-    inv = 1.f / (float)per;
-#pragma unroll
-    for (int k = 0; k < F8_SHARE_ROWS / 32; k++)
-      if (k < each && t[k] >= 0) mine += splits(t[k]);
+    mine = (int)__fdividef((float)t, (float)per);          // ceil(t / per): the quotient in fp32 may be one too small
+    mine += mine * per < t;
+    mine += mine * per < t;
+    mine = lane < a.m ? max(mine, 1) : 0;
     if ((int)__reduce_add_sync(0xffffffffu, mine) <= units) break;
     per += tries < 4 ? 1 : per / 4;                        // (rows of very different lengths; ends where every row has one split)
   }
-  int before = mine;                                       // splits of the lanes up to this one
+  int behind = mine;                                       // splits of the rows up to and with this one
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const int x = __shfl_up_sync(0xffffffffu, before, o);
-    if (lane >= o) before += x;
+    const int x = __shfl_up_sync(0xffffffffu, behind, o);
+    if (lane >= o) behind += x;
   }
-  before -= mine;
-  int row = -1, first = 0, n_sp = 0;
-#pragma unroll
-  for (int k = 0; k < F8_SHARE_ROWS / 32; k++) {
-    if (k >= each || t[k] < 0) break;
-    const int n = splits(t[k]);
-    if (unit >= before && unit < before + n) {
-      row = lane * each + k;
-      first = before;
-      n_sp = n;
-    }
-    before += n;
-  }
-  const uint32_t who = __ballot_sync(0xffffffffu, row >= 0);
-  const int from = max(__ffs(who) - 1, 0);
-  it.r = __shfl_sync(0xffffffffu, row, from);
-  it.first = __shfl_sync(0xffffffffu, first, from);
-  it.n_sp = __shfl_sync(0xffffffffu, n_sp, from);
+  const uint32_t who = __ballot_sync(0xffffffffu, unit < behind && unit >= behind - mine);
+  it.r = __ffs(who) - 1;                                   // (-1: more CTAs than splits)
+  it.n_sp = __shfl_sync(0xffffffffu, mine, max(it.r, 0));
+  it.first = __shfl_sync(0xffffffffu, behind, max(it.r, 0)) - it.n_sp;
   it.sp = unit - it.first;
 }
 
-template <bool GATHER>
+template <bool GATHER, int PARTS>
 __device__ __forceinline__ F8Item f8_item(const MlaArgs& a, const MlaPaged& pg, int idx) {
   F8Item it;
   const int groups = (a.n_heads + F8_HEADS - 1) / F8_HEADS;
   int per;
-  if (!GATHER && a.n_split == 0) {
+  if (!GATHER && PARTS == 1 && a.n_split == 0) {
     it.hg = idx % groups;
+    it.part = 0;
     f8_share(a, pg, idx / groups, gridDim.x / groups, it, per);
     if (it.r < 0) {
       it.n_tiles = it.t0 = 0;
@@ -150,6 +124,8 @@ __device__ __forceinline__ F8Item f8_item(const MlaArgs& a, const MlaPaged& pg, 
     }
     it.row = f8_row<GATHER>(a, pg, it.r);
   } else {
+    it.part = idx % PARTS;
+    idx /= PARTS;
     it.n_sp = a.n_split;
     it.first = 0;
     it.sp = idx % a.n_split;
@@ -218,7 +194,8 @@ __device__ __forceinline__ void f8_tma_box(void* smem_dst, const CUtensorMap* tm
       : "memory");
 }
 
-template <bool GATHER, int FMT>
+// PARTS: CTAs that share a split's output channels
+template <bool GATHER, int FMT, int PARTS>
 __global__ __launch_bounds__(F8_THREADS, 1) void mla8_flash_tc_kernel(MlaArgs a, MlaPaged pg, int* __restrict__ status,
                                                                               const __grid_constant__ CUtensorMap tmap_q) {
   extern __shared__ __align__(1024) uint8_t smem_raw[];
@@ -247,7 +224,7 @@ __global__ __launch_bounds__(F8_THREADS, 1) void mla8_flash_tc_kernel(MlaArgs a,
   }
   if (warp == 0) tc::tmem_alloc(&ms.tmem, 512);
   pdl_wait();
-  const F8Item it = f8_item<GATHER>(a, pg, blockIdx.x);
+  const F8Item it = f8_item<GATHER, PARTS>(a, pg, blockIdx.x);
   tc::fence_before_sync();
   __syncthreads();
   tc::fence_after_sync();
@@ -255,7 +232,7 @@ __global__ __launch_bounds__(F8_THREADS, 1) void mla8_flash_tc_kernel(MlaArgs a,
   // An item of at most two tiles (a decode split) does not need the last tile slot back: S reads Q from there, and moving it is saved.
   const bool direct_q = it.n_tiles < F8_NBUF;
   // Final rows, or a partial: with a number of splits [split][row, head], shared out [CTA][64 heads].
-  const bool final_out = it.n_sp == 1;
+  const bool final_out = PARTS == 1 && it.n_sp == 1;
   const size_t part_row = a.n_split == 0 ? (size_t)blockIdx.x * F8_HEADS : ((size_t)it.sp * a.m + it.r) * a.n_heads + it.hg * F8_HEADS;
   if (a.n_split == 0 && it.r >= 0 && it.sp == 0 && it.hg == 0 && tid == 0) a.shares[it.r] = make_int2(it.first, it.n_sp);
   const int n_tiles = it.n_tiles, h0 = it.hg * F8_HEADS, n_h = min(F8_HEADS, a.n_heads - h0);
@@ -382,14 +359,15 @@ __global__ __launch_bounds__(F8_THREADS, 1) void mla8_flash_tc_kernel(MlaArgs a,
         f8_tma_box(smem + F8S_K + (F8_NBUF - 1) * F8_TILE, &tmap_q, it.r * a.n_heads + h0, &ms.q_full);
       }
       __syncwarp();
-      const uint32_t idesc = tc::make_idesc(64, 256, tc::FMT_F16, tc::FMT_F16, false, true);
+      // all 512 channels as two products of 256, or this CTA's 256 or 128
+      const uint32_t idesc = tc::make_idesc(64, PARTS == 4 ? 128 : 256, tc::FMT_F16, tc::FMT_F16, false, true), v_part = it.part * (8 / PARTS) * F8_BLK;
       for (int t = 0; t < n_tiles; t++) {
         const int b = t & 1, kb = t % F8_NBUF;
         wait_u(&ms.p_full[b], (t >> 1) & 1, 46);
         tc::fence_after_sync();
-        const uint64_t pd = desc(smem + F8S_P + b * F8_P_BYTES, 16), vd = desc(smem + F8S_K + kb * F8_TILE, F8_BLK);
+        const uint64_t pd = desc(smem + F8S_P + b * F8_P_BYTES, 16), vd = desc(smem + F8S_K + kb * F8_TILE + v_part, F8_BLK);
 #pragma unroll
-        for (int nh = 0; nh < 2; nh++)
+        for (int nh = 0; nh < (PARTS == 1 ? 2 : 1); nh++)
 #pragma unroll
           for (int kk = 0; kk < F8_KEYS / 16; kk++)
             tc::mma_ws_f16_if(leader, tmem + F8_O + nh * 128, tc::sdesc_advance(pd, kk * 32), tc::sdesc_advance(vd, nh * 4 * F8_BLK + kk * 2048), idesc,
@@ -484,7 +462,7 @@ __global__ __launch_bounds__(F8_THREADS, 1) void mla8_flash_tc_kernel(MlaArgs a,
         wait_pv(t - 1, 49);
         tc::fence_after_sync();
 #pragma unroll 1
-        for (int c = 0; c < 256; c += 32) {
+        for (int c = 0; c < 256 / PARTS; c += 32) {
           uint32_t o[32];
           tc::tmem_ld32(tmem + F8_O + c + lanes, o);
           tc::tmem_ld_wait();
@@ -534,7 +512,7 @@ __global__ __launch_bounds__(F8_THREADS, 1) void mla8_flash_tc_kernel(MlaArgs a,
     const bool none = l == 0.f;                            // (NaN: a score was none)
     if (half == 0) {
       ms.mx[(n_tiles + 1) & 1][head] = none ? 0.f : final_out ? sref / l : sref;
-      if (!final_out && it.r >= 0 && head < n_h) {
+      if (!final_out && it.r >= 0 && it.part == 0 && head < n_h) {
         const size_t at = part_row + head;
         a.part_m[at] = m == -INFINITY || none ? -INFINITY : m / F8_LOG2E;
         a.part_l[at] = l;
@@ -548,10 +526,11 @@ __global__ __launch_bounds__(F8_THREADS, 1) void mla8_flash_tc_kernel(MlaArgs a,
     asm volatile("bar.sync 4, 384;" ::: "memory");         // factors, and every product is complete
     tc::fence_after_sync();
     const int quarter = warp & 3, head = (quarter & 1) * 32 + lane, half = quarter >> 1, member = warp < 4 ? 0 : warp < 10 ? 1 : 2;
-    const uint32_t elem = final_out ? 2 : 4, pitch = LATENT * elem + 16;
+    constexpr int n_ch = LATENT / PARTS, pieces = 8 / PARTS;
+    const uint32_t elem = final_out ? 2 : 4, pitch = n_ch * elem + 16;
     const float f = ms.mx[(n_tiles + 1) & 1][head];
     uint8_t* orow = smem + F8S_K + head * pitch;
-    for (int c = 32 * (3 * member - (member > 0)); c < 32 * (3 * member + 2); c += 32) {
+    for (int c = pieces * member / 3 * 32; c < pieces * (member + 1) / 3 * 32; c += 32) {
       uint32_t o[32];
       if (n_tiles > 0) {
         tc::tmem_ld32(tmem + F8_O + c + ((uint32_t)(quarter * 32) << 16), o);
@@ -559,7 +538,8 @@ __global__ __launch_bounds__(F8_THREADS, 1) void mla8_flash_tc_kernel(MlaArgs a,
       }
 #pragma unroll
       for (int j = 0; j < 32; j++) o[j] = f == 0.f ? 0u : __float_as_uint(__uint_as_float(o[j]) * f);
-      uint8_t* dst = orow + ((c >> 7) * 256 + half * 128 + (c & 127)) * elem;
+      constexpr int span = PARTS == 4 ? 64 : 128;            // columns of a product: channels 2 span a product, span a lane half
+      uint8_t* dst = orow + (c / span * 2 * span + half * span + c % span) * elem;
       if (final_out) {
 #pragma unroll
         for (int v = 0; v < 4; v++) {
@@ -580,12 +560,12 @@ __global__ __launch_bounds__(F8_THREADS, 1) void mla8_flash_tc_kernel(MlaArgs a,
     asm volatile("bar.sync 4, 384;" ::: "memory");
     if (!*abort_flag) {
       uint8_t* dst = final_out ? reinterpret_cast<uint8_t*>(a.out + ((size_t)it.r * a.n_heads + h0) * LATENT)
-                               : reinterpret_cast<uint8_t*>(a.part_acc + part_row * LATENT);
+                               : reinterpret_cast<uint8_t*>(a.part_acc + part_row * LATENT + it.part * n_ch);
       const int team = warp < 4 ? warp : warp - 2;
-      const int per = final_out ? 2 : 4;                       // 512-byte pieces of a head
+      const int per = n_ch * elem / 512;                   // 512-byte pieces of a head
 #pragma unroll 8
       for (int i = team; i < n_h * per; i += 12) {
-        const int h = final_out ? i >> 1 : i >> 2, c = (final_out ? i & 1 : i & 3) * 512 + lane * 16;
+        const int h = i / per, c = i % per * 512 + lane * 16;
         *reinterpret_cast<uint4*>(dst + (size_t)h * LATENT * elem + c) = *reinterpret_cast<const uint4*>(smem + F8S_K + h * pitch + c);
       }
     }
@@ -596,31 +576,36 @@ __global__ __launch_bounds__(F8_THREADS, 1) void mla8_flash_tc_kernel(MlaArgs a,
   if (tid == 0 && ms.abort_flag && status) atomicExch(status, HK_ERR_TIMEOUT);
 }
 
-template <bool GATHER, int FMT>
+template <bool GATHER, int FMT, int PARTS>
 int f8_launch(const MlaArgs& a, const MlaPaged& pg, const CUtensorMap& q, cudaStream_t s) {
   static bool attr_set[64] = {false};
   const int dev = device_index();
   if (!attr_set[dev]) {
-    if (cudaFuncSetAttribute(mla8_flash_tc_kernel<GATHER, FMT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)F8_SMEM) != cudaSuccess)
+    if (cudaFuncSetAttribute(mla8_flash_tc_kernel<GATHER, FMT, PARTS>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)F8_SMEM) != cudaSuccess)
       return HK_ERR_CUDA;
     attr_set[dev] = true;
   }
   const int groups = (a.n_heads + F8_HEADS - 1) / F8_HEADS;
-  const int64_t items = (a.n_split == 0 ? (int64_t)a.units : (int64_t)a.n_split * a.m) * groups;
+  const int64_t items = (a.n_split == 0 ? (int64_t)a.units : (int64_t)a.n_split * a.m * PARTS) * groups;
   if (items > INT32_MAX) return HK_ERR_UNSUPPORTED;
-  const cudaError_t e = pdl_launch(mla8_flash_tc_kernel<GATHER, FMT>, dim3((unsigned)items), dim3(F8_THREADS), F8_SMEM, s, a, pg, device_status_ptr(), q);
+  const cudaError_t e = pdl_launch(mla8_flash_tc_kernel<GATHER, FMT, PARTS>, dim3((unsigned)items), dim3(F8_THREADS), F8_SMEM, s, a, pg, device_status_ptr(), q);
   return e == cudaSuccess && cudaPeekAtLastError() == cudaSuccess ? HK_OK : HK_ERR_CUDA;
+}
+
+template <bool GATHER, int FMT>
+int f8_launch_parts(int parts, const MlaArgs& a, const MlaPaged& pg, const CUtensorMap& q, cudaStream_t s) {
+  return parts == 1 ? f8_launch<GATHER, FMT, 1>(a, pg, q, s) : parts == 2 ? f8_launch<GATHER, FMT, 2>(a, pg, q, s) : f8_launch<GATHER, FMT, 4>(a, pg, q, s);
 }
 
 // Merge of the splits that the attention kernel shared out: one CTA a (row, head), a thread four channels.  Rows of one split are finished.
 __global__ __launch_bounds__(128) void mla8_merge_kernel(MlaArgs a) {
-  __shared__ float s_w[F8_SHARE_ROWS];                     // (a row has no more splits than there are CTAs)
+  __shared__ float s_w[F8_SHARE_SPLITS];                     // (a row has no more splits than there are CTAs)
   pdl_release();
   pdl_wait();
   const int r = blockIdx.x / a.n_heads, h = blockIdx.x % a.n_heads, lane = threadIdx.x & 31;
   const size_t stride = (size_t)((a.n_heads + F8_HEADS - 1) / F8_HEADS) * F8_HEADS;
   const int2 share = __ldcg(a.shares + r);
-  const int n = min(share.y, F8_SHARE_ROWS);
+  const int n = min(share.y, F8_SHARE_SPLITS);
   if (n <= 1) return;
   const size_t row0 = (size_t)share.x * stride + h;
   const float4* acc = reinterpret_cast<const float4*>(a.part_acc + row0 * LATENT) + threadIdx.x;
@@ -633,9 +618,9 @@ __global__ __launch_bounds__(128) void mla8_merge_kernel(MlaArgs a) {
   };
   load(0);
   // every warp for itself; split s in lane s % 32, the weights of all in shared memory
-  float m[F8_SHARE_ROWS / 32], l[F8_SHARE_ROWS / 32], gm = -INFINITY, gl = 0.f;
+  float m[F8_SHARE_SPLITS / 32], l[F8_SHARE_SPLITS / 32], gm = -INFINITY, gl = 0.f;
 #pragma unroll
-  for (int k = 0; k < F8_SHARE_ROWS / 32; k++) {
+  for (int k = 0; k < F8_SHARE_SPLITS / 32; k++) {
     const int s = lane + 32 * k;
     m[k] = s < n ? __ldcg(a.part_m + row0 + s * stride) : -INFINITY;
     l[k] = s < n ? __ldcg(a.part_l + row0 + s * stride) : 0.f;
@@ -644,7 +629,7 @@ __global__ __launch_bounds__(128) void mla8_merge_kernel(MlaArgs a) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) gm = fmaxf(gm, __shfl_xor_sync(0xffffffffu, gm, o));
 #pragma unroll
-  for (int k = 0; k < F8_SHARE_ROWS / 32; k++) {
+  for (int k = 0; k < F8_SHARE_SPLITS / 32; k++) {
     const float w = m[k] == -INFINITY ? 0.f : __expf(m[k] - gm);
     gl = fmaf(w, l[k], gl);
     if (threadIdx.x < 32) s_w[lane + 32 * k] = w;
@@ -672,14 +657,37 @@ __global__ __launch_bounds__(128) void mla8_merge_kernel(MlaArgs a) {
 // implemented in mla_flash_tc.cu
 bool mla_rows_map(CUtensorMap* m, const void* rows, int64_t n);
 
-// CTAs (of 64 heads) among which the splits of m rows of up to n_keys keys are shared out; 0: every row gets as many splits.  Sharing costs
-// 2.3 us (lengths, splits and where a row's lie are found out on the device), so it is for rows where equal numbers would mean 8 tiles a
-// split or more: 8 rows of 17,000 to 32,768 keys 55.3 -> 51.2 us (29 -> 23 tiles the longest), 48 rows of 17 tiles 20.8 -> 23.5.
+// CTAs (of 64 heads) among which the splits of m rows of up to n_keys keys are shared out; 0: every row gets as many splits.  Sharing costs a
+// microsecond where the rows are equally long (16 rows of 6,000 keys 27.9 us, nine splits each 26.9), and more with more rows, so it is for up to
+// 32 rows where equal numbers would mean 8 tiles a split or more: 8 rows of 17,000 to 32,768 keys 55.3 -> 51.2 us (29 -> 23 tiles the longest).
 int mla8_units(int m, int n_heads, int n_keys) {
-  const int groups = (n_heads + F8_HEADS - 1) / F8_HEADS, units = sm_count() / groups;
+  const int groups = (n_heads + F8_HEADS - 1) / F8_HEADS, units = min(sm_count() / groups, F8_SHARE_SPLITS);
   if (m < 2 || m > units || m > F8_SHARE_ROWS) return 0;
   const int64_t tiles = ((int64_t)n_keys + F8_KEYS - 1) / F8_KEYS, each = units / m;
   return (tiles + each - 1) / each >= 8 ? units : 0;
+}
+
+// CTAs that share a split's output channels, for `ctas` splits of rows in all
+static int f8_parts(int64_t ctas) { return 4 * ctas <= sm_count() ? 4 : 2 * ctas <= sm_count() ? 2 : 1; }
+
+// Splits of each of `rows` rows of n_keys keys, at most a CTA per SM, equal numbers of tiles.  A tile takes 1.3 us, a partial written by one or two
+// CTAs instead of four (and merged with as many others) 5.5 and 2 us more.  One row, us, splits (CTAs each): 5,001 keys 27 (4) 11.1, 40 (2) 11.7, 79 (1) 13.3; 8,192 keys 32 (4) 12.2,
+// 64 (2) 11.6, 128 (1) 13.6; 12,000 63 (2) 12.7, 94 (1) 14.4; 2,052 gathered rows 11 (4) 10.3, 17 (4) 9.4, 33 (4) 9.2, of four rows 9 (4) 11.7, 17 (2) 11.2, 33 (1) 14.5.
+int mla8_splits(int rows, int n_keys) {
+  const int tiles = n_keys / F8_KEYS + (n_keys % F8_KEYS != 0);
+  if (tiles <= F8_MIN_TILES) return 1;
+  int best = 1, least = 13 * tiles;                        // (one split: no merge, which takes about as long as writing the partial)
+  for (int parts = 4; parts >= 1; parts /= 2) {
+    const int room = sm_count() / (parts * rows);
+    if (room < 2) continue;
+    const int even = (tiles + room - 1) / room, per = parts == 4 || even > F8_MIN_TILES ? even : F8_MIN_TILES;
+    const int n = (tiles + per - 1) / per, time = 13 * per + (parts == 4 ? 0 : parts == 2 ? 20 : 55);
+    if (n > 1 && time < least) {
+      best = n;
+      least = time;
+    }
+  }
+  return best;
 }
 
 size_t mla8_units_bytes(int units, int m, int n_heads, MlaArgs* a, void* workspace) {
@@ -698,8 +706,12 @@ size_t mla8_units_bytes(int units, int m, int n_heads, MlaArgs* a, void* workspa
 int mla8_flash_tc_launch(const MlaArgs& a, const MlaPaged& pg, int dtype, cudaStream_t s) {
   alignas(64) CUtensorMap q;
   if (!mla_rows_map(&q, a.q_lat, (int64_t)a.m * a.n_heads)) return HK_ERR_UNSUPPORTED;
-  const int st = a.raw_idx ? (dtype == HK_I8 ? f8_launch<true, CACHE_I8>(a, pg, q, s) : f8_launch<true, CACHE_E4M3>(a, pg, q, s))
-                           : (dtype == HK_I8 ? f8_launch<false, CACHE_I8>(a, pg, q, s) : f8_launch<false, CACHE_E4M3>(a, pg, q, s));
+  // Few splits of few rows: the output channels of each are shared out over two or four CTAs, which compute the scores each for itself and write
+  // a half or a quarter of the partial (of 128 KB, which take 2.1 us).  2,052 gathered rows 11.1 -> 9.1 us (four), 5,001 keys 11.1 -> 10.4 (two).
+  const int64_t ctas = (int64_t)a.n_split * a.m * ((a.n_heads + F8_HEADS - 1) / F8_HEADS);
+  const int parts = a.n_split < 2 ? 1 : f8_parts(ctas);
+  const int st = a.raw_idx ? (dtype == HK_I8 ? f8_launch_parts<true, CACHE_I8>(parts, a, pg, q, s) : f8_launch_parts<true, CACHE_E4M3>(parts, a, pg, q, s))
+                           : (dtype == HK_I8 ? f8_launch_parts<false, CACHE_I8>(parts, a, pg, q, s) : f8_launch_parts<false, CACHE_E4M3>(parts, a, pg, q, s));
   if (st != HK_OK || a.n_split > 0) return st;
   const cudaError_t e = pdl_launch(mla8_merge_kernel, dim3((unsigned)(a.m * a.n_heads)), dim3(128), 0, s, a);
   return e == cudaSuccess ? HK_OK : HK_ERR_CUDA;

@@ -17,6 +17,7 @@ int mla_flash_tc_auto_splits(int m, int n_keys);
 // implemented in mla8_flash_tc.cu
 int mla8_flash_tc_launch(const MlaArgs& a, const MlaPaged& pg, int dtype, cudaStream_t s);
 int mla8_units(int m, int n_heads, int n_keys);
+int mla8_splits(int rows, int n_keys);
 size_t mla8_units_bytes(int units, int m, int n_heads, MlaArgs* a, void* workspace);
 // implemented in mla8_cache.cu
 int mla8_read_launch(const MlaPaged& pg, int dtype, int head, int shift, int n, __half* out, cudaStream_t s, const int* idx = nullptr, int64_t n_idx = 0,
@@ -157,7 +158,7 @@ static int attend8_splits(int m, int n_heads, int n_keys, bool dense, int* units
   *units = dense && !force_simt() ? mla8_units(m, n_heads, n_keys) : 0;
   if (force_simt()) return simt_auto_splits(m, n_heads, n_keys);
   const int64_t rows = (int64_t)m * ((n_heads + 63) / 64);  // every 64 heads of a row are work of their own
-  return mla_flash_tc_auto_splits(rows > INT32_MAX ? INT32_MAX : (int)rows, n_keys);
+  return rows > sm_count() ? 1 : mla8_splits((int)rows, n_keys);
 }
 static size_t attend8_bytes(int m, int n_heads, int n_split, int units) {
   return units > 0 ? mla8_units_bytes(units, m, n_heads, nullptr, nullptr) : n_split > 1 ? partial_layout(n_split, (int64_t)m * n_heads).total : 0;
