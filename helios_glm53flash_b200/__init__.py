@@ -192,6 +192,11 @@ def _scratch(nbytes, device, stream=None):
     return ws
 
 
+def _scratch_like(nbytes, tensor, stream):
+    """_scratch on a tensor's device, through the binding"""
+    return _native.scratch(nbytes, tensor) if stream is None else _scratch(nbytes, tensor.device, stream)
+
+
 # ---------------------------------------------------------------------------------------------
 # helios::aux
 # ---------------------------------------------------------------------------------------------
@@ -452,7 +457,7 @@ def mla_window_prefill(q_lat, ckv, lat_out, qlen, pos_start, window, sinks=0, st
         splits = _native.hk_mla_auto_splits(qlen, 64 * (min(tiles, -(-n // 64)) if n else tiles))
     ws = workspace
     if splits > 1 and ws is None:
-        ws = _scratch(mla_partial_bytes(splits, qlen * n_heads), q_lat.device, stream)
+        ws = _scratch_like(_native.hk_mla_partial_bytes(splits, qlen * n_heads), q_lat, stream)
     _run("hk_mla_window", q_lat, ckv, ckv if ckv_rows is None else ckv_rows, kv_base, kv_len, pos_start, window, sinks, lat_out, qlen,
          n_heads, scale, n_split if n_heads == 64 else splits, ws, ws, stream)
 
@@ -496,7 +501,7 @@ def mla8_dense_prefill(q_lat, ckv8, scales, lat_out, qlen, pos_start, stream=Non
         need = (_native.hk_mla8_dense_workspace_bytes(qlen, n_heads, pos_start, hint, window, sinks, 1 if kv_len is not None or row_seq is not None else 0)
                 if n_split <= 0 else _native.hk_mla_partial_bytes(n_split, qlen * n_heads) if n_split > 1 else 0)
         if need:
-            ws = _scratch(need, q_lat.device, stream)
+            ws = _scratch_like(need, q_lat, stream)
     _run("hk_mla8_dense", q_lat, ckv8, scales, tag, n_blocks, block, block_table, stride, seqs, row_seq, kv_len, pos_start, window, sinks, lat_out,
          qlen, n_heads, scale, n_split, hint, ws, ws, stream)
 
@@ -511,7 +516,7 @@ def mla8_sparse_decode(q_lat, ckv8, scales, raw_idx, kidx, lat_out, m, stream=No
         need = (_native.hk_mla8_sparse_workspace_bytes(m, n_heads, kidx, positions, 0 if row_seq is None else 1) if n_split <= 0
                 else _native.hk_mla_partial_bytes(n_split, m * n_heads) if n_split > 1 else 0)
         if need:
-            ws = _scratch(need, q_lat.device, stream)
+            ws = _scratch_like(need, q_lat, stream)
     _run("hk_mla8_sparse", q_lat, ckv8, scales, tag, n_blocks, block, block_table, stride, seqs, row_seq, raw_idx, kidx, lat_out, m, n_heads, scale,
          n_split, ws, ws, stream)
 

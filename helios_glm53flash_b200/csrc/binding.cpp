@@ -17,6 +17,7 @@
 // the Python layer loaded (bind), so that both sides drive the same build.
 #define PY_SSIZE_T_CLEAN
 #include <Python.h>
+#include <ATen/ops/empty.h>
 #include <c10/cuda/CUDAFunctions.h>
 #include <c10/cuda/CUDAStream.h>
 #include <c10/util/Exception.h>
@@ -241,8 +242,25 @@ PyObject* py_cache8(PyObject*, PyObject* const* args, Py_ssize_t n) {
   }
 }
 
+// scratch(nbytes, tensor) -> a byte tensor of torch's allocator on the tensor's device (torch.empty from Python costs twice the time)
+PyObject* py_scratch(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  long long bytes;
+  if (n != 2 || !THPVariable_Check(args[1])) {
+    bad_arg("scratch: a size and a tensor");
+    return nullptr;
+  }
+  if (!number(args[0], bytes)) return nullptr;
+  try {
+    return THPVariable_Wrap(at::empty({bytes < 256 ? 256 : bytes}, THPVariable_Unpack(args[1]).options().dtype(at::kByte).requires_grad(false)));
+  } catch (const std::exception& e) {          // out of memory among them
+    PyErr_SetString(PyExc_RuntimeError, e.what());
+    return nullptr;
+  }
+}
+
 #define X(name, stream) {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(py_##name)), METH_FASTCALL, nullptr},
 PyMethodDef methods[] = {HK_ENTRIES(X){"cache8", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(py_cache8)), METH_FASTCALL, nullptr},
+                         {"scratch", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(py_scratch)), METH_FASTCALL, nullptr},
                          {"bind", py_bind, METH_O, nullptr}, {nullptr, nullptr, 0, nullptr}};
 #undef X
 
