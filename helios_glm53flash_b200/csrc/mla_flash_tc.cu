@@ -200,7 +200,8 @@ __device__ __forceinline__ void tma_gather4_rows(uint32_t leader, uint32_t smem_
 // P V 3,800, laying out and the barrier of the cluster 1,700, the shares 2,200, the merge 1,600.  2,052 gathered rows of one query 10.8 ->
 // 9.2 us; MLA layer of one token at 5,001 32.1 -> 28.9, selection and attention at 262,144 23.8 -> 21.8.
 // WIN: dense ranges of which a row sees its last keys and its first ones only (a.window, a.sinks).
-template <bool G4, bool CL, bool WIN>
+// PARTS: CTAs that share a partial's output channels, each with the scores for itself (few splits of few rows: 128 KB of a partial take 3 us).
+template <bool G4, bool CL, bool WIN, int PARTS = 1>
 __global__ __launch_bounds__(FT_THREADS, 1) void mla_flash_tc_kernel(
     MlaArgs a, int* __restrict__ status, const __grid_constant__ CUtensorMap tmap_box, const __grid_constant__ CUtensorMap tmap_rows,
     const __grid_constant__ CUtensorMap tmap_q, const __grid_constant__ CUtensorMap tmap_o) {
@@ -208,11 +209,12 @@ __global__ __launch_bounds__(FT_THREADS, 1) void mla_flash_tc_kernel(
   uint8_t* smem = smem_raw + ((1024u - (tc::smem_u32(smem_raw) & 1023u)) & 1023u);
   FtMisc& ms = *reinterpret_cast<FtMisc*>(smem + FS_MISC);
   volatile int* abort_flag = &ms.abort_flag;
+  const int part = PARTS > 1 ? blockIdx.x % PARTS : 0;     // (a CTA has one item then)
 
   const int tid = threadIdx.x, lane = tid & 31;
   // provably warp-uniform role index: the issuing warps' branches stay converged for the compiler
   const int warp = tc::warp_index_uniform();
-  const int n_items = CL ? gridDim.x : a.n_split * a.m, step = gridDim.x;
+  const int n_items = CL ? gridDim.x : PARTS * a.n_split * a.m, step = gridDim.x;
   // A CTA with one item of at most two tiles (a decode split) never needs Q's ring slot back: S reads Q from there, and the
   // 0.6 us of moving it are saved.  In the cluster form Q always stays and the other two slots serve all tiles.
   bool direct_q = CL;
@@ -238,7 +240,7 @@ __global__ __launch_bounds__(FT_THREADS, 1) void mla_flash_tc_kernel(
   }
   if (warp == 0) tc::tmem_alloc(&ms.tmem, 512);
   pdl_wait();
-  if (!CL && step >= n_items) direct_q = ft_item<G4, CL, WIN>(a, blockIdx.x).n_tiles < FT_NBUF;
+  if (!CL && step >= n_items) direct_q = ft_item<G4, CL, WIN>(a, blockIdx.x / PARTS).n_tiles < FT_NBUF;
   tc::fence_before_sync();
   __syncthreads();
   tc::fence_after_sync();
@@ -269,14 +271,14 @@ __global__ __launch_bounds__(FT_THREADS, 1) void mla_flash_tc_kernel(
     auto in_cache = [&](int v) -> int { return (v < 0 || (a.ckv_rows > 0 && (int64_t)v >= a.ckv_rows)) ? -1 : v; };
     // Gathered row numbers are fetched two tiles ahead (the row list of a query is read once, from HBM), across rows.
     int cur = -1, nxt = -1, ahead_item = blockIdx.x, ahead_tile = 0;
-    FtItem ahead = ft_item<G4, CL, WIN>(a, ahead_item);
+    FtItem ahead = ft_item<G4, CL, WIN>(a, ahead_item / PARTS);
     auto fetch = [&]() -> int {
       if (!G4 || ahead_item >= n_items || ahead.n_tiles == 0) return -1;   // (gathered rows: every item has the same keys)
       const int v = row_of(ahead, ahead.nth(ahead_tile));
       if (++ahead_tile == ahead.n_tiles) {
         ahead_tile = 0;
         ahead_item += step;
-        if (ahead_item < n_items) ahead = ft_item<G4, CL, WIN>(a, ahead_item);
+        if (ahead_item < n_items) ahead = ft_item<G4, CL, WIN>(a, ahead_item / PARTS);
       }
       return v;
     };
@@ -293,7 +295,7 @@ __global__ __launch_bounds__(FT_THREADS, 1) void mla_flash_tc_kernel(
       return b;
     };
     for (int idx = blockIdx.x; idx < n_items; idx += step) {
-      const FtItem it = ft_item<G4, CL, WIN>(a, idx);
+      const FtItem it = ft_item<G4, CL, WIN>(a, idx / PARTS);
       if (it.n_tiles == 0) continue;
       {
         const int b = next_slot(it, -1);
@@ -372,7 +374,7 @@ __global__ __launch_bounds__(FT_THREADS, 1) void mla_flash_tc_kernel(
         return tc::make_sdesc_sw128(addr, 16, 1024);
       };
       for (int idx = blockIdx.x; idx < n_items; idx += step) {
-        const FtItem it = ft_item<G4, CL, WIN>(a, idx);
+        const FtItem it = ft_item<G4, CL, WIN>(a, idx / PARTS);
         const int n_tiles = it.n_tiles;
         if (n_tiles == 0) continue;
         if (direct_q) wait_u(&ms.full[0], 0, 15);
@@ -407,9 +409,9 @@ __global__ __launch_bounds__(FT_THREADS, 1) void mla_flash_tc_kernel(
         }
       }
     } else {
-      const uint32_t idesc = tc::make_idesc(64, 256, tc::FMT_F16, tc::FMT_F16, false, true);
+      const uint32_t idesc = tc::make_idesc(64, PARTS == 4 ? 128 : 256, tc::FMT_F16, tc::FMT_F16, false, true);
       for (int idx = blockIdx.x; idx < n_items; idx += step) {
-        const FtItem it = ft_item<G4, CL, WIN>(a, idx);
+        const FtItem it = ft_item<G4, CL, WIN>(a, idx / PARTS);
         if (it.n_tiles == 0) continue;
         u++;
         for (int tile = 0; tile < it.n_tiles; tile++, u++, g++) {
@@ -430,12 +432,12 @@ __global__ __launch_bounds__(FT_THREADS, 1) void mla_flash_tc_kernel(
                 tc::mma_ws_f16_if(leader, tmem + FT_O, tc::sdesc_advance(pd, kk * 32), tc::sdesc_advance(vc, kk * 2048), id, tile > 0 || kk > 0);
           } else
 #pragma unroll
-          for (int nh = 0; nh < 2; nh++)
+          for (int nh = 0; nh < (PARTS == 1 ? 2 : 1); nh++)
 #pragma unroll
             for (int kk = 0; kk < FT_KEYS / 16; kk++)
               if (kk < steps)
                 tc::mma_ws_f16_if(leader, tmem + FT_O + nh * 128, tc::sdesc_advance(pd, kk * 32),
-                                  tc::sdesc_advance(vd, nh * 4 * FT_BLK + kk * 2048), idesc, tile > 0 || kk > 0);
+                                  tc::sdesc_advance(vd, (nh * 4 + part * (8 / PARTS)) * FT_BLK + kk * 2048), idesc, tile > 0 || kk > 0);
           tc::mma_commit_if(leader, &ms.pv_done[b]);
           if (!CL || kb < FT_NBUF) tc::mma_commit_if(leader, &ms.free[kb]);
         }
@@ -480,14 +482,14 @@ __global__ __launch_bounds__(FT_THREADS, 1) void mla_flash_tc_kernel(
       u++;
     };
     auto next_row = [&](int idx) {                         // the first item from idx on that has keys
-      while (idx < n_items && ft_item<G4, CL, WIN>(a, idx).n_tiles == 0) idx += step;
+      while (idx < n_items && ft_item<G4, CL, WIN>(a, idx / PARTS).n_tiles == 0) idx += step;
       return idx;
     };
     int q_item = next_row(blockIdx.x);                     // the row whose Q is moved next
     if (direct_q) u = 1;
     else if (q_item < n_items) move_q();
     for (int idx = blockIdx.x; idx < n_items; idx += step) {
-      const FtItem it = ft_item<G4, CL, WIN>(a, idx);
+      const FtItem it = ft_item<G4, CL, WIN>(a, idx / PARTS);
       float m = -INFINITY, l = 0.f;
       for (int tile = 0; tile < it.n_tiles; tile++, u++, g++) {
         const int b = g & 1, kb = slot_of(it, u, tile);
@@ -524,7 +526,7 @@ __global__ __launch_bounds__(FT_THREADS, 1) void mla_flash_tc_kernel(
           wait_pv(g - 1, 8);
           tc::fence_after_sync();
 #pragma unroll 1
-          for (int c0 = 0; c0 < (CL ? FT_CS_CH / 2 : 256); c0 += 32) {
+          for (int c0 = 0; c0 < (CL ? FT_CS_CH / 2 : 256 / PARTS); c0 += 32) {
             uint32_t o[32];
             tc::tmem_ld32(tmem + FT_O + c0 + lanes, o);
             tc::tmem_ld_wait();
@@ -646,13 +648,14 @@ __global__ __launch_bounds__(FT_THREADS, 1) void mla_flash_tc_kernel(
         asm volatile("bar.sync 3, 128;" ::: "memory");     // P may be written again
       } else {
         // a partial (the CTA's only item): fp32 rows in the idle ring, one bulk copy per head
-        const uint32_t pitch = LATENT * 4 + 16;
+        constexpr int n_ch = LATENT / PARTS, span = PARTS == 4 ? 64 : 128;   // channels of this CTA, of a lane half of a product
+        const uint32_t pitch = n_ch * 4 + 16;
         uint8_t* orow = smem + FS_K + head * pitch;
 #pragma unroll 1
-        for (int c0 = 0; c0 < 256; c0 += 32) {
+        for (int c0 = 0; c0 < 256 / PARTS; c0 += 32) {
           uint32_t o[32];
           load_o(c0, o);
-          const int ch = (c0 >> 7) * 256 + half * 128 + (c0 & 127);
+          const int ch = c0 / span * 2 * span + half * span + c0 % span;
 #pragma unroll
           for (int v = 0; v < 8; v++)
             *reinterpret_cast<uint4*>(orow + ch * 4 + v * 16) = make_uint4(o[4 * v], o[4 * v + 1], o[4 * v + 2], o[4 * v + 3]);
@@ -661,10 +664,12 @@ __global__ __launch_bounds__(FT_THREADS, 1) void mla_flash_tc_kernel(
         asm volatile("bar.sync 3, 128;" ::: "memory");
         const size_t rows = (size_t)a.m * FT_HEADS, rh = (size_t)it.r * FT_HEADS + head;
         if (half == 0 && ok && !*abort_flag) {
-          tc::bulk_s2g(a.part_acc + ((size_t)it.sp * rows + rh) * LATENT, orow, LATENT * 4);
+          tc::bulk_s2g(a.part_acc + ((size_t)it.sp * rows + rh) * LATENT + part * n_ch, orow, n_ch * 4);
           tc::bulk_commit();
-          a.part_m[(size_t)it.sp * rows + rh] = (m == -INFINITY || !(l > 0.f)) ? -INFINITY : m / LOG2E;
-          a.part_l[(size_t)it.sp * rows + rh] = l;
+          if (part == 0) {
+            a.part_m[(size_t)it.sp * rows + rh] = (m == -INFINITY || !some) ? -INFINITY : m / LOG2E;
+            a.part_l[(size_t)it.sp * rows + rh] = l;
+          }
           tc::bulk_wait_read<0>();
         }
       }
@@ -677,7 +682,7 @@ __global__ __launch_bounds__(FT_THREADS, 1) void mla_flash_tc_kernel(
     }
     ok = tc::mbar_wait(&ms.q_ready, 0, abort_flag, 16) && ok;   // every split's share of this CTA's heads has arrived
     cluster_arrive();
-    const FtItem it = ft_item<G4, CL, WIN>(a, blockIdx.x);
+    const FtItem it = ft_item<G4, CL, WIN>(a, blockIdx.x / PARTS);
     const int n_h = FT_HEADS / a.n_split, row = FT_CL_ROW, share = n_h * (row + 8), chunks = row / 16;
     if (!*abort_flag) {
       for (int i = tid; i < n_h * chunks; i += FT_THREADS) {
@@ -745,7 +750,8 @@ static int ft_prepare() {
     auto any_cluster = [](auto* kernel) { return cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) == cudaSuccess; };
     if (!whole_sm(mla_flash_tc_kernel<false, false, false>) || !whole_sm(mla_flash_tc_kernel<true, false, false>) ||
         !whole_sm(mla_flash_tc_kernel<false, true, false>) || !whole_sm(mla_flash_tc_kernel<true, true, false>) ||
-        !whole_sm(mla_flash_tc_kernel<false, false, true>) || !whole_sm(mla_flash_tc_kernel<false, true, true>) || !whole_sm(mla_pair_tc_kernel<false>) ||
+        !whole_sm(mla_flash_tc_kernel<false, false, true>) || !whole_sm(mla_flash_tc_kernel<false, false, true, 2>) ||
+        !whole_sm(mla_flash_tc_kernel<false, false, true, 4>) || !whole_sm(mla_flash_tc_kernel<false, true, true>) || !whole_sm(mla_pair_tc_kernel<false>) ||
         !whole_sm(mla_pair_tc_kernel<true>) ||
         !any_cluster(mla_flash_tc_kernel<false, true, false>) || !any_cluster(mla_flash_tc_kernel<true, true, false>) ||
         !any_cluster(mla_flash_tc_kernel<false, true, true>))
@@ -878,9 +884,17 @@ int mla_flash_tc_launch(const MlaArgs& a, cudaStream_t s, bool clusters) {
     const cudaError_t e = pdl_launch_cluster(a.n_split, kernel, grid, dim3(FT_THREADS), FS_SMEM, s, a, device_status_ptr(), box, rows, qmap, omap);
     return e == cudaSuccess && cudaPeekAtLastError() == cudaSuccess ? HK_OK : HK_ERR_CUDA;
   }
-  const int64_t items = (int64_t)a.n_split * a.m;
+  // A window's few splits of few rows: the output channels of each over two or four CTAs (one row under 3,000 / 4,096 / 8,192
+  // keys 12.1 / 12.8 / 14.5 -> 9.9 / 10.6 / 11.6 us with the merge, four under 1,024 11.5 -> 9.4).
+  const int64_t splits = (int64_t)a.n_split * a.m;
+  const int parts = a.out || a.window <= 0 || 2 * splits > sm_count() ? 1 : 4 * splits > sm_count() ? 2 : 4;
+  const int64_t items = splits * parts;
   const dim3 grid((unsigned)((a.raw_idx || a.window > 0) && a.out && items > sm_count() ? sm_count() : items));
-  const auto kernel = a.raw_idx ? mla_flash_tc_kernel<true, false, false> : a.window ? mla_flash_tc_kernel<false, false, true> : mla_flash_tc_kernel<false, false, false>;
+  const auto kernel = a.raw_idx        ? mla_flash_tc_kernel<true, false, false>
+                      : !a.window    ? mla_flash_tc_kernel<false, false, false>
+                      : parts == 1   ? mla_flash_tc_kernel<false, false, true>
+                      : parts == 2   ? mla_flash_tc_kernel<false, false, true, 2>
+                                     : mla_flash_tc_kernel<false, false, true, 4>;
   const cudaError_t e = pdl_launch(kernel, grid, dim3(FT_THREADS), FS_SMEM, s, a, device_status_ptr(), box, rows, qmap, omap);
   return e == cudaSuccess && cudaPeekAtLastError() == cudaSuccess ? HK_OK : HK_ERR_CUDA;
 }
