@@ -37,10 +37,14 @@ struct AppendArgs {
 // One CTA of sixteen warps a block that gets rows; grid (blocks of a sequence, sequences).  A warp has rows w, w + 16, ... of the block, a lane the
 // channels 4 lane .. + 3 of each quarter of a row (16-byte loads, 4-byte stores, whole lines both).  Up to four rows a warp stay in registers
 // between the largest magnitude and the rounding (KEEP); a block of 128 tokens is read twice, the second time from L2.
+// PARTS: chunks share a block of 64 or 128 tokens out over the CTAs of a cluster, 32 or 64 rows each, which exchange their largest magnitudes (4,096
+// rows, us: blocks of 64 by one CTA / two 6.9 / 5.8; blocks of 128 by one / four 13.1 / 5.9), as long as the CTAs fit the SMs at once (8,192 rows:
+// blocks of 64 by one / two 7.1 / 11.2; blocks of 128 by one / two / four 16.4 / 8.4 / 11.4; 20,000 rows, blocks of 128, one / two 20.1 / 23.1).
+// Under 64 rows the barrier of the cluster costs what it gains (32 rows in blocks of 64, one / two 4.0 / 4.7).
 constexpr int APPEND_WARPS = 16;
-template <int FMT, int ROWS, bool KEEP>
+template <int FMT, int ROWS, bool KEEP, int PARTS>
 __global__ void __launch_bounds__(APPEND_WARPS * 32) mla8_append_kernel(AppendArgs a) {
-  __shared__ float s_amax[2][APPEND_WARPS];
+  __shared__ float s_amax[2][APPEND_WARPS], s_part[2];
   pdl_release();
   pdl_wait();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, seq = blockIdx.y, block = 1 << a.pg.shift;
@@ -58,7 +62,8 @@ __global__ void __launch_bounds__(APPEND_WARPS * 32) mla8_append_kernel(AppendAr
   constexpr float top = latent8_top<FMT>();
   const int64_t end = min((int64_t)p0 + (r1 - r0), (int64_t)INT32_MAX);
   int turn = 0;
-  for (int64_t lb = (p0 >> a.pg.shift) + blockIdx.x; (lb << a.pg.shift) < end; lb += gridDim.x, turn ^= 1) {
+  const int row0 = (int)(blockIdx.x % PARTS) * ROWS * APPEND_WARPS + warp;   // the warp's first row of a block
+  for (int64_t lb = (p0 >> a.pg.shift) + blockIdx.x / PARTS; (lb << a.pg.shift) < end; lb += gridDim.x / PARTS, turn ^= 1) {
     const int64_t start = lb << a.pg.shift;
     const int first = (int)max((int64_t)0, p0 - start), last = (int)min((int64_t)block, end - start);   // new rows of the block
     float y[KEEP ? ROWS : 1][16];
@@ -74,7 +79,7 @@ __global__ void __launch_bounds__(APPEND_WARPS * 32) mla8_append_kernel(AppendAr
     if (KEEP) {
 #pragma unroll
       for (int k = 0; k < ROWS; k++)
-        if (const int i = warp + APPEND_WARPS * k; i >= first && i < last) load(i, y[k]);
+        if (const int i = row0 + APPEND_WARPS * k; i >= first && i < last) load(i, y[k]);
     }
     const int64_t b = a.pg.block_of(seq, (int)start);
     uint2 lw[4];
@@ -92,7 +97,7 @@ __global__ void __launch_bounds__(APPEND_WARPS * 32) mla8_append_kernel(AppendAr
     bool bad = false;
 #pragma unroll
     for (int k = 0; k < ROWS; k++) {
-      const int i = warp + APPEND_WARPS * k;
+      const int i = row0 + APPEND_WARPS * k;
       float(&x)[16] = y[KEEP ? k : 0];
       if (i >= first && i < last) {
         if (!KEEP) load(i, x);
@@ -115,15 +120,27 @@ __global__ void __launch_bounds__(APPEND_WARPS * 32) mla8_append_kernel(AppendAr
     if (lane == 0) s_amax[turn][warp] = amax;
     __syncthreads();                                       // every warp has s0 and this turn's maximum
     amax = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(s_amax[turn][lane % APPEND_WARPS])));
+    if (PARTS > 1) {
+      if (threadIdx.x == 0) s_part[turn] = amax;
+      asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");   // every CTA of the block likewise
+#pragma unroll
+      for (int k = 0; k < PARTS; k++) {
+        uint32_t at;
+        float v;
+        asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"((uint32_t)__cvta_generic_to_shared(&s_part[turn])), "r"(k));
+        asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(at) : "memory");
+        amax = fmaxf(amax, v);
+      }
+    }
     if (b < 0) continue;
     const float need = amax > 1e-25f ? (amax < INFINITY ? __fdiv_rn(amax, top) : NAN) : 0.f;
     const bool grow = need > s0 || need != need;
     const float s = s0 != s0 ? s0 : grow ? need : s0, inv = s > 0.f ? __fdiv_rn(1.f, s) : 0.f;
-    if (threadIdx.x == 0) a.pg.scales[b] = s;
+    if (threadIdx.x == 0 && blockIdx.x % PARTS == 0) a.pg.scales[b] = s;
     uint8_t* rows = a.pg.data + ((size_t)b << a.pg.shift) * LATENT;
     if (grow && s == s) {
       const float ratio = __fdiv_rn(s0, s);
-      for (int i = warp; i < first; i += APPEND_WARPS) {
+      for (int i = row0; i < (PARTS > 1 ? min(first, row0 - warp + ROWS * APPEND_WARPS) : first); i += APPEND_WARPS) {
         uint4* q = reinterpret_cast<uint4*>(rows + (size_t)i * LATENT + lane * 16);
         uint4 v = *q;
         uint32_t* v4 = &v.x;
@@ -139,7 +156,7 @@ __global__ void __launch_bounds__(APPEND_WARPS * 32) mla8_append_kernel(AppendAr
     }
 #pragma unroll
     for (int k = 0; k < ROWS; k++) {
-      const int i = warp + APPEND_WARPS * k;
+      const int i = row0 + APPEND_WARPS * k;
       float(&x)[16] = y[KEEP ? k : 0];
       if (i >= first && i < last) {
         if (!KEEP) {
@@ -163,14 +180,17 @@ __global__ void __launch_bounds__(APPEND_WARPS * 32) mla8_append_kernel(AppendAr
       }
     }
   }
+  if (PARTS > 1) asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");   // nobody reads this CTA's maximum any more
 }
 
 template <int FMT>
-cudaError_t append_launch(const AppendArgs& a, dim3 grid, cudaStream_t s) {
-  const auto kernel = a.pg.shift == 4 ? mla8_append_kernel<FMT, 1, true>
-                      : a.pg.shift == 5 ? mla8_append_kernel<FMT, 2, true>
-                      : a.pg.shift == 6 ? mla8_append_kernel<FMT, 4, true> : mla8_append_kernel<FMT, 8, false>;
-  return pdl_launch(kernel, grid, dim3(APPEND_WARPS * 32), 0, s, a);
+cudaError_t append_launch(const AppendArgs& a, dim3 grid, int parts, cudaStream_t s) {
+  const auto kernel = a.pg.shift == 4 ? mla8_append_kernel<FMT, 1, true, 1>
+                      : a.pg.shift == 5 ? mla8_append_kernel<FMT, 2, true, 1>
+                      : a.pg.shift == 6 ? (parts > 1 ? mla8_append_kernel<FMT, 2, true, 2> : mla8_append_kernel<FMT, 4, true, 1>)
+                                        : (parts == 4   ? mla8_append_kernel<FMT, 2, true, 4>
+                                           : parts == 2 ? mla8_append_kernel<FMT, 4, true, 2> : mla8_append_kernel<FMT, 8, false, 1>);
+  return pdl_launch_cluster(parts, kernel, dim3(grid.x * parts, grid.y), dim3(APPEND_WARPS * 32), 0, s, a);
 }
 
 // rows i of out: position i of the sequence below `head`, i + shift from there on; f16(scale * value), zeros where there is no block.
@@ -280,7 +300,13 @@ HK_API int hk_mla8_append(const float* kv_pre, const void* ln_w_f16, void* ckv8,
     blocks = blocks > (all < room ? all : room) ? blocks : (all < room ? all : room);
   }
   const dim3 grid((unsigned)blocks, (unsigned)n_seqs);
-  return (dtype == HK_I8 ? append_launch<CACHE_I8>(a, grid, as_stream(stream)) : append_launch<CACHE_E4M3>(a, grid, as_stream(stream))) == cudaSuccess
+  int parts = 1;
+  if (n / n_seqs >= 64 && block > 32) {
+    const int64_t ctas = (int64_t)blocks * n_seqs, least = ctas <= sm_count() ? block / 64 : 1;
+    for (parts = block / 32; parts > least && ctas * parts > sm_count();) parts /= 2;
+  }
+  return (dtype == HK_I8 ? append_launch<CACHE_I8>(a, grid, parts, as_stream(stream)) : append_launch<CACHE_E4M3>(a, grid, parts, as_stream(stream))) ==
+                 cudaSuccess
              ? HK_OK
              : HK_ERR_CUDA;
 }

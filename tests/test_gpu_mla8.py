@@ -71,6 +71,28 @@ def test_append(kind, block, pos, rows):
     assert torch.equal(ckv8.view(torch.uint8), again.view(torch.uint8)) and torch.equal(scales, again_s), "the same rows again change nothing"
 
 
+@pytest.mark.parametrize("kind,block,pos,rows", [("i8", 64, [37], [1000]), ("e4m3", 64, [50], [6000]), ("i8", 128, [100], [1500]), ("e4m3", 128, [77], [5000]),
+                                                 ("i8", 128, [1], [19200]), ("i8", 128, [70, 0, 9], [30, 900, 0]), ("e4m3", 64, [63, 33, 9], [2, 0, 700])])
+def test_append_of_blocks_shared_out_over_ctas(kind, block, pos, rows):
+    """blocks of 64 and 128 tokens by one CTA, two and four; a row that is not finite makes its whole block NaN, whichever CTA has it"""
+    gen = gen_of(sum(rows))
+    starts = [0]
+    for r in rows:
+        starts.append(starts[-1] + r)
+    blocks = max((p + r - 1) // block + 1 for p, r in zip(pos, rows))
+    n_blocks = blocks * len(pos)
+    ckv8, scales = cache(gen, kind, n_blocks, block)
+    scales *= 0.02 * torch.exp(0.5 * torch.randn(n_blocks, device="cuda", generator=gen))
+    table = table_for(gen, len(pos), blocks, n_blocks)
+    x, w = inputs(gen, starts[-1])
+    x[starts[-1] - 3, 5] = math.inf
+    old, old_s = ckv8.clone(), scales.clone()
+    hk.mla8_cache_append(x, w, ckv8, scales, ints(pos), starts[-1], ref.EPS, block_table=table, n_seqs=len(pos), seq_start=ints(starts))
+    finish()
+    assert bool(scales.isnan().any())
+    check_append(old, old_s, ckv8, scales, x, w, table.cpu(), pos, starts, kind)
+
+
 @pytest.mark.parametrize("kind", ["i8", "e4m3"])
 def test_append_one_token_after_another_and_read(kind):
     """a block fills token by token: each step against the definition from the state before it; then everything read back"""
@@ -574,3 +596,13 @@ def test_captured_decode_step_replayed():
         assert torch.equal(out, want) and torch.equal(ckv8, c2) and torch.equal(scales, s2)
         pos += 1
         lens += 1
+
+
+def test_scratch_follows_its_tensor_and_is_never_empty():
+    t = torch.zeros(3, device="cuda")
+    for asked in (0, 1, 1000):
+        ws = hk._native.scratch(asked, t)
+        assert ws.dtype == torch.uint8 and ws.device == t.device and ws.numel() == max(asked, 256)
+    for bad in [(), (5,), (5, 7), ("5", t)]:
+        with pytest.raises((TypeError, ValueError)):
+            hk._native.scratch(*bad)
