@@ -511,7 +511,8 @@ __global__ __launch_bounds__(F8_THREADS, 1) void mla8_flash_tc_kernel(MlaArgs a,
     l += ms.mx[n_tiles & 1][tid ^ 64];
     const bool none = l == 0.f;                            // (NaN: a score was none)
     if (half == 0) {
-      ms.mx[(n_tiles + 1) & 1][head] = none ? 0.f : final_out ? sref / l : sref;
+      // NaN has to reach the merge, which weighs a split of nothing else 0
+      ms.mx[(n_tiles + 1) & 1][head] = none ? 0.f : final_out ? sref / l : l == l ? sref : l;
       if (!final_out && it.r >= 0 && it.part == 0 && head < n_h) {
         const size_t at = part_row + head;
         a.part_m[at] = m == -INFINITY || none ? -INFINITY : m / F8_LOG2E;

@@ -374,6 +374,31 @@ def test_a_row_that_is_not_finite_is_seen_in_the_output():
         assert torch.isfinite(out).all()
 
 
+@pytest.mark.parametrize("kind", ["i8", "e4m3"])
+@pytest.mark.parametrize("m,n", [(1, 65), (1, 129), (1, 2049), (1, 5001), (1, 12033), (3, 2113), (4, 8193), (8, 9025), (40, 577), (200, 193)])
+def test_splits_that_see_nothing_but_rows_that_are_not_finite(kind, m, n):
+    """the last block, or two, of a row, which are the keys of a whole split for some of these lengths; and all blocks"""
+    gen, block = gen_of(n), 64
+    blocks = (n + block - 1) // block
+    ckv8, scales = cache(gen, kind, blocks, block)
+    table = table_for(gen, 1, blocks, blocks)
+    q = queries(gen, m, 64)
+    out = torch.zeros(m, 64, 512, dtype=torch.float16, device="cuda")
+    gather = torch.arange(n, device="cuda", dtype=torch.int32).repeat(m, 1)
+    for bad in (1, 2, blocks):
+        scales[table[0, blocks - bad:].long()] = math.nan
+        for n_split in (0, 2, 7):
+            hk.mla8_dense_prefill(q, ckv8, scales, out.zero_(), m, 0, block_table=table, kv_len=ints([n] * m), n_keys_hint=n, n_split=n_split)
+            finish()
+            assert torch.isnan(out).all(), (bad, n_split)
+            hk.mla8_sparse_decode(q, ckv8, scales, gather, n, out.zero_(), m, block_table=table, n_split=n_split)
+            finish()
+            assert torch.isnan(out).all(), (bad, n_split)
+    hk.mla8_dense_prefill(q, ckv8, scales, out.zero_(), m, n, block_table=torch.cat((table, table, table, table, table), 1).contiguous())
+    finish()
+    assert torch.isnan(out).all()
+
+
 @pytest.mark.parametrize("kind,block,heads,m,kidx,n_split", [("i8", 64, 64, 1, 2052, 0), ("e4m3", 16, 64, 3, 130, 0), ("i8", 128, 16, 2, 1, 1), ("i8", 32, 64, 5, 64, 2),
                                                              ("e4m3", 64, 64, 2, 700, 5), ("i8", 64, 64, 200, 70, 0)])
 def test_sparse8(kind, block, heads, m, kidx, n_split):
