@@ -454,7 +454,7 @@ def mla_window_prefill(q_lat, ckv, lat_out, qlen, pos_start, window, sinks=0, st
     if n_split <= 0:
         tiles = -(-sinks // 64) + (window + 62) // 64 + 1      # whole tiles under the window (hk_mla_window chooses by as many)
         n = pos_start if kv_len is not None else pos_start + qlen
-        splits = _native.hk_mla_auto_splits(qlen, 64 * (min(tiles, -(-n // 64)) if n else tiles))
+        splits = _native.hk_mla_auto_splits(qlen, min(64 * (min(tiles, -(-n // 64)) if n else tiles), 2 ** 31 - 1))
     ws = workspace
     if splits > 1 and ws is None:
         ws = _scratch_like(_native.hk_mla_partial_bytes(splits, qlen * n_heads), q_lat, stream)

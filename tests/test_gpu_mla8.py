@@ -623,6 +623,21 @@ def test_captured_decode_step_replayed():
         lens += 1
 
 
+def test_the_widest_window():
+    """a window of all 31 bits with lengths on the device and none given to choose the splits by"""
+    gen = gen_of(77)
+    ckv, q = torch.randn(700, 512, device="cuda", generator=gen).half(), queries(gen, 3, 64)
+    ckv8, scales = cache(gen, "i8", 11, 64)
+    out = torch.empty(3, 64, 512, dtype=torch.float16, device="cuda")
+    for sinks in (0, 5, 2 ** 31 - 1):
+        hk.mla_window_prefill(q, ckv, out, 3, 0, 2 ** 31 - 1, sinks=sinks, kv_len=ints([700, 0, 65]))
+        finish()
+        close(out, [attend(q[r].double(), ckv[:n].double(), 0.0625) for r, n in enumerate([700, 0, 65])])
+        hk.mla8_dense_prefill(q, ckv8, scales, out, 3, 0, window=2 ** 31 - 1, sinks=sinks, kv_len=ints([700, 0, 65]))
+        finish()
+        close(out, [attend(q[r].double(), rows_of(ckv8, scales, torch.arange(11), torch.arange(n)), 0.0625) for r, n in enumerate([700, 0, 65])])
+
+
 def test_scratch_follows_its_tensor_and_is_never_empty():
     t = torch.zeros(3, device="cuda")
     for asked in (0, 1, 1000):
