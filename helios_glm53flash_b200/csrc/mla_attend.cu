@@ -238,7 +238,8 @@ struct GatherPlan {
 };
 static GatherPlan gather_plan(int m, int n_heads, int kidx, int64_t positions, bool per_row) {
   GatherPlan g{};
-  g.on = !per_row && n_heads == 64 && m >= GATHER_ROWS && (int64_t)m * kidx >= GATHER_TIMES * positions && positions <= INT32_MAX && !force_simt();
+  g.on = !per_row && n_heads == 64 && m >= GATHER_ROWS && positions <= INT32_MAX && (int64_t)m * kidx >= GATHER_TIMES * positions && !force_simt();
+  if (!g.on) return g;
   g.rows = (size_t)positions * LATENT * sizeof(__half);
   g.bytes = align_up(g.rows + (size_t)m * kidx * sizeof(int), 256);
   return g;
@@ -247,7 +248,7 @@ static GatherPlan gather_plan(int m, int n_heads, int kidx, int64_t positions, b
 }  // namespace hk
 
 HK_API size_t hk_mla8_sparse_workspace_bytes(int m, int n_heads, int kidx, int64_t positions, int per_row) {
-  if (m <= 0 || n_heads < hk::SIMT_HG || kidx <= 0 || positions < 0 || positions > INT32_MAX) return 0;
+  if (m <= 0 || n_heads < hk::SIMT_HG || kidx <= 0 || positions < 0) return 0;
   int units = 0;
   const hk::GatherPlan g = hk::gather_plan(m, n_heads, kidx, positions, per_row);
   const int splits = g.on ? hk::mla_flash_tc_auto_splits(m, kidx) : hk::attend8_splits(m, n_heads, kidx, false, &units);

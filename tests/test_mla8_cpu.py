@@ -90,3 +90,12 @@ def test_workspaces_are_enough_and_no_more(lib):
     assert gathered >= 256 * 1024 + 300 * 70 * 4
     assert call(lib, "hk_mla8_sparse", SPARSE, m=300, kidx=70, row_seq=None, ws=A, ws_bytes=gathered - 1) == hk.HK_ERR_WORKSPACE
     assert lib.hk_mla8_sparse_workspace_bytes(5000, 64, 2052, 256, 1) == 0 and lib.hk_mla8_sparse_workspace_bytes(1, 64, 64, 256, 1) == 0
+
+
+def test_tables_of_more_positions_than_31_bits_need_no_less_workspace(lib):
+    for m in (1, 3, 300):
+        want = lib.hk_mla8_sparse_workspace_bytes(m, 64, 2052, 1 << 30, 0)
+        assert lib.hk_mla8_sparse_workspace_bytes(m, 64, 2052, 1 << 33, 0) == lib.hk_mla8_sparse_workspace_bytes(m, 64, 2052, 2 ** 63 - 1, 0) == want
+    assert lib.hk_mla8_sparse_workspace_bytes(1, 64, 2052, 1 << 33, 0) > 64 * 2056
+    need = lib.hk_mla8_sparse_workspace_bytes(1, 64, 2052, 1 << 33, 0)
+    assert call(lib, "hk_mla8_sparse", SPARSE, m=1, kidx=2052, row_seq=None, stride=1 << 27, ws=A, ws_bytes=need - 1) == hk.HK_ERR_WORKSPACE
