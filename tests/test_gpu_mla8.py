@@ -638,6 +638,60 @@ def test_the_widest_window():
         close(out, [attend(q[r].double(), rows_of(ckv8, scales, torch.arange(11), torch.arange(n)), 0.0625) for r, n in enumerate([700, 0, 65])])
 
 
+@pytest.mark.parametrize("kind", ["i8", "e4m3"])
+def test_blocks_beyond_four_gigabytes(kind):
+    """blocks at the end of a cache of 9.6 million latents, through a table and by their positions; an fp16 cache of 5 million likewise"""
+    gen, block, n_blocks, n = gen_of(88), 64, 150000, 1000
+    ckv8, scales = torch.empty(n_blocks, block, 512, dtype=torch.int8, device="cuda").view(STORE[kind]), torch.full((n_blocks,), math.nan, device="cuda")
+    table = (n_blocks - 1 - torch.randperm(16, device="cuda", generator=gen)).to(torch.int32)[None].contiguous()
+    x, w = inputs(gen, n)
+    held, out = torch.empty(n, 512, dtype=torch.float16, device="cuda"), torch.empty(n, 512, dtype=torch.float16, device="cuda")
+    hk.mla8_cache_append(x, w, ckv8, scales, ints([0]), n, ref.EPS, block_table=table, ckv_new=held)
+    hk.mla8_cache_read(ckv8, scales, out, 0, n, block_table=table)
+    finish()
+    assert bool(torch.isfinite(held).all()) and torch.equal(held, out)
+    q, o = queries(gen, 2, 64), torch.empty(2, 64, 512, dtype=torch.float16, device="cuda")
+    keys = rows_of(ckv8, scales, table[0], torch.arange(n, device="cuda"))
+    idx = torch.randint(0, n, (2, 300), device="cuda", generator=gen, dtype=torch.int32)
+    hk.mla8_dense_prefill(q, ckv8, scales, o, 2, 0, block_table=table, kv_len=ints([n, n - 7]))
+    finish()
+    close(o, [attend(q[r].double(), keys[:n - 7 * r], 0.0625) for r in range(2)])
+    hk.mla8_sparse_decode(q, ckv8, scales, idx, 300, o, 2, block_table=table)
+    finish()
+    close(o, [attend(q[r].double(), keys[idx[r].long()], 0.0625) for r in range(2)])
+    # by position, without a table: the last 16 blocks in order
+    far = (n_blocks - 16) * block
+    order = torch.arange(n_blocks - 16, n_blocks, device="cuda", dtype=torch.int32)
+    hk.mla8_cache_append(x, w, ckv8, scales, ints([far]), n, ref.EPS, ckv_new=held)
+    hk.mla8_cache_read(ckv8, scales, out, far, n)
+    finish()
+    assert bool(torch.isfinite(held).all()) and torch.equal(held, out)
+    keys = rows_of(ckv8, scales, order, torch.arange(n, device="cuda"))
+    hk.mla8_dense_prefill(q, ckv8, scales, o, 2, 0, kv_len=ints([far + n, far + 900]), window=500, n_keys_hint=far + n)
+    finish()
+    close(o, [attend(q[0].double(), keys[n - 500:], 0.0625), attend(q[1].double(), keys[400:900], 0.0625)])
+    hk.mla8_dense_prefill(q, ckv8, scales, o, 2, far + n - 2, window=500)
+    finish()
+    close(o, [attend(q[r].double(), keys[n - 501 + r:n - 1 + r], 0.0625) for r in range(2)])
+    hk.mla8_sparse_decode(q, ckv8, scales, idx + far, 300, o, 2)
+    finish()
+    close(o, [attend(q[r].double(), keys[idx[r].long()], 0.0625) for r in range(2)])
+
+
+def test_windows_beyond_four_gigabytes():
+    gen, rows, n = gen_of(89), 5000000, 1000
+    ckv, q, o = torch.empty(rows, 512, dtype=torch.float16, device="cuda"), queries(gen, 2, 64), torch.empty(2, 64, 512, dtype=torch.float16, device="cuda")
+    ckv[rows - n:] = torch.randn(n, 512, device="cuda", generator=gen).half()
+    ckv[:100] = torch.randn(100, 512, device="cuda", generator=gen).half()
+    hk.mla_window_prefill(q, ckv, o, 2, 0, 300, sinks=70, kv_base=torch.tensor([rows - n, 0], device="cuda"), kv_len=ints([n, rows]), n_keys_hint=rows)
+    finish()
+    close(o, [attend(q[0].double(), torch.cat((ckv[rows - n:rows - n + 70], ckv[rows - 300:])).double(), 0.0625),
+              attend(q[1].double(), torch.cat((ckv[:70], ckv[rows - 300:])).double(), 0.0625)])
+    hk.mla_window_prefill(q, ckv, o, 2, rows - 2, 300, sinks=70)
+    finish()
+    close(o, [attend(q[r].double(), torch.cat((ckv[:70], ckv[rows - 301 + r:rows - 1 + r])).double(), 0.0625) for r in range(2)])
+
+
 def test_scratch_follows_its_tensor_and_is_never_empty():
     t = torch.zeros(3, device="cuda")
     for asked in (0, 1, 1000):
