@@ -118,9 +118,15 @@ int mla_window_keys(int n, int window, int sinks) {
 static int attend(MlaArgs a, int n_keys_hint, int n_split, bool choose, void* workspace, size_t workspace_bytes,
                   cudaStream_t s) {
   const bool tc = (a.n_heads == 64) && !force_simt();
-  if (n_split <= 0)
+  if (n_split <= 0) {
     n_split = tc ? mla_flash_tc_auto_splits(a.m, n_keys_hint)
                  : simt_auto_splits(a.m, a.n_heads, n_keys_hint);
+    // Windows: half as many, whose output channels two CTAs share, where that has the room and means at most six tiles each.  Splits as they are
+    // / half of them, us: four rows under 4,096 keys 15.4 / 13.1, eight under 2,048 14.2 / 12.6, 24 under 512 13.9 / 13.6, under 1,024 (six tiles)
+    // 15.8 / 15.6, eight under 4,096 (eight) 16.0 / 15.9.
+    const int half = (n_split + 1) / 2, tiles = n_keys_hint / 64 + (n_keys_hint % 64 != 0), room = sm_count();
+    if (tc && a.window > 0 && half > 1 && (int64_t)2 * n_split * a.m > room && (int64_t)2 * half * a.m <= room && (tiles + half - 1) / half <= 6) n_split = half;
+  }
   const int64_t rows = (int64_t)a.m * a.n_heads;
   __half* final_out = a.out;
   a.n_split = n_split;

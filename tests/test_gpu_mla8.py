@@ -450,7 +450,8 @@ def test_sparse8_of_many_rows(kind, block, m, kidx, blocks):
 # ---------------------------------------------------------------------------------------------
 @pytest.mark.parametrize("heads,lens,window,sinks,n_split", [
     (64, [1], 1, 0, 0), (64, [64, 65, 200], 64, 0, 1), (64, [1000], 100, 4, 0), (64, [5000], 2000, 64, 0), (64, [900, 3, 0, 129], 128, 65, 0),
-    (64, [700, 701], 1, 0, 3), (16, [500, 40], 33, 2, 0), (64, [3000], 10000, 10000, 0), (64, [257], 64, 1, 2), (64, [4000], 63, 3999, 0)])
+    (64, [700, 701], 1, 0, 3), (16, [500, 40], 33, 2, 0), (64, [3000], 10000, 10000, 0), (64, [257], 64, 1, 2), (64, [4000], 63, 3999, 0),
+    (64, [5000, 4100, 300, 4999], 4090, 5, 0), (64, [3000, 2999, 2200, 40, 0, 2049, 2600, 2500], 2040, 3, 0)])
 def test_window_rows(heads, lens, window, sinks, n_split):
     gen = gen_of(sum(lens) + window)
     base = [sum(lens[:i]) for i in range(len(lens))]
