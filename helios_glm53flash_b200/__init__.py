@@ -448,6 +448,8 @@ def mla_window_prefill(q_lat, ckv, lat_out, qlen, pos_start, window, sinks=0, st
                        kv_base=None, kv_len=None, n_split=0, workspace=None, n_keys_hint=None, ckv_rows=None):
     """mla_dense_prefill whose rows attend to their last `window` keys and the first `sinks` only (hk_mla_window); qlen = 1 is
     decode, kv_base / kv_len as there.  n_keys_hint: keys of the longest row where kv_len says them on the device."""
+    size = qlen * n_heads * 512
+    _native.tensors("hhhli", ("q_lat", "lat_out", "ckv", "kv_base", "kv_len"), q_lat, size, lat_out, size, ckv, 0, kv_base, qlen, kv_len, qlen)
     if kv_len is not None:
         pos_start = n_keys_hint or pos_start
     splits = n_split
@@ -463,20 +465,20 @@ def mla_window_prefill(q_lat, ckv, lat_out, qlen, pos_start, window, sinks=0, st
 
 
 # ---- the latent cache in 8 bits, paged: ckv8 [n_blocks, block, 512] of torch.int8 or torch.float8_e4m3fn, scales [n_blocks] float32,
-# block_table [n_seqs, blocks of a sequence] int32 (None: one sequence whose i-th block is block i) ----
+# block_table [n_seqs, blocks of a sequence] int32 (None: one sequence whose i-th block is block i).  Tensors of another type, layout, device or
+# size than the call's raise ValueError ----
 def mla8_cache_append(kv_pre, ln_w, ckv8, scales, pos, n, eps, block_table=None, n_seqs=1, seq_start=None, ckv_new=None, stream=None):
     """RMS norm of n new latent rows into the 8-bit cache (hk_mla8_append).  pos: device int32 [n_seqs], position of each sequence's
     first new row; seq_start: device int32 [n_seqs + 1], its rows of kv_pre (None: n / n_seqs each); ckv_new: fp16 [n, 512], the rows as the
     cache holds them."""
-    tag, n_blocks, block, stride, seqs = _native.cache8(ckv8, scales, block_table)
-    if n_seqs > seqs:
-        raise ValueError("block_table: fewer sequences than n_seqs")
-    _run("hk_mla8_append", kv_pre, ln_w, ckv8, scales, tag, n_blocks, block, block_table, stride, n_seqs, seq_start, pos, n, eps, ckv_new, stream)
+    st = _native.append8(ckv8, scales, block_table, kv_pre, ln_w, pos, n, eps, n_seqs, seq_start, ckv_new, stream)
+    if st:
+        raise HeliosB200Error("hk_mla8_append", st)
 
 
 def mla8_cache_read(ckv8, scales, out, pos, n, block_table=None, stream=None):
     """positions pos .. pos + n - 1 of one sequence as fp16 rows (hk_mla8_read); block_table: the sequence's row of the table"""
-    tag, n_blocks, block, stride, seqs = _native.cache8(ckv8, scales, block_table)
+    tag, n_blocks, block, stride, seqs = _native.cache8(ckv8, scales, block_table, "h", ("out",), out, n * 512)
     if seqs != 1:
         raise ValueError("block_table: one sequence's row of the table")
     _run("hk_mla8_read", ckv8, scales, tag, n_blocks, block, block_table, stride, pos, n, out, stream)
@@ -495,7 +497,9 @@ def mla8_dense_prefill(q_lat, ckv8, scales, lat_out, qlen, pos_start, stream=Non
     """mla_dense_prefill over the 8-bit cache (hk_mla8_dense): a chunk of one sequence (kv_len and row_seq None), or rows of sequences
     row_seq[r] (device int32, None: sequence 0) with kv_len[r] keys each (device int32), the longest about n_keys_hint.  window > 0: the
     last `window` keys of a row and the first `sinks` only."""
-    tag, n_blocks, block, stride, seqs = _native.cache8(ckv8, scales, block_table)
+    size = qlen * n_heads * 512
+    tag, n_blocks, block, stride, seqs = _native.cache8(
+        ckv8, scales, block_table, "hhii", ("q_lat", "lat_out", "row_seq", "kv_len"), q_lat, size, lat_out, size, row_seq, qlen, kv_len, qlen)
     ws, hint = workspace, n_keys_hint or 0
     if ws is None:
         need = (_native.hk_mla8_dense_workspace_bytes(qlen, n_heads, pos_start, hint, window, sinks, 1 if kv_len is not None or row_seq is not None else 0)
@@ -509,7 +513,9 @@ def mla8_dense_prefill(q_lat, ckv8, scales, lat_out, qlen, pos_start, stream=Non
 def mla8_sparse_decode(q_lat, ckv8, scales, raw_idx, kidx, lat_out, m, stream=None, scale=0.0625, n_heads=64, block_table=None, row_seq=None,
                        n_split=0, workspace=None):
     """mla_sparse_decode over the 8-bit cache (hk_mla8_sparse): raw_idx holds positions of the row's sequence"""
-    tag, n_blocks, block, stride, seqs = _native.cache8(ckv8, scales, block_table)
+    size = m * n_heads * 512
+    tag, n_blocks, block, stride, seqs = _native.cache8(
+        ckv8, scales, block_table, "hhii", ("q_lat", "lat_out", "raw_idx", "row_seq"), q_lat, size, lat_out, size, raw_idx, m * kidx, row_seq, m)
     ws = workspace
     if ws is None:
         positions = (stride if stride else n_blocks) * block

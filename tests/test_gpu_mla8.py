@@ -177,6 +177,35 @@ def test_tensors_that_are_not_on_the_device_are_refused():
             hk.mla8_dense_prefill(out, c, s, out, 1, 0, block_table=t)
 
 
+def test_tensors_of_another_type_layout_or_size_are_refused():
+    """what the addresses that the library gets cannot tell: the wrappers look at the tensors"""
+    gen = gen_of(12)
+    ckv8, scales = cache(gen, "i8", 8, 16)
+    table = ints([[0, 1, 2, 3], [4, 5, 6, 7]])
+    x, w = inputs(gen, 2)
+    q, out = queries(gen, 2, 64), torch.empty(2, 64, 512, dtype=torch.float16, device="cuda")
+    ckv = torch.randn(64, 512, device="cuda", generator=gen).half()
+    append = (hk.mla8_cache_append, dict(kv_pre=x, ln_w=w, ckv8=ckv8, scales=scales, pos=ints([3, 7]), n=2, eps=ref.EPS, block_table=table, n_seqs=2,
+                                         seq_start=ints([0, 1, 2]), ckv_new=torch.empty(2, 512, dtype=torch.float16, device="cuda")))
+    read = (hk.mla8_cache_read, dict(ckv8=ckv8, scales=scales, out=torch.empty(20, 512, dtype=torch.float16, device="cuda"), pos=3, n=20, block_table=table[0]))
+    dense = (hk.mla8_dense_prefill, dict(q_lat=q, ckv8=ckv8, scales=scales, lat_out=out, qlen=2, pos_start=0, block_table=table, row_seq=ints([0, 1]), kv_len=ints([40, 50])))
+    sparse = (hk.mla8_sparse_decode, dict(q_lat=q, ckv8=ckv8, scales=scales, raw_idx=ints([[1, 2, 3], [4, 5, 6]]), kidx=3, lat_out=out, m=2, block_table=table, row_seq=ints([0, 1])))
+    window = (hk.mla_window_prefill, dict(q_lat=q, ckv=ckv, lat_out=out, qlen=2, pos_start=0, window=9, kv_base=torch.tensor([0, 5], device="cuda"), kv_len=ints([40, 50])))
+    wide = lambda t: torch.stack((t, t), -1)[..., 0]           # every second element
+    for fn, args in (append, read, dense, sparse, window):
+        fn(**args)
+        for name, t in args.items():
+            if not torch.is_tensor(t):
+                continue
+            other = {torch.float32: torch.float16, torch.float16: torch.bfloat16, torch.int32: torch.int64, torch.int64: torch.int32}.get(t.dtype, torch.uint8)
+            small = t if name in ("ckv", "block_table") else t.reshape(-1)[:-1]   # (a shorter table is a table, of fewer positions)
+            for bad in (t.to(other), wide(t), t.cpu(), small):
+                if bad is not t:
+                    with pytest.raises(ValueError):
+                        fn(**{**args, name: bad})
+    finish()
+
+
 def test_lengths_that_are_far_too_long_end_with_the_table():
     """garbage in a padding row's length: as many keys as the table has places, a window behind them sees the sinks alone"""
     gen = gen_of(22)

@@ -99,3 +99,24 @@ def test_tables_of_more_positions_than_31_bits_need_no_less_workspace(lib):
     assert lib.hk_mla8_sparse_workspace_bytes(1, 64, 2052, 1 << 33, 0) > 64 * 2056
     need = lib.hk_mla8_sparse_workspace_bytes(1, 64, 2052, 1 << 33, 0)
     assert call(lib, "hk_mla8_sparse", SPARSE, m=1, kidx=2052, row_seq=None, stride=1 << 27, ws=A, ws_bytes=need - 1) == hk.HK_ERR_WORKSPACE
+
+
+def test_tensors_of_another_type_layout_or_size_raise(lib):
+    import torch
+    from helios_glm53flash_b200 import _binding as nb
+    names = ("half", "single", "ints", "longs")
+    ok = [torch.zeros(4, 8).half(), 32, torch.zeros(3), 3, torch.zeros(5, dtype=torch.int32), 4, torch.zeros(2, dtype=torch.int64), 0]
+    assert nb.tensors("hfil", names, *ok) is None
+    assert nb.tensors("hfil", names, *[x if k % 2 else None for k, x in enumerate(ok)]) is None
+    cache = (torch.zeros(4, 16, 512, dtype=torch.int8), torch.zeros(4), None)
+    assert nb.cache8(*cache, "hfil", names, *ok) == nb.cache8(*cache)
+    for k, bad in ((0, torch.zeros(4, 8)), (0, torch.zeros(8, 4).half().t()), (0, torch.zeros(31).half()), (0, torch.zeros(4, 8).bfloat16()), (0, 5),
+                   (2, torch.zeros(2)), (2, torch.zeros(6)[::2]), (4, torch.zeros(5, dtype=torch.int64)), (4, torch.zeros(3, dtype=torch.int32)),
+                   (6, torch.zeros(2, dtype=torch.int32)), (6, [1, 2])):
+        args = ok[:k] + [bad] + ok[k + 1:]
+        for call_ in (lambda: nb.tensors("hfil", names, *args), lambda: nb.cache8(*cache, "hfil", names, *args)):
+            with pytest.raises(ValueError, match=names[k // 2]):
+                call_()
+    for args in (("hfil", names, *ok[:-1]), ("hfi", names, *ok), (3, names, *ok), ("hfil", list(names), *ok), ()):
+        with pytest.raises(TypeError):
+            nb.tensors(*args)
