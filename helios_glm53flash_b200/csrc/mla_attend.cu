@@ -86,10 +86,10 @@ static int combine_launch(const float* pm, const float* pl, const float* pa, int
              : HK_ERR_CUDA;
 }
 
-template <int GROUPS>
+template <int GROUPS, int PRE>
 static int combine_cs_launch(const float* pm, const float* pl, const float* pa, int n_split, int64_t rows, __half* out,
                              cudaStream_t s) {
-  return pdl_launch(lse_combine_cs_kernel<GROUPS>, dim3((unsigned)rows, LSE_CSPLIT), dim3(32 * GROUPS), 0, s, pm, pl, pa, n_split,
+  return pdl_launch(lse_combine_cs_kernel<GROUPS, PRE>, dim3((unsigned)rows, LSE_CSPLIT), dim3(32 * GROUPS), 0, s, pm, pl, pa, n_split,
                     rows, out) == cudaSuccess
              ? HK_OK
              : HK_ERR_CUDA;
@@ -102,8 +102,10 @@ static int combine(const float* pm, const float* pl, const float* pa, int n_spli
     return pdl_launch(lse_combine_few_kernel, dim3((unsigned)rows), dim3(128), 0, s, pm, pl, pa, n_split, rows, out) == cudaSuccess ? HK_OK : HK_ERR_CUDA;
   // Four CTAs a row, a quarter of the channels each.  Bits as with one CTA of 1,024 threads, which has the rest: the sums are the same eight, in the
   // same order, as long as a thread has one split's weight.  One / four, us: 64 rows of 40 splits 4.0 / 3.0, of 137 5.9 / 4.4, 320 rows of 29
-  // 10.1 / 5.2, 1,024 of 100 57 / 37.
-  if (n_split <= 256) return combine_cs_launch<8>(pm, pl, pa, n_split, rows, out, s);
+  // 10.1 / 5.2, 1,024 of 100 57 / 37.  Up to four CTAs an SM, a thread asks for six pieces before the weights (else three): 64 rows of 33 splits 3.0 ->
+  // 2.6, of 137 4.35 -> 4.25, 128 of 33 3.5 -> 3.2; but 256 of 100 9.0 / 9.5, 1,024 of 100 37 / 39.
+  if (n_split <= 256)
+    return rows <= 128 ? combine_cs_launch<8, 6>(pm, pl, pa, n_split, rows, out, s) : combine_cs_launch<8, 3>(pm, pl, pa, n_split, rows, out, s);
   return combine_launch<LSE_GROUPS>(pm, pl, pa, n_split, rows, out, s);
 }
 

@@ -330,7 +330,7 @@ __global__ __launch_bounds__(128) void lse_combine_few_kernel(const float* __res
 // owning 512 / CSPLIT channels, with GROUPS groups of 32 float4 lanes over the splits, so that 64 rows still cover
 // the machine.  grid = (rows, CSPLIT).
 constexpr int LSE_CSPLIT = 4;
-template <int GROUPS>
+template <int GROUPS, int PRE>
 __global__ __launch_bounds__(32 * GROUPS) void lse_combine_cs_kernel(
     const float* __restrict__ part_m, const float* __restrict__ part_l, const float* __restrict__ part_acc,
     int n_split, int64_t rows, __half* __restrict__ out) {
@@ -341,7 +341,7 @@ __global__ __launch_bounds__(32 * GROUPS) void lse_combine_cs_kernel(
   const int cpart = blockIdx.y;
   float gm, gl;
   float4 o;
-  lse_reduce_row<false, GROUPS, LANES, 3>(part_m, part_l, part_acc, nullptr, nullptr, nullptr, n_split, rows, r,
+  lse_reduce_row<false, GROUPS, LANES, PRE>(part_m, part_l, part_acc, nullptr, nullptr, nullptr, n_split, rows, r,
                                                                 gm, gl, o, cpart);
   if (threadIdx.x < LANES) {
     const float inv = gl > 0.f ? 1.f / gl : 0.f;
