@@ -13,12 +13,14 @@
 // and store them in the 128-byte-swizzle layout that both products read.  Rows that the query does not see become zeros there.
 //
 // What bounds it: about 2,400 cycles a tile, of which shared memory is busy 1,810 at 128 B a cycle (64 KB of fp16 stored, K and V read, Q 16, P
-// 24 KB) and the schedulers 1,500 (6,000 instructions of warps a tile: 2,600 for the conversion, 1,800 for the softmax); with the loads left out
-// it takes as long.  HBM could bring a tile in 1,400.  8 rows of 17,000 to 32,768 keys: 43.7 us and 4.3 to merge (105 MB: 2.2 TB/s, 0.33 of the
-// measured copy).  Tried: raw tiles by the copy engine, converted out of shared memory (296 KB a tile are 2,310 cycles and leave room for two
-// fp16 tiles only: no faster); sixteen converting warps, registers moved to the softmax (47.1 us); one tile ahead (46.6; splits of two tiles
-// 0.2 us faster); rows asked for in L2 three tiles ahead (slower); 16 bytes of two neighbouring keys a lane in place of the exchange of words
-// (64-byte pieces: slower).
+// 24 KB) and the schedulers 1,500 (6,000 instructions of warps a tile: 2,600 for the conversion, 1,800 for the softmax).  Measured with parts left
+// out: loads 2,400, the softmax's arithmetic 2,330, the conversion's 2,320 to 2,450, both 2,040, three quarters of P V's products 2,290: what is over
+// the 1,810 is spread over all of them.  HBM could bring a tile in 1,400.  8 rows of 17,000 to 32,768 keys: 41.4 to 43.4 us and 4.3 to merge (105 MB: 2.5
+// TB/s, 0.37 of the measured copy).  Tried: raw tiles by the copy engine, converted out of shared memory (296 KB a tile are 2,310 cycles and leave
+// room for two fp16 tiles only: no faster); sixteen converting warps, registers moved to the softmax (47.1 us against 43.7); one tile ahead (46.6;
+// splits of two tiles 0.2 us faster); rows asked for in L2 three tiles ahead (slower); 16 bytes of two neighbouring keys a lane in place of the
+// exchange of words (64-byte pieces: slower); softmax warps whose heads are all past the end of 16 or 32 left idle (16 heads 16.7 -> 16.4 us, 64
+// heads 41.4 -> 41.7); the merge released at entry or ahead of the epilogue (one row over 5,001 keys 11.3 -> 11.8, 8 rows 51.0 -> 54.4).
 #include <cuda.h>   // CUtensorMap
 
 #include "latent8.cuh"
