@@ -61,6 +61,7 @@ static int simt_auto_splits(int m, int n_heads, int n_keys) {
 
 template <int FMT>
 static int launch_simt_as(const MlaArgs& a, const MlaPaged& pg, cudaStream_t s) {
+  if (a.m > 65535) return HK_ERR_UNSUPPORTED;              // a row is a CTA's z
   static bool attr_set[64] = {false};
   int dev = 0;
   cudaGetDevice(&dev);

@@ -120,3 +120,8 @@ def test_tensors_of_another_type_layout_or_size_raise(lib):
     for args in (("hfil", names, *ok[:-1]), ("hfi", names, *ok), (3, names, *ok), ("hfil", list(names), *ok), ()):
         with pytest.raises(TypeError):
             nb.tensors(*args)
+
+
+def test_more_rows_than_the_cuda_core_kernel_takes(lib):
+    """heads other than 64 over the fp16 cache: refused on the host, not by a launch that fails"""
+    assert call(lib, "hk_mla_window", WINDOW, m=70000, n_heads=16, kv_len=A, kv_base=A, n_split=1) == hk.HK_ERR_UNSUPPORTED
