@@ -37,10 +37,11 @@ struct AppendArgs {
 // One CTA of sixteen warps a block that gets rows; grid (blocks of a sequence, sequences).  A warp has rows w, w + 16, ... of the block, a lane the
 // channels 4 lane .. + 3 of each quarter of a row (16-byte loads, 4-byte stores, whole lines both).  Up to four rows a warp stay in registers
 // between the largest magnitude and the rounding (KEEP); a block of 128 tokens is read twice, the second time from L2.
-// PARTS: chunks share a block of 64 or 128 tokens out over the CTAs of a cluster, 32 or 64 rows each, which exchange their largest magnitudes (4,096
-// rows, us: blocks of 64 by one CTA / two 6.9 / 5.8; blocks of 128 by one / four 13.1 / 5.9), as long as the CTAs fit the SMs at once (8,192 rows:
-// blocks of 64 by one / two 7.1 / 11.2; blocks of 128 by one / two / four 16.4 / 8.4 / 11.4; 20,000 rows, blocks of 128, one / two 20.1 / 23.1).
-// Under 64 rows the barrier of the cluster costs what it gains (32 rows in blocks of 64, one / two 4.0 / 4.7).
+// PARTS: chunks share a block of 64 or 128 tokens out over the CTAs of a cluster, which exchange their largest magnitudes.  A block of 64 over four CTAs,
+// a row a warp, as long as two of them an SM are enough: one / two / four CTAs, us, 1,000 rows 6.7 / 5.5 / 4.6, 4,096 6.9 / 5.85 / 5.5, 8,192 (516 CTAs)
+// 7.1 / 11.2 / 10.2.  A block of 128 over eight, four or two, the most that the SMs have room for at once: one / four / eight, 1,000 rows 12.7 / 5.5 / 5.25,
+// 4,096 (264 CTAs) 13.1 / 5.85 / 6.9; 8,192 by one / two / four 16.4 / 8.4 / 11.4, 20,000 by one / two 20.1 / 23.1.  Under 64 rows the barrier
+// of the cluster costs what it gains (32 rows in blocks of 64, one / two 4.0 / 4.7).
 constexpr int APPEND_WARPS = 16;
 template <int FMT, int ROWS, bool KEEP, int PARTS>
 __global__ void __launch_bounds__(APPEND_WARPS * 32) mla8_append_kernel(AppendArgs a) {
@@ -187,8 +188,9 @@ template <int FMT>
 cudaError_t append_launch(const AppendArgs& a, dim3 grid, int parts, cudaStream_t s) {
   const auto kernel = a.pg.shift == 4 ? mla8_append_kernel<FMT, 1, true, 1>
                       : a.pg.shift == 5 ? mla8_append_kernel<FMT, 2, true, 1>
-                      : a.pg.shift == 6 ? (parts > 1 ? mla8_append_kernel<FMT, 2, true, 2> : mla8_append_kernel<FMT, 4, true, 1>)
-                                        : (parts == 4   ? mla8_append_kernel<FMT, 2, true, 4>
+                      : a.pg.shift == 6 ? (parts > 1 ? mla8_append_kernel<FMT, 1, true, 4> : mla8_append_kernel<FMT, 4, true, 1>)
+                                        : (parts == 8   ? mla8_append_kernel<FMT, 1, true, 8>
+                                           : parts == 4 ? mla8_append_kernel<FMT, 2, true, 4>
                                            : parts == 2 ? mla8_append_kernel<FMT, 4, true, 2> : mla8_append_kernel<FMT, 8, false, 1>);
   return pdl_launch_cluster(parts, kernel, dim3(grid.x * parts, grid.y), dim3(APPEND_WARPS * 32), 0, s, a);
 }
@@ -302,8 +304,9 @@ HK_API int hk_mla8_append(const float* kv_pre, const void* ln_w_f16, void* ckv8,
   const dim3 grid((unsigned)blocks, (unsigned)n_seqs);
   int parts = 1;
   if (n / n_seqs >= 64 && block > 32) {
-    const int64_t ctas = (int64_t)blocks * n_seqs, least = ctas <= sm_count() ? block / 64 : 1;
-    for (parts = block / 32; parts > least && ctas * parts > sm_count();) parts /= 2;
+    const int64_t ctas = (int64_t)blocks * n_seqs;
+    if (block == 64) parts = 4 * ctas <= 2 * sm_count() ? 4 : 1;
+    else parts = 8 * ctas <= sm_count() ? 8 : 4 * ctas <= sm_count() ? 4 : ctas <= sm_count() ? 2 : 1;
   }
   return (dtype == HK_I8 ? append_launch<CACHE_I8>(a, grid, parts, as_stream(stream)) : append_launch<CACHE_E4M3>(a, grid, parts, as_stream(stream))) ==
                  cudaSuccess

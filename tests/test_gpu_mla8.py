@@ -72,9 +72,9 @@ def test_append(kind, block, pos, rows):
 
 
 @pytest.mark.parametrize("kind,block,pos,rows", [("i8", 64, [37], [1000]), ("e4m3", 64, [50], [6000]), ("i8", 128, [100], [1500]), ("e4m3", 128, [77], [5000]),
-                                                 ("i8", 128, [1], [19200]), ("i8", 128, [70, 0, 9], [30, 900, 0]), ("e4m3", 64, [63, 33, 9], [2, 0, 700])])
+                                                 ("i8", 128, [1], [19200]), ("i8", 128, [70, 0, 9], [30, 900, 0]), ("e4m3", 128, [33], [8000]), ("i8", 64, [5], [9000]), ("i8", 128, [17], [64]), ("e4m3", 64, [63, 33, 9], [2, 0, 700])])
 def test_append_of_blocks_shared_out_over_ctas(kind, block, pos, rows):
-    """blocks of 64 and 128 tokens by one CTA, two and four; a row that is not finite makes its whole block NaN, whichever CTA has it"""
+    """blocks of 64 and 128 tokens by one CTA, two, four and eight; a row that is not finite makes its whole block NaN, whichever CTA has it"""
     gen = gen_of(sum(rows))
     starts = [0]
     for r in rows:
