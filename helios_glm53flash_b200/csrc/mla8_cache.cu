@@ -123,6 +123,7 @@ __global__ void __launch_bounds__(APPEND_WARPS * 32) mla8_append_kernel(AppendAr
     amax = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(s_amax[turn][lane % APPEND_WARPS])));
     if (PARTS > 1) {
       if (threadIdx.x == 0) s_part[turn] = amax;
+      __syncwarp();                                        // whole warps arrive: split ones did not meet
       asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");   // every CTA of the block likewise
 #pragma unroll
       for (int k = 0; k < PARTS; k++) {
@@ -181,6 +182,7 @@ __global__ void __launch_bounds__(APPEND_WARPS * 32) mla8_append_kernel(AppendAr
       }
     }
   }
+  __syncwarp();
   if (PARTS > 1) asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");   // nobody reads this CTA's maximum any more
 }
 
