@@ -4,9 +4,12 @@
 //   S = (Q K8^T) s_key scale,  P = softmax numerators,  O = (P s_key) K8 / sum P        K8: the 8-bit values, s_key: their block's scale
 //
 // int8 and e4m3 values are exact in fp16, so the tensor cores multiply them as fp16 and the scales stay outside: fp32 factors of a score's
-// column, and of a weight before it is rounded to fp16.  That rounding is relative to the largest scale met so far, as the exponentials are
-// relative to the largest score: O is rescaled when a block's scale is more than 16 times the reference (and the scores' when one is over by
-// 2^8), so a weight stays below 2^12, and one that underflows weighs nothing next to what moved the references.
+// column, and of a weight before it is rounded to fp16.  A head has two references: of its scores, which the exponentials and their sum are relative
+// to, and of score + log2(scale), which the weights are relative to, as what a key adds to O is its probability times its scale: a block of large
+// scale that weighs nothing leaves the others their bits.  Either moves when it is exceeded by 2^8, so a weight stays at 2^8 and below.  The second
+// one's maximum is taken key by key only where a tile's scales differ by more than 16 times (8 rows of 18,432 to 32,768 keys of which every tile's do
+// 47.8 us, of one scale 44.2); elsewhere it is the largest score with the largest scale, so that the largest weight is 2^-4 at least and one that
+// underflows (2^-25) is 2^-21 of it.
 //
 // Work item = (query row, 64 heads, key split) -> one CTA.  Roles, tensor-memory plan and products are those of mla_flash_tc_kernel; what is
 // its own are eight warps in place of the copy engine, which load tiles of 64 keys x 512 bytes into registers two ahead, turn them into fp16
@@ -45,7 +48,8 @@ constexpr int F8_CONV_WARPS = 8, F8_ROWS = F8_KEYS / F8_CONV_WARPS, F8_THREADS =
 constexpr int F8_SHARE_ROWS = 32, F8_SHARE_SPLITS = 160;   // rows whose splits are shared out on the device, and splits of one row then at most
 constexpr int F8_MIN_TILES = 2;                   // tiles that a split is worth
 constexpr float F8_LOG2E = 1.4426950408889634f;
-constexpr float F8_MOVE = 8.0f, F8_MOVE_SCALE = 16.0f;
+constexpr float F8_MOVE = 8.0f, F8_EVEN = 16.0f;
+constexpr float F8_LEAST_SCALE = 7.888609e-31f;   // 2^-100: what smaller scales count as, in the weights' reference alone
 
 struct F8Misc {
   uint64_t full[F8_NBUF], free[F8_NBUF];          // tile slot: converted, may be overwritten
@@ -406,13 +410,15 @@ __global__ __launch_bounds__(F8_THREADS, 1) void mla8_flash_tc_kernel(MlaArgs a,
       tc::fence_before_sync();
       tc::mbar_arrive(&ms.q_ready);
     }
-    float m = -INFINITY, l = 0.f, sref = 0.f, inv = 0.f;   // references: of the scores (log2), of the scales
+    float m = -INFINITY, l = 0.f, w_ref = -INFINITY, g = 0.f;   // references: of the scores, of the weights (log2); 2^(m - w_ref)
     for (int t = 0; t < n_tiles; t++) {
       const int b = t & 1, kb = t % F8_NBUF;
       ok = tc::mbar_wait<F8_POLL_NS>(&ms.full[kb], (t / F8_NBUF) & 1, abort_flag, 47) && ok;   // makes the scales visible
       const float sc_lo = ms.sc[kb][lane], sc_hi = ms.sc[kb][lane + 32];
       const bool hidden = __any_sync(0xffffffffu, fminf(sc_lo, sc_hi) < 0.f);
       const float top = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(fmaxf(fmaxf(sc_lo, sc_hi), 0.f))));
+      const uint32_t least = __reduce_min_sync(0xffffffffu, min(__float_as_uint(sc_lo), __float_as_uint(sc_hi)));   // (-1 is above them all as an integer)
+      const bool uneven = least < 0x7f800000u && __uint_as_float(least) * F8_EVEN < top;   // the same for all threads
       ok = tc::mbar_wait<F8_POLL_NS>(&ms.s_full[b], (t >> 1) & 1, abort_flag, 48) && ok;
       tc::fence_after_sync();
       uint32_t sv[32];
@@ -446,21 +452,31 @@ __global__ __launch_bounds__(F8_THREADS, 1) void mla8_flash_tc_kernel(MlaArgs a,
       ms.mx[b][tid] = tmax;
       asm volatile("bar.sync %0, 64;" ::"r"(1 + (warp & 1)) : "memory");   // the two warps of these heads
       tmax = fmaxf(tmax, ms.mx[b][tid ^ 64]);
+      float wmax = tmax + __log2f(fmaxf(top, F8_LEAST_SCALE));
+      if (uneven) {
+        const float* own = &ms.sc[kb][32 * half];
+        wmax = -INFINITY;
+#pragma unroll
+        for (int j = 0; j < 32; j++) wmax = fmaxf(wmax, __uint_as_float(sv[j]) + __log2f(fmaxf(own[j], F8_LEAST_SCALE)));
+        asm volatile("bar.sync %0, 64;" ::"r"(1 + (warp & 1)) : "memory");   // the maxima above have been read
+        ms.mx[b][tid] = wmax;
+        asm volatile("bar.sync %0, 64;" ::"r"(1 + (warp & 1)) : "memory");
+        wmax = fmaxf(wmax, ms.mx[b][tid ^ 64]);
+      }
       const bool move = tmax > m + F8_MOVE || (m == -INFINITY && tmax > -INFINITY);
-      const bool move_sc = top > sref * F8_MOVE_SCALE;     // the same for all threads
+      const bool move_w = wmax > w_ref + F8_MOVE || (w_ref == -INFINITY && wmax > -INFINITY);
       float alpha = 1.f;
       if (move) {
-        alpha = m == -INFINITY ? 0.f : exp2f(m - tmax);
+        l *= m == -INFINITY ? 0.f : exp2f(m - tmax);
         m = tmax;
-        l *= alpha;
       }
-      if (move_sc) {
-        alpha *= sref * __fdiv_rn(1.f, top);
-        sref = top;
-        inv = top > 1e-30f ? __fdiv_rn(1.f, top) : 0.f;
+      if (move_w) {
+        alpha = w_ref == -INFINITY ? 0.f : exp2f(w_ref - wmax);
+        w_ref = wmax;
       }
-      if (t > 0 && __any_sync(0xffffffffu, move || move_sc)) {
-        // rare: a reference moved.  O is rescaled after the tile before has been added and before this one is
+      if (move || move_w) g = exp2f(m - w_ref);
+      if (t > 0 && __any_sync(0xffffffffu, move_w)) {
+        // rare: a head's weights' reference moved.  O is rescaled after the tile before has been added and before this one is
         wait_pv(t - 1, 49);
         tc::fence_after_sync();
 #pragma unroll 1
@@ -477,7 +493,7 @@ __global__ __launch_bounds__(F8_THREADS, 1) void mla8_flash_tc_kernel(MlaArgs a,
       if (t >= 2) wait_pv(t - 2, 50);                      // this parity's P has been read
       uint8_t* prow = smem + F8S_P + b * F8_P_BYTES;
       const float mref = m == -INFINITY ? 0.f : m;         // no key so far: exp2(-inf) = 0 below
-      const uint64_t neg = pack2(-mref, -mref), one = pack2(1.f, 1.f), inv2 = pack2(inv, inv);
+      const uint64_t neg = pack2(-mref, -mref), one = pack2(1.f, 1.f), g2 = pack2(g, g);
       uint64_t sum[2] = {0, 0};
 #pragma unroll
       for (int v = 0; v < 4; v++) {
@@ -491,7 +507,7 @@ __global__ __launch_bounds__(F8_THREADS, 1) void mla8_flash_tc_kernel(MlaArgs a,
           unpack2(fma2(pack2(__uint_as_float(sv[j]), __uint_as_float(sv[j + 1])), one, neg), x0, x1);
           const uint64_t p = pack2(exp2f(x0), exp2f(x1));
           sum[e & 1] = fma2(p, one, sum[e & 1]);
-          unpack2(mul2(p, mul2(e & 1 ? k[e >> 1].y : k[e >> 1].x, inv2)), x0, x1);
+          unpack2(mul2(mul2(p, g2), e & 1 ? k[e >> 1].y : k[e >> 1].x), x0, x1);   // (a scale times g could overflow)
           const __half2 hp = __floats2half2_rn(x0, x1);
           wp[e] = *reinterpret_cast<const uint32_t*>(&hp);
         }
@@ -514,7 +530,8 @@ __global__ __launch_bounds__(F8_THREADS, 1) void mla8_flash_tc_kernel(MlaArgs a,
     const bool none = l == 0.f;                            // (NaN: a score was none)
     if (half == 0) {
       // NaN has to reach the merge, which weighs a split of nothing else 0
-      ms.mx[(n_tiles + 1) & 1][head] = none ? 0.f : final_out ? sref / l : l == l ? sref : l;
+      const float unit = exp2f(w_ref - m);                 // O in units of the scores' reference
+      ms.mx[(n_tiles + 1) & 1][head] = none ? 0.f : final_out ? unit / l : l == l ? unit : l;
       if (!final_out && it.r >= 0 && it.part == 0 && head < n_h) {
         const size_t at = part_row + head;
         a.part_m[at] = m == -INFINITY || none ? -INFINITY : m / F8_LOG2E;

@@ -1,0 +1,122 @@
+"""What the header promises of the 8-bit cache and of windows where ordinary inputs do not go."""
+import pytest
+import torch
+
+import helios_glm53flash_b200 as hk
+from latent8_ref import STORE, TOP, cache, rows_of, visible
+from test_gpu_mla8 import close, finish, gen_of, ints, queries
+
+pytestmark = pytest.mark.gpu
+
+
+# ---------------------------------------------------------------------------------------------
+# blocks of very unequal scales
+# ---------------------------------------------------------------------------------------------
+def attend_by_weight(q, keys, key_scale, top, scale):
+    """q [heads][512], keys [n][512] in 64 bits, key_scale [n]: their blocks' scales -> (output, what it may be off by), by the keys that weigh.
+
+    A score is an fp32 sum of 512 products, scaled twice: 520 roundings at most of relative 2^-24 of its own key's sum of magnitudes, and 2^-20 of
+    itself and of 1 for the exponential; that moves its weight relatively by as much.  A weight times its key's scale is rounded to fp16: half a
+    step, 2^-11, relative, or 2^-25 of the reference where that leaves fp16's normal range; the reference is at most 2^4 of the largest product of
+    the two.  The sum of n weights in fp32 adds n 2^-24, the output's own rounding 2^-11 or half of fp16's smallest step, 2^-25."""
+    s = q @ keys.T * scale
+    p = torch.exp(s - s.amax(1, keepdim=True))
+    tot = p.sum(1, keepdim=True)
+    o = p @ keys / tot
+    eta = torch.expm1((2.0 ** -24 * 520 * (q.abs() @ keys.abs().T) * scale + 2.0 ** -20 * (1 + s.abs())).clamp(max=500.0))
+    moved = p * torch.where(p > 0, eta, torch.zeros_like(eta))
+    mag = p @ keys.abs() / tot
+    tol = (moved @ keys.abs() + moved.sum(1, keepdim=True) * o.abs()) / tot + keys.shape[0] * 2.0 ** -24 * o.abs()
+    least = keys.shape[0] * 2.0 ** -21 * (p * key_scale).amax(1, keepdim=True) * top / tot
+    return o, (tol + 2.0 ** -11 * (mag + o.abs()) + least) * 1.01 + 2.0 ** -25
+
+
+def unequal(gen, kind, block, blocks, heads, m, big, small, low):
+    """a sequence of `blocks` blocks, every third of the scale `big`, the others of `small`; queries that score the big blocks' keys lower by about
+    `low` by one channel, in which all heads are 2; a big block's other values are in channels where the queries are 0"""
+    top = TOP[kind]
+    v = torch.randn(blocks, block, 512, device="cuda", generator=gen).clamp(-3, 3) * (top / 3)
+    heavy = torch.arange(blocks, device="cuda") % 3 == 1
+    v[heavy, :, :256] = 0.0
+    v[heavy, :, 7] = -round(low / (0.0625 * 2 * big)) if kind == "i8" else -low / (0.0625 * 2 * big)
+    ckv8 = (v.round() if kind == "i8" else v).to(STORE[kind])
+    scales = torch.where(heavy, big, small).float()
+    q = torch.randn(m, heads, 512, device="cuda", generator=gen) * 0.7
+    q[:, :, 7] = 2.0
+    q[:, :, 256:] = 0.0
+    return ckv8, scales, q.half()
+
+
+@pytest.mark.parametrize("kind", ["i8", "e4m3"])
+@pytest.mark.parametrize("block", [16, 32, 64, 128])                # several blocks a tile of 64 keys, one, half of one
+@pytest.mark.parametrize("big,small,low", [(100.0, 1e-3, 12.5), (100.0, 1e-4, 37.5), (100.0, 1e-5, 400), (100.0, 1e-5, 25), (1e4, 1e-3, 1250), (2e4, 3e-4, 2500)])
+def test_blocks_that_weigh_keep_their_bits_beside_blocks_of_large_scale(kind, block, big, small, low):
+    """large-scale blocks far below in score, or so that both weigh; decode, one CTA and several, fewer heads, gathered positions, a short chunk"""
+    gen = gen_of(block + int(low))
+    n, m = 700, 3
+    blocks = (n + block - 1) // block
+    ckv8, scales, q = unequal(gen, kind, block, blocks, 64, m, big, small, low)
+    where = torch.randperm(blocks, device="cuda", generator=gen)
+    pool, pool_s = torch.empty_like(ckv8.view(torch.uint8)), torch.empty_like(scales)
+    pool[where], pool_s[where] = ckv8.view(torch.uint8), scales
+    pool, table = pool.view(STORE[kind]), where.to(torch.int32)[None].contiguous()
+    out = torch.empty(m, 64, 512, dtype=torch.float16, device="cuda")
+    lens = [n, n - 1, block + 1]
+
+    def check(got, row, p, heads):
+        keys, ks = rows_of(pool, pool_s, table[0], p), pool_s[table[0][p // block].long()].double()
+        close(got[row:row + 1], [attend_by_weight(q[row, :heads].double(), keys, ks, TOP[kind], 0.0625)])
+
+    for heads, n_split in ((64, 0), (64, 1), (64, 4), (16, 0)):
+        qh, oh = q[:, :heads].contiguous(), out[:, :heads].contiguous()
+        hk.mla8_dense_prefill(qh, pool, pool_s, oh, m, 0, n_heads=heads, block_table=table, kv_len=ints(lens), n_keys_hint=n, n_split=n_split)
+        finish()
+        for r in range(m):
+            check(oh, r, visible(lens[r], 0, 0), heads)
+    hk.mla8_dense_prefill(q, pool, pool_s, out, m, 0, block_table=table, kv_len=ints(lens), n_keys_hint=1 << 20)         # shared out by length
+    finish()
+    for r in range(m):
+        check(out, r, visible(lens[r], 0, 0), 64)
+    hk.mla8_dense_prefill(q, pool, pool_s, out, m, n - m, block_table=table, window=300, sinks=3)
+    finish()
+    for r in range(m):
+        check(out, r, visible(n - m + r + 1, 300, 3), 64)
+    idx = torch.randint(0, n, (m, 333), device="cuda", generator=gen, dtype=torch.int32)
+    for n_split in (0, 1):
+        hk.mla8_sparse_decode(q, pool, pool_s, idx, 333, out, m, block_table=table, n_split=n_split)
+        finish()
+        for r in range(m):
+            check(out, r, idx[r].long(), 64)
+
+
+@pytest.mark.parametrize("kind", ["i8", "e4m3"])
+@pytest.mark.parametrize("big,low", [(0.5, 6.0), (10.0, 12.5)])
+def test_keys_of_zeros_that_score_highest(kind, big, low):
+    """blocks of scale 0 have the score 0, the only keys with values score far below: those weigh little, and what they weigh is right"""
+    gen, block, n = gen_of(61), 16, 600
+    blocks = (n + block - 1) // block
+    ckv8, scales, q = unequal(gen, kind, block, blocks, 64, 2, big, 0.0, low)
+    out = torch.empty(2, 64, 512, dtype=torch.float16, device="cuda")
+    for n_split in (0, 1, 3):
+        hk.mla8_dense_prefill(q, ckv8, scales, out, 2, n - 2, n_split=n_split)
+        finish()
+        want = []
+        for r in range(2):
+            p = visible(n - 1 + r, 0, 0)
+            want.append(attend_by_weight(q[r].double(), rows_of(ckv8, scales, torch.arange(blocks, device="cuda"), p), scales[p // block].double(), TOP[kind], 0.0625))
+        close(out, want)
+
+
+@pytest.mark.parametrize("kind", ["i8", "e4m3"])
+@pytest.mark.parametrize("small", [1e-39, 3e-38, 1e-31, 1e-29])
+def test_blocks_of_zeros_before_blocks_of_the_smallest_scales(kind, small):
+    gen = gen_of(62)
+    ckv8, _ = cache(gen, kind, 4, 64)
+    q, out = queries(gen, 1, 64), torch.empty(1, 64, 512, dtype=torch.float16, device="cuda")
+    for s in ([0.0, small, small, 0.0], [0.0, small, 1.0, small], [small, small, 0.0, 1.0], [0.0, 0.0, 0.0, small]):
+        scales = torch.tensor(s, device="cuda")
+        for n_split in (1, 2, 4):
+            hk.mla8_dense_prefill(q, ckv8, scales, out, 1, 255, n_split=n_split)
+            finish()
+            p = torch.arange(256, device="cuda")
+            close(out, [attend_by_weight(q[0].double(), rows_of(ckv8, scales, torch.arange(4, device="cuda"), p), scales[p // 64].double(), TOP[kind], 0.0625)])
