@@ -26,7 +26,7 @@ struct MlaArgs {
   // n_split == 0 (8-bit cache): splits shared out on the device among `units` CTAs, whose first and number each row's first CTA stores
   int units;
   int2* shares;
-  int keep_nan;             // scores that are no numbers make outputs that are none (0: zeros, as the fp16 cache's callers know it)
+  int keep_nan;             // keys that are not finite make outputs that are NaN (0: zeros where the scores are, as hk_mla_dense's callers know it)
 };
 
 // The 8-bit latent cache: blocks of `1 << shift` tokens x 512 values, one fp32 scale a block; a key is scale * value.

@@ -669,6 +669,7 @@ HK_API int hk_mla_window(const void* q_lat, const void* ckv, int64_t ckv_rows, c
   a.m = m; a.n_heads = n_heads; a.scale = scale;
   a.out = (__half*)lat_out;
   a.window = window; a.sinks = sinks;
+  a.keep_nan = 1;
   return attend(a, mla_window_keys(kv_len ? pos_start : pos_start + m, window, sinks), n_split, n_split <= 0, workspace, workspace_bytes,
                 as_stream(stream));
 }

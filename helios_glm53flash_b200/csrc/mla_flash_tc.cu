@@ -570,8 +570,9 @@ __global__ __launch_bounds__(FT_THREADS, 1) void mla_flash_tc_kernel(
       tc::fence_after_sync();
       asm volatile("bar.sync 3, 128;" ::: "memory");
       l += ms.l[tid ^ 64];
-      const bool some = l > 0.f || (a.keep_nan && l != 0.f);
-      const float f = some ? (final_out && !CL ? 1.f / l : 1.f) : 0.f;
+      // keep_nan: sums that are zero or NaN leave O as it is, zeros where nothing was seen, NaN from a key that is not finite
+      const bool some = l > 0.f || (a.keep_nan && it.n_tiles > 0);
+      const float f = final_out && !CL && l > 0.f ? 1.f / l : 1.f;
       if (CL) cluster_arrive();                            // this CTA's ring is idle
       auto load_o = [&](int c0, uint32_t (&o)[32]) {       // 32 of this thread's 256 channels, weighed
         if (it.n_tiles > 0) {

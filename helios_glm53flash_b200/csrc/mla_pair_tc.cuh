@@ -433,8 +433,8 @@ __global__ __launch_bounds__(PT_THREADS, 1) void mla_pair_tc_kernel(
     tc::fence_after_sync();
     asm volatile("bar.sync 3, 128;" ::: "memory");
     l += ms.l[tid ^ 64];
-    const bool some = l > 0.f || (a.keep_nan && l != 0.f);
-    const float f = some ? 1.f / l : 0.f;
+    const bool some = l > 0.f || a.keep_nan;               // as in mla_flash_tc_kernel
+    const float f = l > 0.f ? 1.f / l : 1.f;
 #pragma unroll 1
     for (int c0 = 0; c0 < 256; c0 += 64) {
       uint8_t* box = smem + FS_P + half * FP_BYTES;

@@ -121,6 +121,7 @@ __global__ __launch_bounds__(256) void mla_simt_kernel(MlaArgs a, MlaPaged pg) {
   }
   __syncthreads();
   const size_t rows = (size_t)a.m * a.n_heads;
+  const bool keep_nan = FMT != CACHE_F16 || a.keep_nan;
   for (int idx = threadIdx.x; idx < SIMT_HG * LATENT; idx += 256) {
     const int h = idx / LATENT, ch = idx % LATENT;
     float gm = -INFINITY;
@@ -135,14 +136,14 @@ __global__ __launch_bounds__(256) void mla_simt_kernel(MlaArgs a, MlaPaged pg) {
         gl += sc * w_l[w * SIMT_HG + h];
         o += sc * w_acc[(w * SIMT_HG + h) * LATENT + ch];
       }
-    } else if (FMT != CACHE_F16) {                         // no key, or scores that are no numbers: NaN stays NaN
+    } else if (keep_nan) {                                 // no key, or scores that are no numbers: NaN stays NaN
 #pragma unroll
       for (int w = 0; w < 8; w++) gl += w_l[w * SIMT_HG + h];
       o = gl;
     }
     const size_t rh = (size_t)r * a.n_heads + h0 + h;
     if (a.out) {
-      a.out[rh * LATENT + ch] = __float2half_rn(gl > 0.f || (FMT != CACHE_F16 && gl != 0.f) ? o / gl : 0.f);
+      a.out[rh * LATENT + ch] = __float2half_rn(gl > 0.f || (keep_nan && gl != 0.f) ? o / gl : 0.f);
     } else {
       a.part_acc[((size_t)sp * rows + rh) * LATENT + ch] = o;
       if (ch == 0) {

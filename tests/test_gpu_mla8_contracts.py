@@ -1,9 +1,11 @@
 """What the header promises of the 8-bit cache and of windows where ordinary inputs do not go."""
+import math
+
 import pytest
 import torch
 
 import helios_glm53flash_b200 as hk
-from latent8_ref import STORE, TOP, cache, rows_of, visible
+from latent8_ref import STORE, TOP, attend, cache, rows_of, visible
 from test_gpu_mla8 import close, finish, gen_of, ints, queries
 
 pytestmark = pytest.mark.gpu
@@ -120,3 +122,56 @@ def test_blocks_of_zeros_before_blocks_of_the_smallest_scales(kind, small):
             finish()
             p = torch.arange(256, device="cuda")
             close(out, [attend_by_weight(q[0].double(), rows_of(ckv8, scales, torch.arange(4, device="cuda"), p), scales[p // 64].double(), TOP[kind], 0.0625)])
+
+
+# ---------------------------------------------------------------------------------------------
+# keys that are not finite under a window
+# ---------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("heads,rows,window,n_split,pos", [
+    (64, 1, 100, 0, 800), (64, 1, 1000, 0, 1700), (64, 1, 3000, 0, 4000), (64, 1, 9000, 0, 9500), (64, 1, 1000, 1, 1700), (64, 1, 1000, 3, 1700), (64, 5, 700, 0, 1100),
+    (64, 30, 300, 0, 600), (64, 200, 300, 0, 600), (64, 7, 2500, 1, 3000), (64, 40, 2500, 0, 3000), (16, 1, 100, 0, 800), (16, 3, 1000, 1, 1500), (16, 3, 1000, 4, 1500)])
+def test_window_rows_that_see_a_key_that_is_not_finite(heads, rows, window, n_split, pos):
+    """one CTA a row, a grid that walks rows, splits of every kind, clusters, pairs, the CUDA cores: a key with a NaN makes every channel of the rows
+    that see it NaN, one with an infinity its own channels; other rows are as they would be without it.  At the window's first key, whose score can
+    be the only one of a split, in its middle and at the row's own"""
+    gen, sinks = gen_of(rows + window), 3
+    clean = torch.randn(pos + rows, 512, device="cuda", generator=gen).half()
+    q = queries(gen, rows, heads)
+    q[:, :, 9] = 0.5                                           # the infinite channel: every head scores it the same way
+    out = torch.empty(rows, heads, 512, dtype=torch.float16, device="cuda")
+    lo, last = pos + rows - window, pos + rows - 1             # the last row's first and own key
+    sees = lambda p: torch.tensor([p < sinks or pos + r + 1 - window <= p <= pos + r for r in range(rows)], device="cuda")
+    for p in (1, lo, lo + window // 2, last):
+        for bad, whole in ((math.nan, True), (math.nan, False), (math.inf, False), (-math.inf, False), (math.inf, True)):
+            ckv = clean.clone()
+            ckv[p, slice(None) if whole else 9] = bad
+            hk.mla_window_prefill(q, ckv, out.zero_(), rows, pos, window, sinks=sinks, n_heads=heads, n_split=n_split)
+            finish()
+            hit = sees(p)
+            if math.isnan(bad) or whole:
+                assert torch.isnan(out[hit]).all(), (p, bad)
+            else:
+                assert not torch.isfinite(out[hit][:, :, 9]).any(), (p, bad)
+            for r in torch.nonzero(~hit)[:, 0].tolist()[::7]:
+                o, tol = attend(q[r].double(), ckv[:pos + r + 1][visible(pos + r + 1, window, sinks)].double(), 0.0625)
+                assert bool(((out[r].double() - o).abs() <= tol).all()), (p, bad, r)
+
+
+def test_window_rows_of_one_key_that_is_not_finite():
+    """nothing else to see: an infinity that scores plus or minus infinity, a NaN; as a row's only split and as one of several"""
+    gen = gen_of(71)
+    ckv = torch.randn(400, 512, device="cuda", generator=gen).half()
+    q = queries(gen, 1, 64)
+    q[:, :, 9] = 0.5
+    out = torch.empty(1, 64, 512, dtype=torch.float16, device="cuda")
+    for bad in (math.inf, -math.inf, math.nan):
+        ckv[399, 9] = bad
+        for n_split in (0, 1, 2):
+            hk.mla_window_prefill(q, ckv, out.zero_(), 1, 399, 1, n_split=n_split)
+            finish()
+            assert not torch.isfinite(out[:, :, 9]).any(), (bad, n_split)
+        ckv[399 - 15:399, 9] = bad                             # sixteen such keys alone in the last tile, and finite ones before them
+        for n_split in (0, 1, 7):
+            hk.mla_window_prefill(q, ckv, out.zero_(), 1, 399, 400, n_split=n_split)
+            finish()
+            assert not torch.isfinite(out[:, :, 9]).any(), (bad, n_split)
