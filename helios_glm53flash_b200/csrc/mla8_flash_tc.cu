@@ -557,7 +557,7 @@ __global__ __launch_bounds__(F8_THREADS, 1) void mla8_flash_tc_kernel(MlaArgs a,
         tc::tmem_ld_wait();
       }
 #pragma unroll
-      for (int j = 0; j < 32; j++) o[j] = f == 0.f ? 0u : __float_as_uint(__uint_as_float(o[j]) * f);
+      for (int j = 0; j < 32; j++) o[j] = n_tiles > 0 ? __float_as_uint(fmaf(__uint_as_float(o[j]), f, 0.f)) : 0u;   // (f 0: O is 0, or NaN)
       constexpr int span = PARTS == 4 ? 64 : 128;            // columns of a product: channels 2 span a product, span a lane half
       uint8_t* dst = orow + (c / span * 2 * span + half * span + c % span) * elem;
       if (final_out) {

@@ -175,3 +175,18 @@ def test_window_rows_of_one_key_that_is_not_finite():
             hk.mla_window_prefill(q, ckv, out.zero_(), 1, 399, 400, n_split=n_split)
             finish()
             assert not torch.isfinite(out[:, :, 9]).any(), (bad, n_split)
+
+
+@pytest.mark.parametrize("kind", ["i8", "e4m3"])
+def test_blocks_whose_scale_is_infinite(kind):
+    """every key's score is infinite or NaN, whichever split has it"""
+    gen = gen_of(72)
+    ckv8, scales = cache(gen, kind, 3, 64)
+    q, out = queries(gen, 1, 64), torch.empty(1, 64, 512, dtype=torch.float16, device="cuda")
+    for bad in ([0, 1, 2], [1], [2]):
+        s = scales.clone()
+        s[bad] = math.inf
+        for n_split in (1, 2, 3):
+            hk.mla8_dense_prefill(q, ckv8, s, out.zero_(), 1, 128, n_split=n_split)
+            finish()
+            assert torch.isnan(out).all(), (bad, n_split)
