@@ -1,5 +1,8 @@
 """What the header promises of the 8-bit cache and of windows where ordinary inputs do not go."""
 import math
+import os
+import subprocess
+import sys
 
 import pytest
 import torch
@@ -190,3 +193,17 @@ def test_blocks_whose_scale_is_infinite(kind):
             hk.mla8_dense_prefill(q, ckv8, s, out.zero_(), 1, 128, n_split=n_split)
             finish()
             assert torch.isnan(out).all(), (bad, n_split)
+
+
+# ---------------------------------------------------------------------------------------------
+# the CUDA-core kernel, streams, the same call again
+# ---------------------------------------------------------------------------------------------
+def test_the_cuda_core_kernel_over_the_8_bit_cache():
+    """the form for machines without an encoder of tensor maps, in a process of its own: holes, sequence numbers out of range, NaN scales, windows, splits"""
+    names = ("test_dense8_rows", "test_dense8_chunk", "test_dense8_rows_and_blocks_that_do_not_count", "test_a_row_that_is_not_finite_is_seen_in_the_output",
+             "test_splits_that_see_nothing", "test_sparse8", "test_window_rows", "test_dense8_without_a_table", "test_blocks_that_weigh", "test_keys_of_zeros")
+    here = os.path.dirname(os.path.abspath(__file__))
+    files = [os.path.join(here, f) for f in ("test_gpu_mla8.py", "test_gpu_mla8_contracts.py")]
+    run = subprocess.run([sys.executable, "-m", "pytest", "-x", "-q", "-m", "gpu", "-p", "no:cacheprovider", "-k", " or ".join(names)] + files,
+                         env={**os.environ, "HK_MLA_FORCE_SIMT": "1"}, capture_output=True, text=True, timeout=600)
+    assert run.returncode == 0, run.stdout[-3000:] + run.stderr[-2000:]
