@@ -8,7 +8,7 @@ import pytest
 import torch
 
 import helios_glm53flash_b200 as hk
-from latent8_ref import STORE, TOP, attend, cache, rows_of, visible
+from latent8_ref import STORE, TOP, attend, cache, rows_of, table_for, visible
 from test_gpu_mla8 import close, finish, gen_of, ints, queries
 
 pytestmark = pytest.mark.gpu
@@ -207,3 +207,38 @@ def test_the_cuda_core_kernel_over_the_8_bit_cache():
     run = subprocess.run([sys.executable, "-m", "pytest", "-x", "-q", "-m", "gpu", "-p", "no:cacheprovider", "-k", " or ".join(names)] + files,
                          env={**os.environ, "HK_MLA_FORCE_SIMT": "1"}, capture_output=True, text=True, timeout=600)
     assert run.returncode == 0, run.stdout[-3000:] + run.stderr[-2000:]
+
+
+def test_windowed_calls_on_two_streams_at_once():
+    gen = gen_of(32)
+    sides = [torch.cuda.Stream() for _ in range(2)]
+    states = [(torch.randn(3000, 512, device="cuda", generator=gen).half(), queries(gen, 2, 64), torch.empty(2, 64, 512, dtype=torch.float16, device="cuda")) for _ in sides]
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for stream, (ckv, q, out) in zip(sides, states):
+            with torch.cuda.stream(stream):
+                hk.mla_window_prefill(q, ckv, out, 2, 2998, 1000, sinks=3)
+    finish()
+    for ckv, q, out in states:
+        close(out, [attend(q[r].double(), ckv[:2999 + r][visible(2999 + r, 1000, 3)].double(), 0.0625) for r in range(2)])
+
+
+def test_the_same_call_gives_the_same_bits():
+    gen, block = gen_of(33), 32
+    ckv8, scales = cache(gen, "e4m3", 300, block, spread=1.0)
+    q, ckv = queries(gen, 40, 64), torch.randn(5000, 512, device="cuda", generator=gen).half()
+    table, lens = table_for(gen, 1, 300, 300), ints([9000 - 31 * i for i in range(40)])
+    idx = torch.randint(0, 9000, (40, 700), device="cuda", generator=gen, dtype=torch.int32)
+    got = []
+    for _ in range(3):
+        outs = [torch.empty(40, 64, 512, dtype=torch.float16, device="cuda") for _ in range(5)]
+        hk.mla8_dense_prefill(q, ckv8, scales, outs[0], 40, 0, block_table=table, kv_len=lens, n_keys_hint=9000)
+        hk.mla8_dense_prefill(q[:5], ckv8, scales, outs[1][:5], 5, 0, block_table=table, kv_len=lens[:5], n_keys_hint=9000)
+        hk.mla8_dense_prefill(q, ckv8, scales, outs[2], 40, 9000, block_table=table, window=500, sinks=9)
+        hk.mla8_sparse_decode(q, ckv8, scales, idx, 700, outs[3], 40, block_table=table)
+        hk.mla_window_prefill(q, ckv, outs[4], 40, 4900, 900, sinks=9)
+        outs[1][5:] = 0
+        finish()
+        got.append(outs)
+    for outs in got[1:]:
+        assert all(torch.equal(a, b) for a, b in zip(outs, got[0]))
