@@ -52,7 +52,7 @@ static bool force_simt() {
 static int simt_auto_splits(int m, int n_heads, int n_keys) {
   long ctas = (long)m * (n_heads / SIMT_HG);
   int want = (int)((2L * sm_count() + ctas - 1) / ctas);
-  int cap = (n_keys + 63) / 64;
+  int cap = n_keys / 64 + (n_keys % 64 != 0);
   int s = want < 1 ? 1 : want;
   if (s > cap) s = cap < 1 ? 1 : cap;
   if (s > 64) s = 64;
@@ -139,7 +139,7 @@ static int attend(MlaArgs a, int n_keys_hint, int n_split, bool choose, void* wo
     if (!aligned(workspace, 256)) return HK_ERR_INVALID;
     // Few rows of few tiles: one kernel whose clusters merge the splits.  The rows' tiles are known for gathered rows and causal
     // ranges; where each row has a length of its own on the device, fewer splits than the GPU has room for mean two tiles each.
-    const int tiles = a.raw_idx || !a.kv_len || a.window ? (n_keys_hint + 63) / 64 : (int64_t)a.m * (n_split + 1) <= sm_count() ? 2 * n_split : 1 << 20;
+    const int tiles = a.raw_idx || !a.kv_len || a.window ? n_keys_hint / 64 + (n_keys_hint % 64 != 0) : (int64_t)a.m * (n_split + 1) <= sm_count() ? 2 * n_split : 1 << 20;
     MlaArgs c = a;
     // That is the form for a call that has the GPU to itself: its 64 SMs where the splits alone are 17 CTAs cost several calls side by
     // side more than each gains, which the library cannot see and the caller says with a number of splits (a step of 11 MLA layers at
@@ -265,7 +265,7 @@ HK_API size_t hk_mla8_sparse_workspace_bytes(int m, int n_heads, int kidx, int64
 }
 
 HK_API size_t hk_mla8_dense_workspace_bytes(int m, int n_heads, int pos_start, int n_keys_hint, int window, int sinks, int per_row) {
-  if (m <= 0 || n_heads < hk::SIMT_HG || pos_start < 0 || sinks < 0) return 0;
+  if (m <= 0 || n_heads < hk::SIMT_HG || pos_start < 0 || sinks < 0 || (int64_t)pos_start + m > INT32_MAX) return 0;   // (a call that is refused)
   const int keys = hk::mla8_dense_keys(m, pos_start, n_keys_hint, window, sinks, per_row);
   const hk::ChunkPlan c = hk::chunk_plan(m, n_heads, pos_start, keys, window, sinks, per_row);
   if (c.on) {

@@ -732,7 +732,7 @@ int mla_flash_tc_auto_splits(int m, int n_keys) {
   // the merge, 1 / 2 / 3 tiles per split, us: 2,052 gathered rows of one query 12.1 / 11.3 / 12.7, of four 16.9 / 12.6 / 13.5 (more
   // partials to write and merge); dense, one row over 2,048 keys 11.8 / 11.2 / 12.7, over 8,192 15.4 / 13.6 / 14.9.
   const int sms = sm_count();
-  const int tiles = (n_keys + FT_KEYS - 1) / FT_KEYS;
+  const int tiles = n_keys / FT_KEYS + (n_keys % FT_KEYS != 0);
   int want = sms / (m > 0 ? m : 1);
   if (want > 256) want = 256;
   if (want < 1) want = 1;
