@@ -74,7 +74,7 @@ __device__ __forceinline__ F8Row f8_row(const MlaArgs& a, const MlaPaged& pg, in
   w.seq = pg.seq_of(r);
   w.keys = key_list(w.seq < 0 ? 0 : GATHER ? a.kidx : a.kv_len ? a.kv_len[r] : a.pos_start + r + 1, a.window, a.sinks);
   if (!GATHER) w.keys.cut(pg.room());                      // behind the table are no keys
-  w.head_tiles = (w.keys.head + F8_KEYS - 1) / F8_KEYS;
+  w.head_tiles = w.keys.head / F8_KEYS + (w.keys.head % F8_KEYS != 0);
   w.jump = max(w.keys.lo / F8_KEYS - w.head_tiles, 0);
   w.tiles = w.keys.n / F8_KEYS + (w.keys.n % F8_KEYS != 0) - w.jump;
   return w;

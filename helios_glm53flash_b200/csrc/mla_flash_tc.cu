@@ -142,7 +142,7 @@ __device__ __forceinline__ FtItem ft_item(const MlaArgs& a, int idx) {
   // split boundaries on tile granularity
   int tiles = (n + FT_KEYS - 1) / FT_KEYS;
   if (WIN) {                                               // (where the cache's end cuts the range, its last tiles may hold no key that is seen)
-    it.head_tiles = min((it.head + FT_KEYS - 1) / FT_KEYS, tiles);
+    it.head_tiles = min(it.head / FT_KEYS + (it.head % FT_KEYS != 0), tiles);
     it.jump = max(min(it.lo / FT_KEYS, tiles) - it.head_tiles, 0);
     tiles -= it.jump;
   }

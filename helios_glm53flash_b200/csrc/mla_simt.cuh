@@ -56,10 +56,11 @@ __global__ __launch_bounds__(256) void mla_simt_kernel(MlaArgs a, MlaPaged pg) {
     if (FMT == CACHE_F16 && a.ckv_rows > 0 && a.window <= 0) n = (int)max((int64_t)0, min((int64_t)n, a.ckv_rows - base));
     list = key_list(seq < 0 ? 0 : n, a.window, a.sinks);
     if (FMT != CACHE_F16) list.cut(pg.room());
+    else if (a.ckv_rows > 0) list.cut(max((int64_t)0, a.ckv_rows - base));
     n = list.count();
   }
-  const int per = (n + a.n_split - 1) / a.n_split;
-  const int k0 = sp * per, k1 = min(n, k0 + per);
+  const int64_t per = ((int64_t)n + a.n_split - 1) / a.n_split;
+  const int k0 = (int)min((int64_t)n, sp * per), k1 = (int)min((int64_t)n, k0 + per);
 
   float qf[SIMT_HG][16];
 #pragma unroll

@@ -242,3 +242,21 @@ def test_the_same_call_gives_the_same_bits():
         got.append(outs)
     for outs in got[1:]:
         assert all(torch.equal(a, b) for a, b in zip(outs, got[0]))
+
+
+@pytest.mark.parametrize("heads", [64, 16])
+@pytest.mark.parametrize("window,sinks", [(1, 2 ** 31 - 1), (2 ** 31 - 1, 0), (2 ** 31 - 1, 2 ** 31 - 1), (2 ** 30, 2 ** 30), (300, 7)])
+def test_windows_and_lengths_of_all_31_bits(heads, window, sinks):
+    """garbage in a padding row's length: the window stands where the length says, the cache's end cuts what is seen; times go by the cache"""
+    gen, held = gen_of(91), 700
+    ckv, q = torch.randn(held, 512, device="cuda", generator=gen).half(), queries(gen, 3, heads)
+    out = torch.empty(3, heads, 512, dtype=torch.float16, device="cuda")
+    lens = [2 ** 31 - 1, 500, 2 ** 31 - 40]
+    want = []
+    for r, n in enumerate(lens):
+        p = torch.arange(min(n, held), device="cuda")
+        want.append(attend(q[r].double(), ckv[p[(p >= n - window) | (p < sinks)]].double(), 0.0625))
+    for n_split in (0, 1, 2, 5):
+        hk.mla_window_prefill(q, ckv, out, 3, 0, window, sinks=sinks, n_heads=heads, kv_len=ints(lens), n_split=n_split, n_keys_hint=held)
+        finish()
+        close(out, want)
