@@ -87,6 +87,8 @@ SIGNATURES = {
     "hk_layernorm_f16": (_i, [_vp, _vp, _vp, _vp, _i, _i, _f, _vp]),
     "hk_mla_decode_prologue": (_i, [_vp, _vp, _vp, _f, _vp, _vp, _vp, _vp, _f, _vp, _vp, _i, _vp, _vp, _i, _vp, _vp]),
     "hk_mla_window": (_i, [_vp, _vp, _i64, _vp, _vp, _i, _i, _i, _vp, _i, _i, _f, _i, _vp, _sz, _vp]),
+    "hk_mla_window_keys": (_i, [_i, _i, _i]),
+    "hk_mla_window_workspace_bytes": (_sz, [_i, _i, _i, _i, _i]),
     "hk_mla8_append": (_i, [_vp, _vp, _vp, _vp, _i, _i64, _i, _vp, _i, _i, _vp, _vp, _i, _f, _vp, _vp]),
     "hk_mla8_read": (_i, [_vp, _vp, _i, _i64, _i, _vp, _i, _i, _i, _vp, _vp]),
     "hk_mla8_sparse_workspace_bytes": (_sz, [_i, _i, _i, _i64, _i]),
@@ -444,6 +446,23 @@ def mla_dense_prefill(q_lat, ckv, lat_out, qlen, pos_start, stream=None, scale=0
          scale, n_split, ws, ws, stream)
 
 
+def _window_splits(lib, m, n_heads, n_keys, window, sinks):
+    """0: the library's; heads other than 64 (the CUDA cores) get as many as 64 heads would"""
+    return 0 if n_heads == 64 else lib.hk_mla_auto_splits(m, lib.hk_mla_window_keys(n_keys, window, sinks))
+
+
+def _window_bytes(lib, m, n_heads, n_keys, window, sinks, n_split):
+    if n_split > 0:
+        return lib.hk_mla_partial_bytes(n_split, m * n_heads) if n_split > 1 else 0
+    return lib.hk_mla_window_workspace_bytes(m, n_heads, n_keys, window, sinks)
+
+
+def mla_window_workspace_bytes(m, n_heads, n_keys, window, sinks=0):
+    """what mla_window_prefill without n_split needs; n_keys: pos_start + qlen, or n_keys_hint where kv_len is given"""
+    lib = load_library()
+    return _window_bytes(lib, m, n_heads, n_keys, window, sinks, _window_splits(lib, m, n_heads, n_keys, window, sinks))
+
+
 def mla_window_prefill(q_lat, ckv, lat_out, qlen, pos_start, window, sinks=0, stream=None, scale=0.0625, n_heads=64,
                        kv_base=None, kv_len=None, n_split=0, workspace=None, n_keys_hint=None, ckv_rows=None):
     """mla_dense_prefill whose rows attend to their last `window` keys and the first `sinks` only (hk_mla_window); qlen = 1 is
@@ -452,16 +471,15 @@ def mla_window_prefill(q_lat, ckv, lat_out, qlen, pos_start, window, sinks=0, st
     _native.tensors("hhhli", ("q_lat", "lat_out", "ckv", "kv_base", "kv_len"), q_lat, size, lat_out, size, ckv, 0, kv_base, qlen, kv_len, qlen)
     if kv_len is not None:
         pos_start = n_keys_hint or pos_start
-    splits = n_split
+    n, ws = pos_start if kv_len is not None else pos_start + qlen, workspace
     if n_split <= 0:
-        tiles = -(-sinks // 64) + (window + 62) // 64 + 1      # whole tiles under the window (hk_mla_window chooses by as many)
-        n = pos_start if kv_len is not None else pos_start + qlen
-        splits = _native.hk_mla_auto_splits(qlen, min(64 * (min(tiles, -(-n // 64)) if n else tiles), 2 ** 31 - 1))
-    ws = workspace
-    if splits > 1 and ws is None:
-        ws = _scratch_like(_native.hk_mla_partial_bytes(splits, qlen * n_heads), q_lat, stream)
+        n_split = _window_splits(_native, qlen, n_heads, n, window, sinks)
+    if ws is None:
+        need = _window_bytes(_native, qlen, n_heads, n, window, sinks, n_split)
+        if need:
+            ws = _scratch_like(need, q_lat, stream)
     _run("hk_mla_window", q_lat, ckv, ckv if ckv_rows is None else ckv_rows, kv_base, kv_len, pos_start, window, sinks, lat_out, qlen,
-         n_heads, scale, n_split if n_heads == 64 else splits, ws, ws, stream)
+         n_heads, scale, n_split, ws, ws, stream)
 
 
 # ---- the latent cache in 8 bits, paged: ckv8 [n_blocks, block, 512] of torch.int8 or torch.float8_e4m3fn, scales [n_blocks] float32,

@@ -176,7 +176,8 @@ struct Entry<R (*)(A...)> {
   X(hk_q_latent_beside, true) X(hk_o_absorb_beside, true) X(hk_kda_decode_layer_beside, true)                                \
   X(hk_mla_cache_append, true) X(hk_layernorm_f16, true) X(hk_mla_decode_prologue, true) X(hk_mla_window, true)              \
   X(hk_mla8_append, true) X(hk_mla8_read, true) X(hk_mla8_dense, true) X(hk_mla8_sparse, true)                                \
-  X(hk_mla8_dense_workspace_bytes, false) X(hk_mla8_sparse_workspace_bytes, false)
+  X(hk_mla8_dense_workspace_bytes, false) X(hk_mla8_sparse_workspace_bytes, false)                                        \
+  X(hk_mla_window_keys, false) X(hk_mla_window_workspace_bytes, false)
 
 #define X(name, stream)                                                                      \
   decltype(&::name) p_##name = nullptr;                                                      \

@@ -116,20 +116,23 @@ int mla_window_keys(int n, int window, int sinks) {
   return (int)((tiles < all ? tiles : all) * 64 > INT32_MAX ? INT32_MAX : (tiles < all ? tiles : all) * 64);
 }
 
+// Splits of a call over fp16 rows that gives no number of them
+static int attend_splits(int m, int n_heads, int n_keys, int window) {
+  if (n_heads != 64 || force_simt()) return simt_auto_splits(m, n_heads, n_keys);
+  const int n_split = mla_flash_tc_auto_splits(m, n_keys);
+  // Windows: half as many, whose output channels two CTAs share, where that has the room and means at most six tiles each.  Splits as they are
+  // / half of them, us: four rows under 4,096 keys 15.4 / 13.1, eight under 2,048 14.2 / 12.6, 24 under 512 13.9 / 13.6, under 1,024 (six tiles)
+  // 15.8 / 15.6, eight under 4,096 (eight) 16.0 / 15.9.
+  const int half = (n_split + 1) / 2, tiles = n_keys / 64 + (n_keys % 64 != 0), room = sm_count();
+  return window > 0 && half > 1 && (int64_t)2 * n_split * m > room && (int64_t)2 * half * m <= room && (tiles + half - 1) / half <= 6 ? half : n_split;
+}
+
 // common driver: final output, optionally through split partials in the workspace.  `choose`: the caller leaves the form to the library,
 // which may then merge one row's splits in clusters; a number of splits that the caller gives means that many CTAs a row.
 static int attend(MlaArgs a, int n_keys_hint, int n_split, bool choose, void* workspace, size_t workspace_bytes,
                   cudaStream_t s) {
   const bool tc = (a.n_heads == 64) && !force_simt();
-  if (n_split <= 0) {
-    n_split = tc ? mla_flash_tc_auto_splits(a.m, n_keys_hint)
-                 : simt_auto_splits(a.m, a.n_heads, n_keys_hint);
-    // Windows: half as many, whose output channels two CTAs share, where that has the room and means at most six tiles each.  Splits as they are
-    // / half of them, us: four rows under 4,096 keys 15.4 / 13.1, eight under 2,048 14.2 / 12.6, 24 under 512 13.9 / 13.6, under 1,024 (six tiles)
-    // 15.8 / 15.6, eight under 4,096 (eight) 16.0 / 15.9.
-    const int half = (n_split + 1) / 2, tiles = n_keys_hint / 64 + (n_keys_hint % 64 != 0), room = sm_count();
-    if (tc && a.window > 0 && half > 1 && (int64_t)2 * n_split * a.m > room && (int64_t)2 * half * a.m <= room && (tiles + half - 1) / half <= 6) n_split = half;
-  }
+  if (n_split <= 0) n_split = attend_splits(a.m, a.n_heads, n_keys_hint, a.window);
   const int64_t rows = (int64_t)a.m * a.n_heads;
   __half* final_out = a.out;
   a.n_split = n_split;
@@ -651,6 +654,16 @@ HK_API int hk_mla_splitkv_sparse_step(const void* q_lat, const void* ckv_shard, 
                           max_wait_ms, signal, as_stream(stream));
 }
 
+
+HK_API int hk_mla_window_keys(int n_keys, int window, int sinks) {
+  return window >= 1 && sinks >= 0 ? hk::mla_window_keys(n_keys, window, sinks) : 0;
+}
+
+HK_API size_t hk_mla_window_workspace_bytes(int m, int n_heads, int n_keys, int window, int sinks) {
+  if (m <= 0 || n_heads < hk::SIMT_HG || window < 1 || sinks < 0) return 0;
+  const int splits = hk::attend_splits(m, n_heads, hk::mla_window_keys(n_keys, window, sinks), window);
+  return splits > 1 ? hk_mla_partial_bytes(splits, (int64_t)m * n_heads) : 0;
+}
 
 // Attention with a window and sinks over the fp16 cache: hk_mla_dense whose row of n keys sees p >= n - window and p < sinks only.
 HK_API int hk_mla_window(const void* q_lat, const void* ckv, int64_t ckv_rows, const int64_t* kv_base, const int* kv_len, int pos_start,

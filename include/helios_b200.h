@@ -294,11 +294,18 @@ int hk_mla_dense(const void* q_lat, const void* ckv, int64_t ckv_rows, const int
  * (p < sinks), each key once; window >= 1, sinks >= 0.  Rows outside are not read (tiles of 64 keys that hold none that the row sees are
  * skipped), and what lies there - infinities and NaN too - has no effect.  A key that is not finite and that a row does see makes NaN of the row's
  * outputs in the key's channels that are not finite, and in all channels where a score is NaN or plus infinity.  Other arguments as in hk_mla_dense; n stays what it is where
- * ckv_rows cuts the range.  The library chooses the splits by the keys under the window.
+ * ckv_rows cuts the range.  The library chooses the splits by the keys in the tiles that a row reads (hk_mla_window_keys).
  * Heads other than 64 (multiples of 4) run on the CUDA cores, up to 65,535 rows a call.                                          */
 int hk_mla_window(const void* q_lat, const void* ckv, int64_t ckv_rows, const int64_t* kv_base, const int* kv_len,
                   int pos_start, int window, int sinks, void* lat_out, int m, int n_heads, float scale, int n_split,
                   void* workspace, size_t workspace_bytes, void* stream);
+
+/* Keys in the whole tiles that a row of n_keys keys (0 or below: not known) reads under a window: what hk_mla_window's splits are chosen by.     */
+int hk_mla_window_keys(int n_keys, int window, int sinks);
+
+/* Workspace of an hk_mla_window call that leaves the splits to the library (n_split <= 0).  n_keys: pos_start + m, or pos_start where kv_len is given.
+ * A call that gives n_split > 1 needs hk_mla_partial_bytes(n_split, m * n_heads).                                                              */
+size_t hk_mla_window_workspace_bytes(int m, int n_heads, int n_keys, int window, int sinks);
 
 /* ---------------------------------------------------------------------------------------------
  * (b'') the latent cache in 8 bits, paged

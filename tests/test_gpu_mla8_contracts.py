@@ -260,3 +260,23 @@ def test_windows_and_lengths_of_all_31_bits(heads, window, sinks):
         hk.mla_window_prefill(q, ckv, out, 3, 0, window, sinks=sinks, n_heads=heads, kv_len=ints(lens), n_split=n_split, n_keys_hint=held)
         finish()
         close(out, want)
+
+
+@pytest.mark.parametrize("heads,rows,pos,window,sinks", [(64, 1, 4999, 128, 0), (64, 1, 4999, 1016, 4), (64, 24, 3000, 1024, 64), (64, 4, 5000, 4096, 0), (16, 3, 2000, 512, 0),
+                                                         (32, 24, 3000, 1024, 64), (64, 200, 500, 300, 5)])
+def test_windows_in_the_workspace_that_is_said(heads, rows, pos, window, sinks):
+    """the size functions' bytes are enough, for the library's own choice and the wrapper's, and nothing behind them is written"""
+    gen = gen_of(rows + pos)
+    ckv, q = torch.randn(pos + rows, 512, device="cuda", generator=gen).half(), queries(gen, rows, heads)
+    out = torch.empty(rows, heads, 512, dtype=torch.float16, device="cuda")
+    want = [attend(q[r].double(), ckv[:pos + r + 1][visible(pos + r + 1, window, sinks)].double(), 0.0625) for r in range(rows)]
+    for wrapped in (False, True):
+        need = (hk.mla_window_workspace_bytes if wrapped else hk.load_library().hk_mla_window_workspace_bytes)(rows, heads, pos + rows, window, sinks)
+        ws = torch.full((need + 4096,), 0x5a, dtype=torch.uint8, device="cuda")
+        if wrapped:
+            hk.mla_window_prefill(q, ckv, out.zero_(), rows, pos, window, sinks=sinks, n_heads=heads, workspace=ws[:need] if need else None)
+        else:
+            hk._run("hk_mla_window", q, ckv, ckv, None, None, pos, window, sinks, out.zero_(), rows, heads, 0.0625, 0, ws[:need] if need else None, need, None)
+        finish()
+        close(out, want)
+        assert (ws[need:] == 0x5a).all()
