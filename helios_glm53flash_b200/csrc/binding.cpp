@@ -264,6 +264,7 @@ bool cache8_of(PyObject* const* args, int device, Cache8& v) {
   const bool i8 = c.scalar_type() == at::kChar;
   if ((!i8 && c.scalar_type() != at::kFloat8_e4m3fn) || c.dim() != 3 || c.size(2) != 512 || !c.is_contiguous())
     return refuse("ckv8: a contiguous [n_blocks, block, 512] tensor of int8 or float8_e4m3fn");
+  if (c.size(1) > INT32_MAX) return refuse("ckv8: blocks of at most 128 tokens");
   if (s.scalar_type() != at::kFloat || s.numel() != c.size(0) || !s.is_contiguous()) return refuse("scales: a contiguous float32 tensor, one a block");
   if (elsewhere(c, device) || elsewhere(s, device) || (args[2] != Py_None && elsewhere(THPVariable_Unpack(args[2]), device)))
     return refuse("the 8-bit cache's tensors: on the current CUDA device");
@@ -276,6 +277,7 @@ bool cache8_of(PyObject* const* args, int device, Cache8& v) {
       return refuse("block_table: a contiguous [n_seqs, blocks of a sequence] tensor of int32");
     v.stride = t.size(-1);
     v.seqs = t.numel() / v.stride;
+    if (v.stride > INT32_MAX || v.seqs > INT32_MAX) return refuse("block_table: at most 2^31 - 1 sequences and blocks of one");
   }
   return true;
 }

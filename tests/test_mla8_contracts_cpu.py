@@ -47,3 +47,16 @@ def test_sizes_of_windows_that_are_refused_are_none(lib):  # noqa: F811
     assert lib.hk_mla_window_keys(500, 0, 0) == lib.hk_mla_window_keys(500, 3, -1) == 0
     assert lib.hk_mla_window_keys(500, 100, 0) == lib.hk_mla_window_keys(0, 100, 0) == 192 and lib.hk_mla_window_keys(100, 1000, 5) == 128
     assert lib.hk_mla_window_keys(2 ** 31 - 1, 2 ** 31 - 1, 2 ** 31 - 1) == 2 ** 31 - 1
+
+
+def test_tables_and_blocks_whose_sizes_do_not_fit_31_bits_raise(lib):  # noqa: F811
+    """(the library takes ints: 2^32 + 4 would arrive as 4)"""
+    import torch
+    from helios_glm53flash_b200 import _binding as nb
+    ckv8, scales = torch.zeros(4, 16, 512, dtype=torch.int8), torch.zeros(4)
+    for shape in ((1, 2 ** 32 + 4), (2 ** 32 + 4, 1), (2 ** 31,), (2, 2 ** 31)):
+        with pytest.raises(ValueError):
+            nb.cache8(ckv8, scales, torch.empty(shape, dtype=torch.int32, device="meta"))
+    with pytest.raises(ValueError):
+        nb.cache8(torch.empty(0, 2 ** 32 + 16, 512, dtype=torch.int8), torch.zeros(0), None)
+    assert nb.cache8(ckv8, scales, torch.empty(2 ** 31 - 1, 1, dtype=torch.int32, device="meta")) == (hk.HK_I8, 4, 16, 1, 2 ** 31 - 1)
