@@ -198,14 +198,16 @@ def test_blocks_whose_scale_is_infinite(kind):
 # ---------------------------------------------------------------------------------------------
 # the CUDA-core kernel, streams, the same call again
 # ---------------------------------------------------------------------------------------------
-def test_the_cuda_core_kernel_over_the_8_bit_cache():
-    """the form for machines without an encoder of tensor maps, in a process of its own: holes, sequence numbers out of range, NaN scales, windows, splits"""
+@pytest.mark.parametrize("switch", ["HK_MLA_FORCE_SIMT", "HK_MLA_NO_TMA"])
+def test_the_cuda_core_kernel_over_the_8_bit_cache(switch):
+    """the form for machines without an encoder of tensor maps, in a process of its own: holes, sequence numbers out of range, NaN scales, windows, splits;
+    asked for, and where the encoder is missing, when long chunks are read as fp16 rows first all the same"""
     names = ("test_dense8_rows", "test_dense8_chunk", "test_dense8_rows_and_blocks_that_do_not_count", "test_a_row_that_is_not_finite_is_seen_in_the_output",
              "test_splits_that_see_nothing", "test_sparse8", "test_window_rows", "test_dense8_without_a_table", "test_blocks_that_weigh", "test_keys_of_zeros")
     here = os.path.dirname(os.path.abspath(__file__))
     files = [os.path.join(here, f) for f in ("test_gpu_mla8.py", "test_gpu_mla8_contracts.py")]
     run = subprocess.run([sys.executable, "-m", "pytest", "-x", "-q", "-m", "gpu", "-p", "no:cacheprovider", "-k", " or ".join(names)] + files,
-                         env={**os.environ, "HK_MLA_FORCE_SIMT": "1"}, capture_output=True, text=True, timeout=600)
+                         env={**os.environ, switch: "1"}, capture_output=True, text=True, timeout=600)
     assert run.returncode == 0, run.stdout[-3000:] + run.stderr[-2000:]
 
 
