@@ -450,10 +450,16 @@ __global__ __launch_bounds__(F8_THREADS, 1) void mla8_flash_tc_kernel(MlaArgs a,
 #pragma unroll
       for (int j = 0; j < 32; j++) tmax = fmaxf(tmax, __uint_as_float(sv[j]));
       ms.mx[b][tid] = tmax;
-      asm volatile("bar.sync %0, 64;" ::"r"(1 + (warp & 1)) : "memory");   // the two warps of these heads
+      // the two warps of these heads; behind a wait that gave up they may have read different scales, and still go the same way
+      uint32_t by_key;
+      asm volatile(
+          "{\n\t.reg .pred p, q;\n\tsetp.ne.u32 q, %2, 0;\n\tbar.red.or.pred p, %1, 64, q;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+          : "=r"(by_key)
+          : "r"(1 + (warp & 1)), "r"((uint32_t)uneven)
+          : "memory");
       tmax = fmaxf(tmax, ms.mx[b][tid ^ 64]);
       float wmax = tmax + __log2f(fmaxf(top, F8_LEAST_SCALE));
-      if (uneven) {
+      if (by_key) {
         const float* own = &ms.sc[kb][32 * half];
         wmax = -INFINITY;
 #pragma unroll
