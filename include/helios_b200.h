@@ -292,9 +292,9 @@ int hk_mla_dense(const void* q_lat, const void* ckv, int64_t ckv_rows, const int
 
 /* hk_mla_dense with a window and sinks: a row of n keys attends to its last `window` keys (p >= n - window) and to the first `sinks`
  * (p < sinks), each key once; window >= 1, sinks >= 0.  Rows outside are not read (tiles of 64 keys that hold none that the row sees are
- * skipped), and what lies there - infinities and NaN too - has no effect.  A key that is not finite and that a row does see makes NaN of the row's
- * outputs in the key's channels that are not finite, and in all channels where a score is NaN or plus infinity.  Other arguments as in hk_mla_dense; n stays what it is where
- * ckv_rows cuts the range.  The library chooses the splits by the keys in the tiles that a row reads (hk_mla_window_keys).
+ * skipped), and what lies there - infinities and NaN too - has no effect.  A key that is not finite and that a row does see makes NaN of the
+ * row's outputs in the key's channels that are not finite, and in all channels where a score is NaN or plus infinity (hk_mla_dense: zeros where
+ * the scores are NaN).  Other arguments as in hk_mla_dense; n stays what it is where ckv_rows cuts the range.  The library chooses the splits by the keys in the tiles that a row reads (hk_mla_window_keys).
  * Heads other than 64 (multiples of 4) run on the CUDA cores, up to 65,535 rows a call.                                          */
 int hk_mla_window(const void* q_lat, const void* ckv, int64_t ckv_rows, const int64_t* kv_base, const int* kv_len,
                   int pos_start, int window, int sinks, void* lat_out, int m, int n_heads, float scale, int n_split,
@@ -345,10 +345,12 @@ size_t hk_mla8_sparse_workspace_bytes(int m, int n_heads, int kidx, int64_t posi
 
 /* hk_mla_dense over the 8-bit cache: row r attends to the first kv_len[r] positions of its sequence (kv_len NULL: pos_start + r + 1).
  * window > 0: of these the last `window` and the first `sinks` only, as in hk_mla_window; window = 0: all.  n_heads: a multiple of 4.
- * Scores and sums are fp32; a row without keys gives zeros.
+ * Scores and sums are fp32; a row without keys gives zeros.  A weight times its key's scale is rounded to fp16: 2^-11 of itself, or 2^-21 of the
+ * largest of its head where it is below 2^-10 of that, whatever the blocks' scales are (up to 2^100; a block below 2^-100 may weigh nothing).
  * A chunk (kv_len and row_seq NULL) is checked on the host, pos_start + m positions have a place in the table (else HK_ERR_INVALID); in it a
  * position whose entry names no block is a latent of zeros, as hk_mla8_read gives it.  A chunk of 64 heads, 8 rows and 65,536 (row, key)
- * pairs or more, with n_split <= 0, reads its positions as fp16 rows into the workspace first and attends to those (latents beyond 65,504 are infinite there).        */
+ * pairs or more, with n_split <= 0, reads its positions as fp16 rows into the workspace first and attends to those as hk_mla_dense does: there a
+ * latent is off by 2^-11 of itself, or 2^-25 where it is below 2^-14, and infinite beyond 65,504, and a weight below 2^-14 of the largest by 2^-25 of it.  */
 int hk_mla8_dense(const void* q_lat, const void* ckv8, const float* scales, int dtype, int64_t n_blocks, int block,
                   const int* block_table, int table_stride, int n_seqs, const int* row_seq, const int* kv_len, int pos_start,
                   int window, int sinks, void* lat_out, int m, int n_heads, float scale, int n_split, int n_keys_hint,
