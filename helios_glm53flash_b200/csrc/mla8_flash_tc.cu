@@ -410,7 +410,9 @@ __global__ __launch_bounds__(F8_THREADS, 1) void mla8_flash_tc_kernel(MlaArgs a,
       tc::fence_before_sync();
       tc::mbar_arrive(&ms.q_ready);
     }
-    float m = -INFINITY, l = 0.f, w_ref = -INFINITY, g = 0.f;   // references: of the scores, of the weights (log2); 2^(m - w_ref)
+    // References (log2): m of the scores, w_score + w_scale of the weights; g = 2^(m - both).  As two numbers, a score and a scale: their sum would
+    // lose the scale beside a score of 2^24, and what is formed of it are differences of scores and differences of scales.
+    float m = -INFINITY, l = 0.f, w_score = -INFINITY, w_scale = 0.f, g = 0.f;
     for (int t = 0; t < n_tiles; t++) {
       const int b = t & 1, kb = t % F8_NBUF;
       ok = tc::mbar_wait<F8_POLL_NS>(&ms.full[kb], (t / F8_NBUF) & 1, abort_flag, 47) && ok;   // makes the scales visible
@@ -458,29 +460,30 @@ __global__ __launch_bounds__(F8_THREADS, 1) void mla8_flash_tc_kernel(MlaArgs a,
           : "r"(1 + (warp & 1)), "r"((uint32_t)uneven)
           : "memory");
       tmax = fmaxf(tmax, ms.mx[b][tid ^ 64]);
-      float wmax = tmax + __log2f(fmaxf(top, F8_LEAST_SCALE));
+      float over = __log2f(fmaxf(top, F8_LEAST_SCALE));     // the tile's largest weight, over tmax
       if (by_key) {
         const float* own = &ms.sc[kb][32 * half];
-        wmax = -INFINITY;
+        over = -INFINITY;
 #pragma unroll
-        for (int j = 0; j < 32; j++) wmax = fmaxf(wmax, __uint_as_float(sv[j]) + __log2f(fmaxf(own[j], F8_LEAST_SCALE)));
+        for (int j = 0; j < 32; j++) over = fmaxf(over, __uint_as_float(sv[j]) - tmax + __log2f(fmaxf(own[j], F8_LEAST_SCALE)));
         asm volatile("bar.sync %0, 64;" ::"r"(1 + (warp & 1)) : "memory");   // the maxima above have been read
-        ms.mx[b][tid] = wmax;
+        ms.mx[b][tid] = over;
         asm volatile("bar.sync %0, 64;" ::"r"(1 + (warp & 1)) : "memory");
-        wmax = fmaxf(wmax, ms.mx[b][tid ^ 64]);
+        over = fmaxf(over, ms.mx[b][tid ^ 64]);
       }
       const bool move = tmax > m + F8_MOVE || (m == -INFINITY && tmax > -INFINITY);
-      const bool move_w = wmax > w_ref + F8_MOVE || (w_ref == -INFINITY && wmax > -INFINITY);
+      const bool move_w = (tmax - w_score) + (over - w_scale) > F8_MOVE;   // (the first key is infinitely more)
       float alpha = 1.f;
       if (move) {
         l *= m == -INFINITY ? 0.f : exp2f(m - tmax);
         m = tmax;
       }
       if (move_w) {
-        alpha = w_ref == -INFINITY ? 0.f : exp2f(w_ref - wmax);
-        w_ref = wmax;
+        alpha = exp2f((w_score - tmax) + (w_scale - over));
+        w_score = tmax;
+        w_scale = over;
       }
-      if (move || move_w) g = exp2f(m - w_ref);
+      if (move || move_w) g = exp2f((m - w_score) - w_scale);
       if (t > 0 && __any_sync(0xffffffffu, move_w)) {
         // rare: a head's weights' reference moved.  O is rescaled after the tile before has been added and before this one is
         wait_pv(t - 1, 49);
@@ -536,7 +539,7 @@ __global__ __launch_bounds__(F8_THREADS, 1) void mla8_flash_tc_kernel(MlaArgs a,
     const bool none = l == 0.f;                            // (NaN: a score was none)
     if (half == 0) {
       // NaN has to reach the merge, which weighs a split of nothing else 0
-      const float unit = exp2f(w_ref - m);                 // O in units of the scores' reference
+      const float unit = exp2f((w_score - m) + w_scale);         // O in units of the scores' reference
       ms.mx[(n_tiles + 1) & 1][head] = none ? 0.f : final_out ? unit / l : l == l ? unit : l;
       if (!final_out && it.r >= 0 && it.part == 0 && head < n_h) {
         const size_t at = part_row + head;

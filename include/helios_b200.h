@@ -293,8 +293,9 @@ int hk_mla_dense(const void* q_lat, const void* ckv, int64_t ckv_rows, const int
 /* hk_mla_dense with a window and sinks: a row of n keys attends to its last `window` keys (p >= n - window) and to the first `sinks`
  * (p < sinks), each key once; window >= 1, sinks >= 0.  Rows outside are not read (tiles of 64 keys that hold none that the row sees are
  * skipped), and what lies there - infinities and NaN too - has no effect.  A key that is not finite and that a row does see makes NaN of the
- * row's outputs in the key's channels that are not finite, and in all channels where a score is NaN or plus infinity (hk_mla_dense: zeros where
- * the scores are NaN).  Other arguments as in hk_mla_dense; n stays what it is where ckv_rows cuts the range.  The library chooses the splits by the keys in the tiles that a row reads (hk_mla_window_keys).
+ * row's outputs in the key's channels that are not finite, and in all channels where a score is NaN or plus infinity; elsewhere it may
+ * (hk_mla_dense: zeros where the scores are NaN).  Other arguments as in hk_mla_dense; n stays what it is where ckv_rows cuts the range.
+ * The library chooses the splits by the keys in the tiles that a row reads (hk_mla_window_keys).
  * Heads other than 64 (multiples of 4) run on the CUDA cores, up to 65,535 rows a call.                                          */
 int hk_mla_window(const void* q_lat, const void* ckv, int64_t ckv_rows, const int64_t* kv_base, const int* kv_len,
                   int pos_start, int window, int sinks, void* lat_out, int m, int n_heads, float scale, int n_split,

@@ -282,3 +282,29 @@ def test_windows_in_the_workspace_that_is_said(heads, rows, pos, window, sinks):
         finish()
         close(out, want)
         assert (ws[need:] == 0x5a).all()
+
+
+@pytest.mark.parametrize("kind", ["i8", "e4m3"])
+@pytest.mark.parametrize("block", [16, 64])
+@pytest.mark.parametrize("q7,scale,small", [(60000.0, 0.0625, 0.01), (60000.0, 1.0, 0.01), (-60000.0, 20.0, 0.01), (60000.0, 1e9, 1e-6), (-60000.0, 1e10, 1e-5)])
+def test_scores_so_large_that_a_scale_is_lost_beside_them(kind, block, q7, scale, small):
+    """one channel makes the scores, 0 for all keys but one, which has 37 at least: a row's output is that key's latent (its weight is rounded to
+    fp16, and the output), whatever its block's scale, the largest or the smallest"""
+    gen, n = gen_of(95), 320
+    blocks, top = n // block, TOP[kind]
+    v = torch.randn(blocks, block, 512, device="cuda", generator=gen).clamp(-3, 3) * (top / 4)
+    ckv8 = (v.round() if kind == "i8" else v).to(STORE[kind])
+    ckv8.view(torch.uint8)[:, :, 7] = 0                         # +0 in both types: the score 0
+    scales = torch.where(torch.arange(blocks, device="cuda") % 2 == 0, 60000.0 / top, small).float()
+    q = torch.zeros(2, 64, 512, dtype=torch.float16, device="cuda")
+    q[:, :, 7] = q7
+    out = torch.empty(2, 64, 512, dtype=torch.float16, device="cuda")
+    for best in (3, n // 2 + 1, block + 5, n - block + 1, n - 1):
+        c = ckv8.clone()
+        c.view(torch.int8 if kind == "i8" else torch.uint8)[best // block, best % block, 7] = {"i8": 1, "e4m3": 0x38}[kind] if q7 > 0 else {"i8": -1, "e4m3": 0xb8}[kind]
+        want = rows_of(c, scales, torch.arange(blocks, device="cuda"), torch.tensor([best], device="cuda"))
+        for n_split in (0, 1, 2):
+            hk.mla8_dense_prefill(q, c, scales, out, 2, 0, kv_len=ints([n, n]), scale=scale, n_split=n_split, n_keys_hint=n)
+            finish()
+            off = (out.double() - want).abs()
+            assert bool((off <= want.abs() * 2.0 ** -10 * 1.01 + 2.0 ** -25).all()), (best, n_split, float(off.max()))
