@@ -95,6 +95,21 @@ SIGNATURES = {
     "hk_mla8_dense_workspace_bytes": (_sz, [_i, _i, _i, _i, _i, _i, _i]),
     "hk_mla8_dense": (_i, [_vp, _vp, _vp, _i, _i64, _i, _vp, _i, _i, _vp, _vp, _i, _i, _i, _vp, _i, _i, _f, _i, _i, _vp, _sz, _vp]),
     "hk_mla8_sparse": (_i, [_vp, _vp, _vp, _i, _i64, _i, _vp, _i, _i, _vp, _vp, _i, _vp, _i, _i, _f, _i, _vp, _sz, _vp]),
+    "hk_mla_tree_workspace_bytes": (_sz, [_i, _i, _i]),
+    "hk_mla_tree": (_i, [_vp, _vp, _i64, _vp, _vp, _i, _vp, _vp, _vp, _i, _vp, _i, _i, _f, _i, _vp, _sz, _vp]),
+    "hk_mla8_tree_workspace_bytes": (_sz, [_i, _i, _i]),
+    "hk_mla8_tree": (_i, [_vp, _vp, _vp, _i, _i64, _i, _vp, _i, _vp, _i, _vp, _vp, _vp, _i, _vp, _i, _i, _f, _i, _vp, _sz, _vp]),
+    "hk_mla_tree_accept": (_i, [_vp, _vp, _i64, _vp, _vp, _i, _vp, _vp, _i, _vp, _i, _vp, _vp]),
+    "hk_mla8_tree_accept": (_i, [_vp, _vp, _vp, _i, _i64, _i, _vp, _i, _vp, _i, _vp, _vp, _i, _vp, _i, _vp, _vp]),
+    "hk_kda_tree_conv": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _vp, _i, _i, _i, _vp]),
+    "hk_kda_tree": (_i, [_vp, _vp, _vp, _vp, _vp, _f, _vp, _vp, _vp, _vp, _i, _vp, _vp, _i, _i, _i, _vp]),
+    "hk_kda_tree_accept": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _f, _vp, _vp, _vp, _vp, _i, _vp, _i, _i, _vp]),
+    "hk_mla8_pages_workspace_bytes": (_sz, [_i64, _i]),
+    "hk_mla8_pages_fork": (_i, [_vp, _vp, _i, _i64, _i, _vp, _vp, _i, _i, _vp, _vp, _vp, _i, _vp, _vp, _sz, _vp]),
+    "hk_mla8_pages_reserve": (_i, [_vp, _vp, _i, _i64, _i, _vp, _vp, _i, _i, _vp, _vp, _i, _vp, _vp, _sz, _vp]),
+    "hk_mla8_pages_free": (_i, [_vp, _vp, _i, _i64, _i, _vp, _vp, _i, _i, _vp, _vp, _i, _vp]),
+    "hk_mla8_pages_compact": (_i, [_vp, _vp, _i, _i64, _i, _vp, _vp, _i, _i, _vp, _vp, _sz, _vp]),
+    "hk_mla8_pages_copy": (_i, [_vp, _vp, _i64, _vp, _vp, _i64, _i, _i, _vp, _vp, _i, _vp]),
     "hk_read_device_status": (_i, [_vp, _i]),
     "hk_tc05_selftest": (_i, [_vp, _vp, _vp, _i, _i, _i, _i, _vp, _vp]),
 }
@@ -543,6 +558,165 @@ def mla8_sparse_decode(q_lat, ckv8, scales, raw_idx, kidx, lat_out, m, stream=No
             ws = _scratch_like(need, q_lat, stream)
     _run("hk_mla8_sparse", q_lat, ckv8, scales, tag, n_blocks, block, block_table, stride, seqs, row_seq, raw_idx, kidx, lat_out, m, n_heads, scale,
          n_split, ws, ws, stream)
+
+
+# ---- trees of drafted tokens: m nodes of n_seqs sequences' trees, rows tree_start[s] .. tree_start[s + 1] - 1 (device int32 [n_seqs + 1]; None: m / n_seqs
+# each); parent: device int32 [m], the number within the tree of the node that a row hangs on, -1: the sequence's last token.  leaf: device int32
+# [n_seqs], the accepted node of each tree, -1: none.  Tensors of another type, layout, device or size than the call's raise ValueError ----
+def mla_tree_workspace_bytes(m, n_heads, n_keys):
+    """what mla_tree_decode without n_split needs; n_keys: pos_start, or n_keys_hint where kv_len is given"""
+    return load_library().hk_mla_tree_workspace_bytes(m, n_heads, n_keys)
+
+
+def mla8_tree_workspace_bytes(m, n_heads, n_keys):
+    return load_library().hk_mla8_tree_workspace_bytes(m, n_heads, n_keys)
+
+
+def mla_tree_decode(q_lat, ckv, tree_kv, parent, lat_out, m, pos_start=0, n_seqs=1, tree_start=None, kv_base=None, kv_len=None, stream=None,
+                    scale=0.0625, n_heads=64, n_split=0, workspace=None, n_keys_hint=None, ckv_rows=None):
+    """Attention of m nodes: a row attends to its sequence's cached rows (kv_len [n_seqs] of them from kv_base [n_seqs] on, or pos_start) and to
+    its path's rows of tree_kv [m, 512] (hk_mla_tree).  n_keys_hint: keys of the longest sequence where kv_len says them on the device."""
+    size = m * n_heads * 512
+    _native.tensors("hhhhiiil", ("q_lat", "lat_out", "ckv", "tree_kv", "parent", "tree_start", "kv_len", "kv_base"), q_lat, size, lat_out, size, ckv, 0,
+                    tree_kv, m * 512, parent, m, tree_start, n_seqs + 1, kv_len, n_seqs, kv_base, n_seqs)
+    if kv_len is not None:
+        pos_start = n_keys_hint or pos_start
+    ws = workspace
+    if ws is None:
+        need = (_native.hk_mla_tree_workspace_bytes(m, n_heads, pos_start) if n_split <= 0
+                else _native.hk_mla_partial_bytes(n_split, m * n_heads) if n_split > 1 else 0)
+        if need:
+            ws = _scratch_like(need, q_lat, stream)
+    _run("hk_mla_tree", q_lat, ckv, ckv if ckv_rows is None else ckv_rows, kv_base, kv_len, pos_start, tree_kv, parent, tree_start, n_seqs, lat_out, m,
+         n_heads, scale, n_split, ws, ws, stream)
+
+
+def mla8_tree_decode(q_lat, ckv8, scales, tree_kv, parent, lat_out, m, pos_start=0, n_seqs=1, tree_start=None, block_table=None, kv_len=None,
+                     stream=None, scale=0.0625, n_heads=64, n_split=0, workspace=None, n_keys_hint=None):
+    """mla_tree_decode over the 8-bit cache (hk_mla8_tree); the nodes' own rows are fp16 here too"""
+    size = m * n_heads * 512
+    tag, n_blocks, block, stride, seqs = _native.cache8(
+        ckv8, scales, block_table, "hhhiii", ("q_lat", "lat_out", "tree_kv", "parent", "tree_start", "kv_len"), q_lat, size, lat_out, size, tree_kv,
+        m * 512, parent, m, tree_start, n_seqs + 1, kv_len, n_seqs)
+    if n_seqs > seqs:
+        raise ValueError("block_table: fewer sequences than n_seqs")
+    if kv_len is not None:
+        pos_start = n_keys_hint or pos_start
+    ws = workspace
+    if ws is None:
+        need = (_native.hk_mla8_tree_workspace_bytes(m, n_heads, pos_start) if n_split <= 0
+                else _native.hk_mla_partial_bytes(n_split, m * n_heads) if n_split > 1 else 0)
+        if need:
+            ws = _scratch_like(need, q_lat, stream)
+    _run("hk_mla8_tree", q_lat, ckv8, scales, tag, n_blocks, block, block_table, stride, kv_len, pos_start, tree_kv, parent, tree_start, n_seqs, lat_out,
+         m, n_heads, scale, n_split, ws, ws, stream)
+
+
+def mla_tree_accept(tree_kv, ckv, parent, leaf, m, pos_start=0, n_seqs=1, tree_start=None, kv_base=None, kv_len=None, len_out=None, stream=None,
+                    ckv_rows=None):
+    """the accepted paths' rows of tree_kv behind their sequences' cached ones (hk_mla_tree_accept); len_out: device int32 [n_seqs], the lengths then"""
+    _native.tensors("hhiiiili", ("tree_kv", "ckv", "parent", "leaf", "tree_start", "kv_len", "kv_base", "len_out"), tree_kv, m * 512, ckv, 0, parent, m, leaf,
+                    n_seqs, tree_start, n_seqs + 1, kv_len, n_seqs, kv_base, n_seqs, len_out, n_seqs)
+    _run("hk_mla_tree_accept", tree_kv, ckv, ckv if ckv_rows is None else ckv_rows, kv_base, kv_len, pos_start, parent, tree_start, n_seqs, leaf, m,
+         len_out, stream)
+
+
+def mla8_tree_accept(tree_kv, ckv8, scales, parent, leaf, m, pos_start=0, n_seqs=1, tree_start=None, block_table=None, kv_len=None, len_out=None,
+                     stream=None):
+    """mla_tree_accept into the 8-bit cache (hk_mla8_tree_accept)"""
+    tag, n_blocks, block, stride, seqs = _native.cache8(
+        ckv8, scales, block_table, "hiiiii", ("tree_kv", "parent", "leaf", "tree_start", "kv_len", "len_out"), tree_kv, m * 512, parent, m, leaf, n_seqs,
+        tree_start, n_seqs + 1, kv_len, n_seqs, len_out, n_seqs)
+    if n_seqs > seqs:
+        raise ValueError("block_table: fewer sequences than n_seqs")
+    _run("hk_mla8_tree_accept", tree_kv, ckv8, scales, tag, n_blocks, block, block_table, stride, kv_len, pos_start, parent, tree_start, n_seqs, leaf, m,
+         len_out, stream)
+
+
+def kda_tree_conv(x32, conv_state, conv_weight, conv_bias, parent, mixed_qkv, m, dim, n_seqs=1, tree_start=None, slots=None, activation=True, stream=None):
+    """kda_cast_conv of nodes, whose windows are their ancestors' rows and then the sequence's conv_state (hk_kda_tree_conv)"""
+    _native.tensors("fbbbbiii", ("x32", "conv_state", "conv_weight", "conv_bias", "mixed_qkv", "parent", "tree_start", "slots"), x32, m * dim, conv_state,
+                    dim * 4 if slots is not None else n_seqs * dim * 4, conv_weight, dim * 4, conv_bias, dim, mixed_qkv, m * dim, parent, m, tree_start, n_seqs + 1, slots, n_seqs)
+    _run("hk_kda_tree_conv", x32, conv_state, slots, conv_weight, conv_bias, parent, tree_start, n_seqs, mixed_qkv, m, dim, 1 if activation else 0, stream)
+
+
+def _kda_tree_checks(mixed_qkv, g, beta, dt_bias, a_log, rec_state, parent, m, num_heads, n_seqs, tree_start, slots):
+    state = num_heads * 128 * 128
+    _native.tensors("bf" + ("b" if a_log is None else "f") + "fffiii", ("mixed_qkv", "g", "beta", "dt_bias", "a_log", "rec_state", "parent", "tree_start",
+                                                                       "slots"), mixed_qkv, m * 3 * num_heads * 128, g, m * num_heads * 128, beta, m * num_heads, dt_bias,
+                    num_heads * 128, a_log, num_heads, rec_state, state if slots is not None else n_seqs * state, parent, m, tree_start, n_seqs + 1, slots, n_seqs)
+
+
+def kda_tree_decode(mixed_qkv, g, beta, rec_state, parent, out, m, num_heads, n_seqs=1, tree_start=None, slots=None, out_f32=None, max_nodes=0,
+                    dt_bias=None, a_log=None, lower_bound=0.0, stream=None):
+    """The KDA recurrence of nodes, each from its parent's state (hk_kda_tree); rec_state stays as it is.  With dt_bias and a_log, g and beta are the raw
+    gate projection and the raw beta logit, as in kda_chunked_prefill_gated.  max_nodes: nodes of the longest tree (0: 64)."""
+    _kda_tree_checks(mixed_qkv, g, beta, dt_bias, a_log, rec_state, parent, m, num_heads, n_seqs, tree_start, slots)
+    _native.tensors("bf", ("out", "out_f32"), out, m * num_heads * 128, out_f32, m * num_heads * 128)
+    _run("hk_kda_tree", mixed_qkv, g, beta, dt_bias, a_log, lower_bound, rec_state, slots, parent, tree_start, n_seqs, out, out_f32, m, num_heads, max_nodes,
+         stream)
+
+
+def kda_tree_accept(x32, conv_state, mixed_qkv, g, beta, rec_state, parent, leaf, m, num_heads, n_seqs=1, tree_start=None, slots=None, dt_bias=None,
+                    a_log=None, lower_bound=0.0, stream=None):
+    """the states and, with x32 and conv_state, the convolution windows step along the accepted paths (hk_kda_tree_accept)"""
+    dim = 3 * num_heads * 128
+    _kda_tree_checks(mixed_qkv, g, beta, dt_bias, a_log, rec_state, parent, m, num_heads, n_seqs, tree_start, slots)
+    _native.tensors("fbi", ("x32", "conv_state", "leaf"), x32, m * dim, conv_state, dim * 4 if slots is not None else n_seqs * dim * 4, leaf, n_seqs)
+    _run("hk_kda_tree_accept", x32, conv_state, mixed_qkv, g, beta, dt_bias, a_log, lower_bound, rec_state, slots, parent, tree_start, n_seqs, leaf, m, num_heads,
+         stream)
+
+
+# ---- pages of the 8-bit cache: refs [n_blocks] int32 counts the entries of block_table [n_seqs, blocks of a sequence] that name a block.  A pool begins
+# with refs 0 and a table of -1.  missing, n_live: optional device int32 [1] ----
+def _pages(ckv8, scales, refs, block_table, types, names, *tensors):
+    tag, n_blocks, block, stride, seqs = _native.cache8(ckv8, scales, block_table, "i" + types, ("refs",) + names, refs, ckv8.shape[0], *tensors)
+    if block_table is None:
+        raise ValueError("block_table: needed")
+    return ckv8, scales, tag, n_blocks, block, refs, block_table, stride, seqs
+
+
+def _pages_scratch(ckv8, n, workspace, stream):
+    return _scratch_like(_native.hk_mla8_pages_workspace_bytes(ckv8.shape[0], n), ckv8, stream) if workspace is None else workspace
+
+
+def mla8_pages_workspace_bytes(n_blocks, n=0):
+    return load_library().hk_mla8_pages_workspace_bytes(n_blocks, n)
+
+
+def mla8_pages_fork(ckv8, scales, refs, block_table, parents, children, lens, n, missing=None, workspace=None, stream=None):
+    """n sequences `children` take over the first lens[i] positions of `parents` (hk_mla8_pages_fork): whole blocks shared, the last one copied"""
+    pool = _pages(ckv8, scales, refs, block_table, "iiii", ("parents", "children", "lens", "missing"), parents, n, children, n, lens, n, missing, 1)
+    ws = _pages_scratch(ckv8, n, workspace, stream)
+    _run("hk_mla8_pages_fork", *pool, parents, children, lens, n, missing, ws, ws, stream)
+
+
+def mla8_pages_reserve(ckv8, scales, refs, block_table, seqs, lens, n, missing=None, workspace=None, stream=None):
+    """n sequences get a free block for every entry of their first lens[i] positions that names none (hk_mla8_pages_reserve)"""
+    pool = _pages(ckv8, scales, refs, block_table, "iii", ("seqs", "lens", "missing"), seqs, n, lens, n, missing, 1)
+    ws = _pages_scratch(ckv8, n, workspace, stream)
+    _run("hk_mla8_pages_reserve", *pool, seqs, lens, n, missing, ws, ws, stream)
+
+
+def mla8_pages_free(ckv8, scales, refs, block_table, seqs, keep, n, stream=None):
+    """n sequences give back the blocks behind their first keep[i] positions (keep None: all of them)"""
+    _run("hk_mla8_pages_free", *_pages(ckv8, scales, refs, block_table, "ii", ("seqs", "keep"), seqs, n, keep, n), seqs, keep, n, stream)
+
+
+def mla8_pages_compact(ckv8, scales, refs, block_table, n_live=None, workspace=None, stream=None):
+    """the live blocks become the pool's first ones (hk_mla8_pages_compact)"""
+    pool = _pages(ckv8, scales, refs, block_table, "i", ("n_live",), n_live, 1)
+    ws = _pages_scratch(ckv8, 0, workspace, stream)
+    _run("hk_mla8_pages_compact", *pool, n_live, ws, ws, stream)
+
+
+def mla8_pages_copy(ckv8, scales, to_ckv8, to_scales, src, dst, n, stream=None):
+    """blocks src[i] of one pool to blocks dst[i] of another, or of the same (hk_mla8_pages_copy)"""
+    tag, n_blocks, block = _native.cache8(ckv8, scales, None, "ii", ("src", "dst"), src, n, dst, n)[:3]
+    to_tag, to_blocks, to_block = _native.cache8(to_ckv8, to_scales, None)[:3]
+    if (tag, block) != (to_tag, to_block):
+        raise ValueError("to_ckv8: blocks of the same type and size")
+    _run("hk_mla8_pages_copy", ckv8, scales, n_blocks, to_ckv8, to_scales, to_blocks, tag, block, src, dst, n, stream)
 
 
 def mla_dense_partial(q_lat, ckv, kv_base, kv_len, pos_start, part_m, part_l, part_acc, m,

@@ -11,7 +11,7 @@ LIB = os.path.join(HERE, "libhelios_b200.so")
 BINDING = os.path.join(HERE, "_binding.so")
 SOURCES = [
     "status.cu", "kda_conv.cu", "kda_glue.cu", "kda_recurrent.cu", "kda_chunked.cu", "indexer_aux.cu",
-    "indexer_score.cu", "dsa_topk.cu", "mla_attend.cu", "mla_flash_tc.cu", "mla_append.cu", "mla8_cache.cu", "mla8_flash_tc.cu", "absorb.cu", "absorb_tc.cu",
+    "indexer_score.cu", "dsa_topk.cu", "mla_attend.cu", "mla_flash_tc.cu", "mla_append.cu", "mla8_cache.cu", "mla8_pages.cu", "mla8_flash_tc.cu", "absorb.cu", "absorb_tc.cu",
     "tc05_selftest.cu", "shim.cu",
 ]
 NVCC_FLAGS = [

@@ -177,7 +177,11 @@ struct Entry<R (*)(A...)> {
   X(hk_mla_cache_append, true) X(hk_layernorm_f16, true) X(hk_mla_decode_prologue, true) X(hk_mla_window, true)              \
   X(hk_mla8_append, true) X(hk_mla8_read, true) X(hk_mla8_dense, true) X(hk_mla8_sparse, true)                                \
   X(hk_mla8_dense_workspace_bytes, false) X(hk_mla8_sparse_workspace_bytes, false)                                        \
-  X(hk_mla_window_keys, false) X(hk_mla_window_workspace_bytes, false)
+  X(hk_mla_window_keys, false) X(hk_mla_window_workspace_bytes, false)                                                       \
+  X(hk_mla_tree, true) X(hk_mla_tree_workspace_bytes, false) X(hk_mla8_tree, true) X(hk_mla8_tree_workspace_bytes, false)    \
+  X(hk_mla_tree_accept, true) X(hk_mla8_tree_accept, true) X(hk_kda_tree_conv, true) X(hk_kda_tree, true)                    \
+  X(hk_kda_tree_accept, true) X(hk_mla8_pages_workspace_bytes, false) X(hk_mla8_pages_fork, true)                            \
+  X(hk_mla8_pages_reserve, true) X(hk_mla8_pages_free, true) X(hk_mla8_pages_compact, true) X(hk_mla8_pages_copy, true)
 
 #define X(name, stream)                                                                      \
   decltype(&::name) p_##name = nullptr;                                                      \
@@ -214,16 +218,16 @@ int device_now() {
 // an address of the host, or of another GPU than the one that the call runs on, would be a fault there
 bool elsewhere(const at::Tensor& t, int device) { return device >= 0 && (!t.is_cuda() || t.device().index() != device); }
 
-// None, or contiguous, of the type (h: float16, f: float32, i: int32, l: int64) and of as many elements as the call reads or writes, or more
+// None, or contiguous, of the type (h: float16, b: bfloat16, f: float32, i: int32, l: int64) and of as many elements as the call reads or writes, or more
 bool check_tensor(PyObject* o, char type, const char* name, long long least, int device) {
   if (o == Py_None) return true;
-  const auto want = type == 'h' ? at::kHalf : type == 'f' ? at::kFloat : type == 'i' ? at::kInt : at::kLong;
+  const auto want = type == 'h' ? at::kHalf : type == 'b' ? at::kBFloat16 : type == 'f' ? at::kFloat : type == 'i' ? at::kInt : at::kLong;
   if (THPVariable_Check(o)) {
     const at::Tensor& t = THPVariable_Unpack(o);
     if (t.scalar_type() == want && t.is_contiguous() && t.numel() >= least && !elsewhere(t, device)) return true;
   }
   PyErr_Format(PyExc_ValueError, "%s: a contiguous tensor of %s on the current CUDA device, of %lld elements or more", name,
-               type == 'h' ? "float16" : type == 'f' ? "float32" : type == 'i' ? "int32" : "int64", least);
+               type == 'h' ? "float16" : type == 'b' ? "bfloat16" : type == 'f' ? "float32" : type == 'i' ? "int32" : "int64", least);
   return false;
 }
 // (types, names, tensor, elements, tensor, elements, ...)

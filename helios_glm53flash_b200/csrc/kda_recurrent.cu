@@ -1368,3 +1368,5 @@ HK_API int hk_kda_decode_layer_beside(const float* x32, void* conv_state, const 
   return hk::decode_layer(x32, conv_state, conv_weight, conv_bias, f, b, dt_bias, a_log, lower_bound, rec_state, out, out_f32, norm_w, w_type,
                           gate_out, g_type, y, y_type, epsilon, constant_bias, gate_act, bsz, num_heads, slots, true, stream);
 }
+
+#include "kda_tree.cuh"

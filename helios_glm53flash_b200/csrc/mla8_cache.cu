@@ -10,6 +10,7 @@
 // times on average (the harmonic sum), fewer where outliers set it, and each move costs the old rows half a step at most.
 #include "hk_common.cuh"
 #include "latent8.cuh"
+#include "tree.cuh"
 
 namespace hk {
 namespace {
@@ -32,6 +33,12 @@ struct AppendArgs {
   int n;
   float eps;
   __half* ckv_new;          // optional [n][512]: the rows as the cache now holds them
+  // accepted nodes of trees of drafted tokens: the rows are those of a path, normalised already, and go behind kv_len (null: pos_start) positions
+  TreeArgs tree;
+  const __half* tree_kv;
+  const int *leaf, *kv_len;
+  int pos_start;
+  int* len_out;
 };
 
 // One CTA of sixteen warps a block that gets rows; grid (blocks of a sequence, sequences).  A warp has rows w, w + 16, ... of the block, a lane the
@@ -43,15 +50,25 @@ struct AppendArgs {
 // 4,096 (264 CTAs) 13.1 / 5.85 / 6.9; 8,192 by one / two / four 16.4 / 8.4 / 11.4, 20,000 by one / two 20.1 / 23.1.  Under 64 rows the barrier
 // of the cluster costs what it gains (32 rows in blocks of 64, one / two 4.0 / 4.7).
 constexpr int APPEND_WARPS = 16;
-template <int FMT, int ROWS, bool KEEP, int PARTS>
+template <int FMT, int ROWS, bool KEEP, int PARTS, bool TREE = false>
 __global__ void __launch_bounds__(APPEND_WARPS * 32) mla8_append_kernel(AppendArgs a) {
   __shared__ float s_amax[2][APPEND_WARPS], s_part[2];
+  __shared__ int s_node[TREE ? TREE_NODES : 1];
   pdl_release();
   pdl_wait();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, seq = blockIdx.y, block = 1 << a.pg.shift;
-  const int p0 = a.pos[seq];
+  const int p0 = TREE ? max(a.kv_len ? a.kv_len[seq] : a.pos_start, 0) : a.pos[seq];
   int r0, r1;
-  if (a.seq_start) {
+  if constexpr (TREE) {
+    const int2 rows = a.tree.rows(seq);
+    const uint64_t path = tree_path(a.tree, rows, a.leaf[seq]);
+    r0 = 0;
+    r1 = __popcll(path);
+    if (a.len_out && blockIdx.x == 0 && threadIdx.x == 0) a.len_out[seq] = p0 + r1;
+    // (a path's nodes are in ascending order)
+    if (threadIdx.x < TREE_NODES && path >> threadIdx.x & 1) s_node[__popcll(path & ((1ull << threadIdx.x) - 1))] = rows.x + threadIdx.x;
+    __syncthreads();
+  } else if (a.seq_start) {
     r0 = min(max(a.seq_start[seq], 0), a.n);
     r1 = min(max(a.seq_start[seq + 1], r0), a.n);
   } else {
@@ -70,6 +87,16 @@ __global__ void __launch_bounds__(APPEND_WARPS * 32) mla8_append_kernel(AppendAr
     float y[KEEP ? ROWS : 1][16];
     float f[ROWS];
     auto load = [&](int i, float (&x)[16]) {               // row i of the block
+      if constexpr (TREE) {
+        const uint2* src = reinterpret_cast<const uint2*>(a.tree_kv + (size_t)s_node[start + i - p0] * LATENT);
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+          const uint2 v = src[j * 32 + lane];
+          const float2 v0 = __half22float2(*reinterpret_cast<const __half2*>(&v.x)), v1 = __half22float2(*reinterpret_cast<const __half2*>(&v.y));
+          x[4 * j] = v0.x; x[4 * j + 1] = v0.y; x[4 * j + 2] = v1.x; x[4 * j + 3] = v1.y;
+        }
+        return;
+      }
       const float4* src = reinterpret_cast<const float4*>(a.kv_pre + (size_t)(r0 + (start + i - p0)) * LATENT);
 #pragma unroll
       for (int j = 0; j < 4; j++) {
@@ -85,8 +112,9 @@ __global__ void __launch_bounds__(APPEND_WARPS * 32) mla8_append_kernel(AppendAr
     const int64_t b = a.pg.block_of(seq, (int)start);
     uint2 lw[4];
 #pragma unroll
-    for (int j = 0; j < 4; j++) lw[j] = reinterpret_cast<const uint2*>(a.ln_w)[j * 32 + lane];
+    for (int j = 0; j < 4; j++) lw[j] = TREE ? make_uint2(0u, 0u) : reinterpret_cast<const uint2*>(a.ln_w)[j * 32 + lane];
     auto weigh = [&](float (&x)[16]) {
+      if (TREE) return;
 #pragma unroll
       for (int j = 0; j < 4; j++) {
         const float2 w0 = __half22float2(*reinterpret_cast<const __half2*>(&lw[j].x)), w1 = __half22float2(*reinterpret_cast<const __half2*>(&lw[j].y));
@@ -105,7 +133,7 @@ __global__ void __launch_bounds__(APPEND_WARPS * 32) mla8_append_kernel(AppendAr
         float ss = 0.f;
 #pragma unroll
         for (int c = 0; c < 16; c++) ss = fmaf(x[c], x[c], ss);
-        f[k] = rsqrtf(warp_sum(ss) / (float)LATENT + a.eps);
+        f[k] = TREE ? 1.f : rsqrtf(warp_sum(ss) / (float)LATENT + a.eps);
         weigh(x);
         float top_x = 0.f;
 #pragma unroll
@@ -195,6 +223,15 @@ cudaError_t append_launch(const AppendArgs& a, dim3 grid, int parts, cudaStream_
                                            : parts == 4 ? mla8_append_kernel<FMT, 2, true, 4>
                                            : parts == 2 ? mla8_append_kernel<FMT, 4, true, 2> : mla8_append_kernel<FMT, 8, false, 1>);
   return pdl_launch_cluster(parts, kernel, dim3(grid.x * parts, grid.y), dim3(APPEND_WARPS * 32), 0, s, a);
+}
+
+template <int FMT>
+cudaError_t accept_launch(const AppendArgs& a, cudaStream_t s) {
+  const int block = 1 << a.pg.shift;
+  const auto kernel = a.pg.shift == 4   ? mla8_append_kernel<FMT, 1, true, 1, true>
+                      : a.pg.shift == 5 ? mla8_append_kernel<FMT, 2, true, 1, true>
+                      : a.pg.shift == 6 ? mla8_append_kernel<FMT, 4, true, 1, true> : mla8_append_kernel<FMT, 8, false, 1, true>;
+  return pdl_launch(kernel, dim3((unsigned)((TREE_NODES + block - 2) / block + 1), (unsigned)a.tree.n_seqs), dim3(APPEND_WARPS * 32), 0, s, a);
 }
 
 // rows i of out: position i of the sequence below `head`, i + shift from there on; f16(scale * value), zeros where there is no block.
@@ -314,6 +351,22 @@ HK_API int hk_mla8_append(const float* kv_pre, const void* ln_w_f16, void* ckv8,
                  cudaSuccess
              ? HK_OK
              : HK_ERR_CUDA;
+}
+
+HK_API int hk_mla8_tree_accept(const void* tree_kv, void* ckv8, float* scales, int dtype, int64_t n_blocks, int block, const int* block_table,
+                               int table_stride, const int* kv_len, int pos_start, const int* parent, const int* tree_start, int n_seqs,
+                               const int* leaf, int m, int* len_out, void* stream) {
+  using namespace hk;
+  AppendArgs a{};
+  HK_REQUIRE((tree_kv || m == 0) && leaf && pos_start >= 0 && aligned(tree_kv, 16) && (!len_out || len_out != kv_len));
+  HK_REQUIRE(tree_args(&a.tree, parent, tree_start, n_seqs, m));
+  HK_REQUIRE(mla8_paged(&a.pg, ckv8, scales, dtype, n_blocks, block, block_table, table_stride, n_seqs, nullptr));
+  a.tree_kv = (const __half*)tree_kv;
+  a.leaf = leaf;
+  a.kv_len = kv_len;
+  a.pos_start = pos_start;
+  a.len_out = len_out;
+  return (dtype == HK_I8 ? accept_launch<CACHE_I8>(a, as_stream(stream)) : accept_launch<CACHE_E4M3>(a, as_stream(stream))) == cudaSuccess ? HK_OK : HK_ERR_CUDA;
 }
 
 HK_API int hk_mla8_read(const void* ckv8, const float* scales, int dtype, int64_t n_blocks, int block, const int* block_table, int table_stride,

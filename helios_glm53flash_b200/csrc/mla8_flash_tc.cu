@@ -68,6 +68,16 @@ struct F8Row {
   KeyList keys;
   int head_tiles, jump, tiles;                    // tile i of the row's list is tile i, or i + jump behind the sinks' tiles
 };
+// a node of a tree: the tile behind those of the cache is the tree's
+__device__ __forceinline__ F8Row f8_tree_row(const MlaTree& t, const MlaPaged& pg) {
+  F8Row w;
+  w.seq = t.seq;
+  w.keys = key_list(t.len, 0, 0);
+  w.keys.cut(pg.room());
+  w.head_tiles = w.jump = 0;
+  w.tiles = t.seq < 0 ? 0 : w.keys.n / F8_KEYS + (w.keys.n % F8_KEYS != 0) + 1;
+  return w;
+}
 template <bool GATHER>
 __device__ __forceinline__ F8Row f8_row(const MlaArgs& a, const MlaPaged& pg, int r) {
   F8Row w;
@@ -115,12 +125,13 @@ __device__ __forceinline__ void f8_share(const MlaArgs& a, const MlaPaged& pg, i
   it.sp = unit - it.first;
 }
 
-template <bool GATHER, int PARTS>
-__device__ __forceinline__ F8Item f8_item(const MlaArgs& a, const MlaPaged& pg, int idx) {
+// tree: the row's (trees' calls; executed by a whole warp then)
+template <bool GATHER, int PARTS, bool TREE>
+__device__ __forceinline__ F8Item f8_item(const MlaArgs& a, const MlaPaged& pg, int idx, MlaTree& tree) {
   F8Item it;
   const int groups = (a.n_heads + F8_HEADS - 1) / F8_HEADS;
   int per;
-  if (!GATHER && PARTS == 1 && a.n_split == 0) {
+  if (!GATHER && !TREE && PARTS == 1 && a.n_split == 0) {
     it.hg = idx % groups;
     it.part = 0;
     f8_share(a, pg, idx / groups, gridDim.x / groups, it, per);
@@ -138,8 +149,13 @@ __device__ __forceinline__ F8Item f8_item(const MlaArgs& a, const MlaPaged& pg, 
     idx /= a.n_split;
     it.hg = idx % groups;
     it.r = idx / groups;
-    if (!GATHER && !a.kv_len) it.r = a.m - 1 - it.r;       // rows of a causal chunk grow: the longest first
-    it.row = f8_row<GATHER>(a, pg, it.r);
+    if (!GATHER && !TREE && !a.kv_len) it.r = a.m - 1 - it.r;   // rows of a causal chunk grow: the longest first
+    if constexpr (TREE) {
+      tree = mla_tree(a, it.r);
+      it.row = f8_tree_row(tree, pg);
+    } else {
+      it.row = f8_row<GATHER>(a, pg, it.r);
+    }
     per = (it.row.tiles + a.n_split - 1) / a.n_split;
   }
   it.t0 = min(it.row.tiles, it.sp * per);
@@ -200,8 +216,9 @@ __device__ __forceinline__ void f8_tma_box(void* smem_dst, const CUtensorMap* tm
       : "memory");
 }
 
-// PARTS: CTAs that share a split's output channels
-template <bool GATHER, int FMT, int PARTS>
+// PARTS: CTAs that share a split's output channels.  TREE: a row is a node of a tree of drafted tokens, whose tile of fp16 rows (a.tree_kv, on the
+// node's path; the others are zeros) is the last of its list.
+template <bool GATHER, int FMT, int PARTS, bool TREE = false>
 __global__ __launch_bounds__(F8_THREADS, 1) void mla8_flash_tc_kernel(MlaArgs a, MlaPaged pg, int* __restrict__ status,
                                                                               const __grid_constant__ CUtensorMap tmap_q) {
   extern __shared__ __align__(1024) uint8_t smem_raw[];
@@ -230,7 +247,8 @@ __global__ __launch_bounds__(F8_THREADS, 1) void mla8_flash_tc_kernel(MlaArgs a,
   }
   if (warp == 0) tc::tmem_alloc(&ms.tmem, 512);
   pdl_wait();
-  const F8Item it = f8_item<GATHER, PARTS>(a, pg, blockIdx.x);
+  MlaTree tree{0, 0, 0, 0, 0, -1};
+  const F8Item it = f8_item<GATHER, PARTS, TREE>(a, pg, blockIdx.x, tree);
   tc::fence_before_sync();
   __syncthreads();
   tc::fence_after_sync();
@@ -269,7 +287,7 @@ __global__ __launch_bounds__(F8_THREADS, 1) void mla8_flash_tc_kernel(MlaArgs a,
       if (at >= 0) v = f8_ld_key(src + (size_t)at * LATENT);
     };
     // row of the cache, -1: none (rows of a cache are counted in 31 bits).  In a chunk a seen position without a block is a key of zeros.
-    const bool zeros = !GATHER && !a.kv_len && !pg.row_seq;
+    const bool zeros = !GATHER && !TREE && !a.kv_len && !pg.row_seq;
     auto row_of = [&](int p, int e) -> int { return e < 0 || e >= pg.n_blocks ? -1 : (e << pg.shift) + (p & in_block); };
     auto scale_of = [&](int row, int p, int e) -> float { return row >= 0 ? f8_ld_float(pg.scales + e) : zeros && p >= 0 ? 0.f : -1.f; };
     // On their way: the keys of two tiles, in registers; table entries of the third; positions of the fourth.
@@ -301,9 +319,23 @@ __global__ __launch_bounds__(F8_THREADS, 1) void mla8_flash_tc_kernel(MlaArgs a,
       p3 = position(t + 4);
       if (t == F8_NBUF - 1) ok = tc::mbar_wait<F8_POLL_NS>(&ms.q_ready, 0, abort_flag, 41) && ok;   // Q came through the last slot
       if (t >= F8_NBUF) ok = tc::mbar_wait<F8_POLL_NS>(&ms.free[b], (t / F8_NBUF - 1) & 1, abort_flag, 42) && ok;
-      if (lane < F8_ROWS) ms.sc[b][k8 + lane] = scale;
+      const bool drafted = TREE && it.t0 + t == it.row.tiles - 1;
+      if (lane < F8_ROWS) ms.sc[b][k8 + lane] = drafted ? (tree.path >> (k8 + lane) & 1 ? 1.f : -1.f) : scale;
       uint8_t* dst = smem + F8S_K + b * F8_TILE + blk * F8_BLK + k8 * 128;
       // 16 channels are two 16-byte chunks of a 128-byte row; lanes four apart write them in the other order (no bank conflicts)
+      if (TREE && drafted) {
+#pragma unroll
+        for (int i = 0; i < F8_ROWS; i++) {
+          uint4 lo = make_uint4(0u, 0u, 0u, 0u), hi = lo;
+          if (tree.path >> (k8 + i) & 1) {
+            const uint8_t* key = reinterpret_cast<const uint8_t*>(a.tree_kv + (size_t)(tree.row0 + k8 + i) * LATENT) + lane * 32;
+            lo = f8_ld_key(key);
+            hi = f8_ld_key(key + 16);
+          }
+          *reinterpret_cast<uint4*>(dst + i * 128 + ((c0 ^ i) << 4)) = lo;
+          *reinterpret_cast<uint4*>(dst + i * 128 + (((c0 + 1) ^ i) << 4)) = hi;
+        }
+      } else
 #pragma unroll
       for (int i = 0; i < F8_ROWS; i++) {
         uint4 lo, hi;                                      // the chunk that is written first, the other
@@ -605,24 +637,28 @@ __global__ __launch_bounds__(F8_THREADS, 1) void mla8_flash_tc_kernel(MlaArgs a,
   if (tid == 0 && ms.abort_flag && status) atomicExch(status, HK_ERR_TIMEOUT);
 }
 
-template <bool GATHER, int FMT, int PARTS>
+template <bool GATHER, int FMT, int PARTS, bool TREE = false>
 int f8_launch(const MlaArgs& a, const MlaPaged& pg, const CUtensorMap& q, cudaStream_t s) {
   static bool attr_set[64] = {false};
   const int dev = device_index();
   if (!attr_set[dev]) {
-    if (cudaFuncSetAttribute(mla8_flash_tc_kernel<GATHER, FMT, PARTS>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)F8_SMEM) != cudaSuccess)
+    if (cudaFuncSetAttribute(mla8_flash_tc_kernel<GATHER, FMT, PARTS, TREE>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)F8_SMEM) != cudaSuccess)
       return HK_ERR_CUDA;
     attr_set[dev] = true;
   }
   const int groups = (a.n_heads + F8_HEADS - 1) / F8_HEADS;
   const int64_t items = (a.n_split == 0 ? (int64_t)a.units : (int64_t)a.n_split * a.m * PARTS) * groups;
   if (items > INT32_MAX) return HK_ERR_UNSUPPORTED;
-  const cudaError_t e = pdl_launch(mla8_flash_tc_kernel<GATHER, FMT, PARTS>, dim3((unsigned)items), dim3(F8_THREADS), F8_SMEM, s, a, pg, device_status_ptr(), q);
+  const cudaError_t e = pdl_launch(mla8_flash_tc_kernel<GATHER, FMT, PARTS, TREE>, dim3((unsigned)items), dim3(F8_THREADS), F8_SMEM, s, a, pg, device_status_ptr(), q);
   return e == cudaSuccess && cudaPeekAtLastError() == cudaSuccess ? HK_OK : HK_ERR_CUDA;
 }
 
 template <bool GATHER, int FMT>
 int f8_launch_parts(int parts, const MlaArgs& a, const MlaPaged& pg, const CUtensorMap& q, cudaStream_t s) {
+  if constexpr (!GATHER)
+    if (a.tree_kv)
+      return parts == 1   ? f8_launch<false, FMT, 1, true>(a, pg, q, s)
+             : parts == 2 ? f8_launch<false, FMT, 2, true>(a, pg, q, s) : f8_launch<false, FMT, 4, true>(a, pg, q, s);
   return parts == 1 ? f8_launch<GATHER, FMT, 1>(a, pg, q, s) : parts == 2 ? f8_launch<GATHER, FMT, 2>(a, pg, q, s) : f8_launch<GATHER, FMT, 4>(a, pg, q, s);
 }
 

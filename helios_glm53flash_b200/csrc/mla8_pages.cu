@@ -1,0 +1,408 @@
+// Pages (blocks) of the 8-bit latent cache: who holds them, handing them out, sharing them, giving them back, moving them together.
+//
+// refs [n_blocks]: how many entries of the table name a block; 0: it is free.  Blocks are handed out lowest number first, in the order of the
+// call's sequences, so that the same calls give the same tables.  Everything is decided on the device: a call reads no length on the host, can be
+// captured, and is one small launch for the bookkeeping and, where pages move, one that moves them.
+//
+// Bookkeeping (pages_kernel): one cluster of eight CTAs, whose 256 warps take a sequence each in turn, or an eighth of a CTA's share of refs; the
+// steps of a call meet at the cluster's barrier, which also orders their accesses to global memory.  A list of free blocks in ascending order: every
+// warp counts its part of refs, the counts are added up through distributed shared memory, and the second pass writes where its count says.
+// What bounds it is latency, a few dependent loads and a barrier a step.
+#include "hk_common.cuh"
+#include "latent8.cuh"
+
+namespace hk {
+
+bool mla8_paged(MlaPaged* pg, const void* ckv8, const float* scales, int dtype, int64_t n_blocks, int block, const int* block_table,
+                int table_stride, int n_seqs, const int* row_seq);
+
+namespace {
+
+constexpr int PG_CTAS = 8, PG_THREADS = 1024, PG_WARPS = PG_CTAS * PG_THREADS / 32;
+constexpr int PG_AHEAD = 8;                       // loads of a lane on their way
+
+struct PagesArgs {
+  MlaPaged pg;
+  int* refs;
+  int* table;
+  const int *seqs, *from, *lens;        // per sequence of the call: its row, the row that it forks, positions (to keep, to have)
+  int n;
+  int* told;                            // optional: blocks that were asked for and not there (fork, reserve), live blocks (compact)
+  // workspace: pages to move (count in front), and free blocks or new numbers
+  int *count, *src, *dst, *list;
+};
+
+enum { PG_FORK, PG_RESERVE, PG_COMPACT };
+
+__device__ __forceinline__ void pg_barrier() {
+  __syncwarp();
+  asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
+}
+__device__ __forceinline__ bool pg_block(const PagesArgs& a, int e) { return e >= 0 && e < a.pg.n_blocks; }
+// entries of a row that `len` positions take, whole blocks and all
+__device__ __forceinline__ int pg_whole(const PagesArgs& a, int len) { return min(max(len, 0) >> a.pg.shift, a.pg.table_stride); }
+__device__ __forceinline__ int pg_entries(const PagesArgs& a, int len) {
+  const int over = len & ((1 << a.pg.shift) - 1);
+  return len <= 0 ? 0 : min((len >> a.pg.shift) + (over != 0), a.pg.table_stride);
+}
+__device__ __forceinline__ bool pg_seq(const PagesArgs& a, int s) { return s >= 0 && s < a.pg.n_seqs; }
+
+// entries from `first` on of a row: each gives its block back and names none (an exchange: named twice, a row is given back once)
+__device__ __forceinline__ void pg_release(const PagesArgs& a, int seq, int first) {
+  int* row = a.table + (size_t)seq * a.pg.table_stride;
+  for (int j = first + (int)(threadIdx.x & 31); j < a.pg.table_stride; j += 32) {
+    if (row[j] < 0) continue;
+    const int e = atomicExch(row + j, -1);
+    if (pg_block(a, e)) atomicSub(a.refs + e, 1);
+  }
+}
+
+__global__ __launch_bounds__(256) void pages_free_kernel(PagesArgs a) {
+  pdl_release();
+  pdl_wait();
+  const int i = blockIdx.x * 8 + (threadIdx.x >> 5);
+  if (i >= a.n) return;
+  const int s = a.seqs[i];
+  if (pg_seq(a, s)) pg_release(a, s, pg_entries(a, a.lens ? a.lens[i] : 0));
+}
+
+// Blocks [b0, b1) of this warp, in ascending order over the cluster's warps.
+struct PagesPart {
+  int64_t b0, b1;
+};
+__device__ __forceinline__ PagesPart pg_part(const PagesArgs& a, int gw) {
+  const int64_t each = (a.pg.n_blocks + PG_WARPS * 32 - 1) / (PG_WARPS * 32) * 32;
+  return {min(gw * each, a.pg.n_blocks), min((gw + 1) * each, a.pg.n_blocks)};
+}
+// f(block, references, in range) for 32 blocks at a time, ascending, by the whole warp
+template <class F>
+__device__ __forceinline__ void pg_walk(const PagesArgs& a, PagesPart p, F f) {
+  const int lane = threadIdx.x & 31;
+  for (int64_t b = p.b0; b < p.b1; b += 32 * PG_AHEAD) {
+    int r[PG_AHEAD];
+#pragma unroll
+    for (int u = 0; u < PG_AHEAD; u++) r[u] = b + 32 * u + lane < p.b1 ? a.refs[b + 32 * u + lane] : 0;
+#pragma unroll
+    for (int u = 0; u < PG_AHEAD; u++)
+      if (b + 32 * u < p.b1) f((int)(b + 32 * u) + lane, r[u], b + 32 * u + lane < p.b1);
+  }
+}
+// Of every warp's number: the sum of those before this one's, and of all.  Executed by all threads of the cluster.
+__device__ __forceinline__ int2 pg_before(int mine, int* s_count, int* s_sum) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  uint32_t rank;
+  asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
+  if (lane == 0) s_count[warp] = mine;
+  pg_barrier();
+  if (warp < PG_CTAS) {                                    // warp w: the numbers of CTA w
+    uint32_t at;
+    int v;
+    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"((uint32_t)__cvta_generic_to_shared(s_count + lane)), "r"(warp));
+    asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(at) : "memory");
+    const int sum = __reduce_add_sync(0xffffffffu, v);
+    if (lane == 0) s_sum[warp] = sum;
+  }
+  __syncthreads();
+  int before = 0, all = 0;
+  for (int c = 0; c < PG_CTAS; c++) {
+    if (c < (int)rank) before += s_sum[c];
+    all += s_sum[c];
+  }
+  before += __reduce_add_sync(0xffffffffu, lane < warp ? s_count[lane] : 0);
+  pg_barrier();                                            // the numbers have been read
+  return make_int2(before, all);
+}
+// The first `want` free blocks, ascending, into a.list; how many there are.  Executed by all threads of the cluster.
+__device__ __forceinline__ int pg_free_list(const PagesArgs& a, int gw, int want, int* s_count, int* s_sum) {
+  const PagesPart p = pg_part(a, gw);
+  const int lane = threadIdx.x & 31;
+  int mine = 0;
+  pg_walk(a, p, [&](int, int r, bool in) { mine += __popc(__ballot_sync(0xffffffffu, in && r == 0)); });
+  const int2 c = pg_before(mine, s_count, s_sum);
+  int at = c.x;
+  if (at < want)
+    pg_walk(a, p, [&](int b, int r, bool in) {
+      const uint32_t free = __ballot_sync(0xffffffffu, in && r == 0);
+      const int i = at + __popc(free & ((1u << lane) - 1));
+      if ((free >> lane & 1) && i < want) a.list[i] = b;
+      at += __popc(free);
+    });
+  return min(c.y, want);
+}
+
+template <int MODE>
+__global__ __launch_bounds__(PG_THREADS) void pages_kernel(PagesArgs a) {
+  __shared__ int s_count[32], s_sum[PG_CTAS];
+  pdl_wait();
+  const int lane = threadIdx.x & 31, gw = (int)(blockIdx.x * (PG_THREADS / 32) + (threadIdx.x >> 5)), stride = a.pg.table_stride;
+  auto row = [&](int s) -> int* { return a.table + (size_t)s * stride; };
+  if constexpr (MODE == PG_FORK) {
+    auto pair = [&](int i) { return pg_seq(a, a.seqs[i]) && pg_seq(a, a.from[i]) && a.seqs[i] != a.from[i]; };
+    for (int i = gw; i < a.n; i += PG_WARPS)
+      if (pair(i)) pg_release(a, a.seqs[i], 0);
+    pg_barrier();
+    // the block that a pair copies, -1: none
+    int want = 0;
+    for (int i0 = 0; i0 < a.n; i0 += 32) {
+      const int i = i0 + lane;
+      int e = -1;
+      if (i < a.n && pair(i)) {
+        const int whole = pg_whole(a, a.lens[i]);
+        if (pg_entries(a, a.lens[i]) > whole) e = row(a.from[i])[whole];
+        if (!pg_block(a, e)) e = -1;
+      }
+      want += __popc(__ballot_sync(0xffffffffu, e >= 0));
+      if (gw == 0 && i < a.n) a.src[i] = e;
+    }
+    const int have = pg_free_list(a, gw, want, s_count, s_sum);
+    pg_barrier();
+    for (int i = gw; i < a.n; i += PG_WARPS) {
+      int before = 0;
+      for (int k0 = 0; k0 < i; k0 += 32) before += __popc(__ballot_sync(0xffffffffu, k0 + lane < i && a.src[k0 + lane] >= 0));
+      const int e = a.src[i], fresh = e >= 0 && before < have ? a.list[before] : -1;
+      if (lane == 0) a.dst[i] = fresh;
+      if (!pair(i)) continue;
+      const int whole = pg_whole(a, a.lens[i]);
+      const int* from = row(a.from[i]);
+      int* to = row(a.seqs[i]);
+      for (int j = lane; j < whole; j += 32) {
+        const int b = from[j];
+        if (!pg_block(a, b)) continue;
+        atomicAdd(a.refs + b, 1);
+        to[j] = b;
+      }
+      if (lane == 0 && fresh >= 0) {
+        to[whole] = fresh;
+        a.refs[fresh] = 1;
+      }
+    }
+    if (gw == 0 && lane == 0) {
+      *a.count = a.n;
+      if (a.told) *a.told = want - have;
+    }
+  } else if constexpr (MODE == PG_RESERVE) {
+    // entries without a block, by sequence of the call
+    for (int i = gw; i < a.n; i += PG_WARPS) {
+      const int s = a.seqs[i], all = pg_seq(a, s) ? pg_entries(a, a.lens[i]) : 0;
+      int need = 0;
+      for (int j0 = 0; j0 < all; j0 += 32) need += __popc(__ballot_sync(0xffffffffu, j0 + lane < all && !pg_block(a, row(s)[j0 + lane])));
+      if (lane == 0) a.src[i] = need;
+    }
+    pg_barrier();
+    int64_t want = 0;
+    for (int i0 = 0; i0 < a.n; i0 += 32) {
+      const int v = i0 + lane < a.n ? a.src[i0 + lane] : 0;
+      want += __reduce_add_sync(0xffffffffu, v);
+    }
+    const int have = pg_free_list(a, gw, (int)min(want, a.pg.n_blocks), s_count, s_sum);
+    pg_barrier();
+    for (int i = gw; i < a.n; i += PG_WARPS) {
+      const int s = a.seqs[i], all = pg_seq(a, s) ? pg_entries(a, a.lens[i]) : 0;
+      int64_t at = 0;
+      for (int k0 = 0; k0 < i; k0 += 32) at += __reduce_add_sync(0xffffffffu, k0 + lane < i ? a.src[k0 + lane] : 0);
+      for (int j0 = 0; j0 < all; j0 += 32) {
+        const int j = j0 + lane, e = j < all ? row(s)[j] : 0;
+        const uint32_t open = __ballot_sync(0xffffffffu, j < all && !pg_block(a, e));
+        const int64_t k = at + __popc(open & ((1u << lane) - 1));
+        if ((open >> lane & 1) && k < have) {
+          const int b = a.list[k];
+          if (atomicCAS(row(s) + j, e, b) == e) a.refs[b] = 1;   // (a sequence that is named twice takes its blocks once)
+        }
+        at += __popc(open);
+      }
+    }
+    if (gw == 0 && lane == 0 && a.told) *a.told = (int)min(want - have, (int64_t)INT32_MAX);
+  } else {
+    // live blocks from number `live` on go to the holes below it, the i-th to the i-th
+    const PagesPart p = pg_part(a, gw);
+    int mine = 0;
+    pg_walk(a, p, [&](int, int r, bool in) { mine += __popc(__ballot_sync(0xffffffffu, in && r != 0)); });
+    const int2 c = pg_before(mine, s_count, s_sum);
+    const int live = c.y;
+    int beyond = 0;                                        // this warp's live blocks at or beyond `live`
+    if (p.b1 > live) pg_walk(a, p, [&](int b, int r, bool in) { beyond += __popc(__ballot_sync(0xffffffffu, in && r != 0 && b >= live)); });
+    const int2 m = pg_before(beyond, s_count, s_sum);
+    int hole = (int)min(p.b0, (int64_t)live) - (c.x - m.x), move = m.x;   // free blocks below `live` before this warp's
+    pg_walk(a, p, [&](int b, int r, bool in) {
+      const uint32_t up = __ballot_sync(0xffffffffu, in && r != 0 && b >= live), down = __ballot_sync(0xffffffffu, in && r == 0 && b < live);
+      if (up >> lane & 1) a.src[move + __popc(up & ((1u << lane) - 1))] = b;
+      if (down >> lane & 1) a.dst[hole + __popc(down & ((1u << lane) - 1))] = b;
+      if (in && r == 0 && b >= live) a.list[b] = -1;
+      move += __popc(up);
+      hole += __popc(down);
+    });
+    pg_barrier();
+    for (int i = gw * 32 + lane; i < m.y; i += PG_WARPS * 32) {
+      const int from = a.src[i], to = a.dst[i];
+      a.list[from] = to;
+      a.refs[to] = a.refs[from];
+      a.refs[from] = 0;
+    }
+    if (gw == 0 && lane == 0) {
+      *a.count = m.y;
+      a.count[1] = live;
+      if (a.told) *a.told = live;
+    }
+  }
+}
+
+// Pages src[i] -> dst[i] (negative: none), 8 KB a turn of a CTA, for *count of them (null: n).  Behind a compaction also the table: entries that named
+// a block which moved.
+struct CopyArgs {
+  const uint8_t* from;
+  uint8_t* to;
+  const float* from_scales;
+  float* to_scales;
+  int64_t from_blocks, to_blocks;
+  int shift;
+  const int *src, *dst, *count;
+  int n;
+  int* table;                           // or null
+  int64_t entries;
+  const int* moved;
+};
+constexpr int COPY_PIECE = 8192;
+__global__ __launch_bounds__(256) void pages_copy_kernel(CopyArgs a) {
+  pdl_wait();
+  const int n = a.count ? *a.count : a.n, lg = a.shift - 4;   // pieces of a page: 2^lg
+  const int64_t pieces = (int64_t)n << lg;
+  for (int64_t i = blockIdx.x; i < pieces; i += gridDim.x) {
+    const int k = (int)(i >> lg), part = (int)(i & ((1 << lg) - 1));
+    const int s = a.src[k], d = a.dst[k];
+    if (s < 0 || d < 0 || s >= a.from_blocks || d >= a.to_blocks) continue;
+    const uint4* x = reinterpret_cast<const uint4*>(a.from + (((size_t)s << lg) + part) * COPY_PIECE) + threadIdx.x;
+    uint4* y = reinterpret_cast<uint4*>(a.to + (((size_t)d << lg) + part) * COPY_PIECE) + threadIdx.x;
+    const uint4 v0 = x[0], v1 = x[256];
+    if (part == 0 && threadIdx.x == 0) a.to_scales[d] = a.from_scales[s];
+    y[0] = v0;
+    y[256] = v1;
+  }
+  if (a.table) {
+    const int live = a.count[1];
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < a.entries; i += (int64_t)gridDim.x * 256) {
+      const int e = a.table[i];
+      if (e >= live && e < a.from_blocks) a.table[i] = a.moved[e];
+    }
+  }
+}
+
+// arguments of a call on a pool; a table is needed
+bool pages_args(PagesArgs* a, const void* ckv8, const float* scales, int dtype, int64_t n_blocks, int block, int* refs, int* table, int stride, int n_seqs) {
+  *a = PagesArgs{};
+  if (!refs || !table || !mla8_paged(&a->pg, ckv8, scales, dtype, n_blocks, block, table, stride, n_seqs, nullptr)) return false;
+  a->refs = refs;
+  a->table = table;
+  return true;
+}
+size_t pages_list(int64_t n_blocks, int n) { return ((size_t)(n_blocks > n ? n_blocks : n) * sizeof(int) + 255) / 256 * 256; }
+bool pages_workspace(PagesArgs* a, void* workspace, size_t bytes, int* status) {
+  const size_t each = pages_list(a->pg.n_blocks, a->n);
+  *status = !workspace || bytes < 256 + 3 * each ? HK_ERR_WORKSPACE : aligned(workspace, 256) ? HK_OK : HK_ERR_INVALID;
+  if (*status != HK_OK) return false;
+  char* ws = (char*)workspace;
+  a->count = (int*)ws;
+  a->src = (int*)(ws + 256);
+  a->dst = (int*)(ws + 256 + each);
+  a->list = (int*)(ws + 256 + 2 * each);
+  return true;
+}
+template <int MODE>
+cudaError_t pages_launch(const PagesArgs& a, cudaStream_t s) {
+  return pdl_launch_cluster(PG_CTAS, pages_kernel<MODE>, dim3(PG_CTAS), dim3(PG_THREADS), 0, s, a);
+}
+CopyArgs pages_moves(const PagesArgs& a) {
+  CopyArgs c{};
+  c.from = c.to = a.pg.data;
+  c.from_scales = c.to_scales = a.pg.scales;
+  c.from_blocks = c.to_blocks = a.pg.n_blocks;
+  c.shift = a.pg.shift;
+  c.src = a.src; c.dst = a.dst; c.count = a.count;
+  return c;
+}
+// CTAs of a copy of up to `pages` pages: eight an SM, less where there is less to do
+unsigned copy_ctas(int64_t pages, int shift) {
+  const int64_t all = pages << (shift - 4), room = 8 * sm_count();
+  return (unsigned)(all < 1 ? 1 : all < room ? all : room);
+}
+
+}  // namespace
+}  // namespace hk
+
+HK_API size_t hk_mla8_pages_workspace_bytes(int64_t n_blocks, int n) {
+  return n_blocks < 1 || n_blocks > INT32_MAX || n < 0 ? 0 : 256 + 3 * hk::pages_list(n_blocks, n);
+}
+
+HK_API int hk_mla8_pages_fork(void* ckv8, float* scales, int dtype, int64_t n_blocks, int block, int* refs, int* block_table, int table_stride,
+                              int n_seqs, const int* parents, const int* children, const int* lens, int n, int* missing, void* workspace,
+                              size_t workspace_bytes, void* stream) {
+  using namespace hk;
+  PagesArgs a;
+  HK_REQUIRE(pages_args(&a, ckv8, scales, dtype, n_blocks, block, refs, block_table, table_stride, n_seqs) && parents && children && lens && n >= 0);
+  if (n == 0) return HK_OK;
+  a.from = parents; a.seqs = children; a.lens = lens;
+  a.n = n;
+  a.told = missing;
+  int st;
+  if (!pages_workspace(&a, workspace, workspace_bytes, &st)) return st;
+  if (pages_launch<PG_FORK>(a, as_stream(stream)) != cudaSuccess) return HK_ERR_CUDA;
+  return pdl_launch(pages_copy_kernel, dim3(copy_ctas(n, a.pg.shift)), dim3(256), 0, as_stream(stream), pages_moves(a)) == cudaSuccess ? HK_OK : HK_ERR_CUDA;
+}
+
+HK_API int hk_mla8_pages_reserve(void* ckv8, float* scales, int dtype, int64_t n_blocks, int block, int* refs, int* block_table, int table_stride,
+                                 int n_seqs, const int* seqs, const int* lens, int n, int* missing, void* workspace, size_t workspace_bytes, void* stream) {
+  using namespace hk;
+  PagesArgs a;
+  HK_REQUIRE(pages_args(&a, ckv8, scales, dtype, n_blocks, block, refs, block_table, table_stride, n_seqs) && seqs && lens && n >= 0);
+  if (n == 0) return HK_OK;
+  a.seqs = seqs; a.lens = lens;
+  a.n = n;
+  a.told = missing;
+  int st;
+  if (!pages_workspace(&a, workspace, workspace_bytes, &st)) return st;
+  return pages_launch<PG_RESERVE>(a, as_stream(stream)) == cudaSuccess ? HK_OK : HK_ERR_CUDA;
+}
+
+HK_API int hk_mla8_pages_free(void* ckv8, float* scales, int dtype, int64_t n_blocks, int block, int* refs, int* block_table, int table_stride,
+                              int n_seqs, const int* seqs, const int* keep, int n, void* stream) {
+  using namespace hk;
+  PagesArgs a;
+  HK_REQUIRE(pages_args(&a, ckv8, scales, dtype, n_blocks, block, refs, block_table, table_stride, n_seqs) && seqs && n >= 0);
+  if (n == 0) return HK_OK;
+  a.seqs = seqs; a.lens = keep;
+  a.n = n;
+  return pdl_launch(pages_free_kernel, dim3((unsigned)((n + 7) / 8)), dim3(256), 0, as_stream(stream), a) == cudaSuccess ? HK_OK : HK_ERR_CUDA;
+}
+
+HK_API int hk_mla8_pages_compact(void* ckv8, float* scales, int dtype, int64_t n_blocks, int block, int* refs, int* block_table, int table_stride,
+                                 int n_seqs, int* n_live, void* workspace, size_t workspace_bytes, void* stream) {
+  using namespace hk;
+  PagesArgs a;
+  HK_REQUIRE(pages_args(&a, ckv8, scales, dtype, n_blocks, block, refs, block_table, table_stride, n_seqs));
+  a.told = n_live;
+  int st;
+  if (!pages_workspace(&a, workspace, workspace_bytes, &st)) return st;
+  if (pages_launch<PG_COMPACT>(a, as_stream(stream)) != cudaSuccess) return HK_ERR_CUDA;
+  CopyArgs c = pages_moves(a);
+  c.table = block_table;
+  c.entries = (int64_t)table_stride * n_seqs;
+  c.moved = a.list;
+  return pdl_launch(pages_copy_kernel, dim3(copy_ctas(n_blocks / 2 + c.entries / 1024, a.pg.shift)), dim3(256), 0, as_stream(stream), c) == cudaSuccess ? HK_OK
+                                                                                                                                             : HK_ERR_CUDA;
+}
+
+HK_API int hk_mla8_pages_copy(const void* from_ckv8, const float* from_scales, int64_t from_blocks, void* to_ckv8, float* to_scales, int64_t to_blocks,
+                              int dtype, int block, const int* src, const int* dst, int n, void* stream) {
+  using namespace hk;
+  MlaPaged x, y;
+  HK_REQUIRE(mla8_paged(&x, from_ckv8, from_scales, dtype, from_blocks, block, nullptr, 0, 1, nullptr) && src && dst && n >= 0);
+  HK_REQUIRE(mla8_paged(&y, to_ckv8, to_scales, dtype, to_blocks, block, nullptr, 0, 1, nullptr));
+  if (n == 0) return HK_OK;
+  CopyArgs c{};
+  c.from = x.data; c.to = y.data;
+  c.from_scales = x.scales; c.to_scales = y.scales;
+  c.from_blocks = from_blocks; c.to_blocks = to_blocks;
+  c.shift = x.shift;
+  c.src = src; c.dst = dst;
+  c.n = n;
+  return pdl_launch(pages_copy_kernel, dim3(copy_ctas(n, x.shift)), dim3(256), 0, as_stream(stream), c) == cudaSuccess ? HK_OK : HK_ERR_CUDA;
+}

@@ -8,6 +8,7 @@
 // those four warps in turn and the four warp sums are combined in the reference's order
 // ((s0 + s2) + (s1 + s3)), so the results are the same bits.
 #include "hk_common.cuh"
+#include "tree.cuh"
 #include "kpool_common.cuh"
 
 namespace hk {
@@ -201,4 +202,43 @@ HK_API int hk_mla_decode_prologue(const float* kv_pre, const void* ln_w_f16, voi
     return HK_ERR_CUDA;
   HK_LAUNCH_CHECK();
   return HK_OK;
+}
+
+// ---------------------------------------------------------------------------------------------
+// The accepted nodes of trees of drafted tokens: rows of a path become cached rows.  One CTA a sequence, a warp a row of 1 KB.
+// ---------------------------------------------------------------------------------------------
+namespace hk {
+__global__ __launch_bounds__(256) void mla_tree_accept_kernel(const uint4* tree_kv, uint4* ckv, int64_t ckv_rows, const int64_t* kv_base, const int* kv_len,
+                                                              int pos_start, TreeArgs tree, const int* leaf, int* len_out) {
+  pdl_release();
+  pdl_wait();
+  const int s = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int2 rows = tree.rows(s);
+  const int len = max(kv_len ? kv_len[s] : pos_start, 0);
+  const uint64_t path = tree_path(tree, rows, leaf[s]);
+  if (len_out && threadIdx.x == 0) len_out[s] = len + __popcll(path);
+  const int64_t to = (kv_base ? kv_base[s] : 0) + len;
+  int i = 0;
+  for (uint64_t m = path; m; m &= m - 1, i++) {            // (a path's nodes are in ascending order)
+    if (i % 8 != warp) continue;
+    const int64_t dst = to + i;
+    if (dst < 0 || (ckv_rows > 0 && dst >= ckv_rows)) continue;
+    const uint4* src = tree_kv + (size_t)(rows.x + __ffsll((long long)m) - 1) * (LATENT / 8);
+    const uint4 a = src[lane], b = src[lane + 32];
+    ckv[dst * (LATENT / 8) + lane] = a;
+    ckv[dst * (LATENT / 8) + lane + 32] = b;
+  }
+}
+}  // namespace hk
+
+HK_API int hk_mla_tree_accept(const void* tree_kv, void* ckv, int64_t ckv_rows, const int64_t* kv_base, const int* kv_len, int pos_start,
+                              const int* parent, const int* tree_start, int n_seqs, const int* leaf, int m, int* len_out, void* stream) {
+  using namespace hk;
+  TreeArgs t;
+  HK_REQUIRE((tree_kv || m == 0) && ckv && leaf && ckv_rows >= 0 && pos_start >= 0 && aligned(tree_kv, 16) && aligned(ckv, 16) && (!len_out || len_out != kv_len));
+  HK_REQUIRE(tree_args(&t, parent, tree_start, n_seqs, m));
+  return pdl_launch(mla_tree_accept_kernel, dim3((unsigned)n_seqs), dim3(256), 0, as_stream(stream), (const uint4*)tree_kv, (uint4*)ckv, ckv_rows, kv_base,
+                    kv_len, pos_start, t, leaf, len_out) == cudaSuccess
+             ? HK_OK
+             : HK_ERR_CUDA;
 }

@@ -1,6 +1,7 @@
 // Argument block shared by the MLA attention kernels of this library.
 #pragma once
 #include "hk_common.cuh"
+#include "tree.cuh"
 
 namespace hk {
 
@@ -26,6 +27,9 @@ struct MlaArgs {
   // n_split == 0 (8-bit cache): splits shared out on the device among `units` CTAs, whose first and number each row's first CTA stores
   int units;
   int2* shares;
+  // trees of drafted tokens: row r is a node of tree.seq_of(r), whose cached keys kv_base and kv_len (then per sequence) say
+  TreeArgs tree;
+  const __half* tree_kv;    // [m][512] the nodes' own latents
   int keep_nan;             // keys that are not finite make outputs that are NaN (0: zeros where the scores are, as hk_mla_dense's callers know it)
 };
 
@@ -52,6 +56,28 @@ struct MlaPaged {
     return s >= n_seqs ? -1 : s;
   }
 };
+
+// A row that is a node of a tree of drafted tokens: its sequence's cached keys, then the nodes of its path (a bit each) out of the tree's rows.
+struct MlaTree {
+  int64_t base;
+  uint64_t path;
+  int seq, len, row0, node;                       // seq < 0: a row of no tree, without keys
+};
+// executed by a whole warp
+__device__ __forceinline__ MlaTree mla_tree(const MlaArgs& a, int r) {
+  MlaTree t{0, 0, a.tree.seq_of(r), 0, 0, -1};
+  if (t.seq < 0) return t;
+  const int2 rows = a.tree.rows(t.seq);
+  TreeParents up;
+  up.load(a.tree, rows);
+  t.row0 = rows.x;
+  t.node = r - rows.x;
+  t.path = up.path(t.node);
+  t.base = a.kv_base ? a.kv_base[t.seq] : 0;
+  t.len = max(a.kv_len ? a.kv_len[t.seq] : a.pos_start, 0);
+  if (a.ckv_rows > 0) t.len = (int)max((int64_t)0, min((int64_t)t.len, a.ckv_rows - t.base));   // never past the end of the cache
+  return t;
+}
 
 // The keys that a row attends to, as a list: the first `head` positions, then lo .. n - 1.
 struct KeyList {

@@ -687,4 +687,67 @@ HK_API int hk_mla_window(const void* q_lat, const void* ckv, int64_t ckv_rows, c
                 as_stream(stream));
 }
 
+namespace hk {
+// keys of a node, for choosing the splits of a tree call: the cached ones (with kv_len pos_start says about how many, 4,096 where it is 0), and the tree's tile
+static int tree_keys(bool lens, int pos_start) {
+  const int n = lens && pos_start == 0 ? 4096 : pos_start;
+  return n > INT32_MAX - TREE_NODES ? n : n + TREE_NODES;
+}
+static bool tree_call(MlaArgs* a, const void* q_lat, const void* tree_kv, const int* parent, const int* tree_start, int n_seqs, const int* kv_len,
+                      int pos_start, void* lat_out, int m, int n_heads, float scale) {
+  *a = MlaArgs{};
+  if ((m > 0 && (!q_lat || !lat_out || !tree_kv)) || !aligned(q_lat, 16) || !aligned(lat_out, 16) || !aligned(tree_kv, 16)) return false;
+  if (pos_start < 0 || n_heads <= 0 || n_heads % SIMT_HG != 0 || !tree_args(&a->tree, parent, tree_start, n_seqs, m)) return false;
+  a->q_lat = (const __half*)q_lat;
+  a->kv_len = kv_len; a->pos_start = pos_start;
+  a->m = m; a->n_heads = n_heads; a->scale = scale;
+  a->out = (__half*)lat_out;
+  a->tree_kv = (const __half*)tree_kv;
+  a->keep_nan = 1;
+  return true;
+}
+}  // namespace hk
+
+HK_API size_t hk_mla_tree_workspace_bytes(int m, int n_heads, int n_keys) {
+  if (m <= 0 || n_heads < hk::SIMT_HG || n_keys < 0) return 0;
+  const int splits = hk::attend_splits(m, n_heads, hk::tree_keys(true, n_keys), 0);
+  return splits > 1 ? hk_mla_partial_bytes(splits, (int64_t)m * n_heads) : 0;
+}
+
+HK_API size_t hk_mla8_tree_workspace_bytes(int m, int n_heads, int n_keys) {
+  if (m <= 0 || n_heads < hk::SIMT_HG || n_keys < 0) return 0;
+  int units = 0;
+  return hk::attend8_bytes(m, n_heads, hk::attend8_splits(m, n_heads, hk::tree_keys(true, n_keys), false, &units), 0);
+}
+
+HK_API int hk_mla_tree(const void* q_lat, const void* ckv, int64_t ckv_rows, const int64_t* kv_base, const int* kv_len, int pos_start,
+                       const void* tree_kv, const int* parent, const int* tree_start, int n_seqs, void* lat_out, int m, int n_heads, float scale,
+                       int n_split, void* workspace, size_t workspace_bytes, void* stream) {
+  using namespace hk;
+  MlaArgs a;
+  HK_REQUIRE(tree_call(&a, q_lat, tree_kv, parent, tree_start, n_seqs, kv_len, pos_start, lat_out, m, n_heads, scale));
+  HK_REQUIRE(ckv && ckv_rows >= 0 && aligned(ckv, 16));
+  if (ckv_rows > 0 && !kv_base && !kv_len) HK_REQUIRE(pos_start <= ckv_rows);
+  if (m == 0) return HK_OK;
+  if (n_split > LSE_MAX_SPLITS) return HK_ERR_UNSUPPORTED;
+  a.ckv = (const __half*)ckv; a.ckv_rows = ckv_rows;
+  a.kv_base = kv_base;
+  return attend(a, tree_keys(kv_len, pos_start), n_split, false, workspace, workspace_bytes, as_stream(stream));
+}
+
+HK_API int hk_mla8_tree(const void* q_lat, const void* ckv8, const float* scales, int dtype, int64_t n_blocks, int block, const int* block_table,
+                        int table_stride, const int* kv_len, int pos_start, const void* tree_kv, const int* parent, const int* tree_start,
+                        int n_seqs, void* lat_out, int m, int n_heads, float scale, int n_split, void* workspace, size_t workspace_bytes,
+                        void* stream) {
+  using namespace hk;
+  MlaArgs a;
+  MlaPaged pg;
+  HK_REQUIRE(tree_call(&a, q_lat, tree_kv, parent, tree_start, n_seqs, kv_len, pos_start, lat_out, m, n_heads, scale));
+  HK_REQUIRE(mla8_paged(&pg, ckv8, scales, dtype, n_blocks, block, block_table, table_stride, n_seqs, nullptr));
+  if (m == 0) return HK_OK;
+  int units = 0;
+  const int keys = tree_keys(kv_len, pos_start);
+  return attend8(a, pg, dtype, keys, n_split > 0 ? n_split : attend8_splits(m, n_heads, keys, false, &units), workspace, workspace_bytes, as_stream(stream));
+}
+
 #include "mla_splitkv_heads.cuh"

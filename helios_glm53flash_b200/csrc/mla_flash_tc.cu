@@ -94,6 +94,7 @@ struct FtMisc {
   float l[128];
   uint32_t tmem;
   int abort_flag;
+  MlaTree tree;
 };
 static_assert(sizeof(FtMisc) <= 2048, "misc area");
 
@@ -105,16 +106,19 @@ struct FtItem {
   // window form: keys p >= lo and p < head of the row's k1 are seen; tile i of its list is tile i, or i + jump behind the sinks' tiles
   int head, lo, head_tiles, jump, t0;
   bool win;
-  __device__ __forceinline__ int key0(int t) const { return win ? (t0 + t < head_tiles ? t0 + t : t0 + t + jump) * FT_KEYS : k0 + t * FT_KEYS; }   // first key of a tile
-  __device__ __forceinline__ int keys(int t) const { return min(FT_KEYS, k1 - key0(t)); }
+  int past, nodes;                                // tree form: tile `past` of the row's list is the tree's, with `nodes` keys (past < 0: no tree)
+  __device__ __forceinline__ bool drafted(int t) const { return past >= 0 && t0 + t == past; }
+  __device__ __forceinline__ int key0(int t) const { return past >= 0 ? (t0 + t) * FT_KEYS : win ? (t0 + t < head_tiles ? t0 + t : t0 + t + jump) * FT_KEYS : k0 + t * FT_KEYS; }   // first key of a tile
+  __device__ __forceinline__ int keys(int t) const { return drafted(t) ? nodes : min(FT_KEYS, k1 - key0(t)); }
   __device__ __forceinline__ bool sees(int p) const { return !win || p >= lo || p < head; }
-  __device__ __forceinline__ bool whole(int t) const { return keys(t) == FT_KEYS && (!win || key0(t) >= lo || key0(t) + FT_KEYS <= head); }
+  __device__ __forceinline__ bool whole(int t) const { return !drafted(t) && keys(t) == FT_KEYS && (!win || key0(t) >= lo || key0(t) + FT_KEYS <= head); }
   __device__ __forceinline__ int nth(int i) const { return mini ? (i ? i - 1 : n_tiles - 1) : i; }   // the tile that is i-th in turn
 };
 template <bool G4, bool CL, bool WIN>
 __device__ __forceinline__ FtItem ft_item(const MlaArgs& a, int idx) {
   FtItem it;
   it.win = WIN;
+  it.past = -1;
   it.sp = idx % a.n_split;
   it.r = idx / a.n_split;
   it.cs = 0;
@@ -165,6 +169,24 @@ __device__ __forceinline__ FtItem ft_item(const MlaArgs& a, int idx) {
   return it;
 }
 
+// tree form: the row is the CTA's only one
+__device__ __forceinline__ FtItem ft_tree_item(const MlaArgs& a, const MlaTree& tree, int idx) {
+  FtItem it;
+  it.win = it.mini = false;
+  it.sp = idx % a.n_split;
+  it.r = idx / a.n_split;
+  it.cs = 0;
+  it.base = tree.base;
+  it.k0 = 0;
+  it.k1 = tree.len;
+  it.past = tree.len / FT_KEYS + (tree.len % FT_KEYS != 0);
+  it.nodes = tree.node + 1;
+  const int tiles = tree.node < 0 ? 0 : it.past + 1, per = (tiles + a.n_split - 1) / a.n_split;
+  it.t0 = min(tiles, it.sp * per);
+  it.n_tiles = min(tiles, it.t0 + per) - it.t0;
+  return it;
+}
+
 __device__ __forceinline__ void tma_load_tile(void* smem_dst, const CUtensorMap* tmap, int row, uint64_t* bar) {
   asm volatile(
       "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(
@@ -201,10 +223,11 @@ __device__ __forceinline__ void tma_gather4_rows(uint32_t leader, uint32_t smem_
 // 9.2 us; MLA layer of one token at 5,001 32.1 -> 28.9, selection and attention at 262,144 23.8 -> 21.8.
 // WIN: dense ranges of which a row sees its last keys and its first ones only (a.window, a.sinks).
 // PARTS: CTAs that share a partial's output channels, each with the scores for itself (few splits of few rows: 128 KB of a partial take 3 us).
-template <bool G4, bool CL, bool WIN, int PARTS = 1>
-__global__ __launch_bounds__(FT_THREADS, 1) void mla_flash_tc_kernel(
-    MlaArgs a, int* __restrict__ status, const __grid_constant__ CUtensorMap tmap_box, const __grid_constant__ CUtensorMap tmap_rows,
-    const __grid_constant__ CUtensorMap tmap_q, const __grid_constant__ CUtensorMap tmap_o) {
+// TREE: a row is a node of a tree of drafted tokens (a.tree).  The tree's tile is the last of the row's list: of its 64 slots those on the node's
+// path are gathered out of a.tree_kv (tmap_tree), the others are zeros, whatever lies there.
+template <bool G4, bool CL, bool WIN, int PARTS, bool TREE>
+__device__ __forceinline__ void ft_body(const MlaArgs& a, int* __restrict__ status, const CUtensorMap& tmap_box, const CUtensorMap& tmap_rows,
+                                        const CUtensorMap& tmap_q, const CUtensorMap& tmap_o, const CUtensorMap& tmap_tree) {
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* smem = smem_raw + ((1024u - (tc::smem_u32(smem_raw) & 1023u)) & 1023u);
   FtMisc& ms = *reinterpret_cast<FtMisc*>(smem + FS_MISC);
@@ -240,10 +263,22 @@ __global__ __launch_bounds__(FT_THREADS, 1) void mla_flash_tc_kernel(
   }
   if (warp == 0) tc::tmem_alloc(&ms.tmem, 512);
   pdl_wait();
-  if (!CL && step >= n_items) direct_q = ft_item<G4, CL, WIN>(a, blockIdx.x / PARTS).n_tiles < FT_NBUF;
+  auto item = [&](int idx) -> FtItem {
+    if constexpr (TREE) return ft_tree_item(a, ms.tree, idx / PARTS);
+    else return ft_item<G4, CL, WIN>(a, idx / PARTS);
+  };
+  if constexpr (TREE) {
+    if (warp == 0) {
+      const MlaTree t = mla_tree(a, blockIdx.x / (PARTS * a.n_split));
+      if (lane == 0) ms.tree = t;
+    }
+  } else {
+    if (!CL && step >= n_items) direct_q = item(blockIdx.x).n_tiles < FT_NBUF;
+  }
   tc::fence_before_sync();
   __syncthreads();
   tc::fence_after_sync();
+  if constexpr (TREE) direct_q = item(blockIdx.x).n_tiles < FT_NBUF;
   const uint32_t tmem = ms.tmem;
   bool ok = true;
 
@@ -260,7 +295,8 @@ __global__ __launch_bounds__(FT_THREADS, 1) void mla_flash_tc_kernel(
     const uint32_t leader = tc::elect_one();
     // cache row of key slot lw * SLOTS + lane of a tile, -1 = hole; volatile, so that a look-ahead load is issued where it stands
     auto row_of = [&](const FtItem& it, int tile) -> int {
-      const int p = it.key0(tile) + lw * FT_SLOTS + lane;
+      const int slot = lw * FT_SLOTS + lane, p = it.key0(tile) + slot;
+      if (TREE && it.drafted(tile)) return lane < FT_SLOTS && (ms.tree.path >> slot & 1) ? ms.tree.row0 + slot : -1;
       if (lane >= FT_SLOTS || p >= it.k1 || !it.sees(p)) return -1;
       if (!G4) return (int)(it.base + p);
       int v;
@@ -271,14 +307,14 @@ __global__ __launch_bounds__(FT_THREADS, 1) void mla_flash_tc_kernel(
     auto in_cache = [&](int v) -> int { return (v < 0 || (a.ckv_rows > 0 && (int64_t)v >= a.ckv_rows)) ? -1 : v; };
     // Gathered row numbers are fetched two tiles ahead (the row list of a query is read once, from HBM), across rows.
     int cur = -1, nxt = -1, ahead_item = blockIdx.x, ahead_tile = 0;
-    FtItem ahead = ft_item<G4, CL, WIN>(a, ahead_item / PARTS);
+    FtItem ahead = item(ahead_item);
     auto fetch = [&]() -> int {
       if (!G4 || ahead_item >= n_items || ahead.n_tiles == 0) return -1;   // (gathered rows: every item has the same keys)
       const int v = row_of(ahead, ahead.nth(ahead_tile));
       if (++ahead_tile == ahead.n_tiles) {
         ahead_tile = 0;
         ahead_item += step;
-        if (ahead_item < n_items) ahead = ft_item<G4, CL, WIN>(a, ahead_item / PARTS);
+        if (ahead_item < n_items) ahead = item(ahead_item);
       }
       return v;
     };
@@ -295,7 +331,7 @@ __global__ __launch_bounds__(FT_THREADS, 1) void mla_flash_tc_kernel(
       return b;
     };
     for (int idx = blockIdx.x; idx < n_items; idx += step) {
-      const FtItem it = ft_item<G4, CL, WIN>(a, idx / PARTS);
+      const FtItem it = item(idx);
       if (it.n_tiles == 0) continue;
       {
         const int b = next_slot(it, -1);
@@ -340,13 +376,14 @@ __global__ __launch_bounds__(FT_THREADS, 1) void mla_flash_tc_kernel(
           __syncwarp();
           if (none) continue;
           const uint32_t dst = tc::smem_u32(smem) + tile_at(b) + lw * FT_SLOTS * 128, bar = tc::smem_u32(full_of(b)), blk_bytes = blk_of(b);
+          const CUtensorMap* rows = TREE && it.drafted(tile) ? &tmap_tree : &tmap_rows;
 #pragma unroll
           for (int j = 0; j < FT_SLOTS / 4; j++) {
             const int r0 = __shfl_sync(0xffffffffu, row, 4 * j), r1 = __shfl_sync(0xffffffffu, row, 4 * j + 1);
             const int r2 = __shfl_sync(0xffffffffu, row, 4 * j + 2), r3 = __shfl_sync(0xffffffffu, row, 4 * j + 3);
 #pragma unroll
             for (int blk = 0; blk < 8; blk++)
-              tma_gather4_rows(leader, dst + blk * blk_bytes + j * 512, &tmap_rows, blk * 64, r0, r1, r2, r3, bar);
+              tma_gather4_rows(leader, dst + blk * blk_bytes + j * 512, rows, blk * 64, r0, r1, r2, r3, bar);
           }
         }
       }
@@ -374,7 +411,7 @@ __global__ __launch_bounds__(FT_THREADS, 1) void mla_flash_tc_kernel(
         return tc::make_sdesc_sw128(addr, 16, 1024);
       };
       for (int idx = blockIdx.x; idx < n_items; idx += step) {
-        const FtItem it = ft_item<G4, CL, WIN>(a, idx / PARTS);
+        const FtItem it = item(idx);
         const int n_tiles = it.n_tiles;
         if (n_tiles == 0) continue;
         if (direct_q) wait_u(&ms.full[0], 0, 15);
@@ -411,7 +448,7 @@ __global__ __launch_bounds__(FT_THREADS, 1) void mla_flash_tc_kernel(
     } else {
       const uint32_t idesc = tc::make_idesc(64, PARTS == 4 ? 128 : 256, tc::FMT_F16, tc::FMT_F16, false, true);
       for (int idx = blockIdx.x; idx < n_items; idx += step) {
-        const FtItem it = ft_item<G4, CL, WIN>(a, idx / PARTS);
+        const FtItem it = item(idx);
         if (it.n_tiles == 0) continue;
         u++;
         for (int tile = 0; tile < it.n_tiles; tile++, u++, g++) {
@@ -482,14 +519,14 @@ __global__ __launch_bounds__(FT_THREADS, 1) void mla_flash_tc_kernel(
       u++;
     };
     auto next_row = [&](int idx) {                         // the first item from idx on that has keys
-      while (idx < n_items && ft_item<G4, CL, WIN>(a, idx / PARTS).n_tiles == 0) idx += step;
+      while (idx < n_items && item(idx).n_tiles == 0) idx += step;
       return idx;
     };
     int q_item = next_row(blockIdx.x);                     // the row whose Q is moved next
     if (direct_q) u = 1;
     else if (q_item < n_items) move_q();
     for (int idx = blockIdx.x; idx < n_items; idx += step) {
-      const FtItem it = ft_item<G4, CL, WIN>(a, idx / PARTS);
+      const FtItem it = item(idx);
       float m = -INFINITY, l = 0.f;
       for (int tile = 0; tile < it.n_tiles; tile++, u++, g++) {
         const int b = g & 1, kb = slot_of(it, u, tile);
@@ -683,7 +720,7 @@ __global__ __launch_bounds__(FT_THREADS, 1) void mla_flash_tc_kernel(
     }
     ok = tc::mbar_wait(&ms.q_ready, 0, abort_flag, 16) && ok;   // every split's share of this CTA's heads has arrived
     cluster_arrive();
-    const FtItem it = ft_item<G4, CL, WIN>(a, blockIdx.x / PARTS);
+    const FtItem it = item(blockIdx.x);
     const int n_h = FT_HEADS / a.n_split, row = FT_CL_ROW, share = n_h * (row + 8), chunks = row / 16;
     if (!*abort_flag) {
       for (int i = tid; i < n_h * chunks; i += FT_THREADS) {
@@ -721,6 +758,19 @@ __global__ __launch_bounds__(FT_THREADS, 1) void mla_flash_tc_kernel(
   if (tid == 0 && ms.abort_flag && status) atomicExch(status, HK_ERR_TIMEOUT);
 }
 
+template <bool G4, bool CL, bool WIN, int PARTS = 1>
+__global__ __launch_bounds__(FT_THREADS, 1) void mla_flash_tc_kernel(
+    MlaArgs a, int* __restrict__ status, const __grid_constant__ CUtensorMap tmap_box, const __grid_constant__ CUtensorMap tmap_rows,
+    const __grid_constant__ CUtensorMap tmap_q, const __grid_constant__ CUtensorMap tmap_o) {
+  ft_body<G4, CL, WIN, PARTS, false>(a, status, tmap_box, tmap_rows, tmap_q, tmap_o, tmap_rows);
+}
+template <int PARTS>
+__global__ __launch_bounds__(FT_THREADS, 1) void mla_tree_tc_kernel(
+    MlaArgs a, int* __restrict__ status, const __grid_constant__ CUtensorMap tmap_box, const __grid_constant__ CUtensorMap tmap_rows,
+    const __grid_constant__ CUtensorMap tmap_q, const __grid_constant__ CUtensorMap tmap_o, const __grid_constant__ CUtensorMap tmap_tree) {
+  ft_body<false, false, false, PARTS, true>(a, status, tmap_box, tmap_rows, tmap_q, tmap_o, tmap_tree);
+}
+
 }  // namespace hk
 #include "mla_pair_tc.cuh"
 namespace hk {
@@ -753,7 +803,7 @@ static int ft_prepare() {
         !whole_sm(mla_flash_tc_kernel<false, true, false>) || !whole_sm(mla_flash_tc_kernel<true, true, false>) ||
         !whole_sm(mla_flash_tc_kernel<false, false, true>) || !whole_sm(mla_flash_tc_kernel<false, false, true, 2>) ||
         !whole_sm(mla_flash_tc_kernel<false, false, true, 4>) || !whole_sm(mla_flash_tc_kernel<false, true, true>) || !whole_sm(mla_pair_tc_kernel<false>) ||
-        !whole_sm(mla_pair_tc_kernel<true>) ||
+        !whole_sm(mla_pair_tc_kernel<true>) || !whole_sm(mla_tree_tc_kernel<1>) || !whole_sm(mla_tree_tc_kernel<2>) || !whole_sm(mla_tree_tc_kernel<4>) ||
         !any_cluster(mla_flash_tc_kernel<false, true, false>) || !any_cluster(mla_flash_tc_kernel<true, true, false>) ||
         !any_cluster(mla_flash_tc_kernel<false, true, true>))
       return HK_ERR_CUDA;
@@ -834,14 +884,15 @@ int mla_flash_tc_launch(const MlaArgs& a, cudaStream_t s, bool clusters) {
   memset(&omap, 0, sizeof(omap));
   const cuuint64_t extent = a.ckv_rows > 0 ? (cuuint64_t)a.ckv_rows : (cuuint64_t)1 << 31;
   const cuuint32_t ones[3] = {1, 1, 1};
-  {
-    const cuuint64_t dims[2] = {LATENT, extent};
+  // single rows x one block of 64 channels, for gather4
+  auto rows_map = [&](CUtensorMap* m, const void* p, cuuint64_t n) {
+    const cuuint64_t dims[2] = {LATENT, n};
     const cuuint64_t strides[1] = {LATENT * 2};
     const cuuint32_t b[2] = {64, 1};
-    if (encode(&rows, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, (void*)a.ckv, dims, strides, b, ones, CU_TENSOR_MAP_INTERLEAVE_NONE,
-               CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
-      return HK_ERR_UNSUPPORTED;
-  }
+    return encode(m, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, const_cast<void*>(p), dims, strides, b, ones, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                  CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+  };
+  if (!rows_map(&rows, a.ckv, extent)) return HK_ERR_UNSUPPORTED;
   // 64 rows x 512 channels as one box: whole key tiles of a dense range, and a row's 64 heads of Q
   auto box_map = [&](CUtensorMap* m, const void* p, cuuint64_t n, cuuint32_t keys = 64, cuuint32_t blocks = 8) {
     const cuuint64_t dims[3] = {64, n, 8};
@@ -859,7 +910,7 @@ int mla_flash_tc_launch(const MlaArgs& a, cudaStream_t s, bool clusters) {
   // not: 2,048 rows at 30,000, persistent / pairs, us, window 1,500 430 / 455, 2,000 535 / 542, 2,800 714 / 702, 4,096 1,003 / 957, 16,384
   // 3,989 / 3,484.
   const int seen = a.window > 0 ? min(a.pos_start + a.m / 2, mla_window_keys(0, a.window, a.sinks)) : a.pos_start + a.m / 2;
-  const bool pairs = !clusters && !a.raw_idx && !a.kv_len && !a.kv_base && a.out && a.n_split == 1 && a.m >= 2 &&
+  const bool pairs = !clusters && !a.raw_idx && !a.tree_kv && !a.kv_len && !a.kv_base && a.out && a.n_split == 1 && a.m >= 2 &&
                      seen >= (a.window > 0 ? FT_WINDOW_PAIR_KEYS : FT_PAIR_KEYS);
   if (!box_map(&qmap, a.q_lat, q_rows) || (!a.raw_idx && !pairs && !box_map(&box, a.ckv, extent))) return HK_ERR_UNSUPPORTED;
   if (a.out) {
@@ -888,9 +939,16 @@ int mla_flash_tc_launch(const MlaArgs& a, cudaStream_t s, bool clusters) {
   // A window's few splits of few rows: the output channels of each over two or four CTAs (one row under 3,000 / 4,096 / 8,192
   // keys 12.1 / 12.8 / 14.5 -> 9.9 / 10.6 / 11.6 us with the merge, four under 1,024 11.5 -> 9.4).
   const int64_t splits = (int64_t)a.n_split * a.m;
-  const int parts = a.out || a.window <= 0 || 2 * splits > sm_count() ? 1 : 4 * splits > sm_count() ? 2 : 4;
+  const int parts = a.out || (a.window <= 0 && !a.tree_kv) || 2 * splits > sm_count() ? 1 : 4 * splits > sm_count() ? 2 : 4;
   const int64_t items = splits * parts;
   const dim3 grid((unsigned)((a.raw_idx || a.window > 0) && a.out && items > sm_count() ? sm_count() : items));
+  if (a.tree_kv) {
+    alignas(64) CUtensorMap tree;
+    if (!rows_map(&tree, a.tree_kv, a.m)) return HK_ERR_UNSUPPORTED;
+    const auto kernel = parts == 1 ? mla_tree_tc_kernel<1> : parts == 2 ? mla_tree_tc_kernel<2> : mla_tree_tc_kernel<4>;
+    const cudaError_t e = pdl_launch(kernel, dim3((unsigned)items), dim3(FT_THREADS), FS_SMEM, s, a, device_status_ptr(), box, rows, qmap, omap, tree);
+    return e == cudaSuccess && cudaPeekAtLastError() == cudaSuccess ? HK_OK : HK_ERR_CUDA;
+  }
   const auto kernel = a.raw_idx        ? mla_flash_tc_kernel<true, false, false>
                       : !a.window    ? mla_flash_tc_kernel<false, false, false>
                       : parts == 1   ? mla_flash_tc_kernel<false, false, true>

@@ -45,11 +45,19 @@ __global__ __launch_bounds__(256) void mla_simt_kernel(MlaArgs a, MlaPaged pg) {
   const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5;
   const int h0 = hg * SIMT_HG;
   const bool sparse = a.raw_idx != nullptr;
-  const int seq = FMT == CACHE_F16 ? 0 : pg.seq_of(r);
+  // a node of a tree: its sequence's cached keys, then the nodes of the tree up to itself, of which those on its path are seen
+  MlaTree tree{0, 0, 0, 0, 0, -1};
+  if (a.tree_kv) tree = mla_tree(a, r);
+  const int seq = a.tree_kv ? tree.seq : FMT == CACHE_F16 ? 0 : pg.seq_of(r);
   int n;
   int64_t base = 0;
   KeyList list = {0, 0, 0};
-  if (sparse) n = seq < 0 ? 0 : a.kidx;
+  if (a.tree_kv) {
+    if (FMT != CACHE_F16) tree.len = (int)min((int64_t)tree.len, pg.room());
+    base = tree.base;
+    list = key_list(tree.len, 0, 0);
+    n = tree.len + tree.node + 1;
+  } else if (sparse) n = seq < 0 ? 0 : a.kidx;
   else {
     n = a.kv_len ? a.kv_len[r] : a.pos_start + r + 1;
     base = a.kv_base ? a.kv_base[r] : 0;
@@ -81,12 +89,15 @@ __global__ __launch_bounds__(256) void mla_simt_kernel(MlaArgs a, MlaPaged pg) {
   for (int i = k0 + wid; i < k1; i += 8) {
     int64_t tok = sparse ? (int64_t)a.raw_idx[(size_t)r * a.kidx + i] : base + list.at(i);
     float kf[16];
-    if (FMT == CACHE_F16) {
+    if (a.tree_kv && i >= tree.len) {
+      if (!(tree.path >> (i - tree.len) & 1)) continue;
+      simt_key<CACHE_F16>(a.tree_kv + (size_t)(tree.row0 + i - tree.len) * LATENT + lane * 16, 1.f, kf);
+    } else if (FMT == CACHE_F16) {
       if (tok < 0 || (a.ckv_rows > 0 && tok >= a.ckv_rows)) continue;  // warp-uniform
       simt_key<CACHE_F16>(a.ckv + (size_t)tok * LATENT + lane * 16, 1.f, kf);
     } else {
       const int64_t b = pg.block_of(seq, (int)tok);
-      if (b < 0 && (sparse || a.kv_len || pg.row_seq)) continue;   // (in a chunk: a key of zeros)
+      if (b < 0 && (sparse || a.kv_len || pg.row_seq || a.tree_kv)) continue;   // (in a chunk: a key of zeros)
       if (b < 0) {
 #pragma unroll
         for (int u = 0; u < 16; u++) kf[u] = 0.f;

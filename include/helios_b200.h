@@ -365,6 +365,36 @@ int hk_mla8_sparse(const void* q_lat, const void* ckv8, const float* scales, int
                    void* lat_out, int m, int n_heads, float scale, int n_split, void* workspace, size_t workspace_bytes,
                    void* stream);
 
+/* Pages of the 8-bit cache: refs [n_blocks] int32 counts the entries of block_table [n_seqs][table_stride] (required here, as every sequence's entries
+ * change) that name a block; 0 is a free block.  A pool begins with refs 0 and a table of -1, and from then on these calls keep both; an entry that names
+ * no block (negative, >= n_blocks) counts nowhere.  Blocks are handed out lowest number first, in the order of the call's sequences.  All arrays are
+ * device memory, nothing is read on the host.  A number outside [0, n_seqs) in a list of sequences is passed over; no list names a sequence
+ * twice.  Calls on one pool, and those that read or write its blocks, are ordered by the caller (a stream).
+ * workspace: hk_mla8_pages_workspace_bytes(n_blocks, n) bytes, 256-byte aligned (n 0 for a compaction).                                           */
+size_t hk_mla8_pages_workspace_bytes(int64_t n_blocks, int n);
+
+/* For each of n pairs sequence children[i] gives back what it holds and takes over the first lens[i] positions of parents[i]: whole blocks are shared
+ * (appending behind the positions that are shared begins a block of the sequence's own), a last block of fewer tokens is copied, with its scale, into a
+ * free one.  missing (optional): how many such blocks were not to be had; their entries name no block.  A child is no pair's parent.          */
+int hk_mla8_pages_fork(void* ckv8, float* scales, int dtype, int64_t n_blocks, int block, int* refs, int* block_table, int table_stride,
+                       int n_seqs, const int* parents, const int* children, const int* lens, int n, int* missing, void* workspace,
+                       size_t workspace_bytes, void* stream);
+/* Sequence seqs[i] gets a free block for every entry of its first lens[i] positions that names none (positions behind the table: none).  What the
+ * block held is still there: hk_mla8_append begins it anew.  missing as above.                                                              */
+int hk_mla8_pages_reserve(void* ckv8, float* scales, int dtype, int64_t n_blocks, int block, int* refs, int* block_table, int table_stride,
+                          int n_seqs, const int* seqs, const int* lens, int n, int* missing, void* workspace, size_t workspace_bytes, void* stream);
+/* Sequence seqs[i] gives back the blocks behind its first keep[i] positions (keep NULL: all).                                              */
+int hk_mla8_pages_free(void* ckv8, float* scales, int dtype, int64_t n_blocks, int block, int* refs, int* block_table, int table_stride,
+                       int n_seqs, const int* seqs, const int* keep, int n, void* stream);
+/* The live blocks (refs not 0) become blocks 0 .. n_live - 1: those beyond move, with their scales, into the free ones below, in ascending order, and
+ * the table and refs go with them.  n_live (optional): their number.                                                                        */
+int hk_mla8_pages_compact(void* ckv8, float* scales, int dtype, int64_t n_blocks, int block, int* refs, int* block_table, int table_stride,
+                          int n_seqs, int* n_live, void* workspace, size_t workspace_bytes, void* stream);
+/* Blocks src[i] of one pool (tokens and scale) to blocks dst[i] of another, or of the same where no block is both; numbers that name no block are
+ * passed over.  refs and tables are the caller's.                                                                                           */
+int hk_mla8_pages_copy(const void* from_ckv8, const float* from_scales, int64_t from_blocks, void* to_ckv8, float* to_scales, int64_t to_blocks,
+                       int dtype, int block, const int* src, const int* dst, int n, void* stream);
+
 /* hk_mla_sparse and hk_mla_dense, but writing un-normalised split partials only (no combine): the building block of
  * split-KV across GPUs.  part_* point at storage for ONE split: m[rows], l[rows], acc[rows][512]. */
 int hk_mla_dense_partial(const void* q_lat, const void* ckv, const int64_t* kv_base,
@@ -530,6 +560,70 @@ int hk_mla_decode_prologue(const float* kv_pre, const void* ln_w_f16, void* ckv,
                            const void* knorm_w, const void* knorm_b, void* idx_kn, float eps_ln, const void* idx_g,
                            void* raw_ring, int raw_rows, void* pool_k_nt, const float* ape, int pos, int* q_pos_out,
                            void* stream);
+
+/* ---------------------------------------------------------------------------------------------
+ * (e) trees of drafted tokens (speculative decoding)
+ *
+ *   A call works on the trees of n_seqs sequences, m rows (nodes) in all: sequence s has rows tree_start[s] .. tree_start[s+1] - 1 (tree_start
+ *   [n_seqs + 1] on the device; NULL: m / n_seqs rows each, at most 64), of which the first 64 are its tree; rows behind them, and rows of no
+ *   sequence, belong to no tree.  parent [m] on the device: the number, within the tree, of the node that a row hangs on; a node comes after its
+ *   parent, and a number that is no earlier node of the tree (-1) hangs the row on the sequence's last token.  A chain is parent[j] = j - 1.
+ *   leaf [n_seqs] on the device: the accepted node of each tree (a number that is no node of it: none is accepted); the nodes from the root to it
+ *   become the sequence's next tokens.  No counterpart in the reference, which decodes token by token.
+ *
+ *   A step: hk_kda_tree_conv, hk_kda_tree and hk_gated_rms_norm in a KDA layer, hk_mla_tree or hk_mla8_tree in an MLA layer, none of which changes a
+ *   state or a cache; once the nodes are accepted, hk_kda_tree_accept for each KDA layer and hk_mla_tree_accept or hk_mla8_tree_accept for each MLA
+ *   layer, which do what decoding the accepted tokens one by one would have done.
+ * ------------------------------------------------------------------------------------------- */
+
+/* Attention of nodes over the fp16 cache: a row attends to the first kv_len[s] cached rows of its sequence (kv_len [n_seqs]; NULL: pos_start for
+ * all; they begin at kv_base[s], NULL: 0) and to its path's rows of tree_kv [m][512] f16 (its ancestors' and its own latents; 16-byte aligned).  Other
+ * nodes' rows have no effect, whatever they hold.  A row of no tree gives zeros.  With kv_len, pos_start says about how many keys the longest
+ * sequence has (0: 4,096; it chooses the splits, no more).  Other arguments as in hk_mla_dense.  Heads other than 64 (multiples of 4) run on the CUDA
+ * cores, up to 65,535 rows a call.  A key that is not finite and that a row sees shows as in hk_mla_window.
+ * Workspace: hk_mla_tree_workspace_bytes(m, n_heads, pos_start), or hk_mla_partial_bytes(n_split, m * n_heads) for n_split > 1.               */
+size_t hk_mla_tree_workspace_bytes(int m, int n_heads, int n_keys);
+int hk_mla_tree(const void* q_lat, const void* ckv, int64_t ckv_rows, const int64_t* kv_base, const int* kv_len, int pos_start,
+                const void* tree_kv, const int* parent, const int* tree_start, int n_seqs, void* lat_out, int m, int n_heads, float scale,
+                int n_split, void* workspace, size_t workspace_bytes, void* stream);
+
+/* The same over the 8-bit paged cache (block_table NULL: one sequence), positions without a block hold no key; tree_kv is fp16 here too: drafts that
+ * are not accepted never touch the cache.  n_heads: a multiple of 4.  Precision as in hk_mla8_dense.                                     */
+size_t hk_mla8_tree_workspace_bytes(int m, int n_heads, int n_keys);
+int hk_mla8_tree(const void* q_lat, const void* ckv8, const float* scales, int dtype, int64_t n_blocks, int block, const int* block_table,
+                 int table_stride, const int* kv_len, int pos_start, const void* tree_kv, const int* parent, const int* tree_start,
+                 int n_seqs, void* lat_out, int m, int n_heads, float scale, int n_split, void* workspace, size_t workspace_bytes,
+                 void* stream);
+
+/* The accepted path's rows of tree_kv become the cached rows kv_len[s] .. of their sequences (kv_len NULL: pos_start; kv_base as in hk_mla_tree; rows
+ * at or beyond ckv_rows, where it is told, are dropped).  len_out (optional) [n_seqs]: kv_len[s] and the number of accepted nodes; not kv_len itself.  */
+int hk_mla_tree_accept(const void* tree_kv, void* ckv, int64_t ckv_rows, const int64_t* kv_base, const int* kv_len, int pos_start,
+                       const int* parent, const int* tree_start, int n_seqs, const int* leaf, int m, int* len_out, void* stream);
+/* The same into the 8-bit cache, as hk_mla8_append appends rows (scales, blocks and rows without one as there; the rows are normalised already).   */
+int hk_mla8_tree_accept(const void* tree_kv, void* ckv8, float* scales, int dtype, int64_t n_blocks, int block, const int* block_table,
+                        int table_stride, const int* kv_len, int pos_start, const int* parent, const int* tree_start, int n_seqs, const int* leaf,
+                        int m, int* len_out, void* stream);
+
+/* hk_kda_cast_conv of nodes: the window of a node is its ancestors' rows of x32 [m][dim] and, behind the root, its sequence's conv_state
+ * [slots][dim][4] bf16 (slots [n_seqs] or NULL), which stays as it is.  mixed_qkv [m][dim] bf16; rows of no tree are left as they were.  x32 16-byte,
+ * the others 8-byte aligned, dim % 4 == 0.  A chain gives hk_kda_cast_conv's bits.                                                        */
+int hk_kda_tree_conv(const float* x32, const void* conv_state, const int* slots, const void* conv_weight, const void* conv_bias,
+                     const int* parent, const int* tree_start, int n_seqs, void* mixed_qkv, int m, int dim, int activation, void* stream);
+
+/* The KDA recurrence of nodes, head dim 128, Hk == Hv: out [m][H][128] bf16 (rz; out_f32 optional) is what hk_kda_recurrent (channelwise) gives for
+ * the node as the last token behind its path, with the state rec_state [slots][H][128][128] of its sequence, which stays as it is.  No node's
+ * state is formed: sums in another order than there.  mixed_qkv [m][3*H*128] bf16 (8-byte aligned), g [m][H][128] log decay f32 (<= 0; 16-byte aligned)
+ * and beta [m][H] bf16 as there; or, with a_log [H] and dt_bias [H][128], the raw gate f32 and the raw beta logit f32 as in
+ * hk_kda_chunked_prefill_gated.  max_nodes: nodes that the longest tree has (0: 64); nodes beyond, and rows of no tree, are left as they were.      */
+int hk_kda_tree(const void* mixed_qkv, const float* g, const void* beta, const float* dt_bias, const float* a_log, float lower_bound,
+                const float* rec_state, const int* slots, const int* parent, const int* tree_start, int n_seqs, void* out, float* out_f32,
+                int m, int num_heads, int max_nodes, void* stream);
+
+/* The states of the sequences step along the accepted paths: rec_state as hk_kda_recurrent (channelwise) leaves it behind the path's tokens, bit for
+ * bit, and the windows conv_state as hk_kda_cast_conv leaves them behind the path's rows of x32 (both NULL: no windows).  Other arguments as in hk_kda_tree.  */
+int hk_kda_tree_accept(const float* x32, void* conv_state, const void* mixed_qkv, const float* g, const void* beta, const float* dt_bias,
+                       const float* a_log, float lower_bound, float* rec_state, const int* slots, const int* parent, const int* tree_start,
+                       int n_seqs, const int* leaf, int m, int num_heads, void* stream);
 
 /* ---------------------------------------------------------------------------------------------
  * diagnostics

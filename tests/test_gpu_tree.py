@@ -1,0 +1,538 @@
+"""Trees of drafted tokens: attention over both latent caches, the KDA convolution and recurrence, and the steps to an accepted node, against
+64 bits and against the calls that decode token by token."""
+import math
+
+import pytest
+import torch
+
+import helios_glm53flash_b200 as hk
+import latent8_ref as ref8
+from latent8_ref import attend, cache, rows_of, table_for
+from tree_ref import TREES, ints, kda_token, layout, path, tree_of
+
+pytestmark = pytest.mark.gpu
+
+NAN, INF = math.nan, math.inf
+
+
+def gen_of(seed):
+    return torch.Generator(device="cuda").manual_seed(seed)
+
+
+def randn(gen, *shape):
+    return torch.randn(*shape, device="cuda", generator=gen)
+
+
+def finish():
+    torch.cuda.synchronize()
+    assert hk.read_device_status() == 0
+
+
+def check_rows(out, want):
+    for r, (o, tol) in enumerate(want):
+        off = (out[r].double() - o).abs()
+        assert bool((off <= tol).all()), "row %d: off %.3e of %.3e" % (r, float((off - tol).max()), float(tol.max()))
+
+
+# ---------------------------------------------------------------------------------------------
+# attention
+# ---------------------------------------------------------------------------------------------
+def wanted(q, past, tree_kv, first, tree, scale):
+    """(output, bound) of a tree's rows; past: the sequence's keys in 64 bits"""
+    return [attend(q[first + j].double(), torch.cat((past, tree_kv[[first + i for i in path(tree, j)]].double())), scale) for j in range(len(tree))]
+
+
+@pytest.mark.parametrize("trees,lens", [
+    (["one"], [0]), (["one"], [1]), (["chain5"], [63]), (["binary15"], [64]), (["wide63"], [65]), (["chain64"], [200]),
+    (["star7", "two_roots", "one"], [0, 129, 1000]), ([(31, 1), (8, 2), (64, 3), (1, 4)], [500, 64, 3, 128]), ([(64, 5)], [2500]), ([(5, 6)] * 9, [777] * 9),
+    ([(16, 7)], [4100]), (["chain5", [], "chain5"], [40, 50, 60]),
+])
+@pytest.mark.parametrize("heads,n_split", [(64, 0), (64, 1), (64, 3), (16, 0), (4, 2)])
+def test_nodes_over_the_fp16_cache(trees, lens, heads, n_split):
+    trees = [tree_of(t) for t in trees]
+    gen = gen_of(len(trees) + sum(lens))
+    starts, parent, tree_start = layout(trees)
+    m, n = starts[-1], len(trees)
+    gap = 3                                                   # rows between the sequences, of which nobody may see any
+    base = [sum(lens[:i]) + gap * (i + 1) for i in range(n)]
+    ckv = torch.full((sum(lens) + gap * (n + 1), 512), NAN, dtype=torch.float16, device="cuda")
+    for b, k in zip(base, lens):
+        ckv[b:b + k] = randn(gen, k, 512).half()
+    q, tree_kv = (randn(gen, m, heads, 512) * 0.7).half(), randn(gen, m, 512).half()
+    out = torch.full((m, heads, 512), 7.0, dtype=torch.float16, device="cuda")
+    hk.mla_tree_decode(q, ckv, tree_kv, parent, out, m, n_seqs=n, tree_start=tree_start, kv_base=torch.tensor(base, device="cuda"), kv_len=ints(lens),
+                       n_heads=heads, n_split=n_split, n_keys_hint=max(lens))
+    finish()
+    check_rows(out, [w for s in range(n) for w in wanted(q, ckv[base[s]:base[s] + lens[s]].double(), tree_kv, starts[s], trees[s], 0.0625)])
+
+
+@pytest.mark.parametrize("kind", ["i8", "e4m3"])
+@pytest.mark.parametrize("block", [16, 64, 128])
+@pytest.mark.parametrize("trees,lens,heads,n_split", [
+    (["one"], [0], 64, 0), (["binary15"], [64], 64, 0), (["wide63", "chain5"], [65, 1000], 64, 0), ([(31, 1), (64, 2), (1, 3)], [500, 3, 128], 16, 0),
+    ([(12, 5)], [3000], 64, 0), (["star7"], [700], 20, 3), (["chain64"], [200], 128, 1), ([(5, 6)] * 9, [777] * 9, 64, 2),
+])
+def test_nodes_over_the_8_bit_cache(kind, block, trees, lens, heads, n_split):
+    trees = [tree_of(t) for t in trees]
+    gen = gen_of(block + sum(lens) + heads)
+    starts, parent, tree_start = layout(trees)
+    m, n = starts[-1], len(trees)
+    blocks = max(1, max((k + block - 1) // block for k in lens))
+    ckv8, scales = cache(gen, kind, n * blocks + 2, block, spread=0.5)
+    table = table_for(gen, n, blocks, n * blocks + 2)
+    q, tree_kv = (randn(gen, m, heads, 512) * 0.7).half(), randn(gen, m, 512).half()
+    out = torch.full((m, heads, 512), 7.0, dtype=torch.float16, device="cuda")
+    hk.mla8_tree_decode(q, ckv8, scales, tree_kv, parent, out, m, n_seqs=n, tree_start=tree_start, block_table=table, kv_len=ints(lens), n_heads=heads,
+                        n_split=n_split, n_keys_hint=max(lens))
+    finish()
+    want = []
+    for s in range(n):
+        past = rows_of(ckv8, scales, table[s], torch.arange(lens[s], device="cuda"))
+        want += [attend(q[starts[s] + j].double(), torch.cat((past, tree_kv[[starts[s] + i for i in path(trees[s], j)]].double())), 0.0625) for j in
+                 range(len(trees[s]))]
+    check_rows(out, want)
+
+
+@pytest.mark.parametrize("over", ["f16", "i8", "f16 of 4 heads"])
+def test_what_a_node_does_not_see_has_no_effect(over):
+    """NaN and infinities in other branches, in rows of no tree and behind a sequence's keys; a key that is not finite shows in the rows that see it"""
+    heads = 4 if "4" in over else 64
+    tree = tree_of("binary15")
+    gen = gen_of(3)
+    starts, parent, tree_start = layout([tree, tree], front=2)
+    m = starts[-1] + 3                                        # rows behind the last tree
+    parent = torch.cat((parent, ints([0, 1, 2])))
+    n = 70
+    q, clean = (randn(gen, m, heads, 512) * 0.7).half(), randn(gen, m, 512).half()
+    ckv = torch.full((4 * n, 512), INF, dtype=torch.float16, device="cuda")
+    base = [1, 2 * n]
+    for b in base:
+        ckv[b:b + n] = randn(gen, n, 512).half()
+    ckv8, scales = cache(gen, "i8", 12, 16)
+    scales[5] = NAN                                          # in nobody's table
+    table = ints([[0, 1, 2, 3, 4, 5], [6, 7, 8, 9, 10, 5]])
+
+    def call(rows):
+        out = torch.full((m, heads, 512), 7.0, dtype=torch.float16, device="cuda")
+        tree_args = dict(n_seqs=2, tree_start=tree_start, kv_len=ints([n, n]), n_heads=heads, n_keys_hint=n)
+        if over == "i8":
+            hk.mla8_tree_decode(q, ckv8, scales, rows, parent, out, m, block_table=table, **tree_args)
+        else:
+            hk.mla_tree_decode(q, ckv, rows, parent, out, m, kv_base=torch.tensor(base, device="cuda"), **tree_args)
+        finish()
+        return out
+
+    good = call(clean)
+    assert bool(torch.isfinite(good).all())
+    assert not bool(good[:2].any()) and not bool(good[starts[-1]:].any()), "rows of no tree"
+    bad = clean.clone()
+    bad[:2], bad[starts[-1]:] = NAN, -INF
+    for node, value in ((4, NAN), (6, INF), (14, -INF)):
+        bad[starts[0] + node] = value
+    out = call(bad)
+    for s in range(2):
+        for j in range(len(tree)):
+            r = starts[s] + j
+            if s == 0 and {4, 6, 14} & set(path(tree, j)):
+                assert bool(torch.isnan(out[r]).any()), (s, j)
+            else:
+                assert torch.equal(out[r], good[r]), (s, j)
+
+
+def test_parents_that_are_no_earlier_node_hang_on_the_sequence():
+    gen = gen_of(4)
+    m, n = 6, 90
+    q, tree_kv, ckv = (randn(gen, m, 64, 512) * 0.7).half(), randn(gen, m, 512).half(), randn(gen, n, 512).half()
+    outs = []
+    for tree in ([0, 5, -7, 2, 1 << 30, 4], [-1, -1, -1, 2, -1, 4]):
+        out = torch.empty(m, 64, 512, dtype=torch.float16, device="cuda")
+        hk.mla_tree_decode(q, ckv, tree_kv, ints(tree), out, m, n)
+        outs.append(out)
+    finish()
+    assert torch.equal(*outs)
+    check_rows(outs[0], wanted(q, ckv.double(), tree_kv, 0, [-1, -1, -1, 2, -1, 4], 0.0625))
+
+
+def test_a_sequence_of_more_rows_than_a_tree_has():
+    """rows from the 65th on belong to no tree; lengths are cut at the cache's end"""
+    gen = gen_of(5)
+    m, n = 70, 50
+    tree = list(range(-1, m - 1))
+    q, tree_kv, ckv = (randn(gen, m, 64, 512) * 0.7).half(), randn(gen, m, 512).half(), randn(gen, n, 512).half()
+    out = torch.full((m, 64, 512), 7.0, dtype=torch.float16, device="cuda")
+    hk.mla_tree_decode(q, ckv, tree_kv, ints(tree), out, m, tree_start=ints([0, m]), kv_len=ints([1 << 30]), n_keys_hint=n)
+    finish()
+    check_rows(out[:64], wanted(q, ckv.double(), tree_kv, 0, tree[:64], 0.0625))
+    assert not bool(out[64:].any())
+
+
+@pytest.mark.parametrize("m,n", [(1, 5001), (12, 9000), (64, 3000)])
+def test_a_chain_agrees_with_a_causal_chunk(m, n):
+    """the nodes of a chain are the rows of a chunk whose keys lie in the cache"""
+    gen = gen_of(6)
+    ckv = randn(gen, n + m, 512).half()
+    q = (randn(gen, m, 64, 512) * 0.7).half()
+    out, chunk = (torch.empty(m, 64, 512, dtype=torch.float16, device="cuda") for _ in range(2))
+    hk.mla_tree_decode(q, ckv, ckv[n:].contiguous(), ints(list(range(-1, m - 1))), out, m, n)
+    hk.mla_dense_prefill(q, ckv, chunk, m, n)
+    finish()
+    want = wanted(q, ckv[:n].double(), ckv[n:], 0, list(range(-1, m - 1)), 0.0625)
+    check_rows(out, want)
+    check_rows(chunk, want)
+
+
+@pytest.mark.parametrize("kind", ["f16", "i8"])
+def test_the_accepted_rows_go_behind_the_cached_ones(kind, monkeypatch):
+    trees = [tree_of(t) for t in ("binary15", "chain64", "one", "star7", (20, 3))]
+    leaves = [13, 63, 0, -1, 99]
+    lens = [30, 61, 5, 40, 7]
+    gen = gen_of(7)
+    starts, parent, tree_start = layout(trees)
+    m, n = starts[-1], len(trees)
+    rows = randn(gen, m, 512).half()
+    len_out = torch.zeros(n, dtype=torch.int32, device="cuda")
+    paths = [path(t, j) if 0 <= j < len(t) else [] for t, j in zip(trees, leaves)]
+    picked = [starts[s] + j for s in range(n) for j in paths[s]]
+    if kind == "f16":
+        room = 130
+        ckv = randn(gen, n * room, 512).half()
+        want = ckv.clone()
+        for s in range(n):
+            want[s * room + lens[s]:s * room + lens[s] + len(paths[s])] = rows[[starts[s] + j for j in paths[s]]]
+        hk.mla_tree_accept(rows, ckv, parent, ints(leaves), m, n_seqs=n, tree_start=tree_start, kv_base=torch.arange(n, device="cuda") * room, kv_len=ints(lens),
+                           len_out=len_out)
+        finish()
+        assert torch.equal(ckv, want)
+    else:
+        for block in (16, 32, 64, 128):
+            blocks = (130 + block - 1) // block
+            ckv8, scales = cache(gen, "i8", n * blocks + 1, block)
+            scales *= 0.5 + torch.rand(n * blocks + 1, device="cuda", generator=gen)
+            table = table_for(gen, n, blocks, n * blocks + 1)
+            before, before_scales = ckv8.clone(), scales.clone()
+            hk.mla8_tree_accept(rows, ckv8, scales, parent, ints(leaves), m, n_seqs=n, tree_start=tree_start, block_table=table, kv_len=ints(lens), len_out=len_out)
+            finish()
+            monkeypatch.setattr(ref8, "normed", lambda x, w, eps: x.double())
+            at = [0]
+            for p in paths:
+                at.append(at[-1] + len(p))
+            ref8.check_append(before, before_scales, ckv8, scales, rows[picked], None, table.cpu(), lens, at, "i8")
+    assert len_out.tolist() == [k + len(p) for k, p in zip(lens, paths)]
+
+
+def test_accepted_rows_beyond_the_cache_are_dropped():
+    gen = gen_of(8)
+    rows, ckv = randn(gen, 5, 512).half(), randn(gen, 12, 512).half()
+    want = ckv.clone()
+    want[7:10] = rows[:3]
+    hk.mla_tree_accept(rows, ckv, ints(TREES["chain5"]), ints([4]), 5, 7, ckv_rows=10)
+    finish()
+    assert torch.equal(ckv, want)
+
+
+# ---------------------------------------------------------------------------------------------
+# KDA
+# ---------------------------------------------------------------------------------------------
+def kda_inputs(gen, m, heads, n_states, g_low=-5.0):
+    return dict(qkv=randn(gen, m, 3 * heads * 128).bfloat16(), g=(g_low * torch.sigmoid(2 * randn(gen, m, heads, 128))).contiguous(),
+                beta=torch.sigmoid(randn(gen, m, heads)).bfloat16(), state=0.3 * randn(gen, n_states, heads, 128, 128))
+
+
+def kda_wanted(x, heads, starts, trees, slots):
+    """outputs in 64 bits, and what they may be off by: sums of 128 products, then the chain of a node's path in fp32 - 200 roundings a token of
+    relative 2^-24 of the magnitudes, 8 ulp for exponentials of arguments down to -5 and the norms - of states, values and their sums that are at most M"""
+    out = torch.zeros(x["qkv"].shape[0], heads, 128, dtype=torch.float64, device="cuda")
+    tol = torch.zeros_like(out)
+    for s, tree in enumerate(trees):
+        made = {-1: x["state"][slots[s]].double()}
+        for j in range(len(tree)):
+            r = starts[s] + j
+            q, k, v = x["qkv"][r].double().view(3, heads, 128)
+            steps = path(tree, j)
+            made[j], out[r] = kda_token(made[steps[-2] if len(steps) > 1 else -1], q, k, v, x["g"][r].double(), x["beta"][r].double())
+            big = 128 ** 0.5 * x["state"][slots[s]].abs().max().double() + sum(x["qkv"][starts[s] + i].double().abs().max() for i in steps)
+            tol[r] = (200 * 2.0 ** -24 + 64 * 2.0 ** -24) * len(steps) * big
+    return out, tol
+
+
+@pytest.mark.parametrize("trees", [["one"], ["chain5"], ["chain64"], ["wide63", "binary15"], ["star7", "one", "two_roots", (33, 1)], [(16, 2)] * 5, ["one", [], "chain5"]])
+@pytest.mark.parametrize("heads", [1, 6, 40])
+def test_recurrence_of_nodes(trees, heads):
+    trees = [tree_of(t) for t in trees]
+    gen = gen_of(heads + len(trees))
+    starts, parent, tree_start = layout(trees, front=1)
+    m = starts[-1] + 2
+    parent = torch.cat((parent, ints([0, 0])))
+    n = len(trees)
+    slots = [(3 * s + 1) % (n + 2) if n < 3 else n + 1 - s for s in range(n)]
+    x = kda_inputs(gen, m, heads, n + 2)
+    held = x["state"].clone()
+    out = torch.full((m, heads, 128), 7.0, dtype=torch.bfloat16, device="cuda")
+    f32 = torch.full((m, heads, 128), 7.0, device="cuda")
+    hk.kda_tree_decode(x["qkv"], x["g"], x["beta"], x["state"], parent, out, m, heads, n_seqs=n, tree_start=tree_start, slots=ints(slots), out_f32=f32)
+    finish()
+    assert torch.equal(x["state"], held), "states stay as they are"
+    want, tol = kda_wanted(x, heads, starts, trees, slots)
+    mine = slice(1, starts[-1])
+    off = (f32.double() - want).abs()
+    assert bool((off <= tol)[mine].all()), float(off[mine].max())
+    toward_zero = (f32.view(torch.int32) & -65536).view(torch.float32)
+    assert torch.equal(out[mine].float(), toward_zero[mine])
+    for r in [0] + list(range(starts[-1], m)):
+        assert bool((f32[r] == 7).all()) and bool((out[r] == 7).all()), "rows of no tree are left as they were"
+
+
+def test_hard_resets_and_gates_of_zero():
+    """log decays of 0, -100 and minus infinity on a long chain: nothing overflows, what is forgotten is nothing"""
+    gen, heads, tree = gen_of(11), 2, TREES["chain64"]
+    x = kda_inputs(gen, 64, heads, 1)
+    x["g"][::3], x["g"][1::7], x["g"][2::9] = 0.0, -100.0, -INF
+    f32 = torch.empty(64, heads, 128, device="cuda")
+    hk.kda_tree_decode(x["qkv"], x["g"], x["beta"], x["state"], ints(tree), torch.empty(64, heads, 128, dtype=torch.bfloat16, device="cuda"), 64, heads, out_f32=f32)
+    finish()
+    want, tol = kda_wanted(x, heads, [0], [tree], [0])
+    assert bool(((f32.double() - want).abs() <= tol).all())
+
+
+def test_what_is_not_on_a_nodes_path_has_no_effect_on_it():
+    gen, heads, tree = gen_of(12), 3, tree_of("binary15")
+    x = kda_inputs(gen, 15, heads, 1)
+
+    def call():
+        f32 = torch.empty(15, heads, 128, device="cuda")
+        hk.kda_tree_decode(x["qkv"], x["g"], x["beta"], x["state"], ints(tree), torch.empty(15, heads, 128, dtype=torch.bfloat16, device="cuda"), 15, heads,
+                           out_f32=f32)
+        finish()
+        return f32
+
+    good = call()
+    x["qkv"][4], x["g"][6], x["beta"][9] = NAN, INF, INF
+    out = call()
+    for j in range(15):
+        if not {4, 6, 9} & set(path(tree, j)):
+            assert torch.equal(out[j], good[j]), j
+
+
+def test_raw_gates_give_what_prepared_gates_give():
+    gen, heads = gen_of(13), 5
+    trees = [tree_of((20, 1)), tree_of("chain5")]
+    starts, parent, tree_start = layout(trees)
+    m = starts[-1]
+    x = kda_inputs(gen, m, heads, 2)
+    f, b, dt, a_log = randn(gen, m, heads, 128), randn(gen, m, heads), 0.5 * randn(gen, heads, 128), randn(gen, heads)
+    g, beta = torch.empty(m, heads, 128, device="cuda"), torch.empty(m, heads, dtype=torch.bfloat16, device="cuda")
+    hk.kda_gate(b, f, dt, a_log, -5.0, beta, g, m, heads, 128)
+    outs, states = [], []
+    for args, more in (((g, beta), {}), ((f, b), dict(dt_bias=dt, a_log=a_log, lower_bound=-5.0))):
+        out, st = torch.empty(m, heads, 128, device="cuda"), x["state"].clone()
+        hk.kda_tree_decode(x["qkv"], *args, st, parent, torch.empty(m, heads, 128, dtype=torch.bfloat16, device="cuda"), m, heads, n_seqs=2, tree_start=tree_start,
+                           out_f32=out, **more)
+        hk.kda_tree_accept(None, None, x["qkv"], *args, st, parent, ints([19, 3]), m, heads, n_seqs=2, tree_start=tree_start, **more)
+        outs.append(out)
+        states.append(st)
+    finish()
+    assert torch.equal(*outs) and torch.equal(*states)
+
+
+@pytest.mark.parametrize("heads,n", [(2, 1), (16, 5), (40, 3)])
+def test_accepted_states_are_those_of_token_by_token_decoding(heads, n):
+    """bit for bit: the states of the recurrence over the path's tokens, the windows of the convolution over them"""
+    trees = [tree_of(t) for t in ("binary15", "chain64", (17, 4), "one", "star7")[:n]]
+    leaves = [14, 63, 16, -1, 7][:n]                          # the last two: none
+    gen, dim = gen_of(heads), 3 * heads * 128
+    starts, parent, tree_start = layout(trees)
+    m = starts[-1]
+    slots = [n - s for s in range(n)]
+    x = kda_inputs(gen, m, heads, n + 1)
+    x32, window = randn(gen, m, dim), randn(gen, n + 1, dim, 4).bfloat16()
+    state, win = x["state"].clone(), window.clone()
+    hk.kda_tree_accept(x32, win, x["qkv"], x["g"], x["beta"], state, parent, ints(leaves), m, heads, n_seqs=n, tree_start=tree_start, slots=ints(slots))
+    finish()
+    for s in range(n):
+        steps = path(trees[s], leaves[s]) if 0 <= leaves[s] < len(trees[s]) else []
+        rows, k = [starts[s] + j for j in steps], len(steps)
+        if k:
+            one = x["state"][slots[s]:slots[s] + 1].clone()
+            out = torch.empty(1, k, heads, 128, dtype=torch.bfloat16, device="cuda")
+            hk.cuda_recurrent_gated_delta_rule(x["qkv"][rows].contiguous(), x["g"][rows].contiguous(), x["beta"][rows].contiguous(), one, out, 1, k, heads, heads, 128, 128, 1,
+                                               None, True, False, force_recurrent=True)
+            w = window[slots[s]:slots[s] + 1].clone()
+            hk.kda_cast_conv(x32[rows].contiguous(), w, None, torch.zeros(dim, 4, dtype=torch.bfloat16, device="cuda"), None, torch.empty(1, k, dim, dtype=torch.bfloat16, device="cuda"),
+                             1, dim, k, True)
+            finish()
+            assert torch.equal(state[slots[s]], one[0]) and torch.equal(win[slots[s]], w[0]), s
+            exact = x["state"][slots[s]].double()
+            for r in rows:
+                q, kk, v = x["qkv"][r].double().view(3, heads, 128)
+                exact, _ = kda_token(exact, q, kk, v, x["g"][r].double(), x["beta"][r].double())
+            assert float((state[slots[s]].double() - exact).norm() / exact.norm()) < 1e-5
+        else:
+            assert torch.equal(state[slots[s]], x["state"][slots[s]]) and torch.equal(win[slots[s]], window[slots[s]]), s
+    assert torch.equal(state[0], x["state"][0]) and torch.equal(win[0], window[0]), "a slot of nobody"
+
+
+@pytest.mark.parametrize("dim", [4, 384, 2060])
+@pytest.mark.parametrize("bias,activation", [(True, True), (False, False)])
+def test_convolution_of_nodes(dim, bias, activation):
+    """bit for bit what the convolution of a node's path gives for its last token; the windows stay as they are"""
+    trees = [tree_of(t) for t in ("binary15", "chain5", "two_roots")]
+    gen = gen_of(dim)
+    starts, parent, tree_start = layout(trees, front=1)
+    m, slots = starts[-1], [2, 0, 3]
+    x, window, w = randn(gen, m, dim), randn(gen, 4, dim, 4).bfloat16(), (0.3 * randn(gen, dim, 4)).bfloat16()
+    b = randn(gen, dim).bfloat16() if bias else None
+    held = window.clone()
+    out = torch.full((m, dim), 7.0, dtype=torch.bfloat16, device="cuda")
+    hk.kda_tree_conv(x, window, w, b, parent, out, m, dim, n_seqs=3, tree_start=tree_start, slots=ints(slots), activation=activation)
+    finish()
+    assert torch.equal(window, held) and bool((out[0] == 7).all())
+    for s, tree in enumerate(trees):
+        for j in range(len(tree)):
+            rows = [starts[s] + i for i in path(tree, j)]
+            one = torch.empty(1, len(rows), dim, dtype=torch.bfloat16, device="cuda")
+            hk.kda_cast_conv(x[rows].contiguous(), window[slots[s]:slots[s] + 1].clone(), None, w, b, one, 1, dim, len(rows), activation)
+            assert torch.equal(out[starts[s] + j], one[0, -1]), (s, j)
+            # and by the formula: three additions in fp32, the exponential, the rounding to bf16
+            back = torch.cat((window[slots[s]].double(), x[rows].bfloat16().double().T), 1)[:, -4:]
+            y = (back * w.double()).sum(1) + (b.double() if bias else 0)
+            mag = (back * w.double()).abs().sum(1) + (b.double().abs() if bias else 0)
+            y = y * torch.sigmoid(y) if activation else y
+            assert bool(((out[starts[s] + j].double() - y).abs() <= 2.0 ** -8 * y.abs() + 2.0 ** -19 * mag + 2.0 ** -30).all())
+
+
+# ---------------------------------------------------------------------------------------------
+# as they are used
+# ---------------------------------------------------------------------------------------------
+def test_a_drafted_step_and_the_tokens_decoded_one_by_one():
+    """verify a tree in a KDA and an MLA layer, accept a node, go on: the same states, windows and cache as decoding the accepted tokens alone"""
+    gen, heads, n = gen_of(20), 4, 137
+    tree = tree_of((24, 9))
+    leaf = max(range(24), key=lambda j: len(path(tree, j)))
+    m, dim, steps = len(tree), 3 * heads * 128, path(tree, leaf)
+    x32, f, b = randn(gen, m, dim), randn(gen, m, heads, 128), randn(gen, m, heads)
+    dt, a_log, w = 0.5 * randn(gen, heads, 128), randn(gen, heads), (0.3 * randn(gen, dim, 4)).bfloat16()
+    state, window = 0.3 * randn(gen, 1, heads, 128, 128), randn(gen, 1, dim, 4).bfloat16()
+    ckv = torch.zeros(n + 64, 512, dtype=torch.float16, device="cuda")
+    ckv[:n] = randn(gen, n, 512).half()
+    kv_pre, ln_w = randn(gen, m, 512), (1 + 0.1 * randn(gen, 512)).half()
+    q = (randn(gen, m, 64, 512) * 0.7).half()
+    parent = ints(tree)
+    # one by one: what decoding does with the accepted tokens
+    st1, w1, c1, outs1, lat1 = state.clone(), window.clone(), ckv.clone(), [], []
+    norm_w, gate = torch.ones(128, dtype=torch.bfloat16, device="cuda"), randn(gen, heads, 128)
+    for i, j in enumerate(steps):
+        out = torch.empty(1, heads, 128, dtype=torch.bfloat16, device="cuda")
+        hk.kda_decode_layer(x32[j].contiguous(), w1, w, None, f[j].contiguous(), b[j].contiguous(), dt, a_log, -5.0, st1, out, norm_w, gate, torch.empty(heads, 128, dtype=torch.float16, device="cuda"), 1, heads)
+        hk.mla_cache_append(kv_pre[j:j + 1].contiguous(), ln_w, c1, n + i, 1, 1e-6)
+        lat = torch.empty(1, 64, 512, dtype=torch.float16, device="cuda")
+        hk.mla_dense_prefill(q[j:j + 1].contiguous(), c1, lat, 1, n + i)
+        outs1.append(out)
+        lat1.append(lat)
+    # the tree
+    qkv, out, lat = (torch.empty(m, dim, dtype=torch.bfloat16, device="cuda"), torch.empty(m, heads, 128, dtype=torch.bfloat16, device="cuda"),
+                     torch.empty(m, 64, 512, dtype=torch.float16, device="cuda"))
+    raw = dict(dt_bias=dt, a_log=a_log, lower_bound=-5.0)
+    rows = torch.empty(m, 512, dtype=torch.float16, device="cuda")
+    hk.kda_tree_conv(x32, window, w, None, parent, qkv, m, dim)
+    hk.kda_tree_decode(qkv, f, b, state, parent, out, m, heads, **raw)
+    hk.mla_cache_append(kv_pre, ln_w, rows, 0, m, 1e-6)          # the nodes' latents, normalised into a buffer of their own
+    hk.mla_tree_decode(q, ckv, rows, parent, lat, m, n)
+    hk.kda_tree_accept(x32, window, qkv, f, b, state, parent, ints([leaf]), m, heads, **raw)
+    length = torch.zeros(1, dtype=torch.int32, device="cuda")
+    hk.mla_tree_accept(rows, ckv, parent, ints([leaf]), m, n, len_out=length)
+    finish()
+    assert torch.equal(state, st1) and torch.equal(window, w1) and torch.equal(ckv, c1) and int(length) == n + len(steps)
+    for i, j in enumerate(steps):
+        # fp32 sums in two orders, rounded to bf16 toward zero: a step of bf16 and 1e-5 of the largest
+        a, c = out[j].double(), outs1[i][0].double()
+        assert bool(((a - c).abs() <= 2.0 ** -7 * c.abs() + 1e-5 * c.abs().max()).all()), i
+        o, tol = attend(q[j].double(), c1[:n + i + 1].double(), 0.0625)
+        assert bool(((lat[j].double() - o).abs() <= tol).all()) and bool(((lat1[i][0].double() - o).abs() <= tol).all()), i
+
+
+@pytest.mark.parametrize("kind", ["tree", "tree8", "kda"])
+def test_captured_and_replayed_and_on_a_stream_of_its_own(kind):
+    """trees, lengths and accepted nodes are the device's: a captured call follows them"""
+    gen, heads = gen_of(30), 64
+    trees = [tree_of((10, 1)), tree_of("chain5")]
+    starts, parent, tree_start = layout(trees)
+    m, lens = starts[-1], ints([300, 90])
+    q, rows = (randn(gen, m, heads, 512) * 0.7).half(), randn(gen, m, 512).half()
+    ckv8, scales = cache(gen, "e4m3", 12, 64)
+    table, ckv = table_for(gen, 2, 6, 12), randn(gen, 800, 512).half()
+    base = torch.tensor([0, 400], device="cuda")
+    x = kda_inputs(gen, m, 8, 2)
+
+    def call(out, stream=None):
+        at = dict(n_seqs=2, tree_start=tree_start, stream=stream)
+        if kind == "tree":
+            hk.mla_tree_decode(q, ckv, rows, parent, out, m, kv_base=base, kv_len=lens, n_keys_hint=384, **at)
+        elif kind == "tree8":
+            hk.mla8_tree_decode(q, ckv8, scales, rows, parent, out, m, block_table=table, kv_len=lens, n_keys_hint=384, **at)
+        else:
+            hk.kda_tree_decode(x["qkv"], x["g"], x["beta"], x["state"], parent, out, m, 8, **at)
+
+    fresh = lambda: torch.zeros(m, 8, 128, dtype=torch.bfloat16, device="cuda") if kind == "kda" else torch.zeros(m, heads, 512, dtype=torch.float16, device="cuda")  # noqa: E731
+    first = fresh()
+    call(first)
+    side, there = torch.cuda.Stream(), fresh()
+    side.wait_stream(torch.cuda.current_stream())
+    call(there, side)
+    finish()
+    assert torch.equal(first, there)
+    out = fresh()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        call(out)
+    graph.replay()
+    finish()
+    assert torch.equal(out, first)
+    # other trees, lengths and inputs under the same graph
+    parent.copy_(ints(tree_of((m, 8))))
+    tree_start.copy_(ints([0, 3, m]))
+    lens.copy_(ints([17, 380]))
+    q.copy_(q.flip(0))
+    x["g"].mul_(0.5)
+    graph.replay()
+    again = fresh()
+    call(again)
+    finish()
+    assert torch.equal(out, again) and not torch.equal(out, first)
+
+
+def test_calls_without_rows_do_nothing():
+    e = lambda *s: torch.empty(*s, dtype=torch.float16, device="cuda")  # noqa: E731
+    none = ints([0])
+    hk.mla_tree_decode(e(0, 64, 512), e(4, 512), e(0, 512), none, e(0, 64, 512), 0, 4)
+    hk.kda_tree_decode(torch.empty(0, 384, dtype=torch.bfloat16, device="cuda"), torch.empty(0, 1, 128, device="cuda"), torch.empty(0, 1, dtype=torch.bfloat16, device="cuda"),
+                       torch.zeros(1, 1, 128, 128, device="cuda"), none, torch.empty(0, 1, 128, dtype=torch.bfloat16, device="cuda"), 0, 1)
+    length = ints([0])
+    hk.mla_tree_accept(e(0, 512), e(4, 512), none, ints([3]), 0, 2, len_out=length)
+    finish()
+    assert int(length) == 2
+
+
+def test_tensors_that_are_not_the_calls_are_refused():
+    m = 3
+    q, kv, out, c = (torch.zeros(s, dtype=torch.float16, device="cuda") for s in ((m, 64, 512), (m, 512), (m, 64, 512), (8, 512)))
+    p = ints([-1, 0, 1])
+    good = dict(q_lat=q, ckv=c, tree_kv=kv, parent=p, lat_out=out, m=m, pos_start=8)
+    hk.mla_tree_decode(**good)
+    for name, bad in (("q_lat", q.float()), ("tree_kv", kv[:2]), ("parent", p.long()), ("parent", p[:2]), ("ckv", c.t()), ("lat_out", out.cpu())):
+        with pytest.raises(ValueError):
+            hk.mla_tree_decode(**{**good, name: bad})
+    for more in (dict(tree_start=ints([0])), dict(kv_len=ints([])), dict(kv_base=ints([0]))):
+        with pytest.raises(ValueError):
+            hk.mla_tree_decode(**good, **more)
+    for more in (dict(pos_start=9), dict(n_seqs=2), dict(n_seqs=0), dict(n_heads=6), dict(pos_start=-1)):
+        with pytest.raises((hk.HeliosB200Error, ValueError)):
+            hk.mla_tree_decode(**{**good, **more})
+    s, b = torch.zeros(1, 1, 128, 128, device="cuda"), torch.bfloat16
+    kda = dict(mixed_qkv=torch.zeros(m, 384, dtype=b, device="cuda"), g=torch.zeros(m, 1, 128, device="cuda"), beta=torch.zeros(m, 1, dtype=b, device="cuda"), rec_state=s, parent=p,
+               out=torch.zeros(m, 1, 128, dtype=b, device="cuda"), m=m, num_heads=1)
+    hk.kda_tree_decode(**kda)
+    for more in (dict(max_nodes=65), dict(max_nodes=-1), dict(rec_state=s[:, :, :64]), dict(beta=kda["beta"].float()), dict(dt_bias=torch.zeros(1, 128, device="cuda")), dict(n_seqs=2),
+                 dict(out=kda["out"].float())):
+        with pytest.raises((hk.HeliosB200Error, ValueError)):
+            hk.kda_tree_decode(**{**kda, **more})
+    finish()
