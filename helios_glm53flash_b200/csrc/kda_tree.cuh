@@ -13,13 +13,14 @@ __global__ __launch_bounds__(256) void kda_tree_conv_kernel(const float* x, cons
   const int r = blockIdx.x, c = (blockIdx.y * 256 + threadIdx.x) * 4, s = tree.seq_of(r);
   if (s < 0) return;
   const int2 rows = tree.rows(s);
-  TreeParents up;
-  up.load(tree, rows);
   int at[4], j = r - rows.x;                               // the node and its next three ancestors; negative: the sequence's -1st, -2nd, ... last token
 #pragma unroll
   for (int i = 0, back = 0; i < 4; i++) {
     at[i] = j >= 0 ? j : --back;
-    j = j >= 0 ? up.parent_of(j) : -1;
+    if (j >= 0) {
+      const int p = tree.parent[rows.x + j];
+      j = p < j ? p : -1;
+    }
   }
   if (c >= dim) return;
   float4 in[4];
@@ -72,23 +73,47 @@ struct KdaTreeArgs {
   const int* leaf;
 };
 
-constexpr int KT_WARPS = 8, KT_THREADS = KT_WARPS * 32;
-template <int COLS>
-__host__ __device__ constexpr size_t kt_smem(int most) {
-  // K, Q, D [most][128]; S [128][COLS]; V, Q S [most][COLS]; A, B [most][most]; paths, betas
-  return (size_t)most * (3 * 128 + 2 * COLS + 2 * most + 3) * 4 + 128 * COLS * 4 + 16;
+// One CTA a (sequence, head, part of the value columns), sixteen warps; a warp has nodes w, w + 16, ... and of every row four channels a lane.
+//   tokens      q and k normalised, decays; k and decays of all nodes to shared memory
+//   pairs       A and B of a node with its ancestors, up its path: a dot product of two rows and the decays between them by the warp
+//   product     rows k E and q E of all nodes (M = 128: k in rows 0-63, q in 64-127) with S_0 on the tensor cores.  Both operands as two bf16 numbers,
+//               x = hi + lo, and three products hi hi + hi lo + lo hi: 2^-16 of the magnitudes, where bf16 keeps the range of fp32 (a state in fp16
+//               would overflow at 65,504)
+//   levels      u of the nodes of a depth, then their part in all nodes below: a node has one ancestor at each depth, so a level is one
+//               multiply-add a node and column, in registers, and one barrier
+constexpr int KT_WARPS = 16, KT_THREADS = KT_WARPS * 32;
+// Shared memory of a form: k E, q E (before them k and the decays, behind them u); S_0, then its products; lists of pairs.
+template <int COLS, int NS>
+struct KtForm {
+  // Up to 32 nodes: M = 64 in the form that spreads them over all lanes (columns from COLS / 2 on in lanes 64-127), half the operand, two CTAs an SM
+  static constexpr bool HALF = NS <= 2 && COLS >= 64;
+  static constexpr int M = HALF ? 64 : 128;
+  static constexpr uint32_t A_BLOCK = M * 128, S_BLOCK = 128 * 128;     // 64 channels of an operand: rows of 128 bytes
+  static constexpr uint32_t A = 0, A_LO = 2 * A_BLOCK, S = 4 * A_BLOCK;
+  static constexpr uint32_t S_BYTES = 128 * COLS * 2;                   // hi or lo
+  static constexpr uint32_t ROW = COLS + 4;                             // floats of a row of products (no bank conflicts)
+  static constexpr uint32_t MISC = S + (M * ROW * 4 > 2 * S_BYTES ? M * ROW * 4 : 2 * S_BYTES);
+};
+__host__ __device__ constexpr int kt_pairs(int nodes) { return nodes * (nodes - 1) / 2; }   // at most: a chain
+struct KtMisc {
+  uint64_t done;
+  uint32_t tmem;
+  int abort_flag;
+  int first[TREE_NODES];                // of a node's ancestors in the lists of pairs
+};
+template <int COLS, int NS>
+constexpr size_t kt_smem(int most) {
+  return 1024 + KtForm<COLS, NS>::MISC + sizeof(KtMisc) + (size_t)kt_pairs(most) * 9 + 16;
 }
 
-// k and decay of a node, four channels a lane
+// decays of a node, four channels a lane
 template <bool GATED>
-__device__ __forceinline__ float4 kt_decay(const KdaTreeArgs& a, int r, int head, int lane, float rate) {
-  float4 x = *reinterpret_cast<const float4*>(a.g + ((size_t)r * a.H + head) * 128 + 4 * lane);
+__device__ __forceinline__ float4 kt_decay(const KdaTreeArgs& a, float4 x, float4 bias, float rate) {
   if (GATED) {
-    const float4 b = *reinterpret_cast<const float4*>(a.dt_bias + head * 128 + 4 * lane);
-    x.x = gate_value(x.x, b.x, rate, a.lower_bound);
-    x.y = gate_value(x.y, b.y, rate, a.lower_bound);
-    x.z = gate_value(x.z, b.z, rate, a.lower_bound);
-    x.w = gate_value(x.w, b.w, rate, a.lower_bound);
+    x.x = gate_value(x.x, bias.x, rate, a.lower_bound);
+    x.y = gate_value(x.y, bias.y, rate, a.lower_bound);
+    x.z = gate_value(x.z, bias.z, rate, a.lower_bound);
+    x.w = gate_value(x.w, bias.w, rate, a.lower_bound);
   }
   return make_float4(__expf(x.x), __expf(x.y), __expf(x.z), __expf(x.w));
 }
@@ -100,172 +125,338 @@ __device__ __forceinline__ float kt_beta(const KdaTreeArgs& a, int r, int head) 
 }
 __device__ __forceinline__ float dot4(float4 a, float4 b) { return fmaf(a.w, b.w, fmaf(a.z, b.z, fmaf(a.y, b.y, a.x * b.x))); }
 __device__ __forceinline__ float4 mul4(float4 a, float4 b) { return make_float4(a.x * b.x, a.y * b.y, a.z * b.z, a.w * b.w); }
+// four numbers as bf16, and what that leaves of them as bf16
+__device__ __forceinline__ void kt_split(float4 x, uint2& hi, uint2& lo) {
+  const __nv_bfloat162 h0 = __floats2bfloat162_rn(x.x, x.y), h1 = __floats2bfloat162_rn(x.z, x.w);
+  const float2 f0 = __bfloat1622float2(h0), f1 = __bfloat1622float2(h1);
+  const __nv_bfloat162 l0 = __floats2bfloat162_rn(x.x - f0.x, x.y - f0.y), l1 = __floats2bfloat162_rn(x.z - f1.x, x.w - f1.y);
+  hi = make_uint2(*reinterpret_cast<const uint32_t*>(&h0), *reinterpret_cast<const uint32_t*>(&h1));
+  lo = make_uint2(*reinterpret_cast<const uint32_t*>(&l0), *reinterpret_cast<const uint32_t*>(&l1));
+}
+// VEC columns of a lane
+template <int VEC>
+struct KtVec {
+  float v[VEC];
+  __device__ __forceinline__ void load(const float* p) {
+    if constexpr (VEC == 4) {
+      const float4 x = *reinterpret_cast<const float4*>(p);
+      v[0] = x.x; v[1] = x.y; v[2] = x.z; v[3] = x.w;
+    } else if constexpr (VEC == 2) {
+      const float2 x = *reinterpret_cast<const float2*>(p);
+      v[0] = x.x; v[1] = x.y;
+    } else {
+      v[0] = *p;
+    }
+  }
+  __device__ __forceinline__ void store(float* p) const {
+    if constexpr (VEC == 4) *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
+    else if constexpr (VEC == 2) *reinterpret_cast<float2*>(p) = make_float2(v[0], v[1]);
+    else *p = v[0];
+  }
+  __device__ __forceinline__ void add(float f, const KtVec& x) {
+#pragma unroll
+    for (int u = 0; u < VEC; u++) v[u] = fmaf(f, x.v[u], v[u]);
+  }
+};
 
-template <bool GATED, int COLS>
-__global__ __launch_bounds__(KT_THREADS) void kda_tree_kernel(const KdaTreeArgs a) {
-  extern __shared__ __align__(16) float kt_mem[];
-  const int most = a.most, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  float* const K = kt_mem;                                 // k, then k E
-  float* const Q = K + most * 128;                         // q E
-  float* const Dc = Q + most * 128;                        // decays, then K S, then u
-  float* const S = Dc + most * 128;
-  float* const V = S + 128 * COLS;
-  float* const QS = V + most * COLS;
-  float* const A = QS + most * COLS;
-  float* const B = A + most * most;
-  float* const be = B + most * most;
-  uint64_t* const paths = reinterpret_cast<uint64_t*>(kt_mem + ((be + most - kt_mem + 1) & ~1));
+// NS: nodes of a warp, 16 NS of a tree at most
+template <bool GATED, int COLS, int NS>
+__global__ __launch_bounds__(KT_THREADS, NS == 1 ? 2 : 1) void kda_tree_kernel(const KdaTreeArgs a, int* __restrict__ status) {
+  extern __shared__ __align__(16) uint8_t kt_raw[];
+  using F = KtForm<COLS, NS>;
+  uint8_t* const smem = kt_raw + ((1024u - (tc::smem_u32(kt_raw) & 1023u)) & 1023u);
+  KtMisc& ms = *reinterpret_cast<KtMisc*>(smem + F::MISC);
+  volatile int* abort_flag = &ms.abort_flag;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tc::warp_index_uniform();
+  float* const K = reinterpret_cast<float*>(smem + F::A);
+  float* const Dc = reinterpret_cast<float*>(smem + F::A_LO);
+  float* const U = reinterpret_cast<float*>(smem + F::A);
+  float* const A = reinterpret_cast<float*>(smem + F::MISC + sizeof(KtMisc));
+  float* const B = A + kt_pairs(a.most);
+  uint8_t* const anc = reinterpret_cast<uint8_t*>(B + kt_pairs(a.most));
   const int head = blockIdx.x / (128 / COLS), v0 = blockIdx.x % (128 / COLS) * COLS, s = blockIdx.y;
+  constexpr int VEC = COLS / 32;
+  if (tid == 0) {
+    tc::mbar_init(&ms.done, 1);
+    tc::mbar_fence_init();
+    ms.abort_flag = 0;
+  }
+  if (warp == 0) tc::tmem_alloc(&ms.tmem, COLS);
   pdl_wait();
   const int2 rows = a.tree.rows(s);
-  const int n = min(rows.y, most);
-  if (n <= 0) return;
-  const float* st = a.state + ((size_t)(a.slots ? a.slots[s] : s) * a.H + head) * 128 * 128 + v0;
-  for (int i = tid; i < 128 * COLS / 4; i += KT_THREADS) {
-    const int c = i / (COLS / 4), v = i % (COLS / 4) * 4;
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(S + c * COLS + v)), "l"(st + (size_t)c * 128 + v) : "memory");
+  const int n = min(rows.y, a.most);                       // (0: the CTA passes through)
+  // ---- loads: the state, the tokens ----
+  constexpr int PIECES = 128 * COLS / 4 / KT_THREADS;
+  float4 st[PIECES];
+  {
+    const float* src = a.state + ((size_t)(a.slots ? a.slots[s] : s) * a.H + head) * 128 * 128 + v0;
+#pragma unroll
+    for (int i = 0; i < PIECES; i++) {
+      const int idx = tid + i * KT_THREADS;
+      st[i] = n > 0 ? *reinterpret_cast<const float4*>(src + (size_t)(idx / (COLS / 4)) * 128 + idx % (COLS / 4) * 4) : make_float4(0.f, 0.f, 0.f, 0.f);
+    }
   }
-  asm volatile("cp.async.commit_group;" ::: "memory");
+  TreePaths paths;
+  paths.load(a.tree, rows);
   const size_t dim = (size_t)3 * a.H * 128;
-  const float rate = GATED ? __expf(a.a_log[head]) : 0.f;
-  TreeParents up;
-  up.load(a.tree, rows);
-  for (int j = warp; j < n; j += KT_WARPS) {
+  float4 q[NS], k[NS], d[NS];
+  KtVec<VEC> kv[NS], o[NS];                                // v - k^T S - sum A u;  q^T S + sum B u
+  float be[NS];
+#pragma unroll
+  for (int t = 0; t < NS; t++) {
+    const int j = warp + t * KT_WARPS;
+    if (j >= n) continue;
     const int r = rows.x + j;
     const __nv_bfloat16* tok = a.qkv + r * dim + head * 128;
-    const float4 q = load4(tok + 4 * lane), k = load4(tok + a.H * 128 + 4 * lane);
-    const float4 d = kt_decay<GATED>(a, r, head, lane, rate);
-    const float qn = rsqrtf(warp_sum(dot4(q, q)) + 1e-6f), kn = rsqrtf(warp_sum(dot4(k, k)) + 1e-6f);
-    *reinterpret_cast<float4*>(Q + j * 128 + 4 * lane) = make_float4(q.x * qn, q.y * qn, q.z * qn, q.w * qn);
-    *reinterpret_cast<float4*>(K + j * 128 + 4 * lane) = make_float4(k.x * kn, k.y * kn, k.z * kn, k.w * kn);
-    *reinterpret_cast<float4*>(Dc + j * 128 + 4 * lane) = d;
-    if (lane < COLS / 4) *reinterpret_cast<float4*>(V + j * COLS + 4 * lane) = load4(tok + 2 * a.H * 128 + v0 + 4 * lane);
-    const uint64_t path = up.path(j);
-    if (lane == 0) {
-      be[j] = kt_beta<GATED>(a, r, head);
-      paths[j] = path;
+    q[t] = load4(tok + 4 * lane);
+    k[t] = load4(tok + a.H * 128 + 4 * lane);
+    d[t] = *reinterpret_cast<const float4*>(a.g + ((size_t)r * a.H + head) * 128 + 4 * lane);
+    const __nv_bfloat16* val = tok + 2 * a.H * 128 + v0 + VEC * lane;
+    if constexpr (VEC == 4) {
+      const float4 x = load4(val);
+      kv[t].v[0] = x.x; kv[t].v[1] = x.y; kv[t].v[2] = x.z; kv[t].v[3] = x.w;
+    } else if constexpr (VEC == 2) {
+      const uint32_t x = *reinterpret_cast<const uint32_t*>(val);
+      kv[t].v[0] = bf16lo(x); kv[t].v[1] = bf16hi(x);
+    } else {
+      kv[t].v[0] = __bfloat162float(*val);
     }
+    be[t] = kt_beta<GATED>(a, r, head);
+  }
+  const float rate = GATED ? __expf(a.a_log[head]) : 0.f;
+  const float4 bias = GATED ? *reinterpret_cast<const float4*>(a.dt_bias + head * 128 + 4 * lane) : make_float4(0.f, 0.f, 0.f, 0.f);
+  if (warp == KT_WARPS - 1) {                              // first pair of every node: nodes lane and lane + 32, sums of the depths before
+    const int depth[2] = {__popcll(paths.lo) - 1, __popcll(paths.hi) - 1};
+    int sum[2] = {depth[0], depth[1]};
+#pragma unroll
+    for (int x = 1; x < 32; x <<= 1) {
+      const int y0 = __shfl_up_sync(0xffffffffu, sum[0], x), y1 = __shfl_up_sync(0xffffffffu, sum[1], x);
+      if (lane >= x) {
+        sum[0] += y0;
+        sum[1] += y1;
+      }
+    }
+    const int low = __shfl_sync(0xffffffffu, sum[0], 31);
+    ms.first[lane] = sum[0] - depth[0];
+    ms.first[lane + 32] = low + sum[1] - depth[1];
+  }
+#pragma unroll
+  for (int t = 0; t < NS; t++) {
+    const int j = warp + t * KT_WARPS;
+    if (j >= n) continue;
+    const float qn = rsqrtf(warp_sum(dot4(q[t], q[t])) + 1e-6f), kn = rsqrtf(warp_sum(dot4(k[t], k[t])) + 1e-6f);
+    q[t] = make_float4(q[t].x * qn, q[t].y * qn, q[t].z * qn, q[t].w * qn);
+    k[t] = make_float4(k[t].x * kn, k[t].y * kn, k[t].z * kn, k[t].w * kn);
+    d[t] = kt_decay<GATED>(a, d[t], bias, rate);
+    *reinterpret_cast<float4*>(K + j * 128 + 4 * lane) = k[t];
+    *reinterpret_cast<float4*>(Dc + j * 128 + 4 * lane) = d[t];
+  }
+  // the state as two bf16 operands: rows of 64 columns, the product's K along the rows' number
+#pragma unroll
+  for (int i = 0; i < PIECES; i++) {
+    const int idx = tid + i * KT_THREADS, c = idx / (COLS / 4), v = idx % (COLS / 4) * 4;
+    const uint32_t off = COLS == 32 ? c * 64 + (((v >> 3) ^ (c >> 1 & 3)) << 4) + (v & 4) * 2
+                                    : (v >> 6) * F::S_BLOCK + c * 128 + (((v >> 3 & 7) ^ (c & 7)) << 4) + (v & 4) * 2;
+    uint2 hi, lo;
+    kt_split(st[i], hi, lo);
+    *reinterpret_cast<uint2*>(smem + F::S + off) = hi;
+    *reinterpret_cast<uint2*>(smem + F::S + F::S_BYTES + off) = lo;
   }
   __syncthreads();
   // ---- tokens with each other, up every node's path ----
-  float4 ke[TREE_NODES / KT_WARPS];
+  float self[NS];
+  int depth[NS], first[NS];
 #pragma unroll
-  for (int t = 0; t < TREE_NODES / KT_WARPS; t++) {
+  for (int t = 0; t < NS; t++) {
     const int j = warp + t * KT_WARPS;
+    depth[t] = -1;
     if (j >= n) continue;
-    const float4 q = *reinterpret_cast<const float4*>(Q + j * 128 + 4 * lane), k = *reinterpret_cast<const float4*>(K + j * 128 + 4 * lane);
-    float4 e = *reinterpret_cast<const float4*>(Dc + j * 128 + 4 * lane);
-    const float own = warp_sum(dot4(q, k));
-    if (lane == 0) B[j * most + j] = own;
-    for (int i = up.parent_of(j); i >= 0; i = up.parent_of(i)) {
-      const float4 x = mul4(*reinterpret_cast<const float4*>(K + i * 128 + 4 * lane), e);
-      float ab = dot4(k, x), bb = dot4(q, x);
-      // two sums at once: lanes 0-15 take the one, 16-31 the other
-      const float mine = lane < 16 ? ab : bb, others = lane < 16 ? bb : ab;
-      float sum = mine + __shfl_xor_sync(0xffffffffu, others, 16);
+    self[t] = warp_sum(dot4(q[t], k[t]));
+    uint64_t above = paths.of(j) & ~(1ull << j);
+    depth[t] = __popcll(above);
+    first[t] = ms.first[j];
+    float4 e = d[t];
+    // four ancestors a turn, the nearest first
+    for (int at = first[t] + depth[t]; above; at -= 4) {
+      int i[4];
+      float4 x[4], y[4];
 #pragma unroll
-      for (int o = 8; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-      if ((lane & 15) == 0) (lane == 0 ? A : B)[j * most + i] = sum;
-      e = mul4(e, *reinterpret_cast<const float4*>(Dc + i * 128 + 4 * lane));
-    }
-    ke[t] = mul4(k, e);
-    *reinterpret_cast<float4*>(Q + j * 128 + 4 * lane) = mul4(q, e);
-  }
-  __syncthreads();
-#pragma unroll
-  for (int t = 0; t < TREE_NODES / KT_WARPS; t++)
-    if (const int j = warp + t * KT_WARPS; j < n) *reinterpret_cast<float4*>(K + j * 128 + 4 * lane) = ke[t];
-  asm volatile("cp.async.wait_group 0;" ::: "memory");
-  __syncthreads();
-  // ---- all nodes' rows with S_0: rows of K and Q (2 n), a thread ROWS of them and four columns ----
-  constexpr int COL_THREADS = COLS / 4, GROUPS = KT_THREADS / COL_THREADS;
-  const int c4 = tid % COL_THREADS * 4, grp = tid / COL_THREADS;
-  auto product = [&](auto rows_each) {
-    constexpr int ROWS = decltype(rows_each)::value;
-    for (int r0 = grp * ROWS; r0 < 2 * n; r0 += GROUPS * ROWS) {
-      const float* x[ROWS];
-      float4 acc[ROWS];
-#pragma unroll
-      for (int i = 0; i < ROWS; i++) {
-        const int row = min(r0 + i, 2 * n - 1);
-        x[i] = row < n ? K + row * 128 : Q + (row - n) * 128;
-        acc[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+      for (int u = 0; u < 4; u++) {
+        i[u] = above ? 63 - __clzll((long long)above) : -1;
+        if (i[u] < 0) continue;
+        above &= ~(1ull << i[u]);
+        x[u] = *reinterpret_cast<const float4*>(K + i[u] * 128 + 4 * lane);
+        y[u] = *reinterpret_cast<const float4*>(Dc + i[u] * 128 + 4 * lane);
       }
-#pragma unroll 2
-      for (int c = 0; c < 128; c += 4) {
-        float4 w[4];
+      float v[8];
 #pragma unroll
-        for (int e = 0; e < 4; e++) w[e] = *reinterpret_cast<const float4*>(S + (c + e) * COLS + c4);
+      for (int u = 0; u < 4; u++) {
+        v[u] = v[4 + u] = 0.f;
+        if (i[u] < 0) continue;
+        x[u] = mul4(x[u], e);
+        v[u] = dot4(k[t], x[u]);
+        v[4 + u] = dot4(q[t], x[u]);
+        e = mul4(e, y[u]);
+      }
+      // the eight sums over the warp, one in every four lanes: halves of the list go to halves of the warp
 #pragma unroll
-        for (int i = 0; i < ROWS; i++) {
-          const float4 y = *reinterpret_cast<const float4*>(x[i] + c);
-          const float ys[4] = {y.x, y.y, y.z, y.w};
+      for (int half = 4, m = 16; half >= 1; half >>= 1, m >>= 1) {
 #pragma unroll
-          for (int e = 0; e < 4; e++) {
-            acc[i].x = fmaf(ys[e], w[e].x, acc[i].x);
-            acc[i].y = fmaf(ys[e], w[e].y, acc[i].y);
-            acc[i].z = fmaf(ys[e], w[e].z, acc[i].z);
-            acc[i].w = fmaf(ys[e], w[e].w, acc[i].w);
-          }
+        for (int u = 0; u < half; u++) {
+          const float mine = lane & m ? v[half + u] : v[u], others = lane & m ? v[u] : v[half + u];
+          v[u] = mine + __shfl_xor_sync(0xffffffffu, others, m);
         }
       }
-#pragma unroll
-      for (int i = 0; i < ROWS; i++)
-        if (const int row = r0 + i; row < 2 * n) *reinterpret_cast<float4*>((row < n ? Dc + row * COLS : QS + (row - n) * COLS) + c4) = acc[i];
-    }
-  };
-  if (2 * n <= 2 * GROUPS) product(std::integral_constant<int, 2>());
-  else if (2 * n <= 4 * GROUPS) product(std::integral_constant<int, 4>());
-  else product(std::integral_constant<int, 8>());
-  __syncthreads();
-  // ---- u, node after node; a thread a column ----
-  float* const U = Dc;
-  if (tid < COLS) {
-    for (int j = 0; j < n; j++) {
-      float x = V[j * COLS + tid] - U[j * COLS + tid];
-      for (uint64_t m = paths[j] & ~(1ull << j); m; m &= m - 1) {
-        const int i = __ffsll((long long)m) - 1;
-        x = fmaf(-A[j * most + i], U[i * COLS + tid], x);
+      v[0] += __shfl_xor_sync(0xffffffffu, v[0], 2);
+      v[0] += __shfl_xor_sync(0xffffffffu, v[0], 1);
+      const int u = lane >> 2 & 3, to = at - 1 - u;        // lanes 0-15: A, 16-31: B
+      const int who = u == 0 ? i[0] : u == 1 ? i[1] : u == 2 ? i[2] : i[3];
+      if ((lane & 3) == 0 && who >= 0) {
+        (lane < 16 ? A : B)[to] = v[0];
+        if (lane < 16) anc[to] = (uint8_t)who;
       }
-      U[j * COLS + tid] = x * be[j];
+    }
+    k[t] = mul4(k[t], e);
+    q[t] = mul4(q[t], e);
+  }
+  __syncthreads();                                         // k and decays have been read
+#pragma unroll
+  for (int t = 0; t < NS; t++) {
+    const int j = warp + t * KT_WARPS;
+    if (j >= n) continue;
+    const uint32_t off = (lane >> 4) * F::A_BLOCK + j * 128 + (((lane >> 1 & 7) ^ (j & 7)) << 4) + (lane & 1) * 8;
+    uint2 hi, lo;
+    kt_split(k[t], hi, lo);
+    *reinterpret_cast<uint2*>(smem + F::A + off) = hi;
+    *reinterpret_cast<uint2*>(smem + F::A_LO + off) = lo;
+    kt_split(q[t], hi, lo);
+    *reinterpret_cast<uint2*>(smem + F::A + off + F::M / 2 * 128) = hi;
+    *reinterpret_cast<uint2*>(smem + F::A_LO + off + F::M / 2 * 128) = lo;
+  }
+  tc::fence_async_smem();
+  tc::fence_before_sync();
+  __syncthreads();
+  tc::fence_after_sync();
+  const uint32_t tmem = ms.tmem;
+  if (warp == 0) {
+    // rows of nodes that there are not are whatever lies there: their products are not read
+    const uint32_t leader = tc::elect_one(), idesc = tc::make_idesc(F::M, COLS, tc::FMT_BF16, tc::FMT_BF16, false, true);
+    const uint32_t base = tc::smem_u32(smem);
+#pragma unroll
+    for (int part = 0; part < 3; part++) {
+      const uint64_t ad = tc::make_sdesc_sw128(base + (part == 2 ? F::A_LO : F::A), 16, 1024);
+      const uint32_t sb = base + F::S + (part == 1 ? F::S_BYTES : 0);
+      const uint64_t bd = COLS == 32 ? tc::make_sdesc_sw64(sb, 128 * 64, 512) : tc::make_sdesc_sw128(sb, F::S_BLOCK, 1024);
+#pragma unroll
+      for (int kk = 0; kk < 8; kk++) {
+        const uint64_t x = tc::sdesc_advance(ad, (kk >> 2) * F::A_BLOCK + (kk & 3) * 32), y = tc::sdesc_advance(bd, kk * (COLS == 32 ? 1024 : 2048));
+        if (F::HALF) tc::mma_ws_f16_if(leader, tmem, x, y, idesc, part > 0 || kk > 0);
+        else tc::mma_f16_if(leader, tmem, x, y, idesc, part > 0 || kk > 0);
+      }
+    }
+    tc::mma_commit_if(leader, &ms.done);
+  }
+  tc::mbar_wait(&ms.done, 0, abort_flag, 51);
+  tc::fence_after_sync();
+  {
+    // products to shared memory, over the state: warp w has lanes 32 (w % 4) .., a quarter of the columns that they hold
+    constexpr int HELD = F::HALF ? COLS / 2 : COLS;
+    float* const R = reinterpret_cast<float*>(smem + F::S);
+    const int at = (warp & 3) * 32 + lane, c0 = (warp >> 2) * (HELD / 4), row = at % F::M, col = at / F::M * HELD + c0;
+    const uint32_t src = tmem + ((uint32_t)((warp & 3) * 32) << 16) + c0;
+    uint32_t x[HELD / 4];
+    if constexpr (HELD == 128) tc::tmem_ld32(src, x);
+    else if constexpr (HELD == 64) tc::tmem_ld16(src, x);
+    else tc::tmem_ld8(src, x);
+    tc::tmem_ld_wait();
+    tc::fence_before_sync();
+#pragma unroll
+    for (int c = 0; c < HELD / 4; c += 4) *reinterpret_cast<uint4*>(R + row * F::ROW + col + c) = make_uint4(x[c], x[c + 1], x[c + 2], x[c + 3]);
+    __syncthreads();
+#pragma unroll
+    for (int t = 0; t < NS; t++) {
+      const int j = warp + t * KT_WARPS;
+      if (j >= n) continue;
+      KtVec<VEC> y;
+      y.load(R + j * F::ROW + VEC * lane);
+      kv[t].add(-1.f, y);
+      o[t].load(R + (F::M / 2 + j) * F::ROW + VEC * lane);
+    }
+  }
+  // ---- level by level ----
+  for (int level = 0;; level++) {
+    bool more = false;
+#pragma unroll
+    for (int t = 0; t < NS; t++) {
+      more |= depth[t] > level;
+      if (depth[t] != level) continue;
+      const int j = warp + t * KT_WARPS;
+      KtVec<VEC> u;
+#pragma unroll
+      for (int e = 0; e < VEC; e++) u.v[e] = kv[t].v[e] * be[t];
+      u.store(U + j * COLS + VEC * lane);
+      o[t].add(self[t], u);
+    }
+    if (!__syncthreads_or(more)) break;
+#pragma unroll
+    for (int t = 0; t < NS; t++) {
+      if (depth[t] <= level) continue;
+      const int at = first[t] + level;
+      KtVec<VEC> u;
+      u.load(U + anc[at] * COLS + VEC * lane);
+      kv[t].add(-A[at], u);
+      o[t].add(B[at], u);
+    }
+  }
+  const float scale = rsqrtf(128.f);
+  if (!*abort_flag) {
+#pragma unroll
+    for (int t = 0; t < NS; t++) {
+      const int j = warp + t * KT_WARPS;
+      if (j >= n) continue;
+      const size_t at = ((size_t)(rows.x + j) * a.H + head) * 128 + v0 + VEC * lane;
+      uint16_t h[VEC];
+#pragma unroll
+      for (int e = 0; e < VEC; e++) {
+        o[t].v[e] *= scale;
+        h[e] = __bfloat16_as_ushort(__float2bfloat16_rz(o[t].v[e]));
+      }
+      uint16_t* out = reinterpret_cast<uint16_t*>(a.out) + at;
+      if constexpr (VEC == 4) *reinterpret_cast<uint2*>(out) = make_uint2(h[0] | (uint32_t)h[1] << 16, h[2] | (uint32_t)h[3] << 16);
+      else if constexpr (VEC == 2) *reinterpret_cast<uint32_t*>(out) = h[0] | (uint32_t)h[1] << 16;
+      else *out = h[0];
+      if (a.out_f32) o[t].store(a.out_f32 + at);
     }
   }
   __syncthreads();
-  const float scale = rsqrtf(128.f);
-  for (int idx = tid; idx < n * COLS; idx += KT_THREADS) {
-    const int j = idx / COLS, c = idx % COLS;
-    float x = QS[idx];
-    for (uint64_t m = paths[j]; m; m &= m - 1) {
-      const int i = __ffsll((long long)m) - 1;
-      x = fmaf(B[j * most + i], U[i * COLS + c], x);
-    }
-    x *= scale;
-    const size_t o = ((size_t)(rows.x + j) * a.H + head) * 128 + v0 + c;
-    a.out[o] = __float2bfloat16_rz(x);
-    if (a.out_f32) a.out_f32[o] = x;
-  }
+  if (warp == 0) tc::tmem_dealloc(tmem, COLS);
+  if (tid == 0 && ms.abort_flag && status) atomicExch(status, HK_ERR_TIMEOUT);
 }
 
-template <bool GATED, int COLS>
+template <bool GATED, int COLS, int NS>
 static int kt_launch(const KdaTreeArgs& a, cudaStream_t s) {
   static bool attr_set[64] = {false};
   const int dev = device_index();
   if (!attr_set[dev]) {
-    if (cudaFuncSetAttribute(kda_tree_kernel<GATED, COLS>, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024) != cudaSuccess) return HK_ERR_CUDA;
+    if (cudaFuncSetAttribute(kda_tree_kernel<GATED, COLS, NS>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kt_smem<COLS, NS>(16 * NS)) != cudaSuccess) return HK_ERR_CUDA;
     attr_set[dev] = true;
   }
-  return pdl_launch(kda_tree_kernel<GATED, COLS>, dim3((unsigned)(a.H * (128 / COLS)), (unsigned)a.tree.n_seqs), dim3(KT_THREADS), kt_smem<COLS>(a.most), s, a) ==
-                 cudaSuccess
+  return pdl_launch(kda_tree_kernel<GATED, COLS, NS>, dim3((unsigned)(a.H * (128 / COLS)), (unsigned)a.tree.n_seqs), dim3(KT_THREADS), kt_smem<COLS, NS>(a.most), s, a,
+                    device_status_ptr()) == cudaSuccess
              ? HK_OK
              : HK_ERR_CUDA;
+}
+template <bool GATED, int COLS>
+static int kt_nodes(const KdaTreeArgs& a, cudaStream_t s) {
+  return a.most <= 16 ? kt_launch<GATED, COLS, 1>(a, s) : a.most <= 32 ? kt_launch<GATED, COLS, 2>(a, s) : kt_launch<GATED, COLS, 4>(a, s);
 }
 template <bool GATED>
 static int kt_run(const KdaTreeArgs& a, cudaStream_t s) {
   // few heads: a head's columns over two or four CTAs, which prepare the tokens each for itself
   const int64_t heads = (int64_t)a.H * a.tree.n_seqs;
-  if (4 * heads <= sm_count()) return kt_launch<GATED, 32>(a, s);
-  if (2 * heads <= 2 * sm_count() || a.most > 32) return kt_launch<GATED, 64>(a, s);
-  return kt_launch<GATED, 128>(a, s);
+  if (4 * heads <= sm_count()) return kt_nodes<GATED, 32>(a, s);
+  if (2 * heads <= sm_count()) return kt_nodes<GATED, 64>(a, s);
+  return kt_nodes<GATED, 128>(a, s);
 }
 
 // ---- the step to an accepted node: the recurrence along its path, in the order of sums that all token-by-token kernels share ----
@@ -399,7 +590,7 @@ HK_API int hk_kda_tree(const void* mixed_qkv, const float* g, const void* beta, 
   using namespace hk;
   KdaTreeArgs a;
   HK_REQUIRE(kda_tree_args(&a, mixed_qkv, g, beta, dt_bias, a_log, lower_bound, const_cast<float*>(rec_state), slots, parent, tree_start, n_seqs, m, num_heads));
-  HK_REQUIRE((out || m == 0) && max_nodes >= 0 && max_nodes <= TREE_NODES);
+  HK_REQUIRE((out || m == 0) && aligned(out, 8) && (!out_f32 || aligned(out_f32, 16)) && max_nodes >= 0 && max_nodes <= TREE_NODES);
   if (m == 0) return HK_OK;
   a.out = (__nv_bfloat16*)out;
   a.out_f32 = out_f32;

@@ -68,11 +68,11 @@ __device__ __forceinline__ MlaTree mla_tree(const MlaArgs& a, int r) {
   MlaTree t{0, 0, a.tree.seq_of(r), 0, 0, -1};
   if (t.seq < 0) return t;
   const int2 rows = a.tree.rows(t.seq);
-  TreeParents up;
-  up.load(a.tree, rows);
+  TreePaths paths;
+  paths.load(a.tree, rows);
   t.row0 = rows.x;
   t.node = r - rows.x;
-  t.path = up.path(t.node);
+  t.path = paths.of(t.node);
   t.base = a.kv_base ? a.kv_base[t.seq] : 0;
   t.len = max(a.kv_len ? a.kv_len[t.seq] : a.pos_start, 0);
   if (a.ckv_rows > 0) t.len = (int)max((int64_t)0, min((int64_t)t.len, a.ckv_rows - t.base));   // never past the end of the cache

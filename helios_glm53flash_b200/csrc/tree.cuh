@@ -36,33 +36,45 @@ struct TreeArgs {
   }
 };
 
-// The parents of a tree's nodes, nodes lane and lane + 32 in a lane; a node's parent comes before it, so a walk to the root ends.
-struct TreeParents {
-  int lo, hi;
+// The paths of a tree's nodes - a node and its ancestors, a bit each - nodes lane and lane + 32 in a lane.  By doubling: after round r a node has its
+// 2^r nearest ancestors and knows the next one up; a chain of 64 takes six rounds, a tree that is eight deep three.
+struct TreePaths {
+  uint64_t lo, hi;
   __device__ __forceinline__ void load(const TreeArgs& t, int2 rows) {
     const int lane = threadIdx.x & 31;
-    auto of = [&](int j) {
+    auto parent = [&](int j) {                             // (a parent comes before its nodes, else there is none)
       const int p = j < rows.y ? t.parent[rows.x + j] : -1;
       return p < 0 || p >= j ? -1 : p;
     };
-    lo = of(lane);
-    hi = of(lane + 32);
+    int up_lo = parent(lane), up_hi = parent(lane + 32);
+    lo = 1ull << lane;
+    hi = 1ull << (lane + 32);
+    while (__any_sync(0xffffffffu, up_lo >= 0 || up_hi >= 0)) {
+      const uint64_t a = of(up_lo), b = of(up_hi);         // (both before either changes)
+      const int next_lo = at(up_lo, up_lo, up_hi), next_hi = at(up_hi, up_lo, up_hi);
+      if (up_lo >= 0) lo |= a;
+      if (up_hi >= 0) hi |= b;
+      up_lo = up_lo >= 0 ? next_lo : -1;
+      up_hi = up_hi >= 0 ? next_hi : -1;
+    }
   }
-  __device__ __forceinline__ int parent_of(int j) const { return __shfl_sync(0xffffffffu, j < 32 ? lo : hi, j & 31); }   // (j: the same in all lanes)
-  // a node and its ancestors, as bits
-  __device__ __forceinline__ uint64_t path(int j) const {
-    uint64_t mask = 0;
-    for (; j >= 0; j = parent_of(j)) mask |= 1ull << j;
-    return mask;
+  static __device__ __forceinline__ int at(int j, int lo, int hi) {
+    const int x = __shfl_sync(0xffffffffu, lo, j & 31), y = __shfl_sync(0xffffffffu, hi, j & 31);
+    return j < 32 ? x : y;
+  }
+  // the path of node j (each lane's own j)
+  __device__ __forceinline__ uint64_t of(int j) const {
+    const uint64_t x = __shfl_sync(0xffffffffu, lo, j & 31), y = __shfl_sync(0xffffffffu, hi, j & 31);
+    return j < 32 ? x : y;
   }
 };
 
 // the path of a sequence's accepted node, as bits; none: 0.  Executed by a whole warp.
 __device__ __forceinline__ uint64_t tree_path(const TreeArgs& t, int2 rows, int leaf) {
   if (leaf < 0 || leaf >= rows.y) return 0;
-  TreeParents up;
-  up.load(t, rows);
-  return up.path(leaf);
+  TreePaths paths;
+  paths.load(t, rows);
+  return paths.of(leaf);
 }
 
 // host: arguments of a tree call; without rows there need be no arrays of rows
