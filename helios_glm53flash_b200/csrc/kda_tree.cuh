@@ -73,20 +73,20 @@ struct KdaTreeArgs {
   const int* leaf;
 };
 
-// One CTA a (sequence, head, part of the value columns), sixteen warps; a warp has nodes w, w + 16, ... and of every row four channels a lane.
+// One CTA a (sequence, head, part of the value columns), sixteen warps; G lanes a node - 8, 16 or 32 for up to 64, 32 or 16 nodes - with 128 / G of a
+// row's channels each, so that every node is somewhere and no phase loops over nodes.
 //   tokens      q and k normalised, decays; k and decays of all nodes to shared memory
-//   pairs       A and B of a node with its ancestors, up its path: a dot product of two rows and the decays between them by the warp
-//   product     rows k E and q E of all nodes (M = 128: k in rows 0-63, q in 64-127) with S_0 on the tensor cores.  Both operands as two bf16 numbers,
-//               x = hi + lo, and three products hi hi + hi lo + lo hi: 2^-16 of the magnitudes, where bf16 keeps the range of fp32 (a state in fp16
-//               would overflow at 65,504)
+//   pairs       A and B of a node with its ancestors, up its path: a dot product of two rows and the decays between them by its G lanes
+//   product     rows k E and q E of all nodes with S_0 on the tensor cores.  Both operands as two bf16 numbers, x = hi + lo, and three products
+//               hi hi + hi lo + lo hi: 2^-16 of the magnitudes, where bf16 keeps the range of fp32 (a state in fp16 would overflow at 65,504)
 //   levels      u of the nodes of a depth, then their part in all nodes below: a node has one ancestor at each depth, so a level is one
 //               multiply-add a node and column, in registers, and one barrier
 constexpr int KT_WARPS = 16, KT_THREADS = KT_WARPS * 32;
 // Shared memory of a form: k E, q E (before them k and the decays, behind them u); S_0, then its products; lists of pairs.
-template <int COLS, int NS>
+template <int COLS, int G>
 struct KtForm {
   // Up to 32 nodes: M = 64 in the form that spreads them over all lanes (columns from COLS / 2 on in lanes 64-127), half the operand, two CTAs an SM
-  static constexpr bool HALF = NS <= 2 && COLS >= 64;
+  static constexpr bool HALF = G >= 16 && COLS >= 64;
   static constexpr int M = HALF ? 64 : 128;
   static constexpr uint32_t A_BLOCK = M * 128, S_BLOCK = 128 * 128;     // 64 channels of an operand: rows of 128 bytes
   static constexpr uint32_t A = 0, A_LO = 2 * A_BLOCK, S = 4 * A_BLOCK;
@@ -94,16 +94,17 @@ struct KtForm {
   static constexpr uint32_t ROW = COLS + 4;                             // floats of a row of products (no bank conflicts)
   static constexpr uint32_t MISC = S + (M * ROW * 4 > 2 * S_BYTES ? M * ROW * 4 : 2 * S_BYTES);
 };
-__host__ __device__ constexpr int kt_pairs(int nodes) { return nodes * (nodes - 1) / 2; }   // at most: a chain
+// Places of pairs of `nodes` nodes, at most (a chain): a node's ancestors from the root on, from a multiple of four on, the last four not whole
+__host__ __device__ constexpr int kt_pairs(int nodes) { return (nodes * (nodes - 1) / 2 + 3 * nodes + 3) / 4 * 4; }
 struct KtMisc {
   uint64_t done;
   uint32_t tmem;
   int abort_flag;
-  int first[TREE_NODES];                // of a node's ancestors in the lists of pairs
+  int first[TREE_NODES];                // of a node's ancestors in the lists of pairs, in fours
 };
-template <int COLS, int NS>
+template <int COLS, int G>
 constexpr size_t kt_smem(int most) {
-  return 1024 + KtForm<COLS, NS>::MISC + sizeof(KtMisc) + (size_t)kt_pairs(most) * 9 + 16;
+  return 1024 + KtForm<COLS, G>::MISC + sizeof(KtMisc) + (size_t)kt_pairs(most) * 9 + 16;
 }
 
 // decays of a node, four channels a lane
@@ -124,7 +125,6 @@ __device__ __forceinline__ float kt_beta(const KdaTreeArgs& a, int r, int head) 
                : __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(a.beta)[i]);
 }
 __device__ __forceinline__ float dot4(float4 a, float4 b) { return fmaf(a.w, b.w, fmaf(a.z, b.z, fmaf(a.y, b.y, a.x * b.x))); }
-__device__ __forceinline__ float4 mul4(float4 a, float4 b) { return make_float4(a.x * b.x, a.y * b.y, a.z * b.z, a.w * b.w); }
 // four numbers as bf16, and what that leaves of them as bf16
 __device__ __forceinline__ void kt_split(float4 x, uint2& hi, uint2& lo) {
   const __nv_bfloat162 h0 = __floats2bfloat162_rn(x.x, x.y), h1 = __floats2bfloat162_rn(x.z, x.w);
@@ -133,37 +133,43 @@ __device__ __forceinline__ void kt_split(float4 x, uint2& hi, uint2& lo) {
   hi = make_uint2(*reinterpret_cast<const uint32_t*>(&h0), *reinterpret_cast<const uint32_t*>(&h1));
   lo = make_uint2(*reinterpret_cast<const uint32_t*>(&l0), *reinterpret_cast<const uint32_t*>(&l1));
 }
-// VEC columns of a lane
-template <int VEC>
-struct KtVec {
-  float v[VEC];
-  __device__ __forceinline__ void load(const float* p) {
-    if constexpr (VEC == 4) {
-      const float4 x = *reinterpret_cast<const float4*>(p);
-      v[0] = x.x; v[1] = x.y; v[2] = x.z; v[3] = x.w;
-    } else if constexpr (VEC == 2) {
-      const float2 x = *reinterpret_cast<const float2*>(p);
-      v[0] = x.x; v[1] = x.y;
-    } else {
-      v[0] = *p;
-    }
+__device__ __forceinline__ void kt_split(uint64_t x, uint64_t y, uint2& hi, uint2& lo) {
+  float4 v;
+  unpack2(x, v.x, v.y);
+  unpack2(y, v.z, v.w);
+  kt_split(v, hi, lo);
+}
+// N numbers of a lane, or of a row from p on
+template <int N>
+__device__ __forceinline__ void kt_load(const float* p, float (&x)[N]) {
+  if constexpr (N == 4) {
+    const float4 v = *reinterpret_cast<const float4*>(p);
+    x[0] = v.x; x[1] = v.y; x[2] = v.z; x[3] = v.w;
+  } else if constexpr (N == 2) {
+    const float2 v = *reinterpret_cast<const float2*>(p);
+    x[0] = v.x; x[1] = v.y;
+  } else {
+    x[0] = *p;
   }
-  __device__ __forceinline__ void store(float* p) const {
-    if constexpr (VEC == 4) *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
-    else if constexpr (VEC == 2) *reinterpret_cast<float2*>(p) = make_float2(v[0], v[1]);
-    else *p = v[0];
-  }
-  __device__ __forceinline__ void add(float f, const KtVec& x) {
+}
+template <int N>
+__device__ __forceinline__ void kt_store(float* p, const float (&x)[N]) {
+  if constexpr (N == 4) *reinterpret_cast<float4*>(p) = make_float4(x[0], x[1], x[2], x[3]);
+  else if constexpr (N == 2) *reinterpret_cast<float2*>(p) = make_float2(x[0], x[1]);
+  else *p = x[0];
+}
+// sum over the G lanes of a node
+template <int G>
+__device__ __forceinline__ float kt_sum(float v) {
 #pragma unroll
-    for (int u = 0; u < VEC; u++) v[u] = fmaf(f, x.v[u], v[u]);
-  }
-};
+  for (int m = G / 2; m > 0; m >>= 1) v += __shfl_xor_sync(0xffffffffu, v, m);
+  return v;
+}
 
-// NS: nodes of a warp, 16 NS of a tree at most
-template <bool GATED, int COLS, int NS>
-__global__ __launch_bounds__(KT_THREADS, NS == 1 ? 2 : 1) void kda_tree_kernel(const KdaTreeArgs a, int* __restrict__ status) {
+template <bool GATED, int COLS, int G>
+__global__ __launch_bounds__(KT_THREADS, G == 32 ? 2 : 1) void kda_tree_kernel(const KdaTreeArgs a, int* __restrict__ status) {
   extern __shared__ __align__(16) uint8_t kt_raw[];
-  using F = KtForm<COLS, NS>;
+  using F = KtForm<COLS, G>;
   uint8_t* const smem = kt_raw + ((1024u - (tc::smem_u32(kt_raw) & 1023u)) & 1023u);
   KtMisc& ms = *reinterpret_cast<KtMisc*>(smem + F::MISC);
   volatile int* abort_flag = &ms.abort_flag;
@@ -175,13 +181,12 @@ __global__ __launch_bounds__(KT_THREADS, NS == 1 ? 2 : 1) void kda_tree_kernel(c
   float* const B = A + kt_pairs(a.most);
   uint8_t* const anc = reinterpret_cast<uint8_t*>(B + kt_pairs(a.most));
   const int head = blockIdx.x / (128 / COLS), v0 = blockIdx.x % (128 / COLS) * COLS, s = blockIdx.y;
-  constexpr int VEC = COLS / 32;
   if (tid == 0) {
     tc::mbar_init(&ms.done, 1);
     tc::mbar_fence_init();
     ms.abort_flag = 0;
   }
-  if (warp == 0) tc::tmem_alloc(&ms.tmem, COLS);
+  if (warp == KT_WARPS - 2) tc::tmem_alloc(&ms.tmem, COLS);
   pdl_wait();
   const int2 rows = a.tree.rows(s);
   const int n = min(rows.y, a.most);                       // (0: the CTA passes through)
@@ -196,37 +201,51 @@ __global__ __launch_bounds__(KT_THREADS, NS == 1 ? 2 : 1) void kda_tree_kernel(c
       st[i] = n > 0 ? *reinterpret_cast<const float4*>(src + (size_t)(idx / (COLS / 4)) * 128 + idx % (COLS / 4) * 4) : make_float4(0.f, 0.f, 0.f, 0.f);
     }
   }
+  // this lane's node, channels 4 l + 4 G m .. + 3 of its rows, and columns VEC l + VEC G m .. of its outputs
+  constexpr int CH = 32 / G, VEC = COLS / G < 4 ? COLS / G : 4, OUT = COLS / (G * VEC);
+  const int j = warp * CH + lane / G, l = lane % G, r = rows.x + j;
+  const bool node = j < n;
+  const size_t dim = (size_t)3 * a.H * 128;
+  uint2 q_raw[CH], k_raw[CH];
+  float4 d[CH];
+  float kv[OUT][VEC], o[OUT][VEC], be = 0.f;               // v - k^T S - sum A u;  q^T S + sum B u
+#pragma unroll
+  for (int m = 0; m < CH; m++) {
+    q_raw[m] = k_raw[m] = make_uint2(0u, 0u);
+    d[m] = make_float4(0.f, 0.f, 0.f, 0.f);
+  }
+#pragma unroll
+  for (int m = 0; m < OUT; m++)
+#pragma unroll
+    for (int e = 0; e < VEC; e++) kv[m][e] = 0.f;
+  if (node) {
+    const __nv_bfloat16* tok = a.qkv + r * dim + head * 128;
+#pragma unroll
+    for (int m = 0; m < CH; m++) {
+      const int c = 4 * l + 4 * G * m;
+      q_raw[m] = *reinterpret_cast<const uint2*>(tok + c);
+      k_raw[m] = *reinterpret_cast<const uint2*>(tok + a.H * 128 + c);
+      d[m] = *reinterpret_cast<const float4*>(a.g + ((size_t)r * a.H + head) * 128 + c);
+    }
+#pragma unroll
+    for (int m = 0; m < OUT; m++) {
+      const __nv_bfloat16* val = tok + 2 * a.H * 128 + v0 + VEC * (l + G * m);
+      if constexpr (VEC == 4) {
+        const float4 x = load4(val);
+        kv[m][0] = x.x; kv[m][1] = x.y; kv[m][2] = x.z; kv[m][3] = x.w;
+      } else if constexpr (VEC == 2) {
+        const uint32_t x = *reinterpret_cast<const uint32_t*>(val);
+        kv[m][0] = bf16lo(x); kv[m][1] = bf16hi(x);
+      } else {
+        kv[m][0] = __bfloat162float(*val);
+      }
+    }
+    be = kt_beta<GATED>(a, r, head);
+  }
   TreePaths paths;
   paths.load(a.tree, rows);
-  const size_t dim = (size_t)3 * a.H * 128;
-  float4 q[NS], k[NS], d[NS];
-  KtVec<VEC> kv[NS], o[NS];                                // v - k^T S - sum A u;  q^T S + sum B u
-  float be[NS];
-#pragma unroll
-  for (int t = 0; t < NS; t++) {
-    const int j = warp + t * KT_WARPS;
-    if (j >= n) continue;
-    const int r = rows.x + j;
-    const __nv_bfloat16* tok = a.qkv + r * dim + head * 128;
-    q[t] = load4(tok + 4 * lane);
-    k[t] = load4(tok + a.H * 128 + 4 * lane);
-    d[t] = *reinterpret_cast<const float4*>(a.g + ((size_t)r * a.H + head) * 128 + 4 * lane);
-    const __nv_bfloat16* val = tok + 2 * a.H * 128 + v0 + VEC * lane;
-    if constexpr (VEC == 4) {
-      const float4 x = load4(val);
-      kv[t].v[0] = x.x; kv[t].v[1] = x.y; kv[t].v[2] = x.z; kv[t].v[3] = x.w;
-    } else if constexpr (VEC == 2) {
-      const uint32_t x = *reinterpret_cast<const uint32_t*>(val);
-      kv[t].v[0] = bf16lo(x); kv[t].v[1] = bf16hi(x);
-    } else {
-      kv[t].v[0] = __bfloat162float(*val);
-    }
-    be[t] = kt_beta<GATED>(a, r, head);
-  }
-  const float rate = GATED ? __expf(a.a_log[head]) : 0.f;
-  const float4 bias = GATED ? *reinterpret_cast<const float4*>(a.dt_bias + head * 128 + 4 * lane) : make_float4(0.f, 0.f, 0.f, 0.f);
-  if (warp == KT_WARPS - 1) {                              // first pair of every node: nodes lane and lane + 32, sums of the depths before
-    const int depth[2] = {__popcll(paths.lo) - 1, __popcll(paths.hi) - 1};
+  if (warp == KT_WARPS - 1) {                              // nodes lane and lane + 32: sums of the fours of ancestors before
+    const int depth[2] = {(__popcll(paths.lo) + 2) / 4, (__popcll(paths.hi) + 2) / 4};
     int sum[2] = {depth[0], depth[1]};
 #pragma unroll
     for (int x = 1; x < 32; x <<= 1) {
@@ -240,16 +259,34 @@ __global__ __launch_bounds__(KT_THREADS, NS == 1 ? 2 : 1) void kda_tree_kernel(c
     ms.first[lane] = sum[0] - depth[0];
     ms.first[lane + 32] = low + sum[1] - depth[1];
   }
+  uint64_t above = paths.of(j & 63);
+  above &= ~(1ull << (j & 63));
+  const int depth = node ? __popcll(above) : -1;
+  // rows in pairs of channels, for packed products
+  uint64_t q[CH][2], k[CH][2], e[CH][2];
+  {
+    float qs = 0.f, ks = 0.f;
 #pragma unroll
-  for (int t = 0; t < NS; t++) {
-    const int j = warp + t * KT_WARPS;
-    if (j >= n) continue;
-    const float qn = rsqrtf(warp_sum(dot4(q[t], q[t])) + 1e-6f), kn = rsqrtf(warp_sum(dot4(k[t], k[t])) + 1e-6f);
-    q[t] = make_float4(q[t].x * qn, q[t].y * qn, q[t].z * qn, q[t].w * qn);
-    k[t] = make_float4(k[t].x * kn, k[t].y * kn, k[t].z * kn, k[t].w * kn);
-    d[t] = kt_decay<GATED>(a, d[t], bias, rate);
-    *reinterpret_cast<float4*>(K + j * 128 + 4 * lane) = k[t];
-    *reinterpret_cast<float4*>(Dc + j * 128 + 4 * lane) = d[t];
+    for (int m = 0; m < CH; m++) {
+      const float4 qf = cvt4(q_raw[m]), kf = cvt4(k_raw[m]);
+      qs += dot4(qf, qf);
+      ks += dot4(kf, kf);
+    }
+    const float qn = rsqrtf(kt_sum<G>(qs) + 1e-6f), kn = rsqrtf(kt_sum<G>(ks) + 1e-6f);
+    const float rate = GATED ? __expf(a.a_log[head]) : 0.f;
+#pragma unroll
+    for (int m = 0; m < CH; m++) {
+      const int c = 4 * l + 4 * G * m;
+      const float4 qf = cvt4(q_raw[m]), kf = cvt4(k_raw[m]);
+      q[m][0] = pack2(qf.x * qn, qf.y * qn); q[m][1] = pack2(qf.z * qn, qf.w * qn);
+      k[m][0] = pack2(kf.x * kn, kf.y * kn); k[m][1] = pack2(kf.z * kn, kf.w * kn);
+      d[m] = kt_decay<GATED>(a, d[m], GATED ? *reinterpret_cast<const float4*>(a.dt_bias + head * 128 + c) : d[m], rate);
+      e[m][0] = pack2(d[m].x, d[m].y); e[m][1] = pack2(d[m].z, d[m].w);
+      if (node) {
+        *reinterpret_cast<ulonglong2*>(K + j * 128 + c) = make_ulonglong2(k[m][0], k[m][1]);
+        *reinterpret_cast<ulonglong2*>(Dc + j * 128 + c) = make_ulonglong2(e[m][0], e[m][1]);
+      }
+    }
   }
   // the state as two bf16 operands: rows of 64 columns, the product's K along the rows' number
 #pragma unroll
@@ -263,75 +300,63 @@ __global__ __launch_bounds__(KT_THREADS, NS == 1 ? 2 : 1) void kda_tree_kernel(c
     *reinterpret_cast<uint2*>(smem + F::S + F::S_BYTES + off) = lo;
   }
   __syncthreads();
-  // ---- tokens with each other, up every node's path ----
-  float self[NS];
-  int depth[NS], first[NS];
+  // ---- tokens with each other, up every node's path, the nearest ancestor first ----
+  auto sum2 = [](uint64_t x) -> float {
+    float x0, x1;
+    unpack2(x, x0, x1);
+    return x0 + x1;
+  };
+  float self;
+  {
+    uint64_t x = 0;
 #pragma unroll
-  for (int t = 0; t < NS; t++) {
-    const int j = warp + t * KT_WARPS;
-    depth[t] = -1;
-    if (j >= n) continue;
-    self[t] = warp_sum(dot4(q[t], k[t]));
-    uint64_t above = paths.of(j) & ~(1ull << j);
-    depth[t] = __popcll(above);
-    first[t] = ms.first[j];
-    float4 e = d[t];
-    // four ancestors a turn, the nearest first
-    for (int at = first[t] + depth[t]; above; at -= 4) {
-      int i[4];
-      float4 x[4], y[4];
+    for (int m = 0; m < CH; m++) x = fma2(q[m][1], k[m][1], fma2(q[m][0], k[m][0], x));
+    self = kt_sum<G>(sum2(x));
+  }
+  const int first = node ? 4 * ms.first[j] : 0;
+  const int steps = __reduce_max_sync(0xffffffffu, depth);
+  for (int t = 0; t < steps; t++) {
+    const int at = depth - 1 - t;                          // (negative: a node of fewer ancestors than its neighbours in the warp)
+    const int i = at >= 0 ? 63 - __clzll((long long)above) : 0;
+    uint64_t ab = 0, bb = 0;
+    if (at >= 0) {
+      above &= ~(1ull << i);
 #pragma unroll
-      for (int u = 0; u < 4; u++) {
-        i[u] = above ? 63 - __clzll((long long)above) : -1;
-        if (i[u] < 0) continue;
-        above &= ~(1ull << i[u]);
-        x[u] = *reinterpret_cast<const float4*>(K + i[u] * 128 + 4 * lane);
-        y[u] = *reinterpret_cast<const float4*>(Dc + i[u] * 128 + 4 * lane);
-      }
-      float v[8];
-#pragma unroll
-      for (int u = 0; u < 4; u++) {
-        v[u] = v[4 + u] = 0.f;
-        if (i[u] < 0) continue;
-        x[u] = mul4(x[u], e);
-        v[u] = dot4(k[t], x[u]);
-        v[4 + u] = dot4(q[t], x[u]);
-        e = mul4(e, y[u]);
-      }
-      // the eight sums over the warp, one in every four lanes: halves of the list go to halves of the warp
-#pragma unroll
-      for (int half = 4, m = 16; half >= 1; half >>= 1, m >>= 1) {
-#pragma unroll
-        for (int u = 0; u < half; u++) {
-          const float mine = lane & m ? v[half + u] : v[u], others = lane & m ? v[u] : v[half + u];
-          v[u] = mine + __shfl_xor_sync(0xffffffffu, others, m);
-        }
-      }
-      v[0] += __shfl_xor_sync(0xffffffffu, v[0], 2);
-      v[0] += __shfl_xor_sync(0xffffffffu, v[0], 1);
-      const int u = lane >> 2 & 3, to = at - 1 - u;        // lanes 0-15: A, 16-31: B
-      const int who = u == 0 ? i[0] : u == 1 ? i[1] : u == 2 ? i[2] : i[3];
-      if ((lane & 3) == 0 && who >= 0) {
-        (lane < 16 ? A : B)[to] = v[0];
-        if (lane < 16) anc[to] = (uint8_t)who;
+      for (int m = 0; m < CH; m++) {
+        const int c = i * 128 + 4 * l + 4 * G * m;
+        const ulonglong2 x = *reinterpret_cast<const ulonglong2*>(K + c), y = *reinterpret_cast<const ulonglong2*>(Dc + c);
+        const uint64_t x0 = mul2(x.x, e[m][0]), x1 = mul2(x.y, e[m][1]);
+        ab = fma2(k[m][1], x1, fma2(k[m][0], x0, ab));
+        bb = fma2(q[m][1], x1, fma2(q[m][0], x0, bb));
+        e[m][0] = mul2(e[m][0], y.x);
+        e[m][1] = mul2(e[m][1], y.y);
       }
     }
-    k[t] = mul4(k[t], e);
-    q[t] = mul4(q[t], e);
+    // two sums at once: half of the node's lanes take the one, half the other
+    const float va = sum2(ab), vb = sum2(bb);
+    const bool second = l >= G / 2;
+    float v = (second ? vb : va) + __shfl_xor_sync(0xffffffffu, second ? va : vb, G / 2);
+#pragma unroll
+    for (int m = G / 4; m > 0; m >>= 1) v += __shfl_xor_sync(0xffffffffu, v, m);
+    if (at >= 0 && l % (G / 2) == 0) {
+      (second ? B : A)[first + at] = v;
+      if (!second) anc[first + at] = (uint8_t)i;
+    }
   }
   __syncthreads();                                         // k and decays have been read
+  if (node) {
 #pragma unroll
-  for (int t = 0; t < NS; t++) {
-    const int j = warp + t * KT_WARPS;
-    if (j >= n) continue;
-    const uint32_t off = (lane >> 4) * F::A_BLOCK + j * 128 + (((lane >> 1 & 7) ^ (j & 7)) << 4) + (lane & 1) * 8;
-    uint2 hi, lo;
-    kt_split(k[t], hi, lo);
-    *reinterpret_cast<uint2*>(smem + F::A + off) = hi;
-    *reinterpret_cast<uint2*>(smem + F::A_LO + off) = lo;
-    kt_split(q[t], hi, lo);
-    *reinterpret_cast<uint2*>(smem + F::A + off + F::M / 2 * 128) = hi;
-    *reinterpret_cast<uint2*>(smem + F::A_LO + off + F::M / 2 * 128) = lo;
+    for (int m = 0; m < CH; m++) {
+      const int c = 4 * l + 4 * G * m;
+      const uint32_t off = (c >> 6) * F::A_BLOCK + j * 128 + (((c >> 3 & 7) ^ (j & 7)) << 4) + (c & 4) * 2;
+      uint2 hi, lo;
+      kt_split(mul2(k[m][0], e[m][0]), mul2(k[m][1], e[m][1]), hi, lo);
+      *reinterpret_cast<uint2*>(smem + F::A + off) = hi;
+      *reinterpret_cast<uint2*>(smem + F::A_LO + off) = lo;
+      kt_split(mul2(q[m][0], e[m][0]), mul2(q[m][1], e[m][1]), hi, lo);
+      *reinterpret_cast<uint2*>(smem + F::A + off + F::M / 2 * 128) = hi;
+      *reinterpret_cast<uint2*>(smem + F::A_LO + off + F::M / 2 * 128) = lo;
+    }
   }
   tc::fence_async_smem();
   tc::fence_before_sync();
@@ -373,59 +398,66 @@ __global__ __launch_bounds__(KT_THREADS, NS == 1 ? 2 : 1) void kda_tree_kernel(c
 #pragma unroll
     for (int c = 0; c < HELD / 4; c += 4) *reinterpret_cast<uint4*>(R + row * F::ROW + col + c) = make_uint4(x[c], x[c + 1], x[c + 2], x[c + 3]);
     __syncthreads();
+    if (node) {
 #pragma unroll
-    for (int t = 0; t < NS; t++) {
-      const int j = warp + t * KT_WARPS;
-      if (j >= n) continue;
-      KtVec<VEC> y;
-      y.load(R + j * F::ROW + VEC * lane);
-      kv[t].add(-1.f, y);
-      o[t].load(R + (F::M / 2 + j) * F::ROW + VEC * lane);
+      for (int m = 0; m < OUT; m++) {
+        float y[VEC];
+        kt_load<VEC>(R + j * F::ROW + VEC * (l + G * m), y);
+#pragma unroll
+        for (int u = 0; u < VEC; u++) kv[m][u] -= y[u];
+        kt_load<VEC>(R + (F::M / 2 + j) * F::ROW + VEC * (l + G * m), o[m]);
+      }
     }
   }
   // ---- level by level ----
   for (int level = 0;; level++) {
-    bool more = false;
+    int who = 0;
+    float fa = 0.f, fb = 0.f;
+    if (depth == level) {
 #pragma unroll
-    for (int t = 0; t < NS; t++) {
-      more |= depth[t] > level;
-      if (depth[t] != level) continue;
-      const int j = warp + t * KT_WARPS;
-      KtVec<VEC> u;
+      for (int m = 0; m < OUT; m++) {
 #pragma unroll
-      for (int e = 0; e < VEC; e++) u.v[e] = kv[t].v[e] * be[t];
-      u.store(U + j * COLS + VEC * lane);
-      o[t].add(self[t], u);
+        for (int u = 0; u < VEC; u++) {
+          kv[m][u] *= be;
+          o[m][u] = fmaf(self, kv[m][u], o[m][u]);
+        }
+        kt_store<VEC>(U + j * COLS + VEC * (l + G * m), kv[m]);
+      }
+    } else if (depth > level) {                            // the node's ancestor of this depth
+      who = anc[first + level];
+      fa = A[first + level];
+      fb = B[first + level];
     }
-    if (!__syncthreads_or(more)) break;
+    if (!__syncthreads_or(depth > level)) break;
+    if (depth > level) {
 #pragma unroll
-    for (int t = 0; t < NS; t++) {
-      if (depth[t] <= level) continue;
-      const int at = first[t] + level;
-      KtVec<VEC> u;
-      u.load(U + anc[at] * COLS + VEC * lane);
-      kv[t].add(-A[at], u);
-      o[t].add(B[at], u);
+      for (int m = 0; m < OUT; m++) {
+        float x[VEC];
+        kt_load<VEC>(U + who * COLS + VEC * (l + G * m), x);
+#pragma unroll
+        for (int u = 0; u < VEC; u++) {
+          kv[m][u] = fmaf(-fa, x[u], kv[m][u]);
+          o[m][u] = fmaf(fb, x[u], o[m][u]);
+        }
+      }
     }
   }
   const float scale = rsqrtf(128.f);
-  if (!*abort_flag) {
+  if (node && !*abort_flag) {
 #pragma unroll
-    for (int t = 0; t < NS; t++) {
-      const int j = warp + t * KT_WARPS;
-      if (j >= n) continue;
-      const size_t at = ((size_t)(rows.x + j) * a.H + head) * 128 + v0 + VEC * lane;
+    for (int m = 0; m < OUT; m++) {
+      const size_t at = ((size_t)r * a.H + head) * 128 + v0 + VEC * (l + G * m);
       uint16_t h[VEC];
 #pragma unroll
-      for (int e = 0; e < VEC; e++) {
-        o[t].v[e] *= scale;
-        h[e] = __bfloat16_as_ushort(__float2bfloat16_rz(o[t].v[e]));
+      for (int u = 0; u < VEC; u++) {
+        o[m][u] *= scale;
+        h[u] = __bfloat16_as_ushort(__float2bfloat16_rz(o[m][u]));
       }
       uint16_t* out = reinterpret_cast<uint16_t*>(a.out) + at;
       if constexpr (VEC == 4) *reinterpret_cast<uint2*>(out) = make_uint2(h[0] | (uint32_t)h[1] << 16, h[2] | (uint32_t)h[3] << 16);
       else if constexpr (VEC == 2) *reinterpret_cast<uint32_t*>(out) = h[0] | (uint32_t)h[1] << 16;
       else *out = h[0];
-      if (a.out_f32) o[t].store(a.out_f32 + at);
+      if (a.out_f32) kt_store<VEC>(a.out_f32 + at, o[m]);
     }
   }
   __syncthreads();
@@ -433,22 +465,22 @@ __global__ __launch_bounds__(KT_THREADS, NS == 1 ? 2 : 1) void kda_tree_kernel(c
   if (tid == 0 && ms.abort_flag && status) atomicExch(status, HK_ERR_TIMEOUT);
 }
 
-template <bool GATED, int COLS, int NS>
+template <bool GATED, int COLS, int G>
 static int kt_launch(const KdaTreeArgs& a, cudaStream_t s) {
   static bool attr_set[64] = {false};
   const int dev = device_index();
   if (!attr_set[dev]) {
-    if (cudaFuncSetAttribute(kda_tree_kernel<GATED, COLS, NS>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kt_smem<COLS, NS>(16 * NS)) != cudaSuccess) return HK_ERR_CUDA;
+    if (cudaFuncSetAttribute(kda_tree_kernel<GATED, COLS, G>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kt_smem<COLS, G>(512 / G)) != cudaSuccess) return HK_ERR_CUDA;
     attr_set[dev] = true;
   }
-  return pdl_launch(kda_tree_kernel<GATED, COLS, NS>, dim3((unsigned)(a.H * (128 / COLS)), (unsigned)a.tree.n_seqs), dim3(KT_THREADS), kt_smem<COLS, NS>(a.most), s, a,
+  return pdl_launch(kda_tree_kernel<GATED, COLS, G>, dim3((unsigned)(a.H * (128 / COLS)), (unsigned)a.tree.n_seqs), dim3(KT_THREADS), kt_smem<COLS, G>(a.most), s, a,
                     device_status_ptr()) == cudaSuccess
              ? HK_OK
              : HK_ERR_CUDA;
 }
 template <bool GATED, int COLS>
 static int kt_nodes(const KdaTreeArgs& a, cudaStream_t s) {
-  return a.most <= 16 ? kt_launch<GATED, COLS, 1>(a, s) : a.most <= 32 ? kt_launch<GATED, COLS, 2>(a, s) : kt_launch<GATED, COLS, 4>(a, s);
+  return a.most <= 16 ? kt_launch<GATED, COLS, 32>(a, s) : a.most <= 32 ? kt_launch<GATED, COLS, 16>(a, s) : kt_launch<GATED, COLS, 8>(a, s);
 }
 template <bool GATED>
 static int kt_run(const KdaTreeArgs& a, cudaStream_t s) {
