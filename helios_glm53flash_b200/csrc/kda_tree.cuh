@@ -492,97 +492,139 @@ static int kt_run(const KdaTreeArgs& a, cudaStream_t s) {
 }
 
 // ---- the step to an accepted node: the recurrence along its path, in the order of sums that all token-by-token kernels share ----
+// A warp has 16 columns of a head's state in registers, all rows of them: row group lane / 4 (groups w and w + 8 of the shared order), columns 4 (lane % 4).
+// The sums over the groups are the shared order's balanced tree, three exchanges inside the warp, so that a step has no barrier and no other warp's
+// numbers in it.  Tokens are prepared eight at a time by all warps, the first eight under the state's loads.
+// SLICES: CTAs a head, each of 8 / SLICES warps with columns; the others prepare tokens.
+constexpr int KA_BATCH = 8, KA_WARPS = 8;
+struct alignas(16) AcceptToken {
+  float k[128], d[128], v[128];
+  float beta;
+};
 template <int SLICES>
-__global__ __launch_bounds__(KD_THREADS + 32) void kda_tree_accept_kernel(const KdaTreeArgs a) {
-  constexpr int SW = KD_STATE_WARPS / SLICES;              // state warps; three more prepare tokens
+__global__ __launch_bounds__(KA_WARPS * 32, 2) void kda_tree_accept_kernel(const KdaTreeArgs a) {
+  constexpr int SW = KA_WARPS / SLICES;
   const int head = blockIdx.x / SLICES, slice = blockIdx.x % SLICES, s = blockIdx.y, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int rg = SLICES == 1 ? warp : 4 * warp + (lane >> 3), cl = SLICES == 1 ? lane : slice * (32 / SLICES) + (lane & 7);
-  __shared__ __align__(16) DecodeToken tok[2];
-  __shared__ __align__(16) float part[8][128];
+  const int rg = lane >> 2, col = (slice * SW + warp) * 16 + 4 * (lane & 3);
+  __shared__ __align__(16) AcceptToken tok[KA_BATCH];
   __shared__ int list[TREE_NODES];
   pdl_wait();
   const int2 rows = a.tree.rows(s);
   const uint64_t path = tree_path(a.tree, rows, a.leaf[s]);
   const int steps = __popcll(path);
   if (steps == 0) return;
-  if (warp == 0) {                                         // a path's nodes are in ascending order
+  const int slot = a.slots ? a.slots[s] : s;
+  float* sp = a.state + ((size_t)slot * a.H + head) * 128 * 128 + col;
+  ulonglong2 S[16];                                        // two pairs of columns
+  if (warp < SW) {
+#pragma unroll
+    for (int i = 0; i < 16; i++) S[i] = *reinterpret_cast<const ulonglong2*>(sp + state_row(rg, i) * 128);
+  }
+  if (warp == KA_WARPS - 1) {                              // a path's nodes are in ascending order
 #pragma unroll
     for (int h = 0; h < 2; h++) {
       const int j = lane + 32 * h;
       if (path >> j & 1) list[__popcll(path & ((1ull << j) - 1))] = rows.x + j;
     }
   }
-  const int slot = a.slots ? a.slots[s] : s;
-  float* sp = a.state + ((size_t)slot * a.H + head) * 128 * 128 + 4 * cl;
-  float4 S[16];
-  if (warp < SW) {
-#pragma unroll
-    for (int i = 0; i < 16; i++) S[i] = *reinterpret_cast<const float4*>(sp + state_row(rg, i) * 128);
-  }
   __syncthreads();
-  auto prepare = [&](int i) {                              // by the warps behind the state's: k, decay, v and beta
-    const int role = warp - SW, r = list[i];
-    DecodeToken& t = tok[i & 1];
-    const __nv_bfloat16* x = a.qkv + ((size_t)r * 3 + (role == 0 ? 1 : 2)) * a.H * 128 + head * 128 + lane;
-    if (role == 0) {
-      float z[4];
+  for (int i0 = 0; i0 < steps; i0 += KA_BATCH) {
+    const int batch = min(steps - i0, KA_BATCH);
+    if (i0 > 0) __syncthreads();                           // the tokens before have been used
+    for (int t = warp; t < 3 * batch; t += KA_WARPS) {     // k; decay; v and beta
+      const int role = t % 3, r = list[i0 + t / 3];
+      AcceptToken& to = tok[t / 3];
+      const __nv_bfloat16* x = a.qkv + ((size_t)r * 3 + (role == 0 ? 1 : 2)) * a.H * 128 + head * 128 + lane;
+      if (role == 0) {
+        float z[4];
 #pragma unroll
-      for (int u = 0; u < 4; u++) z[u] = __bfloat162float(x[32 * u]);
-      const float f = inv_norm(z);
+        for (int u = 0; u < 4; u++) z[u] = __bfloat162float(x[32 * u]);
+        const float f = inv_norm(z);
 #pragma unroll
-      for (int u = 0; u < 4; u++) t.k[lane + 32 * u] = __fmul_rn(z[u], f);
-    } else if (role == 1) {
-      const float rate = a.a_log ? __expf(a.a_log[head]) : 0.f;
+        for (int u = 0; u < 4; u++) to.k[lane + 32 * u] = __fmul_rn(z[u], f);
+      } else if (role == 1) {
+        const float rate = a.a_log ? __expf(a.a_log[head]) : 0.f;
+#pragma unroll
+        for (int u = 0; u < 4; u++) {
+          const int c = lane + 32 * u;
+          const float g = a.g[((size_t)r * a.H + head) * 128 + c];
+          to.d[c] = __expf(a.a_log ? gate_value(g, a.dt_bias[head * 128 + c], rate, a.lower_bound) : g);
+        }
+      } else {
+#pragma unroll
+        for (int u = 0; u < 4; u++) to.v[lane + 32 * u] = __bfloat162float(x[32 * u]);
+        if (lane == 0) to.beta = a.a_log ? kt_beta<true>(a, r, head) : kt_beta<false>(a, r, head);
+      }
+    }
+    __syncthreads();
+    if (warp >= SW) continue;
+#pragma unroll 1
+    for (int i = 0; i < batch; i++) {
+      const AcceptToken& t = tok[i];
+      ulonglong2 sum[4] = {{0, 0}, {0, 0}, {0, 0}, {0, 0}};   // even and odd rows of the two groups
+      float4 k[4];
+#pragma unroll
+      for (int c = 0; c < 4; c++) {                        // four rows at a time
+        const float4 d4 = *reinterpret_cast<const float4*>(&t.d[state_row(rg, 4 * c)]);
+        k[c] = *reinterpret_cast<const float4*>(&t.k[state_row(rg, 4 * c)]);
+        const float ds[4] = {d4.x, d4.y, d4.z, d4.w}, ks[4] = {k[c].x, k[c].y, k[c].z, k[c].w};
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+          ulonglong2& x = S[4 * c + e];
+          ulonglong2& y = sum[2 * (c >> 1) + (e & 1)];
+          const uint64_t dd = pack2(ds[e], ds[e]), kk = pack2(ks[e], ks[e]);
+          x.x = mul2(x.x, dd);
+          x.y = mul2(x.y, dd);
+          y.x = fma2(kk, x.x, y.x);
+          y.y = fma2(kk, x.y, y.y);
+        }
+      }
+      float kv[4], p[4][4];
 #pragma unroll
       for (int u = 0; u < 4; u++) {
-        const int c = lane + 32 * u;
-        const float g = a.g[((size_t)r * a.H + head) * 128 + c];
-        t.d[c] = __expf(a.a_log ? gate_value(g, a.dt_bias[head * 128 + c], rate, a.lower_bound) : g);
+        unpack2(sum[u].x, p[u][0], p[u][1]);
+        unpack2(sum[u].y, p[u][2], p[u][3]);
       }
-    } else {
 #pragma unroll
-      for (int u = 0; u < 4; u++) t.v[lane + 32 * u] = __bfloat162float(x[32 * u]);
-      if (lane == 0) t.beta = a.a_log ? kt_beta<true>(a, r, head) : kt_beta<false>(a, r, head);
-    }
-  };
-  if (warp >= SW && warp < SW + 3) prepare(0);
-  __syncthreads();
-  for (int i = 0; i < steps; i++) {
-    const DecodeToken& t = tok[i & 1];
-    if (warp < SW) state_kv(S, t, rg, cl, part);
-    __syncthreads();
-    if (warp < SW) {
-      const float4 kv = part_tree(part, cl);
-      const float4 v = *reinterpret_cast<const float4*>(&t.v[4 * cl]);
+      for (int u = 0; u < 4; u++) kv[u] = __fadd_rn(__fadd_rn(p[0][u], p[1][u]), __fadd_rn(p[2][u], p[3][u]));
+#pragma unroll
+      for (int m = 4; m <= 16; m <<= 1)
+#pragma unroll
+        for (int u = 0; u < 4; u++) kv[u] = __fadd_rn(kv[u], __shfl_xor_sync(0xffffffffu, kv[u], m));
+      const float4 v = *reinterpret_cast<const float4*>(&t.v[col]);
       const float be = t.beta;
-      const float4 un = make_float4(__fmul_rn(__fsub_rn(v.x, kv.x), be), __fmul_rn(__fsub_rn(v.y, kv.y), be), __fmul_rn(__fsub_rn(v.z, kv.z), be),
-                                    __fmul_rn(__fsub_rn(v.w, kv.w), be));
+      const uint64_t u0 = pack2(__fmul_rn(__fsub_rn(v.x, kv[0]), be), __fmul_rn(__fsub_rn(v.y, kv[1]), be));
+      const uint64_t u1 = pack2(__fmul_rn(__fsub_rn(v.z, kv[2]), be), __fmul_rn(__fsub_rn(v.w, kv[3]), be));
 #pragma unroll
-      for (int r = 0; r < 16; r++) {
-        const float k = t.k[state_row(rg, r)];
-        S[r].x = fmaf(k, un.x, S[r].x);
-        S[r].y = fmaf(k, un.y, S[r].y);
-        S[r].z = fmaf(k, un.z, S[r].z);
-        S[r].w = fmaf(k, un.w, S[r].w);
+      for (int c = 0; c < 4; c++) {
+        const float ks[4] = {k[c].x, k[c].y, k[c].z, k[c].w};
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+          const uint64_t kk = pack2(ks[e], ks[e]);
+          S[4 * c + e].x = fma2(kk, u0, S[4 * c + e].x);
+          S[4 * c + e].y = fma2(kk, u1, S[4 * c + e].y);
+        }
       }
-    } else if (warp < SW + 3 && i + 1 < steps) {
-      prepare(i + 1);
     }
-    __syncthreads();
   }
   if (warp < SW) {
 #pragma unroll
-    for (int i = 0; i < 16; i++) *reinterpret_cast<float4*>(sp + state_row(rg, i) * 128) = S[i];
+    for (int i = 0; i < 16; i++) *reinterpret_cast<ulonglong2*>(sp + state_row(rg, i) * 128) = S[i];
   }
   // the head's windows: their last values, then the path's
   if (slice != 0 || !a.conv_state) return;
-  for (int i = threadIdx.x; i < 3 * 128; i += blockDim.x) {
+  for (int i = threadIdx.x; i < 3 * 128; i += KA_WARPS * 32) {
     const int ch = ((i >> 7) * a.H + head) * 128 + (i & 127);
     uint2* at = reinterpret_cast<uint2*>(a.conv_state + ((size_t)slot * 3 * a.H * 128 + ch) * 4);
     uint2 w = *at;
     for (int j = max(0, steps - 4); j < steps; j++) w = conv4_rolled(w, __float2bfloat16_rn(a.x[(size_t)list[j] * 3 * a.H * 128 + ch]));
     *at = w;
   }
+}
+
+template <int SLICES>
+static cudaError_t ka_launch(const KdaTreeArgs& a, cudaStream_t s) {
+  return pdl_launch(kda_tree_accept_kernel<SLICES>, dim3((unsigned)(a.H * SLICES), (unsigned)a.tree.n_seqs), dim3(KA_WARPS * 32), 0, s, a);
 }
 
 static bool kda_tree_args(KdaTreeArgs* a, const void* mixed_qkv, const float* g, const void* beta, const float* dt_bias, const float* a_log,
@@ -641,9 +683,7 @@ HK_API int hk_kda_tree_accept(const float* x32, void* conv_state, const void* mi
   a.x = x32;
   a.conv_state = (__nv_bfloat16*)conv_state;
   a.leaf = leaf;
-  const bool few = 4 * (int64_t)num_heads * n_seqs <= 2 * sm_count();
-  const dim3 grid((unsigned)(num_heads * (few ? 4 : 1)), (unsigned)n_seqs);
-  const cudaError_t e = few ? pdl_launch(kda_tree_accept_kernel<4>, grid, dim3((KD_STATE_WARPS / 4 + 3) * 32), 0, as_stream(stream), a)
-                            : pdl_launch(kda_tree_accept_kernel<1>, grid, dim3(KD_THREADS), 0, as_stream(stream), a);
+  // up to half a head an SM by two CTAs a head: a path of five of 64 heads 6.2 / 5.4 us (one / two), of 128 6.7 / 7.0; four 32 heads 6.2 / 6.0 / 5.8
+  const cudaError_t e = 2 * (int64_t)num_heads * n_seqs <= sm_count() ? ka_launch<2>(a, as_stream(stream)) : ka_launch<1>(a, as_stream(stream));
   return e == cudaSuccess ? HK_OK : HK_ERR_CUDA;
 }
