@@ -95,7 +95,7 @@ SIGNATURES = {
     "hk_mla8_dense_workspace_bytes": (_sz, [_i, _i, _i, _i, _i, _i, _i]),
     "hk_mla8_dense": (_i, [_vp, _vp, _vp, _i, _i64, _i, _vp, _i, _i, _vp, _vp, _i, _i, _i, _vp, _i, _i, _f, _i, _i, _vp, _sz, _vp]),
     "hk_mla8_sparse": (_i, [_vp, _vp, _vp, _i, _i64, _i, _vp, _i, _i, _vp, _vp, _i, _vp, _i, _i, _f, _i, _vp, _sz, _vp]),
-    "hk_mla_tree_workspace_bytes": (_sz, [_i, _i, _i]),
+    "hk_mla_tree_workspace_bytes": (_sz, [_i, _i, _i, _i]),
     "hk_mla_tree": (_i, [_vp, _vp, _i64, _vp, _vp, _i, _vp, _vp, _vp, _i, _vp, _i, _i, _f, _i, _vp, _sz, _vp]),
     "hk_mla8_tree_workspace_bytes": (_sz, [_i, _i, _i]),
     "hk_mla8_tree": (_i, [_vp, _vp, _vp, _i, _i64, _i, _vp, _i, _vp, _i, _vp, _vp, _vp, _i, _vp, _i, _i, _f, _i, _vp, _sz, _vp]),
@@ -563,9 +563,9 @@ def mla8_sparse_decode(q_lat, ckv8, scales, raw_idx, kidx, lat_out, m, stream=No
 # ---- trees of drafted tokens: m nodes of n_seqs sequences' trees, rows tree_start[s] .. tree_start[s + 1] - 1 (device int32 [n_seqs + 1]; None: m / n_seqs
 # each); parent: device int32 [m], the number within the tree of the node that a row hangs on, -1: the sequence's last token.  leaf: device int32
 # [n_seqs], the accepted node of each tree, -1: none.  Tensors of another type, layout, device or size than the call's raise ValueError ----
-def mla_tree_workspace_bytes(m, n_heads, n_keys):
+def mla_tree_workspace_bytes(m, n_heads, n_seqs, n_keys):
     """what mla_tree_decode without n_split needs; n_keys: pos_start, or n_keys_hint where kv_len is given"""
-    return load_library().hk_mla_tree_workspace_bytes(m, n_heads, n_keys)
+    return load_library().hk_mla_tree_workspace_bytes(m, n_heads, n_seqs, n_keys)
 
 
 def mla8_tree_workspace_bytes(m, n_heads, n_keys):
@@ -583,7 +583,7 @@ def mla_tree_decode(q_lat, ckv, tree_kv, parent, lat_out, m, pos_start=0, n_seqs
         pos_start = n_keys_hint or pos_start
     ws = workspace
     if ws is None:
-        need = (_native.hk_mla_tree_workspace_bytes(m, n_heads, pos_start) if n_split <= 0
+        need = (_native.hk_mla_tree_workspace_bytes(m, n_heads, n_seqs, pos_start) if n_split <= 0
                 else _native.hk_mla_partial_bytes(n_split, m * n_heads) if n_split > 1 else 0)
         if need:
             ws = _scratch_like(need, q_lat, stream)

@@ -619,7 +619,7 @@ __global__ __launch_bounds__(F8_THREADS, 1) void mla8_flash_tc_kernel(MlaArgs a,
       }
     }
     asm volatile("bar.sync 4, 384;" ::: "memory");
-    if (!*abort_flag) {
+    if (!*abort_flag && (!TREE || tree.seq >= 0)) {          // (a row of no tree is left as it was)
       uint8_t* dst = final_out ? reinterpret_cast<uint8_t*>(a.out + ((size_t)it.r * a.n_heads + h0) * LATENT)
                                : reinterpret_cast<uint8_t*>(a.part_acc + part_row * LATENT + it.part * n_ch);
       const int team = warp < 4 ? warp : warp - 2;

@@ -30,6 +30,7 @@ struct MlaArgs {
   // trees of drafted tokens: row r is a node of tree.seq_of(r), whose cached keys kv_base and kv_len (then per sequence) say
   TreeArgs tree;
   const __half* tree_kv;    // [m][512] the nodes' own latents
+  bool tree_pairs;          // two nodes to a pair of CTAs
   int keep_nan;             // keys that are not finite make outputs that are NaN (0: zeros where the scores are, as hk_mla_dense's callers know it)
 };
 

@@ -25,6 +25,7 @@ int mla8_read_launch(const MlaPaged& pg, int dtype, int head, int shift, int n, 
 bool mla8_paged(MlaPaged* pg, const void* ckv8, const float* scales, int dtype, int64_t n_blocks, int block, const int* block_table,
                 int table_stride, int n_seqs, const int* row_seq);
 bool mla_flash_cluster_shape(int m, int tiles, int* n_split);
+bool mla_tree_shape(int m, int n_seqs, bool ragged, int n_keys, int* n_split);
 
 static inline size_t align_up(size_t v, size_t a) { return (v + a - 1) / a * a; }
 
@@ -96,6 +97,17 @@ static int combine_cs_launch(const float* pm, const float* pl, const float* pa, 
              : HK_ERR_CUDA;
 }
 
+// the same over nodes of trees of drafted tokens
+static int combine_tree(const MlaArgs& a, int n_split, __half* out, cudaStream_t s) {
+  const int64_t rows = (int64_t)a.m * a.n_heads;
+  const dim3 grid((unsigned)rows, LSE_CSPLIT);
+  const cudaError_t e =
+      n_split <= LSE_FEW_SPLITS && rows >= 256
+          ? pdl_launch(lse_combine_few_tree_kernel, dim3((unsigned)rows), dim3(128), 0, s, a.part_m, a.part_l, a.part_acc, n_split, rows, out, a.tree, a.n_heads)
+          : pdl_launch(lse_combine_cs_tree_kernel<8, 6>, grid, dim3(256), 0, s, a.part_m, a.part_l, a.part_acc, n_split, rows, out, a.tree, a.n_heads);
+  return e == cudaSuccess ? HK_OK : HK_ERR_CUDA;
+}
+
 static int combine(const float* pm, const float* pl, const float* pa, int n_split, int64_t rows,
                    __half* out, cudaStream_t s) {
   if (n_split > LSE_MAX_SPLITS) return HK_ERR_UNSUPPORTED;
@@ -161,6 +173,7 @@ static int attend(MlaArgs a, int n_keys_hint, int n_split, bool choose, void* wo
   if (tc) st = mla_flash_tc_launch(a, s);
   if (st == HK_ERR_UNSUPPORTED) st = launch_simt(a, s);
   if (st != HK_OK) return st;
+  if (n_split > 1 && a.tree_kv) return combine_tree(a, n_split, final_out, s);
   if (n_split > 1) return combine(a.part_m, a.part_l, a.part_acc, n_split, rows, final_out, s);
   return HK_OK;
 }
@@ -208,6 +221,7 @@ static int attend8(MlaArgs a, const MlaPaged& pg, int dtype, int n_keys_hint, in
     st = dtype == HK_I8 ? launch_simt_as<CACHE_I8>(c, pg, s) : launch_simt_as<CACHE_E4M3>(c, pg, s);
   }
   if (st != HK_OK || n_split == 1) return st;
+  if (a.tree_kv) return combine_tree(a, n_split, a.out, s);
   return combine(a.part_m, a.part_l, a.part_acc, n_split, rows, a.out, s);
 }
 
@@ -708,10 +722,29 @@ static bool tree_call(MlaArgs* a, const void* q_lat, const void* tree_kv, const 
 }
 }  // namespace hk
 
-HK_API size_t hk_mla_tree_workspace_bytes(int m, int n_heads, int n_keys) {
-  if (m <= 0 || n_heads < hk::SIMT_HG || n_keys < 0) return 0;
-  const int splits = hk::attend_splits(m, n_heads, hk::tree_keys(true, n_keys), 0);
-  return splits > 1 ? hk_mla_partial_bytes(splits, (int64_t)m * n_heads) : 0;
+namespace hk {
+// splits of a call over the fp16 cache, and whether pairs of CTAs take two nodes each
+static int tree_splits(int m, int n_heads, int n_seqs, bool ragged, int n_keys, bool* pairs) {
+  int n_split;
+  if (n_heads != 64 || force_simt()) {
+    *pairs = false;
+    return simt_auto_splits(m, n_heads, n_keys);
+  }
+  *pairs = mla_tree_shape(m, n_seqs, ragged, n_keys, &n_split);
+  return n_split;
+}
+}  // namespace hk
+
+HK_API size_t hk_mla_tree_workspace_bytes(int m, int n_heads, int n_seqs, int n_keys) {
+  if (m <= 0 || n_heads < hk::SIMT_HG || n_seqs < 1 || n_keys < 0) return 0;
+  bool pairs;
+  int most = 1;
+  for (int k = 0; k < 4; k++) {                            // (whether the trees are ragged and the lengths on the device)
+    if (k < 2 && m % n_seqs != 0) continue;
+    const int splits = hk::tree_splits(m, n_heads, n_seqs, k >= 2, hk::tree_keys(k & 1, n_keys), &pairs);
+    most = most > splits ? most : splits;
+  }
+  return most > 1 ? hk_mla_partial_bytes(most, (int64_t)m * n_heads) : 0;
 }
 
 HK_API size_t hk_mla8_tree_workspace_bytes(int m, int n_heads, int n_keys) {
@@ -732,7 +765,8 @@ HK_API int hk_mla_tree(const void* q_lat, const void* ckv, int64_t ckv_rows, con
   if (n_split > LSE_MAX_SPLITS) return HK_ERR_UNSUPPORTED;
   a.ckv = (const __half*)ckv; a.ckv_rows = ckv_rows;
   a.kv_base = kv_base;
-  return attend(a, tree_keys(kv_len, pos_start), n_split, false, workspace, workspace_bytes, as_stream(stream));
+  if (n_split <= 0) n_split = tree_splits(m, n_heads, n_seqs, tree_start, tree_keys(kv_len, pos_start), &a.tree_pairs);
+  return attend(a, 0, n_split, false, workspace, workspace_bytes, as_stream(stream));
 }
 
 HK_API int hk_mla8_tree(const void* q_lat, const void* ckv8, const float* scales, int dtype, int64_t n_blocks, int block, const int* block_table,

@@ -224,7 +224,8 @@ __device__ __forceinline__ void tma_gather4_rows(uint32_t leader, uint32_t smem_
 // WIN: dense ranges of which a row sees its last keys and its first ones only (a.window, a.sinks).
 // PARTS: CTAs that share a partial's output channels, each with the scores for itself (few splits of few rows: 128 KB of a partial take 3 us).
 // TREE: a row is a node of a tree of drafted tokens (a.tree).  The tree's tile is the last of the row's list: of its 64 slots those on the node's
-// path are gathered out of a.tree_kv (tmap_tree), the others are zeros, whatever lies there.
+// path are gathered out of a.tree_kv (tmap_tree), the others are zeros, whatever lies there.  (As a box whose unseen rows are cleared ahead of P V, as
+// mla_pair_tree_tc_kernel takes it, this tile and a ragged one were no faster here, and the look at the mask cost long rows 3 %.)
 template <bool G4, bool CL, bool WIN, int PARTS, bool TREE>
 __device__ __forceinline__ void ft_body(const MlaArgs& a, int* __restrict__ status, const CUtensorMap& tmap_box, const CUtensorMap& tmap_rows,
                                         const CUtensorMap& tmap_q, const CUtensorMap& tmap_o, const CUtensorMap& tmap_tree) {
@@ -671,7 +672,7 @@ __device__ __forceinline__ void ft_body(const MlaArgs& a, int* __restrict__ stat
           }
           tc::fence_async_smem();
           asm volatile("bar.sync 3, 128;" ::: "memory");
-          if (tid == 0 && ok && !*abort_flag) {
+          if (tid == 0 && ok && !*abort_flag && (!TREE || it.n_tiles > 0)) {   // (tree form: a row of no tree is left as it was)
 #pragma unroll
             for (int hf = 0; hf < 2; hf++)
               asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%1, %2}], [%3];" ::"l"(&tmap_o),
@@ -792,6 +793,33 @@ int mla_flash_tc_auto_splits(int m, int n_keys) {
   return n_split < 1 ? 1 : n_split;
 }
 
+// pairs of nodes that m rows of n_seqs trees make at most (ragged: trees of any sizes)
+static int64_t mla_tree_pairs(int m, int n_seqs, bool ragged) { return ragged ? ((int64_t)m + n_seqs) / 2 : (int64_t)n_seqs * ((m / n_seqs + 1) / 2); }
+// Form and splits of a tree call: a CTA a node or a pair of CTAs for two, each key range in n_split parts.  A model of the time in units of 10 ns, fitted to
+// 13 shapes with 1 to 36 splits (1 x 2 to 64 nodes at 500 to 32,768 keys, 2 to 16 sequences): a tile takes 1.0 us of a single CTA, 0.87 of a pair (48 KB
+// instead of 64 for each, half the reads of the products); a call 7 and 8, with partials and their merge 8 and 9.5 and 0.06 a partial of 64 heads; another
+// wave 1.5.  us, single / pair at the best number of splits: 2 nodes at 5,001 keys 13.5 / 15.7, 8 18.4 / 18.9, 64 at 2,000 37.0 / 34.8, 16 at 32,768 70.8 /
+// 63.6, 64 266 / 235, 6 x 16 at 10,000 118 / 101, 16 x 8 at 8,000 122 / 106.
+bool mla_tree_shape(int m, int n_seqs, bool ragged, int n_keys, int* n_split) {
+  const int64_t tiles = n_keys / FT_KEYS + 2, sms = sm_count();
+  int64_t best = 0;
+  bool pairs = false;
+  *n_split = 1;
+  for (int form = 0; form < 2; form++) {
+    const int64_t units = form ? 2 * mla_tree_pairs(m, n_seqs, ragged) : m;
+    for (int s = 1; s <= 256 && (s == 1 || (2 * s <= tiles + 1 && units * s <= 4 * sms)); s++) {
+      const int64_t waves = (units * s + sms - 1) / sms, per = (tiles + s - 1) / s;
+      const int64_t time = waves * per * (form ? 87 : 100) + (waves - 1) * 150 + (s == 1 ? (form ? 800 : 700) : (form ? 950 : 800) + 6 * units * s);
+      if (best == 0 || time < best) {
+        best = time;
+        pairs = form;
+        *n_split = s;
+      }
+    }
+  }
+  return pairs;
+}
+
 static int ft_prepare() {
   static bool attr_set[64] = {false};
   int dev = 0;
@@ -804,6 +832,7 @@ static int ft_prepare() {
         !whole_sm(mla_flash_tc_kernel<false, false, true>) || !whole_sm(mla_flash_tc_kernel<false, false, true, 2>) ||
         !whole_sm(mla_flash_tc_kernel<false, false, true, 4>) || !whole_sm(mla_flash_tc_kernel<false, true, true>) || !whole_sm(mla_pair_tc_kernel<false>) ||
         !whole_sm(mla_pair_tc_kernel<true>) || !whole_sm(mla_tree_tc_kernel<1>) || !whole_sm(mla_tree_tc_kernel<2>) || !whole_sm(mla_tree_tc_kernel<4>) ||
+        !whole_sm(mla_pair_tree_tc_kernel) ||
         !any_cluster(mla_flash_tc_kernel<false, true, false>) || !any_cluster(mla_flash_tc_kernel<true, true, false>) ||
         !any_cluster(mla_flash_tc_kernel<false, true, true>))
       return HK_ERR_CUDA;
@@ -912,7 +941,9 @@ int mla_flash_tc_launch(const MlaArgs& a, cudaStream_t s, bool clusters) {
   const int seen = a.window > 0 ? min(a.pos_start + a.m / 2, mla_window_keys(0, a.window, a.sinks)) : a.pos_start + a.m / 2;
   const bool pairs = !clusters && !a.raw_idx && !a.tree_kv && !a.kv_len && !a.kv_base && a.out && a.n_split == 1 && a.m >= 2 &&
                      seen >= (a.window > 0 ? FT_WINDOW_PAIR_KEYS : FT_PAIR_KEYS);
-  if (!box_map(&qmap, a.q_lat, q_rows) || (!a.raw_idx && !pairs && !box_map(&box, a.ckv, extent))) return HK_ERR_UNSUPPORTED;
+  // Nodes of trees by twos: see mla_tree_shape.
+  const bool tree_pairs = a.tree_kv && a.tree_pairs;
+  if (!box_map(&qmap, a.q_lat, q_rows) || (!a.raw_idx && !pairs && !tree_pairs && !box_map(&box, a.ckv, extent))) return HK_ERR_UNSUPPORTED;
   if (a.out) {
     const cuuint64_t dims[2] = {LATENT, q_rows};
     const cuuint64_t strides[1] = {LATENT * 2};
@@ -920,6 +951,16 @@ int mla_flash_tc_launch(const MlaArgs& a, cudaStream_t s, bool clusters) {
     if (encode(&omap, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, a.out, dims, strides, b, ones, CU_TENSOR_MAP_INTERLEAVE_NONE,
                CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
       return HK_ERR_UNSUPPORTED;
+  }
+  if (tree_pairs) {
+    alignas(64) CUtensorMap vbox, tree_k, tree_v;
+    if (!box_map(&box, a.ckv, extent, 32, 8) || !box_map(&vbox, a.ckv, extent, 32, 4) || !box_map(&tree_k, a.tree_kv, a.m, 32, 8) ||
+        !box_map(&tree_v, a.tree_kv, a.m, 32, 4))
+      return HK_ERR_UNSUPPORTED;
+    const int64_t n_pairs = mla_tree_pairs(a.m, a.tree.n_seqs, a.tree.start != nullptr);
+    const cudaError_t e = pdl_launch_cluster(2, mla_pair_tree_tc_kernel, dim3((unsigned)(2 * n_pairs * a.n_split)), dim3(PT_THREADS), FS_SMEM, s, a, device_status_ptr(), box, vbox,
+                                             rows, qmap, omap, tree_k, tree_v);
+    return e == cudaSuccess && cudaPeekAtLastError() == cudaSuccess ? HK_OK : HK_ERR_CUDA;
   }
   if (pairs) {
     alignas(64) CUtensorMap vbox;

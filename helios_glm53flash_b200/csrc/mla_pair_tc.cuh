@@ -19,6 +19,10 @@
 // them, the earlier row's alone, is key 16 of the last tile, whose product leaves the later row's accumulator alone.  Tiles at the edge of
 // what is seen arrive whole, and the softmax warps clear the other keys' rows of V (by four rows at a time, as a ragged tile comes, the three
 // or four such tiles of a pair cost 2,048 rows under a window of 1,023 392 us where they now take 343).
+// TREE: the rows are neighbouring nodes of a tree of drafted tokens, or one node alone.  They share the sequence's cached keys; the keys of a node's own
+// path are a tile of its own, whose P V leaves the other node's accumulator alone.  These tiles, and a ragged last one where the cache's extent is told,
+// arrive whole and have the rows of V that are not seen cleared, as above (by four rows at a time they took 10 us).  Key ranges may be split: partials
+// leave through the idle ring.
 #pragma once
 
 namespace hk {
@@ -38,8 +42,36 @@ struct PtMisc {
   float l[128];
   uint32_t tmem;
   int abort_flag;
+  MlaTree tree[2];                                // the nodes; the second may be the first again
 };
 static_assert(sizeof(PtMisc) <= 2048, "misc area");
+
+// Nodes of pair `pair` of a tree call: pairs of sequence after sequence; row < 0: no such pair.  Executed by a whole warp.
+struct PtPair {
+  int row;
+  bool lone;
+};
+__device__ __forceinline__ PtPair pt_pair(const TreeArgs& tree, int pair) {
+  const int lane = threadIdx.x & 31;
+  int before = 0;
+  for (int s0 = 0; s0 < tree.n_seqs; s0 += 32) {
+    const int2 rows = s0 + lane < tree.n_seqs ? tree.rows(s0 + lane) : make_int2(0, 0);
+    const int mine = (rows.y + 1) / 2;
+    int sum = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int x = __shfl_up_sync(0xffffffffu, sum, o);
+      if (lane >= o) sum += x;
+    }
+    const uint32_t who = __ballot_sync(0xffffffffu, pair < before + sum && pair >= before + sum - mine);
+    if (who) {
+      const int at = __ffs(who) - 1, k = pair - __shfl_sync(0xffffffffu, before + sum - mine, at);
+      return {__shfl_sync(0xffffffffu, rows.x, at) + 2 * k, 2 * k + 1 == __shfl_sync(0xffffffffu, rows.y, at)};
+    }
+    before += __shfl_sync(0xffffffffu, sum, 31);
+  }
+  return {-1, true};
+}
 
 __device__ __forceinline__ void pt_tma_box(void* smem_dst, const CUtensorMap* tmap, int row, int blk, uint64_t* bar) {
   asm volatile(
@@ -122,10 +154,9 @@ __device__ __forceinline__ bool pt_wait(uint64_t* bar, uint32_t parity, volatile
 
 // grid = 2 CTAs a pair of rows, cluster of 2.  tmap_k / tmap_v: boxes of 32 keys x 512 and x 256 channels; tmap_rows, tmap_q, tmap_o as in
 // mla_flash_tc_kernel.
-template <bool WIN>
-__global__ __launch_bounds__(PT_THREADS, 1) void mla_pair_tc_kernel(
-    MlaArgs a, int* __restrict__ status, const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ CUtensorMap tmap_v,
-    const __grid_constant__ CUtensorMap tmap_rows, const __grid_constant__ CUtensorMap tmap_q, const __grid_constant__ CUtensorMap tmap_o) {
+template <bool WIN, bool TREE>
+__device__ __forceinline__ void pt_body(const MlaArgs& a, int* __restrict__ status, const CUtensorMap& tmap_k, const CUtensorMap& tmap_v, const CUtensorMap& tmap_rows,
+                                        const CUtensorMap& tmap_q, const CUtensorMap& tmap_o, const CUtensorMap& tmap_tree_k, const CUtensorMap& tmap_tree_v) {
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* smem = smem_raw + ((1024u - (tc::smem_u32(smem_raw) & 1023u)) & 1023u);
   PtMisc& ms = *reinterpret_cast<PtMisc*>(smem + FS_MISC);
@@ -134,9 +165,27 @@ __global__ __launch_bounds__(PT_THREADS, 1) void mla_pair_tc_kernel(
   const int warp = tc::warp_index_uniform();
   const int rank = blockIdx.x & 1;                         // cluster of 2 along x
   // pairs from the last row on, the longest first; a chunk of an odd number of rows leaves row 0 alone, whose pair is a copy of it
-  const int r1 = a.m - 1 - 2 * (int)(blockIdx.x >> 1), r0 = max(0, r1 - 1), row = rank == 0 ? r0 : r1;
-  const bool lone = r1 == 0, mine = !(lone && rank == 1);
-  const int n = a.pos_start + r0 + 1;                      // the keys of both rows
+  int r1 = a.m - 1 - 2 * (int)(blockIdx.x >> 1), r0 = max(0, r1 - 1);
+  bool lone = r1 == 0;
+  int split = 0;
+  if (TREE) {
+    split = (int)(blockIdx.x >> 1) % a.n_split;
+    pdl_wait();
+    const PtPair p = pt_pair(a.tree, (int)(blockIdx.x >> 1) / a.n_split);
+    if (p.row < 0) return;                                 // (both CTAs, before anything of them is in use)
+    r0 = p.row;
+    lone = p.lone;
+    r1 = lone ? r0 : r0 + 1;
+    if (warp < 2) {
+      const MlaTree t = mla_tree(a, warp == 0 ? r0 : r1);
+      if (lane == 0) ms.tree[warp] = t;
+    }
+    __syncthreads();
+  }
+  const int row = rank == 0 ? r0 : r1;
+  const bool mine = !(lone && rank == 1);
+  const int n = TREE ? ms.tree[0].len : a.pos_start + r0 + 1;   // the keys of both rows
+  const int64_t base = TREE ? ms.tree[0].base : 0;
   // window form: both see the keys p >= lo and p < first_keys of the n; tile t is tile t, or t + jump behind the sinks' tiles; gone: the key that
   // the earlier row alone sees (-1: none)
   int lo = 0, first_keys = 0, first_tiles = 0, jump = 0, gone = -1;
@@ -148,10 +197,21 @@ __global__ __launch_bounds__(PT_THREADS, 1) void mla_pair_tc_kernel(
     first_tiles = (first_keys + FT_KEYS - 1) / FT_KEYS;
     jump = max(lo / FT_KEYS - first_tiles, 0);
   }
-  const int whole = (n + FT_KEYS - 1) / FT_KEYS - jump, n_tiles = whole + (lone ? 0 : 1);
-  auto key0 = [&](int t) -> int { return t >= whole ? n : WIN && t >= first_tiles ? (t + jump) * FT_KEYS : t * FT_KEYS; };
-  auto keys = [&](int t) -> int { return t < whole ? min(FT_KEYS, n - key0(t)) : 1; };
+  // tree form: of the tiles of the cached keys and the one behind them, the nodes', this split's; the nodes' is a tile for each
+  int tile0 = 0, whole = n / FT_KEYS + (n % FT_KEYS != 0) - jump, last_tiles = lone ? 0 : 1;
+  if (TREE) {
+    const int past = whole, per = (past + a.n_split) / a.n_split;
+    tile0 = min(past + 1, split * per);
+    const int end = min(past + 1, tile0 + per);
+    whole = min(end, past) - min(tile0, past);
+    last_tiles = end == past + 1 && end > tile0 ? (lone ? 1 : 2) : 0;
+  }
+  const int n_tiles = whole + last_tiles;
+  auto key0 = [&](int t) -> int { return t >= whole ? n : WIN && t >= first_tiles ? (t + jump) * FT_KEYS : (tile0 + t) * FT_KEYS; };
+  auto keys = [&](int t) -> int { return t < whole ? min(FT_KEYS, n - key0(t)) : TREE ? ms.tree[t - whole].node + 1 : 1; };
   auto edge = [&](int t) -> bool { return WIN && t < whole && keys(t) == FT_KEYS && key0(t) < lo && key0(t) + FT_KEYS > first_keys; };
+  // tree form: a tile that arrives as a box although not all of it is seen
+  auto ragged_box = [&](int t) -> bool { return TREE && (t >= whole || a.ckv_rows > 0); };
   const int last_quads = gone >= 0 ? 2 : 1;                // window form: groups of four keys of the last tile (keys 0 and 16)
 
   if (tid == 0) {
@@ -178,7 +238,7 @@ __global__ __launch_bounds__(PT_THREADS, 1) void mla_pair_tc_kernel(
     asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(tc::smem_u32(&ms.tmem)), "r"(512) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
   }
-  pdl_wait();
+  if (!TREE) pdl_wait();
   tc::fence_before_sync();
   asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");   // both CTAs' barriers and tensor memory
   tc::fence_after_sync();
@@ -191,10 +251,10 @@ __global__ __launch_bounds__(PT_THREADS, 1) void mla_pair_tc_kernel(
   const int other = 32 * (1 - rank);                       // the other CTA's keys of a tile
   // a ragged tile: four rows at a time, those past the end (and those that are not seen) read as zeros
   auto gather = [&](uint32_t leader, int t, int k0, int blk0, int blocks, uint32_t dst, uint64_t* bar) {
-    const int base = key0(t), valid = keys(t);
+    const int from = key0(t), valid = keys(t);
     auto at = [&](int k) -> int {
       if (WIN && t == whole && k == 16) return gone;
-      return k < valid && (!WIN || t == whole || base + k >= lo || base + k < first_keys) ? base + k : -1;
+      return k < valid && (!WIN || t == whole || from + k >= lo || from + k < first_keys) ? (int)(base + from + k) : -1;
     };
 #pragma unroll 1
     for (int q = 0; q < (WIN && t == whole ? 4 * last_quads : 8); q += WIN && t == whole ? 4 : 1)
@@ -222,8 +282,10 @@ __global__ __launch_bounds__(PT_THREADS, 1) void mla_pair_tc_kernel(
       if (lane == 0) tc::mbar_arrive_expect_tx(&ms.k_here[b], !last ? PT_V : rank == 0 ? last_quads * 8 * 512 : 0);
       __syncwarp();
       if (last && rank == 1) continue;
-      if (keys(t) < FT_KEYS) gather(leader, t, 32 * rank, 0, 8, tc::smem_u32(slot(t)), &ms.k_here[b]);
-      else if (lane == 0) pt_tma_box(slot(t), &tmap_k, key0(t) + 32 * rank, 0, &ms.k_here[b]);
+      if (TREE && t >= whole) {
+        if (lane == 0) pt_tma_box(slot(t), &tmap_tree_k, ms.tree[0].row0 + 32 * rank, 0, &ms.k_here[b]);
+      } else if (keys(t) < FT_KEYS && !ragged_box(t)) gather(leader, t, 32 * rank, 0, 8, tc::smem_u32(slot(t)), &ms.k_here[b]);
+      else if (lane == 0) pt_tma_box(slot(t), &tmap_k, (int)(base + key0(t)) + 32 * rank, 0, &ms.k_here[b]);
       __syncwarp();
     }
   } else if (warp == 7) {
@@ -238,8 +300,10 @@ __global__ __launch_bounds__(PT_THREADS, 1) void mla_pair_tc_kernel(
       __syncwarp();
       uint8_t* const dst = slot(t) + PT_V + (1 - rank) * PT_V_HALF;
       if (last && rank == 0) {
-      } else if (keys(t) < FT_KEYS) gather(leader, t, other, 4 * rank, 4, tc::smem_u32(dst), &ms.v_here[b]);
-      else if (lane == 0) pt_tma_box(dst, &tmap_v, key0(t) + other, 4 * rank, &ms.v_here[b]);
+      } else if (TREE && t >= whole) {
+        if (lane == 0) pt_tma_box(dst, &tmap_tree_v, ms.tree[0].row0 + other, 4 * rank, &ms.v_here[b]);
+      } else if (keys(t) < FT_KEYS && !ragged_box(t)) gather(leader, t, other, 4 * rank, 4, tc::smem_u32(dst), &ms.v_here[b]);
+      else if (lane == 0) pt_tma_box(dst, &tmap_v, (int)(base + key0(t)) + other, 4 * rank, &ms.v_here[b]);
       __syncwarp();
       ok = tc::mbar_wait<FT_POLL_NS>(&ms.k_here[b], turn(t), abort_flag, 32) && ok;
       if (lane == 0) {
@@ -299,6 +363,14 @@ __global__ __launch_bounds__(PT_THREADS, 1) void mla_pair_tc_kernel(
               if (kk < steps)
                 pt_mma(leader, tmem + FT_O + nh * 128, tc::sdesc_advance(pd, kk * 32), tc::sdesc_advance(vd, nh * 2 * PT_BLK + (kk >> 1) * PT_V_HALF + (kk & 1) * 2048), idesc,
                        t > 0 || kk > 0);
+        } else if constexpr (TREE) {                       // the keys of one node alone
+#pragma unroll
+          for (int nh = 0; nh < 2; nh++)
+#pragma unroll
+            for (int kk = 0; kk < FT_KEYS / 16; kk++)
+              if (kk < steps)
+                pt_mma_one(t - whole, leader, tmem + FT_O + nh * 128, tc::sdesc_advance(pd, kk * 32),
+                           tc::sdesc_advance(vd, nh * 2 * PT_BLK + (kk >> 1) * PT_V_HALF + (kk & 1) * 2048), idesc, whole > 0 || kk > 0);
         } else {
 #pragma unroll
           for (int nh = 0; nh < 2; nh++) {
@@ -355,7 +427,9 @@ __global__ __launch_bounds__(PT_THREADS, 1) void mla_pair_tc_kernel(
       // keys of this thread: 32 half .. + 31 of the tile; the last tile is the second row's
       const int have = (t < whole || rank == 1 ? keys(t) : 0) - 32 * half;
       uint32_t mask = have >= 32 ? 0xffffffffu : have <= 0 ? 0u : (1u << have) - 1u;
-      if (WIN && t < whole) {
+      if (TREE && t >= whole) {
+        mask = t - whole == rank ? (uint32_t)(ms.tree[rank].path >> (32 * half)) : 0u;
+      } else if (WIN && t < whole) {
         const int p = key0(t) + 32 * half, from = lo - p, to = first_keys - p;   // keys from `from` on and below `to` are seen
         mask &= (from <= 0 ? 0xffffffffu : from >= 32 ? 0u : 0xffffffffu << from) | (to <= 0 ? 0u : to >= 32 ? 0xffffffffu : (1u << to) - 1u);
       } else if (WIN && rank == 0 && half == 0 && gone >= 0) {
@@ -411,6 +485,16 @@ __global__ __launch_bounds__(PT_THREADS, 1) void mla_pair_tc_kernel(
       }
       l += sum;
       ok = tc::mbar_wait<FT_POLL_NS>(&ms.v_here[t % FT_NBUF], (t / FT_NBUF) & 1, abort_flag, 33) && ok;   // this CTA's part of V
+      if (TREE && (t >= whole || (keys(t) < FT_KEYS && ragged_box(t)))) {
+        // as below; two threads a key, each with half of this CTA's channels
+        const int k = tid & 63;
+        const bool seen = t >= whole ? ms.tree[t - whole].path >> k & 1 : k < keys(t);
+        if (!seen) {
+          uint8_t* v_row = slot(t) + PT_V + (k >> 5) * PT_V_HALF + (tid >> 6) * 2 * PT_BLK + (k & 31) * 128;
+#pragma unroll
+          for (int c = 0; c < 16; c++) *reinterpret_cast<uint4*>(v_row + (c >> 3) * PT_BLK + (((c + lane) & 7) << 4)) = make_uint4(0u, 0u, 0u, 0u);
+        }
+      }
       if (WIN && (edge(t) || t == whole)) {
         // keys that are not seen weigh nothing, but nothing times infinity is NaN: their rows of V become zeros (of the last tile, which 32
         // keys are multiplied of, all but keys 0 and 16)
@@ -429,14 +513,39 @@ __global__ __launch_bounds__(PT_THREADS, 1) void mla_pair_tc_kernel(
     // ---- the row's output: 2 x 64 channels at a time through the P buffers, thread half h has channels 256 h .. 256 h + 255 ----
     ms.l[tid] = l;
     if (n_tiles >= 2) wait_pv(n_tiles - 2, 36);
-    wait_pv(n_tiles - 1, 31);
+    if (n_tiles >= 1) wait_pv(n_tiles - 1, 31);
     tc::fence_after_sync();
     asm volatile("bar.sync 3, 128;" ::: "memory");
     l += ms.l[tid ^ 64];
-    const bool some = l > 0.f || a.keep_nan;               // as in mla_flash_tc_kernel
+    const bool some = (l > 0.f || a.keep_nan) && (!TREE || n_tiles > 0);   // as in mla_flash_tc_kernel
+    if (TREE && !a.out) {
+      // a partial, as there: fp32 rows in the idle ring, one bulk copy per head
+      const uint32_t pitch = LATENT * 4 + 16;
+      uint8_t* orow = smem + FS_K + head * pitch;
+#pragma unroll 1
+      for (int c0 = 0; c0 < 256; c0 += 32) {
+        uint32_t o[32];
+        tc::tmem_ld32(tmem + FT_O + c0 + lanes, o);
+        tc::tmem_ld_wait();
+#pragma unroll
+        for (int v = 0; v < 8; v++)
+          *reinterpret_cast<uint4*>(orow + (half * 256 + c0) * 4 + v * 16) =
+              some ? make_uint4(o[4 * v], o[4 * v + 1], o[4 * v + 2], o[4 * v + 3]) : make_uint4(0u, 0u, 0u, 0u);
+      }
+      tc::fence_async_smem();
+      asm volatile("bar.sync 3, 128;" ::: "memory");
+      const size_t rows = (size_t)a.m * FT_HEADS, rh = (size_t)row * FT_HEADS + head;
+      if (half == 0 && mine && ok && !*abort_flag) {
+        tc::bulk_s2g(a.part_acc + ((size_t)split * rows + rh) * LATENT, orow, LATENT * 4);
+        tc::bulk_commit();
+        a.part_m[(size_t)split * rows + rh] = (m == -INFINITY || !some) ? -INFINITY : m / LOG2E;
+        a.part_l[(size_t)split * rows + rh] = l;
+        tc::bulk_wait_read<0>();
+      }
+    }
     const float f = l > 0.f ? 1.f / l : 1.f;
 #pragma unroll 1
-    for (int c0 = 0; c0 < 256; c0 += 64) {
+    for (int c0 = 0; c0 < (TREE && !a.out ? 0 : 256); c0 += 64) {
       uint8_t* box = smem + FS_P + half * FP_BYTES;
       if (tid == 0) tc::bulk_wait_read<0>();
       asm volatile("bar.sync 3, 128;" ::: "memory");
@@ -479,6 +588,20 @@ __global__ __launch_bounds__(PT_THREADS, 1) void mla_pair_tc_kernel(
   asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");   // nothing of either CTA is in use any more
   if (warp == 0) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
   if (tid == 0 && ms.abort_flag && status) atomicExch(status, HK_ERR_TIMEOUT);
+}
+
+template <bool WIN>
+__global__ __launch_bounds__(PT_THREADS, 1) void mla_pair_tc_kernel(
+    MlaArgs a, int* __restrict__ status, const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ CUtensorMap tmap_v,
+    const __grid_constant__ CUtensorMap tmap_rows, const __grid_constant__ CUtensorMap tmap_q, const __grid_constant__ CUtensorMap tmap_o) {
+  pt_body<WIN, false>(a, status, tmap_k, tmap_v, tmap_rows, tmap_q, tmap_o, tmap_rows, tmap_rows);
+}
+// grid = 2 CTAs a pair of nodes and split
+__global__ __launch_bounds__(PT_THREADS, 1) void mla_pair_tree_tc_kernel(
+    MlaArgs a, int* __restrict__ status, const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ CUtensorMap tmap_v,
+    const __grid_constant__ CUtensorMap tmap_rows, const __grid_constant__ CUtensorMap tmap_q, const __grid_constant__ CUtensorMap tmap_o,
+    const __grid_constant__ CUtensorMap tmap_tree_k, const __grid_constant__ CUtensorMap tmap_tree_v) {
+  pt_body<false, true>(a, status, tmap_k, tmap_v, tmap_rows, tmap_q, tmap_o, tmap_tree_k, tmap_tree_v);
 }
 
 }  // namespace hk

@@ -154,6 +154,7 @@ __global__ __launch_bounds__(256) void mla_simt_kernel(MlaArgs a, MlaPaged pg) {
       o = gl;
     }
     const size_t rh = (size_t)r * a.n_heads + h0 + h;
+    if (a.out && a.tree_kv && tree.node < 0) continue;       // (a row of no tree)
     if (a.out) {
       a.out[rh * LATENT + ch] = __float2half_rn(gl > 0.f || (keep_nan && gl != 0.f) ? o / gl : 0.f);
     } else {
@@ -297,10 +298,8 @@ __global__ __launch_bounds__(128 * GROUPS) void lse_combine_kernel(
 
 // The same for few splits of many rows, as two sums of the even and of the odd splits, without shared memory or barriers: a warp keeps a
 // split's weight in a lane, a thread twelve pieces in flight.  1,536 rows of 6 splits 7.3 -> 4.0 us, 3,072 of 3 12.5 -> 5.4.
-__global__ __launch_bounds__(128) void lse_combine_few_kernel(const float* __restrict__ part_m, const float* __restrict__ part_l,
-                                                              const float* __restrict__ part_acc, int n_split, int64_t rows, __half* __restrict__ out) {
-  pdl_release();
-  pdl_wait();
+__device__ __forceinline__ void lse_combine_few(const float* __restrict__ part_m, const float* __restrict__ part_l, const float* __restrict__ part_acc, int n_split,
+                                                int64_t rows, __half* __restrict__ out) {
   const int64_t r = blockIdx.x;
   const int lane = threadIdx.x & 31;
   const bool mine = lane < n_split;
@@ -339,16 +338,29 @@ __global__ __launch_bounds__(128) void lse_combine_few_kernel(const float* __res
   *reinterpret_cast<uint2*>(out + (size_t)r * LATENT + threadIdx.x * 4) = pk;
 }
 
+__global__ __launch_bounds__(128) void lse_combine_few_kernel(const float* __restrict__ part_m, const float* __restrict__ part_l,
+                                                              const float* __restrict__ part_acc, int n_split, int64_t rows, __half* __restrict__ out) {
+  pdl_release();
+  pdl_wait();
+  lse_combine_few(part_m, part_l, part_acc, n_split, rows, out);
+}
+// rows of no tree of drafted tokens, whose partials are whatever lies there, are left as they were
+__global__ __launch_bounds__(128) void lse_combine_few_tree_kernel(const float* __restrict__ part_m, const float* __restrict__ part_l,
+                                                                   const float* __restrict__ part_acc, int n_split, int64_t rows, __half* __restrict__ out,
+                                                                   TreeArgs tree, int n_heads) {
+  pdl_release();
+  pdl_wait();
+  if (tree.seq_of(blockIdx.x / n_heads) < 0) return;
+  lse_combine_few(part_m, part_l, part_acc, n_split, rows, out);
+}
+
 // The same with every row shared by CSPLIT CTAs (few rows, or many splits), each
 // owning 512 / CSPLIT channels, with GROUPS groups of 32 float4 lanes over the splits, so that 64 rows still cover
 // the machine.  grid = (rows, CSPLIT).
 constexpr int LSE_CSPLIT = 4;
 template <int GROUPS, int PRE>
-__global__ __launch_bounds__(32 * GROUPS) void lse_combine_cs_kernel(
-    const float* __restrict__ part_m, const float* __restrict__ part_l, const float* __restrict__ part_acc,
-    int n_split, int64_t rows, __half* __restrict__ out) {
-  pdl_release();
-  pdl_wait();
+__device__ __forceinline__ void lse_combine_cs(const float* __restrict__ part_m, const float* __restrict__ part_l, const float* __restrict__ part_acc, int n_split,
+                                               int64_t rows, __half* __restrict__ out) {
   constexpr int LANES = 128 / LSE_CSPLIT;
   const int64_t r = blockIdx.x;
   const int cpart = blockIdx.y;
@@ -365,6 +377,24 @@ __global__ __launch_bounds__(32 * GROUPS) void lse_combine_cs_kernel(
     pk.y = *reinterpret_cast<uint32_t*>(&h1);
     *reinterpret_cast<uint2*>(out + (size_t)r * LATENT + (cpart * LANES + threadIdx.x) * 4) = pk;
   }
+}
+
+template <int GROUPS, int PRE>
+__global__ __launch_bounds__(32 * GROUPS) void lse_combine_cs_kernel(
+    const float* __restrict__ part_m, const float* __restrict__ part_l, const float* __restrict__ part_acc,
+    int n_split, int64_t rows, __half* __restrict__ out) {
+  pdl_release();
+  pdl_wait();
+  lse_combine_cs<GROUPS, PRE>(part_m, part_l, part_acc, n_split, rows, out);
+}
+template <int GROUPS, int PRE>
+__global__ __launch_bounds__(32 * GROUPS) void lse_combine_cs_tree_kernel(
+    const float* __restrict__ part_m, const float* __restrict__ part_l, const float* __restrict__ part_acc,
+    int n_split, int64_t rows, __half* __restrict__ out, TreeArgs tree, int n_heads) {
+  pdl_release();
+  pdl_wait();
+  if (tree.seq_of(blockIdx.x / n_heads) < 0) return;
+  lse_combine_cs<GROUPS, PRE>(part_m, part_l, part_acc, n_split, rows, out);
 }
 
 // ---- merge of S partial sets into ONE partial set (still un-normalised): the per-GPU reduction before

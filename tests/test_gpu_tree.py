@@ -124,7 +124,7 @@ def test_what_a_node_does_not_see_has_no_effect(over):
 
     good = call(clean)
     assert bool(torch.isfinite(good).all())
-    assert not bool(good[:2].any()) and not bool(good[starts[-1]:].any()), "rows of no tree"
+    assert bool((good[:2] == 7).all()) and bool((good[starts[-1]:] == 7).all()), "rows of no tree are left as they were"
     bad = clean.clone()
     bad[:2], bad[starts[-1]:] = NAN, -INF
     for node, value in ((4, NAN), (6, INF), (14, -INF)):
@@ -137,6 +137,39 @@ def test_what_a_node_does_not_see_has_no_effect(over):
                 assert bool(torch.isnan(out[r]).any()), (s, j)
             else:
                 assert torch.equal(out[r], good[r]), (s, j)
+
+
+@pytest.mark.parametrize("told", [True, False])
+def test_two_nodes_by_a_pair_of_ctas(told):
+    """enough nodes and keys that two of a tree go together: odd trees, an empty one, ragged lengths, splits, branches and gaps that hold NaN"""
+    trees = [tree_of(t) for t in ((33, 1), (64, 2), "one", [], "chain5", (40, 6), "star7")]
+    lens = [2000, 1531, 3001, 5, 64, 2879, 0]
+    gen = gen_of(31)
+    starts, parent, tree_start = layout(trees, front=1)
+    m, n = starts[-1] + 2, len(trees)
+    parent = torch.cat((parent, ints([0, 0])))
+    base = [sum(lens[:i]) + 2 * (i + 1) for i in range(n)]
+    ckv = torch.full((sum(lens) + 2 * (n + 1) + 64, 512), NAN, dtype=torch.float16, device="cuda")
+    for b, k in zip(base, lens):
+        ckv[b:b + k] = randn(gen, k, 512).half()
+    q, rows = (randn(gen, m, 64, 512) * 0.7).half(), randn(gen, m, 512).half()
+    bad = {starts[1] + 60: NAN, starts[0] + 31: INF, starts[6] + 3: -INF, 0: NAN, m - 1: NAN}
+    for r, value in bad.items():
+        rows[r] = value
+    out = torch.full((m, 64, 512), 7.0, dtype=torch.float16, device="cuda")
+    hk.mla_tree_decode(q, ckv, rows, parent, out, m, n_seqs=n, tree_start=tree_start, kv_base=torch.tensor(base, device="cuda"), kv_len=ints(lens),
+                       n_keys_hint=max(lens), ckv_rows=None if told else 0)
+    finish()
+    for s, tree in enumerate(trees):
+        for j in range(len(tree)):
+            r, seen = starts[s] + j, [starts[s] + i for i in path(tree, j)]
+            if set(seen) & set(bad):
+                assert bool(torch.isnan(out[r]).any()), (s, j)
+            else:
+                o, tol = attend(q[r].double(), torch.cat((ckv[base[s]:base[s] + lens[s]].double(), rows[seen].double())), 0.0625)
+                assert bool(((out[r].double() - o).abs() <= tol).all()), (s, j)
+    for r in (0, m - 2, m - 1):
+        assert bool((out[r] == 7).all())
 
 
 def test_parents_that_are_no_earlier_node_hang_on_the_sequence():
@@ -163,7 +196,7 @@ def test_a_sequence_of_more_rows_than_a_tree_has():
     hk.mla_tree_decode(q, ckv, tree_kv, ints(tree), out, m, tree_start=ints([0, m]), kv_len=ints([1 << 30]), n_keys_hint=n)
     finish()
     check_rows(out[:64], wanted(q, ckv.double(), tree_kv, 0, tree[:64], 0.0625))
-    assert not bool(out[64:].any())
+    assert bool((out[64:] == 7).all())
 
 
 @pytest.mark.parametrize("m,n", [(1, 5001), (12, 9000), (64, 3000)])

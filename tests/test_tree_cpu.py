@@ -50,11 +50,11 @@ def test_tree_attention_over_8_bits_refuses(lib, changes, status):
 def test_empty_calls_and_workspaces(lib):
     assert call(lib.hk_mla_tree, TREE, TREE_GOOD, m=0) == hk.HK_OK
     assert call(lib.hk_mla8_tree, TREE8, TREE8_GOOD, m=0) == hk.HK_OK
-    assert lib.hk_mla_tree_workspace_bytes(0, 64, 100) == 0 and lib.hk_mla_tree_workspace_bytes(4, 64, -1) == 0
+    assert lib.hk_mla_tree_workspace_bytes(0, 64, 1, 100) == 0 and lib.hk_mla_tree_workspace_bytes(4, 64, 1, -1) == 0
     for m in (1, 8, 64, 700):
         for keys in (0, 1, 5001, 1 << 20, (1 << 31) - 1):
             for heads in (4, 64):
-                need = lib.hk_mla_tree_workspace_bytes(m, heads, keys)
+                need = lib.hk_mla_tree_workspace_bytes(m, heads, 3, keys)
                 assert need == 0 or need >= lib.hk_mla_partial_bytes(2, m * heads)
             assert lib.hk_mla8_tree_workspace_bytes(m, 64, keys) >= 0
     assert lib.hk_mla8_pages_workspace_bytes(0, 4) == 0 and lib.hk_mla8_pages_workspace_bytes(8, -1) == 0
