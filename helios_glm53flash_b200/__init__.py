@@ -97,7 +97,7 @@ SIGNATURES = {
     "hk_mla8_sparse": (_i, [_vp, _vp, _vp, _i, _i64, _i, _vp, _i, _i, _vp, _vp, _i, _vp, _i, _i, _f, _i, _vp, _sz, _vp]),
     "hk_mla_tree_workspace_bytes": (_sz, [_i, _i, _i, _i]),
     "hk_mla_tree": (_i, [_vp, _vp, _i64, _vp, _vp, _i, _vp, _vp, _vp, _i, _vp, _i, _i, _f, _i, _vp, _sz, _vp]),
-    "hk_mla8_tree_workspace_bytes": (_sz, [_i, _i, _i]),
+    "hk_mla8_tree_workspace_bytes": (_sz, [_i, _i, _i, _i, _i64]),
     "hk_mla8_tree": (_i, [_vp, _vp, _vp, _i, _i64, _i, _vp, _i, _vp, _i, _vp, _vp, _vp, _i, _vp, _i, _i, _f, _i, _vp, _sz, _vp]),
     "hk_mla_tree_accept": (_i, [_vp, _vp, _i64, _vp, _vp, _i, _vp, _vp, _i, _vp, _i, _vp, _vp]),
     "hk_mla8_tree_accept": (_i, [_vp, _vp, _vp, _i, _i64, _i, _vp, _i, _vp, _i, _vp, _vp, _i, _vp, _i, _vp, _vp]),
@@ -568,8 +568,9 @@ def mla_tree_workspace_bytes(m, n_heads, n_seqs, n_keys):
     return load_library().hk_mla_tree_workspace_bytes(m, n_heads, n_seqs, n_keys)
 
 
-def mla8_tree_workspace_bytes(m, n_heads, n_keys):
-    return load_library().hk_mla8_tree_workspace_bytes(m, n_heads, n_keys)
+def mla8_tree_workspace_bytes(m, n_heads, n_seqs, n_keys, positions):
+    """positions: of a sequence in the table (blocks of a sequence x tokens of a block)"""
+    return load_library().hk_mla8_tree_workspace_bytes(m, n_heads, n_seqs, n_keys, positions)
 
 
 def mla_tree_decode(q_lat, ckv, tree_kv, parent, lat_out, m, pos_start=0, n_seqs=1, tree_start=None, kv_base=None, kv_len=None, stream=None,
@@ -604,7 +605,7 @@ def mla8_tree_decode(q_lat, ckv8, scales, tree_kv, parent, lat_out, m, pos_start
         pos_start = n_keys_hint or pos_start
     ws = workspace
     if ws is None:
-        need = (_native.hk_mla8_tree_workspace_bytes(m, n_heads, pos_start) if n_split <= 0
+        need = (_native.hk_mla8_tree_workspace_bytes(m, n_heads, n_seqs, pos_start, (stride if stride else n_blocks) * block) if n_split <= 0
                 else _native.hk_mla_partial_bytes(n_split, m * n_heads) if n_split > 1 else 0)
         if need:
             ws = _scratch_like(need, q_lat, stream)

@@ -238,26 +238,16 @@ cudaError_t accept_launch(const AppendArgs& a, cudaStream_t s) {
 // A warp four rows, a lane eight channels and the eight 256 further on (8-byte loads, 16-byte stores).  CTAs behind those of the rows: the
 // n_idx gathered positions of a sparse call, those without a block as -1.
 constexpr int READ_ROWS = 4, READ_IDX = 8;
-template <int FMT>
-__global__ void __launch_bounds__(256) mla8_read_kernel(MlaPaged pg, int head, int shift, int n, __half* out, const int* idx, int64_t n_idx, int* idx_out) {
-  pdl_release();
-  pdl_wait();
-  const int row_ctas = (n + 8 * READ_ROWS - 1) / (8 * READ_ROWS);
-  if ((int)blockIdx.x >= row_ctas) {
-#pragma unroll
-    for (int k = 0; k < READ_IDX; k++) {
-      const int64_t i = ((int64_t)(blockIdx.x - row_ctas) * READ_IDX + k) * 256 + threadIdx.x;
-      if (i < n_idx) idx_out[i] = pg.block_of(0, idx[i]) >= 0 ? idx[i] : -1;
-    }
-    return;
-  }
-  const int lane = threadIdx.x & 31, i0 = (blockIdx.x * 8 + (threadIdx.x >> 5)) * READ_ROWS;
+// rows i0 .. i0 + READ_ROWS - 1 of n, position at(i) of a sequence each, by a warp
+template <int FMT, class At>
+__device__ __forceinline__ void read_rows(const MlaPaged& pg, int seq, int i0, int n, __half* out, At at) {
+  const int lane = threadIdx.x & 31;
   uint2 v[READ_ROWS][2];
   float s[READ_ROWS];
 #pragma unroll
   for (int k = 0; k < READ_ROWS; k++) {
-    const int i = i0 + k, p = i < head ? i : i + shift;
-    const int64_t b = i < n ? pg.block_of(0, p) : -1;
+    const int i = i0 + k, p = at(i);
+    const int64_t b = i < n ? pg.block_of(seq, p) : -1;
     s[k] = 0.f;
     v[k][0] = v[k][1] = make_uint2(0u, 0u);
     if (b >= 0) {
@@ -280,6 +270,31 @@ __global__ void __launch_bounds__(256) mla8_read_kernel(MlaPaged pg, int head, i
       reinterpret_cast<uint4*>(out + (size_t)(i0 + k) * LATENT)[lane + 32 * h] = w;
     }
   }
+}
+template <int FMT>
+__global__ void __launch_bounds__(256) mla8_read_kernel(MlaPaged pg, int head, int shift, int n, __half* out, const int* idx, int64_t n_idx, int* idx_out) {
+  pdl_release();
+  pdl_wait();
+  const int row_ctas = (n + 8 * READ_ROWS - 1) / (8 * READ_ROWS);
+  if ((int)blockIdx.x >= row_ctas) {
+#pragma unroll
+    for (int k = 0; k < READ_IDX; k++) {
+      const int64_t i = ((int64_t)(blockIdx.x - row_ctas) * READ_IDX + k) * 256 + threadIdx.x;
+      if (i < n_idx) idx_out[i] = pg.block_of(0, idx[i]) >= 0 ? idx[i] : -1;
+    }
+    return;
+  }
+  read_rows<FMT>(pg, 0, (blockIdx.x * 8 + (threadIdx.x >> 5)) * READ_ROWS, n, out, [&](int i) { return i < head ? i : i + shift; });
+}
+
+// The first positions of every sequence, lens[s] (or len) of them and `cap` at most, as fp16 rows from row s * cap on; grid (CTAs of a sequence, sequences).
+template <int FMT>
+__global__ void __launch_bounds__(256) mla8_read_seqs_kernel(MlaPaged pg, const int* lens, int len, int cap, __half* out) {
+  pdl_release();
+  pdl_wait();
+  const int seq = blockIdx.y, n = min(lens ? lens[seq] : len, cap);
+  for (int64_t i0 = ((int64_t)blockIdx.x * 8 + (threadIdx.x >> 5)) * READ_ROWS; i0 < n; i0 += (int64_t)gridDim.x * 8 * READ_ROWS)
+    read_rows<FMT>(pg, seq, (int)i0, n, out + (size_t)seq * cap * LATENT, [](int i) { return i; });
 }
 
 }  // namespace
@@ -309,6 +324,15 @@ int mla8_read_launch(const MlaPaged& pg, int dtype, int head, int shift, int n, 
   if (ctas > INT32_MAX) return HK_ERR_UNSUPPORTED;
   return pdl_launch(dtype == HK_I8 ? mla8_read_kernel<CACHE_I8> : mla8_read_kernel<CACHE_E4M3>, dim3((unsigned)ctas), dim3(256), 0, s, pg, head, shift, n,
                     out, idx, n_idx, idx_out) == cudaSuccess
+             ? HK_OK
+             : HK_ERR_CUDA;
+}
+
+// the sequences' positions for a tree call, about n_keys each
+int mla8_read_seqs_launch(const MlaPaged& pg, int dtype, const int* lens, int len, int cap, int n_keys, __half* out, cudaStream_t s) {
+  const int64_t ctas = ((int64_t)n_keys + 8 * READ_ROWS - 1) / (8 * READ_ROWS);
+  return pdl_launch(dtype == HK_I8 ? mla8_read_seqs_kernel<CACHE_I8> : mla8_read_seqs_kernel<CACHE_E4M3>, dim3((unsigned)ctas, (unsigned)pg.n_seqs), dim3(256), 0, s, pg,
+                    lens, len, cap, out) == cudaSuccess
              ? HK_OK
              : HK_ERR_CUDA;
 }

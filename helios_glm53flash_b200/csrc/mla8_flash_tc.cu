@@ -59,6 +59,7 @@ struct F8Misc {
   float mx[2][128];                               // tile maxima by softmax thread and tile parity; at the end sums, and the heads' factors
   uint32_t tmem;
   int abort_flag;
+  uint32_t bad[4];
 };
 static_assert(sizeof(F8Misc) <= 2048, "misc area");
 
@@ -69,7 +70,7 @@ struct F8Row {
   int head_tiles, jump, tiles;                    // tile i of the row's list is tile i, or i + jump behind the sinks' tiles
 };
 // a node of a tree: the tile behind those of the cache is the tree's
-__device__ __forceinline__ F8Row f8_tree_row(const MlaTree& t, const MlaPaged& pg) {
+__device__ __forceinline__ F8Row f8_tree_row(const MlaNodes& t, const MlaPaged& pg) {
   F8Row w;
   w.seq = t.seq;
   w.keys = key_list(t.len, 0, 0);
@@ -90,6 +91,7 @@ __device__ __forceinline__ F8Row f8_row(const MlaArgs& a, const MlaPaged& pg, in
   return w;
 }
 struct F8Item {
+  int q_row;                                      // first query row, of [m][n_heads]
   int r, hg, sp, n_sp, first;                     // row, 64 heads, split of how many, unit of split 0 (shared out splits); r < 0: nothing to do
   int part;                                       // part of the output channels
   F8Row row;
@@ -125,9 +127,9 @@ __device__ __forceinline__ void f8_share(const MlaArgs& a, const MlaPaged& pg, i
   it.sp = unit - it.first;
 }
 
-// tree: the row's (trees' calls; executed by a whole warp then)
+// tree: of the nodes (trees' calls; executed by a whole warp then)
 template <bool GATHER, int PARTS, bool TREE>
-__device__ __forceinline__ F8Item f8_item(const MlaArgs& a, const MlaPaged& pg, int idx, MlaTree& tree) {
+__device__ __forceinline__ F8Item f8_item(const MlaArgs& a, const MlaPaged& pg, int idx, MlaNodes& tree) {
   F8Item it;
   const int groups = (a.n_heads + F8_HEADS - 1) / F8_HEADS;
   int per;
@@ -151,13 +153,14 @@ __device__ __forceinline__ F8Item f8_item(const MlaArgs& a, const MlaPaged& pg, 
     it.r = idx / groups;
     if (!GATHER && !TREE && !a.kv_len) it.r = a.m - 1 - it.r;   // rows of a causal chunk grow: the longest first
     if constexpr (TREE) {
-      tree = mla_tree(a, it.r);
+      tree = mla_nodes(a, it.r);
       it.row = f8_tree_row(tree, pg);
     } else {
       it.row = f8_row<GATHER>(a, pg, it.r);
     }
     per = (it.row.tiles + a.n_split - 1) / a.n_split;
   }
+  it.q_row = TREE ? (tree.row0 + tree.node) * a.n_heads : it.r * a.n_heads;
   it.t0 = min(it.row.tiles, it.sp * per);
   it.n_tiles = min(it.row.tiles, it.t0 + per) - it.t0;
   return it;
@@ -247,7 +250,7 @@ __global__ __launch_bounds__(F8_THREADS, 1) void mla8_flash_tc_kernel(MlaArgs a,
   }
   if (warp == 0) tc::tmem_alloc(&ms.tmem, 512);
   pdl_wait();
-  MlaTree tree{0, 0, 0, 0, 0, -1};
+  MlaNodes tree{0, 0, 0, 0, 0, 0, 0, 0};
   const F8Item it = f8_item<GATHER, PARTS, TREE>(a, pg, blockIdx.x, tree);
   tc::fence_before_sync();
   __syncthreads();
@@ -257,9 +260,9 @@ __global__ __launch_bounds__(F8_THREADS, 1) void mla8_flash_tc_kernel(MlaArgs a,
   const bool direct_q = it.n_tiles < F8_NBUF;
   // Final rows, or a partial: with a number of splits [split][row, head], shared out [CTA][64 heads].
   const bool final_out = PARTS == 1 && it.n_sp == 1;
-  const size_t part_row = a.n_split == 0 ? (size_t)blockIdx.x * F8_HEADS : ((size_t)it.sp * a.m + it.r) * a.n_heads + it.hg * F8_HEADS;
+  const size_t part_row = a.n_split == 0 ? (size_t)blockIdx.x * F8_HEADS : (size_t)it.sp * a.m * a.n_heads + it.q_row + it.hg * F8_HEADS;
   if (a.n_split == 0 && it.r >= 0 && it.sp == 0 && it.hg == 0 && tid == 0) a.shares[it.r] = make_int2(it.first, it.n_sp);
-  const int n_tiles = it.n_tiles, h0 = it.hg * F8_HEADS, n_h = min(F8_HEADS, a.n_heads - h0);
+  const int n_tiles = it.n_tiles, h0 = it.hg * F8_HEADS, n_h = TREE ? min(F8_HEADS, tree.count * a.n_heads - h0) : min(F8_HEADS, a.n_heads - h0);
   bool ok = true;
 
   if (warp >= 6) {
@@ -287,7 +290,7 @@ __global__ __launch_bounds__(F8_THREADS, 1) void mla8_flash_tc_kernel(MlaArgs a,
       if (at >= 0) v = f8_ld_key(src + (size_t)at * LATENT);
     };
     // row of the cache, -1: none (rows of a cache are counted in 31 bits).  In a chunk a seen position without a block is a key of zeros.
-    const bool zeros = !GATHER && !TREE && !a.kv_len && !pg.row_seq;
+    const bool zeros = !GATHER && (TREE || (!a.kv_len && !pg.row_seq));
     auto row_of = [&](int p, int e) -> int { return e < 0 || e >= pg.n_blocks ? -1 : (e << pg.shift) + (p & in_block); };
     auto scale_of = [&](int row, int p, int e) -> float { return row >= 0 ? f8_ld_float(pg.scales + e) : zeros && p >= 0 ? 0.f : -1.f; };
     // On their way: the keys of two tiles, in registers; table entries of the third; positions of the fourth.
@@ -320,14 +323,14 @@ __global__ __launch_bounds__(F8_THREADS, 1) void mla8_flash_tc_kernel(MlaArgs a,
       if (t == F8_NBUF - 1) ok = tc::mbar_wait<F8_POLL_NS>(&ms.q_ready, 0, abort_flag, 41) && ok;   // Q came through the last slot
       if (t >= F8_NBUF) ok = tc::mbar_wait<F8_POLL_NS>(&ms.free[b], (t / F8_NBUF - 1) & 1, abort_flag, 42) && ok;
       const bool drafted = TREE && it.t0 + t == it.row.tiles - 1;
-      if (lane < F8_ROWS) ms.sc[b][k8 + lane] = drafted ? (tree.path >> (k8 + lane) & 1 ? 1.f : -1.f) : scale;
+      if (lane < F8_ROWS) ms.sc[b][k8 + lane] = drafted ? (tree.any >> (k8 + lane) & 1 ? 1.f : -1.f) : scale;
       uint8_t* dst = smem + F8S_K + b * F8_TILE + blk * F8_BLK + k8 * 128;
       // 16 channels are two 16-byte chunks of a 128-byte row; lanes four apart write them in the other order (no bank conflicts)
       if (TREE && drafted) {
 #pragma unroll
         for (int i = 0; i < F8_ROWS; i++) {
           uint4 lo = make_uint4(0u, 0u, 0u, 0u), hi = lo;
-          if (tree.path >> (k8 + i) & 1) {
+          if (tree.any >> (k8 + i) & 1) {
             const uint8_t* key = reinterpret_cast<const uint8_t*>(a.tree_kv + (size_t)(tree.row0 + k8 + i) * LATENT) + lane * 32;
             lo = f8_ld_key(key);
             hi = f8_ld_key(key + 16);
@@ -394,7 +397,7 @@ __global__ __launch_bounds__(F8_THREADS, 1) void mla8_flash_tc_kernel(MlaArgs a,
     } else {
       if (n_tiles > 0 && lane == 0) {
         tc::mbar_arrive_expect_tx(&ms.q_full, F8_TILE);
-        f8_tma_box(smem + F8S_K + (F8_NBUF - 1) * F8_TILE, &tmap_q, it.r * a.n_heads + h0, &ms.q_full);
+        f8_tma_box(smem + F8S_K + (F8_NBUF - 1) * F8_TILE, &tmap_q, it.q_row + h0, &ms.q_full);
       }
       __syncwarp();
       // all 512 channels as two products of 256, or this CTA's 256 or 128
@@ -462,6 +465,21 @@ __global__ __launch_bounds__(F8_THREADS, 1) void mla8_flash_tc_kernel(MlaArgs a,
       tc::fence_before_sync();
       tc::mbar_arrive(&ms.s_free[b]);
       float tmax = -INFINITY;
+      const bool grouped = TREE && a.tree_group > 1 && it.t0 + t == it.row.tiles - 1;
+      uint32_t bad = 0;
+      if (grouped) {                                       // several nodes in the tile of the tree: as in mla_flash_tc_kernel
+#pragma unroll
+        for (int j = 0; j < 32; j++) bad |= fabsf(__uint_as_float(sv[j])) < INFINITY ? 0u : 1u << j;
+        bad = __reduce_and_sync(0xffffffffu, bad);
+        if (lane == 0) ms.bad[warp] = bad;
+        asm volatile("bar.sync 3, 128;" ::: "memory");
+        bad = ms.bad[2 * half] & ms.bad[2 * half + 1];
+        if (ms.bad[head >> 4 & 2] & ms.bad[(head >> 4 & 2) + 1] & 1u << (head & 31)) {   // key `head` of the tile, half of its channels
+          uint8_t* key = smem + F8S_K + kb * F8_TILE + half * 4 * F8_BLK + head * 128;
+#pragma unroll
+          for (int c = 0; c < 32; c++) *reinterpret_cast<uint4*>(key + (c >> 3) * F8_BLK + (((c + lane) & 7) << 4)) = make_uint4(0u, 0u, 0u, 0u);
+        }
+      }
       const uint64_t sc22 = pack2(sc2, sc2);
 #pragma unroll
       for (int j = 0; j < 8; j++) {
@@ -480,6 +498,13 @@ __global__ __launch_bounds__(F8_THREADS, 1) void mla8_flash_tc_kernel(MlaArgs a,
 #pragma unroll
         for (int j = 0; j < 32; j++)
           if (own[j] < 0.f) sv[j] = __float_as_uint(-INFINITY);
+      }
+      if (grouped) {
+        const uint32_t mine = (uint32_t)(__shfl_sync(0xffffffffu, tree.mine, head / a.n_heads) >> (32 * half));
+#pragma unroll
+        for (int j = 0; j < 32; j++)
+          if (!(mine >> j & 1)) sv[j] = __float_as_uint(-INFINITY);
+          else if (bad >> j & 1) sv[j] = 0x7fffffffu;
       }
 #pragma unroll
       for (int j = 0; j < 32; j++) tmax = fmaxf(tmax, __uint_as_float(sv[j]));
@@ -620,7 +645,7 @@ __global__ __launch_bounds__(F8_THREADS, 1) void mla8_flash_tc_kernel(MlaArgs a,
     }
     asm volatile("bar.sync 4, 384;" ::: "memory");
     if (!*abort_flag && (!TREE || tree.seq >= 0)) {          // (a row of no tree is left as it was)
-      uint8_t* dst = final_out ? reinterpret_cast<uint8_t*>(a.out + ((size_t)it.r * a.n_heads + h0) * LATENT)
+      uint8_t* dst = final_out ? reinterpret_cast<uint8_t*>(a.out + ((size_t)it.q_row + h0) * LATENT)
                                : reinterpret_cast<uint8_t*>(a.part_acc + part_row * LATENT + it.part * n_ch);
       const int team = warp < 4 ? warp : warp - 2;
       const int per = n_ch * elem / 512;                   // 512-byte pieces of a head
@@ -647,7 +672,7 @@ int f8_launch(const MlaArgs& a, const MlaPaged& pg, const CUtensorMap& q, cudaSt
     attr_set[dev] = true;
   }
   const int groups = (a.n_heads + F8_HEADS - 1) / F8_HEADS;
-  const int64_t items = (a.n_split == 0 ? (int64_t)a.units : (int64_t)a.n_split * a.m * PARTS) * groups;
+  const int64_t items = (a.n_split == 0 ? (int64_t)a.units : (int64_t)a.n_split * (TREE ? a.tree_units : a.m) * PARTS) * groups;
   if (items > INT32_MAX) return HK_ERR_UNSUPPORTED;
   const cudaError_t e = pdl_launch(mla8_flash_tc_kernel<GATHER, FMT, PARTS, TREE>, dim3((unsigned)items), dim3(F8_THREADS), F8_SMEM, s, a, pg, device_status_ptr(), q);
   return e == cudaSuccess && cudaPeekAtLastError() == cudaSuccess ? HK_OK : HK_ERR_CUDA;
@@ -773,7 +798,7 @@ int mla8_flash_tc_launch(const MlaArgs& a, const MlaPaged& pg, int dtype, cudaSt
   if (!mla_rows_map(&q, a.q_lat, (int64_t)a.m * a.n_heads)) return HK_ERR_UNSUPPORTED;
   // Few splits of few rows: the output channels of each are shared out over two or four CTAs, which compute the scores each for itself and write
   // a half or a quarter of the partial (of 128 KB, which take 2.1 us).  2,052 gathered rows 11.1 -> 9.1 us (four), 5,001 keys 11.1 -> 10.4 (two).
-  const int64_t ctas = (int64_t)a.n_split * a.m * ((a.n_heads + F8_HEADS - 1) / F8_HEADS);
+  const int64_t ctas = (int64_t)a.n_split * (a.tree_kv ? a.tree_units : a.m) * ((a.n_heads + F8_HEADS - 1) / F8_HEADS);
   const int parts = a.n_split < 2 ? 1 : f8_parts(ctas);
   const int st = a.raw_idx ? (dtype == HK_I8 ? f8_launch_parts<true, CACHE_I8>(parts, a, pg, q, s) : f8_launch_parts<true, CACHE_E4M3>(parts, a, pg, q, s))
                            : (dtype == HK_I8 ? f8_launch_parts<false, CACHE_I8>(parts, a, pg, q, s) : f8_launch_parts<false, CACHE_E4M3>(parts, a, pg, q, s));

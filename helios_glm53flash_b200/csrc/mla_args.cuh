@@ -29,8 +29,11 @@ struct MlaArgs {
   int2* shares;
   // trees of drafted tokens: row r is a node of tree.seq_of(r), whose cached keys kv_base and kv_len (then per sequence) say
   TreeArgs tree;
+  int64_t kv_stride;        // without kv_base: a sequence's rows begin at this times its number and end before the next one's (0: all at row 0)
   const __half* tree_kv;    // [m][512] the nodes' own latents
   bool tree_pairs;          // two nodes to a pair of CTAs
+  int tree_group;           // otherwise: neighbouring nodes that share a CTA's 64 query rows (64 / heads)
+  int64_t tree_units;       // and the groups that there may be
   int keep_nan;             // keys that are not finite make outputs that are NaN (0: zeros where the scores are, as hk_mla_dense's callers know it)
 };
 
@@ -74,8 +77,34 @@ __device__ __forceinline__ MlaTree mla_tree(const MlaArgs& a, int r) {
   t.row0 = rows.x;
   t.node = r - rows.x;
   t.path = paths.of(t.node);
-  t.base = a.kv_base ? a.kv_base[t.seq] : 0;
+  t.base = a.kv_base ? a.kv_base[t.seq] : t.seq * a.kv_stride;
   t.len = max(a.kv_len ? a.kv_len[t.seq] : a.pos_start, 0);
+  if (a.kv_stride > 0) t.len = (int)min((int64_t)t.len, a.kv_stride);
+  if (a.ckv_rows > 0) t.len = (int)max((int64_t)0, min((int64_t)t.len, a.ckv_rows - t.base));   // never past the end of the cache
+  return t;
+}
+
+// Neighbouring nodes of a tree, a.tree_group of them, whose heads are a CTA's 64 query rows.
+constexpr int MLA_GROUP = 16;
+struct MlaNodes {
+  int64_t base;
+  uint64_t any, mine;                             // what some of them sees of the tree; what the lane-th of them sees
+  int seq, len, row0, node, count;                // the tree's first row, the first node and how many; seq < 0: no such group
+};
+// executed by a whole warp
+__device__ __forceinline__ MlaNodes mla_nodes(const MlaArgs& a, int unit) {
+  const int lane = threadIdx.x & 31;
+  const TreeUnit u = tree_unit(a.tree, unit, a.tree_group);
+  MlaNodes t{0, 0, 0, u.seq, 0, u.row0, u.node, u.count};
+  if (t.seq < 0) return t;
+  TreePaths paths;
+  paths.load(a.tree, a.tree.rows(t.seq));
+  t.mine = paths.of((t.node + lane) & 63);
+  if (lane >= t.count) t.mine = 0;
+  t.any = (uint64_t)__reduce_or_sync(0xffffffffu, (uint32_t)(t.mine >> 32)) << 32 | __reduce_or_sync(0xffffffffu, (uint32_t)t.mine);
+  t.base = a.kv_base ? a.kv_base[t.seq] : t.seq * a.kv_stride;
+  t.len = max(a.kv_len ? a.kv_len[t.seq] : a.pos_start, 0);
+  if (a.kv_stride > 0) t.len = (int)min((int64_t)t.len, a.kv_stride);
   if (a.ckv_rows > 0) t.len = (int)max((int64_t)0, min((int64_t)t.len, a.ckv_rows - t.base));   // never past the end of the cache
   return t;
 }

@@ -22,10 +22,13 @@ size_t mla8_units_bytes(int units, int m, int n_heads, MlaArgs* a, void* workspa
 // implemented in mla8_cache.cu
 int mla8_read_launch(const MlaPaged& pg, int dtype, int head, int shift, int n, __half* out, cudaStream_t s, const int* idx = nullptr, int64_t n_idx = 0,
                      int* idx_out = nullptr);
+int mla8_read_seqs_launch(const MlaPaged& pg, int dtype, const int* lens, int len, int cap, int n_keys, __half* out, cudaStream_t s);
 bool mla8_paged(MlaPaged* pg, const void* ckv8, const float* scales, int dtype, int64_t n_blocks, int block, const int* block_table,
                 int table_stride, int n_seqs, const int* row_seq);
 bool mla_flash_cluster_shape(int m, int tiles, int* n_split);
-bool mla_tree_shape(int m, int n_seqs, bool ragged, int n_keys, int* n_split);
+bool mla_tree_shape(int m, int n_seqs, bool ragged, int group, int n_keys, int* n_split);
+// neighbouring nodes of a tree whose heads fill 64 query rows
+static int tree_group(int n_heads) { return n_heads < 64 && 64 % n_heads == 0 ? 64 / n_heads : 1; }
 
 static inline size_t align_up(size_t v, size_t a) { return (v + a - 1) / a * a; }
 
@@ -143,7 +146,7 @@ static int attend_splits(int m, int n_heads, int n_keys, int window) {
 // which may then merge one row's splits in clusters; a number of splits that the caller gives means that many CTAs a row.
 static int attend(MlaArgs a, int n_keys_hint, int n_split, bool choose, void* workspace, size_t workspace_bytes,
                   cudaStream_t s) {
-  const bool tc = (a.n_heads == 64) && !force_simt();
+  const bool tc = (a.n_heads == 64 || a.tree_group > 1) && !force_simt();
   if (n_split <= 0) n_split = attend_splits(a.m, a.n_heads, n_keys_hint, a.window);
   const int64_t rows = (int64_t)a.m * a.n_heads;
   __half* final_out = a.out;
@@ -717,6 +720,8 @@ static bool tree_call(MlaArgs* a, const void* q_lat, const void* tree_kv, const 
   a->m = m; a->n_heads = n_heads; a->scale = scale;
   a->out = (__half*)lat_out;
   a->tree_kv = (const __half*)tree_kv;
+  a->tree_group = tree_group(n_heads);
+  if (m > 0) a->tree_units = tree_units(m, n_seqs, tree_start, a->tree_group);
   a->keep_nan = 1;
   return true;
 }
@@ -726,11 +731,12 @@ namespace hk {
 // splits of a call over the fp16 cache, and whether pairs of CTAs take two nodes each
 static int tree_splits(int m, int n_heads, int n_seqs, bool ragged, int n_keys, bool* pairs) {
   int n_split;
-  if (n_heads != 64 || force_simt()) {
+  const int group = tree_group(n_heads);
+  if (group * n_heads != 64 || force_simt()) {
     *pairs = false;
     return simt_auto_splits(m, n_heads, n_keys);
   }
-  *pairs = mla_tree_shape(m, n_seqs, ragged, n_keys, &n_split);
+  *pairs = mla_tree_shape(m, n_seqs, ragged, group, n_keys, &n_split);
   return n_split;
 }
 }  // namespace hk
@@ -747,10 +753,56 @@ HK_API size_t hk_mla_tree_workspace_bytes(int m, int n_heads, int n_seqs, int n_
   return most > 1 ? hk_mla_partial_bytes(most, (int64_t)m * n_heads) : 0;
 }
 
-HK_API size_t hk_mla8_tree_workspace_bytes(int m, int n_heads, int n_keys) {
-  if (m <= 0 || n_heads < hk::SIMT_HG || n_keys < 0) return 0;
-  int units = 0;
-  return hk::attend8_bytes(m, n_heads, hk::attend8_splits(m, n_heads, hk::tree_keys(true, n_keys), false, &units), 0);
+// The 8-bit cache: as it is, or where that is the faster its positions as fp16 rows in the workspace first, a sequence every `cap` rows.  By a model of the
+// time as in mla_tree_shape: a tile takes 1.3 us of a CTA that converts it, a position 0.35 ns to read and write.
+namespace hk {
+struct Tree8Plan {
+  bool read_first, pairs;
+  int n_split, cap;
+  size_t rows_bytes;
+};
+constexpr int64_t TREE8_ROWS = (int64_t)1 << 20;           // positions that are read first, at most: 1 GB of workspace
+static Tree8Plan tree8_plan(int m, int n_heads, int n_seqs, bool ragged, bool lens, int n_keys, int64_t positions) {
+  Tree8Plan p{};
+  const int group = tree_group(n_heads);
+  const int64_t groups = (n_heads + 63) / 64, units = tree_units(m, n_seqs, ragged, group) * groups;
+  if (force_simt()) {
+    p.n_split = simt_auto_splits(m, n_heads, n_keys);
+    return p;
+  }
+  p.n_split = units > sm_count() ? 1 : mla8_splits((int)units, n_keys);
+  const int64_t cap = lens || positions < n_keys ? positions : n_keys;
+  if (group * n_heads != 64 || cap * n_seqs > TREE8_ROWS) return p;
+  const int64_t sms = sm_count(), tiles = n_keys / 64 + 1;
+  auto time = [&](int64_t u, int s, int tile, int start) {
+    const int64_t waves = (u * s + sms - 1) / sms;
+    return waves * ((tiles + s - 1) / s) * tile + (waves - 1) * 150 + start + (s > 1 ? 6 * u * s : 0);
+  };
+  int s;
+  const bool pairs = mla_tree_shape(m, n_seqs, ragged, group, n_keys, &s);
+  const int64_t u = pairs ? 2 * tree_units(m, n_seqs, ragged, 2) : units;
+  const int64_t read = 300 + (int64_t)n_seqs * n_keys * 35 / 1000;
+  if (read + time(u, s, pairs ? 87 : 100, s == 1 ? (pairs ? 800 : 700) : (pairs ? 950 : 800)) < time(units, p.n_split, 130, p.n_split == 1 ? 700 : 800)) {
+    p.read_first = true;
+    p.pairs = pairs;
+    p.n_split = s;
+    p.cap = (int)cap;
+    p.rows_bytes = (size_t)cap * n_seqs * LATENT * sizeof(__half);
+  }
+  return p;
+}
+}  // namespace hk
+
+HK_API size_t hk_mla8_tree_workspace_bytes(int m, int n_heads, int n_seqs, int n_keys, int64_t positions) {
+  if (m <= 0 || n_heads < hk::SIMT_HG || n_seqs < 1 || n_keys < 0 || positions < 0 || positions > INT32_MAX) return 0;
+  size_t most = 0;
+  for (int k = 0; k < 4; k++) {                            // (whether the trees are ragged and the lengths on the device)
+    if (k < 2 && m % n_seqs != 0) continue;
+    const hk::Tree8Plan p = hk::tree8_plan(m, n_heads, n_seqs, k >= 2, k & 1, hk::tree_keys(k & 1, n_keys), positions);
+    const size_t need = p.rows_bytes + (p.n_split > 1 ? hk_mla_partial_bytes(p.n_split, (int64_t)m * n_heads) : 0);
+    most = most > need ? most : need;
+  }
+  return most;
 }
 
 HK_API int hk_mla_tree(const void* q_lat, const void* ckv, int64_t ckv_rows, const int64_t* kv_base, const int* kv_len, int pos_start,
@@ -779,9 +831,19 @@ HK_API int hk_mla8_tree(const void* q_lat, const void* ckv8, const float* scales
   HK_REQUIRE(tree_call(&a, q_lat, tree_kv, parent, tree_start, n_seqs, kv_len, pos_start, lat_out, m, n_heads, scale));
   HK_REQUIRE(mla8_paged(&pg, ckv8, scales, dtype, n_blocks, block, block_table, table_stride, n_seqs, nullptr));
   if (m == 0) return HK_OK;
-  int units = 0;
   const int keys = tree_keys(kv_len, pos_start);
-  return attend8(a, pg, dtype, keys, n_split > 0 ? n_split : attend8_splits(m, n_heads, keys, false, &units), workspace, workspace_bytes, as_stream(stream));
+  if (n_split > 0) return attend8(a, pg, dtype, keys, n_split, workspace, workspace_bytes, as_stream(stream));
+  const Tree8Plan p = tree8_plan(m, n_heads, n_seqs, tree_start, kv_len, keys, (block_table ? (int64_t)table_stride : n_blocks) * block);
+  if (!p.read_first) return attend8(a, pg, dtype, keys, p.n_split, workspace, workspace_bytes, as_stream(stream));
+  if (!workspace || workspace_bytes < p.rows_bytes) return HK_ERR_WORKSPACE;
+  if (!aligned(workspace, 256)) return HK_ERR_INVALID;
+  const int st = mla8_read_seqs_launch(pg, dtype, kv_len, pos_start, p.cap, keys, (__half*)workspace, as_stream(stream));
+  if (st != HK_OK) return st;
+  a.ckv = (const __half*)workspace;
+  a.ckv_rows = (int64_t)p.cap * n_seqs;
+  a.kv_stride = p.cap;
+  a.tree_pairs = p.pairs;
+  return attend(a, 0, p.n_split, false, (char*)workspace + p.rows_bytes, workspace_bytes - p.rows_bytes, as_stream(stream));
 }
 
 #include "mla_splitkv_heads.cuh"

@@ -94,13 +94,15 @@ struct FtMisc {
   float l[128];
   uint32_t tmem;
   int abort_flag;
-  MlaTree tree;
+  MlaNodes tree;
+  uint64_t paths[MLA_GROUP];
+  uint32_t bad[4];                                // tree form: keys of the tree's tile that are not finite, by warp
 };
 static_assert(sizeof(FtMisc) <= 2048, "misc area");
 
 // One work item: a row and a key split (cluster form: and a part of the output channels).
 struct FtItem {
-  int r, sp, cs, k0, k1, n_tiles;                 // cs: part of the output channels (cluster form)
+  int r, q_row, sp, cs, k0, k1, n_tiles;          // q_row: first of the 64 query rows; cs: part of the output channels (cluster form)
   bool mini;                                      // cluster form: the ragged last tile comes first, from memory of its own
   int64_t base;
   // window form: keys p >= lo and p < head of the row's k1 are seen; tile i of its list is tile i, or i + jump behind the sinks' tiles
@@ -128,6 +130,7 @@ __device__ __forceinline__ FtItem ft_item(const MlaArgs& a, int idx) {
   }
   // rows of a causal chunk grow with their number: the longest first, so that the CTAs end together
   if (!G4 && !a.kv_len) it.r = a.m - 1 - it.r;
+  it.q_row = it.r * FT_HEADS;
   int n;
   it.base = 0;
   if (G4) {
@@ -169,19 +172,20 @@ __device__ __forceinline__ FtItem ft_item(const MlaArgs& a, int idx) {
   return it;
 }
 
-// tree form: the row is the CTA's only one
-__device__ __forceinline__ FtItem ft_tree_item(const MlaArgs& a, const MlaTree& tree, int idx) {
+// tree form: the nodes are the CTA's only ones
+__device__ __forceinline__ FtItem ft_tree_item(const MlaArgs& a, const MlaNodes& tree, int idx) {
   FtItem it;
   it.win = it.mini = false;
   it.sp = idx % a.n_split;
   it.r = idx / a.n_split;
+  it.q_row = (tree.row0 + tree.node) * a.n_heads;
   it.cs = 0;
   it.base = tree.base;
   it.k0 = 0;
   it.k1 = tree.len;
   it.past = tree.len / FT_KEYS + (tree.len % FT_KEYS != 0);
-  it.nodes = tree.node + 1;
-  const int tiles = tree.node < 0 ? 0 : it.past + 1, per = (tiles + a.n_split - 1) / a.n_split;
+  it.nodes = tree.node + tree.count;
+  const int tiles = tree.seq < 0 ? 0 : it.past + 1, per = (tiles + a.n_split - 1) / a.n_split;
   it.t0 = min(tiles, it.sp * per);
   it.n_tiles = min(tiles, it.t0 + per) - it.t0;
   return it;
@@ -223,8 +227,9 @@ __device__ __forceinline__ void tma_gather4_rows(uint32_t leader, uint32_t smem_
 // 9.2 us; MLA layer of one token at 5,001 32.1 -> 28.9, selection and attention at 262,144 23.8 -> 21.8.
 // WIN: dense ranges of which a row sees its last keys and its first ones only (a.window, a.sinks).
 // PARTS: CTAs that share a partial's output channels, each with the scores for itself (few splits of few rows: 128 KB of a partial take 3 us).
-// TREE: a row is a node of a tree of drafted tokens (a.tree).  The tree's tile is the last of the row's list: of its 64 slots those on the node's
-// path are gathered out of a.tree_kv (tmap_tree), the others are zeros, whatever lies there.  (As a box whose unseen rows are cleared ahead of P V, as
+// TREE: the 64 query rows are the heads of a node of a tree of drafted tokens (a.tree), or of 64 / heads neighbouring nodes where a GPU has 4 to 32 heads.
+// The tree's tile is the last of the list: of its 64 slots those on the nodes' paths are gathered out of a.tree_kv (tmap_tree), the others are zeros,
+// whatever lies there; each head's row sees those on its own node's.  (As a box whose unseen rows are cleared ahead of P V, as
 // mla_pair_tree_tc_kernel takes it, this tile and a ragged one were no faster here, and the look at the mask cost long rows 3 %.)
 template <bool G4, bool CL, bool WIN, int PARTS, bool TREE>
 __device__ __forceinline__ void ft_body(const MlaArgs& a, int* __restrict__ status, const CUtensorMap& tmap_box, const CUtensorMap& tmap_rows,
@@ -238,7 +243,7 @@ __device__ __forceinline__ void ft_body(const MlaArgs& a, int* __restrict__ stat
   const int tid = threadIdx.x, lane = tid & 31;
   // provably warp-uniform role index: the issuing warps' branches stay converged for the compiler
   const int warp = tc::warp_index_uniform();
-  const int n_items = CL ? gridDim.x : PARTS * a.n_split * a.m, step = gridDim.x;
+  const int n_items = CL || TREE ? gridDim.x : PARTS * a.n_split * a.m, step = gridDim.x;
   // A CTA with one item of at most two tiles (a decode split) never needs Q's ring slot back: S reads Q from there, and the
   // 0.6 us of moving it are saved.  In the cluster form Q always stays and the other two slots serve all tiles.
   bool direct_q = CL;
@@ -270,8 +275,9 @@ __device__ __forceinline__ void ft_body(const MlaArgs& a, int* __restrict__ stat
   };
   if constexpr (TREE) {
     if (warp == 0) {
-      const MlaTree t = mla_tree(a, blockIdx.x / (PARTS * a.n_split));
+      const MlaNodes t = mla_nodes(a, blockIdx.x / (PARTS * a.n_split));
       if (lane == 0) ms.tree = t;
+      if (lane < MLA_GROUP) ms.paths[lane] = t.mine;
     }
   } else {
     if (!CL && step >= n_items) direct_q = item(blockIdx.x).n_tiles < FT_NBUF;
@@ -297,7 +303,7 @@ __device__ __forceinline__ void ft_body(const MlaArgs& a, int* __restrict__ stat
     // cache row of key slot lw * SLOTS + lane of a tile, -1 = hole; volatile, so that a look-ahead load is issued where it stands
     auto row_of = [&](const FtItem& it, int tile) -> int {
       const int slot = lw * FT_SLOTS + lane, p = it.key0(tile) + slot;
-      if (TREE && it.drafted(tile)) return lane < FT_SLOTS && (ms.tree.path >> slot & 1) ? ms.tree.row0 + slot : -1;
+      if (TREE && it.drafted(tile)) return lane < FT_SLOTS && (ms.tree.any >> slot & 1) ? ms.tree.row0 + slot : -1;
       if (lane >= FT_SLOTS || p >= it.k1 || !it.sees(p)) return -1;
       if (!G4) return (int)(it.base + p);
       int v;
@@ -339,7 +345,7 @@ __device__ __forceinline__ void ft_body(const MlaArgs& a, int* __restrict__ stat
         if (lane == 0) {
           if (lw == 0) {
             tc::mbar_arrive_expect_tx(&ms.full[b], FT_TILE);
-            tma_load_tile(smem + FS_K + b * FT_TILE, &tmap_q, it.r * FT_HEADS, &ms.full[b]);
+            tma_load_tile(smem + FS_K + b * FT_TILE, &tmap_q, it.q_row, &ms.full[b]);
           } else {
             tc::mbar_arrive(&ms.full[b]);
           }
@@ -539,7 +545,27 @@ __device__ __forceinline__ void ft_body(const MlaArgs& a, int* __restrict__ stat
         tc::tmem_ld_wait();
         tc::fence_before_sync();
         tc::mbar_arrive(&ms.s_free[b]);
-        const uint32_t mask = *reinterpret_cast<const uint32_t*>(&ms.mask[kb][4 * half]);
+        uint32_t mask = *reinterpret_cast<const uint32_t*>(&ms.mask[kb][4 * half]);
+        if (TREE && a.tree_group > 1 && it.drafted(tile)) {
+          // Several nodes' rows, a product for all of them: a weight of nothing would not keep one node's infinities and NaN out of another.  A key that is
+          // not finite has no finite score with any row; it leaves the tile, and the rows that do see it become NaN by their weights.
+          uint32_t bad = 0;
+#pragma unroll
+          for (int j = 0; j < 32; j++) bad |= fabsf(__uint_as_float(sv[j])) < INFINITY ? 0u : 1u << j;
+          bad = __reduce_and_sync(0xffffffffu, bad);
+          if (lane == 0) ms.bad[warp] = bad;
+          asm volatile("bar.sync 3, 128;" ::: "memory");
+          mask = (uint32_t)(ms.paths[head / a.n_heads] >> (32 * half));
+          bad = ms.bad[2 * half] & ms.bad[2 * half + 1];
+#pragma unroll
+          for (int j = 0; j < 32; j++)
+            if (bad >> j & 1) sv[j] = 0x7fffffffu;
+          if (ms.bad[head >> 4 & 2] & ms.bad[(head >> 4 & 2) + 1] & 1u << (head & 31)) {   // key `head` of the tile, half of its channels
+            uint8_t* key = smem + tile_at(kb) + half * 4 * FT_BLK + head * 128;
+#pragma unroll
+            for (int c = 0; c < 32; c++) *reinterpret_cast<uint4*>(key + (c >> 3) * FT_BLK + (((c + lane) & 7) << 4)) = make_uint4(0u, 0u, 0u, 0u);
+          }
+        }
         float tmax = -INFINITY;
 #pragma unroll
         for (int j = 0; j < 32; j++) {
@@ -646,6 +672,27 @@ __device__ __forceinline__ void ft_body(const MlaArgs& a, int* __restrict__ stat
                            cluster_addr(tc::smem_u32(smem + FS_K) + it.sp * share, tid)),
                        "r"(tc::smem_u32(smem + FS_K + FT_CL_STAGE) + tid * share), "r"(share), "r"(cluster_addr(tc::smem_u32(&ms.q_ready), tid))
                        : "memory");
+      } else if (TREE && final_out && a.tree_group > 1) {
+        // rows of the nodes that there are, straight from the accumulator
+        const bool mine = head < ms.tree.count * a.n_heads && ok && !*abort_flag;
+        uint8_t* row = reinterpret_cast<uint8_t*>(a.out + ((size_t)it.q_row + head) * LATENT);
+#pragma unroll 1
+        for (int c0 = 0; c0 < 256; c0 += 32) {
+          uint32_t o[32];
+          load_o(c0, o);                                   // (whole warps)
+          const int ch = (c0 >> 7) * 256 + half * 128 + (c0 & 127);
+#pragma unroll
+          for (int v = 0; v < 4; v++) {
+            uint4 w;
+            uint32_t* wp = &w.x;
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+              const __half2 h2 = __floats2half2_rn(__uint_as_float(o[8 * v + 2 * e]), __uint_as_float(o[8 * v + 2 * e + 1]));
+              wp[e] = *reinterpret_cast<const uint32_t*>(&h2);
+            }
+            if (mine) *reinterpret_cast<uint4*>(row + ch * 2 + v * 16) = w;
+          }
+        }
       } else if (final_out) {
         // Four rounds of 2 x 64 channels through the P buffers: channels 256 (c0 / 128) + 128 half + c0 % 128 ... of all heads
         // as a swizzled box each.
@@ -676,7 +723,7 @@ __device__ __forceinline__ void ft_body(const MlaArgs& a, int* __restrict__ stat
 #pragma unroll
             for (int hf = 0; hf < 2; hf++)
               asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%1, %2}], [%3];" ::"l"(&tmap_o),
-                           "r"((c0 >> 7) * 256 + hf * 128 + (c0 & 127)), "r"(it.r * FT_HEADS), "r"(tc::smem_u32(smem + FS_P + hf * FP_BYTES))
+                           "r"((c0 >> 7) * 256 + hf * 128 + (c0 & 127)), "r"(it.q_row), "r"(tc::smem_u32(smem + FS_P + hf * FP_BYTES))
                            : "memory");
             tc::bulk_commit();
           }
@@ -701,8 +748,8 @@ __device__ __forceinline__ void ft_body(const MlaArgs& a, int* __restrict__ stat
         }
         tc::fence_async_smem();
         asm volatile("bar.sync 3, 128;" ::: "memory");
-        const size_t rows = (size_t)a.m * FT_HEADS, rh = (size_t)it.r * FT_HEADS + head;
-        if (half == 0 && ok && !*abort_flag) {
+        const size_t rows = (size_t)a.m * a.n_heads, rh = (size_t)it.q_row + head;
+        if (half == 0 && ok && !*abort_flag && (!TREE || head < ms.tree.count * a.n_heads)) {
           tc::bulk_s2g(a.part_acc + ((size_t)it.sp * rows + rh) * LATENT + part * n_ch, orow, n_ch * 4);
           tc::bulk_commit();
           if (part == 0) {
@@ -793,20 +840,18 @@ int mla_flash_tc_auto_splits(int m, int n_keys) {
   return n_split < 1 ? 1 : n_split;
 }
 
-// pairs of nodes that m rows of n_seqs trees make at most (ragged: trees of any sizes)
-static int64_t mla_tree_pairs(int m, int n_seqs, bool ragged) { return ragged ? ((int64_t)m + n_seqs) / 2 : (int64_t)n_seqs * ((m / n_seqs + 1) / 2); }
-// Form and splits of a tree call: a CTA a node or a pair of CTAs for two, each key range in n_split parts.  A model of the time in units of 10 ns, fitted to
+// Form and splits of a tree call: a CTA a node (or `group` of them) or a pair of CTAs for two, each key range in n_split parts.  A model of the time in units of 10 ns, fitted to
 // 13 shapes with 1 to 36 splits (1 x 2 to 64 nodes at 500 to 32,768 keys, 2 to 16 sequences): a tile takes 1.0 us of a single CTA, 0.87 of a pair (48 KB
 // instead of 64 for each, half the reads of the products); a call 7 and 8, with partials and their merge 8 and 9.5 and 0.06 a partial of 64 heads; another
 // wave 1.5.  us, single / pair at the best number of splits: 2 nodes at 5,001 keys 13.5 / 15.7, 8 18.4 / 18.9, 64 at 2,000 37.0 / 34.8, 16 at 32,768 70.8 /
 // 63.6, 64 266 / 235, 6 x 16 at 10,000 118 / 101, 16 x 8 at 8,000 122 / 106.
-bool mla_tree_shape(int m, int n_seqs, bool ragged, int n_keys, int* n_split) {
+bool mla_tree_shape(int m, int n_seqs, bool ragged, int group, int n_keys, int* n_split) {
   const int64_t tiles = n_keys / FT_KEYS + 2, sms = sm_count();
   int64_t best = 0;
   bool pairs = false;
   *n_split = 1;
-  for (int form = 0; form < 2; form++) {
-    const int64_t units = form ? 2 * mla_tree_pairs(m, n_seqs, ragged) : m;
+  for (int form = 0; form < (group == 1 ? 2 : 1); form++) {
+    const int64_t units = form ? 2 * tree_units(m, n_seqs, ragged, 2) : tree_units(m, n_seqs, ragged, group);
     for (int s = 1; s <= 256 && (s == 1 || (2 * s <= tiles + 1 && units * s <= 4 * sms)); s++) {
       const int64_t waves = (units * s + sms - 1) / sms, per = (tiles + s - 1) / s;
       const int64_t time = waves * per * (form ? 87 : 100) + (waves - 1) * 150 + (s == 1 ? (form ? 800 : 700) : (form ? 950 : 800) + 6 * units * s);
@@ -902,7 +947,7 @@ bool mla_rows_map(CUtensorMap* m, const void* rows, int64_t n) {
 
 int mla_flash_tc_launch(const MlaArgs& a, cudaStream_t s, bool clusters) {
   FtEncodeFn encode = ft_encode_fn();
-  if (a.n_heads != FT_HEADS || !encode) return HK_ERR_UNSUPPORTED;
+  if ((a.n_heads != FT_HEADS && !(a.tree_kv && a.tree_group * a.n_heads == FT_HEADS)) || !encode) return HK_ERR_UNSUPPORTED;
   if (ft_prepare() != HK_OK) return HK_ERR_CUDA;
   // Tensor maps over the latent cache.  The row extent is the cache's row count when the caller gave it (the copy engine
   // zero-fills anything past the end), else an upper bound.
@@ -931,7 +976,7 @@ int mla_flash_tc_launch(const MlaArgs& a, cudaStream_t s, bool clusters) {
                   CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
   };
   static_assert(FT_KEYS == 64 && FT_HEADS == 64, "one box shape for keys and queries");
-  const cuuint64_t q_rows = (cuuint64_t)a.m * FT_HEADS;
+  const cuuint64_t q_rows = (cuuint64_t)a.m * a.n_heads;
   // Two rows of a causal chunk share their keys.  Below 700 keys a row on average the pair's own costs (a cluster to start, the later row's own
   // key as a tile) are more than it gains: us, a CTA a row / pairs, 148 rows at 300 15.3 / 15.4, at 600 19.7 / 19.5, at 1,000 25.5 / 24.2;
   // 500 at 300 65.7 / 67.8, at 700 89.7 / 86.5; 1,200 at 0 151 / 154, 1,500 209 / 208, 2,500 470 / 431.
@@ -957,7 +1002,7 @@ int mla_flash_tc_launch(const MlaArgs& a, cudaStream_t s, bool clusters) {
     if (!box_map(&box, a.ckv, extent, 32, 8) || !box_map(&vbox, a.ckv, extent, 32, 4) || !box_map(&tree_k, a.tree_kv, a.m, 32, 8) ||
         !box_map(&tree_v, a.tree_kv, a.m, 32, 4))
       return HK_ERR_UNSUPPORTED;
-    const int64_t n_pairs = mla_tree_pairs(a.m, a.tree.n_seqs, a.tree.start != nullptr);
+    const int64_t n_pairs = tree_units(a.m, a.tree.n_seqs, a.tree.start, 2);
     const cudaError_t e = pdl_launch_cluster(2, mla_pair_tree_tc_kernel, dim3((unsigned)(2 * n_pairs * a.n_split)), dim3(PT_THREADS), FS_SMEM, s, a, device_status_ptr(), box, vbox,
                                              rows, qmap, omap, tree_k, tree_v);
     return e == cudaSuccess && cudaPeekAtLastError() == cudaSuccess ? HK_OK : HK_ERR_CUDA;
@@ -979,7 +1024,7 @@ int mla_flash_tc_launch(const MlaArgs& a, cudaStream_t s, bool clusters) {
   }
   // A window's few splits of few rows: the output channels of each over two or four CTAs (one row under 3,000 / 4,096 / 8,192
   // keys 12.1 / 12.8 / 14.5 -> 9.9 / 10.6 / 11.6 us with the merge, four under 1,024 11.5 -> 9.4).
-  const int64_t splits = (int64_t)a.n_split * a.m;
+  const int64_t splits = (int64_t)a.n_split * (a.tree_kv ? a.tree_units : a.m);
   const int parts = a.out || (a.window <= 0 && !a.tree_kv) || 2 * splits > sm_count() ? 1 : 4 * splits > sm_count() ? 2 : 4;
   const int64_t items = splits * parts;
   const dim3 grid((unsigned)((a.raw_idx || a.window > 0) && a.out && items > sm_count() ? sm_count() : items));

@@ -46,33 +46,6 @@ struct PtMisc {
 };
 static_assert(sizeof(PtMisc) <= 2048, "misc area");
 
-// Nodes of pair `pair` of a tree call: pairs of sequence after sequence; row < 0: no such pair.  Executed by a whole warp.
-struct PtPair {
-  int row;
-  bool lone;
-};
-__device__ __forceinline__ PtPair pt_pair(const TreeArgs& tree, int pair) {
-  const int lane = threadIdx.x & 31;
-  int before = 0;
-  for (int s0 = 0; s0 < tree.n_seqs; s0 += 32) {
-    const int2 rows = s0 + lane < tree.n_seqs ? tree.rows(s0 + lane) : make_int2(0, 0);
-    const int mine = (rows.y + 1) / 2;
-    int sum = mine;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int x = __shfl_up_sync(0xffffffffu, sum, o);
-      if (lane >= o) sum += x;
-    }
-    const uint32_t who = __ballot_sync(0xffffffffu, pair < before + sum && pair >= before + sum - mine);
-    if (who) {
-      const int at = __ffs(who) - 1, k = pair - __shfl_sync(0xffffffffu, before + sum - mine, at);
-      return {__shfl_sync(0xffffffffu, rows.x, at) + 2 * k, 2 * k + 1 == __shfl_sync(0xffffffffu, rows.y, at)};
-    }
-    before += __shfl_sync(0xffffffffu, sum, 31);
-  }
-  return {-1, true};
-}
-
 __device__ __forceinline__ void pt_tma_box(void* smem_dst, const CUtensorMap* tmap, int row, int blk, uint64_t* bar) {
   asm volatile(
       "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(
@@ -171,10 +144,10 @@ __device__ __forceinline__ void pt_body(const MlaArgs& a, int* __restrict__ stat
   if (TREE) {
     split = (int)(blockIdx.x >> 1) % a.n_split;
     pdl_wait();
-    const PtPair p = pt_pair(a.tree, (int)(blockIdx.x >> 1) / a.n_split);
-    if (p.row < 0) return;                                 // (both CTAs, before anything of them is in use)
-    r0 = p.row;
-    lone = p.lone;
+    const TreeUnit p = tree_unit(a.tree, (int)(blockIdx.x >> 1) / a.n_split, 2);
+    if (p.seq < 0) return;                                 // (both CTAs, before anything of them is in use)
+    r0 = p.row0 + p.node;
+    lone = p.count < 2;
     r1 = lone ? r0 : r0 + 1;
     if (warp < 2) {
       const MlaTree t = mla_tree(a, warp == 0 ? r0 : r1);

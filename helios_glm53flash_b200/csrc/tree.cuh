@@ -36,6 +36,32 @@ struct TreeArgs {
   }
 };
 
+// Neighbouring nodes of a tree, `group` at a time, sequence after sequence: the unit-th such group.  seq < 0: there are fewer.  Executed by a whole warp.
+struct TreeUnit {
+  int seq, row0, node, count;                              // the tree's first row; its first node in the group, and how many
+};
+__device__ __forceinline__ TreeUnit tree_unit(const TreeArgs& t, int unit, int group) {
+  const int lane = threadIdx.x & 31;
+  int before = 0;
+  for (int s0 = 0; s0 < t.n_seqs; s0 += 32) {
+    const int2 rows = s0 + lane < t.n_seqs ? t.rows(s0 + lane) : make_int2(0, 0);
+    const int mine = (rows.y + group - 1) / group;
+    int sum = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int x = __shfl_up_sync(0xffffffffu, sum, o);
+      if (lane >= o) sum += x;
+    }
+    const uint32_t who = __ballot_sync(0xffffffffu, unit < before + sum && unit >= before + sum - mine);
+    if (who) {
+      const int at = __ffs(who) - 1, node = (unit - __shfl_sync(0xffffffffu, before + sum - mine, at)) * group;
+      return {s0 + at, __shfl_sync(0xffffffffu, rows.x, at), node, min(group, __shfl_sync(0xffffffffu, rows.y, at) - node)};
+    }
+    before += __shfl_sync(0xffffffffu, sum, 31);
+  }
+  return {-1, 0, 0, 0};
+}
+
 // The paths of a tree's nodes - a node and its ancestors, a bit each - nodes lane and lane + 32 in a lane.  By doubling: after round r a node has its
 // 2^r nearest ancestors and knows the next one up; a chain of 64 takes six rounds, a tree that is eight deep three.
 struct TreePaths {
@@ -75,6 +101,11 @@ __device__ __forceinline__ uint64_t tree_path(const TreeArgs& t, int2 rows, int 
   TreePaths paths;
   paths.load(t, rows);
   return paths.of(leaf);
+}
+
+// host: groups that m rows of n_seqs trees make at most (ragged: trees of any sizes)
+inline int64_t tree_units(int m, int n_seqs, bool ragged, int group) {
+  return ragged ? ((int64_t)m + (int64_t)n_seqs * (group - 1)) / group : (int64_t)n_seqs * ((m / n_seqs + group - 1) / group);
 }
 
 // host: arguments of a tree call; without rows there need be no arrays of rows

@@ -579,17 +579,19 @@ int hk_mla_decode_prologue(const float* kv_pre, const void* ln_w_f16, void* ckv,
 /* Attention of nodes over the fp16 cache: a row attends to the first kv_len[s] cached rows of its sequence (kv_len [n_seqs]; NULL: pos_start for
  * all; they begin at kv_base[s], NULL: 0) and to its path's rows of tree_kv [m][512] f16 (its ancestors' and its own latents; 16-byte aligned).  Other
  * nodes' rows have no effect, whatever they hold.  Rows of no tree are left as they were.  With kv_len, pos_start says about how many keys the longest
- * sequence has (0: 4,096; it chooses the splits, no more).  Other arguments as in hk_mla_dense.  Heads other than 64 (multiples of 4) run on the CUDA
- * cores, up to 65,535 rows a call.  A key that is not finite and that a row sees shows as in hk_mla_window.
+ * sequence has (0: 4,096; it chooses the splits, no more).  Other arguments as in hk_mla_dense.  n_heads: a multiple of 4; other than 4, 8, 16, 32
+ * and 64 run on the CUDA cores, up to 65,535 rows a call.  A key that is not finite and that a row sees shows as in hk_mla_window.
  * Workspace: hk_mla_tree_workspace_bytes(m, n_heads, n_seqs, pos_start), or hk_mla_partial_bytes(n_split, m * n_heads) for n_split > 1.               */
 size_t hk_mla_tree_workspace_bytes(int m, int n_heads, int n_seqs, int n_keys);
 int hk_mla_tree(const void* q_lat, const void* ckv, int64_t ckv_rows, const int64_t* kv_base, const int* kv_len, int pos_start,
                 const void* tree_kv, const int* parent, const int* tree_start, int n_seqs, void* lat_out, int m, int n_heads, float scale,
                 int n_split, void* workspace, size_t workspace_bytes, void* stream);
 
-/* The same over the 8-bit paged cache (block_table NULL: one sequence), positions without a block hold no key; tree_kv is fp16 here too: drafts that
- * are not accepted never touch the cache.  n_heads: a multiple of 4.  Precision as in hk_mla8_dense.                                     */
-size_t hk_mla8_tree_workspace_bytes(int m, int n_heads, int n_keys);
+/* The same over the 8-bit paged cache (block_table NULL: one sequence); tree_kv is fp16 here too: drafts that are not accepted never touch the cache.
+ * Positions behind the table hold no key, one whose entry names no block is a latent of zeros, as in a chunk of hk_mla8_dense.  n_heads: a multiple of 4.
+ * Precision as in hk_mla8_dense; where many nodes share the keys the call reads the positions as fp16 rows into the workspace first, as a chunk there.
+ * Workspace: hk_mla8_tree_workspace_bytes, positions: table_stride * block, or n_blocks * block without a table.                             */
+size_t hk_mla8_tree_workspace_bytes(int m, int n_heads, int n_seqs, int n_keys, int64_t positions);
 int hk_mla8_tree(const void* q_lat, const void* ckv8, const float* scales, int dtype, int64_t n_blocks, int block, const int* block_table,
                  int table_stride, const int* kv_len, int pos_start, const void* tree_kv, const int* parent, const int* tree_start,
                  int n_seqs, void* lat_out, int m, int n_heads, float scale, int n_split, void* workspace, size_t workspace_bytes,

@@ -47,7 +47,7 @@ def wanted(q, past, tree_kv, first, tree, scale):
     (["star7", "two_roots", "one"], [0, 129, 1000]), ([(31, 1), (8, 2), (64, 3), (1, 4)], [500, 64, 3, 128]), ([(64, 5)], [2500]), ([(5, 6)] * 9, [777] * 9),
     ([(16, 7)], [4100]), (["chain5", [], "chain5"], [40, 50, 60]),
 ])
-@pytest.mark.parametrize("heads,n_split", [(64, 0), (64, 1), (64, 3), (16, 0), (4, 2)])
+@pytest.mark.parametrize("heads,n_split", [(64, 0), (64, 1), (64, 3), (16, 0), (32, 2), (8, 1), (4, 5), (20, 0), (128, 2)])
 def test_nodes_over_the_fp16_cache(trees, lens, heads, n_split):
     trees = [tree_of(t) for t in trees]
     gen = gen_of(len(trees) + sum(lens))
@@ -71,6 +71,8 @@ def test_nodes_over_the_fp16_cache(trees, lens, heads, n_split):
 @pytest.mark.parametrize("trees,lens,heads,n_split", [
     (["one"], [0], 64, 0), (["binary15"], [64], 64, 0), (["wide63", "chain5"], [65, 1000], 64, 0), ([(31, 1), (64, 2), (1, 3)], [500, 3, 128], 16, 0),
     ([(12, 5)], [3000], 64, 0), (["star7"], [700], 20, 3), (["chain64"], [200], 128, 1), ([(5, 6)] * 9, [777] * 9, 64, 2),
+    (["chain64", (60, 3), "one"], [3000, 2100, 900], 64, 0), (["chain5"] * 12, [3000 - 100 * i for i in range(12)], 16, 0), ([(64, 3)] * 3, [2000, 1999, 300], 32, 0),
+    (["star7", "one"], [90, 0], 4, 2),
 ])
 def test_nodes_over_the_8_bit_cache(kind, block, trees, lens, heads, n_split):
     trees = [tree_of(t) for t in trees]
@@ -88,15 +90,38 @@ def test_nodes_over_the_8_bit_cache(kind, block, trees, lens, heads, n_split):
     want = []
     for s in range(n):
         past = rows_of(ckv8, scales, table[s], torch.arange(lens[s], device="cuda"))
-        want += [attend(q[starts[s] + j].double(), torch.cat((past, tree_kv[[starts[s] + i for i in path(trees[s], j)]].double())), 0.0625) for j in
-                 range(len(trees[s]))]
+        # (many nodes over many keys: the positions are rounded to fp16 rows first)
+        want += [attend(q[starts[s] + j].double(), torch.cat((past, tree_kv[[starts[s] + i for i in path(trees[s], j)]].double())), 0.0625, rows16=m * max(lens) > 100000)
+                 for j in range(len(trees[s]))]
     check_rows(out, want)
 
 
-@pytest.mark.parametrize("over", ["f16", "i8", "f16 of 4 heads"])
+@pytest.mark.parametrize("nodes,stride", [(3, 30), (64, 30), (64, 60)])
+def test_positions_without_a_block_and_behind_the_table(nodes, stride):
+    """an entry that names no block is a latent of zeros, positions behind the table are none; the same whether the positions are read first or not"""
+    gen, block = gen_of(9), 64
+    ckv8, scales = cache(gen, "i8", 64, block)
+    table = table_for(gen, 1, stride, 64)
+    table[0, 3], table[0, 11] = -1, 64
+    q, rows, tree = (randn(gen, nodes, 64, 512) * 0.7).half(), randn(gen, nodes, 512).half(), list(range(-1, nodes - 1))
+    out = torch.full((nodes, 64, 512), 7.0, dtype=torch.float16, device="cuda")
+    n = stride * block + 500 if stride < 60 else stride * block - 37
+    hk.mla8_tree_decode(q, ckv8, scales, rows, ints(tree), out, nodes, block_table=table, kv_len=ints([n]), n_keys_hint=n)
+    also = torch.empty_like(out)
+    hk.mla8_tree_decode(q, ckv8, scales, rows, ints(tree), also, nodes, n, block_table=table)
+    finish()
+    p = torch.arange(min(n, stride * block), device="cuda")
+    named = torch.where((table[0] >= 0) & (table[0] < 64), table[0], 0).long()[p // block]
+    past = ref8.as_f64(ckv8.view(torch.uint8)[named, p % block].view(ckv8.dtype)) * scales[named].double()[:, None]
+    past[(p // block == 3) | (p // block == 11)] = 0
+    for got in (out, also):
+        check_rows(got, [attend(q[j].double(), torch.cat((past, rows[:j + 1].double())), 0.0625, rows16=True) for j in range(nodes)])
+
+
+@pytest.mark.parametrize("over", ["f16", "i8", "f16 of 4", "f16 of 16", "f16 of 32", "f16 of 20", "i8 of 16", "i8 of 8", "i8 of 20"])
 def test_what_a_node_does_not_see_has_no_effect(over):
     """NaN and infinities in other branches, in rows of no tree and behind a sequence's keys; a key that is not finite shows in the rows that see it"""
-    heads = 4 if "4" in over else 64
+    heads = int(over.split(" of ")[1]) if " of " in over else 64
     tree = tree_of("binary15")
     gen = gen_of(3)
     starts, parent, tree_start = layout([tree, tree], front=2)
@@ -115,7 +140,7 @@ def test_what_a_node_does_not_see_has_no_effect(over):
     def call(rows):
         out = torch.full((m, heads, 512), 7.0, dtype=torch.float16, device="cuda")
         tree_args = dict(n_seqs=2, tree_start=tree_start, kv_len=ints([n, n]), n_heads=heads, n_keys_hint=n)
-        if over == "i8":
+        if over.startswith("i8"):
             hk.mla8_tree_decode(q, ckv8, scales, rows, parent, out, m, block_table=table, **tree_args)
         else:
             hk.mla_tree_decode(q, ckv, rows, parent, out, m, kv_base=torch.tensor(base, device="cuda"), **tree_args)

@@ -56,7 +56,7 @@ def test_empty_calls_and_workspaces(lib):
             for heads in (4, 64):
                 need = lib.hk_mla_tree_workspace_bytes(m, heads, 3, keys)
                 assert need == 0 or need >= lib.hk_mla_partial_bytes(2, m * heads)
-            assert lib.hk_mla8_tree_workspace_bytes(m, 64, keys) >= 0
+            assert lib.hk_mla8_tree_workspace_bytes(m, 64, 3, keys, 1 << 17) >= 0
     assert lib.hk_mla8_pages_workspace_bytes(0, 4) == 0 and lib.hk_mla8_pages_workspace_bytes(8, -1) == 0
     assert lib.hk_mla8_pages_workspace_bytes(1000, 5) >= 3 * 4000 and lib.hk_mla8_pages_workspace_bytes(5, 1000) >= 3 * 4000
 
