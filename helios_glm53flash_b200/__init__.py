@@ -670,15 +670,10 @@ def kda_tree_accept(x32, conv_state, mixed_qkv, g, beta, rec_state, parent, leaf
 
 # ---- pages of the 8-bit cache: refs [n_blocks] int32 counts the entries of block_table [n_seqs, blocks of a sequence] that name a block.  A pool begins
 # with refs 0 and a table of -1.  missing, n_live: optional device int32 [1] ----
-def _pages(ckv8, scales, refs, block_table, types, names, *tensors):
-    tag, n_blocks, block, stride, seqs = _native.cache8(ckv8, scales, block_table, "i" + types, ("refs",) + names, refs, ckv8.shape[0], *tensors)
-    if block_table is None:
-        raise ValueError("block_table: needed")
-    return ckv8, scales, tag, n_blocks, block, refs, block_table, stride, seqs
-
-
-def _pages_scratch(ckv8, n, workspace, stream):
-    return _scratch_like(_native.hk_mla8_pages_workspace_bytes(ckv8.shape[0], n), ckv8, stream) if workspace is None else workspace
+def _pages(name, op, *args):
+    st = _native.pages(op, *args)
+    if st:
+        raise HeliosB200Error(name, st)
 
 
 def mla8_pages_workspace_bytes(n_blocks, n=0):
@@ -687,28 +682,22 @@ def mla8_pages_workspace_bytes(n_blocks, n=0):
 
 def mla8_pages_fork(ckv8, scales, refs, block_table, parents, children, lens, n, missing=None, workspace=None, stream=None):
     """n sequences `children` take over the first lens[i] positions of `parents` (hk_mla8_pages_fork): whole blocks shared, the last one copied"""
-    pool = _pages(ckv8, scales, refs, block_table, "iiii", ("parents", "children", "lens", "missing"), parents, n, children, n, lens, n, missing, 1)
-    ws = _pages_scratch(ckv8, n, workspace, stream)
-    _run("hk_mla8_pages_fork", *pool, parents, children, lens, n, missing, ws, ws, stream)
+    _pages("hk_mla8_pages_fork", 0, ckv8, scales, refs, block_table, parents, children, lens, n, missing, workspace, stream)
 
 
 def mla8_pages_reserve(ckv8, scales, refs, block_table, seqs, lens, n, missing=None, workspace=None, stream=None):
     """n sequences get a free block for every entry of their first lens[i] positions that names none (hk_mla8_pages_reserve)"""
-    pool = _pages(ckv8, scales, refs, block_table, "iii", ("seqs", "lens", "missing"), seqs, n, lens, n, missing, 1)
-    ws = _pages_scratch(ckv8, n, workspace, stream)
-    _run("hk_mla8_pages_reserve", *pool, seqs, lens, n, missing, ws, ws, stream)
+    _pages("hk_mla8_pages_reserve", 1, ckv8, scales, refs, block_table, seqs, lens, None, n, missing, workspace, stream)
 
 
 def mla8_pages_free(ckv8, scales, refs, block_table, seqs, keep, n, stream=None):
     """n sequences give back the blocks behind their first keep[i] positions (keep None: all of them)"""
-    _run("hk_mla8_pages_free", *_pages(ckv8, scales, refs, block_table, "ii", ("seqs", "keep"), seqs, n, keep, n), seqs, keep, n, stream)
+    _pages("hk_mla8_pages_free", 2, ckv8, scales, refs, block_table, seqs, keep, None, n, None, None, stream)
 
 
 def mla8_pages_compact(ckv8, scales, refs, block_table, n_live=None, workspace=None, stream=None):
     """the live blocks become the pool's first ones (hk_mla8_pages_compact)"""
-    pool = _pages(ckv8, scales, refs, block_table, "i", ("n_live",), n_live, 1)
-    ws = _pages_scratch(ckv8, 0, workspace, stream)
-    _run("hk_mla8_pages_compact", *pool, n_live, ws, ws, stream)
+    _pages("hk_mla8_pages_compact", 3, ckv8, scales, refs, block_table, None, None, None, 0, n_live, workspace, stream)
 
 
 def mla8_pages_copy(ckv8, scales, to_ckv8, to_scales, src, dst, n, stream=None):

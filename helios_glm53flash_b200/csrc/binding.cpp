@@ -345,6 +345,61 @@ PyObject* py_append8(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
   }
 }
 
+// pages(op, ckv8, scales, refs, block_table, list, list, list, n, told, workspace or None, stream): the checks, the scratch and one of the calls on pages in one
+// call (op 0: fork of children from parents with lens; 1: reserve for seqs with lens; 2: free of seqs with keep; 3: compact).  us of host time a fork
+// as calls from Python 8.9, here 4.3.
+PyObject* py_pages(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
+  if (n_args != 12 || !p_hk_mla8_pages_fork) {
+    bad_arg("pages: 12 arguments, of a bound binding");
+    return nullptr;
+  }
+  try {
+    const int device = device_now();
+    Cache8 c;
+    int op, n, *refs, *table, *told;
+    const int* list[3];
+    void *ckv8, *stream;
+    float* scales;
+    PyObject* const cache[3] = {args[1], args[2], args[4]};
+    static const char* const names[4][3] = {{"parents", "children", "lens"}, {"seqs", "lens", ""}, {"seqs", "keep", ""}, {"", "", ""}};
+    if (!convert(args[0], op) || op < 0 || op > 3) return PyErr_Occurred() ? nullptr : (bad_arg("pages: op 0 to 3"), nullptr);
+    if (!convert(args[8], n) || !cache8_of(cache, device, c)) return nullptr;
+    if (args[4] == Py_None) {
+      PyErr_SetString(PyExc_ValueError, "block_table: needed");
+      return nullptr;
+    }
+    if (!check_tensor(args[3], 'i', "refs", c.n_blocks, device) || !check_tensor(args[9], 'i', op == 3 ? "n_live" : "missing", 1, device)) return nullptr;
+    for (int i = 0; i < 3; i++)
+      if (!check_tensor(args[5 + i], 'i', names[op][i], n, device) || !convert(args[5 + i], list[i])) return nullptr;
+    if (!convert(args[1], ckv8) || !convert(args[2], scales) || !convert(args[3], refs) || !convert(args[4], table) || !convert(args[9], told) ||
+        !convert_stream(args[11], stream))
+      return nullptr;
+    at::Tensor own;
+    void* ws = nullptr;
+    size_t bytes = 0;
+    if (args[10] != Py_None) {
+      if (!convert(args[10], ws) || !convert(args[10], bytes)) return nullptr;
+    } else if (op != 2) {
+      bytes = p_hk_mla8_pages_workspace_bytes(c.n_blocks, n);
+      own = at::empty({(long long)(bytes < 256 ? 256 : bytes)}, THPVariable_Unpack(args[1]).options().dtype(at::kByte).requires_grad(false));
+      ws = own.mutable_data_ptr();
+      if (args[11] != Py_None) own.record_stream(c10::cuda::getStreamFromExternal(static_cast<cudaStream_t>(stream), (c10::DeviceIndex)device));
+    }
+    int status;
+    Py_BEGIN_ALLOW_THREADS;      // as in call
+    const int block = (int)c.block, stride = (int)c.stride, seqs = (int)c.seqs;
+    status = op == 0   ? p_hk_mla8_pages_fork(ckv8, scales, c.dtype, c.n_blocks, block, refs, table, stride, seqs, list[0], list[1], list[2], n, told, ws, bytes, stream)
+             : op == 1 ? p_hk_mla8_pages_reserve(ckv8, scales, c.dtype, c.n_blocks, block, refs, table, stride, seqs, list[0], list[1], n, told, ws, bytes, stream)
+             : op == 2 ? p_hk_mla8_pages_free(ckv8, scales, c.dtype, c.n_blocks, block, refs, table, stride, seqs, list[0], list[1], n, stream)
+                       : p_hk_mla8_pages_compact(ckv8, scales, c.dtype, c.n_blocks, block, refs, table, stride, seqs, told, ws, bytes, stream);
+    Py_END_ALLOW_THREADS;
+    return PyLong_FromLong(status);
+  } catch (const std::exception& e) {
+    PyErr_SetString(PyExc_RuntimeError, e.what());
+    return nullptr;
+  }
+}
+
 // scratch(nbytes, tensor) -> a byte tensor of torch's allocator on the tensor's device (torch.empty from Python costs twice the time)
 PyObject* py_scratch(PyObject*, PyObject* const* args, Py_ssize_t n) {
   long long bytes;
@@ -364,6 +419,7 @@ PyObject* py_scratch(PyObject*, PyObject* const* args, Py_ssize_t n) {
 #define X(name, stream) {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(py_##name)), METH_FASTCALL, nullptr},
 PyMethodDef methods[] = {HK_ENTRIES(X){"cache8", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(py_cache8)), METH_FASTCALL, nullptr},
                          {"append8", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(py_append8)), METH_FASTCALL, nullptr},
+                         {"pages", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(py_pages)), METH_FASTCALL, nullptr},
                          {"tensors", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(py_tensors)), METH_FASTCALL, nullptr},
                          {"scratch", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(py_scratch)), METH_FASTCALL, nullptr},
                          {"bind", py_bind, METH_O, nullptr}, {nullptr, nullptr, 0, nullptr}};

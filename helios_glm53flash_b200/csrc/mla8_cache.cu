@@ -238,16 +238,26 @@ cudaError_t accept_launch(const AppendArgs& a, cudaStream_t s) {
 // A warp four rows, a lane eight channels and the eight 256 further on (8-byte loads, 16-byte stores).  CTAs behind those of the rows: the
 // n_idx gathered positions of a sparse call, those without a block as -1.
 constexpr int READ_ROWS = 4, READ_IDX = 8;
-// rows i0 .. i0 + READ_ROWS - 1 of n, position at(i) of a sequence each, by a warp
-template <int FMT, class At>
-__device__ __forceinline__ void read_rows(const MlaPaged& pg, int seq, int i0, int n, __half* out, At at) {
-  const int lane = threadIdx.x & 31;
+template <int FMT>
+__global__ void __launch_bounds__(256) mla8_read_kernel(MlaPaged pg, int head, int shift, int n, __half* out, const int* idx, int64_t n_idx, int* idx_out) {
+  pdl_release();
+  pdl_wait();
+  const int row_ctas = (n + 8 * READ_ROWS - 1) / (8 * READ_ROWS);
+  if ((int)blockIdx.x >= row_ctas) {
+#pragma unroll
+    for (int k = 0; k < READ_IDX; k++) {
+      const int64_t i = ((int64_t)(blockIdx.x - row_ctas) * READ_IDX + k) * 256 + threadIdx.x;
+      if (i < n_idx) idx_out[i] = pg.block_of(0, idx[i]) >= 0 ? idx[i] : -1;
+    }
+    return;
+  }
+  const int lane = threadIdx.x & 31, i0 = (blockIdx.x * 8 + (threadIdx.x >> 5)) * READ_ROWS;
   uint2 v[READ_ROWS][2];
   float s[READ_ROWS];
 #pragma unroll
   for (int k = 0; k < READ_ROWS; k++) {
-    const int i = i0 + k, p = at(i);
-    const int64_t b = i < n ? pg.block_of(seq, p) : -1;
+    const int i = i0 + k, p = i < head ? i : i + shift;
+    const int64_t b = i < n ? pg.block_of(0, p) : -1;
     s[k] = 0.f;
     v[k][0] = v[k][1] = make_uint2(0u, 0u);
     if (b >= 0) {
@@ -271,30 +281,45 @@ __device__ __forceinline__ void read_rows(const MlaPaged& pg, int seq, int i0, i
     }
   }
 }
-template <int FMT>
-__global__ void __launch_bounds__(256) mla8_read_kernel(MlaPaged pg, int head, int shift, int n, __half* out, const int* idx, int64_t n_idx, int* idx_out) {
-  pdl_release();
-  pdl_wait();
-  const int row_ctas = (n + 8 * READ_ROWS - 1) / (8 * READ_ROWS);
-  if ((int)blockIdx.x >= row_ctas) {
-#pragma unroll
-    for (int k = 0; k < READ_IDX; k++) {
-      const int64_t i = ((int64_t)(blockIdx.x - row_ctas) * READ_IDX + k) * 256 + threadIdx.x;
-      if (i < n_idx) idx_out[i] = pg.block_of(0, idx[i]) >= 0 ? idx[i] : -1;
-    }
-    return;
-  }
-  read_rows<FMT>(pg, 0, (blockIdx.x * 8 + (threadIdx.x >> 5)) * READ_ROWS, n, out, [&](int i) { return i < head ? i : i + shift; });
-}
 
 // The first positions of every sequence, lens[s] (or len) of them and `cap` at most, as fp16 rows from row s * cap on; grid (CTAs of a sequence, sequences).
 template <int FMT>
 __global__ void __launch_bounds__(256) mla8_read_seqs_kernel(MlaPaged pg, const int* lens, int len, int cap, __half* out) {
   pdl_release();
   pdl_wait();
-  const int seq = blockIdx.y, n = min(lens ? lens[seq] : len, cap);
-  for (int64_t i0 = ((int64_t)blockIdx.x * 8 + (threadIdx.x >> 5)) * READ_ROWS; i0 < n; i0 += (int64_t)gridDim.x * 8 * READ_ROWS)
-    read_rows<FMT>(pg, seq, (int)i0, n, out + (size_t)seq * cap * LATENT, [](int i) { return i; });
+  const int lane = threadIdx.x & 31, seq = blockIdx.y, n = min(lens ? lens[seq] : len, cap);
+  __half* rows = out + (size_t)seq * cap * LATENT;
+  for (int64_t first = ((int64_t)blockIdx.x * 8 + (threadIdx.x >> 5)) * READ_ROWS; first < n; first += (int64_t)gridDim.x * 8 * READ_ROWS) {
+    const int i0 = (int)first;
+    uint2 v[READ_ROWS][2];
+    float s[READ_ROWS];
+#pragma unroll
+    for (int k = 0; k < READ_ROWS; k++) {
+      const int i = i0 + k;
+      const int64_t b = i < n ? pg.block_of(seq, i) : -1;
+      s[k] = 0.f;
+      v[k][0] = v[k][1] = make_uint2(0u, 0u);
+      if (b >= 0) {
+        const uint2* row = reinterpret_cast<const uint2*>(pg.data + (((size_t)b << pg.shift) + (i & ((1 << pg.shift) - 1))) * LATENT);
+        v[k][0] = row[lane];
+        v[k][1] = row[lane + 32];
+        s[k] = pg.scales[b];
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < READ_ROWS; k++) {
+      if (i0 + k >= n) break;
+#pragma unroll
+      for (int h = 0; h < 2; h++) {
+        const uint8_t* v8 = reinterpret_cast<const uint8_t*>(&v[k][h]);
+        uint4 w;
+        __half2* w2 = reinterpret_cast<__half2*>(&w);
+#pragma unroll
+        for (int c = 0; c < 4; c++) w2[c] = __floats2half2_rn(latent8_value<FMT>(v8[2 * c]) * s[k], latent8_value<FMT>(v8[2 * c + 1]) * s[k]);
+        reinterpret_cast<uint4*>(rows + (size_t)(i0 + k) * LATENT)[lane + 32 * h] = w;
+      }
+    }
+  }
 }
 
 }  // namespace

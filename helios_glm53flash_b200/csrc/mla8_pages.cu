@@ -4,9 +4,9 @@
 // call's sequences, so that the same calls give the same tables.  Everything is decided on the device: a call reads no length on the host, can be
 // captured, and is one small launch for the bookkeeping and, where pages move, one that moves them.
 //
-// Bookkeeping (pages_kernel): one cluster of eight CTAs, whose 256 warps take a sequence each in turn, or an eighth of a CTA's share of refs; the
-// steps of a call meet at the cluster's barrier, which also orders their accesses to global memory.  A list of free blocks in ascending order: every
-// warp counts its part of refs, the counts are added up through distributed shared memory, and the second pass writes where its count says.
+// Bookkeeping (pages_kernel): one CTA, or for large pools a cluster of eight, whose warps take a sequence each in turn, or a part of refs; the steps of a call
+// meet at a barrier, which also orders their accesses to global memory.  A list of free blocks in ascending order: every warp counts its part of
+// refs, the counts are added up through (distributed) shared memory, and the second pass writes where its count says.
 // What bounds it is latency, a few dependent loads and a barrier a step.
 #include "hk_common.cuh"
 #include "latent8.cuh"
@@ -18,8 +18,9 @@ bool mla8_paged(MlaPaged* pg, const void* ckv8, const float* scales, int dtype, 
 
 namespace {
 
-constexpr int PG_CTAS = 8, PG_THREADS = 1024, PG_WARPS = PG_CTAS * PG_THREADS / 32;
+constexpr int PG_MAX_CTAS = 8, PG_THREADS = 1024, PG_CTA_WARPS = PG_THREADS / 32;
 constexpr int PG_AHEAD = 8;                       // loads of a lane on their way
+constexpr int PG_SMALL = PG_CTA_WARPS * 32 * PG_AHEAD;   // blocks of a pool that one CTA looks after
 
 struct PagesArgs {
   MlaPaged pg;
@@ -34,9 +35,14 @@ struct PagesArgs {
 
 enum { PG_FORK, PG_RESERVE, PG_COMPACT };
 
+template <int CTAS>
 __device__ __forceinline__ void pg_barrier() {
-  __syncwarp();
-  asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
+  if constexpr (CTAS == 1) {
+    __syncthreads();
+  } else {
+    __syncwarp();
+    asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
+  }
 }
 __device__ __forceinline__ bool pg_block(const PagesArgs& a, int e) { return e >= 0 && e < a.pg.n_blocks; }
 // entries of a row that `len` positions take, whole blocks and all
@@ -70,58 +76,77 @@ __global__ __launch_bounds__(256) void pages_free_kernel(PagesArgs a) {
 struct PagesPart {
   int64_t b0, b1;
 };
+template <int CTAS>
 __device__ __forceinline__ PagesPart pg_part(const PagesArgs& a, int gw) {
-  const int64_t each = (a.pg.n_blocks + PG_WARPS * 32 - 1) / (PG_WARPS * 32) * 32;
+  constexpr int WARPS = CTAS * PG_CTA_WARPS;
+  const int64_t each = (a.pg.n_blocks + WARPS * 32 - 1) / (WARPS * 32) * 32;
   return {min(gw * each, a.pg.n_blocks), min((gw + 1) * each, a.pg.n_blocks)};
 }
-// f(block, references, in range) for 32 blocks at a time, ascending, by the whole warp
-template <class F>
-__device__ __forceinline__ void pg_walk(const PagesArgs& a, PagesPart p, F f) {
-  const int lane = threadIdx.x & 31;
-  for (int64_t b = p.b0; b < p.b1; b += 32 * PG_AHEAD) {
-    int r[PG_AHEAD];
+// A warp's part of refs, 32 blocks at a time.  One CTA: at most PG_SMALL blocks, a warp's part is read once and stays in registers.
+template <int CTAS>
+struct PagesWalk {
+  PagesPart p;
+  int r[PG_AHEAD];
+  __device__ __forceinline__ void load(const PagesArgs& a, int64_t b) {
 #pragma unroll
-    for (int u = 0; u < PG_AHEAD; u++) r[u] = b + 32 * u + lane < p.b1 ? a.refs[b + 32 * u + lane] : 0;
-#pragma unroll
-    for (int u = 0; u < PG_AHEAD; u++)
-      if (b + 32 * u < p.b1) f((int)(b + 32 * u) + lane, r[u], b + 32 * u + lane < p.b1);
+    for (int u = 0; u < PG_AHEAD; u++) r[u] = b + 32 * u + (int)(threadIdx.x & 31) < p.b1 ? a.refs[b + 32 * u + (threadIdx.x & 31)] : 0;
   }
-}
-// Of every warp's number: the sum of those before this one's, and of all.  Executed by all threads of the cluster.
+  __device__ __forceinline__ PagesWalk(const PagesArgs& a, int gw) : p(pg_part<CTAS>(a, gw)) {
+    if (CTAS == 1) load(a, p.b0);
+  }
+  // f(block, references, in range), ascending, by the whole warp
+  template <class F>
+  __device__ __forceinline__ void operator()(const PagesArgs& a, F f) {
+    const int lane = threadIdx.x & 31;
+    for (int64_t b = p.b0; b < p.b1; b += 32 * PG_AHEAD) {
+      if (CTAS > 1) load(a, b);
+#pragma unroll
+      for (int u = 0; u < PG_AHEAD; u++)
+        if (b + 32 * u < p.b1) f((int)(b + 32 * u) + lane, r[u], b + 32 * u + lane < p.b1);
+    }
+  }
+};
+// Of every warp's number: the sum of those before this one's, and of all.  Executed by all threads.
+template <int CTAS>
 __device__ __forceinline__ int2 pg_before(int mine, int* s_count, int* s_sum) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  uint32_t rank;
-  asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
   if (lane == 0) s_count[warp] = mine;
-  pg_barrier();
-  if (warp < PG_CTAS) {                                    // warp w: the numbers of CTA w
-    uint32_t at;
-    int v;
-    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"((uint32_t)__cvta_generic_to_shared(s_count + lane)), "r"(warp));
-    asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(at) : "memory");
-    const int sum = __reduce_add_sync(0xffffffffu, v);
-    if (lane == 0) s_sum[warp] = sum;
-  }
-  __syncthreads();
+  pg_barrier<CTAS>();
   int before = 0, all = 0;
-  for (int c = 0; c < PG_CTAS; c++) {
-    if (c < (int)rank) before += s_sum[c];
-    all += s_sum[c];
+  if constexpr (CTAS > 1) {
+    uint32_t rank;
+    asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
+    if (warp < CTAS) {                                     // warp w: the numbers of CTA w
+      uint32_t at;
+      int v;
+      asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"((uint32_t)__cvta_generic_to_shared(s_count + lane)), "r"(warp));
+      asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(at) : "memory");
+      const int sum = __reduce_add_sync(0xffffffffu, v);
+      if (lane == 0) s_sum[warp] = sum;
+    }
+    __syncthreads();
+    for (int c = 0; c < CTAS; c++) {
+      if (c < (int)rank) before += s_sum[c];
+      all += s_sum[c];
+    }
+  } else {
+    all = __reduce_add_sync(0xffffffffu, s_count[lane]);
   }
   before += __reduce_add_sync(0xffffffffu, lane < warp ? s_count[lane] : 0);
-  pg_barrier();                                            // the numbers have been read
+  pg_barrier<CTAS>();                                      // the numbers have been read
   return make_int2(before, all);
 }
-// The first `want` free blocks, ascending, into a.list; how many there are.  Executed by all threads of the cluster.
+// The first `want` free blocks, ascending, into a.list; how many there are.  Executed by all threads.
+template <int CTAS>
 __device__ __forceinline__ int pg_free_list(const PagesArgs& a, int gw, int want, int* s_count, int* s_sum) {
-  const PagesPart p = pg_part(a, gw);
+  PagesWalk<CTAS> walk(a, gw);
   const int lane = threadIdx.x & 31;
   int mine = 0;
-  pg_walk(a, p, [&](int, int r, bool in) { mine += __popc(__ballot_sync(0xffffffffu, in && r == 0)); });
-  const int2 c = pg_before(mine, s_count, s_sum);
+  walk(a, [&](int, int r, bool in) { mine += __popc(__ballot_sync(0xffffffffu, in && r == 0)); });
+  const int2 c = pg_before<CTAS>(mine, s_count, s_sum);
   int at = c.x;
   if (at < want)
-    pg_walk(a, p, [&](int b, int r, bool in) {
+    walk(a, [&](int b, int r, bool in) {
       const uint32_t free = __ballot_sync(0xffffffffu, in && r == 0);
       const int i = at + __popc(free & ((1u << lane) - 1));
       if ((free >> lane & 1) && i < want) a.list[i] = b;
@@ -130,17 +155,19 @@ __device__ __forceinline__ int pg_free_list(const PagesArgs& a, int gw, int want
   return min(c.y, want);
 }
 
-template <int MODE>
+template <int MODE, int CTAS>
 __global__ __launch_bounds__(PG_THREADS) void pages_kernel(PagesArgs a) {
-  __shared__ int s_count[32], s_sum[PG_CTAS];
+  constexpr int WARPS = CTAS * PG_CTA_WARPS;
+  __shared__ int s_count[PG_CTA_WARPS], s_sum[PG_MAX_CTAS];
+  pdl_release();
   pdl_wait();
-  const int lane = threadIdx.x & 31, gw = (int)(blockIdx.x * (PG_THREADS / 32) + (threadIdx.x >> 5)), stride = a.pg.table_stride;
+  const int lane = threadIdx.x & 31, gw = (int)(blockIdx.x * PG_CTA_WARPS + (threadIdx.x >> 5)), stride = a.pg.table_stride;
   auto row = [&](int s) -> int* { return a.table + (size_t)s * stride; };
   if constexpr (MODE == PG_FORK) {
     auto pair = [&](int i) { return pg_seq(a, a.seqs[i]) && pg_seq(a, a.from[i]) && a.seqs[i] != a.from[i]; };
-    for (int i = gw; i < a.n; i += PG_WARPS)
+    for (int i = gw; i < a.n; i += WARPS)
       if (pair(i)) pg_release(a, a.seqs[i], 0);
-    pg_barrier();
+    pg_barrier<CTAS>();
     // the block that a pair copies, -1: none
     int want = 0;
     for (int i0 = 0; i0 < a.n; i0 += 32) {
@@ -154,9 +181,9 @@ __global__ __launch_bounds__(PG_THREADS) void pages_kernel(PagesArgs a) {
       want += __popc(__ballot_sync(0xffffffffu, e >= 0));
       if (gw == 0 && i < a.n) a.src[i] = e;
     }
-    const int have = pg_free_list(a, gw, want, s_count, s_sum);
-    pg_barrier();
-    for (int i = gw; i < a.n; i += PG_WARPS) {
+    const int have = pg_free_list<CTAS>(a, gw, want, s_count, s_sum);
+    pg_barrier<CTAS>();
+    for (int i = gw; i < a.n; i += WARPS) {
       int before = 0;
       for (int k0 = 0; k0 < i; k0 += 32) before += __popc(__ballot_sync(0xffffffffu, k0 + lane < i && a.src[k0 + lane] >= 0));
       const int e = a.src[i], fresh = e >= 0 && before < have ? a.list[before] : -1;
@@ -182,21 +209,21 @@ __global__ __launch_bounds__(PG_THREADS) void pages_kernel(PagesArgs a) {
     }
   } else if constexpr (MODE == PG_RESERVE) {
     // entries without a block, by sequence of the call
-    for (int i = gw; i < a.n; i += PG_WARPS) {
+    for (int i = gw; i < a.n; i += WARPS) {
       const int s = a.seqs[i], all = pg_seq(a, s) ? pg_entries(a, a.lens[i]) : 0;
       int need = 0;
       for (int j0 = 0; j0 < all; j0 += 32) need += __popc(__ballot_sync(0xffffffffu, j0 + lane < all && !pg_block(a, row(s)[j0 + lane])));
       if (lane == 0) a.src[i] = need;
     }
-    pg_barrier();
+    pg_barrier<CTAS>();
     int64_t want = 0;
     for (int i0 = 0; i0 < a.n; i0 += 32) {
       const int v = i0 + lane < a.n ? a.src[i0 + lane] : 0;
       want += __reduce_add_sync(0xffffffffu, v);
     }
-    const int have = pg_free_list(a, gw, (int)min(want, a.pg.n_blocks), s_count, s_sum);
-    pg_barrier();
-    for (int i = gw; i < a.n; i += PG_WARPS) {
+    const int have = pg_free_list<CTAS>(a, gw, (int)min(want, a.pg.n_blocks), s_count, s_sum);
+    pg_barrier<CTAS>();
+    for (int i = gw; i < a.n; i += WARPS) {
       const int s = a.seqs[i], all = pg_seq(a, s) ? pg_entries(a, a.lens[i]) : 0;
       int64_t at = 0;
       for (int k0 = 0; k0 < i; k0 += 32) at += __reduce_add_sync(0xffffffffu, k0 + lane < i ? a.src[k0 + lane] : 0);
@@ -214,16 +241,17 @@ __global__ __launch_bounds__(PG_THREADS) void pages_kernel(PagesArgs a) {
     if (gw == 0 && lane == 0 && a.told) *a.told = (int)min(want - have, (int64_t)INT32_MAX);
   } else {
     // live blocks from number `live` on go to the holes below it, the i-th to the i-th
-    const PagesPart p = pg_part(a, gw);
+    PagesWalk<CTAS> walk(a, gw);
+    const PagesPart p = walk.p;
     int mine = 0;
-    pg_walk(a, p, [&](int, int r, bool in) { mine += __popc(__ballot_sync(0xffffffffu, in && r != 0)); });
-    const int2 c = pg_before(mine, s_count, s_sum);
+    walk(a, [&](int, int r, bool in) { mine += __popc(__ballot_sync(0xffffffffu, in && r != 0)); });
+    const int2 c = pg_before<CTAS>(mine, s_count, s_sum);
     const int live = c.y;
     int beyond = 0;                                        // this warp's live blocks at or beyond `live`
-    if (p.b1 > live) pg_walk(a, p, [&](int b, int r, bool in) { beyond += __popc(__ballot_sync(0xffffffffu, in && r != 0 && b >= live)); });
-    const int2 m = pg_before(beyond, s_count, s_sum);
+    if (p.b1 > live) walk(a, [&](int b, int r, bool in) { beyond += __popc(__ballot_sync(0xffffffffu, in && r != 0 && b >= live)); });
+    const int2 m = pg_before<CTAS>(beyond, s_count, s_sum);
     int hole = (int)min(p.b0, (int64_t)live) - (c.x - m.x), move = m.x;   // free blocks below `live` before this warp's
-    pg_walk(a, p, [&](int b, int r, bool in) {
+    walk(a, [&](int b, int r, bool in) {
       const uint32_t up = __ballot_sync(0xffffffffu, in && r != 0 && b >= live), down = __ballot_sync(0xffffffffu, in && r == 0 && b < live);
       if (up >> lane & 1) a.src[move + __popc(up & ((1u << lane) - 1))] = b;
       if (down >> lane & 1) a.dst[hole + __popc(down & ((1u << lane) - 1))] = b;
@@ -231,8 +259,8 @@ __global__ __launch_bounds__(PG_THREADS) void pages_kernel(PagesArgs a) {
       move += __popc(up);
       hole += __popc(down);
     });
-    pg_barrier();
-    for (int i = gw * 32 + lane; i < m.y; i += PG_WARPS * 32) {
+    pg_barrier<CTAS>();
+    for (int i = gw * 32 + lane; i < m.y; i += WARPS * 32) {
       const int from = a.src[i], to = a.dst[i];
       a.list[from] = to;
       a.refs[to] = a.refs[from];
@@ -263,6 +291,7 @@ struct CopyArgs {
 };
 constexpr int COPY_PIECE = 8192;
 __global__ __launch_bounds__(256) void pages_copy_kernel(CopyArgs a) {
+  pdl_release();
   pdl_wait();
   const int n = a.count ? *a.count : a.n, lg = a.shift - 4;   // pieces of a page: 2^lg
   const int64_t pieces = (int64_t)n << lg;
@@ -308,7 +337,9 @@ bool pages_workspace(PagesArgs* a, void* workspace, size_t bytes, int* status) {
 }
 template <int MODE>
 cudaError_t pages_launch(const PagesArgs& a, cudaStream_t s) {
-  return pdl_launch_cluster(PG_CTAS, pages_kernel<MODE>, dim3(PG_CTAS), dim3(PG_THREADS), 0, s, a);
+  // us, one CTA / eight: a compaction with nothing to move of 4,000 blocks 7.7 / 8.3, of 16,000 11.4 / 8.6, of 131,072 66 / 15; a fork out of 123 9.2 / 11.6
+  return a.pg.n_blocks <= PG_SMALL ? pdl_launch(pages_kernel<MODE, 1>, dim3(1), dim3(PG_THREADS), 0, s, a)
+                               : pdl_launch_cluster(PG_MAX_CTAS, pages_kernel<MODE, PG_MAX_CTAS>, dim3(PG_MAX_CTAS), dim3(PG_THREADS), 0, s, a);
 }
 CopyArgs pages_moves(const PagesArgs& a) {
   CopyArgs c{};

@@ -852,13 +852,19 @@ bool mla_tree_shape(int m, int n_seqs, bool ragged, int group, int n_keys, int* 
   *n_split = 1;
   for (int form = 0; form < (group == 1 ? 2 : 1); form++) {
     const int64_t units = form ? 2 * tree_units(m, n_seqs, ragged, 2) : tree_units(m, n_seqs, ragged, group);
-    for (int s = 1; s <= 256 && (s == 1 || (2 * s <= tiles + 1 && units * s <= 4 * sms)); s++) {
-      const int64_t waves = (units * s + sms - 1) / sms, per = (tiles + s - 1) / s;
+    for (int fill = 0; fill <= 4; fill++) {                // one split; as many as fill the GPU once, twice, ..., fewer where that means as many tiles each
+      int64_t s = fill * sms / units < 256 ? fill * sms / units : 256, per = 0;
+      if (2 * s > tiles + 1) s = (tiles + 1) / 2;
+      if (fill > 0 && s < 2) continue;
+      if (fill == 0) s = 1;
+      per = (tiles + s - 1) / s;
+      s = (tiles + per - 1) / per;
+      const int64_t waves = (units * s + sms - 1) / sms;
       const int64_t time = waves * per * (form ? 87 : 100) + (waves - 1) * 150 + (s == 1 ? (form ? 800 : 700) : (form ? 950 : 800) + 6 * units * s);
       if (best == 0 || time < best) {
         best = time;
         pairs = form;
-        *n_split = s;
+        *n_split = (int)s;
       }
     }
   }
