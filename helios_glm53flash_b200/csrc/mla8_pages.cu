@@ -53,23 +53,37 @@ __device__ __forceinline__ int pg_entries(const PagesArgs& a, int len) {
 }
 __device__ __forceinline__ bool pg_seq(const PagesArgs& a, int s) { return s >= 0 && s < a.pg.n_seqs; }
 
-// entries from `first` on of a row: each gives its block back and names none (an exchange: named twice, a row is given back once)
-__device__ __forceinline__ void pg_release(const PagesArgs& a, int seq, int first) {
-  int* row = a.table + (size_t)seq * a.pg.table_stride;
-  for (int j = first + (int)(threadIdx.x & 31); j < a.pg.table_stride; j += 32) {
-    if (row[j] < 0) continue;
-    const int e = atomicExch(row + j, -1);
-    if (pg_block(a, e)) atomicSub(a.refs + e, 1);
+// 128 entries of a row from j0 on, four a lane on their way at once; -1 from `end` on
+constexpr int PG_ROW = 4, PG_TURN = 32 * PG_ROW;
+__device__ __forceinline__ void pg_row(const int* row, int j0, int end, int (&e)[PG_ROW]) {
+#pragma unroll
+  for (int u = 0; u < PG_ROW; u++) {
+    const int j = j0 + 32 * u + (int)(threadIdx.x & 31);
+    e[u] = j < end ? row[j] : -1;
   }
 }
 
-__global__ __launch_bounds__(256) void pages_free_kernel(PagesArgs a) {
+// entries from `first` on of a row, PG_TURN of every `step`: each gives its block back and names none (an exchange: named twice, a row is given back once)
+__device__ __forceinline__ void pg_release(const PagesArgs& a, int seq, int first, int step) {
+  int* row = a.table + (size_t)seq * a.pg.table_stride;
+  for (int j0 = first; j0 < a.pg.table_stride; j0 += step) {
+    int e[PG_ROW];
+    pg_row(row, j0, a.pg.table_stride, e);
+#pragma unroll
+    for (int u = 0; u < PG_ROW; u++)
+      if (e[u] >= 0) e[u] = atomicExch(row + j0 + 32 * u + (threadIdx.x & 31), -1);
+#pragma unroll
+    for (int u = 0; u < PG_ROW; u++)
+      if (pg_block(a, e[u])) atomicSub(a.refs + e[u], 1);
+  }
+}
+
+// a CTA of four warps a sequence
+__global__ __launch_bounds__(128) void pages_free_kernel(PagesArgs a) {
   pdl_release();
   pdl_wait();
-  const int i = blockIdx.x * 8 + (threadIdx.x >> 5);
-  if (i >= a.n) return;
-  const int s = a.seqs[i];
-  if (pg_seq(a, s)) pg_release(a, s, pg_entries(a, a.lens ? a.lens[i] : 0));
+  const int s = a.seqs[blockIdx.x];
+  if (pg_seq(a, s)) pg_release(a, s, pg_entries(a, a.lens ? a.lens[blockIdx.x] : 0) + (threadIdx.x >> 5) * PG_TURN, 4 * PG_TURN);
 }
 
 // Blocks [b0, b1) of this warp, in ascending order over the cluster's warps.
@@ -166,7 +180,7 @@ __global__ __launch_bounds__(PG_THREADS) void pages_kernel(PagesArgs a) {
   if constexpr (MODE == PG_FORK) {
     auto pair = [&](int i) { return pg_seq(a, a.seqs[i]) && pg_seq(a, a.from[i]) && a.seqs[i] != a.from[i]; };
     for (int i = gw; i < a.n; i += WARPS)
-      if (pair(i)) pg_release(a, a.seqs[i], 0);
+      if (pair(i)) pg_release(a, a.seqs[i], 0, PG_TURN);
     pg_barrier<CTAS>();
     // the block that a pair copies, -1: none
     int want = 0;
@@ -192,11 +206,15 @@ __global__ __launch_bounds__(PG_THREADS) void pages_kernel(PagesArgs a) {
       const int whole = pg_whole(a, a.lens[i]);
       const int* from = row(a.from[i]);
       int* to = row(a.seqs[i]);
-      for (int j = lane; j < whole; j += 32) {
-        const int b = from[j];
-        if (!pg_block(a, b)) continue;
-        atomicAdd(a.refs + b, 1);
-        to[j] = b;
+      for (int j0 = 0; j0 < whole; j0 += PG_TURN) {
+        int b[PG_ROW];
+        pg_row(from, j0, whole, b);
+#pragma unroll
+        for (int u = 0; u < PG_ROW; u++) {
+          if (!pg_block(a, b[u])) continue;
+          atomicAdd(a.refs + b[u], 1);
+          to[j0 + 32 * u + lane] = b[u];
+        }
       }
       if (lane == 0 && fresh >= 0) {
         to[whole] = fresh;
@@ -212,7 +230,12 @@ __global__ __launch_bounds__(PG_THREADS) void pages_kernel(PagesArgs a) {
     for (int i = gw; i < a.n; i += WARPS) {
       const int s = a.seqs[i], all = pg_seq(a, s) ? pg_entries(a, a.lens[i]) : 0;
       int need = 0;
-      for (int j0 = 0; j0 < all; j0 += 32) need += __popc(__ballot_sync(0xffffffffu, j0 + lane < all && !pg_block(a, row(s)[j0 + lane])));
+      for (int j0 = 0; j0 < all; j0 += PG_TURN) {
+        int e[PG_ROW];
+        pg_row(row(s), j0, all, e);
+#pragma unroll
+        for (int u = 0; u < PG_ROW; u++) need += __popc(__ballot_sync(0xffffffffu, j0 + 32 * u + lane < all && !pg_block(a, e[u])));
+      }
       if (lane == 0) a.src[i] = need;
     }
     pg_barrier<CTAS>();
@@ -227,15 +250,22 @@ __global__ __launch_bounds__(PG_THREADS) void pages_kernel(PagesArgs a) {
       const int s = a.seqs[i], all = pg_seq(a, s) ? pg_entries(a, a.lens[i]) : 0;
       int64_t at = 0;
       for (int k0 = 0; k0 < i; k0 += 32) at += __reduce_add_sync(0xffffffffu, k0 + lane < i ? a.src[k0 + lane] : 0);
-      for (int j0 = 0; j0 < all; j0 += 32) {
-        const int j = j0 + lane, e = j < all ? row(s)[j] : 0;
-        const uint32_t open = __ballot_sync(0xffffffffu, j < all && !pg_block(a, e));
-        const int64_t k = at + __popc(open & ((1u << lane) - 1));
-        if ((open >> lane & 1) && k < have) {
-          const int b = a.list[k];
-          if (atomicCAS(row(s) + j, e, b) == e) a.refs[b] = 1;   // (a sequence that is named twice takes its blocks once)
+      for (int j0 = 0; j0 < all; j0 += PG_TURN) {
+        int e[PG_ROW], b[PG_ROW];
+        pg_row(row(s), j0, all, e);
+#pragma unroll
+        for (int u = 0; u < PG_ROW; u++) {
+          const uint32_t open = __ballot_sync(0xffffffffu, j0 + 32 * u + lane < all && !pg_block(a, e[u]));
+          const int64_t k = at + __popc(open & ((1u << lane) - 1));
+          b[u] = (open >> lane & 1) && k < have ? a.list[k] : -1;
+          at += __popc(open);
         }
-        at += __popc(open);
+#pragma unroll
+        for (int u = 0; u < PG_ROW; u++)                   // (a sequence that is named twice takes its blocks once)
+          if (b[u] >= 0 && atomicCAS(row(s) + j0 + 32 * u + lane, e[u], b[u]) != e[u]) b[u] = -1;
+#pragma unroll
+        for (int u = 0; u < PG_ROW; u++)
+          if (b[u] >= 0) a.refs[b[u]] = 1;
       }
     }
     if (gw == 0 && lane == 0 && a.told) *a.told = (int)min(want - have, (int64_t)INT32_MAX);
@@ -401,7 +431,7 @@ HK_API int hk_mla8_pages_free(void* ckv8, float* scales, int dtype, int64_t n_bl
   if (n == 0) return HK_OK;
   a.seqs = seqs; a.lens = keep;
   a.n = n;
-  return pdl_launch(pages_free_kernel, dim3((unsigned)((n + 7) / 8)), dim3(256), 0, as_stream(stream), a) == cudaSuccess ? HK_OK : HK_ERR_CUDA;
+  return pdl_launch(pages_free_kernel, dim3((unsigned)n), dim3(128), 0, as_stream(stream), a) == cudaSuccess ? HK_OK : HK_ERR_CUDA;
 }
 
 HK_API int hk_mla8_pages_compact(void* ckv8, float* scales, int dtype, int64_t n_blocks, int block, int* refs, int* block_table, int table_stride,
