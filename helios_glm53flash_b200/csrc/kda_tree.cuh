@@ -501,6 +501,51 @@ struct alignas(16) AcceptToken {
   float k[128], d[128], v[128];
   float beta;
 };
+// one token on a warp's columns: decay, k^T S, u, S + k u^T
+__device__ __forceinline__ void ka_step(ulonglong2 (&S)[16], const float* kp, const float* dp, float4 v, float be, int rg) {
+  ulonglong2 sum[4] = {{0, 0}, {0, 0}, {0, 0}, {0, 0}};   // even and odd rows of the two groups
+  float4 k[4];
+#pragma unroll
+  for (int c = 0; c < 4; c++) {                        // four rows at a time
+    const float4 d4 = *reinterpret_cast<const float4*>(&dp[state_row(rg, 4 * c)]);
+    k[c] = *reinterpret_cast<const float4*>(&kp[state_row(rg, 4 * c)]);
+    const float ds[4] = {d4.x, d4.y, d4.z, d4.w}, ks[4] = {k[c].x, k[c].y, k[c].z, k[c].w};
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+      ulonglong2& x = S[4 * c + e];
+      ulonglong2& y = sum[2 * (c >> 1) + (e & 1)];
+      const uint64_t dd = pack2(ds[e], ds[e]), kk = pack2(ks[e], ks[e]);
+      x.x = mul2(x.x, dd);
+      x.y = mul2(x.y, dd);
+      y.x = fma2(kk, x.x, y.x);
+      y.y = fma2(kk, x.y, y.y);
+    }
+  }
+  float kv[4], p[4][4];
+#pragma unroll
+  for (int u = 0; u < 4; u++) {
+    unpack2(sum[u].x, p[u][0], p[u][1]);
+    unpack2(sum[u].y, p[u][2], p[u][3]);
+  }
+#pragma unroll
+  for (int u = 0; u < 4; u++) kv[u] = __fadd_rn(__fadd_rn(p[0][u], p[1][u]), __fadd_rn(p[2][u], p[3][u]));
+#pragma unroll
+  for (int m = 4; m <= 16; m <<= 1)
+#pragma unroll
+    for (int u = 0; u < 4; u++) kv[u] = __fadd_rn(kv[u], __shfl_xor_sync(0xffffffffu, kv[u], m));
+  const uint64_t u0 = pack2(__fmul_rn(__fsub_rn(v.x, kv[0]), be), __fmul_rn(__fsub_rn(v.y, kv[1]), be));
+  const uint64_t u1 = pack2(__fmul_rn(__fsub_rn(v.z, kv[2]), be), __fmul_rn(__fsub_rn(v.w, kv[3]), be));
+#pragma unroll
+  for (int c = 0; c < 4; c++) {
+    const float ks[4] = {k[c].x, k[c].y, k[c].z, k[c].w};
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+      const uint64_t kk = pack2(ks[e], ks[e]);
+      S[4 * c + e].x = fma2(kk, u0, S[4 * c + e].x);
+      S[4 * c + e].y = fma2(kk, u1, S[4 * c + e].y);
+    }
+  }
+}
 template <int SLICES>
 __global__ __launch_bounds__(KA_WARPS * 32, 2) void kda_tree_accept_kernel(const KdaTreeArgs a) {
   constexpr int SW = KA_WARPS / SLICES;
@@ -509,17 +554,17 @@ __global__ __launch_bounds__(KA_WARPS * 32, 2) void kda_tree_accept_kernel(const
   __shared__ __align__(16) AcceptToken tok[KA_BATCH];
   __shared__ int list[TREE_NODES];
   pdl_wait();
+  const int leaf = a.leaf[s], slot = a.slots ? a.slots[s] : s;
   const int2 rows = a.tree.rows(s);
-  const uint64_t path = tree_path(a.tree, rows, a.leaf[s]);
-  const int steps = __popcll(path);
-  if (steps == 0) return;
-  const int slot = a.slots ? a.slots[s] : s;
+  if (leaf < 0 || leaf >= rows.y) return;
   float* sp = a.state + ((size_t)slot * a.H + head) * 128 * 128 + col;
   ulonglong2 S[16];                                        // two pairs of columns
   if (warp < SW) {
 #pragma unroll
     for (int i = 0; i < 16; i++) S[i] = *reinterpret_cast<const ulonglong2*>(sp + state_row(rg, i) * 128);
   }
+  const uint64_t path = tree_path(a.tree, rows, leaf);
+  const int steps = __popcll(path);
   if (warp == KA_WARPS - 1) {                              // a path's nodes are in ascending order
 #pragma unroll
     for (int h = 0; h < 2; h++) {
@@ -561,50 +606,7 @@ __global__ __launch_bounds__(KA_WARPS * 32, 2) void kda_tree_accept_kernel(const
 #pragma unroll 1
     for (int i = 0; i < batch; i++) {
       const AcceptToken& t = tok[i];
-      ulonglong2 sum[4] = {{0, 0}, {0, 0}, {0, 0}, {0, 0}};   // even and odd rows of the two groups
-      float4 k[4];
-#pragma unroll
-      for (int c = 0; c < 4; c++) {                        // four rows at a time
-        const float4 d4 = *reinterpret_cast<const float4*>(&t.d[state_row(rg, 4 * c)]);
-        k[c] = *reinterpret_cast<const float4*>(&t.k[state_row(rg, 4 * c)]);
-        const float ds[4] = {d4.x, d4.y, d4.z, d4.w}, ks[4] = {k[c].x, k[c].y, k[c].z, k[c].w};
-#pragma unroll
-        for (int e = 0; e < 4; e++) {
-          ulonglong2& x = S[4 * c + e];
-          ulonglong2& y = sum[2 * (c >> 1) + (e & 1)];
-          const uint64_t dd = pack2(ds[e], ds[e]), kk = pack2(ks[e], ks[e]);
-          x.x = mul2(x.x, dd);
-          x.y = mul2(x.y, dd);
-          y.x = fma2(kk, x.x, y.x);
-          y.y = fma2(kk, x.y, y.y);
-        }
-      }
-      float kv[4], p[4][4];
-#pragma unroll
-      for (int u = 0; u < 4; u++) {
-        unpack2(sum[u].x, p[u][0], p[u][1]);
-        unpack2(sum[u].y, p[u][2], p[u][3]);
-      }
-#pragma unroll
-      for (int u = 0; u < 4; u++) kv[u] = __fadd_rn(__fadd_rn(p[0][u], p[1][u]), __fadd_rn(p[2][u], p[3][u]));
-#pragma unroll
-      for (int m = 4; m <= 16; m <<= 1)
-#pragma unroll
-        for (int u = 0; u < 4; u++) kv[u] = __fadd_rn(kv[u], __shfl_xor_sync(0xffffffffu, kv[u], m));
-      const float4 v = *reinterpret_cast<const float4*>(&t.v[col]);
-      const float be = t.beta;
-      const uint64_t u0 = pack2(__fmul_rn(__fsub_rn(v.x, kv[0]), be), __fmul_rn(__fsub_rn(v.y, kv[1]), be));
-      const uint64_t u1 = pack2(__fmul_rn(__fsub_rn(v.z, kv[2]), be), __fmul_rn(__fsub_rn(v.w, kv[3]), be));
-#pragma unroll
-      for (int c = 0; c < 4; c++) {
-        const float ks[4] = {k[c].x, k[c].y, k[c].z, k[c].w};
-#pragma unroll
-        for (int e = 0; e < 4; e++) {
-          const uint64_t kk = pack2(ks[e], ks[e]);
-          S[4 * c + e].x = fma2(kk, u0, S[4 * c + e].x);
-          S[4 * c + e].y = fma2(kk, u1, S[4 * c + e].y);
-        }
-      }
+      ka_step(S, t.k, t.d, *reinterpret_cast<const float4*>(&t.v[col]), t.beta, rg);
     }
   }
   if (warp < SW) {
@@ -620,6 +622,175 @@ __global__ __launch_bounds__(KA_WARPS * 32, 2) void kda_tree_accept_kernel(const
     for (int j = max(0, steps - 4); j < steps; j++) w = conv4_rolled(w, __float2bfloat16_rn(a.x[(size_t)list[j] * 3 * a.H * 128 + ch]));
     *at = w;
   }
+}
+
+// The same for many heads: persistent CTAs, two an SM, whose ninth warp is a head ahead - it finds the path, asks for the next head's 64 KB as one bulk copy as
+// soon as this one's sit in registers, and for the first eight tokens - and whose tenth moves the windows.  The eight warps with columns share nothing but the
+// copies: each prepares every token for itself (a quarter more work a step, and no barrier).
+struct AcceptMeta {
+  uint64_t full[2], s_empty, t_empty[2];
+  uint64_t path[2];
+  float beta[2][KA_BATCH];
+  int abort_flag;
+};
+constexpr uint32_t KA_RAW = 1024;                 // a token: k and v of 256 bytes, log decays of 512
+constexpr uint32_t KAS_S = 0, KAS_RAW = 65536, KAS_TOK = KAS_RAW + 2 * KA_BATCH * KA_RAW, KAS_META = KAS_TOK + KA_WARPS * 2 * 1024,
+                   KAS_SMEM = KAS_META + (uint32_t)sizeof(AcceptMeta);
+constexpr int KA_STREAM_THREADS = (KA_WARPS + 2) * 32;
+__global__ __launch_bounds__(KA_STREAM_THREADS, 2) void kda_tree_accept_stream_kernel(const KdaTreeArgs a, int* __restrict__ status) {
+  extern __shared__ __align__(16) uint8_t ka_mem[];
+  AcceptMeta& ms = *reinterpret_cast<AcceptMeta*>(ka_mem + KAS_META);
+  volatile int* abort_flag = &ms.abort_flag;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tc::warp_index_uniform(), n_items = a.H * a.tree.n_seqs;
+  if (tid == 0) {
+    tc::mbar_init(&ms.full[0], 1);
+    tc::mbar_init(&ms.full[1], 1);
+    tc::mbar_init(&ms.s_empty, KA_WARPS);
+    tc::mbar_init(&ms.t_empty[0], KA_WARPS);
+    tc::mbar_init(&ms.t_empty[1], KA_WARPS);
+    tc::mbar_fence_init();
+    ms.abort_flag = 0;
+  }
+  pdl_wait();
+  __syncthreads();
+  // Tokens are handed over eight at a time, at least once a head, also of a sequence without an accepted node (no path, no copies).
+  if (warp == KA_WARPS) {
+    int turn = 0;
+    uint32_t moved = 0;                                    // heads whose state went through shared memory
+    for (int idx = blockIdx.x; idx < n_items; idx += gridDim.x) {
+      const int s = idx / a.H, head = idx - s * a.H, slot = a.slots ? a.slots[s] : s;
+      const int2 rows = a.tree.rows(s);
+      const uint64_t path = tree_path(a.tree, rows, a.leaf[s]);
+      const int steps = __popcll(path);
+      uint64_t rest = path;
+      for (int i0 = 0; i0 == 0 || i0 < steps; i0 += KA_BATCH, turn++) {
+        const int b = turn & 1, batch = min(steps - i0, KA_BATCH);
+        if (turn >= 2) tc::mbar_wait<40>(&ms.t_empty[b], (turn / 2 - 1) & 1, abort_flag, 61);
+        // lane i: the i-th node of the rest of the path
+        int r = rows.x;
+        {
+          uint64_t m = rest;
+          for (int i = 0; i < KA_BATCH; i++) {
+            if (i == lane && m) r += __ffsll((long long)m) - 1;
+            m &= m - 1;
+          }
+          rest = m;
+        }
+        if (lane < batch) ms.beta[b][lane] = a.a_log ? kt_beta<true>(a, r, head) : kt_beta<false>(a, r, head);
+        if (lane == 0) ms.path[b] = path;
+        __syncwarp();
+        if (lane == 0) {
+          if (steps == 0) tc::mbar_arrive(&ms.full[b]);
+          else tc::mbar_arrive_expect_tx(&ms.full[b], (i0 == 0 ? 65536 : 0) + batch * KA_RAW);
+        }
+        __syncwarp();
+        if (lane < batch) {
+          uint8_t* to = ka_mem + KAS_RAW + (b * KA_BATCH + lane) * KA_RAW;
+          const __nv_bfloat16* x = a.qkv + (size_t)r * 3 * a.H * 128 + head * 128;
+          tc::bulk_g2s(to, x + a.H * 128, 256, &ms.full[b]);
+          tc::bulk_g2s(to + 256, x + 2 * a.H * 128, 256, &ms.full[b]);
+          tc::bulk_g2s(to + 512, a.g + ((size_t)r * a.H + head) * 128, 512, &ms.full[b]);
+        }
+        if (i0 > 0 || steps == 0) continue;
+        if (moved > 0) tc::mbar_wait<40>(&ms.s_empty, (moved - 1) & 1, abort_flag, 62);
+        moved++;
+        if (lane == 0) tc::bulk_g2s(ka_mem + KAS_S, a.state + ((size_t)slot * a.H + head) * 128 * 128, 65536, &ms.full[b]);
+        __syncwarp();
+      }
+    }
+  } else if (warp > KA_WARPS) {
+    // the windows, by a warp that nobody waits for
+    for (int idx = blockIdx.x; a.conv_state && idx < n_items; idx += gridDim.x) {
+      const int s = idx / a.H, head = idx - s * a.H, slot = a.slots ? a.slots[s] : s;
+      const int2 rows = a.tree.rows(s);
+      const uint64_t path = tree_path(a.tree, rows, a.leaf[s]);
+      const int steps = __popcll(path);
+      if (steps == 0) continue;
+      uint64_t m = path;
+      for (int i = 4; i < steps; i++) m &= m - 1;        // its last four nodes
+      int node[4];
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        node[i] = m ? rows.x + __ffsll((long long)m) - 1 : -1;
+        m &= m - 1;
+      }
+#pragma unroll
+      for (int c0 = 0; c0 < 3 * 128; c0 += 128) {
+        uint2 w[4];
+        float x[4][4];
+        uint2* at[4];
+#pragma unroll
+        for (int u = 0; u < 4; u++) {
+          const int ch = ((c0 >> 7) * a.H + head) * 128 + 32 * u + lane;
+          at[u] = reinterpret_cast<uint2*>(a.conv_state + ((size_t)slot * 3 * a.H * 128 + ch) * 4);
+          w[u] = *at[u];
+#pragma unroll
+          for (int i = 0; i < 4; i++) x[u][i] = node[i] >= 0 ? a.x[(size_t)node[i] * 3 * a.H * 128 + ch] : 0.f;
+        }
+#pragma unroll
+        for (int u = 0; u < 4; u++) {
+#pragma unroll
+          for (int i = 0; i < 4; i++)
+            if (node[i] >= 0) w[u] = conv4_rolled(w[u], __float2bfloat16_rn(x[u][i]));
+          *at[u] = w[u];
+        }
+      }
+    }
+  } else {
+    const int rg = lane >> 2, col = warp * 16 + 4 * (lane & 3);
+    float* const tok = reinterpret_cast<float*>(ka_mem + KAS_TOK) + warp * 512;   // k and decay of a token, two in turn
+    int turn = 0;
+    for (int idx = blockIdx.x; idx < n_items; idx += gridDim.x) {
+      const int s = idx / a.H, head = idx - s * a.H, slot = a.slots ? a.slots[s] : s;
+      int steps = 0;
+      ulonglong2 S[16];
+      const float rate = a.a_log ? __expf(a.a_log[head]) : 0.f;
+      for (int i0 = 0; i0 == 0 || i0 < steps; i0 += KA_BATCH, turn++) {
+        const int b = turn & 1;
+        tc::mbar_wait<40>(&ms.full[b], (turn / 2) & 1, abort_flag, 63);
+        if (i0 == 0) {
+          steps = __popcll(ms.path[b]);
+          if (steps > 0) {
+            const float* from = reinterpret_cast<const float*>(ka_mem + KAS_S) + col;
+#pragma unroll
+            for (int i = 0; i < 16; i++) S[i] = *reinterpret_cast<const ulonglong2*>(from + state_row(rg, i) * 128);
+            __syncwarp();
+            if (lane == 0) tc::mbar_arrive(&ms.s_empty);
+          }
+        }
+#pragma unroll 1
+        for (int i = 0; i < min(steps - i0, KA_BATCH); i++) {
+          const uint8_t* raw = ka_mem + KAS_RAW + (b * KA_BATCH + i) * KA_RAW;
+          const __nv_bfloat16* k = reinterpret_cast<const __nv_bfloat16*>(raw);
+          const float* g = reinterpret_cast<const float*>(raw + 512);
+          float* to = tok + (i & 1) * 256;
+          float z[4];
+#pragma unroll
+          for (int u = 0; u < 4; u++) z[u] = __bfloat162float(k[lane + 32 * u]);
+          const float f = inv_norm(z);
+#pragma unroll
+          for (int u = 0; u < 4; u++) {
+            const int c = lane + 32 * u;
+            const float x = g[c];
+            to[c] = __fmul_rn(z[u], f);
+            to[128 + c] = __expf(a.a_log ? gate_value(x, a.dt_bias[head * 128 + c], rate, a.lower_bound) : x);
+          }
+          const float4 v4 = load4(k + 128 + col);
+          __syncwarp();
+          ka_step(S, to, to + 128, v4, ms.beta[b][i], rg);
+        }
+        __syncwarp();
+        if (lane == 0) tc::mbar_arrive(&ms.t_empty[b]);
+      }
+      if (steps > 0 && !*abort_flag) {
+        float* sp = a.state + ((size_t)slot * a.H + head) * 128 * 128 + col;
+#pragma unroll
+        for (int i = 0; i < 16; i++) *reinterpret_cast<ulonglong2*>(sp + state_row(rg, i) * 128) = S[i];
+      }
+    }
+  }
+  __syncthreads();
+  if (tid == 0 && ms.abort_flag && status) atomicExch(status, HK_ERR_TIMEOUT);
 }
 
 template <int SLICES>
@@ -684,6 +855,21 @@ HK_API int hk_kda_tree_accept(const float* x32, void* conv_state, const void* mi
   a.conv_state = (__nv_bfloat16*)conv_state;
   a.leaf = leaf;
   // up to half a head an SM by two CTAs a head: a path of five of 64 heads 6.2 / 5.4 us (one / two), of 128 6.7 / 7.0; four 32 heads 6.2 / 6.0 / 5.8
+  const int64_t heads = (int64_t)num_heads * n_seqs;
+  // more than three heads an SM stream through shared memory: us, a CTA a head / streamed, paths of five, 320 heads 10.5 / 14.4, 384 14.4 / 14.9, 512 21.9 / 19.7,
+  // 1,024 39.3 / 32.4, 1,536 55.3 / 45.5
+  if (heads > 3 * sm_count() && aligned(mixed_qkv, 16)) {
+    static bool attr_set[64] = {false};
+    const int dev = device_index();
+    if (!attr_set[dev]) {
+      if (cudaFuncSetAttribute(kda_tree_accept_stream_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)KAS_SMEM) != cudaSuccess) return HK_ERR_CUDA;
+      attr_set[dev] = true;
+    }
+    const int64_t ctas = heads < 2 * sm_count() ? heads : 2 * sm_count();
+    return pdl_launch(kda_tree_accept_stream_kernel, dim3((unsigned)ctas), dim3(KA_STREAM_THREADS), KAS_SMEM, as_stream(stream), a, device_status_ptr()) == cudaSuccess
+               ? HK_OK
+               : HK_ERR_CUDA;
+  }
   const cudaError_t e = 2 * (int64_t)num_heads * n_seqs <= sm_count() ? ka_launch<2>(a, as_stream(stream)) : ka_launch<1>(a, as_stream(stream));
   return e == cudaSuccess ? HK_OK : HK_ERR_CUDA;
 }

@@ -371,8 +371,9 @@ def test_what_is_not_on_a_nodes_path_has_no_effect_on_it():
             assert torch.equal(out[j], good[j]), j
 
 
-def test_raw_gates_give_what_prepared_gates_give():
-    gen, heads = gen_of(13), 5
+@pytest.mark.parametrize("heads", [5, 230])
+def test_raw_gates_give_what_prepared_gates_give(heads):
+    gen = gen_of(13)
     trees = [tree_of((20, 1)), tree_of("chain5")]
     starts, parent, tree_start = layout(trees)
     m = starts[-1]
@@ -392,7 +393,7 @@ def test_raw_gates_give_what_prepared_gates_give():
     assert torch.equal(*outs) and torch.equal(*states)
 
 
-@pytest.mark.parametrize("heads,n", [(2, 1), (16, 5), (40, 3)])
+@pytest.mark.parametrize("heads,n", [(2, 1), (16, 5), (40, 3), (96, 5)])
 def test_accepted_states_are_those_of_token_by_token_decoding(heads, n):
     """bit for bit: the states of the recurrence over the path's tokens, the windows of the convolution over them"""
     trees = [tree_of(t) for t in ("binary15", "chain64", (17, 4), "one", "star7")[:n]]
