@@ -398,8 +398,8 @@ HK_API int hk_mla8_pages_fork(void* ckv8, float* scales, int dtype, int64_t n_bl
                               size_t workspace_bytes, void* stream) {
   using namespace hk;
   PagesArgs a;
-  HK_REQUIRE(pages_args(&a, ckv8, scales, dtype, n_blocks, block, refs, block_table, table_stride, n_seqs) && parents && children && lens && n >= 0);
-  if (n == 0) return HK_OK;
+  HK_REQUIRE(pages_args(&a, ckv8, scales, dtype, n_blocks, block, refs, block_table, table_stride, n_seqs) && n >= 0 && (n == 0 || (parents && children && lens)));
+  if (n == 0 && !missing) return HK_OK;
   a.from = parents; a.seqs = children; a.lens = lens;
   a.n = n;
   a.told = missing;
@@ -413,8 +413,8 @@ HK_API int hk_mla8_pages_reserve(void* ckv8, float* scales, int dtype, int64_t n
                                  int n_seqs, const int* seqs, const int* lens, int n, int* missing, void* workspace, size_t workspace_bytes, void* stream) {
   using namespace hk;
   PagesArgs a;
-  HK_REQUIRE(pages_args(&a, ckv8, scales, dtype, n_blocks, block, refs, block_table, table_stride, n_seqs) && seqs && lens && n >= 0);
-  if (n == 0) return HK_OK;
+  HK_REQUIRE(pages_args(&a, ckv8, scales, dtype, n_blocks, block, refs, block_table, table_stride, n_seqs) && n >= 0 && (n == 0 || (seqs && lens)));
+  if (n == 0 && !missing) return HK_OK;
   a.seqs = seqs; a.lens = lens;
   a.n = n;
   a.told = missing;
@@ -427,7 +427,7 @@ HK_API int hk_mla8_pages_free(void* ckv8, float* scales, int dtype, int64_t n_bl
                               int n_seqs, const int* seqs, const int* keep, int n, void* stream) {
   using namespace hk;
   PagesArgs a;
-  HK_REQUIRE(pages_args(&a, ckv8, scales, dtype, n_blocks, block, refs, block_table, table_stride, n_seqs) && seqs && n >= 0);
+  HK_REQUIRE(pages_args(&a, ckv8, scales, dtype, n_blocks, block, refs, block_table, table_stride, n_seqs) && n >= 0 && (n == 0 || seqs));
   if (n == 0) return HK_OK;
   a.seqs = seqs; a.lens = keep;
   a.n = n;
@@ -455,7 +455,7 @@ HK_API int hk_mla8_pages_copy(const void* from_ckv8, const float* from_scales, i
                               int dtype, int block, const int* src, const int* dst, int n, void* stream) {
   using namespace hk;
   MlaPaged x, y;
-  HK_REQUIRE(mla8_paged(&x, from_ckv8, from_scales, dtype, from_blocks, block, nullptr, 0, 1, nullptr) && src && dst && n >= 0);
+  HK_REQUIRE(mla8_paged(&x, from_ckv8, from_scales, dtype, from_blocks, block, nullptr, 0, 1, nullptr) && n >= 0 && (n == 0 || (src && dst)));
   HK_REQUIRE(mla8_paged(&y, to_ckv8, to_scales, dtype, to_blocks, block, nullptr, 0, 1, nullptr));
   if (n == 0) return HK_OK;
   CopyArgs c{};

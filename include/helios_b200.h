@@ -370,6 +370,8 @@ int hk_mla8_sparse(const void* q_lat, const void* ckv8, const float* scales, int
  * no block (negative, >= n_blocks) counts nowhere.  Blocks are handed out lowest number first, in the order of the call's sequences.  All arrays are
  * device memory, nothing is read on the host.  A number outside [0, n_seqs) in a list of sequences is passed over; no list names a sequence
  * twice.  Calls on one pool, and those that read or write its blocks, are ordered by the caller (a stream).
+ * A block that several entries name is read by all of them and appended to by none: a sequence that was cut back into one (hk_mla8_pages_free) goes on
+ * as a fork of itself in another row, which has a copy of that block.  With n 0 the lists may be NULL.
  * workspace: hk_mla8_pages_workspace_bytes(n_blocks, n) bytes, 256-byte aligned (n 0 for a compaction).                                           */
 size_t hk_mla8_pages_workspace_bytes(int64_t n_blocks, int n);
 
@@ -616,13 +618,15 @@ int hk_kda_tree_conv(const float* x32, const void* conv_state, const int* slots,
  * the node as the last token behind its path, with the state rec_state [slots][H][128][128] of its sequence, which stays as it is.  No node's
  * state is formed: sums in another order than there.  mixed_qkv [m][3*H*128] bf16 (8-byte aligned), g [m][H][128] log decay f32 (<= 0; 16-byte aligned)
  * and beta [m][H] bf16 as there; or, with a_log [H] and dt_bias [H][128], the raw gate f32 and the raw beta logit f32 as in
- * hk_kda_chunked_prefill_gated.  max_nodes: nodes that the longest tree has (0: 64); nodes beyond, and rows of no tree, are left as they were.      */
+ * hk_kda_chunked_prefill_gated.  max_nodes: nodes that the longest tree has (0: 64); nodes beyond, and rows of no tree, are left as they were.
+ * out 8-byte, out_f32 and rec_state 16-byte aligned.                                                                                        */
 int hk_kda_tree(const void* mixed_qkv, const float* g, const void* beta, const float* dt_bias, const float* a_log, float lower_bound,
                 const float* rec_state, const int* slots, const int* parent, const int* tree_start, int n_seqs, void* out, float* out_f32,
                 int m, int num_heads, int max_nodes, void* stream);
 
 /* The states of the sequences step along the accepted paths: rec_state as hk_kda_recurrent (channelwise) leaves it behind the path's tokens, bit for
- * bit, and the windows conv_state as hk_kda_cast_conv leaves them behind the path's rows of x32 (both NULL: no windows).  Other arguments as in hk_kda_tree.  */
+ * bit, and the windows conv_state as hk_kda_cast_conv leaves them behind the path's rows of x32 (both NULL: no windows).  Other arguments as in hk_kda_tree;
+ * no slot belongs to two sequences that accept nodes.                                                                                        */
 int hk_kda_tree_accept(const float* x32, void* conv_state, const void* mixed_qkv, const float* g, const void* beta, const float* dt_bias,
                        const float* a_log, float lower_bound, float* rec_state, const int* slots, const int* parent, const int* tree_start,
                        int n_seqs, const int* leaf, int m, int num_heads, void* stream);

@@ -172,6 +172,21 @@ def test_the_same_sequence_twice_is_given_back_once():
     pool.check()
 
 
+def test_calls_without_sequences_tell_that_nothing_is_missing():
+    pool = Pool("i8", 30, 16, 3, 6)
+    pool.reserve([(0, 40)])
+    none = ints([])
+    hk.mla8_pages_fork(*pool.tensors, none, none, none, 0)
+    hk.mla8_pages_free(*pool.tensors, none, None, 0)
+    hk.mla8_pages_copy(*pool.tensors[:2], *pool.tensors[:2], none, none, 0)
+    for call in (lambda told: hk.mla8_pages_fork(*pool.tensors, none, none, none, 0, missing=told),
+                 lambda told: hk.mla8_pages_reserve(*pool.tensors, none, none, 0, missing=told)):
+        told = ints([7])
+        call(told)
+        assert int(told) == 0
+    pool.check()
+
+
 def test_long_pools_and_offsets_beyond_four_gigabytes():
     """blocks beyond 2^32 bytes of the cache: fork copies one there, compaction brings it back"""
     n, block = (1 << 32) // (128 * 512) + 40, 128

@@ -520,7 +520,7 @@ def test_captured_and_replayed_and_on_a_stream_of_its_own(kind):
     ckv8, scales = cache(gen, "e4m3", 12, 64)
     table, ckv = table_for(gen, 2, 6, 12), randn(gen, 800, 512).half()
     base = torch.tensor([0, 400], device="cuda")
-    x = kda_inputs(gen, m, 8, 2)
+    x = kda_inputs(gen, m, 6, 2)
 
     def call(out, stream=None):
         at = dict(n_seqs=2, tree_start=tree_start, stream=stream)
@@ -529,9 +529,9 @@ def test_captured_and_replayed_and_on_a_stream_of_its_own(kind):
         elif kind == "tree8":
             hk.mla8_tree_decode(q, ckv8, scales, rows, parent, out, m, block_table=table, kv_len=lens, n_keys_hint=384, **at)
         else:
-            hk.kda_tree_decode(x["qkv"], x["g"], x["beta"], x["state"], parent, out, m, 8, **at)
+            hk.kda_tree_decode(x["qkv"], x["g"], x["beta"], x["state"], parent, out, m, 6, **at)
 
-    fresh = lambda: torch.zeros(m, 8, 128, dtype=torch.bfloat16, device="cuda") if kind == "kda" else torch.zeros(m, heads, 512, dtype=torch.float16, device="cuda")  # noqa: E731
+    fresh = lambda: torch.zeros(m, 6, 128, dtype=torch.bfloat16, device="cuda") if kind == "kda" else torch.zeros(m, heads, 512, dtype=torch.float16, device="cuda")  # noqa: E731
     first = fresh()
     call(first)
     side, there = torch.cuda.Stream(), fresh()

@@ -124,7 +124,9 @@ def test_pages_refuse_lists(lib):
     assert call(lib.hk_mla8_pages_reserve, RESERVE, POOL, b=None) == BAD and call(lib.hk_mla8_pages_free, FREE, POOL, a=None) == BAD
     for fn, names in ((lib.hk_mla8_pages_fork, FORK), (lib.hk_mla8_pages_reserve, RESERVE), (lib.hk_mla8_pages_free, FREE)):
         assert call(fn, names, POOL, n=-1) == BAD and call(fn, names, POOL, n=0) == hk.HK_OK
+    assert call(lib.hk_mla8_pages_fork, FORK, POOL, n=0, a=None, b=None, c=None) == hk.HK_OK
+    assert call(lib.hk_mla8_pages_reserve, RESERVE, POOL, n=0, a=None, b=None) == call(lib.hk_mla8_pages_free, FREE, POOL, n=0, a=None) == hk.HK_OK
     copy = "ckv8 scales blocks ckv8 scales blocks dtype block a b n stream"
-    assert call(lib.hk_mla8_pages_copy, copy, POOL, n=0) == hk.HK_OK
+    assert call(lib.hk_mla8_pages_copy, copy, POOL, n=0) == call(lib.hk_mla8_pages_copy, copy, POOL, n=0, a=None, b=None) == hk.HK_OK
     for changes in (dict(a=None), dict(n=-1), dict(block=8), dict(dtype=0), dict(blocks=0)):
         assert call(lib.hk_mla8_pages_copy, copy, POOL, **changes) == BAD
