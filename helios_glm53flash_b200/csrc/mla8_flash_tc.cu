@@ -259,7 +259,7 @@ __global__ __launch_bounds__(F8_THREADS, 1) void mla8_flash_tc_kernel(MlaArgs a,
   // An item of at most two tiles (a decode split) does not need the last tile slot back: S reads Q from there, and moving it is saved.
   const bool direct_q = it.n_tiles < F8_NBUF;
   // Final rows, or a partial: with a number of splits [split][row, head], shared out [CTA][64 heads].
-  const bool final_out = PARTS == 1 && it.n_sp == 1;
+  const bool final_out = (TREE || PARTS == 1) && it.n_sp == 1;
   const size_t part_row = a.n_split == 0 ? (size_t)blockIdx.x * F8_HEADS : (size_t)it.sp * a.m * a.n_heads + it.q_row + it.hg * F8_HEADS;
   if (a.n_split == 0 && it.r >= 0 && it.sp == 0 && it.hg == 0 && tid == 0) a.shares[it.r] = make_int2(it.first, it.n_sp);
   const int n_tiles = it.n_tiles, h0 = it.hg * F8_HEADS, n_h = TREE ? min(F8_HEADS, tree.count * a.n_heads - h0) : min(F8_HEADS, a.n_heads - h0);
@@ -645,13 +645,13 @@ __global__ __launch_bounds__(F8_THREADS, 1) void mla8_flash_tc_kernel(MlaArgs a,
     }
     asm volatile("bar.sync 4, 384;" ::: "memory");
     if (!*abort_flag && (!TREE || tree.seq >= 0)) {          // (a row of no tree is left as it was)
-      uint8_t* dst = final_out ? reinterpret_cast<uint8_t*>(a.out + ((size_t)it.q_row + h0) * LATENT)
+      uint8_t* dst = final_out ? reinterpret_cast<uint8_t*>(a.out + ((size_t)it.q_row + h0) * LATENT + it.part * n_ch)
                                : reinterpret_cast<uint8_t*>(a.part_acc + part_row * LATENT + it.part * n_ch);
       const int team = warp < 4 ? warp : warp - 2;
-      const int per = n_ch * elem / 512;                   // 512-byte pieces of a head
+      const int lg = (final_out ? 6 : 7) - (PARTS == 4 ? 2 : PARTS - 1);   // a head's pieces of 16 bytes are 1 << lg
 #pragma unroll 8
-      for (int i = team; i < n_h * per; i += 12) {
-        const int h = i / per, c = i % per * 512 + lane * 16;
+      for (int i = team * 32 + lane; i < n_h << lg; i += 384) {
+        const int h = i >> lg, c = (i & ((1 << lg) - 1)) * 16;
         *reinterpret_cast<uint4*>(dst + (size_t)h * LATENT * elem + c) = *reinterpret_cast<const uint4*>(smem + F8S_K + h * pitch + c);
       }
     }
@@ -799,7 +799,7 @@ int mla8_flash_tc_launch(const MlaArgs& a, const MlaPaged& pg, int dtype, cudaSt
   // Few splits of few rows: the output channels of each are shared out over two or four CTAs, which compute the scores each for itself and write
   // a half or a quarter of the partial (of 128 KB, which take 2.1 us).  2,052 gathered rows 11.1 -> 9.1 us (four), 5,001 keys 11.1 -> 10.4 (two).
   const int64_t ctas = (int64_t)a.n_split * (a.tree_kv ? a.tree_units : a.m) * ((a.n_heads + F8_HEADS - 1) / F8_HEADS);
-  const int parts = a.n_split < 2 ? 1 : f8_parts(ctas);
+  const int parts = a.n_split < 2 && !a.tree_kv ? 1 : f8_parts(ctas);   // (of few nodes of trees also final rows)
   const int st = a.raw_idx ? (dtype == HK_I8 ? f8_launch_parts<true, CACHE_I8>(parts, a, pg, q, s) : f8_launch_parts<true, CACHE_E4M3>(parts, a, pg, q, s))
                            : (dtype == HK_I8 ? f8_launch_parts<false, CACHE_I8>(parts, a, pg, q, s) : f8_launch_parts<false, CACHE_E4M3>(parts, a, pg, q, s));
   if (st != HK_OK || a.n_split > 0) return st;

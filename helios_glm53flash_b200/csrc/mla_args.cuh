@@ -67,21 +67,29 @@ struct MlaTree {
   uint64_t path;
   int seq, len, row0, node;                       // seq < 0: a row of no tree, without keys
 };
-// executed by a whole warp
-__device__ __forceinline__ MlaTree mla_tree(const MlaArgs& a, int r) {
-  MlaTree t{0, 0, a.tree.seq_of(r), 0, 0, -1};
-  if (t.seq < 0) return t;
-  const int2 rows = a.tree.rows(t.seq);
+// where the cached keys of a tree's sequence begin, and how many there are
+__device__ __forceinline__ int mla_tree_keys(const MlaArgs& a, int seq, int64_t* base) {
+  int len = max(a.kv_len ? a.kv_len[seq] : a.pos_start, 0);
+  *base = a.kv_base ? a.kv_base[seq] : seq * a.kv_stride;
+  if (a.kv_stride > 0) len = (int)min((int64_t)len, a.kv_stride);
+  if (a.ckv_rows > 0) len = (int)max((int64_t)0, min((int64_t)len, a.ckv_rows - *base));   // never past the end of the cache
+  return len;
+}
+// node `node` of the tree in rows.x .. rows.x + rows.y - 1; executed by a whole warp
+__device__ __forceinline__ MlaTree mla_tree(const MlaArgs& a, int seq, int2 rows, int node) {
+  MlaTree t{0, 0, seq, 0, rows.x, node};
+  t.len = mla_tree_keys(a, seq, &t.base);                  // (on its way with the parents)
   TreePaths paths;
   paths.load(a.tree, rows);
-  t.row0 = rows.x;
-  t.node = r - rows.x;
-  t.path = paths.of(t.node);
-  t.base = a.kv_base ? a.kv_base[t.seq] : t.seq * a.kv_stride;
-  t.len = max(a.kv_len ? a.kv_len[t.seq] : a.pos_start, 0);
-  if (a.kv_stride > 0) t.len = (int)min((int64_t)t.len, a.kv_stride);
-  if (a.ckv_rows > 0) t.len = (int)max((int64_t)0, min((int64_t)t.len, a.ckv_rows - t.base));   // never past the end of the cache
+  t.path = paths.of(node);
   return t;
+}
+// row r, which may be of no tree; executed by a whole warp
+__device__ __forceinline__ MlaTree mla_tree(const MlaArgs& a, int r) {
+  const int seq = a.tree.seq_of(r);
+  if (seq < 0) return {0, 0, -1, 0, 0, -1};
+  const int2 rows = a.tree.rows(seq);
+  return mla_tree(a, seq, rows, r - rows.x);
 }
 
 // Neighbouring nodes of a tree, a.tree_group of them, whose heads are a CTA's 64 query rows.
@@ -97,15 +105,12 @@ __device__ __forceinline__ MlaNodes mla_nodes(const MlaArgs& a, int unit) {
   const TreeUnit u = tree_unit(a.tree, unit, a.tree_group);
   MlaNodes t{0, 0, 0, u.seq, 0, u.row0, u.node, u.count};
   if (t.seq < 0) return t;
+  t.len = mla_tree_keys(a, t.seq, &t.base);                // (on its way with the parents)
   TreePaths paths;
-  paths.load(a.tree, a.tree.rows(t.seq));
+  paths.load(a.tree, make_int2(u.row0, u.size));
   t.mine = paths.of((t.node + lane) & 63);
   if (lane >= t.count) t.mine = 0;
   t.any = (uint64_t)__reduce_or_sync(0xffffffffu, (uint32_t)(t.mine >> 32)) << 32 | __reduce_or_sync(0xffffffffu, (uint32_t)t.mine);
-  t.base = a.kv_base ? a.kv_base[t.seq] : t.seq * a.kv_stride;
-  t.len = max(a.kv_len ? a.kv_len[t.seq] : a.pos_start, 0);
-  if (a.kv_stride > 0) t.len = (int)min((int64_t)t.len, a.kv_stride);
-  if (a.ckv_rows > 0) t.len = (int)max((int64_t)0, min((int64_t)t.len, a.ckv_rows - t.base));   // never past the end of the cache
   return t;
 }
 

@@ -26,7 +26,7 @@ int mla8_read_seqs_launch(const MlaPaged& pg, int dtype, const int* lens, int le
 bool mla8_paged(MlaPaged* pg, const void* ckv8, const float* scales, int dtype, int64_t n_blocks, int block, const int* block_table,
                 int table_stride, int n_seqs, const int* row_seq);
 bool mla_flash_cluster_shape(int m, int tiles, int* n_split);
-bool mla_tree_shape(int m, int n_seqs, bool ragged, int group, int n_keys, int* n_split);
+int64_t mla_tree_shape(int m, int n_seqs, bool ragged, int group, int n_keys, int* n_split, bool* pairs);
 // neighbouring nodes of a tree whose heads fill 64 query rows
 static int tree_group(int n_heads) { return n_heads < 64 && 64 % n_heads == 0 ? 64 / n_heads : 1; }
 
@@ -736,7 +736,7 @@ static int tree_splits(int m, int n_heads, int n_seqs, bool ragged, int n_keys, 
     *pairs = false;
     return simt_auto_splits(m, n_heads, n_keys);
   }
-  *pairs = mla_tree_shape(m, n_seqs, ragged, group, n_keys, &n_split);
+  mla_tree_shape(m, n_seqs, ragged, group, n_keys, &n_split, pairs);
   return n_split;
 }
 }  // namespace hk
@@ -745,8 +745,8 @@ HK_API size_t hk_mla_tree_workspace_bytes(int m, int n_heads, int n_seqs, int n_
   if (m <= 0 || n_heads < hk::SIMT_HG || n_seqs < 1 || n_keys < 0) return 0;
   bool pairs;
   int most = 1;
-  for (int k = 0; k < 4; k++) {                            // (whether the trees are ragged and the lengths on the device)
-    if (k < 2 && m % n_seqs != 0) continue;
+  for (int k = 0; k < 4; k++) {                            // (whether the trees are ragged and the lengths on the device, which may mean other keys)
+    if ((k < 2 && m % n_seqs != 0) || ((k & 1) && n_keys > 0)) continue;
     const int splits = hk::tree_splits(m, n_heads, n_seqs, k >= 2, hk::tree_keys(k & 1, n_keys), &pairs);
     most = most > splits ? most : splits;
   }
@@ -754,7 +754,7 @@ HK_API size_t hk_mla_tree_workspace_bytes(int m, int n_heads, int n_seqs, int n_
 }
 
 // The 8-bit cache: as it is, or where that is the faster its positions as fp16 rows in the workspace first, a sequence every `cap` rows.  By a model of the
-// time as in mla_tree_shape: a tile takes 1.3 us of a CTA that converts it, a position 0.35 ns to read and write.
+// time as in mla_tree_shape, fitted to 8 shapes: a tile takes 1.3 us of a CTA that converts it, a position 0.35 ns to read and write.
 namespace hk {
 struct Tree8Plan {
   bool read_first, pairs;
@@ -770,22 +770,17 @@ static Tree8Plan tree8_plan(int m, int n_heads, int n_seqs, bool ragged, bool le
     p.n_split = simt_auto_splits(m, n_heads, n_keys);
     return p;
   }
-  p.n_split = units > sm_count() ? 1 : mla8_splits((int)units, n_keys);
+  constexpr TreeCost direct = {{115, 125, 130}, {650, 700, 780}, 800, 300, 500};
+  const int64_t time = tree_best_splits(direct, units, n_keys / 64 + 1, sm_count(), &p.n_split);
   const int64_t cap = lens || positions < n_keys ? positions : n_keys;
   if (group * n_heads != 64 || cap * n_seqs > TREE8_ROWS) return p;
-  const int64_t sms = sm_count(), tiles = n_keys / 64 + 1;
-  auto time = [&](int64_t u, int s, int tile, int start) {
-    const int64_t waves = (u * s + sms - 1) / sms;
-    return waves * ((tiles + s - 1) / s) * tile + (waves - 1) * 150 + start + (s > 1 ? 6 * u * s : 0);
-  };
-  int s;
-  const bool pairs = mla_tree_shape(m, n_seqs, ragged, group, n_keys, &s);
-  const int64_t u = pairs ? 2 * tree_units(m, n_seqs, ragged, 2) : units;
+  int n_split;
+  bool pairs;
   const int64_t read = 300 + (int64_t)n_seqs * n_keys * 35 / 1000;
-  if (read + time(u, s, pairs ? 87 : 100, s == 1 ? (pairs ? 800 : 700) : (pairs ? 950 : 800)) < time(units, p.n_split, 130, p.n_split == 1 ? 700 : 800)) {
+  if (read + mla_tree_shape(m, n_seqs, ragged, group, n_keys, &n_split, &pairs) < time) {
     p.read_first = true;
     p.pairs = pairs;
-    p.n_split = s;
+    p.n_split = n_split;
     p.cap = (int)cap;
     p.rows_bytes = (size_t)cap * n_seqs * LATENT * sizeof(__half);
   }

@@ -141,8 +141,49 @@ __device__ __forceinline__ void pt_body(const MlaArgs& a, int* __restrict__ stat
   int r1 = a.m - 1 - 2 * (int)(blockIdx.x >> 1), r0 = max(0, r1 - 1);
   bool lone = r1 == 0;
   int split = 0;
+  // barriers and tensor memory of both CTAs; in the tree form by warps that have no node to look up
+  auto begin = [&]() {
+    if (tid == (TREE ? 96 : 0)) {
+      for (int b = 0; b < FT_NBUF; b++) {
+        tc::mbar_init(&ms.k_here[b], 1);
+        tc::mbar_init(&ms.v_here[b], 1);
+        tc::mbar_init(&ms.k_full[b], 2);
+        tc::mbar_init(&ms.k_free[b], 1);
+        tc::mbar_init(&ms.v_free[b], 1);
+      }
+      for (int b = 0; b < 2; b++) {
+        tc::mbar_init(&ms.s_full[b], 1);
+        tc::mbar_init(&ms.s_free[b], 8);
+        tc::mbar_init(&ms.p_full[b], 8);
+        tc::mbar_init(&ms.pv_done[b], 1);
+      }
+      tc::mbar_init(&ms.q_full, 1);
+      tc::mbar_init(&ms.q_moved, 4);
+      tc::mbar_init(&ms.q_ready, 8);
+      tc::mbar_fence_init();
+      ms.abort_flag = 0;
+    }
+    if (warp == (TREE ? 2 : 0)) {
+      asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(tc::smem_u32(&ms.tmem)), "r"(512) : "memory");
+      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+    }
+    if (!TREE) pdl_wait();
+    tc::fence_before_sync();
+    __syncwarp();
+    asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
+    tc::fence_after_sync();
+  };
   if (TREE) {
     split = (int)(blockIdx.x >> 1) % a.n_split;
+    if (warp == 6 && lane == 0) {
+      tc::prefetch_map(&tmap_q);
+      tc::prefetch_map(&tmap_k);
+      tc::prefetch_map(&tmap_tree_k);
+    }
+    if (warp == 7 && lane == 0) {
+      tc::prefetch_map(&tmap_v);
+      tc::prefetch_map(&tmap_tree_v);
+    }
     pdl_wait();
     const TreeUnit p = tree_unit(a.tree, (int)(blockIdx.x >> 1) / a.n_split, 2);
     if (p.seq < 0) return;                                 // (both CTAs, before anything of them is in use)
@@ -150,10 +191,10 @@ __device__ __forceinline__ void pt_body(const MlaArgs& a, int* __restrict__ stat
     lone = p.count < 2;
     r1 = lone ? r0 : r0 + 1;
     if (warp < 2) {
-      const MlaTree t = mla_tree(a, warp == 0 ? r0 : r1);
+      const MlaTree t = mla_tree(a, p.seq, make_int2(p.row0, p.size), (warp == 0 ? r0 : r1) - p.row0);
       if (lane == 0) ms.tree[warp] = t;
     }
-    __syncthreads();
+    begin();
   }
   const int row = rank == 0 ? r0 : r1;
   const bool mine = !(lone && rank == 1);
@@ -187,34 +228,7 @@ __device__ __forceinline__ void pt_body(const MlaArgs& a, int* __restrict__ stat
   auto ragged_box = [&](int t) -> bool { return TREE && (t >= whole || a.ckv_rows > 0); };
   const int last_quads = gone >= 0 ? 2 : 1;                // window form: groups of four keys of the last tile (keys 0 and 16)
 
-  if (tid == 0) {
-    for (int b = 0; b < FT_NBUF; b++) {
-      tc::mbar_init(&ms.k_here[b], 1);
-      tc::mbar_init(&ms.v_here[b], 1);
-      tc::mbar_init(&ms.k_full[b], 2);
-      tc::mbar_init(&ms.k_free[b], 1);
-      tc::mbar_init(&ms.v_free[b], 1);
-    }
-    for (int b = 0; b < 2; b++) {
-      tc::mbar_init(&ms.s_full[b], 1);
-      tc::mbar_init(&ms.s_free[b], 8);
-      tc::mbar_init(&ms.p_full[b], 8);
-      tc::mbar_init(&ms.pv_done[b], 1);
-    }
-    tc::mbar_init(&ms.q_full, 1);
-    tc::mbar_init(&ms.q_moved, 4);
-    tc::mbar_init(&ms.q_ready, 8);
-    tc::mbar_fence_init();
-    ms.abort_flag = 0;
-  }
-  if (warp == 0) {
-    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(tc::smem_u32(&ms.tmem)), "r"(512) : "memory");
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
-  }
-  if (!TREE) pdl_wait();
-  tc::fence_before_sync();
-  asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");   // both CTAs' barriers and tensor memory
-  tc::fence_after_sync();
+  if (!TREE) begin();
   const uint32_t tmem = ms.tmem;
   auto first = [&](uint64_t* bar) -> uint32_t { return cluster_addr(tc::smem_u32(bar), 0); };   // the first CTA's
   bool ok = true;
@@ -491,34 +505,18 @@ __device__ __forceinline__ void pt_body(const MlaArgs& a, int* __restrict__ stat
     asm volatile("bar.sync 3, 128;" ::: "memory");
     l += ms.l[tid ^ 64];
     const bool some = (l > 0.f || a.keep_nan) && (!TREE || n_tiles > 0);   // as in mla_flash_tc_kernel
-    if (TREE && !a.out) {
-      // a partial, as there: fp32 rows in the idle ring, one bulk copy per head
-      const uint32_t pitch = LATENT * 4 + 16;
-      uint8_t* orow = smem + FS_K + head * pitch;
-#pragma unroll 1
-      for (int c0 = 0; c0 < 256; c0 += 32) {
-        uint32_t o[32];
-        tc::tmem_ld32(tmem + FT_O + c0 + lanes, o);
-        tc::tmem_ld_wait();
-#pragma unroll
-        for (int v = 0; v < 8; v++)
-          *reinterpret_cast<uint4*>(orow + (half * 256 + c0) * 4 + v * 16) =
-              some ? make_uint4(o[4 * v], o[4 * v + 1], o[4 * v + 2], o[4 * v + 3]) : make_uint4(0u, 0u, 0u, 0u);
-      }
-      tc::fence_async_smem();
-      asm volatile("bar.sync 3, 128;" ::: "memory");
-      const size_t rows = (size_t)a.m * FT_HEADS, rh = (size_t)row * FT_HEADS + head;
-      if (half == 0 && mine && ok && !*abort_flag) {
-        tc::bulk_s2g(a.part_acc + ((size_t)split * rows + rh) * LATENT, orow, LATENT * 4);
-        tc::bulk_commit();
-        a.part_m[(size_t)split * rows + rh] = (m == -INFINITY || !some) ? -INFINITY : m / LOG2E;
-        a.part_l[(size_t)split * rows + rh] = l;
-        tc::bulk_wait_read<0>();
+    if (TREE && half == 0) {                               // (the rows leave below)
+      ms.mx[0][head] = !some ? 0.f : a.out && l > 0.f ? 1.f / l : 1.f;
+      if (!a.out && mine && !*abort_flag) {
+        const size_t at = ((size_t)split * a.m + row) * FT_HEADS + head;
+        a.part_m[at] = (m == -INFINITY || !some) ? -INFINITY : m / LOG2E;
+        a.part_l[at] = l;
       }
     }
+    if (TREE) tc::fence_before_sync();
     const float f = l > 0.f ? 1.f / l : 1.f;
 #pragma unroll 1
-    for (int c0 = 0; c0 < (TREE && !a.out ? 0 : 256); c0 += 64) {
+    for (int c0 = 0; c0 < (TREE ? 0 : 256); c0 += 64) {
       uint8_t* box = smem + FS_P + half * FP_BYTES;
       if (tid == 0) tc::bulk_wait_read<0>();
       asm volatile("bar.sync 3, 128;" ::: "memory");
@@ -551,7 +549,54 @@ __device__ __forceinline__ void pt_body(const MlaArgs& a, int* __restrict__ stat
         tc::bulk_commit();
       }
     }
-    if (tid == 0) tc::bulk_wait_read<0>();
+    if (!TREE && tid == 0) tc::bulk_wait_read<0>();
+  }
+  if constexpr (TREE) {
+    // final rows, or a partial's, through the idle ring, by all eight warps (see mla_tree_tc_kernel)
+    __syncthreads();
+    tc::fence_after_sync();
+    const int quarter = warp & 3, head = (quarter & 1) * 32 + lane, half = quarter >> 1, c_first = warp < 4 ? 0 : 128;
+    const bool final_out = a.out != nullptr;
+    const uint32_t elem = final_out ? 2 : 4, pitch = LATENT * elem + 16;
+    const float f = ms.mx[0][head];
+    if (mine) {
+#pragma unroll 1
+      for (int c = c_first; c < c_first + 128; c += 32) {
+        uint32_t o[32];
+        tc::tmem_ld32(tmem + FT_O + c + ((uint32_t)(quarter * 32) << 16), o);
+        tc::tmem_ld_wait();
+#pragma unroll
+        for (int j = 0; j < 32; j++) o[j] = f != 0.f ? __float_as_uint(__uint_as_float(o[j]) * f) : 0u;
+        uint8_t* dst = smem + FS_K + head * pitch + (half * 256 + c) * elem;
+        if (final_out) {
+#pragma unroll
+          for (int v = 0; v < 4; v++) {
+            uint4 w;
+            uint32_t* wp = &w.x;
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+              const __half2 h2 = __floats2half2_rn(__uint_as_float(o[8 * v + 2 * e]), __uint_as_float(o[8 * v + 2 * e + 1]));
+              wp[e] = *reinterpret_cast<const uint32_t*>(&h2);
+            }
+            *reinterpret_cast<uint4*>(dst + v * 16) = w;
+          }
+        } else {
+#pragma unroll
+          for (int v = 0; v < 8; v++) *reinterpret_cast<uint4*>(dst + v * 16) = make_uint4(o[4 * v], o[4 * v + 1], o[4 * v + 2], o[4 * v + 3]);
+        }
+      }
+    }
+    __syncthreads();
+    if (mine && !*abort_flag) {
+      uint8_t* dst = final_out ? reinterpret_cast<uint8_t*>(a.out + (size_t)row * FT_HEADS * LATENT)
+                               : reinterpret_cast<uint8_t*>(a.part_acc + ((size_t)split * a.m + row) * FT_HEADS * LATENT);
+      const int lg = final_out ? 6 : 7;                    // 16-byte pieces of a head
+#pragma unroll 8
+      for (int i = tid; i < FT_HEADS << lg; i += PT_THREADS) {
+        const int h = i >> lg, c = i & ((1 << lg) - 1);
+        reinterpret_cast<uint4*>(dst)[i] = *reinterpret_cast<const uint4*>(smem + FS_K + h * pitch + c * 16);
+      }
+    }
   }
   // Behind a wait that gave up the loops above ran on: what they asked for ends first (far less than a millisecond).
   if (*abort_flag)
@@ -559,7 +604,7 @@ __device__ __forceinline__ void pt_body(const MlaArgs& a, int* __restrict__ stat
   tc::fence_before_sync();
   __syncwarp();
   asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");   // nothing of either CTA is in use any more
-  if (warp == 0) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
+  if (warp == (TREE ? 2 : 0)) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
   if (tid == 0 && ms.abort_flag && status) atomicExch(status, HK_ERR_TIMEOUT);
 }
 
