@@ -20,6 +20,7 @@ namespace {
 
 constexpr int PG_MAX_CTAS = 8, PG_THREADS = 1024, PG_CTA_WARPS = PG_THREADS / 32;
 constexpr int PG_AHEAD = 8;                       // loads of a lane on their way
+constexpr int PG_LOCAL = 1024;                    // lists up to here stay in shared memory
 constexpr int PG_SMALL = PG_CTA_WARPS * 32 * PG_AHEAD;   // blocks of a pool that one CTA looks after
 
 struct PagesArgs {
@@ -88,22 +89,27 @@ __global__ __launch_bounds__(128) void pages_free_kernel(PagesArgs a) {
 
 // Blocks [b0, b1) of this warp, in ascending order over the cluster's warps.
 struct PagesPart {
-  int64_t b0, b1;
+  int b0, b1;
 };
 template <int CTAS>
 __device__ __forceinline__ PagesPart pg_part(const PagesArgs& a, int gw) {
   constexpr int WARPS = CTAS * PG_CTA_WARPS;
-  const int64_t each = (a.pg.n_blocks + WARPS * 32 - 1) / (WARPS * 32) * 32;
-  return {min(gw * each, a.pg.n_blocks), min((gw + 1) * each, a.pg.n_blocks)};
+  const int n = (int)a.pg.n_blocks, each = (n + WARPS * 32 - 1) / (WARPS * 32) * 32;   // (a pool has at most 2^27 blocks)
+  return {min(gw * each, n), min((gw + 1) * each, n)};
 }
 // A warp's part of refs, 32 blocks at a time.  One CTA: at most PG_SMALL blocks, a warp's part is read once and stays in registers.
 template <int CTAS>
 struct PagesWalk {
   PagesPart p;
   int r[PG_AHEAD];
-  __device__ __forceinline__ void load(const PagesArgs& a, int64_t b) {
+  __device__ __forceinline__ void load(const PagesArgs& a, int b) {
+    const int lane = threadIdx.x & 31;
 #pragma unroll
-    for (int u = 0; u < PG_AHEAD; u++) r[u] = b + 32 * u + (int)(threadIdx.x & 31) < p.b1 ? a.refs[b + 32 * u + (threadIdx.x & 31)] : 0;
+    for (int u = 0; u < PG_AHEAD; u++) {
+      r[u] = 0;
+      if (b + 32 * u >= p.b1) continue;                    // (the whole warp)
+      if (b + 32 * u + lane < p.b1) r[u] = a.refs[b + 32 * u + lane];
+    }
   }
   __device__ __forceinline__ PagesWalk(const PagesArgs& a, int gw) : p(pg_part<CTAS>(a, gw)) {
     if (CTAS == 1) load(a, p.b0);
@@ -112,11 +118,11 @@ struct PagesWalk {
   template <class F>
   __device__ __forceinline__ void operator()(const PagesArgs& a, F f) {
     const int lane = threadIdx.x & 31;
-    for (int64_t b = p.b0; b < p.b1; b += 32 * PG_AHEAD) {
+    for (int b = p.b0; b < p.b1; b += 32 * PG_AHEAD) {
       if (CTAS > 1) load(a, b);
 #pragma unroll
       for (int u = 0; u < PG_AHEAD; u++)
-        if (b + 32 * u < p.b1) f((int)(b + 32 * u) + lane, r[u], b + 32 * u + lane < p.b1);
+        if (b + 32 * u < p.b1) f(b + 32 * u + lane, r[u], b + 32 * u + lane < p.b1);
     }
   }
 };
@@ -150,10 +156,9 @@ __device__ __forceinline__ int2 pg_before(int mine, int* s_count, int* s_sum) {
   pg_barrier<CTAS>();                                      // the numbers have been read
   return make_int2(before, all);
 }
-// The first `want` free blocks, ascending, into a.list; how many there are.  Executed by all threads.
+// The first `want` free blocks, ascending, into `list`; how many there are.  Executed by all threads.
 template <int CTAS>
-__device__ __forceinline__ int pg_free_list(const PagesArgs& a, int gw, int want, int* s_count, int* s_sum) {
-  PagesWalk<CTAS> walk(a, gw);
+__device__ __forceinline__ int pg_free_list(const PagesArgs& a, PagesWalk<CTAS>& walk, int* list, int want, int* s_count, int* s_sum) {
   const int lane = threadIdx.x & 31;
   int mine = 0;
   walk(a, [&](int, int r, bool in) { mine += __popc(__ballot_sync(0xffffffffu, in && r == 0)); });
@@ -163,7 +168,7 @@ __device__ __forceinline__ int pg_free_list(const PagesArgs& a, int gw, int want
     walk(a, [&](int b, int r, bool in) {
       const uint32_t free = __ballot_sync(0xffffffffu, in && r == 0);
       const int i = at + __popc(free & ((1u << lane) - 1));
-      if ((free >> lane & 1) && i < want) a.list[i] = b;
+      if ((free >> lane & 1) && i < want) list[i] = b;
       at += __popc(free);
     });
   return min(c.y, want);
@@ -173,18 +178,20 @@ template <int MODE, int CTAS>
 __global__ __launch_bounds__(PG_THREADS) void pages_kernel(PagesArgs a) {
   constexpr int WARPS = CTAS * PG_CTA_WARPS;
   __shared__ int s_count[PG_CTA_WARPS], s_sum[PG_MAX_CTAS];
+  __shared__ int s_want[PG_CTA_WARPS];                     // fork
+  __shared__ int s_src[MODE != PG_COMPACT && CTAS == 1 ? PG_LOCAL : 1], s_list[MODE != PG_COMPACT && CTAS == 1 ? PG_LOCAL : 1];
   pdl_release();
   pdl_wait();
+  // short lists of one CTA stay in shared memory
+  const bool local = CTAS == 1 && a.n <= PG_LOCAL;
+  int* const src = local ? s_src : a.src;
   const int lane = threadIdx.x & 31, gw = (int)(blockIdx.x * PG_CTA_WARPS + (threadIdx.x >> 5)), stride = a.pg.table_stride;
   auto row = [&](int s) -> int* { return a.table + (size_t)s * stride; };
   if constexpr (MODE == PG_FORK) {
     auto pair = [&](int i) { return pg_seq(a, a.seqs[i]) && pg_seq(a, a.from[i]) && a.seqs[i] != a.from[i]; };
-    for (int i = gw; i < a.n; i += WARPS)
-      if (pair(i)) pg_release(a, a.seqs[i], 0, PG_TURN);
-    pg_barrier<CTAS>();
     // the block that a pair copies, -1: none
-    int want = 0;
-    for (int i0 = 0; i0 < a.n; i0 += 32) {
+    int want = 0;                                          // one CTA: every warp its part of the pairs
+    for (int i0 = CTAS == 1 ? gw * 32 : 0; i0 < a.n; i0 += CTAS == 1 ? WARPS * 32 : 32) {
       const int i = i0 + lane;
       int e = -1;
       if (i < a.n && pair(i)) {
@@ -193,32 +200,46 @@ __global__ __launch_bounds__(PG_THREADS) void pages_kernel(PagesArgs a) {
         if (!pg_block(a, e)) e = -1;
       }
       want += __popc(__ballot_sync(0xffffffffu, e >= 0));
-      if (gw == 0 && i < a.n) a.src[i] = e;
+      if ((CTAS == 1 || gw == 0) && i < a.n) {
+        if (local) s_src[i] = e;
+        a.src[i] = e;
+      }
     }
-    const int have = pg_free_list<CTAS>(a, gw, want, s_count, s_sum);
+    if (CTAS == 1 && lane == 0) s_want[gw] = want;
+    for (int i = WARPS - 1 - gw; i < a.n; i += WARPS)      // (from the last warp on: the first ones have pairs)
+      if (pair(i)) pg_release(a, a.seqs[i], 0, PG_TURN);
     pg_barrier<CTAS>();
-    for (int i = gw; i < a.n; i += WARPS) {
-      int before = 0;
-      for (int k0 = 0; k0 < i; k0 += 32) before += __popc(__ballot_sync(0xffffffffu, k0 + lane < i && a.src[k0 + lane] >= 0));
-      const int e = a.src[i], fresh = e >= 0 && before < have ? a.list[before] : -1;
-      if (lane == 0) a.dst[i] = fresh;
-      if (!pair(i)) continue;
-      const int whole = pg_whole(a, a.lens[i]);
-      const int* from = row(a.from[i]);
-      int* to = row(a.seqs[i]);
-      for (int j0 = 0; j0 < whole; j0 += PG_TURN) {
+    if (CTAS == 1) want = __reduce_add_sync(0xffffffffu, s_want[lane]);
+    PagesWalk<CTAS> walk(a, gw);
+    int* const list = local ? s_list : a.list;             // (at most one a pair)
+    const int have = pg_free_list<CTAS>(a, walk, list, want, s_count, s_sum);
+    pg_barrier<CTAS>();
+    const int turns = (stride + PG_TURN - 1) / PG_TURN;    // a warp has 128 entries of a child
+    for (int64_t item = gw; item < (int64_t)a.n * turns; item += WARPS) {
+      const int i = (int)(item / turns), j0 = (int)(item - (int64_t)i * turns) * PG_TURN;
+      const bool both = pair(i);
+      const int whole = both ? pg_whole(a, a.lens[i]) : 0;
+      if (both && j0 < whole) {
         int b[PG_ROW];
-        pg_row(from, j0, whole, b);
+        pg_row(row(a.from[i]), j0, whole, b);
+        int* to = row(a.seqs[i]) + j0 + lane;
 #pragma unroll
         for (int u = 0; u < PG_ROW; u++) {
           if (!pg_block(a, b[u])) continue;
           atomicAdd(a.refs + b[u], 1);
-          to[j0 + 32 * u + lane] = b[u];
+          to[32 * u] = b[u];
         }
       }
-      if (lane == 0 && fresh >= 0) {
-        to[whole] = fresh;
-        a.refs[fresh] = 1;
+      if (j0 > 0) continue;
+      int before = 0;
+      for (int k0 = 0; k0 < i; k0 += 32) before += __popc(__ballot_sync(0xffffffffu, k0 + lane < i && src[k0 + lane] >= 0));
+      const int e = src[i], fresh = e >= 0 && before < have ? list[before] : -1;
+      if (lane == 0) {
+        a.dst[i] = fresh;
+        if (fresh >= 0) {
+          row(a.seqs[i])[whole] = fresh;
+          a.refs[fresh] = 1;
+        }
       }
     }
     if (gw == 0 && lane == 0) {
@@ -226,6 +247,7 @@ __global__ __launch_bounds__(PG_THREADS) void pages_kernel(PagesArgs a) {
       if (a.told) *a.told = want - have;
     }
   } else if constexpr (MODE == PG_RESERVE) {
+    PagesWalk<CTAS> walk(a, gw);                           // (on its way with the rows)
     // entries without a block, by sequence of the call
     for (int i = gw; i < a.n; i += WARPS) {
       const int s = a.seqs[i], all = pg_seq(a, s) ? pg_entries(a, a.lens[i]) : 0;
@@ -236,20 +258,21 @@ __global__ __launch_bounds__(PG_THREADS) void pages_kernel(PagesArgs a) {
 #pragma unroll
         for (int u = 0; u < PG_ROW; u++) need += __popc(__ballot_sync(0xffffffffu, j0 + 32 * u + lane < all && !pg_block(a, e[u])));
       }
-      if (lane == 0) a.src[i] = need;
+      if (lane == 0) src[i] = need;
     }
     pg_barrier<CTAS>();
     int64_t want = 0;
     for (int i0 = 0; i0 < a.n; i0 += 32) {
-      const int v = i0 + lane < a.n ? a.src[i0 + lane] : 0;
+      const int v = i0 + lane < a.n ? src[i0 + lane] : 0;
       want += __reduce_add_sync(0xffffffffu, v);
     }
-    const int have = pg_free_list<CTAS>(a, gw, (int)min(want, a.pg.n_blocks), s_count, s_sum);
+    int* const list = local && want <= PG_LOCAL ? s_list : a.list;
+    const int have = pg_free_list<CTAS>(a, walk, list, (int)min(want, a.pg.n_blocks), s_count, s_sum);
     pg_barrier<CTAS>();
     for (int i = gw; i < a.n; i += WARPS) {
       const int s = a.seqs[i], all = pg_seq(a, s) ? pg_entries(a, a.lens[i]) : 0;
       int64_t at = 0;
-      for (int k0 = 0; k0 < i; k0 += 32) at += __reduce_add_sync(0xffffffffu, k0 + lane < i ? a.src[k0 + lane] : 0);
+      for (int k0 = 0; k0 < i; k0 += 32) at += __reduce_add_sync(0xffffffffu, k0 + lane < i ? src[k0 + lane] : 0);
       for (int j0 = 0; j0 < all; j0 += PG_TURN) {
         int e[PG_ROW], b[PG_ROW];
         pg_row(row(s), j0, all, e);
@@ -257,7 +280,7 @@ __global__ __launch_bounds__(PG_THREADS) void pages_kernel(PagesArgs a) {
         for (int u = 0; u < PG_ROW; u++) {
           const uint32_t open = __ballot_sync(0xffffffffu, j0 + 32 * u + lane < all && !pg_block(a, e[u]));
           const int64_t k = at + __popc(open & ((1u << lane) - 1));
-          b[u] = (open >> lane & 1) && k < have ? a.list[k] : -1;
+          b[u] = (open >> lane & 1) && k < have ? list[k] : -1;
           at += __popc(open);
         }
 #pragma unroll
@@ -280,7 +303,7 @@ __global__ __launch_bounds__(PG_THREADS) void pages_kernel(PagesArgs a) {
     int beyond = 0;                                        // this warp's live blocks at or beyond `live`
     if (p.b1 > live) walk(a, [&](int b, int r, bool in) { beyond += __popc(__ballot_sync(0xffffffffu, in && r != 0 && b >= live)); });
     const int2 m = pg_before<CTAS>(beyond, s_count, s_sum);
-    int hole = (int)min(p.b0, (int64_t)live) - (c.x - m.x), move = m.x;   // free blocks below `live` before this warp's
+    int hole = min(p.b0, live) - (c.x - m.x), move = m.x;   // free blocks below `live` before this warp's
     walk(a, [&](int b, int r, bool in) {
       const uint32_t up = __ballot_sync(0xffffffffu, in && r != 0 && b >= live), down = __ballot_sync(0xffffffffu, in && r == 0 && b < live);
       if (up >> lane & 1) a.src[move + __popc(up & ((1u << lane) - 1))] = b;
