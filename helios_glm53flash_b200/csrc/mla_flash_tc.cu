@@ -1034,7 +1034,7 @@ int mla_flash_tc_launch(const MlaArgs& a, cudaStream_t s, bool clusters) {
   // Nodes of trees by twos: see mla_tree_shape.
   const bool tree_pairs = a.tree_kv && a.tree_pairs;
   if (!box_map(&qmap, a.q_lat, q_rows) || (!a.raw_idx && !pairs && !tree_pairs && !box_map(&box, a.ckv, extent))) return HK_ERR_UNSUPPORTED;
-  if (a.out) {
+  if (a.out && !a.tree_kv) {
     const cuuint64_t dims[2] = {LATENT, q_rows};
     const cuuint64_t strides[1] = {LATENT * 2};
     const cuuint32_t b[2] = {64, 64};
