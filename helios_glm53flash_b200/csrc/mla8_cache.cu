@@ -282,14 +282,15 @@ __global__ void __launch_bounds__(256) mla8_read_kernel(MlaPaged pg, int head, i
   }
 }
 
-// The first positions of every sequence, lens[s] (or len) of them and `cap` at most, as fp16 rows from row s * cap on; grid (CTAs of a sequence, sequences).
+// The first positions of every sequence, lens[s] (or len) of them and `cap` at most, as fp16 rows from row s * cap on and a factor each (mla_scale_power:
+// the rows are exact; scale * value as fp16 cost attention two fifths of its precision over a few hundred keys); grid (CTAs of a sequence, sequences).
 template <int FMT>
-__global__ void __launch_bounds__(256) mla8_read_seqs_kernel(MlaPaged pg, const int* lens, int len, int cap, __half* out) {
+__global__ void __launch_bounds__(256) mla8_read_seqs_kernel(MlaPaged pg, const int* lens, int len, int cap, __half* out, float* factor, int64_t factor_stride) {
   pdl_release();
   pdl_wait();
-  const int lane = threadIdx.x & 31, seq = blockIdx.y, n = min(lens ? lens[seq] : len, cap);
+  const int lane = threadIdx.x & 31, seq = blockIdx.y, n = min(lens ? lens[seq] : len, cap), whole = (n + 63) & ~63;
   __half* rows = out + (size_t)seq * cap * LATENT;
-  for (int64_t first = ((int64_t)blockIdx.x * 8 + (threadIdx.x >> 5)) * READ_ROWS; first < n; first += (int64_t)gridDim.x * 8 * READ_ROWS) {
+  for (int64_t first = ((int64_t)blockIdx.x * 8 + (threadIdx.x >> 5)) * READ_ROWS; first < whole; first += (int64_t)gridDim.x * 8 * READ_ROWS) {
     const int i0 = (int)first;
     uint2 v[READ_ROWS][2];
     float s[READ_ROWS];
@@ -297,7 +298,7 @@ __global__ void __launch_bounds__(256) mla8_read_seqs_kernel(MlaPaged pg, const 
     for (int k = 0; k < READ_ROWS; k++) {
       const int i = i0 + k;
       const int64_t b = i < n ? pg.block_of(seq, i) : -1;
-      s[k] = 0.f;
+      s[k] = 1.f;
       v[k][0] = v[k][1] = make_uint2(0u, 0u);
       if (b >= 0) {
         const uint2* row = reinterpret_cast<const uint2*>(pg.data + (((size_t)b << pg.shift) + (i & ((1 << pg.shift) - 1))) * LATENT);
@@ -308,14 +309,17 @@ __global__ void __launch_bounds__(256) mla8_read_seqs_kernel(MlaPaged pg, const 
     }
 #pragma unroll
     for (int k = 0; k < READ_ROWS; k++) {
-      if (i0 + k >= n) break;
+      float f;
+      const float power = mla_scale_power(s[k], &f);
+      if (lane == 0 && i0 + k < whole) factor[seq * factor_stride + i0 + k] = f;
+      if (i0 + k >= n) continue;
 #pragma unroll
       for (int h = 0; h < 2; h++) {
         const uint8_t* v8 = reinterpret_cast<const uint8_t*>(&v[k][h]);
         uint4 w;
         __half2* w2 = reinterpret_cast<__half2*>(&w);
 #pragma unroll
-        for (int c = 0; c < 4; c++) w2[c] = __floats2half2_rn(latent8_value<FMT>(v8[2 * c]) * s[k], latent8_value<FMT>(v8[2 * c + 1]) * s[k]);
+        for (int c = 0; c < 4; c++) w2[c] = __floats2half2_rn(latent8_value<FMT>(v8[2 * c]) * power, latent8_value<FMT>(v8[2 * c + 1]) * power);
         reinterpret_cast<uint4*>(rows + (size_t)(i0 + k) * LATENT)[lane + 32 * h] = w;
       }
     }
@@ -354,10 +358,11 @@ int mla8_read_launch(const MlaPaged& pg, int dtype, int head, int shift, int n, 
 }
 
 // the sequences' positions for a tree call, about n_keys each
-int mla8_read_seqs_launch(const MlaPaged& pg, int dtype, const int* lens, int len, int cap, int n_keys, __half* out, cudaStream_t s) {
+int mla8_read_seqs_launch(const MlaPaged& pg, int dtype, const int* lens, int len, int cap, int n_keys, __half* out, float* factor, int64_t factor_stride,
+                          cudaStream_t s) {
   const int64_t ctas = ((int64_t)n_keys + 8 * READ_ROWS - 1) / (8 * READ_ROWS);
   return pdl_launch(dtype == HK_I8 ? mla8_read_seqs_kernel<CACHE_I8> : mla8_read_seqs_kernel<CACHE_E4M3>, dim3((unsigned)ctas, (unsigned)pg.n_seqs), dim3(256), 0, s, pg,
-                    lens, len, cap, out) == cudaSuccess
+                    lens, len, cap, out, factor, factor_stride) == cudaSuccess
              ? HK_OK
              : HK_ERR_CUDA;
 }

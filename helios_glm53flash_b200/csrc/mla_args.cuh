@@ -30,6 +30,8 @@ struct MlaArgs {
   // trees of drafted tokens: row r is a node of tree.seq_of(r), whose cached keys kv_base and kv_len (then per sequence) say
   TreeArgs tree;
   int64_t kv_stride;        // without kv_base: a sequence's rows begin at this times its number and end before the next one's (0: all at row 0)
+  const float* kv_factor;   // or null: what the cached rows are still to be multiplied by, [sequences][factor_stride]
+  int64_t factor_stride;    // a multiple of 64; up to the next multiple of 64 behind a sequence's length they are 1
   const __half* tree_kv;    // [m][512] the nodes' own latents
   bool tree_pairs;          // two nodes to a pair of CTAs
   int tree_group;           // otherwise: neighbouring nodes that share a CTA's 64 query rows (64 / heads)
@@ -60,6 +62,19 @@ struct MlaPaged {
     return s >= n_seqs ? -1 : s;
   }
 };
+
+// A scale as a power of two that 8-bit values times it fit in fp16 with, exactly, and the factor that is left: 1 to 2 for scales of 2^-15 up to 2^8
+__device__ __forceinline__ float mla_scale_power(float s, float* factor) {
+  const int e = min(max((int)(__float_as_uint(s) >> 23 & 255) - 127, -15), 7);
+  *factor = s * __uint_as_float((uint32_t)(127 - e) << 23);
+  return __uint_as_float((uint32_t)(127 + e) << 23);
+}
+// 32 factors of a thread's keys, asked for where they stand
+__device__ __forceinline__ void mla_factors(const float* p, float4 (&f)[8]) {
+#pragma unroll
+  for (int j = 0; j < 8; j++)
+    asm volatile("ld.global.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(f[j].x), "=f"(f[j].y), "=f"(f[j].z), "=f"(f[j].w) : "l"(p + 4 * j));
+}
 
 // A row that is a node of a tree of drafted tokens: its sequence's cached keys, then the nodes of its path (a bit each) out of the tree's rows.
 struct MlaTree {

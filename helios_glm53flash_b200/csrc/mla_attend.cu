@@ -22,7 +22,7 @@ size_t mla8_units_bytes(int units, int m, int n_heads, MlaArgs* a, void* workspa
 // implemented in mla8_cache.cu
 int mla8_read_launch(const MlaPaged& pg, int dtype, int head, int shift, int n, __half* out, cudaStream_t s, const int* idx = nullptr, int64_t n_idx = 0,
                      int* idx_out = nullptr);
-int mla8_read_seqs_launch(const MlaPaged& pg, int dtype, const int* lens, int len, int cap, int n_keys, __half* out, cudaStream_t s);
+int mla8_read_seqs_launch(const MlaPaged& pg, int dtype, const int* lens, int len, int cap, int n_keys, __half* out, float* factor, int64_t factor_stride, cudaStream_t s);
 bool mla8_paged(MlaPaged* pg, const void* ckv8, const float* scales, int dtype, int64_t n_blocks, int block, const int* block_table,
                 int table_stride, int n_seqs, const int* row_seq);
 bool mla_flash_cluster_shape(int m, int tiles, int* n_split);
@@ -753,15 +753,16 @@ HK_API size_t hk_mla_tree_workspace_bytes(int m, int n_heads, int n_seqs, int n_
   return most > 1 ? hk_mla_partial_bytes(most, (int64_t)m * n_heads) : 0;
 }
 
-// The 8-bit cache: as it is, or where that is the faster its positions as fp16 rows in the workspace first, a sequence every `cap` rows.  By a model of the
+// The 8-bit cache: as it is, or where that is the faster its positions as fp16 rows and factors in the workspace first, a sequence every `cap` rows.  By a model of the
 // time as in mla_tree_shape, fitted to 8 shapes: a tile takes 1.3 us of a CTA that converts it, a position 0.35 ns to read and write.
 namespace hk {
 struct Tree8Plan {
   bool read_first, pairs;
   int n_split, cap;
-  size_t rows_bytes;
+  size_t factors, rows_bytes;             // where the factors are, and where they end
 };
 constexpr int64_t TREE8_ROWS = (int64_t)1 << 20;           // positions that are read first, at most: 1 GB of workspace
+static size_t tree8_factors(int cap) { return ((size_t)cap + 63) / 64 * 64; }   // of a sequence
 static Tree8Plan tree8_plan(int m, int n_heads, int n_seqs, bool ragged, bool lens, int n_keys, int64_t positions) {
   Tree8Plan p{};
   const int group = tree_group(n_heads);
@@ -782,7 +783,8 @@ static Tree8Plan tree8_plan(int m, int n_heads, int n_seqs, bool ragged, bool le
     p.pairs = pairs;
     p.n_split = n_split;
     p.cap = (int)cap;
-    p.rows_bytes = (size_t)cap * n_seqs * LATENT * sizeof(__half);
+    p.factors = ((size_t)cap * n_seqs * LATENT * sizeof(__half) + 255) / 256 * 256;
+    p.rows_bytes = p.factors + tree8_factors(p.cap) * n_seqs * sizeof(float);   // (256 bytes each 64)
   }
   return p;
 }
@@ -832,7 +834,9 @@ HK_API int hk_mla8_tree(const void* q_lat, const void* ckv8, const float* scales
   if (!p.read_first) return attend8(a, pg, dtype, keys, p.n_split, workspace, workspace_bytes, as_stream(stream));
   if (!workspace || workspace_bytes < p.rows_bytes) return HK_ERR_WORKSPACE;
   if (!aligned(workspace, 256)) return HK_ERR_INVALID;
-  const int st = mla8_read_seqs_launch(pg, dtype, kv_len, pos_start, p.cap, keys, (__half*)workspace, as_stream(stream));
+  a.kv_factor = (const float*)((const char*)workspace + p.factors);
+  a.factor_stride = (int64_t)tree8_factors(p.cap);
+  const int st = mla8_read_seqs_launch(pg, dtype, kv_len, pos_start, p.cap, keys, (__half*)workspace, const_cast<float*>(a.kv_factor), a.factor_stride, as_stream(stream));
   if (st != HK_OK) return st;
   a.ckv = (const __half*)workspace;
   a.ckv_rows = (int64_t)p.cap * n_seqs;

@@ -232,7 +232,8 @@ __device__ __forceinline__ void tma_gather4_rows(uint32_t leader, uint32_t smem_
 // The tree's tile is the last of the list: of its 64 slots those on the nodes' paths are gathered out of a.tree_kv (tmap_tree), the others are zeros,
 // whatever lies there; each head's row sees those on its own node's.  (As a box whose unseen rows are cleared ahead of P V, as
 // mla_pair_tree_tc_kernel takes it, this tile and a ragged one were no faster here, and the look at the mask cost long rows 3 %.)
-template <bool G4, bool CL, bool WIN, int PARTS, bool TREE>
+// FACT: with a.kv_factor, factors of a cached key's score and of its weight.
+template <bool G4, bool CL, bool WIN, int PARTS, bool TREE, bool FACT = false>
 __device__ __forceinline__ void ft_body(const MlaArgs& a, int* __restrict__ status, const CUtensorMap& tmap_box, const CUtensorMap& tmap_rows,
                                         const CUtensorMap& tmap_q, const CUtensorMap& tmap_o, const CUtensorMap& tmap_tree) {
   extern __shared__ __align__(1024) uint8_t smem_raw[];
@@ -546,8 +547,17 @@ __device__ __forceinline__ void ft_body(const MlaArgs& a, int* __restrict__ stat
     for (int idx = blockIdx.x; idx < n_items; idx += step) {
       const FtItem it = item(idx);
       float m = -INFINITY, l = 0.f;
+      const float* const factor = FACT ? a.kv_factor + ms.tree.seq * a.factor_stride + 32 * half : nullptr;
+      float4 fac[8], fac_next[8];                          // of this tile's 32 keys of this thread, of the next one's
+      if (FACT && it.n_tiles > 0 && !it.drafted(0)) mla_factors(factor + it.key0(0), fac_next);
       for (int tile = 0; tile < it.n_tiles; tile++, u++, g++) {
         const int b = g & 1, kb = slot_of(it, u, tile);
+        if (FACT) {
+#pragma unroll
+          for (int j = 0; j < 8; j++) fac[j] = it.drafted(tile) ? make_float4(1.f, 1.f, 1.f, 1.f) : fac_next[j];
+          if (tile + 1 < it.n_tiles && !it.drafted(tile + 1)) mla_factors(factor + it.key0(tile + 1), fac_next);
+        }
+        auto fac_of = [&](int j) -> float { return j % 4 == 0 ? fac[j / 4].x : j % 4 == 1 ? fac[j / 4].y : j % 4 == 2 ? fac[j / 4].z : fac[j / 4].w; };
         ok = tc::mbar_wait<FT_POLL_NS>(full_of(kb), turn_of(it, u, tile) & 1, abort_flag, 6) && ok;   // makes the tile's mask visible
         ok = tc::mbar_wait<FT_POLL_NS>(&ms.s_full[b], (g >> 1) & 1, abort_flag, 7) && ok;
         tc::fence_after_sync();
@@ -580,7 +590,7 @@ __device__ __forceinline__ void ft_body(const MlaArgs& a, int* __restrict__ stat
         float tmax = -INFINITY;
 #pragma unroll
         for (int j = 0; j < 32; j++) {
-          const float v = (mask >> j) & 1u ? __uint_as_float(sv[j]) * sc2 : -INFINITY;
+          const float v = (mask >> j) & 1u ? __uint_as_float(sv[j]) * (FACT ? fac_of(j) * sc2 : sc2) : -INFINITY;
           sv[j] = __float_as_uint(v);
           tmax = fmaxf(tmax, v);
         }
@@ -625,7 +635,7 @@ __device__ __forceinline__ void ft_body(const MlaArgs& a, int* __restrict__ stat
           for (int e = 0; e < 4; e++) {
             const float p0 = exp2f(__uint_as_float(sv[8 * v + 2 * e]) - mref), p1 = exp2f(__uint_as_float(sv[8 * v + 2 * e + 1]) - mref);
             sum += p0 + p1;
-            const __half2 hp = __floats2half2_rn(p0, p1);
+            const __half2 hp = FACT ? __floats2half2_rn(p0 * fac_of(8 * v + 2 * e), p1 * fac_of(8 * v + 2 * e + 1)) : __floats2half2_rn(p0, p1);
             wp[e] = *reinterpret_cast<const uint32_t*>(&hp);
           }
           *reinterpret_cast<uint4*>(prow + tc::sw128_off(head, half * 4 + v, FT_BLK)) = w;
@@ -863,11 +873,11 @@ __global__ __launch_bounds__(FT_THREADS, 1) void mla_flash_tc_kernel(
     const __grid_constant__ CUtensorMap tmap_q, const __grid_constant__ CUtensorMap tmap_o) {
   ft_body<G4, CL, WIN, PARTS, false>(a, status, tmap_box, tmap_rows, tmap_q, tmap_o, tmap_rows);
 }
-template <int PARTS>
+template <int PARTS, bool FACT>
 __global__ __launch_bounds__(FT_THREADS, 1) void mla_tree_tc_kernel(
     MlaArgs a, int* __restrict__ status, const __grid_constant__ CUtensorMap tmap_box, const __grid_constant__ CUtensorMap tmap_rows,
     const __grid_constant__ CUtensorMap tmap_q, const __grid_constant__ CUtensorMap tmap_o, const __grid_constant__ CUtensorMap tmap_tree) {
-  ft_body<false, false, false, PARTS, true>(a, status, tmap_box, tmap_rows, tmap_q, tmap_o, tmap_tree);
+  ft_body<false, false, false, PARTS, true, FACT>(a, status, tmap_box, tmap_rows, tmap_q, tmap_o, tmap_tree);
 }
 
 }  // namespace hk
@@ -921,8 +931,9 @@ static int ft_prepare() {
         !whole_sm(mla_flash_tc_kernel<false, true, false>) || !whole_sm(mla_flash_tc_kernel<true, true, false>) ||
         !whole_sm(mla_flash_tc_kernel<false, false, true>) || !whole_sm(mla_flash_tc_kernel<false, false, true, 2>) ||
         !whole_sm(mla_flash_tc_kernel<false, false, true, 4>) || !whole_sm(mla_flash_tc_kernel<false, true, true>) || !whole_sm(mla_pair_tc_kernel<false>) ||
-        !whole_sm(mla_pair_tc_kernel<true>) || !whole_sm(mla_tree_tc_kernel<1>) || !whole_sm(mla_tree_tc_kernel<2>) || !whole_sm(mla_tree_tc_kernel<4>) ||
-        !whole_sm(mla_pair_tree_tc_kernel) ||
+        !whole_sm(mla_pair_tc_kernel<true>) || !whole_sm(mla_tree_tc_kernel<1, false>) || !whole_sm(mla_tree_tc_kernel<2, false>) ||
+        !whole_sm(mla_tree_tc_kernel<4, false>) || !whole_sm(mla_tree_tc_kernel<1, true>) || !whole_sm(mla_tree_tc_kernel<2, true>) ||
+        !whole_sm(mla_tree_tc_kernel<4, true>) || !whole_sm(mla_pair_tree_tc_kernel<false>) || !whole_sm(mla_pair_tree_tc_kernel<true>) ||
         !any_cluster(mla_flash_tc_kernel<false, true, false>) || !any_cluster(mla_flash_tc_kernel<true, true, false>) ||
         !any_cluster(mla_flash_tc_kernel<false, true, true>))
       return HK_ERR_CUDA;
@@ -1048,8 +1059,8 @@ int mla_flash_tc_launch(const MlaArgs& a, cudaStream_t s, bool clusters) {
         !box_map(&tree_v, a.tree_kv, a.m, 32, 4))
       return HK_ERR_UNSUPPORTED;
     const int64_t n_pairs = tree_units(a.m, a.tree.n_seqs, a.tree.start, 2);
-    const cudaError_t e = pdl_launch_cluster(2, mla_pair_tree_tc_kernel, dim3((unsigned)(2 * n_pairs * a.n_split)), dim3(PT_THREADS), FS_SMEM, s, a, device_status_ptr(), box, vbox,
-                                             rows, qmap, omap, tree_k, tree_v);
+    const cudaError_t e = pdl_launch_cluster(2, a.kv_factor ? mla_pair_tree_tc_kernel<true> : mla_pair_tree_tc_kernel<false>, dim3((unsigned)(2 * n_pairs * a.n_split)), dim3(PT_THREADS),
+                                             FS_SMEM, s, a, device_status_ptr(), box, vbox, rows, qmap, omap, tree_k, tree_v);
     return e == cudaSuccess && cudaPeekAtLastError() == cudaSuccess ? HK_OK : HK_ERR_CUDA;
   }
   if (pairs) {
@@ -1077,7 +1088,8 @@ int mla_flash_tc_launch(const MlaArgs& a, cudaStream_t s, bool clusters) {
   if (a.tree_kv) {
     alignas(64) CUtensorMap tree;
     if (!rows_map(&tree, a.tree_kv, a.m)) return HK_ERR_UNSUPPORTED;
-    const auto kernel = parts == 1 ? mla_tree_tc_kernel<1> : parts == 2 ? mla_tree_tc_kernel<2> : mla_tree_tc_kernel<4>;
+    const auto kernel = a.kv_factor ? (parts == 1 ? mla_tree_tc_kernel<1, true> : parts == 2 ? mla_tree_tc_kernel<2, true> : mla_tree_tc_kernel<4, true>)
+                                    : (parts == 1 ? mla_tree_tc_kernel<1, false> : parts == 2 ? mla_tree_tc_kernel<2, false> : mla_tree_tc_kernel<4, false>);
     const cudaError_t e = pdl_launch(kernel, dim3((unsigned)items), dim3(FT_THREADS), FS_SMEM, s, a, device_status_ptr(), box, rows, qmap, omap, tree);
     return e == cudaSuccess && cudaPeekAtLastError() == cudaSuccess ? HK_OK : HK_ERR_CUDA;
   }

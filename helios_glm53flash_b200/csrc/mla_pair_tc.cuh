@@ -127,7 +127,7 @@ __device__ __forceinline__ bool pt_wait(uint64_t* bar, uint32_t parity, volatile
 
 // grid = 2 CTAs a pair of rows, cluster of 2.  tmap_k / tmap_v: boxes of 32 keys x 512 and x 256 channels; tmap_rows, tmap_q, tmap_o as in
 // mla_flash_tc_kernel.
-template <bool WIN, bool TREE>
+template <bool WIN, bool TREE, bool FACT = false>
 __device__ __forceinline__ void pt_body(const MlaArgs& a, int* __restrict__ status, const CUtensorMap& tmap_k, const CUtensorMap& tmap_v, const CUtensorMap& tmap_rows,
                                         const CUtensorMap& tmap_q, const CUtensorMap& tmap_o, const CUtensorMap& tmap_tree_k, const CUtensorMap& tmap_tree_v) {
   extern __shared__ __align__(1024) uint8_t smem_raw[];
@@ -402,8 +402,17 @@ __device__ __forceinline__ void pt_body(const MlaArgs& a, int* __restrict__ stat
       if (lane == 0) tc::mbar_arrive(&ms.q_moved);
     }
     float m = -INFINITY, l = 0.f;
+    const float* const factor = FACT ? a.kv_factor + ms.tree[0].seq * a.factor_stride + 32 * half : nullptr;
+    float4 fac[8], fac_next[8];                            // as in mla_tree_tc_kernel
+    if (FACT && whole > 0) mla_factors(factor + key0(0), fac_next);
     for (int t = 0; t < n_tiles; t++) {
       const int b = t & 1;
+      if (FACT) {
+#pragma unroll
+        for (int j = 0; j < 8; j++) fac[j] = t >= whole ? make_float4(1.f, 1.f, 1.f, 1.f) : fac_next[j];
+        if (t + 1 < whole) mla_factors(factor + key0(t + 1), fac_next);
+      }
+      auto fac_of = [&](int j) -> float { return j % 4 == 0 ? fac[j / 4].x : j % 4 == 1 ? fac[j / 4].y : j % 4 == 2 ? fac[j / 4].z : fac[j / 4].w; };
       ok = pt_wait(&ms.s_full[b], (t >> 1) & 1, abort_flag, 28) && ok;
       tc::fence_after_sync();
       uint32_t sv[32];
@@ -425,7 +434,7 @@ __device__ __forceinline__ void pt_body(const MlaArgs& a, int* __restrict__ stat
       float tmax = -INFINITY;
 #pragma unroll
       for (int j = 0; j < 32; j++) {
-        const float v = (mask >> j) & 1u ? __uint_as_float(sv[j]) * sc2 : -INFINITY;
+        const float v = (mask >> j) & 1u ? __uint_as_float(sv[j]) * (FACT ? fac_of(j) * sc2 : sc2) : -INFINITY;
         sv[j] = __float_as_uint(v);
         tmax = fmaxf(tmax, v);
       }
@@ -465,7 +474,7 @@ __device__ __forceinline__ void pt_body(const MlaArgs& a, int* __restrict__ stat
         for (int e = 0; e < 4; e++) {
           const float p0 = exp2f(__uint_as_float(sv[8 * v + 2 * e]) - mref), p1 = exp2f(__uint_as_float(sv[8 * v + 2 * e + 1]) - mref);
           sum += p0 + p1;
-          const __half2 hp = __floats2half2_rn(p0, p1);
+          const __half2 hp = FACT ? __floats2half2_rn(p0 * fac_of(8 * v + 2 * e), p1 * fac_of(8 * v + 2 * e + 1)) : __floats2half2_rn(p0, p1);
           wp[e] = *reinterpret_cast<const uint32_t*>(&hp);
         }
         *reinterpret_cast<uint4*>(prow + tc::sw128_off(head, half * 4 + v, FT_BLK)) = w;
@@ -615,11 +624,12 @@ __global__ __launch_bounds__(PT_THREADS, 1) void mla_pair_tc_kernel(
   pt_body<WIN, false>(a, status, tmap_k, tmap_v, tmap_rows, tmap_q, tmap_o, tmap_rows, tmap_rows);
 }
 // grid = 2 CTAs a pair of nodes and split
+template <bool FACT>
 __global__ __launch_bounds__(PT_THREADS, 1) void mla_pair_tree_tc_kernel(
     MlaArgs a, int* __restrict__ status, const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ CUtensorMap tmap_v,
     const __grid_constant__ CUtensorMap tmap_rows, const __grid_constant__ CUtensorMap tmap_q, const __grid_constant__ CUtensorMap tmap_o,
     const __grid_constant__ CUtensorMap tmap_tree_k, const __grid_constant__ CUtensorMap tmap_tree_v) {
-  pt_body<false, true>(a, status, tmap_k, tmap_v, tmap_rows, tmap_q, tmap_o, tmap_tree_k, tmap_tree_v);
+  pt_body<false, true, FACT>(a, status, tmap_k, tmap_v, tmap_rows, tmap_q, tmap_o, tmap_tree_k, tmap_tree_v);
 }
 
 }  // namespace hk

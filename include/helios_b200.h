@@ -591,7 +591,8 @@ int hk_mla_tree(const void* q_lat, const void* ckv, int64_t ckv_rows, const int6
 
 /* The same over the 8-bit paged cache (block_table NULL: one sequence); tree_kv is fp16 here too: drafts that are not accepted never touch the cache.
  * Positions behind the table hold no key, one whose entry names no block is a latent of zeros, as in a chunk of hk_mla8_dense.  n_heads: a multiple of 4.
- * Precision as in hk_mla8_dense; where many nodes share the keys the call reads the positions as fp16 rows into the workspace first, as a chunk there.
+ * Precision as in a decode call of hk_mla8_dense.  Where many nodes share the keys the call reads the positions into the workspace first, as fp16 rows that are
+ * exact and a factor each (scales of up to 2^14).
  * Workspace: hk_mla8_tree_workspace_bytes, positions: table_stride * block, or n_blocks * block without a table.                             */
 size_t hk_mla8_tree_workspace_bytes(int m, int n_heads, int n_seqs, int n_keys, int64_t positions);
 int hk_mla8_tree(const void* q_lat, const void* ckv8, const float* scales, int dtype, int64_t n_blocks, int block, const int* block_table,

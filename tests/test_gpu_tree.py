@@ -90,9 +90,34 @@ def test_nodes_over_the_8_bit_cache(kind, block, trees, lens, heads, n_split):
     want = []
     for s in range(n):
         past = rows_of(ckv8, scales, table[s], torch.arange(lens[s], device="cuda"))
-        # (many nodes over many keys: the positions are rounded to fp16 rows first)
-        want += [attend(q[starts[s] + j].double(), torch.cat((past, tree_kv[[starts[s] + i for i in path(trees[s], j)]].double())), 0.0625, rows16=m * max(lens) > 100000)
-                 for j in range(len(trees[s]))]
+        want += wanted(q, past, tree_kv, starts[s], trees[s], 0.0625)
+    check_rows(out, want)
+
+
+@pytest.mark.parametrize("kind", ["i8", "e4m3"])
+@pytest.mark.parametrize("heads,seqs,nodes,n,factor", [(64, 3, 33, 1153, 1.0), (32, 3, 52, 802, 1.0), (64, 3, 33, 1153, 2.0 ** 11), (32, 3, 52, 802, 2.0 ** -16), (64, 2, 64, 1500, 0.0)])
+def test_scales_where_many_nodes_share_the_keys(kind, heads, seqs, nodes, n, factor):
+    """positions that are read first lose nothing, whatever their scales; outputs follow a common factor of all keys and queries' inverse"""
+    gen, block = gen_of(12), 32
+    blocks = (n + block - 1) // block
+    ckv8, scales = cache(gen, kind, seqs * blocks, block, spread=0.7)
+    scales *= factor
+    table = table_for(gen, seqs, blocks, seqs * blocks)
+    trees = [tree_of((nodes, i)) for i in range(seqs)]
+    starts, parent, tree_start = layout(trees)
+    m, back = starts[-1], 1.0 / factor if factor else 1.0
+    q, tree_kv = (randn(gen, m, heads, 512) * 0.7).half(), (randn(gen, m, 512) * min(factor, 1.0)).half()
+    out = torch.empty(m, heads, 512, dtype=torch.float16, device="cuda")
+    scale = 0.0625 * back
+    hk.mla8_tree_decode(q, ckv8, scales, tree_kv, parent, out, m, n_seqs=seqs, tree_start=tree_start, block_table=table, kv_len=ints([n] * seqs), n_heads=heads, scale=scale,
+                        n_keys_hint=n)
+    finish()
+    want = [w for s in range(seqs) for w in wanted(q, rows_of(ckv8, scales, table[s], torch.arange(n, device="cuda")), tree_kv, starts[s], trees[s], scale)]
+    # values of 65,520 (half a step above the largest of fp16) or more are infinities in fp16: where one is within the bound, infinity is right too
+    for r, (o, tol) in enumerate(want):
+        beyond = (o.abs() + tol >= 65520) & torch.isinf(out[r]) & (torch.sign(out[r]) == torch.sign(o))
+        out[r] = torch.where(beyond, o.clamp(-65504, 65504).half(), out[r])
+        want[r] = (torch.where(beyond, o.clamp(-65504, 65504), o), tol)
     check_rows(out, want)
 
 
@@ -115,7 +140,7 @@ def test_positions_without_a_block_and_behind_the_table(nodes, stride):
     past = ref8.as_f64(ckv8.view(torch.uint8)[named, p % block].view(ckv8.dtype)) * scales[named].double()[:, None]
     past[(p // block == 3) | (p // block == 11)] = 0
     for got in (out, also):
-        check_rows(got, [attend(q[j].double(), torch.cat((past, rows[:j + 1].double())), 0.0625, rows16=True) for j in range(nodes)])
+        check_rows(got, [attend(q[j].double(), torch.cat((past, rows[:j + 1].double())), 0.0625) for j in range(nodes)])
 
 
 @pytest.mark.parametrize("over", ["f16", "i8", "f16 of 4", "f16 of 16", "f16 of 32", "f16 of 20", "i8 of 16", "i8 of 8", "i8 of 20"])
