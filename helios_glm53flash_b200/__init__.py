@@ -670,34 +670,36 @@ def kda_tree_accept(x32, conv_state, mixed_qkv, g, beta, rec_state, parent, leaf
 
 # ---- pages of the 8-bit cache: refs [n_blocks] int32 counts the entries of block_table [n_seqs, blocks of a sequence] that name a block.  A pool begins
 # with refs 0 and a table of -1.  missing, n_live: optional device int32 [1] ----
-def _pages(name, op, *args):
-    st = _native.pages(op, *args)
-    if st:
-        raise HeliosB200Error(name, st)
-
-
 def mla8_pages_workspace_bytes(n_blocks, n=0):
     return load_library().hk_mla8_pages_workspace_bytes(n_blocks, n)
 
 
 def mla8_pages_fork(ckv8, scales, refs, block_table, parents, children, lens, n, missing=None, workspace=None, stream=None):
     """n sequences `children` take over the first lens[i] positions of `parents` (hk_mla8_pages_fork): whole blocks shared, the last one copied"""
-    _pages("hk_mla8_pages_fork", 0, ckv8, scales, refs, block_table, parents, children, lens, n, missing, workspace, stream)
+    st = _native.pages(0, ckv8, scales, refs, block_table, parents, children, lens, n, missing, workspace, stream)
+    if st:
+        raise HeliosB200Error("hk_mla8_pages_fork", st)
 
 
 def mla8_pages_reserve(ckv8, scales, refs, block_table, seqs, lens, n, missing=None, workspace=None, stream=None):
     """n sequences get a free block for every entry of their first lens[i] positions that names none (hk_mla8_pages_reserve)"""
-    _pages("hk_mla8_pages_reserve", 1, ckv8, scales, refs, block_table, seqs, lens, None, n, missing, workspace, stream)
+    st = _native.pages(1, ckv8, scales, refs, block_table, seqs, lens, None, n, missing, workspace, stream)
+    if st:
+        raise HeliosB200Error("hk_mla8_pages_reserve", st)
 
 
 def mla8_pages_free(ckv8, scales, refs, block_table, seqs, keep, n, stream=None):
     """n sequences give back the blocks behind their first keep[i] positions (keep None: all of them)"""
-    _pages("hk_mla8_pages_free", 2, ckv8, scales, refs, block_table, seqs, keep, None, n, None, None, stream)
+    st = _native.pages(2, ckv8, scales, refs, block_table, seqs, keep, None, n, None, None, stream)
+    if st:
+        raise HeliosB200Error("hk_mla8_pages_free", st)
 
 
 def mla8_pages_compact(ckv8, scales, refs, block_table, n_live=None, workspace=None, stream=None):
     """the live blocks become the pool's first ones (hk_mla8_pages_compact)"""
-    _pages("hk_mla8_pages_compact", 3, ckv8, scales, refs, block_table, None, None, None, 0, n_live, workspace, stream)
+    st = _native.pages(3, ckv8, scales, refs, block_table, None, None, None, 0, n_live, workspace, stream)
+    if st:
+        raise HeliosB200Error("hk_mla8_pages_compact", st)
 
 
 def mla8_pages_copy(ckv8, scales, to_ckv8, to_scales, src, dst, n, stream=None):
