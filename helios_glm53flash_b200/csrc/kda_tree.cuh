@@ -6,46 +6,75 @@
 namespace hk {
 
 // ---- short convolution (window 4): a node's window is its ancestors' inputs, then the sequence's ----
-// Grid (rows, groups of 1,024 channels): a thread has four channels of a row.  fp32 chain over the window, taps ascending, as conv4_silu_bf16.
-__global__ __launch_bounds__(256) void kda_tree_conv_kernel(const float* x, const __nv_bfloat16* conv_state, const int* slots, const __nv_bfloat16* w,
-                                                            const __nv_bfloat16* bias, __nv_bfloat16* out, TreeArgs tree, int dim, int activation) {
+// Grid (groups of 256 channels, sequences): a thread has four channels of every fourth node.  The tree's inputs go through shared memory as bf16, so each is read
+// once; fp32 chain over the window, taps ascending, as conv4_silu_bf16.  us, 8 x 61 nodes of 12,288 channels 11.9
+// (36 MB; load, then exponentials and stores, with 2.6 CTAs an SM to overlap them), 24 x 13 of 24,576 16.0 (46 MB), 1 x 8 2.6; a CTA a row and 1,024 channels, which
+// looks up its ancestors one after the other and reads four inputs for one, 20.5, 24.7 and 2.7.
+constexpr int KTC_GROUPS = 64, KTC_NODES = 4;              // channel groups of four, nodes at once
+__global__ __launch_bounds__(KTC_GROUPS * KTC_NODES) void kda_tree_conv_kernel(const float* x, const __nv_bfloat16* conv_state, const int* slots, const __nv_bfloat16* w,
+                                                                               const __nv_bfloat16* bias, __nv_bfloat16* out, TreeArgs tree, int dim, int activation) {
+  __shared__ uint2 s_in[TREE_NODES][KTC_GROUPS];
+  __shared__ int s_parent[TREE_NODES];
   pdl_wait();
-  const int r = blockIdx.x, c = (blockIdx.y * 256 + threadIdx.x) * 4, s = tree.seq_of(r);
-  if (s < 0) return;
+  const int s = blockIdx.y, group = threadIdx.x % KTC_GROUPS, first = threadIdx.x / KTC_GROUPS, c = (blockIdx.x * KTC_GROUPS + group) * 4;
   const int2 rows = tree.rows(s);
-  int at[4], j = r - rows.x;                               // the node and its next three ancestors; negative: the sequence's -1st, -2nd, ... last token
-#pragma unroll
-  for (int i = 0, back = 0; i < 4; i++) {
-    at[i] = j >= 0 ? j : --back;
-    if (j >= 0) {
-      const int p = tree.parent[rows.x + j];
-      j = p < j ? p : -1;
+  if (rows.y == 0) return;
+  if (threadIdx.x < rows.y) s_parent[threadIdx.x] = tree.parent[rows.x + threadIdx.x];
+  const bool mine = c < dim;
+  if (mine) {
+#pragma unroll 4
+    for (int j = first; j < rows.y; j += KTC_NODES) {
+      const float4 v = *reinterpret_cast<const float4*>(x + (size_t)(rows.x + j) * dim + c);
+      const __nv_bfloat162 a = __floats2bfloat162_rn(v.x, v.y), b = __floats2bfloat162_rn(v.z, v.w);
+      s_in[j][group] = make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
     }
   }
-  if (c >= dim) return;
-  float4 in[4];
+  uint2 taps[4], before[3];                                // the sequence's last three tokens, the last first
+  float start[4] = {0.f, 0.f, 0.f, 0.f};
+  if (mine) {
+    const int slot = slots ? slots[s] : s;
+    const uint2* st = reinterpret_cast<const uint2*>(conv_state + ((size_t)slot * dim + c) * 4);
+    uint2 win[4];
 #pragma unroll
-  for (int i = 0; i < 4; i++)
-    if (at[i] >= 0) in[i] = *reinterpret_cast<const float4*>(x + (size_t)(rows.x + at[i]) * dim + c);
-  const int slot = slots ? slots[s] : s;
-  const uint2* st = reinterpret_cast<const uint2*>(conv_state + ((size_t)slot * dim + c) * 4);
-  uint16_t y[4];
-#pragma unroll
-  for (int u = 0; u < 4; u++) {
-    const uint2 win = st[u], taps = *reinterpret_cast<const uint2*>(w + (size_t)(c + u) * 4);
-    auto value = [&](int i) -> float {                     // input i tokens back
-      if (at[i] >= 0) return __bfloat162float(__float2bfloat16_rn(reinterpret_cast<const float*>(&in[i])[u]));
-      return at[i] == -1 ? bf16hi(win.y) : at[i] == -2 ? bf16lo(win.y) : bf16hi(win.x);
-    };
-    float acc = bias ? __bfloat162float(bias[c + u]) : 0.f;
-    acc = fmaf(bf16lo(taps.x), value(3), acc);
-    acc = fmaf(bf16hi(taps.x), value(2), acc);
-    acc = fmaf(bf16lo(taps.y), value(1), acc);
-    acc = fmaf(bf16hi(taps.y), value(0), acc);
-    if (activation) acc = acc * (1.0f / (1.0f + __expf(-acc)));
-    y[u] = __bfloat16_as_ushort(__float2bfloat16_rn(acc));
+    for (int u = 0; u < 4; u++) {
+      win[u] = st[u];
+      taps[u] = *reinterpret_cast<const uint2*>(w + (size_t)(c + u) * 4);
+      if (bias) start[u] = __bfloat162float(bias[c + u]);
+    }
+    before[0] = make_uint2(__byte_perm(win[0].y, win[1].y, 0x7632), __byte_perm(win[2].y, win[3].y, 0x7632));
+    before[1] = make_uint2(__byte_perm(win[0].y, win[1].y, 0x5410), __byte_perm(win[2].y, win[3].y, 0x5410));
+    before[2] = make_uint2(__byte_perm(win[0].x, win[1].x, 0x7632), __byte_perm(win[2].x, win[3].x, 0x7632));
   }
-  *reinterpret_cast<uint2*>(out + (size_t)r * dim + c) = make_uint2(y[0] | (uint32_t)y[1] << 16, y[2] | (uint32_t)y[3] << 16);
+  __syncthreads();
+  if (!mine) return;
+#pragma unroll 2
+  for (int j = first; j < rows.y; j += KTC_NODES) {
+    uint2 in[4];                                           // the node's inputs and those of its next three ancestors, then the sequence's
+#pragma unroll
+    for (int i = 0, at = j, back = 0; i < 4; i++) {        // (the same for the whole warp)
+      if (at >= 0) {
+        in[i] = s_in[at][group];
+        const int p = s_parent[at];
+        at = p < at ? p : -1;
+      } else {
+        in[i] = back == 0 ? before[0] : back == 1 ? before[1] : before[2];
+        back++;
+      }
+    }
+    uint16_t y[4];
+#pragma unroll
+    for (int u = 0; u < 4; u++) {
+      auto value = [&](int i) -> float { return u == 0 ? bf16lo(in[i].x) : u == 1 ? bf16hi(in[i].x) : u == 2 ? bf16lo(in[i].y) : bf16hi(in[i].y); };   // i tokens back
+      float acc = start[u];
+      acc = fmaf(bf16lo(taps[u].x), value(3), acc);
+      acc = fmaf(bf16hi(taps[u].x), value(2), acc);
+      acc = fmaf(bf16lo(taps[u].y), value(1), acc);
+      acc = fmaf(bf16hi(taps[u].y), value(0), acc);
+      if (activation) acc = acc * (1.0f / (1.0f + __expf(-acc)));
+      y[u] = __bfloat16_as_ushort(__float2bfloat16_rn(acc));
+    }
+    *reinterpret_cast<uint2*>(out + (size_t)(rows.x + j) * dim + c) = make_uint2(y[0] | (uint32_t)y[1] << 16, y[2] | (uint32_t)y[3] << 16);
+  }
 }
 
 // ---- the recurrence of every node ----
@@ -81,6 +110,10 @@ struct KdaTreeArgs {
 //               hi hi + hi lo + lo hi: 2^-16 of the magnitudes, where bf16 keeps the range of fp32 (a state in fp16 would overflow at 65,504)
 //   levels      u of the nodes of a depth, then their part in all nodes below: a node has one ancestor at each depth, so a level is one
 //               multiply-add a node and column, in registers, and one barrier
+// What bounds it: latency where a CTA is alone (8 nodes of 32 heads 4.6 us), then shared memory and the barriers between phases.  A CTA of 61 nodes takes 20,700
+// cycles: loads 5,300, splitting 950, pairs 5,700, operands 1,600, products 500, their way out 1,200, levels 4,800, output 650; 8 x 32 heads of 61 nodes 24.8 us (40 MB
+// at 1.6 TB/s), 24 x 64 of 16 nodes 52 (131 MB at 2.5).  Lanes a node, us with 8 / 16 / 32: 24 x 64 heads of 8 nodes 74.8 / 63.5 / 44.6, of 16 84.5 / 72.8 / 51.9,
+// of 30 99.0 / 86.4, 32 heads of 8 5.2 / 4.6 / 4.6.
 constexpr int KT_WARPS = 16, KT_THREADS = KT_WARPS * 32;
 // Shared memory of a form: k E, q E (before them k and the decays, behind them u); S_0, then its products; lists of pairs.
 template <int COLS, int G>
@@ -484,7 +517,8 @@ static int kt_nodes(const KdaTreeArgs& a, cudaStream_t s) {
 }
 template <bool GATED>
 static int kt_run(const KdaTreeArgs& a, cudaStream_t s) {
-  // few heads: a head's columns over two or four CTAs, which prepare the tokens each for itself
+  // Few heads: a head's columns over two or four CTAs, which prepare the tokens each for itself.  us with 32 / 64 / 128 columns: 32 heads of 8 nodes 4.6 / 4.6 / 5.4,
+  // of 61 10.1 / 10.6 / 12.0; 64 heads 6.2 / 4.7 / 5.4 and 19.2 / 10.7 / 12.1; 128 heads 11.5 / 7.2 / 6.3 and 38.6 / 21.1 / 12.9
   const int64_t heads = (int64_t)a.H * a.tree.n_seqs;
   if (4 * heads <= sm_count()) return kt_nodes<GATED, 32>(a, s);
   if (2 * heads <= sm_count()) return kt_nodes<GATED, 64>(a, s);
@@ -822,7 +856,7 @@ HK_API int hk_kda_tree_conv(const float* x32, const void* conv_state, const int*
   HK_REQUIRE(aligned(x32, 16) && aligned(conv_state, 8) && aligned(conv_weight, 8) && aligned(mixed_qkv, 8));
   HK_REQUIRE(tree_args(&t, parent, tree_start, n_seqs, m));
   if (m == 0) return HK_OK;
-  return pdl_launch(kda_tree_conv_kernel, dim3((unsigned)m, (unsigned)((dim + 1023) / 1024)), dim3(256), 0, as_stream(stream), x32,
+  return pdl_launch(kda_tree_conv_kernel, dim3((unsigned)((dim + 4 * KTC_GROUPS - 1) / (4 * KTC_GROUPS)), (unsigned)n_seqs), dim3(KTC_GROUPS * KTC_NODES), 0, as_stream(stream), x32,
                     (const __nv_bfloat16*)conv_state, slots, (const __nv_bfloat16*)conv_weight, (const __nv_bfloat16*)conv_bias, (__nv_bfloat16*)mixed_qkv, t,
                     dim, activation) == cudaSuccess
              ? HK_OK

@@ -114,7 +114,7 @@ __global__ void __launch_bounds__(APPEND_WARPS * 32) mla8_append_kernel(AppendAr
 #pragma unroll
     for (int j = 0; j < 4; j++) lw[j] = TREE ? make_uint2(0u, 0u) : reinterpret_cast<const uint2*>(a.ln_w)[j * 32 + lane];
     auto weigh = [&](float (&x)[16]) {
-      if (TREE) return;
+      if constexpr (TREE) return;
 #pragma unroll
       for (int j = 0; j < 4; j++) {
         const float2 w0 = __half22float2(*reinterpret_cast<const __half2*>(&lw[j].x)), w1 = __half22float2(*reinterpret_cast<const __half2*>(&lw[j].y));
@@ -225,6 +225,8 @@ cudaError_t append_launch(const AppendArgs& a, dim3 grid, int parts, cudaStream_
   return pdl_launch_cluster(parts, kernel, dim3(grid.x * parts, grid.y), dim3(APPEND_WARPS * 32), 0, s, a);
 }
 
+// Accepted nodes: the append of rows that are normalised already, a CTA a block that the longest path may touch; 2.7 us for one sequence, 3.0 for 24 (path, then
+// lengths, table, scale and rows: four dependent loads).
 template <int FMT>
 cudaError_t accept_launch(const AppendArgs& a, cudaStream_t s) {
   const int block = 1 << a.pg.shift;

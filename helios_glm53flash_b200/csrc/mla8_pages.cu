@@ -7,7 +7,8 @@
 // Bookkeeping (pages_kernel): one CTA, or for large pools a cluster of eight, whose warps take a sequence each in turn, or a part of refs; the steps of a call
 // meet at a barrier, which also orders their accesses to global memory.  A list of free blocks in ascending order: every warp counts its part of
 // refs, the counts are added up through (distributed) shared memory, and the second pass writes where its count says.
-// What bounds it is latency, a few dependent loads and a barrier a step.
+// What bounds it is latency, a few dependent loads and a barrier a step, and the issue slots of one SM: what all 32 warps do costs eight cycles an
+// instruction, so warps without blocks or rows stand aside (a fork of four 6.8 -> 6.0 us).
 #include "hk_common.cuh"
 #include "latent8.cuh"
 
@@ -390,7 +391,8 @@ bool pages_workspace(PagesArgs* a, void* workspace, size_t bytes, int* status) {
 }
 template <int MODE>
 cudaError_t pages_launch(const PagesArgs& a, cudaStream_t s) {
-  // us, one CTA / eight: a compaction with nothing to move of 4,000 blocks 7.7 / 8.3, of 16,000 11.4 / 8.6, of 131,072 66 / 15; a fork out of 123 9.2 / 11.6
+  // us, one CTA / eight: a compaction with nothing to move of 123 blocks 3.7 / 6.3, of 4,000 4.8 / 7.8, of 8,192 6.0 / 8.0 (of 131,072 66, when one CTA walked them, / 13.7);
+  // a fork of four out of 123 6.4 / 9.6, of 8,192 6.9 / 10.0
   return a.pg.n_blocks <= PG_SMALL ? pdl_launch(pages_kernel<MODE, 1>, dim3(1), dim3(PG_THREADS), 0, s, a)
                                : pdl_launch_cluster(PG_MAX_CTAS, pages_kernel<MODE, PG_MAX_CTAS>, dim3(PG_MAX_CTAS), dim3(PG_THREADS), 0, s, a);
 }

