@@ -276,7 +276,7 @@ __global__ __launch_bounds__(KT_THREADS, G == 32 ? 2 : 1) void kda_tree_kernel(c
     be = kt_beta<GATED>(a, r, head);
   }
   TreePaths paths;
-  paths.load(a.tree, rows);
+  paths.load<G == 8 ? 33 : 0, G == 16 ? 32 : TREE_NODES>(a.tree, rows);   // (one way each; with sixteen nodes the shorter code was 4 % slower)
   if (warp == KT_WARPS - 1) {                              // nodes lane and lane + 32: sums of the fours of ancestors before
     const int depth[2] = {(__popcll(paths.lo) + 2) / 4, (__popcll(paths.hi) + 2) / 4};
     int sum[2] = {depth[0], depth[1]};

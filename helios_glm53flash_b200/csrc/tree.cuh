@@ -67,6 +67,8 @@ __device__ __forceinline__ TreeUnit tree_unit(const TreeArgs& t, int unit, int g
 // 2^r nearest ancestors and knows the next one up; a chain of 64 takes six rounds, a tree that is eight deep three.
 struct TreePaths {
   uint64_t lo, hi;
+  // LEAST, MOST: the sizes of trees that there may be (of more nodes than MOST the first MOST are asked for)
+  template <int LEAST = 0, int MOST = TREE_NODES>
   __device__ __forceinline__ void load(const TreeArgs& t, int2 rows) {
     const int lane = threadIdx.x & 31;
     auto parent = [&](int j) {                             // (a parent comes before its nodes, else there is none)
@@ -76,7 +78,7 @@ struct TreePaths {
     int up_lo = parent(lane), up_hi = parent(lane + 32);
     lo = 1ull << lane;
     hi = 1ull << (lane + 32);
-    if (rows.y <= 32) {                                    // (half the numbers, a third of the exchanges)
+    if (MOST <= 32 || (LEAST <= 32 && rows.y <= 32)) {     // (half the numbers, a third of the exchanges)
       uint32_t m = 1u << lane;
       while (__any_sync(0xffffffffu, up_lo >= 0)) {
         const uint32_t a = __shfl_sync(0xffffffffu, m, up_lo & 31);
