@@ -121,6 +121,10 @@ struct KtForm {
   // Up to 32 nodes: M = 64 in the form that spreads them over all lanes (columns from COLS / 2 on in lanes 64-127), half the operand, two CTAs an SM
   static constexpr bool HALF = G >= 16 && COLS >= 64;
   static constexpr int M = HALF ? 64 : 128;
+  // Rows of q E behind those of k E.  Up to 16 nodes: the second numbers of both are 32 rows of the same operand, so S_0 is read by two products instead of
+  // three (the fourth, lo lo, comes with them).
+  static constexpr bool STACK = G == 32;
+  static constexpr int Q_ROW = STACK ? 16 : M / 2, LO_ROW = STACK ? 32 : 0;
   static constexpr uint32_t A_BLOCK = M * 128, S_BLOCK = 128 * 128;     // 64 channels of an operand: rows of 128 bytes
   static constexpr uint32_t A = 0, A_LO = 2 * A_BLOCK, S = 4 * A_BLOCK;
   static constexpr uint32_t S_BYTES = 128 * COLS * 2;                   // hi or lo
@@ -382,13 +386,14 @@ __global__ __launch_bounds__(KT_THREADS, G == 32 ? 2 : 1) void kda_tree_kernel(c
     for (int m = 0; m < CH; m++) {
       const int c = 4 * l + 4 * G * m;
       const uint32_t off = (c >> 6) * F::A_BLOCK + j * 128 + (((c >> 3 & 7) ^ (j & 7)) << 4) + (c & 4) * 2;
+      constexpr uint32_t second = F::STACK ? F::A + F::LO_ROW * 128 : F::A_LO;
       uint2 hi, lo;
       kt_split(mul2(k[m][0], e[m][0]), mul2(k[m][1], e[m][1]), hi, lo);
       *reinterpret_cast<uint2*>(smem + F::A + off) = hi;
-      *reinterpret_cast<uint2*>(smem + F::A_LO + off) = lo;
+      *reinterpret_cast<uint2*>(smem + second + off) = lo;
       kt_split(mul2(q[m][0], e[m][0]), mul2(q[m][1], e[m][1]), hi, lo);
-      *reinterpret_cast<uint2*>(smem + F::A + off + F::M / 2 * 128) = hi;
-      *reinterpret_cast<uint2*>(smem + F::A_LO + off + F::M / 2 * 128) = lo;
+      *reinterpret_cast<uint2*>(smem + F::A + off + F::Q_ROW * 128) = hi;
+      *reinterpret_cast<uint2*>(smem + second + off + F::Q_ROW * 128) = lo;
     }
   }
   tc::fence_async_smem();
@@ -401,7 +406,7 @@ __global__ __launch_bounds__(KT_THREADS, G == 32 ? 2 : 1) void kda_tree_kernel(c
     const uint32_t leader = tc::elect_one(), idesc = tc::make_idesc(F::M, COLS, tc::FMT_BF16, tc::FMT_BF16, false, true);
     const uint32_t base = tc::smem_u32(smem);
 #pragma unroll
-    for (int part = 0; part < 3; part++) {
+    for (int part = 0; part < (F::STACK ? 2 : 3); part++) {
       const uint64_t ad = tc::make_sdesc_sw128(base + (part == 2 ? F::A_LO : F::A), 16, 1024);
       const uint32_t sb = base + F::S + (part == 1 ? F::S_BYTES : 0);
       const uint64_t bd = COLS == 32 ? tc::make_sdesc_sw64(sb, 128 * 64, 512) : tc::make_sdesc_sw128(sb, F::S_BLOCK, 1024);
@@ -438,7 +443,15 @@ __global__ __launch_bounds__(KT_THREADS, G == 32 ? 2 : 1) void kda_tree_kernel(c
         kt_load<VEC>(R + j * F::ROW + VEC * (l + G * m), y);
 #pragma unroll
         for (int u = 0; u < VEC; u++) kv[m][u] -= y[u];
-        kt_load<VEC>(R + (F::M / 2 + j) * F::ROW + VEC * (l + G * m), o[m]);
+        kt_load<VEC>(R + (F::Q_ROW + j) * F::ROW + VEC * (l + G * m), o[m]);
+        if (F::STACK) {
+          kt_load<VEC>(R + (F::LO_ROW + j) * F::ROW + VEC * (l + G * m), y);
+#pragma unroll
+          for (int u = 0; u < VEC; u++) kv[m][u] -= y[u];
+          kt_load<VEC>(R + (F::LO_ROW + F::Q_ROW + j) * F::ROW + VEC * (l + G * m), y);
+#pragma unroll
+          for (int u = 0; u < VEC; u++) o[m][u] += y[u];
+        }
       }
     }
   }
