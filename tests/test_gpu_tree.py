@@ -365,6 +365,87 @@ def test_recurrence_of_nodes(trees, heads):
         assert bool((f32[r] == 7).all()) and bool((out[r] == 7).all()), "rows of no tree are left as they were"
 
 
+@pytest.mark.parametrize("nodes", [1, 2, 15, 16, 17, 31, 32, 33, 64])
+@pytest.mark.parametrize("heads", [2, 20, 60])
+def test_recurrence_of_trees_of_a_told_size(nodes, heads):
+    """the forms for up to 16, 32 and 64 nodes, with 32, 64 and 128 columns a CTA"""
+    trees = [tree_of((nodes, 1)), tree_of((max(1, nodes - 3), 2)), tree_of((nodes, 5))]
+    gen = gen_of(nodes + heads)
+    starts, parent, tree_start = layout(trees)
+    m = starts[-1]
+    x = kda_inputs(gen, m, heads, 3)
+    out, f32 = torch.empty(m, heads, 128, dtype=torch.bfloat16, device="cuda"), torch.empty(m, heads, 128, device="cuda")
+    hk.kda_tree_decode(x["qkv"], x["g"], x["beta"], x["state"], parent, out, m, heads, n_seqs=3, tree_start=tree_start, out_f32=f32, max_nodes=nodes)
+    finish()
+    want, tol = kda_wanted(x, heads, starts, trees, [0, 1, 2])
+    off = (f32.double() - want).abs()
+    assert bool((off <= tol).all()), float((off - tol).max())
+
+
+@pytest.mark.parametrize("most", [1, 7, 16, 20, 40])
+def test_nodes_beyond_the_told_number_are_left_as_they_were(most):
+    gen, heads, tree = gen_of(21), 3, tree_of((50, 4))
+    x = kda_inputs(gen, 50, heads, 1)
+    all_of, some = (torch.full((50, heads, 128), 7.0, dtype=torch.bfloat16, device="cuda") for _ in range(2))
+    a = (x["qkv"], x["g"], x["beta"], x["state"], ints(tree))
+    hk.kda_tree_decode(*a, all_of, 50, heads, tree_start=ints([0, 50]))
+    hk.kda_tree_decode(*a, some, 50, heads, tree_start=ints([0, 50]), max_nodes=most)
+    finish()
+    assert bool((some[most:] == 7).all())
+    # the same sums in other orders, rounded to bf16 toward zero: a step of bf16 and 1e-5 of the largest
+    off = (some[:most].double() - all_of[:most].double()).abs()
+    assert bool((off <= 2.0 ** -7 * all_of[:most].double().abs() + 1e-5 * all_of.double().abs().max()).all())
+
+
+def test_rows_and_states_beyond_four_gigabytes():
+    """caches of 4.3 million rows and 70,000 blocks, states in slot 70,000"""
+    gen, n, rows = gen_of(22), 700, 4_300_000
+    tree = tree_of("binary15")
+    q, kv = (randn(gen, 15, 64, 512) * 0.7).half(), randn(gen, 15, 512).half()
+    ckv = torch.empty(rows, 512, dtype=torch.float16, device="cuda")
+    first = rows - n - 20
+    ckv[first:first + n] = randn(gen, n, 512).half()
+    base, lens, leaf, told = torch.tensor([first], device="cuda"), ints([n]), ints([14]), ints([0])
+    want = wanted(q, ckv[first:first + n].double(), kv, 0, tree, 0.0625)
+    for splits in (0, 1, 4):
+        out = torch.empty(15, 64, 512, dtype=torch.float16, device="cuda")
+        hk.mla_tree_decode(q, ckv, kv, ints(tree), out, 15, kv_base=base, kv_len=lens, n_keys_hint=n, n_split=splits)
+        finish()
+        check_rows(out, want)
+    hk.mla_tree_accept(kv, ckv, ints(tree), leaf, 15, kv_base=base, kv_len=lens, len_out=told)
+    finish()
+    steps = path(tree, 14)
+    assert int(told) == n + len(steps) and torch.equal(ckv[first + n:first + n + len(steps)], kv[steps])
+    del ckv
+    blocks = 70_000                                          # of 128 tokens: 4.6 GB
+    ckv8 = torch.empty(blocks, 128, 512, dtype=torch.int8, device="cuda")
+    scales = torch.ones(blocks, device="cuda")
+    some, s = cache(gen, "i8", 6, 128)
+    ckv8[-6:], scales[-6:] = some, s
+    table = ints([list(range(blocks - 6, blocks))])
+    want = wanted(q, rows_of(ckv8, scales, table[0], torch.arange(n, device="cuda")), kv, 0, tree, 0.0625)
+    out = torch.empty(15, 64, 512, dtype=torch.float16, device="cuda")
+    hk.mla8_tree_decode(q, ckv8, scales, kv, ints(tree), out, 15, block_table=table, kv_len=lens, n_keys_hint=n)
+    finish()
+    check_rows(out, want)
+    hk.mla8_tree_accept(kv, ckv8, scales, ints(tree), leaf, 15, block_table=table, kv_len=lens)
+    finish()
+    got = rows_of(ckv8, scales, table[0], torch.arange(n, n + len(steps), device="cuda"))
+    assert bool(((got - kv[steps].double()).abs() <= 0.5 * scales[-1].double() * 1.01 + 0.5 * float(s[-1])).all()), "half a step of the block's scale, before and after it grew"
+    del ckv8
+    x = kda_inputs(gen, 15, 1, 1)
+    state = torch.empty(70_001, 1, 128, 128, device="cuda")
+    state[-1] = x["state"][0]
+    near, far = (torch.empty(15, 1, 128, dtype=torch.bfloat16, device="cuda") for _ in range(2))
+    a = (x["qkv"], x["g"], x["beta"])
+    hk.kda_tree_decode(*a, x["state"], ints(tree), near, 15, 1)
+    hk.kda_tree_decode(*a, state, ints(tree), far, 15, 1, slots=ints([70_000]))
+    hk.kda_tree_accept(None, None, *a, x["state"], ints(tree), leaf, 15, 1)
+    hk.kda_tree_accept(None, None, *a, state, ints(tree), leaf, 15, 1, slots=ints([70_000]))
+    finish()
+    assert torch.equal(near, far) and torch.equal(state[-1], x["state"][0])
+
+
 def test_hard_resets_and_gates_of_zero():
     """log decays of 0, -100 and minus infinity on a long chain: nothing overflows, what is forgotten is nothing"""
     gen, heads, tree = gen_of(11), 2, TREES["chain64"]
@@ -582,6 +663,31 @@ def test_captured_and_replayed_and_on_a_stream_of_its_own(kind):
     call(again)
     finish()
     assert torch.equal(out, again) and not torch.equal(out, first)
+
+
+def test_two_calls_at_once():
+    """calls on two streams, each with scratch of its own, give what each gives alone"""
+    gen, tree = gen_of(31), tree_of((40, 3))
+    parent, lens = ints(tree), ints([1500])
+    q, kv, ckv = (randn(gen, 40, 64, 512) * 0.7).half(), randn(gen, 40, 512).half(), randn(gen, 1500, 512).half()
+    ckv8, scales = cache(gen, "e4m3", 24, 64)
+    x = kda_inputs(gen, 40, 50, 1)
+    calls = (lambda o, st: hk.mla_tree_decode(q, ckv, kv, parent, o, 40, kv_len=lens, n_keys_hint=1500, stream=st),
+             lambda o, st: hk.mla8_tree_decode(q, ckv8, scales, kv, parent, o, 40, kv_len=lens, n_keys_hint=1500, stream=st),
+             lambda o, st: hk.kda_tree_decode(x["qkv"], x["g"], x["beta"], x["state"], parent, o, 40, 50, stream=st))
+    fresh = lambda i: torch.empty(40, 50, 128, dtype=torch.bfloat16, device="cuda") if i == 2 else torch.empty(40, 64, 512, dtype=torch.float16, device="cuda")  # noqa: E731
+    alone = [fresh(i) for i in range(3)]
+    for i, call in enumerate(calls):
+        call(alone[i], None)
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    outs = [[fresh(i) for i in range(3)] for _ in range(8)]
+    finish()
+    for k, out in enumerate(outs):
+        for i in range(3):
+            calls[(i + k) % 3](out[(i + k) % 3], streams[k % 2])
+    finish()
+    for out in outs:
+        assert all(torch.equal(a, b) for a, b in zip(out, alone))
 
 
 def test_calls_without_rows_do_nothing():
