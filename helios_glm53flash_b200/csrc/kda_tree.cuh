@@ -279,7 +279,7 @@ __global__ __launch_bounds__(KT_THREADS, G == 32 ? 2 : 1) void kda_tree_kernel(c
     }
     be = kt_beta<GATED>(a, r, head);
   }
-  TreePaths paths;
+  TreePaths paths{};
   paths.load<G == 8 ? 33 : 0, G == 16 ? 32 : TREE_NODES>(a.tree, rows);   // (one way each; with sixteen nodes the shorter code was 4 % slower)
   if (warp == KT_WARPS - 1) {                              // nodes lane and lane + 32: sums of the fours of ancestors before
     const int depth[2] = {(__popcll(paths.lo) + 2) / 4, (__popcll(paths.hi) + 2) / 4};
@@ -671,17 +671,20 @@ __global__ __launch_bounds__(KA_WARPS * 32, 2) void kda_tree_accept_kernel(const
   }
 }
 
-// The same for many heads: persistent CTAs, two an SM, whose ninth warp is a head ahead - it finds the path, asks for the next head's 64 KB as one bulk copy as
-// soon as this one's sit in registers, and for the first eight tokens - and whose tenth moves the windows.  The eight warps with columns share nothing but the
-// copies: each prepares every token for itself (a quarter more work a step, and no barrier).
+// The same for many heads: persistent CTAs, two an SM.  Warp 8 is a head ahead: it finds the path, asks for the next head's 64 KB as one bulk copy as soon as this
+// one's sit in registers, and for the tokens, eight at a time.  Warp 9 normalises keys and takes exponentials for all (each of the eight warps for itself: chains of
+// 16 90.7 us for 82), then moves the head's windows.  The eight warps with columns have only these arrivals between them.  All that comes from memory comes as
+// bulk copies, up to two heads ahead: behind 19 MB of states on their way a load takes up to 9,000 cycles.  Bound by HBM for short paths (24 x 64 heads, 201 MB in 37 us,
+// 5.4 TB/s), by the products of the steps for long ones (two heads of an SM 1,500 cycles a step: a packed multiply-add takes two issue slots).
 struct AcceptMeta {
-  uint64_t full[2], s_empty, t_empty[2];
+  uint64_t full[2], ready[2], t_empty[2];        // tokens: landed, prepared, used
+  uint64_t s_full, s_empty, w_full[2], w_empty[2];   // the state; windows and the inputs that enter them
   uint64_t path[2];
   float beta[2][KA_BATCH];
   int abort_flag;
 };
-constexpr uint32_t KA_RAW = 1024;                 // a token: k and v of 256 bytes, log decays of 512
-constexpr uint32_t KAS_S = 0, KAS_RAW = 65536, KAS_TOK = KAS_RAW + 2 * KA_BATCH * KA_RAW, KAS_META = KAS_TOK + KA_WARPS * 2 * 1024,
+constexpr uint32_t KA_RAW = 1024, KA_K = 512, KA_WIN = 3 * 1024 + 4 * 3 * 512;   // a token: k and v of 256 bytes, log decays of 512, whose place the decays take; k prepared; windows, inputs
+constexpr uint32_t KAS_S = 0, KAS_RAW = 65536, KAS_K = KAS_RAW + 2 * KA_BATCH * KA_RAW, KAS_WIN = KAS_K + 2 * KA_BATCH * KA_K, KAS_META = KAS_WIN + 2 * KA_WIN,
                    KAS_SMEM = KAS_META + (uint32_t)sizeof(AcceptMeta);
 constexpr int KA_STREAM_THREADS = (KA_WARPS + 2) * 32;
 __global__ __launch_bounds__(KA_STREAM_THREADS, 2) void kda_tree_accept_stream_kernel(const KdaTreeArgs a, int* __restrict__ status) {
@@ -690,19 +693,27 @@ __global__ __launch_bounds__(KA_STREAM_THREADS, 2) void kda_tree_accept_stream_k
   volatile int* abort_flag = &ms.abort_flag;
   const int tid = threadIdx.x, lane = tid & 31, warp = tc::warp_index_uniform(), n_items = a.H * a.tree.n_seqs;
   if (tid == 0) {
-    tc::mbar_init(&ms.full[0], 1);
-    tc::mbar_init(&ms.full[1], 1);
+    for (int b = 0; b < 2; b++) {
+      tc::mbar_init(&ms.full[b], 1);
+      tc::mbar_init(&ms.ready[b], 1);
+      tc::mbar_init(&ms.t_empty[b], KA_WARPS);
+      tc::mbar_init(&ms.w_full[b], 1);
+      tc::mbar_init(&ms.w_empty[b], 1);
+    }
+    tc::mbar_init(&ms.s_full, 1);
     tc::mbar_init(&ms.s_empty, KA_WARPS);
-    tc::mbar_init(&ms.t_empty[0], KA_WARPS);
-    tc::mbar_init(&ms.t_empty[1], KA_WARPS);
     tc::mbar_fence_init();
     ms.abort_flag = 0;
   }
   pdl_wait();
   __syncthreads();
+  auto last_nodes = [](uint64_t path, int steps) -> uint64_t {   // the last four at most
+    for (int i = 4; i < steps; i++) path &= path - 1;
+    return path;
+  };
   // Tokens are handed over eight at a time, at least once a head, also of a sequence without an accepted node (no path, no copies).
+  int turn = 0;
   if (warp == KA_WARPS) {
-    int turn = 0;
     uint32_t moved = 0;                                    // heads whose state went through shared memory
     for (int idx = blockIdx.x; idx < n_items; idx += gridDim.x) {
       const int s = idx / a.H, head = idx - s * a.H, slot = a.slots ? a.slots[s] : s;
@@ -728,7 +739,7 @@ __global__ __launch_bounds__(KA_STREAM_THREADS, 2) void kda_tree_accept_stream_k
         __syncwarp();
         if (lane == 0) {
           if (steps == 0) tc::mbar_arrive(&ms.full[b]);
-          else tc::mbar_arrive_expect_tx(&ms.full[b], (i0 == 0 ? 65536 : 0) + batch * KA_RAW);
+          else tc::mbar_arrive_expect_tx(&ms.full[b], batch * KA_RAW);
         }
         __syncwarp();
         if (lane < batch) {
@@ -741,63 +752,103 @@ __global__ __launch_bounds__(KA_STREAM_THREADS, 2) void kda_tree_accept_stream_k
         if (i0 > 0 || steps == 0) continue;
         if (moved > 0) tc::mbar_wait<40>(&ms.s_empty, (moved - 1) & 1, abort_flag, 62);
         moved++;
-        if (lane == 0) tc::bulk_g2s(ka_mem + KAS_S, a.state + ((size_t)slot * a.H + head) * 128 * 128, 65536, &ms.full[b]);
+        if (lane == 0) {
+          tc::mbar_arrive_expect_tx(&ms.s_full, 65536);
+          tc::bulk_g2s(ka_mem + KAS_S, a.state + ((size_t)slot * a.H + head) * 128 * 128, 65536, &ms.s_full);
+        }
+        __syncwarp();
+        if (!a.conv_state) continue;
+        const int wb = (moved - 1) & 1;
+        if (moved > 2) tc::mbar_wait<40>(&ms.w_empty[wb], ((moved - 1) / 2 - 1) & 1, abort_flag, 67);
+        const int n_last = min(steps, 4), i = (lane - 3) / 3, part = lane % 3;   // lanes 0-2: q's, k's and v's windows; then three a node
+        if (lane == 0) tc::mbar_arrive_expect_tx(&ms.w_full[wb], 3 * 1024 + n_last * 3 * 512);
+        __syncwarp();
+        const size_t ch = ((size_t)part * a.H + head) * 128;
+        if (lane < 3) {
+          tc::bulk_g2s(ka_mem + KAS_WIN + wb * KA_WIN + part * 1024, a.conv_state + ((size_t)slot * 3 * a.H * 128 + ch) * 4, 1024, &ms.w_full[wb]);
+        } else if (i < n_last) {
+          uint64_t m = last_nodes(path, steps);
+          for (int k = 0; k < i; k++) m &= m - 1;
+          tc::bulk_g2s(ka_mem + KAS_WIN + wb * KA_WIN + 3 * 1024 + (i * 3 + part) * 512, a.x + (size_t)(rows.x + __ffsll((long long)m) - 1) * 3 * a.H * 128 + ch, 512, &ms.w_full[wb]);
+        }
         __syncwarp();
       }
     }
   } else if (warp > KA_WARPS) {
-    // the windows, by a warp that nobody waits for
-    for (int idx = blockIdx.x; a.conv_state && idx < n_items; idx += gridDim.x) {
-      const int s = idx / a.H, head = idx - s * a.H, slot = a.slots ? a.slots[s] : s;
-      const int2 rows = a.tree.rows(s);
-      const uint64_t path = tree_path(a.tree, rows, a.leaf[s]);
-      const int steps = __popcll(path);
-      if (steps == 0) continue;
-      uint64_t m = path;
-      for (int i = 4; i < steps; i++) m &= m - 1;        // its last four nodes
-      int node[4];
-#pragma unroll
-      for (int i = 0; i < 4; i++) {
-        node[i] = m ? rows.x + __ffsll((long long)m) - 1 : -1;
-        m &= m - 1;
-      }
-#pragma unroll
-      for (int c0 = 0; c0 < 3 * 128; c0 += 128) {
-        uint2 w[4];
-        float x[4][4];
-        uint2* at[4];
-#pragma unroll
-        for (int u = 0; u < 4; u++) {
-          const int ch = ((c0 >> 7) * a.H + head) * 128 + 32 * u + lane;
-          at[u] = reinterpret_cast<uint2*>(a.conv_state + ((size_t)slot * 3 * a.H * 128 + ch) * 4);
-          w[u] = *at[u];
-#pragma unroll
-          for (int i = 0; i < 4; i++) x[u][i] = node[i] >= 0 ? a.x[(size_t)node[i] * 3 * a.H * 128 + ch] : 0.f;
-        }
-#pragma unroll
-        for (int u = 0; u < 4; u++) {
-#pragma unroll
-          for (int i = 0; i < 4; i++)
-            if (node[i] >= 0) w[u] = conv4_rolled(w[u], __float2bfloat16_rn(x[u][i]));
-          *at[u] = w[u];
-        }
-      }
-    }
-  } else {
-    const int rg = lane >> 2, col = warp * 16 + 4 * (lane & 3);
-    float* const tok = reinterpret_cast<float*>(ka_mem + KAS_TOK) + warp * 512;   // k and decay of a token, two in turn
-    int turn = 0;
+    uint32_t moved = 0;
     for (int idx = blockIdx.x; idx < n_items; idx += gridDim.x) {
       const int s = idx / a.H, head = idx - s * a.H, slot = a.slots ? a.slots[s] : s;
-      int steps = 0;
-      ulonglong2 S[16];
+      const int2 rows = a.tree.rows(s);
       const float rate = a.a_log ? __expf(a.a_log[head]) : 0.f;
+      float bias[4] = {0.f, 0.f, 0.f, 0.f};
+      if (a.a_log) {
+#pragma unroll
+        for (int u = 0; u < 4; u++) bias[u] = a.dt_bias[head * 128 + lane + 32 * u];
+      }
+      uint64_t path = 0;
+      int steps = 0;
       for (int i0 = 0; i0 == 0 || i0 < steps; i0 += KA_BATCH, turn++) {
         const int b = turn & 1;
         tc::mbar_wait<40>(&ms.full[b], (turn / 2) & 1, abort_flag, 63);
         if (i0 == 0) {
+          path = ms.path[b] & (rows.y < TREE_NODES ? (1ull << rows.y) - 1 : ~0ull);   // (whatever was read behind a wait that gave up)
+          steps = __popcll(path);
+        }
+#pragma unroll 2
+        for (int i = 0; i < min(steps - i0, KA_BATCH); i++) {
+          uint8_t* raw = ka_mem + KAS_RAW + (b * KA_BATCH + i) * KA_RAW;
+          const __nv_bfloat16* k = reinterpret_cast<const __nv_bfloat16*>(raw);
+          float* g = reinterpret_cast<float*>(raw + 512);
+          float* to = reinterpret_cast<float*>(ka_mem + KAS_K + (b * KA_BATCH + i) * KA_K);
+          float z[4];
+#pragma unroll
+          for (int u = 0; u < 4; u++) z[u] = __bfloat162float(k[lane + 32 * u]);
+          const float f = inv_norm(z);
+#pragma unroll
+          for (int u = 0; u < 4; u++) {
+            const int c = lane + 32 * u;
+            const float x = g[c];
+            to[c] = __fmul_rn(z[u], f);
+            g[c] = __expf(a.a_log ? gate_value(x, bias[u], rate, a.lower_bound) : x);
+          }
+        }
+        tc::fence_async_smem();                            // (copies will write where the decays are)
+        __syncwarp();
+        if (lane == 0) tc::mbar_arrive(&ms.ready[b]);
+      }
+      if (steps == 0 || !a.conv_state) continue;
+      // the head's windows
+      const int wb = moved & 1;
+      const uint8_t* mem = ka_mem + KAS_WIN + wb * KA_WIN;
+      tc::mbar_wait<40>(&ms.w_full[wb], (moved / 2) & 1, abort_flag, 68);
+      moved++;
+      uint2* const windows = reinterpret_cast<uint2*>(a.conv_state) + (size_t)slot * 3 * a.H * 128;
+#pragma unroll 4
+      for (int u = 0; u < 12; u++) {
+        const int part = u >> 2, c = 32 * (u & 3) + lane;
+        uint2 w = *reinterpret_cast<const uint2*>(mem + part * 1024 + c * 8);
+        for (int i = 0; i < min(steps, 4); i++) w = conv4_rolled(w, __float2bfloat16_rn(reinterpret_cast<const float*>(mem + 3 * 1024 + (i * 3 + part) * 512)[c]));
+        if (!*abort_flag) windows[((size_t)part * a.H + head) * 128 + c] = w;
+      }
+      __syncwarp();
+      if (lane == 0) tc::mbar_arrive(&ms.w_empty[wb]);
+    }
+  } else {
+    const int rg = lane >> 2, col = warp * 16 + 4 * (lane & 3);
+    uint32_t moved = 0;
+    for (int idx = blockIdx.x; idx < n_items; idx += gridDim.x) {
+      const int s = idx / a.H, head = idx - s * a.H, slot = a.slots ? a.slots[s] : s;
+      int steps = 0;
+      ulonglong2 S[16];
+      for (int i0 = 0; i0 == 0 || i0 < steps; i0 += KA_BATCH, turn++) {
+        const int b = turn & 1;
+        tc::mbar_wait<40>(&ms.ready[b], (turn / 2) & 1, abort_flag, 64);
+        tc::mbar_wait<40>(&ms.full[b], (turn / 2) & 1, abort_flag, 65);   // (passed: what the copies brought is this thread's to read too)
+        if (i0 == 0) {
           steps = __popcll(ms.path[b]);
           if (steps > 0) {
+            tc::mbar_wait<40>(&ms.s_full, moved & 1, abort_flag, 66);
+            moved++;
             const float* from = reinterpret_cast<const float*>(ka_mem + KAS_S) + col;
 #pragma unroll
             for (int i = 0; i < 16; i++) S[i] = *reinterpret_cast<const ulonglong2*>(from + state_row(rg, i) * 128);
@@ -808,23 +859,8 @@ __global__ __launch_bounds__(KA_STREAM_THREADS, 2) void kda_tree_accept_stream_k
 #pragma unroll 1
         for (int i = 0; i < min(steps - i0, KA_BATCH); i++) {
           const uint8_t* raw = ka_mem + KAS_RAW + (b * KA_BATCH + i) * KA_RAW;
-          const __nv_bfloat16* k = reinterpret_cast<const __nv_bfloat16*>(raw);
-          const float* g = reinterpret_cast<const float*>(raw + 512);
-          float* to = tok + (i & 1) * 256;
-          float z[4];
-#pragma unroll
-          for (int u = 0; u < 4; u++) z[u] = __bfloat162float(k[lane + 32 * u]);
-          const float f = inv_norm(z);
-#pragma unroll
-          for (int u = 0; u < 4; u++) {
-            const int c = lane + 32 * u;
-            const float x = g[c];
-            to[c] = __fmul_rn(z[u], f);
-            to[128 + c] = __expf(a.a_log ? gate_value(x, a.dt_bias[head * 128 + c], rate, a.lower_bound) : x);
-          }
-          const float4 v4 = load4(k + 128 + col);
-          __syncwarp();
-          ka_step(S, to, to + 128, v4, ms.beta[b][i], rg);
+          const float4 v4 = load4(reinterpret_cast<const __nv_bfloat16*>(raw) + 128 + col);
+          ka_step(S, reinterpret_cast<const float*>(ka_mem + KAS_K + (b * KA_BATCH + i) * KA_K), reinterpret_cast<const float*>(raw + 512), v4, ms.beta[b][i], rg);
         }
         __syncwarp();
         if (lane == 0) tc::mbar_arrive(&ms.t_empty[b]);
@@ -903,9 +939,9 @@ HK_API int hk_kda_tree_accept(const float* x32, void* conv_state, const void* mi
   a.leaf = leaf;
   // up to half a head an SM by two CTAs a head: a path of five of 64 heads 6.2 / 5.4 us (one / two), of 128 6.7 / 7.0; four 32 heads 6.2 / 6.0 / 5.8
   const int64_t heads = (int64_t)num_heads * n_seqs;
-  // more than three heads an SM stream through shared memory: us, a CTA a head / streamed, paths of five, 320 heads 10.5 / 14.4, 384 14.4 / 14.9, 512 21.9 / 19.7,
-  // 1,024 39.3 / 32.4, 1,536 55.3 / 45.5
-  if (heads > 3 * sm_count() && aligned(mixed_qkv, 16)) {
+  // More than five heads to two SMs stream through shared memory.  us with states that are not in the L2, a CTA a head / streamed, trees of 1 and of 13 nodes: 320 heads
+  // 10.5 / 13.6 and 13.5 / 17.0, 384 14.2 / 13.5 and 20.3 / 17.0, 512 17.0 / 15.6 and 23.4 / 20.2, 1,024 29.5 / 26.5 and 40.5 / 31.6, 1,536 42.5 / 37.2 and 57.4 / 43.9
+  if (2 * heads > 5 * sm_count() && aligned(mixed_qkv, 16) && aligned(conv_state, 16) && aligned(x32, 16)) {
     static bool attr_set[64] = {false};
     const int dev = device_index();
     if (!attr_set[dev]) {

@@ -89,15 +89,15 @@ struct TreePaths {
         }
       }
       lo = m;
-      return;
-    }
-    while (__any_sync(0xffffffffu, up_lo >= 0 || up_hi >= 0)) {
-      const uint64_t a = of(up_lo), b = of(up_hi);         // (both before either changes)
-      const int next_lo = at(up_lo, up_lo, up_hi), next_hi = at(up_hi, up_lo, up_hi);
-      if (up_lo >= 0) lo |= a;
-      if (up_hi >= 0) hi |= b;
-      up_lo = up_lo >= 0 ? next_lo : -1;
-      up_hi = up_hi >= 0 ? next_hi : -1;
+    } else {
+      while (__any_sync(0xffffffffu, up_lo >= 0 || up_hi >= 0)) {
+        const uint64_t a = of(up_lo), b = of(up_hi);       // (both before either changes)
+        const int next_lo = at(up_lo, up_lo, up_hi), next_hi = at(up_hi, up_lo, up_hi);
+        if (up_lo >= 0) lo |= a;
+        if (up_hi >= 0) hi |= b;
+        up_lo = up_lo >= 0 ? next_lo : -1;
+        up_hi = up_hi >= 0 ? next_hi : -1;
+      }
     }
   }
   static __device__ __forceinline__ int at(int j, int lo, int hi) {
