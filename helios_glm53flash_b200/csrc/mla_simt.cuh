@@ -298,8 +298,10 @@ __global__ __launch_bounds__(128 * GROUPS) void lse_combine_kernel(
 
 // The same for few splits of many rows, as two sums of the even and of the odd splits, without shared memory or barriers: a warp keeps a
 // split's weight in a lane, a thread twelve pieces in flight.  1,536 rows of 6 splits 7.3 -> 4.0 us, 3,072 of 3 12.5 -> 5.4.
+// keep(): whether the row is written, asked for once everything has been loaded
+template <class KEEP>
 __device__ __forceinline__ void lse_combine_few(const float* __restrict__ part_m, const float* __restrict__ part_l, const float* __restrict__ part_acc, int n_split,
-                                                int64_t rows, __half* __restrict__ out) {
+                                                int64_t rows, __half* __restrict__ out, KEEP keep) {
   const int64_t r = blockIdx.x;
   const int lane = threadIdx.x & 31;
   const bool mine = lane < n_split;
@@ -332,6 +334,7 @@ __device__ __forceinline__ void lse_combine_few(const float* __restrict__ part_m
   }
   const float inv = gl > 0.f ? 1.f / gl : 0.f;
   const __half2 h0 = __floats2half2_rn((o[0].x + o[1].x) * inv, (o[0].y + o[1].y) * inv), h1 = __floats2half2_rn((o[0].z + o[1].z) * inv, (o[0].w + o[1].w) * inv);
+  if (!keep()) return;
   uint2 pk;
   pk.x = *reinterpret_cast<const uint32_t*>(&h0);
   pk.y = *reinterpret_cast<const uint32_t*>(&h1);
@@ -342,25 +345,25 @@ __global__ __launch_bounds__(128) void lse_combine_few_kernel(const float* __res
                                                               const float* __restrict__ part_acc, int n_split, int64_t rows, __half* __restrict__ out) {
   pdl_release();
   pdl_wait();
-  lse_combine_few(part_m, part_l, part_acc, n_split, rows, out);
+  lse_combine_few(part_m, part_l, part_acc, n_split, rows, out, [] { return true; });
 }
 // rows of no tree of drafted tokens, whose partials are whatever lies there, are left as they were
-__global__ __launch_bounds__(128) void lse_combine_few_tree_kernel(const float* __restrict__ part_m, const float* __restrict__ part_l,
+__global__ __launch_bounds__(128, 7) void lse_combine_few_tree_kernel(const float* __restrict__ part_m, const float* __restrict__ part_l,
                                                                    const float* __restrict__ part_acc, int n_split, int64_t rows, __half* __restrict__ out,
                                                                    TreeArgs tree, int n_heads) {
   pdl_release();
   pdl_wait();
-  if (tree.seq_of(blockIdx.x / n_heads) < 0) return;
-  lse_combine_few(part_m, part_l, part_acc, n_split, rows, out);
+  const int2 asked = tree.ask();
+  lse_combine_few(part_m, part_l, part_acc, n_split, rows, out, [&] { return tree.seq_of(blockIdx.x / n_heads, asked) >= 0; });
 }
 
 // The same with every row shared by CSPLIT CTAs (few rows, or many splits), each
 // owning 512 / CSPLIT channels, with GROUPS groups of 32 float4 lanes over the splits, so that 64 rows still cover
 // the machine.  grid = (rows, CSPLIT).
 constexpr int LSE_CSPLIT = 4;
-template <int GROUPS, int PRE>
+template <int GROUPS, int PRE, class KEEP>
 __device__ __forceinline__ void lse_combine_cs(const float* __restrict__ part_m, const float* __restrict__ part_l, const float* __restrict__ part_acc, int n_split,
-                                               int64_t rows, __half* __restrict__ out) {
+                                               int64_t rows, __half* __restrict__ out, KEEP keep) {
   constexpr int LANES = 128 / LSE_CSPLIT;
   const int64_t r = blockIdx.x;
   const int cpart = blockIdx.y;
@@ -368,6 +371,7 @@ __device__ __forceinline__ void lse_combine_cs(const float* __restrict__ part_m,
   float4 o;
   lse_reduce_row<false, GROUPS, LANES, PRE>(part_m, part_l, part_acc, nullptr, nullptr, nullptr, n_split, rows, r,
                                                                 gm, gl, o, cpart);
+  if (!keep()) return;
   if (threadIdx.x < LANES) {
     const float inv = gl > 0.f ? 1.f / gl : 0.f;
     __half2 h0 = __floats2half2_rn(o.x * inv, o.y * inv);
@@ -385,7 +389,7 @@ __global__ __launch_bounds__(32 * GROUPS) void lse_combine_cs_kernel(
     int n_split, int64_t rows, __half* __restrict__ out) {
   pdl_release();
   pdl_wait();
-  lse_combine_cs<GROUPS, PRE>(part_m, part_l, part_acc, n_split, rows, out);
+  lse_combine_cs<GROUPS, PRE>(part_m, part_l, part_acc, n_split, rows, out, [] { return true; });
 }
 template <int GROUPS, int PRE>
 __global__ __launch_bounds__(32 * GROUPS) void lse_combine_cs_tree_kernel(
@@ -393,8 +397,8 @@ __global__ __launch_bounds__(32 * GROUPS) void lse_combine_cs_tree_kernel(
     int n_split, int64_t rows, __half* __restrict__ out, TreeArgs tree, int n_heads) {
   pdl_release();
   pdl_wait();
-  if (tree.seq_of(blockIdx.x / n_heads) < 0) return;
-  lse_combine_cs<GROUPS, PRE>(part_m, part_l, part_acc, n_split, rows, out);
+  const int2 asked = tree.ask();
+  lse_combine_cs<GROUPS, PRE>(part_m, part_l, part_acc, n_split, rows, out, [&] { return tree.seq_of(blockIdx.x / n_heads, asked) >= 0; });
 }
 
 // ---- merge of S partial sets into ONE partial set (still un-normalised): the per-GPU reduction before

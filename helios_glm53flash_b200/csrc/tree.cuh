@@ -23,12 +23,17 @@ struct TreeArgs {
     }
     return make_int2(r0, min(r1 - r0, TREE_NODES));
   }
-  // the sequence of a row, -1: none.  Executed by a whole warp, as the two below.
-  __device__ __forceinline__ int seq_of(int r) const {
+  // the sequence of a row, -1: none.  Executed by a whole warp, as the two below.  With what ask() has asked for before, so that other loads go with it.
+  __device__ __forceinline__ int2 ask() const {
+    const int s = threadIdx.x & 31;
+    return start && s < n_seqs ? rows(s) : make_int2(0, 0);
+  }
+  __device__ __forceinline__ int seq_of(int r) const { return seq_of(r, ask()); }
+  __device__ __forceinline__ int seq_of(int r, int2 asked) const {
     if (!start) return r / (m / n_seqs);
     for (int s0 = 0; s0 < n_seqs; s0 += 32) {
       const int s = s0 + (int)(threadIdx.x & 31);
-      const int2 t = s < n_seqs ? rows(s) : make_int2(0, 0);
+      const int2 t = s0 == 0 ? asked : s < n_seqs ? rows(s) : make_int2(0, 0);
       const uint32_t who = __ballot_sync(0xffffffffu, r >= t.x && r < t.x + t.y);
       if (who) return s0 + __ffs(who) - 1;
     }
