@@ -716,6 +716,7 @@ __global__ __launch_bounds__(KA_STREAM_THREADS, 2) void kda_tree_accept_stream_k
   if (warp == KA_WARPS) {
     uint32_t moved = 0;                                    // heads whose state went through shared memory
     for (int idx = blockIdx.x; idx < n_items; idx += gridDim.x) {
+      if (__any_sync(0xffffffffu, *abort_flag != 0)) break;   // (behind a wait that gave up nothing more is asked for)
       const int s = idx / a.H, head = idx - s * a.H, slot = a.slots ? a.slots[s] : s;
       const int2 rows = a.tree.rows(s);
       const uint64_t path = tree_path(a.tree, rows, a.leaf[s]);
@@ -872,6 +873,8 @@ __global__ __launch_bounds__(KA_STREAM_THREADS, 2) void kda_tree_accept_stream_k
       }
     }
   }
+  if (*abort_flag)                                         // what was on its way ends first (far less than a millisecond)
+    for (const long long t0 = clock64(); clock64() - t0 < 4000000;) __nanosleep(1000);
   __syncthreads();
   if (tid == 0 && ms.abort_flag && status) atomicExch(status, HK_ERR_TIMEOUT);
 }
