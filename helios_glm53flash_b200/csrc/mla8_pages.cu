@@ -21,6 +21,7 @@ namespace {
 
 constexpr int PG_MAX_CTAS = 8, PG_THREADS = 1024, PG_CTA_WARPS = PG_THREADS / 32;
 constexpr int PG_AHEAD = 8;                       // loads of a lane on their way
+constexpr int PG_MANY = 2500;                     // entries of a fork's rows from which on references are counted in shared memory
 constexpr int PG_LOCAL = 1024;                    // lists up to here stay in shared memory
 constexpr int PG_SMALL = PG_CTA_WARPS * 32 * PG_AHEAD;   // blocks of a pool that one CTA looks after
 
@@ -35,7 +36,7 @@ struct PagesArgs {
   int *count, *src, *dst, *list;
 };
 
-enum { PG_FORK, PG_RESERVE, PG_COMPACT };
+enum { PG_FORK, PG_FORK_MANY, PG_RESERVE, PG_COMPACT };   // PG_FORK_MANY: one CTA that counts references in shared memory
 
 template <int CTAS>
 __device__ __forceinline__ void pg_barrier() {
@@ -65,8 +66,10 @@ __device__ __forceinline__ void pg_row(const int* row, int j0, int end, int (&e)
   }
 }
 
-// entries from `first` on of a row, PG_TURN of every `step`: each gives its block back and names none (an exchange: named twice, a row is given back once)
-__device__ __forceinline__ void pg_release(const PagesArgs& a, int seq, int first, int step) {
+// entries from `first` on of a row, PG_TURN of every `step`: each gives its block back (back(block)) and names none (an exchange: named twice, a row is given
+// back once)
+template <class BACK>
+__device__ __forceinline__ void pg_release(const PagesArgs& a, int seq, int first, int step, BACK back) {
   int* row = a.table + (size_t)seq * a.pg.table_stride;
   for (int j0 = first; j0 < a.pg.table_stride; j0 += step) {
     int e[PG_ROW];
@@ -76,7 +79,7 @@ __device__ __forceinline__ void pg_release(const PagesArgs& a, int seq, int firs
       if (e[u] >= 0) e[u] = atomicExch(row + j0 + 32 * u + (threadIdx.x & 31), -1);
 #pragma unroll
     for (int u = 0; u < PG_ROW; u++)
-      if (pg_block(a, e[u])) atomicSub(a.refs + e[u], 1);
+      if (pg_block(a, e[u])) back(e[u]);
   }
 }
 
@@ -85,7 +88,7 @@ __global__ __launch_bounds__(128) void pages_free_kernel(PagesArgs a) {
   pdl_release();
   pdl_wait();
   const int s = a.seqs[blockIdx.x];
-  if (pg_seq(a, s)) pg_release(a, s, pg_entries(a, a.lens ? a.lens[blockIdx.x] : 0) + (threadIdx.x >> 5) * PG_TURN, 4 * PG_TURN);
+  if (pg_seq(a, s)) pg_release(a, s, pg_entries(a, a.lens ? a.lens[blockIdx.x] : 0) + (threadIdx.x >> 5) * PG_TURN, 4 * PG_TURN, [&](int b) { atomicSub(a.refs + b, 1); });
 }
 
 // Blocks [b0, b1) of this warp, in ascending order over the cluster's warps.
@@ -103,24 +106,24 @@ template <int CTAS>
 struct PagesWalk {
   PagesPart p;
   int r[PG_AHEAD];
-  __device__ __forceinline__ void load(const PagesArgs& a, int b) {
+  __device__ __forceinline__ void load(const int* refs, int b) {
     const int lane = threadIdx.x & 31;
 #pragma unroll
     for (int u = 0; u < PG_AHEAD; u++) {
       r[u] = 0;
       if (b + 32 * u >= p.b1) continue;                    // (the whole warp)
-      if (b + 32 * u + lane < p.b1) r[u] = a.refs[b + 32 * u + lane];
+      if (b + 32 * u + lane < p.b1) r[u] = refs[b + 32 * u + lane];
     }
   }
-  __device__ __forceinline__ PagesWalk(const PagesArgs& a, int gw) : p(pg_part<CTAS>(a, gw)) {
-    if (CTAS == 1) load(a, p.b0);
+  __device__ __forceinline__ PagesWalk(const PagesArgs& a, int gw, bool now = true) : p(pg_part<CTAS>(a, gw)) {
+    if (CTAS == 1 && now) load(a.refs, p.b0);
   }
   // f(block, references, in range), ascending, by the whole warp
   template <class F>
   __device__ __forceinline__ void operator()(const PagesArgs& a, F f) {
     const int lane = threadIdx.x & 31;
     for (int b = p.b0; b < p.b1; b += 32 * PG_AHEAD) {
-      if (CTAS > 1) load(a, b);
+      if (CTAS > 1) load(a.refs, b);
 #pragma unroll
       for (int u = 0; u < PG_AHEAD; u++)
         if (b + 32 * u < p.b1) f(b + 32 * u + lane, r[u], b + 32 * u + lane < p.b1);
@@ -180,6 +183,8 @@ __global__ __launch_bounds__(PG_THREADS) void pages_kernel(PagesArgs a) {
   constexpr int WARPS = CTAS * PG_CTA_WARPS;
   __shared__ int s_count[PG_CTA_WARPS], s_sum[PG_MAX_CTAS];
   __shared__ int s_want[PG_CTA_WARPS];                     // fork
+  constexpr bool SHARED = MODE == PG_FORK_MANY;
+  __shared__ int s_refs[SHARED ? PG_SMALL : 1];
   __shared__ int s_src[MODE != PG_COMPACT && CTAS == 1 ? PG_LOCAL : 1], s_list[MODE != PG_COMPACT && CTAS == 1 ? PG_LOCAL : 1];
   pdl_release();
   pdl_wait();
@@ -188,7 +193,13 @@ __global__ __launch_bounds__(PG_THREADS) void pages_kernel(PagesArgs a) {
   int* const src = local ? s_src : a.src;
   const int lane = threadIdx.x & 31, gw = (int)(blockIdx.x * PG_CTA_WARPS + (threadIdx.x >> 5)), stride = a.pg.table_stride;
   auto row = [&](int s) -> int* { return a.table + (size_t)s * stride; };
-  if constexpr (MODE == PG_FORK) {
+  if constexpr (MODE == PG_FORK || SHARED) {
+    PagesWalk<CTAS> walk(a, gw, SHARED);                   // (on its way with the pairs)
+    const int b_first = walk.p.b0 + lane;
+    auto count = [&](int b, int by) {
+      if constexpr (SHARED) atomicAdd(&s_refs[b], by);
+      else atomicAdd(a.refs + b, by);
+    };
     auto pair = [&](int i) { return pg_seq(a, a.seqs[i]) && pg_seq(a, a.from[i]) && a.seqs[i] != a.from[i]; };
     // the block that a pair copies, -1: none
     int want = 0;                                          // one CTA: every warp its part of the pairs
@@ -207,17 +218,38 @@ __global__ __launch_bounds__(PG_THREADS) void pages_kernel(PagesArgs a) {
       }
     }
     if (CTAS == 1 && lane == 0) s_want[gw] = want;
+    if (SHARED) {
+#pragma unroll
+      for (int u = 0; u < PG_AHEAD; u++)
+        if (b_first + 32 * u < walk.p.b1) s_refs[b_first + 32 * u] = walk.r[u];
+      __syncthreads();
+    }
     for (int i = WARPS - 1 - gw; i < a.n; i += WARPS)      // (from the last warp on: the first ones have pairs)
-      if (pair(i)) pg_release(a, a.seqs[i], 0, PG_TURN);
+      if (pair(i)) pg_release(a, a.seqs[i], 0, PG_TURN, [&](int b) { count(b, -1); });
     pg_barrier<CTAS>();
+    int before[PG_AHEAD];                                  // the references as they were
     if (CTAS == 1) want = __reduce_add_sync(0xffffffffu, s_want[lane]);
-    PagesWalk<CTAS> walk(a, gw);
+    if (SHARED) {
+#pragma unroll
+      for (int u = 0; u < PG_AHEAD; u++) before[u] = walk.r[u];
+      walk.load(s_refs, walk.p.b0);
+    } else if (CTAS == 1) {
+      walk.load(a.refs, walk.p.b0);
+    }
     int* const list = local ? s_list : a.list;             // (at most one a pair)
     const int have = pg_free_list<CTAS>(a, walk, list, want, s_count, s_sum);
     pg_barrier<CTAS>();
     const int turns = (stride + PG_TURN - 1) / PG_TURN;    // a warp has 128 entries of a child
-    for (int64_t item = gw; item < (int64_t)a.n * turns; item += WARPS) {
-      const int i = (int)(item / turns), j0 = (int)(item - (int64_t)i * turns) * PG_TURN;
+    // (step by step: a division of 64 bits an item was a third of this loop's instructions)
+    int i = gw, turn = 0, step_i = WARPS, step_turn = 0;
+    if (turns > 1) {
+      i = gw / turns;
+      turn = gw - i * turns;
+      step_i = WARPS / turns;
+      step_turn = WARPS - step_i * turns;
+    }
+    while (i < a.n) {
+      const int j0 = turn * PG_TURN;
       const bool both = pair(i);
       const int whole = both ? pg_whole(a, a.lens[i]) : 0;
       if (both && j0 < whole) {
@@ -227,20 +259,36 @@ __global__ __launch_bounds__(PG_THREADS) void pages_kernel(PagesArgs a) {
 #pragma unroll
         for (int u = 0; u < PG_ROW; u++) {
           if (!pg_block(a, b[u])) continue;
-          atomicAdd(a.refs + b[u], 1);
+          count(b[u], 1);
           to[32 * u] = b[u];
         }
       }
-      if (j0 > 0) continue;
-      int before = 0;
-      for (int k0 = 0; k0 < i; k0 += 32) before += __popc(__ballot_sync(0xffffffffu, k0 + lane < i && src[k0 + lane] >= 0));
-      const int e = src[i], fresh = e >= 0 && before < have ? list[before] : -1;
-      if (lane == 0) {
-        a.dst[i] = fresh;
-        if (fresh >= 0) {
-          row(a.seqs[i])[whole] = fresh;
-          a.refs[fresh] = 1;
+      if (turn == 0) {
+        int copies = 0;
+        for (int k0 = 0; k0 < i; k0 += 32) copies += __popc(__ballot_sync(0xffffffffu, k0 + lane < i && src[k0 + lane] >= 0));
+        const int e = src[i], fresh = e >= 0 && copies < have ? list[copies] : -1;
+        if (lane == 0) {
+          a.dst[i] = fresh;
+          if (fresh >= 0) {
+            row(a.seqs[i])[whole] = fresh;
+            if (SHARED) s_refs[fresh] = 1;
+            else a.refs[fresh] = 1;
+          }
         }
+      }
+      i += step_i;
+      turn += step_turn;
+      if (turn >= turns) {
+        turn -= turns;
+        i++;
+      }
+    }
+    if (SHARED) {
+      __syncthreads();
+#pragma unroll
+      for (int u = 0; u < PG_AHEAD; u++) {
+        const int b = b_first + 32 * u;
+        if (b < walk.p.b1 && s_refs[b] != before[u]) a.refs[b] = s_refs[b];
       }
     }
     if (gw == 0 && lane == 0) {
@@ -430,7 +478,11 @@ HK_API int hk_mla8_pages_fork(void* ckv8, float* scales, int dtype, int64_t n_bl
   a.told = missing;
   int st;
   if (!pages_workspace(&a, workspace, workspace_bytes, &st)) return st;
-  if (pages_launch<PG_FORK>(a, as_stream(stream)) != cudaSuccess) return HK_ERR_CUDA;
+  // Scattered additions to global memory leave an SM one a cycle: many entries are counted in shared memory, for which the pool's references are read and written back
+  // once.  us, global / shared: 320 entries of 4 rows 6.0 / 6.8, 632 of 8 6.2 / 7.2, 2,528 of 32 8.5 / 7.5, 5,000 of 16 11.7 / 10.3, 10,000 of 32 16.3 / 11.4
+  const bool many = n_blocks <= PG_SMALL && (int64_t)n * table_stride >= PG_MANY;
+  const cudaError_t e = many ? pdl_launch(pages_kernel<PG_FORK_MANY, 1>, dim3(1), dim3(PG_THREADS), 0, as_stream(stream), a) : pages_launch<PG_FORK>(a, as_stream(stream));
+  if (e != cudaSuccess) return HK_ERR_CUDA;
   return pdl_launch(pages_copy_kernel, dim3(copy_ctas(n, a.pg.shift)), dim3(256), 0, as_stream(stream), pages_moves(a)) == cudaSuccess ? HK_OK : HK_ERR_CUDA;
 }
 

@@ -119,7 +119,7 @@ class Pool:
             assert int(self.told) == told
 
 
-@pytest.mark.parametrize("n_blocks,block,n_seqs,stride", [(1, 16, 3, 2), (7, 128, 4, 3), (31, 16, 5, 9), (33, 64, 9, 40), (600, 32, 40, 33), (1024, 16, 20, 40), (8192, 16, 60, 150), (9000, 16, 70, 150)])
+@pytest.mark.parametrize("n_blocks,block,n_seqs,stride", [(1, 16, 3, 2), (7, 128, 4, 3), (31, 16, 5, 9), (33, 64, 9, 40), (600, 32, 40, 33), (1024, 16, 20, 40), (300, 16, 60, 100), (1500, 128, 90, 70), (8192, 16, 60, 150), (9000, 16, 70, 150)])
 def test_pages_come_and_go(n_blocks, block, n_seqs, stride):
     pool = Pool("i8" if block < 64 else "e4m3", n_blocks, block, n_seqs, stride)
     rng = random.Random(n_blocks)
