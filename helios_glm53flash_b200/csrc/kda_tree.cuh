@@ -352,32 +352,41 @@ __global__ __launch_bounds__(KT_THREADS, G == 32 ? 2 : 1) void kda_tree_kernel(c
   }
   const int first = node ? 4 * ms.first[j] : 0;
   const int steps = __reduce_max_sync(0xffffffffu, depth);
-  for (int t = 0; t < steps; t++) {
-    const int at = depth - 1 - t;                          // (negative: a node of fewer ancestors than its neighbours in the warp)
-    const int i = at >= 0 ? 63 - __clzll((long long)above) : 0;
-    uint64_t ab = 0, bb = 0;
-    if (at >= 0) {
-      above &= ~(1ull << i);
+  for (int t = 0; t < steps; t += 2) {                     // two ancestors at once
+    float va[2], vb[2];
+    int up[2], who[2];
 #pragma unroll
-      for (int m = 0; m < CH; m++) {
-        const int c = i * 128 + 4 * l + 4 * G * m;
-        const ulonglong2 x = *reinterpret_cast<const ulonglong2*>(K + c), y = *reinterpret_cast<const ulonglong2*>(Dc + c);
-        const uint64_t x0 = mul2(x.x, e[m][0]), x1 = mul2(x.y, e[m][1]);
-        ab = fma2(k[m][1], x1, fma2(k[m][0], x0, ab));
-        bb = fma2(q[m][1], x1, fma2(q[m][0], x0, bb));
-        e[m][0] = mul2(e[m][0], y.x);
-        e[m][1] = mul2(e[m][1], y.y);
+    for (int h = 0; h < 2; h++) {
+      up[h] = depth - 1 - t - h;                           // (negative: a node of fewer ancestors than its neighbours in the warp)
+      who[h] = up[h] >= 0 ? 63 - __clzll((long long)above) : 0;
+      uint64_t ab = 0, bb = 0;
+      if (up[h] >= 0) {
+        above &= ~(1ull << who[h]);
+#pragma unroll
+        for (int m = 0; m < CH; m++) {
+          const int c = who[h] * 128 + 4 * l + 4 * G * m;
+          const ulonglong2 x = *reinterpret_cast<const ulonglong2*>(K + c), y = *reinterpret_cast<const ulonglong2*>(Dc + c);
+          const uint64_t x0 = mul2(x.x, e[m][0]), x1 = mul2(x.y, e[m][1]);
+          ab = fma2(k[m][1], x1, fma2(k[m][0], x0, ab));
+          bb = fma2(q[m][1], x1, fma2(q[m][0], x0, bb));
+          e[m][0] = mul2(e[m][0], y.x);
+          e[m][1] = mul2(e[m][1], y.y);
+        }
       }
+      va[h] = sum2(ab);
+      vb[h] = sum2(bb);
     }
-    // two sums at once: half of the node's lanes take the one, half the other
-    const float va = sum2(ab), vb = sum2(bb);
-    const bool second = l >= G / 2;
-    float v = (second ? vb : va) + __shfl_xor_sync(0xffffffffu, second ? va : vb, G / 2);
+    // four sums at once, a quarter of the node's lanes each
+    const bool second = l & (G / 2), later = l & (G / 4);
+    const float x0 = (second ? vb[0] : va[0]) + __shfl_xor_sync(0xffffffffu, second ? va[0] : vb[0], G / 2);
+    const float x1 = (second ? vb[1] : va[1]) + __shfl_xor_sync(0xffffffffu, second ? va[1] : vb[1], G / 2);
+    float v = (later ? x1 : x0) + __shfl_xor_sync(0xffffffffu, later ? x0 : x1, G / 4);
 #pragma unroll
-    for (int m = G / 4; m > 0; m >>= 1) v += __shfl_xor_sync(0xffffffffu, v, m);
-    if (at >= 0 && l % (G / 2) == 0) {
+    for (int m = G / 8; m > 0; m >>= 1) v += __shfl_xor_sync(0xffffffffu, v, m);
+    const int at = later ? up[1] : up[0];
+    if (at >= 0 && l % (G / 4) == 0) {
       (second ? B : A)[first + at] = v;
-      if (!second) anc[first + at] = (uint8_t)i;
+      if (!second) anc[first + at] = (uint8_t)(later ? who[1] : who[0]);
     }
   }
   __syncthreads();                                         // k and decays have been read
