@@ -138,6 +138,7 @@ struct KtMisc {
   uint32_t tmem;
   int abort_flag;
   int first[TREE_NODES];                // of a node's ancestors in the lists of pairs, in fours
+  int last;                             // the deepest node's depth, -1: no nodes
 };
 template <int COLS, int G>
 constexpr size_t kt_smem(int most) {
@@ -295,6 +296,8 @@ __global__ __launch_bounds__(KT_THREADS, G == 32 ? 2 : 1) void kda_tree_kernel(c
     const int low = __shfl_sync(0xffffffffu, sum[0], 31);
     ms.first[lane] = sum[0] - depth[0];
     ms.first[lane + 32] = low + sum[1] - depth[1];
+    const int last = __reduce_max_sync(0xffffffffu, max(lane < n ? __popcll(paths.lo) : 0, lane + 32 < n ? __popcll(paths.hi) : 0)) - 1;
+    if (lane == 0) ms.last = last;
   }
   uint64_t above = paths.of(j & 63);
   above &= ~(1ull << (j & 63));
@@ -465,7 +468,8 @@ __global__ __launch_bounds__(KT_THREADS, G == 32 ? 2 : 1) void kda_tree_kernel(c
     }
   }
   // ---- level by level ----
-  for (int level = 0;; level++) {
+  const int last = ms.last;
+  for (int level = 0; level <= last; level++) {
     int who = 0;
     float fa = 0.f, fb = 0.f;
     if (depth == level) {
@@ -483,7 +487,8 @@ __global__ __launch_bounds__(KT_THREADS, G == 32 ? 2 : 1) void kda_tree_kernel(c
       fa = A[first + level];
       fb = B[first + level];
     }
-    if (!__syncthreads_or(depth > level)) break;
+    if (level == last) break;
+    __syncthreads();
     if (depth > level) {
 #pragma unroll
       for (int m = 0; m < OUT; m++) {
