@@ -110,10 +110,10 @@ struct KdaTreeArgs {
 //               hi hi + hi lo + lo hi: 2^-16 of the magnitudes, where bf16 keeps the range of fp32 (a state in fp16 would overflow at 65,504)
 //   levels      u of the nodes of a depth, then their part in all nodes below: a node has one ancestor at each depth, so a level is one
 //               multiply-add a node and column, in registers, and one barrier
-// What bounds it: latency where a CTA is alone (8 nodes of 32 heads 4.6 us), then shared memory and the barriers between phases.  A CTA of 61 nodes takes 20,700
-// cycles: loads 5,300, splitting 950, pairs 5,700, operands 1,600, products 500, their way out 1,200, levels 4,800, output 650; 8 x 32 heads of 61 nodes 24.8 us (40 MB
-// at 1.6 TB/s), 24 x 64 of 16 nodes 52 (131 MB at 2.5).  Lanes a node, us with 8 / 16 / 32: 24 x 64 heads of 8 nodes 74.8 / 63.5 / 44.6, of 16 84.5 / 72.8 / 51.9,
-// of 30 99.0 / 86.4, 32 heads of 8 5.2 / 4.6 / 4.6.
+// What bounds it: latency where a CTA is alone (8 nodes of 32 heads 4.4 us: 5,900 cycles), then shared memory and the barriers between phases.  A CTA of 61 nodes takes
+// 20,300 cycles: loads, paths and norms 5,100, splitting 740, pairs 5,400, operands 550, products 1,800, their way out 1,200, levels 4,500, output 640; 8 x 32 heads of
+// 61 nodes 24-26 us (40 MB at 1.6 TB/s), 24 x 64 of 16 nodes 52 (131 MB at 2.5).  Lanes a node, us with 8 / 16 / 32: 24 x 64 heads of 8 nodes 74.8 / 63.5 / 44.6, of 16
+// 84.5 / 72.8 / 51.9, of 30 99.0 / 86.4, 32 heads of 8 5.2 / 4.6 / 4.6.
 constexpr int KT_WARPS = 16, KT_THREADS = KT_WARPS * 32;
 // Shared memory of a form: k E, q E (before them k and the decays, behind them u); S_0, then its products; lists of pairs.
 template <int COLS, int G>
