@@ -95,6 +95,11 @@ __global__ __launch_bounds__(256) void mla_simt_kernel(MlaArgs a, MlaPaged pg) {
     } else if (FMT == CACHE_F16) {
       if (tok < 0 || (a.ckv_rows > 0 && tok >= a.ckv_rows)) continue;  // warp-uniform
       simt_key<CACHE_F16>(a.ckv + (size_t)tok * LATENT + lane * 16, 1.f, kf);
+      if (a.kv_factor) {                                   // trees over 8-bit positions that were read first
+        const float f = a.kv_factor[seq * a.factor_stride + i];
+#pragma unroll
+        for (int u = 0; u < 16; u++) kf[u] *= f;
+      }
     } else {
       const int64_t b = pg.block_of(seq, (int)tok);
       if (b < 0 && (sparse || ((a.kv_len || pg.row_seq) && !a.tree_kv))) continue;   // (in a chunk: a key of zeros)

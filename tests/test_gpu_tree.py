@@ -1,6 +1,9 @@
 """Trees of drafted tokens: attention over both latent caches, the KDA convolution and recurrence, and the steps to an accepted node, against
 64 bits and against the calls that decode token by token."""
 import math
+import os
+import subprocess
+import sys
 
 import pytest
 import torch
@@ -220,6 +223,16 @@ def test_two_nodes_by_a_pair_of_ctas(told):
                 assert bool(((out[r].double() - o).abs() <= tol).all()), (s, j)
     for r in (0, m - 2, m - 1):
         assert bool((out[r] == 7).all())
+
+
+@pytest.mark.parametrize("switch", ["HK_MLA_FORCE_SIMT", "HK_MLA_NO_TMA"])
+def test_trees_on_the_cuda_cores(switch):
+    """asked for, and where there is no encoder of tensor maps, when positions of the 8-bit cache are read first all the same; in a process of its own"""
+    names = ("test_nodes_over", "test_scales_where_many_nodes_share_the_keys", "test_positions_without_a_block_and_behind_the_table", "test_what_a_node_does_not_see_has_no_effect",
+             "test_two_nodes_by_a_pair_of_ctas", "test_parents_that_are_no_earlier_node", "test_a_sequence_of_more_rows", "test_a_chain_agrees_with_a_causal_chunk")
+    run = subprocess.run([sys.executable, "-m", "pytest", "-x", "-q", "-m", "gpu", "-p", "no:cacheprovider", "-k", " or ".join(names), os.path.abspath(__file__)],
+                         env={**os.environ, switch: "1"}, capture_output=True, text=True, timeout=600)
+    assert run.returncode == 0, run.stdout[-3000:] + run.stderr[-2000:]
 
 
 def test_parents_that_are_no_earlier_node_hang_on_the_sequence():
