@@ -63,21 +63,25 @@ static int simt_auto_splits(int m, int n_heads, int n_keys) {
   return s;
 }
 
-template <int FMT>
-static int launch_simt_as(const MlaArgs& a, const MlaPaged& pg, cudaStream_t s) {
+template <int FMT, bool TREE>
+static int launch_simt_for(const MlaArgs& a, const MlaPaged& pg, cudaStream_t s) {
   if (a.m > 65535) return HK_ERR_UNSUPPORTED;              // a row is a CTA's z
   static bool attr_set[64] = {false};
   int dev = 0;
   cudaGetDevice(&dev);
   if (dev >= 0 && dev < 64 && !attr_set[dev]) {
-    if (cudaFuncSetAttribute(mla_simt_kernel<FMT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+    if (cudaFuncSetAttribute(mla_simt_kernel<FMT, TREE>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                              (int)MLA_SIMT_SMEM) != cudaSuccess)
       return HK_ERR_CUDA;
     attr_set[dev] = true;
   }
   dim3 grid(a.n_heads / SIMT_HG, a.n_split, a.m);
-  mla_simt_kernel<FMT><<<grid, 256, MLA_SIMT_SMEM, s>>>(a, pg);
+  mla_simt_kernel<FMT, TREE><<<grid, 256, MLA_SIMT_SMEM, s>>>(a, pg);
   return cudaPeekAtLastError() == cudaSuccess ? HK_OK : HK_ERR_CUDA;
+}
+template <int FMT>
+static int launch_simt_as(const MlaArgs& a, const MlaPaged& pg, cudaStream_t s) {
+  return a.tree_kv ? launch_simt_for<FMT, true>(a, pg, s) : launch_simt_for<FMT, false>(a, pg, s);
 }
 static int launch_simt(const MlaArgs& a, cudaStream_t s) { return launch_simt_as<CACHE_F16>(a, MlaPaged{}, s); }
 

@@ -35,7 +35,8 @@ __device__ __forceinline__ void simt_key(const void* row, float scale, float (&k
 
 // grid (n_heads/4, n_split, m), 256 threads.  Warp w walks keys k0+w, k0+w+8, ...; lane owns 16
 // channels; the 8 warps are merged through shared memory at the end.
-template <int FMT>
+// TREE: rows are nodes of trees of drafted tokens (of an instance of its own: the look-up costs the other calls a tenth of their time).
+template <int FMT, bool TREE>
 __global__ __launch_bounds__(256) void mla_simt_kernel(MlaArgs a, MlaPaged pg) {
   extern __shared__ float smem[];
   float* w_acc = smem;                           // [8][4][512]
@@ -47,12 +48,12 @@ __global__ __launch_bounds__(256) void mla_simt_kernel(MlaArgs a, MlaPaged pg) {
   const bool sparse = a.raw_idx != nullptr;
   // a node of a tree: its sequence's cached keys, then the nodes of the tree up to itself, of which those on its path are seen
   MlaTree tree{0, 0, 0, 0, 0, -1};
-  if (a.tree_kv) tree = mla_tree(a, r);
-  const int seq = a.tree_kv ? tree.seq : FMT == CACHE_F16 ? 0 : pg.seq_of(r);
+  if (TREE) tree = mla_tree(a, r);
+  const int seq = TREE ? tree.seq : FMT == CACHE_F16 ? 0 : pg.seq_of(r);
   int n;
   int64_t base = 0;
   KeyList list = {0, 0, 0};
-  if (a.tree_kv) {
+  if (TREE) {
     if (FMT != CACHE_F16) tree.len = (int)min((int64_t)tree.len, pg.room());
     base = tree.base;
     list = key_list(tree.len, 0, 0);
@@ -89,20 +90,20 @@ __global__ __launch_bounds__(256) void mla_simt_kernel(MlaArgs a, MlaPaged pg) {
   for (int i = k0 + wid; i < k1; i += 8) {
     int64_t tok = sparse ? (int64_t)a.raw_idx[(size_t)r * a.kidx + i] : base + list.at(i);
     float kf[16];
-    if (a.tree_kv && i >= tree.len) {
+    if (TREE && i >= tree.len) {
       if (!(tree.path >> (i - tree.len) & 1)) continue;
       simt_key<CACHE_F16>(a.tree_kv + (size_t)(tree.row0 + i - tree.len) * LATENT + lane * 16, 1.f, kf);
     } else if (FMT == CACHE_F16) {
       if (tok < 0 || (a.ckv_rows > 0 && tok >= a.ckv_rows)) continue;  // warp-uniform
       simt_key<CACHE_F16>(a.ckv + (size_t)tok * LATENT + lane * 16, 1.f, kf);
-      if (a.kv_factor) {                                   // trees over 8-bit positions that were read first
+      if (TREE && a.kv_factor) {                           // 8-bit positions that were read first
         const float f = a.kv_factor[seq * a.factor_stride + i];
 #pragma unroll
         for (int u = 0; u < 16; u++) kf[u] *= f;
       }
     } else {
       const int64_t b = pg.block_of(seq, (int)tok);
-      if (b < 0 && (sparse || ((a.kv_len || pg.row_seq) && !a.tree_kv))) continue;   // (in a chunk: a key of zeros)
+      if (b < 0 && !TREE && (sparse || a.kv_len || pg.row_seq)) continue;   // (in a chunk: a key of zeros)
       if (b < 0) {
 #pragma unroll
         for (int u = 0; u < 16; u++) kf[u] = 0.f;
@@ -159,7 +160,7 @@ __global__ __launch_bounds__(256) void mla_simt_kernel(MlaArgs a, MlaPaged pg) {
       o = gl;
     }
     const size_t rh = (size_t)r * a.n_heads + h0 + h;
-    if (a.out && a.tree_kv && tree.node < 0) continue;       // (a row of no tree)
+    if (TREE && a.out && tree.node < 0) continue;            // (a row of no tree)
     if (a.out) {
       a.out[rh * LATENT + ch] = __float2half_rn(gl > 0.f || (keep_nan && gl != 0.f) ? o / gl : 0.f);
     } else {
