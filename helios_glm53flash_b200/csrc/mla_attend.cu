@@ -778,7 +778,7 @@ static Tree8Plan tree8_plan(int m, int n_heads, int n_seqs, bool ragged, bool le
   constexpr TreeCost direct = {{115, 125, 130}, {650, 700, 780}, 800, 300, 500};
   const int64_t time = tree_best_splits(direct, units, n_keys / 64 + 1, sm_count(), &p.n_split);
   const int64_t cap = lens || positions < n_keys ? positions : n_keys;
-  if (group * n_heads != 64 || cap * n_seqs > TREE8_ROWS) return p;
+  if (group * n_heads != 64 || cap > TREE8_ROWS / n_seqs) return p;
   int n_split;
   bool pairs;
   const int64_t read = 300 + (int64_t)n_seqs * n_keys * 35 / 1000;
@@ -795,7 +795,7 @@ static Tree8Plan tree8_plan(int m, int n_heads, int n_seqs, bool ragged, bool le
 }  // namespace hk
 
 HK_API size_t hk_mla8_tree_workspace_bytes(int m, int n_heads, int n_seqs, int n_keys, int64_t positions) {
-  if (m <= 0 || n_heads < hk::SIMT_HG || n_seqs < 1 || n_keys < 0 || positions < 0 || positions > INT32_MAX) return 0;
+  if (m <= 0 || n_heads < hk::SIMT_HG || n_seqs < 1 || n_keys < 0 || positions < 0) return 0;
   size_t most = 0;
   for (int k = 0; k < 4; k++) {                            // (whether the trees are ragged and the lengths on the device)
     if (k < 2 && m % n_seqs != 0) continue;

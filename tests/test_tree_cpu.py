@@ -61,6 +61,20 @@ def test_empty_calls_and_workspaces(lib):
     assert lib.hk_mla8_pages_workspace_bytes(1000, 5) >= 3 * 4000 and lib.hk_mla8_pages_workspace_bytes(5, 1000) >= 3 * 4000
 
 
+def test_tables_of_more_positions_than_31_bits_need_no_less_workspace(lib):
+    for m, heads, keys in ((8, 64, 5001), (64, 64, 32768), (7, 20, 900), (96, 16, 3000)):
+        for seqs in (1, 2, 65535):
+            want = lib.hk_mla8_tree_workspace_bytes(m, heads, seqs, keys, 1 << 30)
+            for positions in (1 << 31, 1 << 38, 2 ** 63 - 1):
+                assert lib.hk_mla8_tree_workspace_bytes(m, heads, seqs, keys, positions) == want
+    # 5,001 keys in a table of 2^31 positions, and the call itself: what is less than the size is refused
+    need = lib.hk_mla8_tree_workspace_bytes(8, 64, 2, 5001, 1 << 31)
+    assert need >= lib.hk_mla_partial_bytes(2, 8 * 64)
+    wide = dict(block=128, stride=1 << 24, pos=5001, split=0)
+    assert call(lib.hk_mla8_tree, TREE8, TREE8_GOOD, **wide) == hk.HK_ERR_WORKSPACE
+    assert call(lib.hk_mla8_tree, TREE8, TREE8_GOOD, **wide, len=A, ws=A, bytes=lib.hk_mla_partial_bytes(2, 8 * 64) - 1) == hk.HK_ERR_WORKSPACE
+
+
 ACCEPT = "kv ckv rows base len pos parent start seqs leaf m told stream"
 ACCEPT_GOOD = dict(kv=A, ckv=A, rows=9, base=None, len=A, pos=0, parent=A, start=A, seqs=2, leaf=A, m=4, told=None, stream=None)
 
