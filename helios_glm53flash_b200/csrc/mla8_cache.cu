@@ -11,6 +11,7 @@
 #include "hk_common.cuh"
 #include "latent8.cuh"
 #include "tree.cuh"
+#include <type_traits>
 
 namespace hk {
 namespace {
@@ -33,7 +34,10 @@ struct AppendArgs {
   int n;
   float eps;
   __half* ckv_new;          // optional [n][512]: the rows as the cache now holds them
-  // accepted nodes of trees of drafted tokens: the rows are those of a path, normalised already, and go behind kv_len (null: pos_start) positions
+};
+// Accepted nodes of trees of drafted tokens: the rows are those of a path, normalised already, and go behind kv_len (null: pos_start) positions.  (A block of
+// arguments of its own: a longer one moved the registers of every append, blocks of 32 82 -> 64, of 16 as e4m3 40 -> 60.)
+struct AcceptArgs : AppendArgs {
   TreeArgs tree;
   const __half* tree_kv;
   const int *leaf, *kv_len;
@@ -49,16 +53,18 @@ struct AppendArgs {
 // 7.1 / 11.2 / 10.2.  A block of 128 over eight, four or two, the most that the SMs have room for at once: one / four / eight, 1,000 rows 12.7 / 5.5 / 5.25,
 // 4,096 (264 CTAs) 13.1 / 5.85 / 6.9; 8,192 by one / two / four 16.4 / 8.4 / 11.4, 20,000 by one / two 20.1 / 23.1.  Under 64 rows the barrier
 // of the cluster costs what it gains (32 rows in blocks of 64, one / two 4.0 / 4.7).
+// MIN: CTAs that an SM is to have room for, 0 as the compiler likes (append_launch).
 constexpr int APPEND_WARPS = 16;
-template <int FMT, int ROWS, bool KEEP, int PARTS, bool TREE = false>
-__global__ void __launch_bounds__(APPEND_WARPS * 32) mla8_append_kernel(AppendArgs a) {
+template <int FMT, int ROWS, bool KEEP, int PARTS, bool TREE = false, int MIN = 0>
+__global__ void __launch_bounds__(APPEND_WARPS * 32, MIN) mla8_append_kernel(std::conditional_t<TREE, AcceptArgs, AppendArgs> a) {
   __shared__ float s_amax[2][APPEND_WARPS], s_part[2];
   __shared__ int s_node[TREE ? TREE_NODES : 1];
   pdl_release();
   pdl_wait();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, seq = blockIdx.y, block = 1 << a.pg.shift;
-  const int p0 = TREE ? max(a.kv_len ? a.kv_len[seq] : a.pos_start, 0) : a.pos[seq];
-  int r0, r1;
+  int p0, r0, r1;
+  if constexpr (TREE) p0 = max(a.kv_len ? a.kv_len[seq] : a.pos_start, 0);
+  else p0 = a.pos[seq];
   if constexpr (TREE) {
     const int2 rows = a.tree.rows(seq);
     const uint64_t path = tree_path(a.tree, rows, a.leaf[seq]);
@@ -214,21 +220,31 @@ __global__ void __launch_bounds__(APPEND_WARPS * 32) mla8_append_kernel(AppendAr
   if (PARTS > 1) asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");   // nobody reads this CTA's maximum any more
 }
 
+// What a CTA has for itself it uses: up to a CTA an SM the kernels take the registers they like best (MIN 1), beyond that as many CTAs an SM as go
+// together.  us, MIN 0 / 1 / 2, e4m3: blocks of 16, one sequence's token 2.2 / 2.0 / 2.2, 256 sequences 3.2 / 3.8 / 2.7, 1,000 6.6 / 11.7 / 7.8; of 32,
+// 4,096 rows (129 CTAs) 3.4 / 3.2 / 4.4, 1,000 sequences 13.0 / 12.5 / 8.6; of 64, 64 rows (four CTAs a block) 3.9 / 3.6 / 3.9, 1,000 sequences 13.5 / 13.4 / 16.6; of
+// 128, 1,000 rows 4.4 / 4.0 / 4.4, 1,000 sequences 10.2 / 15.3 / 10.1.
+template <int FMT, int ROWS, bool KEEP, int PARTS, int MANY>
+cudaError_t append_as(const AppendArgs& a, dim3 grid, bool alone, cudaStream_t s) {
+  return pdl_launch_cluster(PARTS, alone ? mla8_append_kernel<FMT, ROWS, KEEP, PARTS, false, 1> : mla8_append_kernel<FMT, ROWS, KEEP, PARTS, false, MANY>,
+                            dim3(grid.x * PARTS, grid.y), dim3(APPEND_WARPS * 32), 0, s, a);
+}
 template <int FMT>
 cudaError_t append_launch(const AppendArgs& a, dim3 grid, int parts, cudaStream_t s) {
-  const auto kernel = a.pg.shift == 4 ? mla8_append_kernel<FMT, 1, true, 1>
-                      : a.pg.shift == 5 ? mla8_append_kernel<FMT, 2, true, 1>
-                      : a.pg.shift == 6 ? (parts > 1 ? mla8_append_kernel<FMT, 1, true, 4> : mla8_append_kernel<FMT, 4, true, 1>)
-                                        : (parts == 8   ? mla8_append_kernel<FMT, 1, true, 8>
-                                           : parts == 4 ? mla8_append_kernel<FMT, 2, true, 4>
-                                           : parts == 2 ? mla8_append_kernel<FMT, 4, true, 2> : mla8_append_kernel<FMT, 8, false, 1>);
-  return pdl_launch_cluster(parts, kernel, dim3(grid.x * parts, grid.y), dim3(APPEND_WARPS * 32), 0, s, a);
+  const int64_t ctas = (int64_t)grid.x * parts * grid.y;
+  const bool alone = ctas <= sm_count();
+  if (a.pg.shift == 4) return ctas <= 3 * (int64_t)sm_count() ? append_as<FMT, 1, true, 1, 2>(a, grid, alone, s) : append_as<FMT, 1, true, 1, 0>(a, grid, false, s);
+  if (a.pg.shift == 5) return append_as<FMT, 2, true, 1, 2>(a, grid, alone, s);
+  if (a.pg.shift == 6) return parts > 1 ? append_as<FMT, 1, true, 4, 0>(a, grid, alone, s) : append_as<FMT, 4, true, 1, 1>(a, grid, alone, s);
+  return parts == 8   ? append_as<FMT, 1, true, 8, 0>(a, grid, alone, s)
+         : parts == 4 ? append_as<FMT, 2, true, 4, 0>(a, grid, alone, s)
+         : parts == 2 ? append_as<FMT, 4, true, 2, 0>(a, grid, alone, s) : append_as<FMT, 8, false, 1, 0>(a, grid, alone, s);
 }
 
 // Accepted nodes: the append of rows that are normalised already, a CTA a block that the longest path may touch; 2.7 us for one sequence, 3.0 for 24 (path, then
 // lengths, table, scale and rows: four dependent loads).
 template <int FMT>
-cudaError_t accept_launch(const AppendArgs& a, cudaStream_t s) {
+cudaError_t accept_launch(const AcceptArgs& a, cudaStream_t s) {
   const int block = 1 << a.pg.shift;
   const auto kernel = a.pg.shift == 4   ? mla8_append_kernel<FMT, 1, true, 1, true>
                       : a.pg.shift == 5 ? mla8_append_kernel<FMT, 2, true, 1, true>
@@ -413,7 +429,7 @@ HK_API int hk_mla8_tree_accept(const void* tree_kv, void* ckv8, float* scales, i
                                int table_stride, const int* kv_len, int pos_start, const int* parent, const int* tree_start, int n_seqs,
                                const int* leaf, int m, int* len_out, void* stream) {
   using namespace hk;
-  AppendArgs a{};
+  AcceptArgs a{};
   HK_REQUIRE((tree_kv || m == 0) && leaf && pos_start >= 0 && aligned(tree_kv, 16) && (!len_out || len_out != kv_len));
   HK_REQUIRE(tree_args(&a.tree, parent, tree_start, n_seqs, m));
   HK_REQUIRE(mla8_paged(&a.pg, ckv8, scales, dtype, n_blocks, block, block_table, table_stride, n_seqs, nullptr));
