@@ -140,6 +140,25 @@ def test_pages_come_and_go(n_blocks, block, n_seqs, stride):
             pool.reserve([(s, length()) for s in some()])
 
 
+@pytest.mark.parametrize("n_blocks,block,n_seqs,stride", [(700, 16, 12, 4096), (90, 64, 4, 16384), (9000, 16, 10, 2049)])
+def test_tables_that_are_wider_than_what_is_held(n_blocks, block, n_seqs, stride):
+    """room for long contexts, of which the sequences use a part; once a sequence takes more than there is"""
+    pool = Pool("i8", n_blocks, block, n_seqs, stride)
+    rng = random.Random(stride)
+    some = lambda: rng.sample(range(n_seqs), rng.randint(1, n_seqs))  # noqa: E731
+    length = lambda: rng.choice([0, 1, block, block * 5 + 1, rng.randint(0, block * 40)])  # noqa: E731
+    pool.reserve([(s, length()) for s in range(n_seqs)])
+    for turn in range(2):
+        pool.fork([(rng.choice([0, 1]), s, length()) for s in range(2, n_seqs)])
+        pool.free([(s, rng.choice([0, length()])) for s in some()])
+        pool.compact()
+        pool.reserve([(s, length()) for s in some()])
+    pool.free([(0, 0)])
+    pool.reserve([(0, min(block * stride, block * (n_blocks + 3)))])
+    pool.fork([(0, 1, block * stride - 1)])
+    pool.compact()
+
+
 def test_what_names_no_sequence_and_no_block_is_passed_over():
     pool = Pool("i8", 40, 16, 6, 8)
     pool.reserve([(0, 50), (-1, 100), (6, 100), (1, 100), (1 << 30, 7), (2, -3)])
@@ -270,6 +289,74 @@ def test_a_captured_turn_of_calls_follows_the_device():
     gone.copy_(ints([5]))
     want.copy_(ints([112]))
     model([(3, 1, 112), (3, 0, 7)], 5, 112)
+
+
+def same(pool, other):
+    return all(torch.equal(a.view(torch.uint8) if a.element_size() == 1 else a, b.view(torch.uint8) if b.element_size() == 1 else b) for a, b in zip(pool.tensors, other.tensors))
+
+
+def test_a_captured_turn_with_scratch_of_its_own():
+    """the calls take and give back their scratch inside the capture, where other tensors are made and let go too"""
+    pool, other = Pool("e4m3", 60, 16, 6, 7), Pool("e4m3", 60, 16, 6, 7)
+    for p in (pool, other):
+        p.reserve([(0, 100), (1, 60), (2, 33), (3, 112)])
+    par, chi, lens, gone, want = ints([0, 1]), ints([4, 5]), ints([90, 50]), ints([2]), ints([40])
+    side, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.graph(graph, stream=side):
+        hk.mla8_pages_fork(*pool.tensors, par, chi, lens, 2)
+        kept = torch.full((5000,), 5, dtype=torch.int32, device="cuda")
+        hk.mla8_pages_free(*pool.tensors, gone, None, 1)
+        torch.full((300,), 9, dtype=torch.int32, device="cuda")
+        hk.mla8_pages_compact(*pool.tensors)
+        last = torch.full((300,), 7, dtype=torch.int32, device="cuda")
+        hk.mla8_pages_reserve(*pool.tensors, gone, want, 1)
+    for pairs, s, n in (([(0, 4, 90), (1, 5, 50)], 2, 40), ([(3, 1, 112), (3, 0, 7)], 5, 112), ([(1, 2, 17), (4, 3, 90)], 0, 1)):
+        for t, v in ((par, [x[0] for x in pairs]), (chi, [x[1] for x in pairs]), (lens, [x[2] for x in pairs]), (gone, [s]), (want, [n])):
+            t.copy_(ints(v))
+        graph.replay()
+        finish()
+        other.fork(pairs)
+        other.free([(s, 0)])
+        other.compact()
+        other.reserve([(s, n)])
+        assert same(pool, other) and bool((kept == 5).all()) and bool((last == 7).all())
+
+
+@pytest.mark.parametrize("given", [True, False])
+def test_two_pools_on_two_streams_at_once(given):
+    """given: the stream as an argument, else the current one; scratch of the calls is each stream's own"""
+    pools = [Pool("i8", 3000, 16, 40, 60), Pool("e4m3", 900, 32, 30, 40)]
+    others = [Pool("i8", 3000, 16, 40, 60), Pool("e4m3", 900, 32, 30, 40)]
+    rng, turns = random.Random(5), []
+    for p in others:
+        turns.append([])
+        n_seqs, room = len(p.rows), p.block * len(p.rows[0])
+        lens = [rng.randint(0, room) for _ in range(n_seqs)]
+        turns[-1].append(("reserve", [(s, n) for s, n in enumerate(lens)]))
+        for _ in range(4):
+            seqs = rng.sample(range(n_seqs), n_seqs)
+            turns[-1].append(("fork", [(seqs[i % 5], c, rng.randint(0, room)) for i, c in enumerate(seqs[5:20])]))
+            turns[-1].append(("free", [(s, rng.choice([0, rng.randint(0, room)])) for s in seqs[:12]]))
+            turns[-1].append(("compact",))
+            turns[-1].append(("reserve", [(s, rng.randint(0, room)) for s in seqs[::2]]))
+    lists = [[[ints([x[i] for x in t[1]]) for i in range(len(t[1][0]))] if len(t) > 1 else None for t in ts] for ts in turns]
+    sides = [torch.cuda.Stream() for _ in range(2)]
+    finish()
+    calls = dict(fork=hk.mla8_pages_fork, free=hk.mla8_pages_free, reserve=hk.mla8_pages_reserve, compact=hk.mla8_pages_compact)
+    for step in range(len(turns[0])):
+        for p, ts, ls, side in zip(pools, turns, lists, sides):
+            args = p.tensors + ((*ls[step], len(ts[step][1])) if ls[step] else ())
+            if given:
+                calls[ts[step][0]](*args, stream=side)
+            else:
+                with torch.cuda.stream(side):
+                    calls[ts[step][0]](*args)
+    finish()
+    for p, ts in zip(others, turns):
+        for what, *rest in ts:
+            getattr(p, what)(*rest)
+    assert same(pools[0], others[0]) and same(pools[1], others[1])
 
 
 def test_samples_of_one_prompt_append_and_attend_on_their_own():

@@ -471,6 +471,33 @@ def test_hard_resets_and_gates_of_zero():
     assert bool(((f32.double() - want).abs() <= tol).all())
 
 
+@pytest.mark.parametrize("nodes", [1, 16, 17, 33, 64])
+@pytest.mark.parametrize("heads", [3, 40, 90])
+def test_how_precise_the_products_with_the_state_are(nodes, heads):
+    """Children of the sequence alone, so that out_f32 is (q E)^T S + (q k) u, u = beta (v - (k E)^T S).  A number is two of bf16 and at most 2^-16 of it: of a product's
+    four parts the smallest may be left out, 3 * 2^-16 of the product at most, and 384 additions in fp32 lose 2^-23 of the magnitudes each (the tensor cores may cut off).
+    Rows are fp32: norm, product and exponential of an argument down to -5 are within 16 roundings of 2^-24.  q k is a sum of 128 products of such rows."""
+    gen = gen_of(nodes + heads)
+    x = kda_inputs(gen, nodes, heads, 1)
+    f32 = torch.empty(nodes, heads, 128, device="cuda")
+    hk.kda_tree_decode(x["qkv"], x["g"], x["beta"], x["state"], ints([-1] * nodes), torch.empty(nodes, heads, 128, dtype=torch.bfloat16, device="cuda"), nodes, heads, out_f32=f32)
+    finish()
+    q, k, v = x["qkv"].double().view(nodes, 3, heads, 128).unbind(1)
+    q, k = (r / torch.sqrt(r.pow(2).sum(-1, keepdim=True) + 1e-6) for r in (q, k))
+    e, s, beta = torch.exp(x["g"].double()), x["state"][0].double(), x["beta"].double()[..., None]
+    dot = lambda a, b: torch.einsum("nhk,hkv->nhv", a, b)  # noqa: E731
+    row = 16 * 2.0 ** -24
+    part = 3 * 2.0 ** -16 + 384 * 2.0 ** -23 + row
+    u = beta * (v - dot(k * e, s))
+    u_mag = beta * (v.abs() + dot((k * e).abs(), s.abs()))
+    u_off = beta * part * dot((k * e).abs(), s.abs()) + 4 * 2.0 ** -24 * u_mag
+    qk, qk_mag = (q * k).sum(-1, keepdim=True), (q * k).abs().sum(-1, keepdim=True)
+    want = dot(q * e, s) + qk * u
+    mag = dot((q * e).abs(), s.abs()) + qk_mag * u_mag
+    tol = part * dot((q * e).abs(), s.abs()) + qk.abs() * u_off + (130 * 2.0 ** -24 + 2 * row) * qk_mag * (u.abs() + u_off) + 8 * 2.0 ** -24 * mag
+    assert bool(((f32.double() - want * 128 ** -0.5).abs() <= tol * 128 ** -0.5).all())
+
+
 def test_what_is_not_on_a_nodes_path_has_no_effect_on_it():
     gen, heads, tree = gen_of(12), 3, tree_of("binary15")
     x = kda_inputs(gen, 15, heads, 1)
@@ -547,6 +574,47 @@ def test_accepted_states_are_those_of_token_by_token_decoding(heads, n):
         else:
             assert torch.equal(state[slots[s]], x["state"][slots[s]]) and torch.equal(win[slots[s]], window[slots[s]]), s
     assert torch.equal(state[0], x["state"][0]) and torch.equal(win[0], window[0]), "a slot of nobody"
+
+
+@pytest.mark.parametrize("raw", [False, True])
+def test_accepted_states_that_stream_through_shared_memory(raw):
+    """four accepted heads a CTA and more, so that every buffer is used again: paths of one to eight batches of tokens, sequences without an accepted node in between;
+    bit for bit what decoding token by token gives"""
+    heads, lengths = 64, [1, 8, 9, 16, 64, 2, 7, 17, 3, 24, 5]
+    sms = torch.cuda.get_device_properties(0).multi_processor_count
+    n = (8 * sms // heads + 1) * 4 // 3 + 2
+    gen, dim = gen_of(77), 3 * heads * 128
+    trees = [list(range(-1, lengths[s % len(lengths)] - 1)) if s % 3 else tree_of((20 + s, s)) for s in range(n)]
+    leaves = [(-1, 64)[s % 8 == 3] if s % 4 == 3 else len(t) - 1 for s, t in enumerate(trees)]
+    assert heads * sum(s % 4 != 3 for s in range(n)) >= 4 * 2 * sms
+    starts, parent, tree_start = layout(trees)
+    m, slots = starts[-1], [(5 * s + 2) % n for s in range(n)]
+    if math.gcd(5, n) > 1:
+        slots = list(range(n))[::-1]
+    x = kda_inputs(gen, m, heads, n)
+    x32, window = randn(gen, m, dim), randn(gen, n, dim, 4).bfloat16()
+    gates, more = (x["g"], x["beta"]), {}
+    if raw:
+        f, b, dt, a_log = randn(gen, m, heads, 128), randn(gen, m, heads), 0.5 * randn(gen, heads, 128), randn(gen, heads)
+        hk.kda_gate(b, f, dt, a_log, -5.0, x["beta"], x["g"], m, heads, 128)
+        gates, more = (f, b), dict(dt_bias=dt, a_log=a_log, lower_bound=-5.0)
+    state, win = x["state"].clone(), window.clone()
+    hk.kda_tree_accept(x32, win, x["qkv"], *gates, state, parent, ints(leaves), m, heads, n_seqs=n, tree_start=tree_start, slots=ints(slots), **more)
+    alone = x["state"].clone()                               # the states without windows
+    hk.kda_tree_accept(None, None, x["qkv"], *gates, alone, parent, ints(leaves), m, heads, n_seqs=n, tree_start=tree_start, slots=ints(slots), **more)
+    finish()
+    assert torch.equal(alone, state)
+    taps = torch.zeros(dim, 4, dtype=torch.bfloat16, device="cuda")
+    for s in range(n):
+        at = slice(slots[s], slots[s] + 1)
+        one, w = x["state"][at].clone(), window[at].clone()
+        rows = [starts[s] + j for j in path(trees[s], leaves[s])] if 0 <= leaves[s] < len(trees[s]) else []
+        if rows:
+            k = len(rows)
+            hk.cuda_recurrent_gated_delta_rule(x["qkv"][rows].contiguous(), x["g"][rows].contiguous(), x["beta"][rows].contiguous(), one,
+                                               torch.empty(1, k, heads, 128, dtype=torch.bfloat16, device="cuda"), 1, k, heads, heads, 128, 128, 1, None, True, False, force_recurrent=True)
+            hk.kda_cast_conv(x32[rows].contiguous(), w, None, taps, None, torch.empty(1, k, dim, dtype=torch.bfloat16, device="cuda"), 1, dim, k, True)
+        assert torch.equal(state[at], one) and torch.equal(win[at], w), s
 
 
 @pytest.mark.parametrize("dim", [4, 384, 2060])
@@ -701,6 +769,34 @@ def test_two_calls_at_once():
     finish()
     for out in outs:
         assert all(torch.equal(a, b) for a, b in zip(out, alone))
+
+
+def test_the_same_call_gives_the_same_bits():
+    """a CTA a node with splits, pairs of CTAs, several nodes a CTA; the 8-bit cache converted and read first; every form of the recurrence and of the accepted step"""
+    gen = gen_of(41)
+    ckv = randn(gen, 9000, 512).half()
+    ckv8, scales = cache(gen, "e4m3", 150, 64, spread=0.7)
+    calls, keep = [], []
+    for nodes, heads, n in ((8, 64, 5001), (64, 64, 4000), (40, 16, 2000), (1, 64, 9000), (3, 20, 700)):
+        tree, q, rows = ints(tree_of((nodes, 1))), (randn(gen, nodes, heads, 512) * 0.7).half(), randn(gen, nodes, 512).half()
+        calls.append((lambda o, a=(tree, q, rows, nodes, heads, n): hk.mla_tree_decode(a[1], ckv, a[2], a[0], o, a[3], a[5], n_heads=a[4]), (nodes, heads, 512), torch.float16))
+        calls.append((lambda o, a=(tree, q, rows, nodes, heads, n): hk.mla8_tree_decode(a[1], ckv8, scales, a[2], a[0], o, a[3], a[5], n_heads=a[4]), (nodes, heads, 512), torch.float16))
+    for nodes, heads in ((8, 2), (30, 60), (61, 200), (13, 400)):
+        x, tree = kda_inputs(gen, nodes, heads, 1), ints(tree_of((nodes, 2)))
+        keep.append(x)
+        calls.append((lambda o, a=(x, tree, nodes, heads): hk.kda_tree_decode(a[0]["qkv"], a[0]["g"], a[0]["beta"], a[0]["state"], a[1], o, a[2], a[3]), (nodes, heads, 128), torch.bfloat16))
+
+        def accept(o, a=(x, tree, nodes, heads)):
+            o.copy_(a[0]["state"])
+            hk.kda_tree_accept(None, None, a[0]["qkv"], a[0]["g"], a[0]["beta"], o, a[1], ints([a[2] - 1]), a[2], a[3])
+
+        calls.append((accept, (1, heads, 128, 128), torch.float32))
+    for call, shape, dtype in calls:
+        outs = [torch.empty(shape, dtype=dtype, device="cuda") for _ in range(4)]
+        for o in outs:
+            call(o)
+        finish()
+        assert all(torch.equal(o, outs[0]) for o in outs), shape
 
 
 def test_calls_without_rows_do_nothing():
