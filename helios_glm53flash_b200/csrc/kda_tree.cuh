@@ -163,9 +163,15 @@ __device__ __forceinline__ float kt_beta(const KdaTreeArgs& a, int r, int head) 
                : __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(a.beta)[i]);
 }
 __device__ __forceinline__ float dot4(float4 a, float4 b) { return fmaf(a.w, b.w, fmaf(a.z, b.z, fmaf(a.y, b.y, a.x * b.x))); }
-// four numbers as bf16, and what that leaves of them as bf16
+// Four numbers as bf16, and what that leaves of them as bf16.  WIDE: of all fp32; the largest bf16 stands for what would round to infinity, so that something finite
+// stays finite (3.3895e38 to 3.4028e38; an infinite number leaves an infinite one).
+template <bool WIDE = false>
 __device__ __forceinline__ void kt_split(float4 x, uint2& hi, uint2& lo) {
-  const __nv_bfloat162 h0 = __floats2bfloat162_rn(x.x, x.y), h1 = __floats2bfloat162_rn(x.z, x.w);
+  __nv_bfloat162 h0 = __floats2bfloat162_rn(x.x, x.y), h1 = __floats2bfloat162_rn(x.z, x.w);
+  if (WIDE) {
+    asm("cvt.rn.satfinite.bf16x2.f32 %0, %1, %2;" : "=r"(*reinterpret_cast<uint32_t*>(&h0)) : "f"(x.y), "f"(x.x));
+    asm("cvt.rn.satfinite.bf16x2.f32 %0, %1, %2;" : "=r"(*reinterpret_cast<uint32_t*>(&h1)) : "f"(x.w), "f"(x.z));
+  }
   const float2 f0 = __bfloat1622float2(h0), f1 = __bfloat1622float2(h1);
   const __nv_bfloat162 l0 = __floats2bfloat162_rn(x.x - f0.x, x.y - f0.y), l1 = __floats2bfloat162_rn(x.z - f1.x, x.w - f1.y);
   hi = make_uint2(*reinterpret_cast<const uint32_t*>(&h0), *reinterpret_cast<const uint32_t*>(&h1));
@@ -335,7 +341,7 @@ __global__ __launch_bounds__(KT_THREADS, G == 32 ? 2 : 1) void kda_tree_kernel(c
     const uint32_t off = COLS == 32 ? c * 64 + (((v >> 3) ^ (c >> 1 & 3)) << 4) + (v & 4) * 2
                                     : (v >> 6) * F::S_BLOCK + c * 128 + (((v >> 3 & 7) ^ (c & 7)) << 4) + (v & 4) * 2;
     uint2 hi, lo;
-    kt_split(st[i], hi, lo);
+    kt_split<true>(st[i], hi, lo);
     *reinterpret_cast<uint2*>(smem + F::S + off) = hi;
     *reinterpret_cast<uint2*>(smem + F::S + F::S_BYTES + off) = lo;
   }

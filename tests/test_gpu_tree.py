@@ -471,6 +471,32 @@ def test_hard_resets_and_gates_of_zero():
     assert bool(((f32.double() - want).abs() <= tol).all())
 
 
+@pytest.mark.parametrize("nodes", [9, 30, 60])
+@pytest.mark.parametrize("heads", [2, 60, 200])
+def test_states_of_the_largest_numbers(nodes, heads):
+    """states up to the largest number of fp32, which bf16 has no neighbour above for; one that is not finite shows in its column of every node, and nowhere else"""
+    gen, tree = gen_of(nodes), tree_of((nodes, 1))
+    x = kda_inputs(gen, nodes, heads, 1)
+
+    def call():
+        f32 = torch.empty(nodes, heads, 128, device="cuda")
+        hk.kda_tree_decode(x["qkv"], x["g"], x["beta"], x["state"], ints(tree), torch.empty(nodes, heads, 128, dtype=torch.bfloat16, device="cuda"), nodes, heads, out_f32=f32)
+        finish()
+        return f32
+
+    x["state"][0, :, [5, 100, 3, 64], [7, 70, 127, 0]] = 0.0
+    base = call()
+    x["state"][0, :, [5, 100, 3, 64], [7, 70, 127, 0]] = torch.tensor([3.4e38, -3.395e38, torch.finfo(torch.float32).max, -3.38953139e38], device="cuda")
+    out, (want, tol) = call(), kda_wanted(x, heads, [0], [tree], [0])
+    large = [0, 7, 70, 127]
+    rest = [c for c in range(128) if c not in large]
+    assert bool(torch.isfinite(out).all()) and torch.equal(out[..., rest], base[..., rest])
+    assert bool(((out.double() - want).abs() <= tol)[..., large].all())
+    x["state"][0, :, [5, 100, 3, 64], [7, 70, 127, 0]] = torch.tensor([INF, -INF, NAN, INF], device="cuda")
+    out = call()
+    assert not bool(torch.isfinite(out[..., large]).any()) and torch.equal(out[..., rest], base[..., rest])
+
+
 @pytest.mark.parametrize("nodes", [1, 16, 17, 33, 64])
 @pytest.mark.parametrize("heads", [3, 40, 90])
 def test_how_precise_the_products_with_the_state_are(nodes, heads):
