@@ -876,8 +876,8 @@ __global__ __launch_bounds__(FT_THREADS, 1) void mla_flash_tc_kernel(
 template <int PARTS, bool FACT>
 __global__ __launch_bounds__(FT_THREADS, 1) void mla_tree_tc_kernel(
     MlaArgs a, int* __restrict__ status, const __grid_constant__ CUtensorMap tmap_box, const __grid_constant__ CUtensorMap tmap_rows,
-    const __grid_constant__ CUtensorMap tmap_q, const __grid_constant__ CUtensorMap tmap_o, const __grid_constant__ CUtensorMap tmap_tree) {
-  ft_body<false, false, false, PARTS, true, FACT>(a, status, tmap_box, tmap_rows, tmap_q, tmap_o, tmap_tree);
+    const __grid_constant__ CUtensorMap tmap_q, const __grid_constant__ CUtensorMap tmap_tree) {
+  ft_body<false, false, false, PARTS, true, FACT>(a, status, tmap_box, tmap_rows, tmap_q, tmap_rows, tmap_tree);   // (rows of nodes leave without a map)
 }
 
 }  // namespace hk
@@ -1060,7 +1060,7 @@ int mla_flash_tc_launch(const MlaArgs& a, cudaStream_t s, bool clusters) {
       return HK_ERR_UNSUPPORTED;
     const int64_t n_pairs = tree_units(a.m, a.tree.n_seqs, a.tree.start, 2);
     const cudaError_t e = pdl_launch_cluster(2, a.kv_factor ? mla_pair_tree_tc_kernel<true> : mla_pair_tree_tc_kernel<false>, dim3((unsigned)(2 * n_pairs * a.n_split)), dim3(PT_THREADS),
-                                             FS_SMEM, s, a, device_status_ptr(), box, vbox, rows, qmap, omap, tree_k, tree_v);
+                                             FS_SMEM, s, a, device_status_ptr(), box, vbox, rows, qmap, tree_k, tree_v);
     return e == cudaSuccess && cudaPeekAtLastError() == cudaSuccess ? HK_OK : HK_ERR_CUDA;
   }
   if (pairs) {
@@ -1090,7 +1090,7 @@ int mla_flash_tc_launch(const MlaArgs& a, cudaStream_t s, bool clusters) {
     if (!rows_map(&tree, a.tree_kv, a.m)) return HK_ERR_UNSUPPORTED;
     const auto kernel = a.kv_factor ? (parts == 1 ? mla_tree_tc_kernel<1, true> : parts == 2 ? mla_tree_tc_kernel<2, true> : mla_tree_tc_kernel<4, true>)
                                     : (parts == 1 ? mla_tree_tc_kernel<1, false> : parts == 2 ? mla_tree_tc_kernel<2, false> : mla_tree_tc_kernel<4, false>);
-    const cudaError_t e = pdl_launch(kernel, dim3((unsigned)items), dim3(FT_THREADS), FS_SMEM, s, a, device_status_ptr(), box, rows, qmap, omap, tree);
+    const cudaError_t e = pdl_launch(kernel, dim3((unsigned)items), dim3(FT_THREADS), FS_SMEM, s, a, device_status_ptr(), box, rows, qmap, tree);
     return e == cudaSuccess && cudaPeekAtLastError() == cudaSuccess ? HK_OK : HK_ERR_CUDA;
   }
   const auto kernel = a.raw_idx        ? mla_flash_tc_kernel<true, false, false>

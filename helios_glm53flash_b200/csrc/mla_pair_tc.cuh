@@ -627,9 +627,9 @@ __global__ __launch_bounds__(PT_THREADS, 1) void mla_pair_tc_kernel(
 template <bool FACT>
 __global__ __launch_bounds__(PT_THREADS, 1) void mla_pair_tree_tc_kernel(
     MlaArgs a, int* __restrict__ status, const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ CUtensorMap tmap_v,
-    const __grid_constant__ CUtensorMap tmap_rows, const __grid_constant__ CUtensorMap tmap_q, const __grid_constant__ CUtensorMap tmap_o,
-    const __grid_constant__ CUtensorMap tmap_tree_k, const __grid_constant__ CUtensorMap tmap_tree_v) {
-  pt_body<false, true, FACT>(a, status, tmap_k, tmap_v, tmap_rows, tmap_q, tmap_o, tmap_tree_k, tmap_tree_v);
+    const __grid_constant__ CUtensorMap tmap_rows, const __grid_constant__ CUtensorMap tmap_q, const __grid_constant__ CUtensorMap tmap_tree_k,
+    const __grid_constant__ CUtensorMap tmap_tree_v) {
+  pt_body<false, true, FACT>(a, status, tmap_k, tmap_v, tmap_rows, tmap_q, tmap_rows, tmap_tree_k, tmap_tree_v);
 }
 
 }  // namespace hk
