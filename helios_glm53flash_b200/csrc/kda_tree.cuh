@@ -7,9 +7,10 @@ namespace hk {
 
 // ---- short convolution (window 4): a node's window is its ancestors' inputs, then the sequence's ----
 // Grid (groups of 256 channels, sequences): a thread has four channels of every fourth node.  The tree's inputs go through shared memory as bf16, so each is read
-// once; fp32 chain over the window, taps ascending, as conv4_silu_bf16.  us, 8 x 61 nodes of 12,288 channels 11.9
-// (36 MB; load, then exponentials and stores, with 2.6 CTAs an SM to overlap them), 24 x 13 of 24,576 16.0 (46 MB), 1 x 8 2.6; a CTA a row and 1,024 channels, which
-// looks up its ancestors one after the other and reads four inputs for one, 20.5, 24.7 and 2.7.
+// once; fp32 chain over the window, taps ascending, as conv4_silu_bf16.  us, inputs in the L2 / from HBM: 8 x 61
+// nodes of 12,288 channels 11.8 / 14.8 (36 MB), 24 x 13 of 24,576 16.3 / 22.2 (46 MB, 2.1 TB/s), 1 x 8 2.5.  Bound by waiting: a CTA loads its tree, meets a barrier, then takes
+// exponentials and stores, with 2.6 and 15.6 CTAs an SM, four at a time, to overlap these.  A CTA a row and 1,024 channels, which looks up its ancestors one after the other and reads four
+// inputs for one, took 20.5, 24.7 (in the L2) and 2.7.
 constexpr int KTC_GROUPS = 64, KTC_NODES = 4;              // channel groups of four, nodes at once
 __global__ __launch_bounds__(KTC_GROUPS * KTC_NODES) void kda_tree_conv_kernel(const float* x, const __nv_bfloat16* conv_state, const int* slots, const __nv_bfloat16* w,
                                                                                const __nv_bfloat16* bias, __nv_bfloat16* out, TreeArgs tree, int dim, int activation) {
@@ -107,18 +108,20 @@ struct KdaTreeArgs {
 //   tokens      q and k normalised, decays; k and decays of all nodes to shared memory
 //   pairs       A and B of a node with its ancestors, up its path: a dot product of two rows and the decays between them by its G lanes
 //   product     rows k E and q E of all nodes with S_0 on the tensor cores.  Both operands as two bf16 numbers, x = hi + lo, and three products
-//               hi hi + hi lo + lo hi: 2^-16 of the magnitudes, where bf16 keeps the range of fp32 (a state in fp16 would overflow at 65,504)
+//               hi hi + hi lo + lo hi: off by 3 * 2^-16 of the magnitudes at most (lo lo and what two bf16 leave of either), where bf16 keeps the range of fp32 (a
+//               state in fp16 would overflow at 65,504)
 //   levels      u of the nodes of a depth, then their part in all nodes below: a node has one ancestor at each depth, so a level is one
 //               multiply-add a node and column, in registers, and one barrier
-// What bounds it: latency where a CTA is alone (8 nodes of 32 heads 4.4 us: 5,900 cycles), then shared memory and the barriers between phases.  A CTA of 61 nodes takes
+// What bounds it: latency where a CTA is alone (8 nodes of 32 heads 4.1 us in a graph: 5,900 cycles), then shared memory and the barriers between phases.  A CTA of 61 nodes takes
 // 20,300 cycles: loads, paths and norms 5,100, splitting 740, pairs 5,400, operands 550, products 1,800, their way out 1,200, levels 4,500, output 640; 8 x 32 heads of
-// 61 nodes 24-26 us (40 MB at 1.6 TB/s), 24 x 64 of 16 nodes 52 (131 MB at 2.5).  Lanes a node, us with 8 / 16 / 32: 24 x 64 heads of 8 nodes 74.8 / 63.5 / 44.6, of 16
-// 84.5 / 72.8 / 51.9, of 30 99.0 / 86.4, 32 heads of 8 5.2 / 4.6 / 4.6.
+// 61 nodes 25.6 us (40 MB at 1.6 TB/s), 24 x 64 of 16 nodes 50.8 (131 MB at 2.6).  Lanes a node, us in a graph with 8 / 16 / 32: 24 x 64 heads of 8 nodes 71.2 / 59.9 /
+// 43.5, of 16 80.2 / 68.8 / 50.8, of 30 93.6 / 81.1.
 constexpr int KT_WARPS = 16, KT_THREADS = KT_WARPS * 32;
 // Shared memory of a form: k E, q E (before them k and the decays, behind them u); S_0, then its products; lists of pairs.
 template <int COLS, int G>
 struct KtForm {
-  // Up to 32 nodes: M = 64 in the form that spreads them over all lanes (columns from COLS / 2 on in lanes 64-127), half the operand, two CTAs an SM
+  // Up to 32 nodes: M = 64 in the form that spreads them over all lanes (columns from COLS / 2 on in lanes 64-127), half the operand.  Two CTAs an SM up to 16 nodes
+  // only: 17 to 32 take 72 to 120 registers a thread, of 512
   static constexpr bool HALF = G >= 16 && COLS >= 64;
   static constexpr int M = HALF ? 64 : 128;
   // Rows of q E behind those of k E.  Up to 16 nodes: the second numbers of both are 32 rows of the same operand, so S_0 is read by two products instead of
@@ -550,8 +553,8 @@ static int kt_nodes(const KdaTreeArgs& a, cudaStream_t s) {
 }
 template <bool GATED>
 static int kt_run(const KdaTreeArgs& a, cudaStream_t s) {
-  // Few heads: a head's columns over two or four CTAs, which prepare the tokens each for itself.  us with 32 / 64 / 128 columns: 32 heads of 8 nodes 4.6 / 4.6 / 5.4,
-  // of 61 10.1 / 10.6 / 12.0; 64 heads 6.2 / 4.7 / 5.4 and 19.2 / 10.7 / 12.1; 128 heads 11.5 / 7.2 / 6.3 and 38.6 / 21.1 / 12.9
+  // Few heads: a head's columns over two or four CTAs, which prepare the tokens each for itself.  us in a graph with 32 / 64 / 128 columns: 32 heads
+  // of 8 nodes 4.1 / 4.3 / 4.9, of 61 9.1 / 9.8 / 11.5; 64 heads 5.5 / 4.3 / 5.0 and 17.5 / 10.0 / 11.6; 128 heads 9.7 / 5.8 / 5.1 and 34.2 / 19.3 / 11.7
   const int64_t heads = (int64_t)a.H * a.tree.n_seqs;
   if (4 * heads <= sm_count()) return kt_nodes<GATED, 32>(a, s);
   if (2 * heads <= sm_count()) return kt_nodes<GATED, 64>(a, s);
@@ -960,7 +963,7 @@ HK_API int hk_kda_tree_accept(const float* x32, void* conv_state, const void* mi
   a.x = x32;
   a.conv_state = (__nv_bfloat16*)conv_state;
   a.leaf = leaf;
-  // up to half a head an SM by two CTAs a head: a path of five of 64 heads 6.2 / 5.4 us (one / two), of 128 6.7 / 7.0; four 32 heads 6.2 / 6.0 / 5.8
+  // up to half a head an SM by two CTAs a head: us in a graph with one / two / four, the path of a tree of 8 nodes, 32 heads 5.4 / 4.9 / 4.5, 64 5.5 / 5.0 / 5.3, 128 5.6 / 6.1 / 8.5
   const int64_t heads = (int64_t)num_heads * n_seqs;
   // More than five heads to two SMs stream through shared memory.  us with states that are not in the L2, a CTA a head / streamed, trees of 1 and of 13 nodes: 320 heads
   // 10.5 / 13.6 and 13.5 / 17.0, 384 14.2 / 13.5 and 20.3 / 17.0, 512 17.0 / 15.6 and 23.4 / 20.2, 1,024 29.5 / 26.5 and 40.5 / 31.6, 1,536 42.5 / 37.2 and 57.4 / 43.9

@@ -52,7 +52,7 @@ struct AcceptArgs : AppendArgs {
 // a row a warp, as long as two of them an SM are enough: one / two / four CTAs, us, 1,000 rows 6.7 / 5.5 / 4.6, 4,096 6.9 / 5.85 / 5.5, 8,192 (516 CTAs)
 // 7.1 / 11.2 / 10.2.  A block of 128 over eight, four or two, the most that the SMs have room for at once: one / four / eight, 1,000 rows 12.7 / 5.5 / 5.25,
 // 4,096 (264 CTAs) 13.1 / 5.85 / 6.9; 8,192 by one / two / four 16.4 / 8.4 / 11.4, 20,000 by one / two 20.1 / 23.1.  Under 64 rows the barrier
-// of the cluster costs what it gains (32 rows in blocks of 64, one / two 4.0 / 4.7).
+// of the cluster costs what it gains (32 rows in blocks of 64, one / two 4.0 / 4.7).  (With MIN 0; as they run, 1,000 rows take 4.0 and 4.4.)
 // MIN: CTAs that an SM is to have room for, 0 as the compiler likes (append_launch).
 constexpr int APPEND_WARPS = 16;
 template <int FMT, int ROWS, bool KEEP, int PARTS, bool TREE = false, int MIN = 0>

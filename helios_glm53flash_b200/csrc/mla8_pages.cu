@@ -8,7 +8,9 @@
 // meet at a barrier, which also orders their accesses to global memory.  A list of free blocks in ascending order: every warp counts its part of
 // refs, the counts are added up through (distributed) shared memory, and the second pass writes where its count says.
 // What bounds it is latency, a few dependent loads and a barrier a step, and the issue slots of one SM: what all 32 warps do costs eight cycles an
-// instruction, so warps without blocks or rows stand aside (a fork of four 6.8 -> 6.0 us).
+// instruction, so warps without blocks or rows stand aside (a fork of four 6.8 -> 6.0 us).  A row is given back and filled by one warp, over the table's whole width: a
+// fork of four at 5,001 in a table of 100 entries a row takes 5.9 us, of 640 8.9, of 4,096 20, of 16,384 55 (in a graph).  And every sequence of a fork or a
+// reserve adds up those before it: 64, 256, 1,024 and 4,096 sequences of three blocks, fork 10.3, 23, 89, 219 us, reserve and free 9.2, 26, 111, 152.
 #include "hk_common.cuh"
 #include "latent8.cuh"
 
@@ -439,8 +441,8 @@ bool pages_workspace(PagesArgs* a, void* workspace, size_t bytes, int* status) {
 }
 template <int MODE>
 cudaError_t pages_launch(const PagesArgs& a, cudaStream_t s) {
-  // us, one CTA / eight: a compaction with nothing to move of 123 blocks 3.7 / 6.3, of 4,000 4.8 / 7.8, of 8,192 6.0 / 8.0 (of 131,072 66, when one CTA walked them, / 13.7);
-  // a fork of four out of 123 6.4 / 9.6, of 8,192 6.9 / 10.0
+  // us in a graph, one CTA / eight: a compaction with nothing to move of 123 blocks 3.5 / 6.1, of 4,000 4.6 / 7.6, of 8,192 5.7 / 7.6 (of 131,072 66, when one CTA walked
+  // them, / 13.3); a fork of four out of 123 5.9 / 8.8, of 8,192 6.8 / 9.6
   return a.pg.n_blocks <= PG_SMALL ? pdl_launch(pages_kernel<MODE, 1>, dim3(1), dim3(PG_THREADS), 0, s, a)
                                : pdl_launch_cluster(PG_MAX_CTAS, pages_kernel<MODE, PG_MAX_CTAS>, dim3(PG_MAX_CTAS), dim3(PG_THREADS), 0, s, a);
 }
@@ -479,7 +481,8 @@ HK_API int hk_mla8_pages_fork(void* ckv8, float* scales, int dtype, int64_t n_bl
   int st;
   if (!pages_workspace(&a, workspace, workspace_bytes, &st)) return st;
   // Scattered additions to global memory leave an SM one a cycle: many entries are counted in shared memory, for which the pool's references are read and written back
-  // once.  us, global / shared: 320 entries of 4 rows 6.0 / 6.8, 632 of 8 6.2 / 7.2, 2,528 of 32 8.5 / 7.5, 5,000 of 16 11.7 / 10.3, 10,000 of 32 16.3 / 11.4
+  // once.  us, global / shared: 320 entries of 4 rows 6.0 / 6.8, 632 of 8 6.2 / 7.2, 2,528 of 32 8.5 / 7.5, 5,000 of 16 11.7 / 10.3, 10,000 of 32 16.3 / 11.4 (the
+  // last three of one parent 7.7 / 8.1, 10.3 / 11.0, 11.6 / 11.9).  Lengths are the device's: it goes by the table's width, so a few entries of a wide table go this way too.
   const bool many = n_blocks <= PG_SMALL && (int64_t)n * table_stride >= PG_MANY;
   const cudaError_t e = many ? pdl_launch(pages_kernel<PG_FORK_MANY, 1>, dim3(1), dim3(PG_THREADS), 0, as_stream(stream), a) : pages_launch<PG_FORK>(a, as_stream(stream));
   if (e != cudaSuccess) return HK_ERR_CUDA;

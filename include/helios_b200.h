@@ -575,7 +575,14 @@ int hk_mla_decode_prologue(const float* kv_pre, const void* ln_w_f16, void* ckv,
  *
  *   A step: hk_kda_tree_conv, hk_kda_tree and hk_gated_rms_norm in a KDA layer, hk_mla_tree or hk_mla8_tree in an MLA layer, none of which changes a
  *   state or a cache; once the nodes are accepted, hk_kda_tree_accept for each KDA layer and hk_mla_tree_accept or hk_mla8_tree_accept for each MLA
- *   layer, which do what decoding the accepted tokens one by one would have done.
+ *   layer.  States, windows and fp16 rows are then bit for bit what decoding the accepted tokens one by one leaves (hk_kda_cast_conv, hk_kda_recurrent,
+ *   hk_mla_cache_append); the 8-bit cache is not (hk_mla8_tree_accept says how it differs).
+ *
+ *   Nodes attend densely: to every cached row, and to their path.  Layers that decode through the indexer (hk_indexer_select, hk_mla_sparse) attend to the
+ *   selected pools and the last four tokens instead; trees have no such form.  Beyond the selection's reach (512 pools, 2,048 tokens) a draft is
+ *   verified here by another distribution than those layers sample from; below it too where the newest whole pool is selected, whose tokens
+ *   hk_pool_expand names twice.  The indexer's ring and pooled keys are not touched either: an engine that uses both hands the accepted nodes' keys, in the
+ *   order of the path, to hk_layernorm_f16 and hk_kpool_write.
  * ------------------------------------------------------------------------------------------- */
 
 /* Attention of nodes over the fp16 cache: a row attends to the first kv_len[s] cached rows of its sequence (kv_len [n_seqs]; NULL: pos_start for
@@ -604,7 +611,9 @@ int hk_mla8_tree(const void* q_lat, const void* ckv8, const float* scales, int d
  * at or beyond ckv_rows, where it is told, are dropped).  len_out (optional) [n_seqs]: kv_len[s] and the number of accepted nodes; not kv_len itself.  */
 int hk_mla_tree_accept(const void* tree_kv, void* ckv, int64_t ckv_rows, const int64_t* kv_base, const int* kv_len, int pos_start,
                        const int* parent, const int* tree_start, int n_seqs, const int* leaf, int m, int* len_out, void* stream);
-/* The same into the 8-bit cache, as hk_mla8_append appends rows (scales, blocks and rows without one as there; the rows are normalised already).   */
+/* The same into the 8-bit cache, as one call of hk_mla8_append appends rows (scales, blocks and rows without one as there; the rows are normalised
+ * already).  Not the bits of appending token by token: tree_kv has been rounded to fp16 before it becomes 8 bits, and a block's scale grows once for the
+ * whole path, where token by token the block's older values are rounded again with each growth.                                            */
 int hk_mla8_tree_accept(const void* tree_kv, void* ckv8, float* scales, int dtype, int64_t n_blocks, int block, const int* block_table,
                         int table_stride, const int* kv_len, int pos_start, const int* parent, const int* tree_start, int n_seqs, const int* leaf,
                         int m, int* len_out, void* stream);
@@ -617,7 +626,9 @@ int hk_kda_tree_conv(const float* x32, const void* conv_state, const int* slots,
 
 /* The KDA recurrence of nodes, head dim 128, Hk == Hv: out [m][H][128] bf16 (rz; out_f32 optional) is what hk_kda_recurrent (channelwise) gives for
  * the node as the last token behind its path, with the state rec_state [slots][H][128][128] of its sequence, which stays as it is.  No node's
- * state is formed: sums in another order than there.  mixed_qkv [m][3*H*128] bf16 (8-byte aligned), g [m][H][128] log decay f32 (<= 0; 16-byte aligned)
+ * state is formed: sums in another order than there, and the products with rec_state are tensor-core products of two bf16 numbers for each fp32 one, up to
+ * 3 * 2^-16 of a product off (out_f32 is 1.3e-6 to 3.6e-6 from 64 bits in the 2-norm, hk_kda_recurrent's 1.1e-7; out 3.3e-3 both, of its
+ * rounding).  A state element that is not finite makes its column of every node not finite.  mixed_qkv [m][3*H*128] bf16 (8-byte aligned), g [m][H][128] log decay f32 (<= 0; 16-byte aligned)
  * and beta [m][H] bf16 as there; or, with a_log [H] and dt_bias [H][128], the raw gate f32 and the raw beta logit f32 as in
  * hk_kda_chunked_prefill_gated.  max_nodes: nodes that the longest tree has (0: 64); nodes beyond, and rows of no tree, are left as they were.
  * out 8-byte, out_f32 and rec_state 16-byte aligned.                                                                                        */
