@@ -253,7 +253,7 @@ int hk_mla_auto_splits(int m, int n_keys);
  * explicit softmax scale and head count (the reference pins 0.0625 and 64).
  *   q_lat [m][n_heads][512] f16, ckv [ckv_rows][512] f16, lat_out [m][n_heads][512] f16.
  * ckv_rows: rows the cache buffer holds; row numbers at or beyond it are treated as holes instead of being read
- * (0 = not told, as in the reference's signature: every non-negative row number is read).
+ * (0 = not told, as in the reference's signature: row numbers up to the end of the allocation that ckv lies in are read).
  * n_split > 0: that many splits, a CTA each, through the workspace.  n_split <= 0 lets the library choose number and form
  * (hk_mla_auto_splits says the number; workspace may be NULL when it is 1): the fastest form of a call that has the GPU to
  * itself.  One row of 129 to 2,112 keys then runs as clusters on 64 SMs.  Calls that run beside others on streams of their own

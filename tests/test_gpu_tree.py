@@ -235,6 +235,41 @@ def test_trees_on_the_cuda_cores(switch):
     assert run.returncode == 0, run.stdout[-3000:] + run.stderr[-2000:]
 
 
+@pytest.mark.parametrize("behind", [0, 1, 13, 40, 200])
+def test_caches_at_the_end_of_their_memory_whose_rows_are_not_told(behind):
+    """a cache that ends `behind` rows before the end of its allocation, several of them (what follows an allocation may be nothing): the same bits as with its rows told"""
+    torch.cuda.empty_cache()
+    gen, held, rows = gen_of(51 + behind), 200, 17 << 11         # 34 MB, an allocation of its own
+    trees = [tree_of((46, 1)), tree_of((27, 3))]
+    starts, parent, tree_start = layout(trees)
+    m, base = starts[-1], torch.tensor([10, 90], device="cuda")
+    kv = randn(gen, m, 512).half()
+    whole = [torch.empty(rows, 512, dtype=torch.float16, device="cuda") for _ in range(4)]
+    idx = torch.full((3, 64), -1, dtype=torch.int32, device="cuda")
+    idx[:, :5] = ints([[0, 7, 199, 100, 199], [198, 199, -1, 5, 5], [199, -1, -1, -1, -1]])
+    for ckv in (w[rows - behind - held:rows - behind] for w in whole):
+        ckv.copy_(randn(gen, held, 512))
+        for lens in ([0, 3], [64, 110], [70, 1], [128, 96]):
+            for heads, n_split in ((64, 0), (64, 3), (16, 0), (4, 24)):
+                q = (randn(gen, m, heads, 512) * 0.7).half()
+                got = [torch.empty_like(q) for _ in range(2)]
+                for out, told in zip(got, (0, None)):
+                    hk.mla_tree_decode(q, ckv, kv, parent, out, m, n_seqs=2, tree_start=tree_start, kv_base=base, kv_len=ints(lens), n_heads=heads, n_split=n_split,
+                                       n_keys_hint=128, ckv_rows=told)
+                finish()
+                assert torch.equal(*got), (lens, heads)
+            q = (randn(gen, 3, 64, 512) * 0.7).half()
+            for call in (lambda o, told: hk.mla_dense_prefill(q, ckv, o, 3, 0, kv_base=torch.tensor([10, 90, 199], device="cuda"), kv_len=ints(lens + [1]), n_keys_hint=128, ckv_rows=told),
+                         lambda o, told: hk.mla_window_prefill(q, ckv, o, 3, 0, 60, 3, kv_base=torch.tensor([10, 90, 199], device="cuda"), kv_len=ints(lens + [1]), n_keys_hint=128, ckv_rows=told),
+                         lambda o, told: hk.mla_dense_prefill(q, ckv, o, 3, held - 3, ckv_rows=told),
+                         lambda o, told: hk.mla_sparse_decode(q, ckv, idx, 64, o, 3, ckv_rows=told)):
+                got = [torch.empty_like(q) for _ in range(2)]
+                call(got[0], 0)
+                call(got[1], None)
+                finish()
+                assert torch.equal(*got), lens
+
+
 def test_parents_that_are_no_earlier_node_hang_on_the_sequence():
     gen = gen_of(4)
     m, n = 6, 90
